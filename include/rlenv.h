@@ -61,6 +61,9 @@ extern "C" {
  * 0-1 of N bytes). A caller that streams T steps of actions from host memory moves a quarter
  * of the uint8 bytes. No counterpart in the reference, whose kernels read int32 actions. */
 #define RLENV_U2 3
+/* Element types of the memory policy's operators (below). */
+#define RLENV_F32 4
+#define RLENV_BF16 5
 
 /* Human-readable message for a status code; the string is static. */
 RLENV_API const char* rlenv_strerror(int code);
@@ -331,6 +334,94 @@ RLENV_API int rlenv_es_update(const float* theta, const float* ranks, int64_t d,
  * (cartpole_mlx.py:30-31, legged_mlx.py:21-22) on the device. */
 RLENV_API int rlenv_reset_uniform(float* out, int rows, int64_t n, const float* center, float bound,
                         uint32_t seed, int64_t index_offset, void* stream);
+
+/* ---- Operators of a memory policy ---------------------------------------------
+ * No counterparts in the reference, whose policies are two-layer MLPs without memory
+ * (es.py:156-164): the pieces of a policy that remembers, trained by gradient over the
+ * trajectories that the step_many entry points give.
+ *
+ * Decayed linear attention. A head of an environment carries a (d, d) float32 state S; a
+ * token with query q, key k and value v does
+ *     S <- keep * decay[h] * S + k' v,    out = scale * q S,
+ * keep = 0 where resets marks the token as the first of an episode (S from before it is
+ * dropped, whatever it holds), 1 elsewhere. Trajectories are time-major: q, k, v are
+ * (t, n, h, d) of dtype RLENV_F32 or RLENV_BF16, d in {16, 32, 64, 128}; resets (t, n), one
+ * byte each, or NULL; decay (h) float32 in [0, 1]. strides (host) holds the elements between
+ * steps, environments and heads of q, then of k, then of v; the last axis is dense. Bases and
+ * strides must keep rows on 16-byte boundaries. state_in (n, h, d, d) may be NULL for zero.
+ * scale is finite and not zero. Sums and states are held in 32 bits or more. Products of bf16
+ * values that pass through 16 bits keep a second 16-bit term.
+ *
+ * forward: out (t, n, h, d) dense and state_out, the state after the last token; state_out
+ * must not alias state_in. t = 0 copies the state. scratch: device memory of at least
+ * rlenv_linear_attention_scratch_bytes(..., 0) bytes, 256-byte aligned (NULL when that is 0);
+ * nothing in it needs to be initialised. */
+RLENV_API int64_t rlenv_linear_attention_scratch_bytes(int dtype, int d, int64_t t, int64_t n, int64_t h,
+                                                       int backward);
+
+RLENV_API int rlenv_linear_attention_forward(int dtype, int d, int64_t t, int64_t n, int64_t h, const void* q,
+                                             const void* k, const void* v, const int64_t* strides,
+                                             const float* decay, const uint8_t* resets, float scale,
+                                             const float* state_in, void* out, float* state_out, void* scratch,
+                                             int64_t scratch_bytes, void* stream);
+
+/* The gradient of the forward pass with respect to q, k, v and state_in (the decay is a constant
+ * of the architecture): grad_out as q with its own strides (first of the four triples in strides:
+ * grad_out, q, k, v), grad_state_out (n, h, d, d) or NULL for zero; grad_q, grad_k, grad_v
+ * (t, n, h, d) dense; grad_state_in may be NULL and must not alias grad_state_out. */
+RLENV_API int rlenv_linear_attention_backward(int dtype, int d, int64_t t, int64_t n, int64_t h,
+                                              const void* grad_out, const void* q, const void* k, const void* v,
+                                              const int64_t* strides, const float* decay, const uint8_t* resets,
+                                              float scale, const float* state_in, const float* grad_state_out,
+                                              void* grad_q, void* grad_k, void* grad_v, float* grad_state_in,
+                                              void* scratch, int64_t scratch_bytes, void* stream);
+
+/* One token for every environment, the state updated in place: q, k, v (n, h, d), strides
+ * (environment, head) of each, resets (n) or NULL, out (n, h, d) dense. */
+RLENV_API int rlenv_linear_attention_step(int dtype, int d, int64_t n, int64_t h, const void* q, const void* k,
+                                          const void* v, const int64_t* strides, const float* decay,
+                                          const uint8_t* resets, float scale, float* state, void* out,
+                                          void* stream);
+
+/* Gated feed-forward block: out = act(x w_gate) * (x w_up), x (m, k), weights (k, f), out (m, f),
+ * all dense row-major of one dtype (RLENV_F32 or RLENV_BF16), products summed in 32 bits.
+ * activation: RLENV_SILU, or RLENV_GELU with the exact normal distribution. scratch: device
+ * memory of at least rlenv_gated_ffn_scratch_bytes bytes, 256-byte aligned (NULL when that is 0). */
+#define RLENV_SILU 0
+#define RLENV_GELU 1
+RLENV_API int64_t rlenv_gated_ffn_scratch_bytes(int dtype, int64_t m, int64_t k, int64_t f, int backward);
+
+RLENV_API int rlenv_gated_ffn_forward(int dtype, int activation, int64_t m, int64_t k, int64_t f, const void* x,
+                                      const void* w_gate, const void* w_up, void* out, void* scratch,
+                                      int64_t scratch_bytes, void* stream);
+
+/* Its gradient with respect to x, w_gate and w_up from grad_out (m, f); both products are formed
+ * again. m, k and f are at least 1. */
+RLENV_API int rlenv_gated_ffn_backward(int dtype, int activation, int64_t m, int64_t k, int64_t f,
+                                       const void* grad_out, const void* x, const void* w_gate, const void* w_up,
+                                       void* grad_x, void* grad_w_gate, void* grad_w_up, void* scratch,
+                                       int64_t scratch_bytes, void* stream);
+
+/* One AdamW step over many tensors, in place:
+ *     m <- beta1 m + (1 - beta1) g,  v <- beta2 v + (1 - beta2) g^2,
+ *     p <- p (1 - lr weight_decay) - lr (m / (1 - beta1^step)) / (sqrt(v / (1 - beta2^step)) + eps).
+ * params, grads, copies and sizes are host arrays of `tensors` entries: float32 parameters,
+ * gradients of grad_dtype (RLENV_F32 or RLENV_BF16), optional bf16 copies of the parameters to
+ * write (copies or an entry may be NULL), element counts. grad_scale, a device float or NULL,
+ * multiplies every gradient. The moments are flat arrays in which each tensor starts at the next
+ * multiple of 256 elements: float32 with state_bits 32 (m_exp and v_exp unused); with state_bits 8
+ * a byte an element and a byte of exponent for every 256, the values being those of
+ * rlenv_adamw_moments, rounded stochastically by a hash of (seed, step, place). All-zero bytes
+ * stand for zero moments. step counts from 1. At most 2^32 elements in all. */
+RLENV_API int rlenv_adamw_step(int state_bits, int grad_dtype, int64_t tensors, float* const* params,
+                               const void* const* grads, void* const* copies, const int64_t* sizes, void* m,
+                               void* v, uint8_t* m_exp, uint8_t* v_exp, double lr, double beta1, double beta2,
+                               double eps, double weight_decay, const float* grad_scale, int64_t step,
+                               uint32_t seed, void* stream);
+
+/* The float32 values of 8-bit moments: `blocks` blocks of 256 elements. */
+RLENV_API int rlenv_adamw_moments(int64_t blocks, const uint8_t* m, const uint8_t* v, const uint8_t* m_exp,
+                                  const uint8_t* v_exp, float* m_out, float* v_out, void* stream);
 
 #ifdef __cplusplus
 }

@@ -1,0 +1,79 @@
+"""Gated feed-forward block: out = act(x w_gate) * (x w_up), both products, the activation and the
+product in one sm_100a kernel, and its gradient.
+
+x is (..., K), the weights (K, F) as es.unflatten's (in, out) layout, out (..., F), all of one type,
+float32 or bfloat16; sums are in 32 bits. activation is "silu" or "gelu" (the exact normal
+distribution). `backward` forms both products again instead of keeping them. `apply` is the
+differentiable form. The projection back to K is a plain matrix product and is left to the caller.
+The reference's policies are tanh MLPs (es.py:156-164); there is no counterpart there.
+"""
+
+import torch
+
+import rlenv_lib as _rl
+
+ACTIVATIONS = {"silu": 0, "gelu": 1}
+
+
+def _check(x, w_gate, w_up, activation, grad_out=None):
+    _rl.as_floats("x", x)
+    if x.dim() < 1:
+        raise ValueError("x must have at least one axis")
+    _rl.as_floats("w_gate", w_gate, (x.shape[-1], None), x.dtype)
+    _rl.as_floats("w_up", w_up, w_gate.shape, x.dtype)
+    if grad_out is not None:
+        _rl.as_floats("grad_out", grad_out, (*x.shape[:-1], w_gate.shape[1]), x.dtype)
+    if activation not in ACTIVATIONS:
+        raise ValueError(f"activation must be one of {sorted(ACTIVATIONS)}; got {activation!r}")
+    dev = _rl.same_device(x=x, w_gate=w_gate, w_up=w_up, grad_out=grad_out)
+    m = x.numel() // x.shape[-1] if x.shape[-1] else torch.Size(x.shape[:-1]).numel()
+    return m, x.shape[-1], w_gate.shape[1], _rl.FLOAT_DTYPES[x.dtype], dev
+
+
+def forward(x, w_gate, w_up, activation="silu"):
+    """act(x w_gate) * (x w_up), (..., F)."""
+    m, k, f, code, dev = _check(x, w_gate, w_up, activation)
+    x, w_gate, w_up = x.contiguous(), w_gate.contiguous(), w_up.contiguous()
+    lib = _rl.lib()
+    with torch.cuda.device(dev):
+        out = torch.empty((*x.shape[:-1], f), dtype=x.dtype, device=dev)
+        nbytes = lib.gated_ffn_scratch_bytes(code, m, k, f, 0)
+        tmp = _rl.scratch(nbytes, dev)
+        _rl.check(lib.gated_ffn_forward(code, ACTIVATIONS[activation], m, k, f, x.data_ptr(), w_gate.data_ptr(),
+                                        w_up.data_ptr(), out.data_ptr(), _rl.ptr(tmp), nbytes, _rl.stream_ptr(dev)))
+    return out
+
+
+def backward(grad_out, x, w_gate, w_up, activation="silu"):
+    """(dx, dw_gate, dw_up) of `forward` from grad_out (..., F)."""
+    m, k, f, code, dev = _check(x, w_gate, w_up, activation, grad_out)
+    if 0 in (m, k, f):  # sums over nothing
+        return torch.zeros_like(x), torch.zeros_like(w_gate), torch.zeros_like(w_up)
+    grad_out, x, w_gate, w_up = (y.contiguous() for y in (grad_out, x, w_gate, w_up))
+    lib = _rl.lib()
+    with torch.cuda.device(dev):
+        dx, dwg, dwu = torch.empty_like(x), torch.empty_like(w_gate), torch.empty_like(w_up)
+        nbytes = lib.gated_ffn_scratch_bytes(code, m, k, f, 1)
+        tmp = _rl.scratch(nbytes, dev)
+        _rl.check(lib.gated_ffn_backward(code, ACTIVATIONS[activation], m, k, f, grad_out.data_ptr(), x.data_ptr(),
+                                         w_gate.data_ptr(), w_up.data_ptr(), dx.data_ptr(), dwg.data_ptr(),
+                                         dwu.data_ptr(), _rl.ptr(tmp), nbytes, _rl.stream_ptr(dev)))
+    return dx, dwg, dwu
+
+
+class _Apply(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, w_gate, w_up, activation):
+        ctx.save_for_backward(x, w_gate, w_up)
+        ctx.activation = activation
+        return forward(x, w_gate, w_up, activation)
+
+    @staticmethod
+    def backward(ctx, grad_out):
+        x, w_gate, w_up = ctx.saved_tensors
+        return (*backward(grad_out, x, w_gate, w_up, ctx.activation), None)
+
+
+def apply(x, w_gate, w_up, activation="silu"):
+    """`forward` as a differentiable operation of x and both weights."""
+    return _Apply.apply(x, w_gate, w_up, activation)

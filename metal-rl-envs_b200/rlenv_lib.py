@@ -14,7 +14,7 @@ There is no CPU path: a missing library or a missing CUDA device raises.
 
 import ctypes
 import os
-from ctypes import c_float, c_int, c_int64, c_uint32, c_uint64, c_void_p
+from ctypes import c_double, c_float, c_int, c_int64, c_uint32, c_uint64, c_void_p
 from pathlib import Path
 
 import numpy as np
@@ -24,11 +24,13 @@ LIB_PATH = Path(__file__).resolve().parent / "librlenv.so"
 # RLENV_LIBRARY=checks loads the check build instead (rlenv_build.build(checks=True))
 CHECKS_LIB_PATH = Path(__file__).resolve().parent / "librlenv_checks.so"
 
-I32, I64, U8, U2 = 0, 1, 2, 3
+I32, I64, U8, U2, F32, BF16 = 0, 1, 2, 3, 4, 5
+FLOAT_DTYPES = {torch.float32: F32, torch.bfloat16: BF16}  # of the memory policy's operators
 _DTYPES = {torch.int32: I32, torch.int64: I64, torch.uint8: U8, torch.bool: U8}
 
 # name -> argument types; every function returns int except those in _RESTYPES
-_RESTYPES = {"rlenv_es_ranks_scratch_bytes": c_int64}
+_RESTYPES = {"rlenv_es_ranks_scratch_bytes": c_int64, "rlenv_linear_attention_scratch_bytes": c_int64,
+             "rlenv_gated_ffn_scratch_bytes": c_int64}
 _SIGNATURES = {
     "rlenv_abi_version": [],
     "rlenv_checks_status": [c_void_p, c_int],
@@ -73,6 +75,24 @@ _SIGNATURES = {
     "rlenv_es_centered_ranks_sorted": [c_void_p, c_int64, c_void_p, c_void_p, c_int64, c_void_p],
     "rlenv_es_centered_ranks_static": [c_void_p, c_int64, c_void_p, c_void_p],
     "rlenv_es_update": [c_void_p, c_void_p, c_int64, c_int64, c_float, c_float, c_uint64, c_uint64, c_void_p, c_void_p],
+    "rlenv_linear_attention_scratch_bytes": [c_int, c_int, c_int64, c_int64, c_int64, c_int],
+    "rlenv_linear_attention_forward": [c_int, c_int, c_int64, c_int64, c_int64, c_void_p, c_void_p, c_void_p, c_void_p,
+                                       c_void_p, c_void_p, c_float, c_void_p, c_void_p, c_void_p, c_void_p, c_int64,
+                                       c_void_p],
+    "rlenv_linear_attention_backward": [c_int, c_int, c_int64, c_int64, c_int64, c_void_p, c_void_p, c_void_p,
+                                        c_void_p, c_void_p, c_void_p, c_void_p, c_float, c_void_p, c_void_p, c_void_p,
+                                        c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_void_p],
+    "rlenv_linear_attention_step": [c_int, c_int, c_int64, c_int64, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
+                                    c_void_p, c_float, c_void_p, c_void_p, c_void_p],
+    "rlenv_gated_ffn_scratch_bytes": [c_int, c_int64, c_int64, c_int64, c_int],
+    "rlenv_gated_ffn_forward": [c_int, c_int, c_int64, c_int64, c_int64, c_void_p, c_void_p, c_void_p, c_void_p,
+                                c_void_p, c_int64, c_void_p],
+    "rlenv_gated_ffn_backward": [c_int, c_int, c_int64, c_int64, c_int64, c_void_p, c_void_p, c_void_p, c_void_p,
+                                 c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_void_p],
+    "rlenv_adamw_step": [c_int, c_int, c_int64, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
+                         c_void_p, c_double, c_double, c_double, c_double, c_double, c_void_p, c_int64, c_uint32,
+                         c_void_p],
+    "rlenv_adamw_moments": [c_int64, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p],
     "rlenv_reset_uniform": [c_void_p, c_int, c_int64, c_void_p, c_float, c_uint32, c_int64, c_void_p],
 }
 
@@ -388,3 +408,35 @@ def as_theta(theta, p, d, dev):
     if theta.shape[-1] != d:
         raise ValueError(f"theta_pop rows must have {d} parameters for this hidden width; got {theta.shape[-1]}")
     return theta, stride
+
+
+# ---- operators of a memory policy --------------------------------------------------------------
+
+
+def as_floats(name, x, shape=None, dtype=None):
+    """x checked as a CUDA tensor of the operators' types (float32, bfloat16), of `shape` (None
+    entries are free) and `dtype` where given. Nothing is copied: these calls sit between a
+    program's other GPU work, and there is no CPU path."""
+    if not isinstance(x, torch.Tensor) or x.device.type != "cuda":
+        raise ValueError(f"{name} must be a CUDA tensor: there is no CPU path")
+    if x.dtype not in FLOAT_DTYPES or (dtype is not None and x.dtype != dtype):
+        raise ValueError(f"{name} must be {dtype or 'float32 or bfloat16'}; got {x.dtype}")
+    if shape is not None and (x.dim() != len(shape) or any(w is not None and w != g for w, g in zip(shape, x.shape))):
+        raise ValueError(f"{name} must have shape {tuple('*' if w is None else w for w in shape)}; got {tuple(x.shape)}")
+    return x
+
+
+def same_device(**tensors):
+    """The one device of the tensors given (None entries aside); anything else raises."""
+    devs = {x.device for x in tensors.values() if x is not None}
+    if len(devs) != 1:
+        raise ValueError(f"{', '.join(tensors)} must be on one device; got {sorted(map(str, devs))}")
+    return devs.pop()
+
+
+def scratch(nbytes, dev):
+    """Working memory for one call, from torch's caching allocator: it belongs to the current
+    stream, which the call's kernels run on."""
+    if nbytes < 0:
+        check(-1)
+    return torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None

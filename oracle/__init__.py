@@ -18,6 +18,8 @@ Each module restates one reference file's algorithm in float32 numpy:
   rollout.py   the fused rollout kernels' semantics (cartpole_rollout_metal.py,
                acrobot_rollout_metal.py, legged_rollout_metal.py)
   es.py        es.py's numpy backend: loop_fitness, centered_ranks, generation, train
+  policy.py    the memory policy's operators in 64 bits, from their definitions (no counterpart
+               in the reference)
 
 The restatement is pinned against golden vectors produced by running the
 reference's own numpy modules (tests/golden/make_golden.py) and against the
