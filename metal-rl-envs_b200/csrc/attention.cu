@@ -9,29 +9,375 @@ using attn::Problem;
 using attn::Scan;
 using attn::Strides;
 
-constexpr int kScanThreads = 128;
+// A sequence (one head of one environment) or, where there are few of them, a segment of one:
+// `segments` runs of `per` chunks. Split sequences take three launches: chunk_kernel<local> forms each
+// segment's own carry from zero, join_kernel the carry at each segment's start, and
+// chunk_kernel<whole> the outputs.
+struct Split {
+  int64_t segments, per;
+  float* carry;    // (scans, sequences, segments, D, D): a segment's own, then the one at its start
+  float* through;  // (scans, sequences, segments): the decay over a segment, -1 where a reset cuts it
+};
 
-// Block (seq * column tiles + tile, scan): one head of one environment from its first token to its last.
-template <typename T, int D>
-__global__ void __launch_bounds__(kScanThreads) scan_kernel(const __grid_constant__ Problem p) {
-  constexpr int DB = D < 64 ? D : 64;
-  extern __shared__ float buf[];
-  const Scan& s = p.scan[blockIdx.y];
-  constexpr int kTiles = D / DB;
-  const int64_t seq = blockIdx.x / kTiles;
-  const int col = int(blockIdx.x % kTiles) * DB;
+template <typename T, int D, bool kLocal>
+__global__ void __launch_bounds__(attn::kThreads)
+chunk_kernel(const __grid_constant__ Problem p, const __grid_constant__ Split split) {
+  using namespace attn;
+  using C = Shape<T, D>;
+  constexpr int DB = C::DB, kTiles = D / DB;
+  extern __shared__ __align__(16) unsigned char smem[];
+  __shared__ float left[kChunk];       // l_j
+  __shared__ uint32_t reset_words[2];
+  __nv_bfloat16* const X = reinterpret_cast<__nv_bfloat16*>(smem);
+  __nv_bfloat16* const A = X + C::kIn * C::kX;
+  __nv_bfloat16* const B = A + C::kIn * C::kX;
+  __nv_bfloat16* const S = B + C::kIn * C::kB;
+
+  int64_t id = blockIdx.x;
+  const int col = int(id % kTiles) * DB;
+  id /= kTiles;
+  const Scan& s = p.scan[id % p.scans];
+  const int64_t scan = id % p.scans;
+  id /= p.scans;
+  const int64_t segment = id % split.segments, seq = id / split.segments;
   const int64_t n = seq / p.h, h = seq % p.h;
-  attn::scan_tokens<T, D, DB, kScanThreads, true>(
-      s, p, n, h, col, 0, p.t, s.carry_in ? s.carry_in + seq * D * D : nullptr, s.turned, s.in_mul, buf,
-      s.carry_out ? s.carry_out + seq * D * D : nullptr, s.turned, s.out_mul);
+  const int64_t slot = (scan * p.n * p.h + seq) * split.segments + segment;
+  const int64_t first = segment * split.per * kChunk;
+  const int64_t last = first + split.per * kChunk < p.t ? first + split.per * kChunk : p.t;
+  const bool whole = split.segments == 1;
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int gr = lane >> 2, gc = (lane & 3) * 2;  // a fragment's row and column
+  const float log2_g = log2f(__ldg(p.decay + h));
+  const int f = s.reverse ? 0 : 1;
+
+  // The carry, float32 in registers: rows srow + 16 m + (gr, gr + 8), columns scol + 8 t + (gc, gc + 1).
+  const int rg = warp % C::RG, cg = warp / C::RG;
+  const bool holds = cg < C::CG;
+  const int srow = rg * 16 * C::MT, scol = cg * 8 * C::NT;
+  float z[C::MT][C::NT][4];
+  const float* start = kLocal ? nullptr : whole ? s.carry_in : split.carry + slot * D * D;
+  if (!kLocal && whole && start) start += seq * D * D;
+  const bool turned = whole && s.turned;
+  const float start_mul = whole ? s.in_mul : 1.0f;
+#pragma unroll
+  for (int m = 0; m < C::MT; ++m)
+#pragma unroll
+    for (int t = 0; t < C::NT; ++t)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const int r = srow + 16 * m + gr + (q & 2) * 4, c = col + scol + 8 * t + gc + (q & 1);
+        z[m][t][q] = start && holds ? start_mul * __ldg(start + (turned ? c * D + r : r * D + c)) : 0.0f;
+      }
+
+  // The weights between a warp's rows and 16 columns: on the diagonal, and one block to its left.
+  float near[8], next[8], row_decay[2];
+  if constexpr (!kLocal) {
+#pragma unroll
+    for (int q = 0; q < 8; ++q) {
+      const int apart = gr + (q & 2) * 4 - (gc + (q & 1) + (q & 4) * 2);
+      near[q] = apart >= 0 ? power(log2_g, apart) : 0.0f;
+      next[q] = power(log2_g, 16 + apart);
+    }
+    row_decay[0] = power(log2_g, 16 * warp + gr + f);
+    row_decay[1] = power(log2_g, 16 * warp + gr + 8 + f);
+  }
+
+  const T* const xs = static_cast<const T*>(s.x) + n * s.xs.n + h * s.xs.h;
+  const T* const as = static_cast<const T*>(s.a) + n * s.as.n + h * s.as.h;
+  const T* const bs = static_cast<const T*>(s.b) + n * s.bs.n + h * s.bs.h + col;
+  float bad = 0.0f;      // NaN once any value is not finite
+  bool cut = false;      // a reset anywhere in the segment
+
+  for (int64_t i0 = first; i0 < last; i0 += kChunk) {
+    const int len = int(last - i0 < kChunk ? last - i0 : kChunk);
+    if constexpr (!kLocal) {
+      load_tile<T, D, C::PX, C::kX>(xs, s.xs.t, s, p.t, i0, last, X);
+      // the carry at the chunk's start as planes
+      if (holds) {
+#pragma unroll
+        for (int m = 0; m < C::MT; ++m)
+#pragma unroll
+          for (int t = 0; t < C::NT; ++t)
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+              uint32_t v[C::kMid];
+              split_pair<C::kMid>(z[m][t][2 * half], z[m][t][2 * half + 1], v, 1);
+#pragma unroll
+              for (int q = 0; q < C::kMid; ++q)
+                *reinterpret_cast<uint32_t*>(S + q * C::kS + (srow + 16 * m + gr + 8 * half) * C::PB + scol + 8 * t +
+                                             gc) = v[q];
+            }
+      }
+    }
+    load_tile<T, D, C::PX, C::kX>(as, s.as.t, s, p.t, i0, last, A);
+    load_tile<T, DB, C::PB, C::kB>(bs, s.bs.t, s, p.t, i0, last, B);
+    if (threadIdx.x < kChunk) {
+      const int j = threadIdx.x;
+      bool reset = false;
+      if (p.resets && j < len) {
+        const int64_t t = s.reverse ? p.t - 1 - (i0 + j) : i0 + j;
+        reset = __ldg(p.resets + t * p.n + n) != 0;
+      }
+      const uint32_t word = __ballot_sync(0xffffffffu, reset);
+      if (lane == 0) reset_words[warp] = word;
+    }
+    copies_landed();
+    __syncthreads();
+    const uint64_t resets = uint64_t(reset_words[1]) << 32 | reset_words[0];
+    // resets that act before position i is used
+    const auto count = [&](int i) { return __popcll(resets & ((uint64_t(f + 1) << i) - 1)); };
+    if (threadIdx.x < kChunk) {
+      const int j = threadIdx.x;
+      const bool reaches = j < len && (resets == 0 || count(j) == __popcll(resets));
+      left[j] = reaches ? power(log2_g, len - f - j) : 0.0f;
+    }
+    __syncthreads();
+
+    if constexpr (!kLocal) {
+      float o[DB / 8][4];
+#pragma unroll
+      for (int t = 0; t < DB / 8; ++t)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) o[t][q] = 0.0f;
+      const uint32_t xa = shared_address(X + (16 * warp + (lane & 15)) * C::PX + (lane >> 4) * 8);
+      const uint32_t sa = shared_address(S + (lane & 15) * C::PB + (lane >> 4) * 8);
+      // x Z
+#pragma unroll
+      for (int k = 0; k < D / 16; ++k) {
+        uint32_t x[C::kIn][4];
+#pragma unroll
+        for (int q = 0; q < C::kIn; ++q) load_matrices(x[q], xa + 2 * (q * C::kX + 16 * k));
+#pragma unroll
+        for (int t = 0; t < DB / 16; ++t)
+#pragma unroll
+          for (int q = 0; q < C::kMid; ++q) {
+            uint32_t v[4];
+            load_matrices_turned(v, sa + 2 * (q * C::kS + 16 * k * C::PB + 16 * t));
+#pragma unroll
+            for (int u = 0; u < C::kIn && u + q < 3; ++u) {
+              multiply(o[2 * t], x[u], v[0], v[1]);
+              multiply(o[2 * t + 1], x[u], v[2], v[3]);
+            }
+          }
+      }
+      const int row[2] = {16 * warp + gr, 16 * warp + gr + 8};
+      int seen[2] = {0, 0};
+      if (resets) seen[0] = count(row[0]), seen[1] = count(row[1]);
+#pragma unroll
+      for (int t = 0; t < DB / 8; ++t)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) o[t][q] = seen[q >> 1] == 0 ? row_decay[q >> 1] * o[t][q] : 0.0f;
+      // (W * x a') b, 16 tokens at a time up to the diagonal
+      const uint32_t aa = shared_address(A + ((lane & 7) + (lane >> 4) * 8) * C::PX + ((lane >> 3) & 1) * 8);
+      const uint32_t ba = shared_address(B + (lane & 15) * C::PB + (lane >> 4) * 8);
+      for (int jb = 0; jb <= warp; ++jb) {
+        float w[2][4] = {};
+#pragma unroll
+        for (int k = 0; k < D / 16; ++k) {
+          uint32_t x[C::kIn][4];
+#pragma unroll
+          for (int q = 0; q < C::kIn; ++q) load_matrices(x[q], xa + 2 * (q * C::kX + 16 * k));
+#pragma unroll
+          for (int q = 0; q < C::kIn; ++q) {
+            uint32_t v[4];
+            load_matrices(v, aa + 2 * (q * C::kX + 16 * jb * C::PX + 16 * k));
+#pragma unroll
+            for (int u = 0; u < C::kIn && u + q < 3; ++u) {
+              multiply(w[0], x[u], v[0], v[1]);
+              multiply(w[1], x[u], v[2], v[3]);
+            }
+          }
+        }
+        const float far = jb < warp ? power(log2_g, 16 * (warp - 1 - jb)) : 1.0f;
+#pragma unroll
+        for (int q = 0; q < 8; ++q) {
+          bool linked = jb < warp || gr + (q & 2) * 4 >= gc + (q & 1) + (q & 4) * 2;
+          if (resets) linked = linked && seen[(q >> 1) & 1] == count(16 * jb + gc + (q & 1) + (q & 4) * 2);
+          const float weight = jb < warp ? next[q] * far : near[q];
+          w[q >> 2][q & 3] = linked ? weight * w[q >> 2][q & 3] : 0.0f;
+        }
+        uint32_t wp[C::kMid][4];
+        split_pair<C::kMid>(w[0][0], w[0][1], &wp[0][0], 4);
+        split_pair<C::kMid>(w[0][2], w[0][3], &wp[0][1], 4);
+        split_pair<C::kMid>(w[1][0], w[1][1], &wp[0][2], 4);
+        split_pair<C::kMid>(w[1][2], w[1][3], &wp[0][3], 4);
+#pragma unroll
+        for (int t = 0; t < DB / 16; ++t)
+#pragma unroll
+          for (int q = 0; q < C::kIn; ++q) {
+            uint32_t v[4];
+            load_matrices_turned(v, ba + 2 * (q * C::kB + 16 * jb * C::PB + 16 * t));
+#pragma unroll
+            for (int u = 0; u < C::kMid && u + q < 3; ++u) {
+              multiply(o[2 * t], wp[u], v[0], v[1]);
+              multiply(o[2 * t + 1], wp[u], v[2], v[3]);
+            }
+          }
+      }
+      T* const out = static_cast<T*>(s.out);
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        const int64_t i = i0 + row[half];
+        const bool real = row[half] < len;
+        const int64_t t_ = s.reverse ? p.t - 1 - i : i;
+        T* const at = out + ((t_ * p.n + n) * p.h + h) * D + col + gc;
+#pragma unroll
+        for (int t = 0; t < DB / 8; ++t) {
+          const float lo = p.scale * o[t][2 * half], hi = p.scale * o[t][2 * half + 1];
+          bad = fmaf(lo, 0.0f, bad), bad = fmaf(hi, 0.0f, bad);
+          if (real) {
+            if constexpr (sizeof(T) == 2)
+              *reinterpret_cast<uint32_t*>(at + 8 * t) = pack(lo, hi);
+            else
+              *reinterpret_cast<float2*>(at + 8 * t) = make_float2(lo, hi);
+          }
+        }
+      }
+    }
+
+    // Z <- g^L Z + (l * A)' B
+    if (holds) {
+      const float through = resets ? 0.0f : power(log2_g, len);
+#pragma unroll
+      for (int m = 0; m < C::MT; ++m)
+#pragma unroll
+        for (int t = 0; t < C::NT; ++t)
+#pragma unroll
+          for (int q = 0; q < 4; ++q) z[m][t][q] = resets ? 0.0f : through * z[m][t][q];
+      const uint32_t at = shared_address(A + ((lane & 7) + (lane >> 4) * 8) * C::PX + ((lane >> 3) & 1) * 8 + srow);
+      const uint32_t bt = shared_address(B + (lane & 15) * C::PB + (lane >> 4) * 8 + scol);
+#pragma unroll
+      for (int j = 0; j < kChunk / 16; ++j) {
+        const float l0 = left[16 * j + gc], l1 = left[16 * j + gc + 1];
+        const float l2 = left[16 * j + gc + 8], l3 = left[16 * j + gc + 9];
+        uint32_t key[C::MT][C::kKeys][4];
+#pragma unroll
+        for (int m = 0; m < C::MT; ++m) {
+          float lo[4] = {}, hi[4] = {};
+#pragma unroll
+          for (int q = C::kIn - 1; q >= 0; --q) {  // the planes' sum is the float32 value again
+            uint32_t v[4];
+            load_matrices_turned(v, at + 2 * (q * C::kX + 16 * j * C::PX + 16 * m));
+#pragma unroll
+            for (int u = 0; u < 4; ++u) lo[u] += low_half(v[u]), hi[u] += high_half(v[u]);
+          }
+#pragma unroll
+          for (int u = 0; u < 4; ++u)
+            split_pair<C::kKeys>((u & 2 ? l2 : l0) * lo[u], (u & 2 ? l3 : l1) * hi[u], &key[m][0][u], 4);
+        }
+#pragma unroll
+        for (int t = 0; t < C::NT / 2; ++t)
+#pragma unroll
+          for (int q = 0; q < C::kIn; ++q) {
+            uint32_t v[4];
+            load_matrices_turned(v, bt + 2 * (q * C::kB + 16 * j * C::PB + 16 * t));
+#pragma unroll
+            for (int m = 0; m < C::MT; ++m)
+#pragma unroll
+              for (int u = 0; u < C::kKeys && u + q < 3; ++u) {
+                multiply(z[m][2 * t], key[m][u], v[0], v[1]);
+                multiply(z[m][2 * t + 1], key[m][u], v[2], v[3]);
+              }
+          }
+      }
+    }
+    cut = cut || resets != 0;
+    __syncthreads();
+  }
+
+#pragma unroll
+  for (int m = 0; m < C::MT; ++m)
+#pragma unroll
+    for (int t = 0; t < C::NT; ++t)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) bad = fmaf(z[m][t][q], 0.0f, bad);
+  float* const end = kLocal ? split.carry + slot * D * D : whole && s.carry_out ? s.carry_out + seq * D * D : nullptr;
+  const bool end_turned = !kLocal && s.turned;
+  const float end_mul = kLocal ? 1.0f : s.out_mul;
+  if (kLocal && threadIdx.x == 0 && col == 0) split.through[slot] = cut ? -1.0f : power(log2_g, last - first);
+  // A value that is not finite may have met a masked zero on its way: the definition decides.
+  if (__syncthreads_or(bad != bad)) {
+    scan_tokens<T, D, DB, attn::kThreads, !kLocal>(s, p, n, h, col, first, last, start, turned, start_mul,
+                                                   reinterpret_cast<float*>(smem), end, end_turned, end_mul);
+    return;
+  }
+  if (end && holds) {
+#pragma unroll
+    for (int m = 0; m < C::MT; ++m)
+#pragma unroll
+      for (int t = 0; t < C::NT; ++t)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const int r = srow + 16 * m + gr + (q & 2) * 4, c = col + scol + 8 * t + gc + (q & 1);
+          end[end_turned ? c * D + r : r * D + c] = end_mul * z[m][t][q];
+        }
+  }
+}
+
+// The carry at each segment's start from the segments' own, one thread an element.
+__global__ void __launch_bounds__(256)
+join_kernel(const __grid_constant__ Problem p, const __grid_constant__ Split split, int d) {
+  const int64_t size = int64_t(d) * d, sequences = p.n * p.h;
+  const int64_t e = int64_t(blockIdx.x) * 256 + threadIdx.x;
+  if (e >= p.scans * sequences * size) return;
+  const int64_t which = e / size, scan = which / sequences, seq = which % sequences;
+  const int at = int(e % size);
+  const Scan& s = p.scan[scan];
+  const int64_t outside = seq * size + (s.turned ? at % d * d + at / d : at);
+  float z = s.carry_in ? s.in_mul * __ldg(s.carry_in + outside) : 0.0f;
+  for (int64_t g = 0; g < split.segments; ++g) {
+    float* const own = split.carry + (which * split.segments + g) * size + at;
+    const float through = split.through[which * split.segments + g];
+    const float mine = *own;
+    *own = z;
+    z = (through < 0.0f ? 0.0f : through * z) + mine;
+  }
+  if (s.carry_out) s.carry_out[outside] = s.out_mul * z;
+}
+
+// How a call is split over the time axis: not at all where the sequences fill the GPU, else into
+// segments of whole chunks until there are some kBlocksWanted blocks.
+constexpr int64_t kBlocksWanted = 148 * 4;
+
+int64_t split_segments(int64_t t, int64_t blocks, int64_t* per) {
+  const int64_t chunks = (t + attn::kChunk - 1) / attn::kChunk;
+  int64_t want = blocks >= kBlocksWanted / 2 ? 1 : kBlocksWanted / (blocks > 0 ? blocks : 1);
+  if (want > chunks) want = chunks;
+  if (want < 1) want = 1;
+  *per = chunks > 0 ? (chunks + want - 1) / want : 1;
+  return chunks > 0 ? (chunks + *per - 1) / *per : 1;
+}
+
+int64_t attention_scratch(int d, int64_t t, int64_t n, int64_t h, int scans) {
+  int64_t per;
+  const int64_t tiles = d > 64 ? d / 64 : 1;
+  const int64_t segments = split_segments(t, n * h * scans * tiles, &per);
+  return segments == 1 ? 0 : scans * n * h * segments * (int64_t(d) * d + 1) * 4;
 }
 
 template <typename T, int D>
-int launch_scan(const Problem& p, cudaStream_t stream) {
-  constexpr int DB = D < 64 ? D : 64;
-  const int smem = int(sizeof(float)) * (D * DB + 2 * D + DB + kScanThreads);
-  const dim3 grid(unsigned(p.n * p.h * (D / DB)), unsigned(p.scans));
-  scan_kernel<T, D><<<grid, kScanThreads, smem, stream>>>(p);
+int launch_scan(const Problem& p, void* scratch, cudaStream_t stream) {
+  using C = attn::Shape<T, D>;
+  constexpr int kTiles = D / C::DB;
+  Split split{};
+  const int64_t sequences = p.n * p.h;
+  split.segments = split_segments(p.t, sequences * p.scans * kTiles, &split.per);
+  const int64_t blocks = sequences * p.scans * kTiles * split.segments;
+  if (blocks > 0x7fffffff) return RLENV_EINVAL;
+  if (cudaError_t e = cudaFuncSetAttribute(chunk_kernel<T, D, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem))
+    return int(e);
+  if (split.segments > 1) {
+    split.carry = static_cast<float*>(scratch);
+    split.through = split.carry + p.scans * sequences * split.segments * D * D;
+    if (cudaError_t e = cudaFuncSetAttribute(chunk_kernel<T, D, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem))
+      return int(e);
+    chunk_kernel<T, D, true><<<unsigned(blocks), attn::kThreads, C::kSmem, stream>>>(p, split);
+    if (const int rc = launch_status()) return rc;
+    join_kernel<<<grid_for(p.scans * sequences * D * D, 256), 256, 0, stream>>>(p, split, D);
+    if (const int rc = launch_status()) return rc;
+  }
+  chunk_kernel<T, D, false><<<unsigned(blocks), attn::kThreads, C::kSmem, stream>>>(p, split);
   return launch_status();
 }
 
@@ -125,9 +471,10 @@ bool aligned_rows(const void* p, const int64_t* st, int dtype, int axes) {
 
 struct Runner {
   const Problem& p;
+  void* scratch;
   cudaStream_t stream;
   template <typename T, int D>
-  int operator()() const { return launch_scan<T, D>(p, stream); }
+  int operator()() const { return launch_scan<T, D>(p, scratch, stream); }
 };
 
 constexpr int64_t kMaxBlocks = 0x7fffffff;
@@ -147,8 +494,7 @@ extern "C" {
 
 int64_t rlenv_linear_attention_scratch_bytes(int dtype, int d, int64_t t, int64_t n, int64_t h, int backward) {
   using namespace rlenv;
-  (void)backward;
-  return check_sizes(dtype, d, t, n, h, 1.0f) == RLENV_OK ? 0 : -1;
+  return check_sizes(dtype, d, t, n, h, 1.0f) == RLENV_OK ? attention_scratch(d, t, n, h, backward ? 3 : 1) : -1;
 }
 
 int rlenv_linear_attention_forward(int dtype, int d, int64_t t, int64_t n, int64_t h, const void* q, const void* k,
@@ -164,13 +510,12 @@ int rlenv_linear_attention_forward(int dtype, int d, int64_t t, int64_t n, int64
   const int64_t* st = t > 0 ? strides : kNone;
   if (!aligned_rows(q, st, dtype, 3) || !aligned_rows(k, st + 3, dtype, 3) || !aligned_rows(v, st + 6, dtype, 3))
     return RLENV_EINVAL;
-  (void)scratch;
-  (void)scratch_bytes;
+  if (!scratch_holds(scratch, scratch_bytes, attention_scratch(d, t, n, h, 1))) return RLENV_EINVAL;
   Problem p{};
   p.t = t, p.n = n, p.h = h, p.decay = decay, p.resets = resets, p.scale = scale, p.scans = 1;
   p.scan[0] = Scan{q, k, v, {st[0], st[1], st[2]}, {st[3], st[4], st[5]}, {st[6], st[7], st[8]},
                    out, state_in, state_out, 1.0f, 1.0f, 0, 0};
-  return dispatch(dtype, d, Runner{p, as_stream(stream)});
+  return dispatch(dtype, d, Runner{p, scratch, as_stream(stream)});
 }
 
 int rlenv_linear_attention_backward(int dtype, int d, int64_t t, int64_t n, int64_t h, const void* grad_out,
@@ -188,8 +533,7 @@ int rlenv_linear_attention_backward(int dtype, int d, int64_t t, int64_t n, int6
   if (!aligned_rows(grad_out, st, dtype, 3) || !aligned_rows(q, st + 3, dtype, 3) ||
       !aligned_rows(k, st + 6, dtype, 3) || !aligned_rows(v, st + 9, dtype, 3))
     return RLENV_EINVAL;
-  (void)scratch;
-  (void)scratch_bytes;
+  if (!scratch_holds(scratch, scratch_bytes, attention_scratch(d, t, n, h, 3))) return RLENV_EINVAL;
   const Strides ds{st[0], st[1], st[2]}, qs{st[3], st[4], st[5]}, ks{st[6], st[7], st[8]}, vs{st[9], st[10], st[11]};
   Problem p{};
   p.t = t, p.n = n, p.h = h, p.decay = decay, p.resets = resets, p.scale = scale, p.scans = 3;
@@ -198,7 +542,7 @@ int rlenv_linear_attention_backward(int dtype, int d, int64_t t, int64_t n, int6
   p.scan[0] = Scan{grad_out, v, k, ds, vs, ks, grad_q, state_in, nullptr, 1.0f, 1.0f, 1, 0};
   p.scan[1] = Scan{v, grad_out, q, vs, ds, qs, grad_k, grad_state_out, nullptr, inv, scale, 1, 1};
   p.scan[2] = Scan{k, q, grad_out, ks, qs, ds, grad_v, grad_state_out, grad_state_in, inv, scale, 0, 1};
-  return dispatch(dtype, d, Runner{p, as_stream(stream)});
+  return dispatch(dtype, d, Runner{p, scratch, as_stream(stream)});
 }
 
 }  // extern "C"

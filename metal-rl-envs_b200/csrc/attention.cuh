@@ -118,5 +118,102 @@ RLENV_D void scan_tokens(const Scan& s, const Problem& p, int64_t n, int64_t h, 
       state_out[out_turned ? (col + c) * D + r : r * D + col + c] = out_mul * S[r * DB + c];
 }
 
+// ---------------------------------------------------------------------------
+// The chunked form. kChunk tokens at a time: with Z the carry at the chunk's start,
+//     out = scale (w_i x_i Z + (W * (X A')) B),    Z <- g^L Z + (l * A)' B,
+// W the weights w_ij (zero above the diagonal) and l_j = g^(L - f - j) the decay from token j to
+// the chunk's end: four matrix products on mma.sync with float32 accumulators.
+//
+// Precision. A matrix operand is a sum of 16-bit planes. bfloat16 inputs are one plane, exactly;
+// float32 inputs three (8 + 8 + 8 bits of mantissa); the weighted products and the carry, which
+// are float32, two for bfloat16 outputs (their own rounding is 2^-9) and three for float32 ones;
+// the decayed keys three, since the carry goes out in float32. Of the products of planes those
+// below 2^-24 of the whole are left out.
+constexpr int kChunk = 64;
+constexpr int kThreads = 128;  // four warps, each 16 tokens of the chunk
+
+template <typename T, int D>
+struct Shape {
+  static constexpr int kIn = sizeof(T) == 4 ? 3 : 1;    // planes of x, a, b
+  static constexpr int kMid = sizeof(T) == 4 ? 3 : 2;   // of the weighted products and the carry
+  static constexpr int kKeys = 3;                       // of the decayed keys
+  static constexpr int DB = D < 64 ? D : 64;            // columns of the carry that a block owns
+  static constexpr int PX = D + 8, PB = DB + 8;         // row pitches: 16 bytes past a multiple of 32,
+                                                        // so that eight rows' pieces fall in distinct banks
+  static constexpr int kX = kChunk * PX, kB = kChunk * PB, kS = D * PB;  // a plane's elements
+  static constexpr int kSmem = 2 * (kIn * (2 * kX + kB) + kMid * kS);
+  // The carry's rows and columns by warp: RG groups of rows, CG of columns.
+  static constexpr int MT = D > 64 ? D / 64 : 1;        // 16-row tiles a warp
+  static constexpr int RG = D / (16 * MT);
+  static constexpr int CG = 4 / RG < DB / 16 ? 4 / RG : DB / 16;
+  static constexpr int NT = DB / CG / 8;                // 8-column tiles a warp
+};
+
+RLENV_D uint32_t shared_address(const void* p) { return uint32_t(__cvta_generic_to_shared(p)); }
+
+RLENV_D void load_matrices(uint32_t r[4], uint32_t at) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at) : "memory");
+}
+RLENV_D void load_matrices_turned(uint32_t r[4], uint32_t at) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at) : "memory");
+}
+RLENV_D void multiply(float c[4], const uint32_t a[4], uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+               "{%0,%1,%2,%3};"
+               : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+               : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+RLENV_D uint32_t pack(float lo, float hi) {
+  const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+RLENV_D float low_half(uint32_t v) { return __uint_as_float(v << 16); }
+RLENV_D float high_half(uint32_t v) { return __uint_as_float(v & 0xffff0000u); }
+
+// A pair of float32 values as N planes of bfloat16 pairs: each the rest of the ones before it.
+template <int N>
+RLENV_D void split_pair(float lo, float hi, uint32_t* planes, int stride) {
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const uint32_t v = pack(lo, hi);
+    planes[i * stride] = v;
+    lo -= low_half(v), hi -= high_half(v);
+  }
+}
+
+RLENV_D void copy_async_16(uint32_t to, const void* from, bool real) {  // zeros where not real
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(real ? 16 : 0) : "memory");
+}
+RLENV_D void copies_landed() { asm volatile("cp.async.wait_all;" ::: "memory"); }
+
+// W columns of kChunk rows from token position `first` (positions past `last` are zeros) into planes
+// at `to`, pitch P.
+template <typename T, int W, int P, int kPlane>
+RLENV_D void load_tile(const T* base, int64_t stride, const Scan& s, int64_t tokens, int64_t first, int64_t last,
+                       __nv_bfloat16* to) {
+  constexpr int kPer = 16 / sizeof(T), kPieces = W / kPer;
+  const uint32_t at = shared_address(to);
+#pragma unroll 4
+  for (int e = threadIdx.x; e < kChunk * kPieces; e += kThreads) {
+    const int r = e / kPieces, c = e % kPieces * kPer;
+    const int64_t i = first + r;
+    const bool real = i < last;
+    const T* from = base + (real ? (s.reverse ? tokens - 1 - i : i) : 0) * stride + c;
+    if constexpr (sizeof(T) == 2) {
+      copy_async_16(at + (r * P + c) * 2, from, real);
+    } else {
+      const float4 v = real ? __ldg(reinterpret_cast<const float4*>(from)) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      uint32_t lo[3], hi[3];
+      split_pair<3>(v.x, v.y, lo, 1);
+      split_pair<3>(v.z, v.w, hi, 1);
+#pragma unroll
+      for (int q = 0; q < 3; ++q) *reinterpret_cast<uint2*>(to + q * kPlane + r * P + c) = make_uint2(lo[q], hi[q]);
+    }
+  }
+}
+
 }  // namespace attn
 }  // namespace rlenv

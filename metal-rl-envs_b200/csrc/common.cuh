@@ -269,6 +269,11 @@ inline int launch_status() {
   return e == cudaSuccess ? RLENV_OK : int(e);
 }
 
+// Whether a caller's working memory has the size needed, on a 256-byte boundary.
+inline bool scratch_holds(const void* scratch, int64_t bytes, int64_t need) {
+  return need == 0 || (scratch && bytes >= need && reinterpret_cast<uintptr_t>(scratch) % 256 == 0);
+}
+
 inline cudaStream_t as_stream(void* s) { return reinterpret_cast<cudaStream_t>(s); }
 
 inline bool valid_dtype(int dt) { return dt == RLENV_I32 || dt == RLENV_I64 || dt == RLENV_U8; }

@@ -193,9 +193,8 @@ int rlenv_gated_ffn_backward(int dtype, int activation, int64_t m, int64_t k, in
   using namespace rlenv;
   if (const int rc = check_ffn(dtype, activation, m, k, f)) return rc;
   if (m == 0 || k == 0 || f == 0) return RLENV_EINVAL;
-  if (!grad_out || !x || !w_gate || !w_up || !grad_x || !grad_w_gate || !grad_w_up || !scratch) return RLENV_EINVAL;
-  if (scratch_bytes < rlenv_gated_ffn_scratch_bytes(dtype, m, k, f, 1) || reinterpret_cast<uintptr_t>(scratch) % 256)
-    return RLENV_EINVAL;
+  if (!grad_out || !x || !w_gate || !w_up || !grad_x || !grad_w_gate || !grad_w_up) return RLENV_EINVAL;
+  if (!scratch_holds(scratch, scratch_bytes, rlenv_gated_ffn_scratch_bytes(dtype, m, k, f, 1))) return RLENV_EINVAL;
   return dtype == RLENV_F32
              ? ffn_backward<float>(grad_out, x, w_gate, w_up, m, k, f, activation, grad_x, grad_w_gate, grad_w_up,
                                    scratch, as_stream(stream))
