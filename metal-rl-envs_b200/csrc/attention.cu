@@ -149,17 +149,12 @@ chunk_kernel(const __grid_constant__ Problem p, const __grid_constant__ Split sp
 #pragma unroll
         for (int q = 0; q < C::kIn; ++q) load_matrices(x[q], xa + 2 * (q * C::kX + 16 * k));
 #pragma unroll
-        for (int t = 0; t < DB / 16; ++t)
+        for (int t = 0; t < DB / 16; ++t) {
+          uint32_t v[C::kMid][4];
 #pragma unroll
-          for (int q = 0; q < C::kMid; ++q) {
-            uint32_t v[4];
-            load_matrices_turned(v, sa + 2 * (q * C::kS + 16 * k * C::PB + 16 * t));
-#pragma unroll
-            for (int u = 0; u < C::kIn && u + q < 3; ++u) {
-              multiply(o[2 * t], x[u], v[0], v[1]);
-              multiply(o[2 * t + 1], x[u], v[2], v[3]);
-            }
-          }
+          for (int q = 0; q < C::kMid; ++q) load_matrices_turned(v[q], sa + 2 * (q * C::kS + 16 * k * C::PB + 16 * t));
+          multiply_planes<C::kIn, C::kMid, C::kFloat>(o[2 * t], o[2 * t + 1], x, v);
+        }
       }
       const int row[2] = {16 * warp + gr, 16 * warp + gr + 8};
       int seen[2] = {0, 0};
@@ -178,16 +173,10 @@ chunk_kernel(const __grid_constant__ Problem p, const __grid_constant__ Split sp
           uint32_t x[C::kIn][4];
 #pragma unroll
           for (int q = 0; q < C::kIn; ++q) load_matrices(x[q], xa + 2 * (q * C::kX + 16 * k));
+          uint32_t v[C::kIn][4];
 #pragma unroll
-          for (int q = 0; q < C::kIn; ++q) {
-            uint32_t v[4];
-            load_matrices(v, aa + 2 * (q * C::kX + 16 * jb * C::PX + 16 * k));
-#pragma unroll
-            for (int u = 0; u < C::kIn && u + q < 3; ++u) {
-              multiply(w[0], x[u], v[0], v[1]);
-              multiply(w[1], x[u], v[2], v[3]);
-            }
-          }
+          for (int q = 0; q < C::kIn; ++q) load_matrices(v[q], aa + 2 * (q * C::kX + 16 * jb * C::PX + 16 * k));
+          multiply_planes<C::kIn, C::kIn, C::kFloat>(w[0], w[1], x, v);
         }
         const float far = jb < warp ? power(log2_g, 16 * (warp - 1 - jb)) : 1.0f;
 #pragma unroll
@@ -203,17 +192,12 @@ chunk_kernel(const __grid_constant__ Problem p, const __grid_constant__ Split sp
         split_pair<C::kMid>(w[1][0], w[1][1], &wp[0][2], 4);
         split_pair<C::kMid>(w[1][2], w[1][3], &wp[0][3], 4);
 #pragma unroll
-        for (int t = 0; t < DB / 16; ++t)
+        for (int t = 0; t < DB / 16; ++t) {
+          uint32_t v[C::kIn][4];
 #pragma unroll
-          for (int q = 0; q < C::kIn; ++q) {
-            uint32_t v[4];
-            load_matrices_turned(v, ba + 2 * (q * C::kB + 16 * jb * C::PB + 16 * t));
-#pragma unroll
-            for (int u = 0; u < C::kMid && u + q < 3; ++u) {
-              multiply(o[2 * t], wp[u], v[0], v[1]);
-              multiply(o[2 * t + 1], wp[u], v[2], v[3]);
-            }
-          }
+          for (int q = 0; q < C::kIn; ++q) load_matrices_turned(v[q], ba + 2 * (q * C::kB + 16 * jb * C::PB + 16 * t));
+          multiply_planes<C::kMid, C::kIn, C::kFloat>(o[2 * t], o[2 * t + 1], wp, v);
+        }
       }
       T* const out = static_cast<T*>(s.out);
 #pragma unroll
@@ -267,19 +251,14 @@ chunk_kernel(const __grid_constant__ Problem p, const __grid_constant__ Split sp
             split_pair<C::kKeys>((u & 2 ? l2 : l0) * lo[u], (u & 2 ? l3 : l1) * hi[u], &key[m][0][u], 4);
         }
 #pragma unroll
-        for (int t = 0; t < C::NT / 2; ++t)
+        for (int t = 0; t < C::NT / 2; ++t) {
+          uint32_t v[C::kIn][4];
 #pragma unroll
-          for (int q = 0; q < C::kIn; ++q) {
-            uint32_t v[4];
-            load_matrices_turned(v, bt + 2 * (q * C::kB + 16 * j * C::PB + 16 * t));
+          for (int q = 0; q < C::kIn; ++q) load_matrices_turned(v[q], bt + 2 * (q * C::kB + 16 * j * C::PB + 16 * t));
 #pragma unroll
-            for (int m = 0; m < C::MT; ++m)
-#pragma unroll
-              for (int u = 0; u < C::kKeys && u + q < 3; ++u) {
-                multiply(z[m][2 * t], key[m][u], v[0], v[1]);
-                multiply(z[m][2 * t + 1], key[m][u], v[2], v[3]);
-              }
-          }
+          for (int m = 0; m < C::MT; ++m)
+            multiply_planes<C::kKeys, C::kIn, C::kFloat>(z[m][2 * t], z[m][2 * t + 1], key[m], v);
+        }
       }
     }
     cut = cut || resets != 0;

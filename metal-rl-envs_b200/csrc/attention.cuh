@@ -137,6 +137,7 @@ struct Shape {
   static constexpr int kIn = sizeof(T) == 4 ? 3 : 1;    // planes of x, a, b
   static constexpr int kMid = sizeof(T) == 4 ? 3 : 2;   // of the weighted products and the carry
   static constexpr int kKeys = 3;                       // of the decayed keys
+  static constexpr bool kFloat = sizeof(T) == 4;
   static constexpr int DB = D < 64 ? D : 64;            // columns of the carry that a block owns
   static constexpr int PX = D + 8, PB = DB + 8;         // row pitches: 16 bytes past a multiple of 32,
                                                         // so that eight rows' pieces fall in distinct banks
@@ -164,6 +165,28 @@ RLENV_D void multiply(float c[4], const uint32_t a[4], uint32_t b0, uint32_t b1)
                "{%0,%1,%2,%3};"
                : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+// c0, c1 (two 8-column tiles) += a b over all pairs of planes worth it, the small ones first. The tensor
+// core truncates as it accumulates: for float32 results (three planes of data) the pairs are summed from
+// zero and added to c in a rounded addition, or the error of long sums grows to a few 1e-6.
+template <int NA, int NB, bool kFloat>
+RLENV_D void multiply_planes(float c0[4], float c1[4], const uint32_t (&a)[NA][4], const uint32_t (&b)[NB][4]) {
+  float s0[4] = {}, s1[4] = {};
+#pragma unroll
+  for (int order = 2; order >= 0; --order)
+#pragma unroll
+    for (int u = 0; u <= order; ++u) {
+      const int q = order - u;
+      if (u < NA && q < NB) {
+        multiply(kFloat ? s0 : c0, a[u], b[q][0], b[q][1]);
+        multiply(kFloat ? s1 : c1, a[u], b[q][2], b[q][3]);
+      }
+    }
+  if constexpr (kFloat) {
+#pragma unroll
+    for (int q = 0; q < 4; ++q) c0[q] += s0[q], c1[q] += s1[q];
+  }
 }
 
 RLENV_D uint32_t pack(float lo, float hi) {

@@ -1,0 +1,142 @@
+// The sm_100a instructions that the matrix kernels are written with: barriers in shared memory,
+// tensor copies, and the tensor cores with their accumulators in tensor memory.
+#pragma once
+
+#include <cuda.h>
+
+#include "common.cuh"
+
+namespace rlenv {
+namespace bw {
+
+RLENV_D uint32_t shared_at(const void* p) { return uint32_t(__cvta_generic_to_shared(p)); }
+
+// ---- barriers ---------------------------------------------------------------------------------
+RLENV_D void barrier_init(uint32_t bar, uint32_t count) {
+  asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count) : "memory");
+}
+RLENV_D void barrier_arrive(uint32_t bar) {
+  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+RLENV_D void barrier_expect(uint32_t bar, uint32_t bytes) {
+  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
+}
+RLENV_D bool barrier_try(uint32_t bar, uint32_t parity) {
+  uint32_t done;
+  asm volatile(
+      "{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}"
+      : "=r"(done) : "r"(bar), "r"(parity) : "memory");
+  return done != 0;
+}
+// Waits for the phase of `parity` to end. Every wait is bounded: past kTries attempts, each of which the
+// hardware suspends for a while, `dead` is set, and from then on every wait of the block gives up at once.
+constexpr int kTries = 1 << 22;
+RLENV_D bool barrier_wait(uint32_t bar, uint32_t parity, volatile int* dead) {
+  for (int i = 0; i < kTries; ++i) {
+    if (barrier_try(bar, parity)) return true;
+    if (*dead) return false;
+  }
+  *dead = 1;
+  return false;
+}
+
+// ---- tensor copies ------------------------------------------------------------------------------
+RLENV_D void prefetch_map(const CUtensorMap* map) {
+  asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory");
+}
+RLENV_D void copy_tile(uint32_t to, const CUtensorMap* map, uint32_t bar, int x, int y, int z) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(to),
+      "l"(map), "r"(bar), "r"(x), "r"(y), "r"(z)
+      : "memory");
+}
+
+// ---- tensor memory and tensor cores ---------------------------------------------------------------
+template <int kColumns>
+RLENV_D void tmem_alloc(uint32_t slot) {  // one warp
+  asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(slot), "r"(kColumns) : "memory");
+  asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+}
+template <int kColumns>
+RLENV_D void tmem_free(uint32_t at) {  // the same warp
+  asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(at), "r"(kColumns) : "memory");
+}
+RLENV_D void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+RLENV_D void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+RLENV_D void commit(uint32_t bar) {  // arrives at bar when the matrix products issued so far are done
+  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+}
+RLENV_D void multiply(uint32_t d, uint64_t a, uint64_t b, uint32_t kind, bool accumulate) {
+  asm volatile(
+      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
+      " tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}" ::"r"(d),
+      "l"(a), "l"(b), "r"(kind), "r"(uint32_t(accumulate))
+      : "memory");
+}
+// 32 columns of this warp's 32 lanes: lane l gets its row's columns. The wait stands in the same
+// statement, so that no use of the registers comes before it.
+RLENV_D void tmem_load32(float (&v)[32], uint32_t at) {
+  uint32_t r[32];
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+      "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,"
+      "%30,%31}, [%32];\n"
+      "tcgen05.wait::ld.sync.aligned;"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
+        "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+        "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(at)
+      : "memory");
+#pragma unroll
+  for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
+}
+
+// A bfloat16 operand in shared memory, rows of 128 bytes swizzled by eights as the tensor copies write
+// them. K-major: a row is 64 elements of the contraction, eight rows 1,024 bytes apart from the next
+// eight. MN-major: a row is 64 elements of the other axis, eight steps of the contraction 1,024 bytes
+// apart from the next eight and the next 64 elements `block` bytes away.
+RLENV_D uint64_t operand(uint32_t at, bool mn_major, uint32_t block) {
+  return uint64_t((at & 0x3ffff) >> 4) | uint64_t(mn_major ? block >> 4 : 1) << 16 | uint64_t(1024 >> 4) << 32 |
+         uint64_t(1) << 46 | uint64_t(2) << 61;
+}
+// bfloat16 x bfloat16 -> float32, M x N.
+constexpr uint32_t product_kind(int m, int n, bool a_mn, bool b_mn) {
+  return 1u << 4 | 1u << 7 | 1u << 10 | uint32_t(a_mn) << 15 | uint32_t(b_mn) << 16 | uint32_t(n >> 3) << 17 |
+         uint32_t(m >> 4) << 24;
+}
+
+// ---- host: tensor maps -----------------------------------------------------------------------------
+using EncodeTiled = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
+                                 const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
+                                 CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+inline EncodeTiled encode_tiled() {  // the driver's function, looked up once
+  static const EncodeTiled fn = [] {
+    void* p = nullptr;
+    cudaDriverEntryPointQueryResult found;
+    if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &p, 12000, cudaEnableDefault, &found) != cudaSuccess ||
+        found != cudaDriverEntryPointSuccess)
+      p = nullptr;
+    return reinterpret_cast<EncodeTiled>(p);
+  }();
+  return fn;
+}
+
+// A (slices, rows, cols) bfloat16 array with `pitch` elements between rows, copied in boxes of 64
+// columns and box_rows rows; what lies past cols or rows reads as zero. 0 or a cudaError_t.
+inline int tile_map(CUtensorMap* map, const void* base, int64_t cols, int64_t rows, int64_t slices, int64_t pitch,
+                    int box_rows) {
+  const EncodeTiled encode = encode_tiled();
+  if (!encode) return int(cudaErrorNotSupported);
+  const cuuint64_t dims[3] = {cuuint64_t(cols), cuuint64_t(rows), cuuint64_t(slices)};
+  const cuuint64_t strides[2] = {cuuint64_t(pitch) * 2, cuuint64_t(pitch) * 2 * cuuint64_t(rows)};
+  const cuuint32_t box[3] = {64, cuuint32_t(box_rows), 1}, steps[3] = {1, 1, 1};
+  const CUresult rc = encode(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(base), dims, strides, box,
+                             steps, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                             CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return rc == CUDA_SUCCESS ? 0 : int(cudaErrorInvalidValue);
+}
+
+}  // namespace bw
+}  // namespace rlenv

@@ -5,7 +5,9 @@ x is (..., K), the weights (K, F) as es.unflatten's (in, out) layout, out (..., 
 float32 or bfloat16; sums are in 32 bits. activation is "silu" or "gelu" (the exact normal
 distribution). `backward` forms both products again instead of keeping them. `apply` is the
 differentiable form. The projection back to K is a plain matrix product and is left to the caller.
-The reference's policies are tanh MLPs (es.py:156-164); there is no counterpart there.
+float32 operands
+go through the tensor cores as sums of three bfloat16 terms: results have float32's precision, but an
+infinity, or a magnitude above bfloat16's 3.39e38, comes out as NaN. The reference's policies are tanh MLPs (es.py:156-164); there is no counterpart there.
 """
 
 import torch
@@ -13,6 +15,12 @@ import torch
 import rlenv_lib as _rl
 
 ACTIVATIONS = {"silu": 0, "gelu": 1}
+
+
+def _dense(x):
+    """x itself where it is dense and on a 16-byte boundary, else a copy that is."""
+    x = x.contiguous()
+    return x if x.data_ptr() % 16 == 0 else x.clone()
 
 
 def _check(x, w_gate, w_up, activation, grad_out=None):
@@ -33,7 +41,7 @@ def _check(x, w_gate, w_up, activation, grad_out=None):
 def forward(x, w_gate, w_up, activation="silu"):
     """act(x w_gate) * (x w_up), (..., F)."""
     m, k, f, code, dev = _check(x, w_gate, w_up, activation)
-    x, w_gate, w_up = x.contiguous(), w_gate.contiguous(), w_up.contiguous()
+    x, w_gate, w_up = _dense(x), _dense(w_gate), _dense(w_up)
     lib = _rl.lib()
     with torch.cuda.device(dev):
         out = torch.empty((*x.shape[:-1], f), dtype=x.dtype, device=dev)
@@ -49,7 +57,7 @@ def backward(grad_out, x, w_gate, w_up, activation="silu"):
     m, k, f, code, dev = _check(x, w_gate, w_up, activation, grad_out)
     if 0 in (m, k, f):  # sums over nothing
         return torch.zeros_like(x), torch.zeros_like(w_gate), torch.zeros_like(w_up)
-    grad_out, x, w_gate, w_up = (y.contiguous() for y in (grad_out, x, w_gate, w_up))
+    grad_out, x, w_gate, w_up = (_dense(y) for y in (grad_out, x, w_gate, w_up))
     lib = _rl.lib()
     with torch.cuda.device(dev):
         dx, dwg, dwu = torch.empty_like(x), torch.empty_like(w_gate), torch.empty_like(w_up)
