@@ -15,8 +15,14 @@ RLENV_D uint32_t shared_at(const void* p) { return uint32_t(__cvta_generic_to_sh
 RLENV_D void barrier_init(uint32_t bar, uint32_t count) {
   asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count) : "memory");
 }
-RLENV_D void barrier_arrive(uint32_t bar) {
-  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
+// The same place in the shared memory of block `rank` of the cluster.
+RLENV_D uint32_t in_block(uint32_t at, uint32_t rank) {
+  uint32_t r;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(at), "r"(rank));
+  return r;
+}
+RLENV_D void barrier_arrive(uint32_t cluster_bar) {
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_bar) : "memory");
 }
 RLENV_D void barrier_expect(uint32_t bar, uint32_t bytes) {
   asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
@@ -24,7 +30,7 @@ RLENV_D void barrier_expect(uint32_t bar, uint32_t bytes) {
 RLENV_D bool barrier_try(uint32_t bar, uint32_t parity) {
   uint32_t done;
   asm volatile(
-      "{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}"
+      "{\n .reg .pred p;\n mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}"
       : "=r"(done) : "r"(bar), "r"(parity) : "memory");
   return done != 0;
 }
@@ -44,32 +50,49 @@ RLENV_D bool barrier_wait(uint32_t bar, uint32_t parity, volatile int* dead) {
 RLENV_D void prefetch_map(const CUtensorMap* map) {
   asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory");
 }
-RLENV_D void copy_tile(uint32_t to, const CUtensorMap* map, uint32_t bar, int x, int y, int z) {
+// Into this block's shared memory; the bytes are counted at a barrier of either block of the pair.
+RLENV_D void copy_tile(uint32_t to, const CUtensorMap* map, uint32_t cluster_bar, int x, int y, int z) {
   asm volatile(
-      "cp.async.bulk.tensor.3d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(to),
-      "l"(map), "r"(bar), "r"(x), "r"(y), "r"(z)
+      "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.cta_group::2 "
+      "[%0], [%1, {%3, %4, %5}], [%2];" ::"r"(to),
+      "l"(map), "r"(cluster_bar), "r"(x), "r"(y), "r"(z)
       : "memory");
+}
+RLENV_D uint32_t cluster_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+RLENV_D void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
 // ---- tensor memory and tensor cores ---------------------------------------------------------------
+// The two blocks of a cluster work as a pair (cta_group::2): a product of 2 x 128 rows has each block's
+// rows of A and half of B's columns in its own shared memory, and each block's rows of the result in its
+// own tensor memory. Allocation is a matter of both blocks, products of the first block's one thread.
 template <int kColumns>
 RLENV_D void tmem_alloc(uint32_t slot) {  // one warp
-  asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(slot), "r"(kColumns) : "memory");
-  asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(slot), "r"(kColumns) : "memory");
+  asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
 }
 template <int kColumns>
 RLENV_D void tmem_free(uint32_t at) {  // the same warp
-  asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(at), "r"(kColumns) : "memory");
+  asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(at), "r"(kColumns) : "memory");
 }
 RLENV_D void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 RLENV_D void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
-RLENV_D void commit(uint32_t bar) {  // arrives at bar when the matrix products issued so far are done
-  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+// Arrives at `bar` of both blocks when the matrix products issued so far are done.
+RLENV_D void commit(uint32_t bar) {
+  asm volatile(
+      "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar),
+      "h"(uint16_t(3))
+      : "memory");
 }
 RLENV_D void multiply(uint32_t d, uint64_t a, uint64_t b, uint32_t kind, bool accumulate) {
   asm volatile(
       "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
-      " tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}" ::"r"(d),
+      " tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n}" ::"r"(d),
       "l"(a), "l"(b), "r"(kind), "r"(uint32_t(accumulate))
       : "memory");
 }

@@ -5,9 +5,11 @@
 // The backward pass forms g and u again from x instead of keeping them: 2 M F values less to
 // store and read, and no rounding of g and u to the inputs' type.
 //
-// All four products run on one kernel, product_kernel: tiles of 128 rows on the tensor cores
-// (tcgen05), operands brought by tensor copies (TMA) into a ring of shared memory buffers, two
-// accumulators in tensor memory so that one tile's epilogue runs under the next one's products.
+// The products run on one kernel, product_kernel, on pairs of SMs: tiles of 2 x 128 rows on the tensor
+// cores (tcgen05, cta_group::2), operands brought by tensor copies (TMA) into rings of shared memory
+// buffers, two accumulators in tensor memory so that a tile's epilogue runs under the next one's products.
+// A pair reads a 256 x 256 tile's operands once between its two SMs, 64 bytes a clock for each; with
+// 128 x 256 tiles on single SMs it was 96, more than L2 gives, and the tensor cores ran at 56%.
 // float32 operands are sums of three bfloat16 planes (8 + 8 + 8 bits of mantissa), laid out by
 // pack_kernel; a product of two is six products of planes, the three below 2^-24 left out.
 #include <cuda_bf16.h>
@@ -55,13 +57,15 @@ pack_kernel(const T* __restrict__ from, int64_t rows, int64_t cols, int64_t pitc
 
 // ---- the product kernel ---------------------------------------------------------------------------
 
-enum Op { kForward, kGates, kInput, kWeights };  // h; dg and du; dx; dWg and dWu
+enum Op { kForward, kGates, kGradients };  // h; dg and du; dx, dWg and dWu
 
-constexpr int kRows = 128;       // of a tile
+constexpr int kRows = 128;       // of a tile, in each block of a pair
 constexpr int kStep = 64;        // of the contraction, a ring buffer's
 constexpr int kProductThreads = 384;  // copies, products, two idle warps, eight warps of epilogue
 constexpr int kEpilogueWarps = 8;
 constexpr int kTmemColumns = 512;
+constexpr int kStagePitch = 33;  // floats: a 32 x 32 tile is written by rows and read by columns, or the other
+                                 // way round, without bank conflicts
 
 template <typename T>
 struct Tile {
@@ -69,58 +73,93 @@ struct Tile {
   static constexpr int kPlanes = kFloat ? 3 : 1;
   static constexpr int kPairs = kFloat ? 6 : 1;  // products of planes
   static constexpr int kCols = kFloat ? 128 : 256;
-  static constexpr int kStageBytes = (kRows + kCols) * kStep * 2;
-  static constexpr int kStages = 196608 / kStageBytes;
-  static constexpr int kSmem = kStages * kStageBytes + 1024;  // the ring starts on a 1,024-byte boundary
+  static constexpr int kHalf = kCols / 2;        // columns of B in each block
+  static constexpr int kABytes = kRows * kStep * 2;
+  static constexpr int kRingBytes = kABytes + kHalf * kStep * 2;
+  static constexpr int kStages = kFloat ? 7 : 5;
+  static constexpr int kStageAt = kStages * kRingBytes;  // the epilogue's 32 x 32 tiles, one a warp
+  // the ring starts on a 1,024-byte boundary
+  static constexpr int kSmem = kStageAt + kEpilogueWarps * 32 * kStagePitch * 4 + 1024;
   // Steps of the contraction summed in tensor memory before the epilogue takes them out into registers
-  // (0: all). The tensor core truncates as it accumulates; rounded additions of short sums keep float32
-  // results at float32's error. Only the leading planes' product, the last to be formed, is large
-  // enough to matter.
-  static constexpr int kRun = kFloat ? 4 : 0, kSmallRun = 32;
+  // (float32 only). The tensor core truncates as it accumulates; rounded additions of short sums keep
+  // float32 results at float32's error. Of the products of planes only the leading one, the last to be
+  // formed, is large enough to need the short sums.
+  static constexpr int kRun = 4, kSmallRun = 32;
 };
 
-struct alignas(64) Product {
+struct Operands {
   CUtensorMap a, b0, b1;
-  int64_t rows, cols;     // of the result (cols: F for kForward, kGates; of one weight for kWeights)
-  int64_t depth;          // of one contraction (kInput has two, over dg Wg' and du Wu')
-  int row_tiles, col_tiles;
+};
+struct alignas(64) Product {
+  Operands in[2];         // kGradients: of dx, then of the weights' gradients; else the first
+  int64_t m, k, f;
   int act;
-  const void* dh;         // kGates
-  void *out0, *out1;      // h; dx; dWg and dWu
-  __nv_bfloat16* gates;   // kGates: (plane, dg or du, rows, pitch)
+  // Tiles: of h or the gates; of dx and of both weights.
+  int row_tiles, col_tiles, weight_rows, weight_cols;
+  int splits, split_blocks;  // of the contraction over tokens in the weights' gradients
+  const void* dh;            // kGates
+  void *out, *dwg, *dwu;     // h or dx; the weights' gradients
+  float* parts;              // (splits, 2, K, F) where splits > 1
+  __nv_bfloat16* gates;      // (plane, dg or du, M, pitch)
   int64_t pitch;
 };
 
 // Tiles are taken in bands of kBand rows of tiles, column by column, so that those in flight share
 // operands that lie in L2.
-constexpr int kBand = 16;
-struct Place {
-  int row, col;
+constexpr int kBand = 8;
+
+// A tile of work: columns from c0, rows from row tile `row`, a contraction over `blocks` steps of each of
+// `segs` segments from block k0.
+struct Work {
+  bool weights;
+  int weight, split, row, c0, k0, blocks, segs;
 };
-RLENV_D Place place(const Product& p, int tile) {
-  const int per = kBand * p.col_tiles, band = tile / per, in = tile % per;
-  const int high = min(kBand, p.row_tiles - band * kBand);
-  return {band * kBand + in % high, in / high};
+template <typename T, int kOp>
+RLENV_D Work work_of(const Product& p, int item) {
+  Work w{};
+  int rows = p.row_tiles, cols = p.col_tiles;
+  w.segs = 1;
+  if constexpr (kOp == kGradients) {
+    // the weights' longer contractions first
+    const int per = p.weight_rows * p.weight_cols;
+    w.weights = item < per * p.splits;
+    if (w.weights) {
+      w.split = item / per, item %= per;
+      rows = p.weight_rows, cols = p.weight_cols;
+      w.k0 = w.split * p.split_blocks;
+      w.blocks = min(p.split_blocks, int((p.m + kStep - 1) / kStep) - w.k0);
+    } else {
+      item -= per * p.splits;
+      w.segs = 2, w.blocks = int((p.f + kStep - 1) / kStep);
+    }
+  } else {
+    w.blocks = int((p.k + kStep - 1) / kStep);
+  }
+  const int per = kBand * cols, band = item / per, in = item % per;
+  const int high = min(kBand, rows - band * kBand);
+  w.row = band * kBand + in % high;
+  int col = in / high;
+  if (w.weights && col >= cols / 2) w.weight = 1, col -= cols / 2;
+  w.c0 = col * (kOp == kGradients ? Tile<T>::kCols : Tile<T>::kHalf);
+  return w;
 }
 
-// What a step of a tile's contraction multiplies: planes a and b (small products first), segment seg
-// (kInput), block k of the contraction.
+// What a step multiplies: planes a and b, the small products first; segment; block of the contraction.
 struct Step {
   int a, b, seg, k;
 };
-template <typename T, int kOp>
-RLENV_D Step step_of(int it, int blocks) {
-  constexpr int kSegs = kOp == kInput ? 2 : 1;
-  const int pair = it / (kSegs * blocks), in = it % (kSegs * blocks);
-  Step s{0, 0, in / blocks, in % blocks};
-  if (Tile<T>::kPairs > 1) {
+template <typename T>
+RLENV_D Step step_of(const Work& w, int it) {
+  const int per = w.segs * w.blocks, pair = it / per, in = it % per;
+  Step s{0, 0, in / w.blocks, w.k0 + in % w.blocks};
+  if (Tile<T>::kFloat) {
     switch (pair) {
       case 0: s.a = 0, s.b = 2; break;
       case 1: s.a = 2, s.b = 0; break;
       case 2: s.a = 1, s.b = 1; break;
       case 3: s.a = 0, s.b = 1; break;
       case 4: s.a = 1, s.b = 0; break;
-      default: s.a = 0, s.b = 0;
+      default: break;
     }
   }
   return s;
@@ -129,52 +168,135 @@ RLENV_D Step step_of(int it, int blocks) {
 template <typename T>
 RLENV_D bool run_ends(int it, int steps) {
   if (it + 1 == steps) return true;
-  if constexpr (!Tile<T>::kFloat) return false;
+  if (!Tile<T>::kFloat) return false;
   const int small = steps / Tile<T>::kPairs * (Tile<T>::kPairs - 1);
   if (it + 1 <= small) return it + 1 == small || (it + 1) % Tile<T>::kSmallRun == 0;
   return (it + 1 - small) % Tile<T>::kRun == 0;
 }
 
+// A warp's 32 x 32 tile between registers (a row a lane) and an array (row pitch `pitch`), rows and
+// columns past the ends left out, through shared memory so that global accesses run along rows.
 template <typename T>
-RLENV_D float load_one(const T* p, int64_t i) { return float(p[i]); }
-
-// n <= 32 values to consecutive places, by 16 bytes where the whole run is there and on the boundary.
-template <typename T>
-RLENV_D void store_run(T* to, const float (&v)[32], int n) {
-  if constexpr (sizeof(T) == 2) {
-    if (n >= 32 && reinterpret_cast<uintptr_t>(to) % 16 == 0) {
+RLENV_D void store_tile(T* to, int64_t pitch, int rows, int cols, const float (&v)[32], float* stage) {
+  const int lane = threadIdx.x & 31;
+  __syncwarp();
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        uint32_t w[4];
+  for (int i = 0; i < 32; ++i) stage[lane * kStagePitch + i] = v[i];
+  __syncwarp();
+  if (cols >= 32 && (reinterpret_cast<uintptr_t>(to) | uintptr_t(pitch * sizeof(T))) % (4 * sizeof(T)) == 0) {
+    const int c = lane % 8 * 4;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const __nv_bfloat162 x = __floats2bfloat162_rn(v[8 * i + 2 * j], v[8 * i + 2 * j + 1]);
-          w[j] = *reinterpret_cast<const uint32_t*>(&x);
+    for (int i = 0; i < 8; ++i) {
+      const int r = 4 * i + lane / 8;
+      const float* s = stage + r * kStagePitch + c;
+      if (r < rows) {
+        if constexpr (sizeof(T) == 2) {
+          const __nv_bfloat162 lo = __floats2bfloat162_rn(s[0], s[1]), hi = __floats2bfloat162_rn(s[2], s[3]);
+          *reinterpret_cast<uint2*>(to + r * pitch + c) =
+              make_uint2(*reinterpret_cast<const uint32_t*>(&lo), *reinterpret_cast<const uint32_t*>(&hi));
+        } else {
+          *reinterpret_cast<float4*>(to + r * pitch + c) = make_float4(s[0], s[1], s[2], s[3]);
         }
-        reinterpret_cast<uint4*>(to)[i] = make_uint4(w[0], w[1], w[2], w[3]);
       }
-      return;
     }
   } else {
-    if (n >= 32 && reinterpret_cast<uintptr_t>(to) % 16 == 0) {
+#pragma unroll 8
+    for (int r = 0; r < 32; ++r)
+      if (r < rows && lane < cols) to[r * pitch + lane] = T(stage[r * kStagePitch + lane]);
+  }
+}
+template <typename T>
+RLENV_D void load_tile(const T* from, int64_t pitch, int rows, int cols, float (&v)[32], float* stage) {
+  const int lane = threadIdx.x & 31;
+  __syncwarp();
+  if (cols >= 32 && (reinterpret_cast<uintptr_t>(from) | uintptr_t(pitch * sizeof(T))) % (4 * sizeof(T)) == 0) {
+    const int c = lane % 8 * 4;
 #pragma unroll
-      for (int i = 0; i < 8; ++i)
-        reinterpret_cast<float4*>(to)[i] = make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
-      return;
+    for (int i = 0; i < 8; ++i) {
+      const int r = 4 * i + lane / 8;
+      float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      if (r < rows) {
+        if constexpr (sizeof(T) == 2) {
+          const uint2 w = __ldg(reinterpret_cast<const uint2*>(from + r * pitch + c));
+          x = make_float4(__uint_as_float(w.x << 16), __uint_as_float(w.x & 0xffff0000u), __uint_as_float(w.y << 16),
+                          __uint_as_float(w.y & 0xffff0000u));
+        } else {
+          x = __ldg(reinterpret_cast<const float4*>(from + r * pitch + c));
+        }
+      }
+      float* s = stage + r * kStagePitch + c;
+      s[0] = x.x, s[1] = x.y, s[2] = x.z, s[3] = x.w;
+    }
+  } else {
+#pragma unroll 8
+    for (int r = 0; r < 32; ++r)
+      stage[r * kStagePitch + lane] = r < rows && lane < cols ? float(from[r * pitch + lane]) : 0.0f;
+  }
+  __syncwarp();
+#pragma unroll
+  for (int i = 0; i < 32; ++i) v[i] = stage[lane * kStagePitch + i];
+}
+
+// A 32 x 32 piece of a tile's results: rows from r0, columns from c (of h, a weight or dx). v holds its
+// values or gates, u its ups.
+template <typename T, int kOp>
+RLENV_D void finish(const Product& p, const Work& w, int64_t r0, int64_t c, float (&v)[32], float (&u)[32],
+                    float* stage) {
+  constexpr bool kFast = !Tile<T>::kFloat;
+  if constexpr (kOp == kGradients) {
+    const int64_t all_rows = w.weights ? p.k : p.m, all_cols = w.weights ? p.f : p.k;
+    if (r0 >= all_rows || c >= all_cols) return;
+    const int rows = int(min(int64_t(32), all_rows - r0)), cols = int(min(int64_t(32), all_cols - c));
+    if (w.weights && p.splits > 1) {
+      store_tile(p.parts + ((int64_t(w.split) * 2 + w.weight) * p.k + r0) * p.f + c, p.f, rows, cols, v, stage);
+    } else {
+      T* to = static_cast<T*>(w.weights ? (w.weight ? p.dwu : p.dwg) : p.out);
+      store_tile(to + r0 * all_cols + c, all_cols, rows, cols, v, stage);
+    }
+  } else {
+    if (r0 >= p.m || c >= p.f) return;
+    const int rows = int(min(int64_t(32), p.m - r0)), cols = int(min(int64_t(32), p.f - c));
+    if constexpr (kOp == kForward) {
+#pragma unroll
+      for (int i = 0; i < 32; ++i) {
+        float y, slope;
+        activate<kFast>(p.act, v[i], &y, &slope);
+        v[i] = y * u[i];
+      }
+      store_tile(static_cast<T*>(p.out) + r0 * p.f + c, p.f, rows, cols, v, stage);
+    } else {
+      float d[32];
+      load_tile(static_cast<const T*>(p.dh) + r0 * p.f + c, p.f, rows, cols, d, stage);
+#pragma unroll
+      for (int i = 0; i < 32; ++i) {
+        float y, slope;
+        activate<kFast>(p.act, v[i], &y, &slope);
+        v[i] = d[i] * u[i] * slope;
+        u[i] = d[i] * y;
+      }
+#pragma unroll 1
+      for (int q = 0; q < Tile<T>::kPlanes; ++q) {
+        __nv_bfloat16* to = p.gates + (2 * q * p.m + r0) * p.pitch + c;
+        store_tile(to, p.pitch, rows, cols, v, stage);
+        store_tile(to + p.m * p.pitch, p.pitch, rows, cols, u, stage);
+        if (Tile<T>::kPlanes > 1) {
+#pragma unroll
+          for (int i = 0; i < 32; ++i) {
+            v[i] -= __bfloat162float(__float2bfloat16_rn(v[i]));
+            u[i] -= __bfloat162float(__float2bfloat16_rn(u[i]));
+          }
+        }
+      }
     }
   }
-#pragma unroll
-  for (int i = 0; i < 32; ++i)
-    if (i < n) to[i] = T(v[i]);
 }
 
 template <typename T, int kOp>
-__global__ void __launch_bounds__(kProductThreads, 1) product_kernel(const __grid_constant__ Product p) {
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kProductThreads, 1)
+product_kernel(const __grid_constant__ Product p, int items) {
   using C = Tile<T>;
-  constexpr bool kPaired = kOp == kForward || kOp == kGates;  // half a tile's columns are gates, half ups
-  constexpr bool kMnA = kOp == kWeights, kMnB = kOp != kInput;
-  constexpr int kSegs = kOp == kInput ? 2 : 1;
-  constexpr uint32_t kABytes = kRows * kStep * 2, kHalfB = C::kCols / 2 * kStep * 2, kBox = 64 * kStep * 2;
+  constexpr bool kPaired = kOp != kGradients;  // half of a tile's columns are gates, half ups
+  constexpr uint32_t kBox = 64 * kStep * 2;
   extern __shared__ unsigned char raw[];
   __shared__ __align__(8) uint64_t bars[2 * C::kStages + 4];
   __shared__ uint32_t tmem_slot;
@@ -184,88 +306,80 @@ __global__ void __launch_bounds__(kProductThreads, 1) product_kernel(const __gri
   const uint32_t full = bw::shared_at(bars), empty = full + 8 * C::kStages;
   const uint32_t summed = empty + 8 * C::kStages, taken = summed + 16;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int rank = int(bw::cluster_rank());
   if (threadIdx.x == 0) {
     for (int i = 0; i < C::kStages; ++i) bw::barrier_init(full + 8 * i, 1), bw::barrier_init(empty + 8 * i, 1);
-    for (int i = 0; i < 2; ++i) bw::barrier_init(summed + 8 * i, 1), bw::barrier_init(taken + 8 * i, kEpilogueWarps);
+    for (int i = 0; i < 2; ++i) bw::barrier_init(summed + 8 * i, 1), bw::barrier_init(taken + 8 * i, 2 * kEpilogueWarps);
     dead_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (warp == 2) bw::tmem_alloc<kTmemColumns>(bw::shared_at(&tmem_slot));
   bw::fence_before();
   __syncthreads();
+  bw::cluster_sync();
   bw::fence_after();
   const uint32_t tmem = tmem_slot;
-  const int tiles = p.row_tiles * p.col_tiles;
-  const int blocks = int((p.depth + kStep - 1) / kStep), steps = C::kPairs * kSegs * blocks;
+  const int first = blockIdx.x / 2, stride = gridDim.x / 2;
 
   if (warp == 0) {
     if (lane == 0) {
-      bw::prefetch_map(&p.a);
-      bw::prefetch_map(&p.b0);
-      if (kOp != kWeights) bw::prefetch_map(&p.b1);
+      // Both blocks copy their rows of A and their columns of B; all bytes count at the first block's barrier.
       int stage = 0;
       uint32_t phase = 0, used = 0;  // used: stages that have been filled at least once
       bool ok = true;
-      for (int tile = blockIdx.x; tile < tiles && ok; tile += gridDim.x) {
-        const Place at = place(p, tile);
-        const int half_cols = p.col_tiles / 2;
-        const int weight = kOp == kWeights && at.col >= half_cols;
-        const int r0 = at.row * kRows;
-        const int c0 = (kOp == kWeights ? at.col - weight * half_cols : at.col) * (kPaired ? C::kCols / 2 : C::kCols);
+      const uint32_t full_at = bw::in_block(full, 0);
+      for (int item = first; item < items && ok; item += stride) {
+        const Work w = work_of<T, kOp>(p, item);
+        const Operands& in = p.in[kOp == kGradients && w.weights];
+        const int r0 = (2 * w.row + rank) * kRows, steps = C::kPairs * w.segs * w.blocks;
         for (int it = 0; it < steps; ++it) {
-          const Step s = step_of<T, kOp>(it, blocks);
+          const Step s = step_of<T>(w, it);
           const int k0 = s.k * kStep;
           if (!(ok = bw::barrier_wait(empty + 8 * stage, phase ^ 1, dead))) break;
-          const uint32_t bar = full + 8 * stage, a = ring + stage * C::kStageBytes, b = a + kABytes;
-          bw::barrier_expect(bar, C::kStageBytes);
-          if (kMnA) {
-            for (int i = 0; i < kRows / 64; ++i) bw::copy_tile(a + i * kBox, &p.a, bar, r0 + 64 * i, k0, s.a);
+          if (rank == 0) bw::barrier_expect(full + 8 * stage, 2 * C::kRingBytes);
+          const uint32_t bar = full_at + 8 * stage, a = ring + stage * C::kRingBytes, b = a + C::kABytes;
+          if (kPaired) {  // A by rows of the contraction's axis; gates in the first block, ups in the second
+            bw::copy_tile(a, &in.a, bar, k0, r0, s.a);
+            for (int i = 0; i < C::kHalf / 64; ++i)
+              bw::copy_tile(b + i * kBox, rank ? &in.b1 : &in.b0, bar, w.c0 + 64 * i, k0, s.b);
+          } else if (w.weights) {
+            for (int i = 0; i < kRows / 64; ++i) bw::copy_tile(a + i * kBox, &in.a, bar, r0 + 64 * i, k0, s.a);
+            for (int i = 0; i < C::kHalf / 64; ++i)
+              bw::copy_tile(b + i * kBox, &in.b0, bar, w.c0 + rank * C::kHalf + 64 * i, k0, 2 * s.b + w.weight);
           } else {
-            bw::copy_tile(a, &p.a, bar, k0, r0, kOp == kInput ? 2 * s.a + s.seg : s.a);
-          }
-          if (kPaired) {
-            for (int i = 0; i < C::kCols / 128; ++i) {
-              bw::copy_tile(b + i * kBox, &p.b0, bar, c0 + 64 * i, k0, s.b);
-              bw::copy_tile(b + kHalfB + i * kBox, &p.b1, bar, c0 + 64 * i, k0, s.b);
-            }
-          } else if (kOp == kInput) {
-            for (int i = 0; i < C::kCols / 128; ++i)
-              bw::copy_tile(b + i * 2 * kBox, s.seg ? &p.b1 : &p.b0, bar, k0, c0 + 128 * i, s.b);
-          } else {
-            for (int i = 0; i < C::kCols / 64; ++i)
-              bw::copy_tile(b + i * kBox, &p.b0, bar, c0 + 64 * i, k0, 2 * s.b + weight);
+            bw::copy_tile(a, &in.a, bar, k0, r0, 2 * s.a + s.seg);
+            bw::copy_tile(b, s.seg ? &in.b1 : &in.b0, bar, k0, w.c0 + rank * C::kHalf, s.b);
           }
           used |= 1u << stage;
           if (++stage == C::kStages) stage = 0, phase ^= 1;
         }
       }
-      if (!ok) {  // the copies in flight land before the block may end
+      if (!ok && rank == 0) {  // the copies in flight land before the blocks may end
         int unused = 0;
         for (int i = 0; i < C::kStages; ++i)
-          if (used >> i & 1) {
-            const uint32_t last = i < stage ? phase : phase ^ 1;
-            bw::barrier_wait(full + 8 * i, last, &unused);
-            unused = 0;
-          }
+          if (used >> i & 1) bw::barrier_wait(full + 8 * i, i < stage ? phase : phase ^ 1, &unused), unused = 0;
       }
     }
   } else if (warp == 1) {
-    if (lane == 0) {
-      constexpr uint32_t kind = bw::product_kind(kRows, C::kCols, kMnA, kMnB);
+    if (lane == 0 && rank == 0) {
       int stage = 0, buffer = 0;
       uint32_t phase = 0, buffer_phase = 0;
       bool ok = true;
-      for (int tile = blockIdx.x; tile < tiles && ok; tile += gridDim.x) {
+      for (int item = first; item < items && ok; item += stride) {
+        const Work w = work_of<T, kOp>(p, item);
+        const int steps = C::kPairs * w.segs * w.blocks;
+        const bool mn_a = w.weights, mn_b = kPaired || w.weights;
+        const uint32_t kind = bw::product_kind(2 * kRows, C::kCols, mn_a, mn_b);
         bool fresh = true;
         for (int it = 0; it < steps; ++it) {
           if (fresh && !(ok = bw::barrier_wait(taken + 8 * buffer, buffer_phase ^ 1, dead))) break;
           if (!(ok = bw::barrier_wait(full + 8 * stage, phase, dead))) break;
           bw::fence_after();
-          const uint32_t a = ring + stage * C::kStageBytes, b = a + kABytes;
+          const uint32_t a = ring + stage * C::kRingBytes, b = a + C::kABytes;
 #pragma unroll
           for (int k = 0; k < kStep / 16; ++k)
-            bw::multiply(tmem + buffer * C::kCols, bw::operand(a + k * (kMnA ? 2048 : 32), kMnA, kBox),
-                         bw::operand(b + k * (kMnB ? 2048 : 32), kMnB, kBox), kind, !(fresh && k == 0));
+            bw::multiply(tmem + buffer * C::kCols, bw::operand(a + k * (mn_a ? 2048 : 32), mn_a, kBox),
+                         bw::operand(b + k * (mn_b ? 2048 : 32), mn_b, kBox), kind, !(fresh && k == 0));
           bw::commit(empty + 8 * stage);
           fresh = run_ends<T>(it, steps);
           if (fresh) {
@@ -278,62 +392,28 @@ __global__ void __launch_bounds__(kProductThreads, 1) product_kernel(const __gri
     }
   } else if (warp >= 4) {
     const int quarter = warp & 3, half = (warp - 4) >> 2;
+    float* const own_stage = reinterpret_cast<float*>(raw + (ring - bw::shared_at(raw)) + C::kStageAt) +
+                             (warp - 4) * 32 * kStagePitch;
     constexpr int kMine = C::kCols / 2;  // columns of the accumulator that a thread reads
     int buffer = 0;
     uint32_t buffer_phase = 0;
     bool ok = true;
-    for (int tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
-      const Place at = place(p, tile);
-      const int half_cols = p.col_tiles / 2;
-      const int weight = kOp == kWeights && at.col >= half_cols;
-      const int64_t row = int64_t(at.row) * kRows + 32 * quarter + lane;
-      const int64_t c0 = int64_t(kOp == kWeights ? at.col - weight * half_cols : at.col) *
-                         (kPaired ? C::kCols / 2 : C::kCols);
-      // Columns of the accumulator by 32: run j of this thread's. A paired tile's second half of runs are ups.
-      const auto column = [&](int j) {
-        return kPaired ? (j < kMine / 64 ? 0 : C::kCols / 2 - kMine / 2) + half * (kMine / 2) + 32 * j : half * kMine + 32 * j;
-      };
-      const auto finish = [&](float (&v)[32], float (&u)[32], int j) {
-        const int64_t c = c0 + column(j);
-        if (row >= p.rows || c >= p.cols) return;
-        const int n = p.cols - c < 32 ? int(p.cols - c) : 32;
-        if constexpr (kOp == kForward) {
-#pragma unroll
-          for (int i = 0; i < 32; ++i) {
-            float y, slope;
-            activate<!C::kFloat>(p.act, v[i], &y, &slope);
-            v[i] = y * u[i];
-          }
-          store_run(static_cast<T*>(p.out0) + row * p.cols + c, v, n);
-        } else if constexpr (kOp == kGates) {
-          const T* dh = static_cast<const T*>(p.dh) + row * p.cols + c;
-#pragma unroll
-          for (int i = 0; i < 32; ++i) {
-            float y, slope;
-            activate<!C::kFloat>(p.act, v[i], &y, &slope);
-            const float d = i < n ? load_one(dh, i) : 0.0f;
-            v[i] = d * u[i] * slope;
-            u[i] = d * y;
-          }
-          for (int q = 0; q < C::kPlanes; ++q) {
-            __nv_bfloat16* to = p.gates + (2 * q * p.rows + row) * p.pitch + c;
-            store_run(to, v, n);
-            store_run(to + p.rows * p.pitch, u, n);
-            if (C::kPlanes > 1) {
-#pragma unroll
-              for (int i = 0; i < 32; ++i) {
-                v[i] -= __bfloat162float(__float2bfloat16_rn(v[i]));
-                u[i] -= __bfloat162float(__float2bfloat16_rn(u[i]));
-              }
-            }
-          }
-        } else {
-          T* out = static_cast<T*>(kOp == kWeights && weight ? p.out1 : p.out0);
-          store_run(out + row * p.cols + c, v, n);
-        }
-      };
-      const uint32_t lanes = uint32_t(32 * quarter) << 16;
+    const uint32_t taken_at = bw::in_block(taken, 0), lanes = uint32_t(32 * quarter) << 16;
+    const auto take_next = [&] {
+      bw::fence_before();
+      __syncwarp();
+      if (lane == 0) bw::barrier_arrive(taken_at + 8 * buffer);
+      if (++buffer == 2) buffer = 0, buffer_phase ^= 1;
+    };
+    // Run j of 32 columns of this thread's; a paired tile's second half of runs are ups.
+    const auto column = [&](int j) {
+      return kPaired ? (j < kMine / 64 ? 0 : C::kHalf - kMine / 2) + half * (kMine / 2) + 32 * j : half * kMine + 32 * j;
+    };
+    for (int item = first; item < items; item += stride) {
+      const Work w = work_of<T, kOp>(p, item);
+      const int64_t r0 = int64_t(2 * w.row + rank) * kRows + 32 * quarter;
       if constexpr (C::kFloat) {
+        const int steps = C::kPairs * w.segs * w.blocks;
         float sum[kMine / 32][32];
 #pragma unroll
         for (int j = 0; j < kMine / 32; ++j)
@@ -352,22 +432,20 @@ __global__ void __launch_bounds__(kProductThreads, 1) product_kernel(const __gri
 #pragma unroll
             for (int i = 0; i < 32; ++i) sum[j][i] += v[i];
           }
-          bw::fence_before();
-          __syncwarp();
-          if (lane == 0) bw::barrier_arrive(taken + 8 * buffer);
-          if (++buffer == 2) buffer = 0, buffer_phase ^= 1;
+          take_next();
         }
-        if (!ok) {
+        if (!ok) {  // a wait ran out: the results say so
 #pragma unroll
           for (int j = 0; j < kMine / 32; ++j)
 #pragma unroll
             for (int i = 0; i < 32; ++i) sum[j][i] = __uint_as_float(0x7fffffffu);
         }
         if constexpr (kPaired) {
-          finish(sum[0], sum[1], 0);
+          finish<T, kOp>(p, w, r0, w.c0 + column(0), sum[0], sum[1], own_stage);
         } else {
 #pragma unroll
-          for (int j = 0; j < kMine / 32; ++j) finish(sum[j], sum[j], j);
+          for (int j = 0; j < kMine / 32; ++j)
+            finish<T, kOp>(p, w, r0, w.c0 + column(j), sum[j], sum[j], own_stage);
         }
       } else {
         ok = ok && bw::barrier_wait(summed + 8 * buffer, buffer_phase, dead);
@@ -383,20 +461,29 @@ __global__ void __launch_bounds__(kProductThreads, 1) product_kernel(const __gri
 #pragma unroll
             for (int i = 0; i < 32; ++i) v[i] = u[i] = __uint_as_float(0x7fffffffu);
           }
-          finish(v, u, j);
+          finish<T, kOp>(p, w, r0, w.c0 + column(j), v, u, own_stage);
         }
-        bw::fence_before();
-        __syncwarp();
-        if (lane == 0) bw::barrier_arrive(taken + 8 * buffer);
-        if (++buffer == 2) buffer = 0, buffer_phase ^= 1;
+        take_next();
       }
     }
   }
   __syncwarp();
   bw::fence_before();
   __syncthreads();
+  bw::cluster_sync();
   bw::fence_after();
   if (warp == 2) bw::tmem_free<kTmemColumns>(tmem);
+}
+
+// The weights' gradients from the sums over runs of tokens.
+template <typename T>
+__global__ void __launch_bounds__(256)
+add_parts_kernel(const float* __restrict__ parts, int splits, int64_t size, T* __restrict__ dwg, T* __restrict__ dwu) {
+  const int64_t e = int64_t(blockIdx.x) * 256 + threadIdx.x;
+  if (e >= 2 * size) return;
+  float sum = 0.0f;
+  for (int s = 0; s < splits; ++s) sum += __ldg(parts + s * 2 * size + e);
+  (e < size ? dwg : dwu)[e < size ? e : e - size] = T(sum);
 }
 
 // ---- host ------------------------------------------------------------------------------------------
@@ -437,15 +524,39 @@ int64_t planes(int dtype) { return dtype == RLENV_F32 ? 3 : 1; }
 
 struct Layout {  // scratch of a call
   void *x, *wg, *wu, *gates;
+  float* parts;
+  int splits, split_blocks;
   int64_t bytes;
 };
+
+constexpr int kPairsOfSms = 74;
+constexpr int64_t kFewestBlocks = 8;
+
+// The contraction over tokens of the weights' gradients is split where a tile of them would take longer
+// than a pair of SMs' share of all the work: a small block's weights are a few tiles, each a sum over every
+// token. The sums of each run of tokens are kept in float32 and added up in order.
+void split_tokens(int dtype, int64_t m, int64_t k, int64_t f, Layout* l) {
+  const int64_t wide = dtype == RLENV_F32 ? 128 : 256, high = 2 * kRows;
+  const int64_t blocks = (m + kStep - 1) / kStep, tiles = (k + high - 1) / high * ((f + wide - 1) / wide) * 2;
+  const int64_t dx = (m + high - 1) / high * ((k + wide - 1) / wide) * 2 * ((f + kStep - 1) / kStep);
+  int64_t share = (tiles * blocks + dx) / kPairsOfSms;
+  if (share < kFewestBlocks) share = kFewestBlocks;
+  int64_t splits = (blocks + share - 1) / share;
+  if (splits < 1) splits = 1;
+  l->split_blocks = int((blocks + splits - 1) / splits);
+  l->splits = int((blocks + l->split_blocks - 1) / l->split_blocks);
+}
 Layout lay_out(int dtype, int64_t m, int64_t k, int64_t f, bool backward, void* scratch) {
   Scratch s{static_cast<unsigned char*>(scratch), 0};
   Layout l{};
   const int64_t n = planes(dtype);
   if (packs(dtype, k)) l.x = s.take(n * m * round_up(k, 8) * 2);
   if (packs(dtype, f)) l.wg = s.take(n * k * round_up(f, 8) * 2), l.wu = s.take(n * k * round_up(f, 8) * 2);
-  if (backward) l.gates = s.take(2 * n * m * round_up(f, 8) * 2);
+  if (backward) {
+    l.gates = s.take(2 * n * m * round_up(f, 8) * 2);
+    if (m > 0 && k > 0 && f > 0) split_tokens(dtype, m, k, f, &l);
+    if (l.splits > 1) l.parts = static_cast<float*>(s.take(int64_t(l.splits) * 2 * k * f * 4));
+  }
   l.bytes = s.used;
   return l;
 }
@@ -465,50 +576,53 @@ int operand(const void* from, int64_t rows, int64_t cols, void* packed, cudaStre
 }
 
 template <typename T, int kOp>
-int run_product(Product& p, cudaStream_t s) {
+int run_product(const Product& p, cudaStream_t s) {
   using C = Tile<T>;
-  constexpr bool kPaired = kOp == kForward || kOp == kGates;
-  const int64_t wide = kPaired ? C::kCols / 2 : C::kCols;
-  const int64_t rt = (p.rows + kRows - 1) / kRows, ct = (p.cols + wide - 1) / wide * (kOp == kWeights ? 2 : 1);
-  if (rt * ct > 0x7fffffff) return RLENV_EINVAL;
-  p.row_tiles = int(rt), p.col_tiles = int(ct);
+  const int64_t items = int64_t(p.row_tiles) * p.col_tiles + int64_t(p.weight_rows) * p.weight_cols * p.splits;
+  if (items > 0x7fffffff) return RLENV_EINVAL;
   int dev = 0, sms = 0;
   if (cudaError_t e = cudaGetDevice(&dev)) return int(e);
   if (cudaError_t e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev)) return int(e);
   if (cudaError_t e = cudaFuncSetAttribute(product_kernel<T, kOp>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem))
     return int(e);
-  const int grid = int(rt * ct < sms ? rt * ct : sms);
-  product_kernel<T, kOp><<<grid, kProductThreads, C::kSmem, s>>>(p);
+  const int grid = 2 * int(items < sms / 2 ? items : sms / 2);
+  product_kernel<T, kOp><<<grid, kProductThreads, C::kSmem, s>>>(p, int(items));
   return launch_status();
 }
+
+int tile_count(int64_t n, int64_t of) { return int((n + of - 1) / of); }
 
 template <typename T>
 int ffn(const void* dh, const void* x, const void* wg, const void* wu, int64_t m, int64_t k, int64_t f, int act,
         void* out, void* dx, void* dwg, void* dwu, const Layout& l, cudaStream_t s) {
+  using C = Tile<T>;
   Operand X, G, U;
   if (const int rc = operand<T>(x, m, k, l.x, s, &X)) return rc;
   if (const int rc = operand<T>(wg, k, f, l.wg, s, &G)) return rc;
   if (const int rc = operand<T>(wu, k, f, l.wu, s, &U)) return rc;
   Product p{};
-  p.rows = m, p.cols = f, p.depth = k, p.act = act, p.out0 = out, p.dh = dh;
+  p.m = m, p.k = k, p.f = f, p.act = act, p.out = out, p.dh = dh;
   p.gates = static_cast<__nv_bfloat16*>(l.gates), p.pitch = round_up(f, 8);
-  if (const int rc = X.map(&p.a, kRows)) return rc;
-  if (const int rc = G.map(&p.b0, 64)) return rc;
-  if (const int rc = U.map(&p.b1, 64)) return rc;
+  p.row_tiles = tile_count(m, 2 * kRows), p.col_tiles = tile_count(f, C::kHalf);
+  if (const int rc = X.map(&p.in[0].a, kRows)) return rc;
+  if (const int rc = G.map(&p.in[0].b0, 64)) return rc;
+  if (const int rc = U.map(&p.in[0].b1, 64)) return rc;
   if (!dh) return run_product<T, kForward>(p, s);
   if (const int rc = run_product<T, kGates>(p, s)) return rc;
-  const Operand D{p.gates, m, f, p.pitch, 2 * Tile<T>::kPlanes};
-  Product q{};
-  q.rows = m, q.cols = k, q.depth = f, q.out0 = dx;
-  if (const int rc = D.map(&q.a, kRows)) return rc;
-  if (const int rc = G.map(&q.b0, 128)) return rc;
-  if (const int rc = U.map(&q.b1, 128)) return rc;
-  if (const int rc = run_product<T, kInput>(q, s)) return rc;
-  Product w{};
-  w.rows = k, w.cols = f, w.depth = m, w.out0 = dwg, w.out1 = dwu;
-  if (const int rc = X.map(&w.a, 64)) return rc;
-  if (const int rc = D.map(&w.b0, 64)) return rc;
-  return run_product<T, kWeights>(w, s);
+  const Operand D{p.gates, m, f, p.pitch, 2 * C::kPlanes};
+  p.out = dx, p.dwg = dwg, p.dwu = dwu, p.parts = l.parts, p.splits = l.splits, p.split_blocks = l.split_blocks;
+  p.col_tiles = tile_count(k, C::kCols);
+  p.weight_rows = tile_count(k, 2 * kRows), p.weight_cols = 2 * tile_count(f, C::kCols);
+  if (const int rc = D.map(&p.in[0].a, kRows)) return rc;
+  if (const int rc = G.map(&p.in[0].b0, C::kHalf)) return rc;
+  if (const int rc = U.map(&p.in[0].b1, C::kHalf)) return rc;
+  if (const int rc = X.map(&p.in[1].a, 64)) return rc;
+  if (const int rc = D.map(&p.in[1].b0, 64)) return rc;
+  if (const int rc = run_product<T, kGradients>(p, s)) return rc;
+  if (l.splits == 1) return RLENV_OK;
+  add_parts_kernel<T><<<grid_for(2 * k * f, 256), 256, 0, s>>>(l.parts, l.splits, k * f, static_cast<T*>(dwg),
+                                                               static_cast<T*>(dwu));
+  return launch_status();
 }
 
 bool off_boundary(const void* a, const void* b, const void* c) {
