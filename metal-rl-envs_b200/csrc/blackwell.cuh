@@ -21,8 +21,11 @@ RLENV_D uint32_t in_block(uint32_t at, uint32_t rank) {
   asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(at), "r"(rank));
   return r;
 }
+// (Default scopes, here and in the waits: what passes between the blocks is tensor memory, ordered by
+// tcgen05.fence, and shared memory, ordered by the copies' and products' own arrivals. At cluster scope
+// each would carry a fence of all memory.)
 RLENV_D void barrier_arrive(uint32_t cluster_bar) {
-  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_bar) : "memory");
+  asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(cluster_bar) : "memory");
 }
 RLENV_D void barrier_expect(uint32_t bar, uint32_t bytes) {
   asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
@@ -30,7 +33,7 @@ RLENV_D void barrier_expect(uint32_t bar, uint32_t bytes) {
 RLENV_D bool barrier_try(uint32_t bar, uint32_t parity) {
   uint32_t done;
   asm volatile(
-      "{\n .reg .pred p;\n mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}"
+      "{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}"
       : "=r"(done) : "r"(bar), "r"(parity) : "memory");
   return done != 0;
 }
@@ -96,20 +99,19 @@ RLENV_D void multiply(uint32_t d, uint64_t a, uint64_t b, uint32_t kind, bool ac
       "l"(a), "l"(b), "r"(kind), "r"(uint32_t(accumulate))
       : "memory");
 }
-// 32 columns of this warp's 32 lanes: lane l gets its row's columns. The wait stands in the same
-// statement, so that no use of the registers comes before it.
-RLENV_D void tmem_load32(float (&v)[32], uint32_t at) {
+// 16 columns at each of two places, of this warp's 32 lanes: lane l gets its row's columns. The wait
+// stands in the same statement, so that no use of the registers comes before it.
+RLENV_D void tmem_load16x2(float (&v)[32], uint32_t at, uint32_t and_at) {
   uint32_t r[32];
   asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
-      "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,"
-      "%30,%31}, [%32];\n"
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%32];\n"
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%33];\n"
       "tcgen05.wait::ld.sync.aligned;"
       : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
         "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
         "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
         "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
-      : "r"(at)
+      : "r"(at), "r"(and_at)
       : "memory");
 #pragma unroll
   for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);

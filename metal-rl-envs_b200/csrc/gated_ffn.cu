@@ -23,9 +23,9 @@ enum Activation { kSilu = 0, kGelu = 1 };
 
 // act(g) and act'(g): silu g / (1 + e^-g), or gelu g Phi(g) with the exact normal distribution. For
 // bfloat16 results the fast exponential and division, good to 2^-20, are enough.
-template <bool kFast>
-RLENV_D void activate(int act, float g, float* y, float* slope) {
-  if (act == kSilu) {
+template <bool kFast, int kAct>
+RLENV_D void activate(float g, float* y, float* slope) {
+  if constexpr (kAct == kSilu) {
     const float s = kFast ? __fdividef(1.0f, 1.0f + __expf(-g)) : 1.0f / (1.0f + expf(-g));
     *y = g * s;
     *slope = s * (1.0f + g * (1.0f - s));
@@ -64,8 +64,7 @@ constexpr int kStep = 64;        // of the contraction, a ring buffer's
 constexpr int kProductThreads = 384;  // copies, products, two idle warps, eight warps of epilogue
 constexpr int kEpilogueWarps = 8;
 constexpr int kTmemColumns = 512;
-constexpr int kStagePitch = 33;  // floats: a 32 x 32 tile is written by rows and read by columns, or the other
-                                 // way round, without bank conflicts
+constexpr int kStageFloats = 32 * 32;  // the epilogue's tile of a warp
 
 template <typename T>
 struct Tile {
@@ -76,10 +75,10 @@ struct Tile {
   static constexpr int kHalf = kCols / 2;        // columns of B in each block
   static constexpr int kABytes = kRows * kStep * 2;
   static constexpr int kRingBytes = kABytes + kHalf * kStep * 2;
-  static constexpr int kStages = kFloat ? 7 : 5;
+  static constexpr int kStages = kFloat ? 8 : 6;
   static constexpr int kStageAt = kStages * kRingBytes;  // the epilogue's 32 x 32 tiles, one a warp
   // the ring starts on a 1,024-byte boundary
-  static constexpr int kSmem = kStageAt + kEpilogueWarps * 32 * kStagePitch * 4 + 1024;
+  static constexpr int kSmem = kStageAt + kEpilogueWarps * kStageFloats * 4 + 1024;
   // Steps of the contraction summed in tensor memory before the epilogue takes them out into registers
   // (float32 only). The tensor core truncates as it accumulates; rounded additions of short sums keep
   // float32 results at float32's error. Of the products of planes only the leading one, the last to be
@@ -102,6 +101,7 @@ struct alignas(64) Product {
   float* parts;              // (splits, 2, K, F) where splits > 1
   __nv_bfloat16* gates;      // (plane, dg or du, M, pitch)
   int64_t pitch;
+  bool wide;                 // rows of h and dh start on the boundaries of fours
 };
 
 // Tiles are taken in bands of kBand rows of tiles, column by column, so that those in flight share
@@ -144,26 +144,11 @@ RLENV_D Work work_of(const Product& p, int item) {
   return w;
 }
 
-// What a step multiplies: planes a and b, the small products first; segment; block of the contraction.
-struct Step {
-  int a, b, seg, k;
-};
+// The pairs of planes, the small products first: a's and b's, two bits each.
 template <typename T>
-RLENV_D Step step_of(const Work& w, int it) {
-  const int per = w.segs * w.blocks, pair = it / per, in = it % per;
-  Step s{0, 0, in / w.blocks, w.k0 + in % w.blocks};
-  if (Tile<T>::kFloat) {
-    switch (pair) {
-      case 0: s.a = 0, s.b = 2; break;
-      case 1: s.a = 2, s.b = 0; break;
-      case 2: s.a = 1, s.b = 1; break;
-      case 3: s.a = 0, s.b = 1; break;
-      case 4: s.a = 1, s.b = 0; break;
-      default: break;
-    }
-  }
-  return s;
-}
+RLENV_D int plane_a(int pair) { return Tile<T>::kFloat ? 0x118 >> (2 * pair) & 3 : 0; }  // 0 2 1 0 1 0
+template <typename T>
+RLENV_D int plane_b(int pair) { return Tile<T>::kFloat ? 0x052 >> (2 * pair) & 3 : 0; }  // 2 0 1 1 0 0
 // Whether the accumulator is handed over after step `it` of `steps`.
 template <typename T>
 RLENV_D bool run_ends(int it, int steps) {
@@ -174,120 +159,155 @@ RLENV_D bool run_ends(int it, int steps) {
   return (it + 1 - small) % Tile<T>::kRun == 0;
 }
 
-// A warp's 32 x 32 tile between registers (a row a lane) and an array (row pitch `pitch`), rows and
-// columns past the ends left out, through shared memory so that global accesses run along rows.
-template <typename T>
-RLENV_D void store_tile(T* to, int64_t pitch, int rows, int cols, const float (&v)[32], float* stage) {
-  const int lane = threadIdx.x & 31;
-  __syncwarp();
-#pragma unroll
-  for (int i = 0; i < 32; ++i) stage[lane * kStagePitch + i] = v[i];
-  __syncwarp();
-  if (cols >= 32 && (reinterpret_cast<uintptr_t>(to) | uintptr_t(pitch * sizeof(T))) % (4 * sizeof(T)) == 0) {
-    const int c = lane % 8 * 4;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const int r = 4 * i + lane / 8;
-      const float* s = stage + r * kStagePitch + c;
-      if (r < rows) {
-        if constexpr (sizeof(T) == 2) {
-          const __nv_bfloat162 lo = __floats2bfloat162_rn(s[0], s[1]), hi = __floats2bfloat162_rn(s[2], s[3]);
-          *reinterpret_cast<uint2*>(to + r * pitch + c) =
-              make_uint2(*reinterpret_cast<const uint32_t*>(&lo), *reinterpret_cast<const uint32_t*>(&hi));
-        } else {
-          *reinterpret_cast<float4*>(to + r * pitch + c) = make_float4(s[0], s[1], s[2], s[3]);
-        }
-      }
-    }
+// Four neighbouring values of a row, the first n of them there: in one access where all are and `wide`
+// says that rows start on the boundaries of fours.
+RLENV_D void store_four(float* to, float4 v, bool wide, int n) {
+  if (wide && n >= 4) {
+    *reinterpret_cast<float4*>(to) = v;
   } else {
-#pragma unroll 8
-    for (int r = 0; r < 32; ++r)
-      if (r < rows && lane < cols) to[r * pitch + lane] = T(stage[r * kStagePitch + lane]);
+    if (n > 0) to[0] = v.x;
+    if (n > 1) to[1] = v.y;
+    if (n > 2) to[2] = v.z;
+    if (n > 3) to[3] = v.w;
+  }
+}
+RLENV_D uint2 pack_four(float4 v) {
+  const __nv_bfloat162 lo = __floats2bfloat162_rn(v.x, v.y), hi = __floats2bfloat162_rn(v.z, v.w);
+  return make_uint2(*reinterpret_cast<const uint32_t*>(&lo), *reinterpret_cast<const uint32_t*>(&hi));
+}
+RLENV_D float4 unpack_four(uint2 w) {
+  return make_float4(__uint_as_float(w.x << 16), __uint_as_float(w.x & 0xffff0000u), __uint_as_float(w.y << 16),
+                     __uint_as_float(w.y & 0xffff0000u));
+}
+RLENV_D float4 unpack_four(float4 w) { return w; }
+RLENV_D void store_four(__nv_bfloat16* to, float4 v, bool wide, int n) {
+  if (wide && n >= 4) {
+    *reinterpret_cast<uint2*>(to) = pack_four(v);
+  } else {
+    if (n > 0) to[0] = __float2bfloat16_rn(v.x);
+    if (n > 1) to[1] = __float2bfloat16_rn(v.y);
+    if (n > 2) to[2] = __float2bfloat16_rn(v.z);
+    if (n > 3) to[3] = __float2bfloat16_rn(v.w);
+  }
+}
+RLENV_D void load_four(const float* from, float4* v, bool wide, int n) {
+  if (wide && n >= 4)
+    *v = __ldg(reinterpret_cast<const float4*>(from));
+  else
+    *v = make_float4(n > 0 ? from[0] : 0.0f, n > 1 ? from[1] : 0.0f, n > 2 ? from[2] : 0.0f, n > 3 ? from[3] : 0.0f);
+}
+RLENV_D void load_four(const __nv_bfloat16* from, uint2* v, bool wide, int n) {
+  if (wide && n >= 4) {
+    *v = __ldg(reinterpret_cast<const uint2*>(from));
+  } else {
+    const unsigned short* f = reinterpret_cast<const unsigned short*>(from);
+    *v = make_uint2((n > 0 ? f[0] : 0u) | (n > 1 ? uint32_t(f[1]) << 16 : 0u),
+                    (n > 2 ? f[2] : 0u) | (n > 3 ? uint32_t(f[3]) << 16 : 0u));
   }
 }
 template <typename T>
-RLENV_D void load_tile(const T* from, int64_t pitch, int rows, int cols, float (&v)[32], float* stage) {
-  const int lane = threadIdx.x & 31;
-  __syncwarp();
-  if (cols >= 32 && (reinterpret_cast<uintptr_t>(from) | uintptr_t(pitch * sizeof(T))) % (4 * sizeof(T)) == 0) {
-    const int c = lane % 8 * 4;
+struct Four {
+  using type = float4;
+};
+template <>
+struct Four<__nv_bfloat16> {
+  using type = uint2;
+};
+
+// A warp's 32 x 32 tile of results goes through shared memory, written a row a lane and read four
+// neighbours a lane, so that global accesses run along rows. Fours of columns are exchanged by the row's
+// low three bits, which keeps both sides free of bank conflicts.
+RLENV_D float4* stage_at(float* stage, int row, int four) {
+  return reinterpret_cast<float4*>(stage) + row * 8 + (four ^ (row & 7));
+}
+// A gated tile is 16 columns of gates and their 16 ups: lane l has columns 4 (l % 4) .. + 3 of rows
+// gated_row(l) + 8 i.
+RLENV_D int gated_row(int lane) { return (lane >> 2 & 1) * 4 + (lane >> 3); }
+
+// The gradient dh of a gated tile.
+template <typename T>
+RLENV_D void load_gradient(const Product& p, int64_t r0, int64_t c, typename Four<T>::type (&d)[4]) {
+  const int lane = threadIdx.x & 31, col = lane % 4 * 4;
+  const int n = int(min(int64_t(4), max(int64_t(0), p.f - c - col)));
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const int r = 4 * i + lane / 8;
-      float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-      if (r < rows) {
-        if constexpr (sizeof(T) == 2) {
-          const uint2 w = __ldg(reinterpret_cast<const uint2*>(from + r * pitch + c));
-          x = make_float4(__uint_as_float(w.x << 16), __uint_as_float(w.x & 0xffff0000u), __uint_as_float(w.y << 16),
-                          __uint_as_float(w.y & 0xffff0000u));
-        } else {
-          x = __ldg(reinterpret_cast<const float4*>(from + r * pitch + c));
-        }
-      }
-      float* s = stage + r * kStagePitch + c;
-      s[0] = x.x, s[1] = x.y, s[2] = x.z, s[3] = x.w;
-    }
-  } else {
-#pragma unroll 8
-    for (int r = 0; r < 32; ++r)
-      stage[r * kStagePitch + lane] = r < rows && lane < cols ? float(from[r * pitch + lane]) : 0.0f;
+  for (int i = 0; i < 4; ++i) {
+    const int64_t r = r0 + gated_row(lane) + 8 * i;
+    load_four(static_cast<const T*>(p.dh) + r * p.f + c + col, &d[i], p.wide, r < p.m ? n : 0);
   }
-  __syncwarp();
-#pragma unroll
-  for (int i = 0; i < 32; ++i) v[i] = stage[lane * kStagePitch + i];
 }
 
-// A 32 x 32 piece of a tile's results: rows from r0, columns from c (of h, a weight or dx). v holds its
-// values or gates, u its ups.
-template <typename T, int kOp>
-RLENV_D void finish(const Product& p, const Work& w, int64_t r0, int64_t c, float (&v)[32], float (&u)[32],
-                    float* stage) {
+template <typename T, int kOp, int kAct>
+RLENV_D void finish_gated(const Product& p, int64_t r0, int64_t c, const typename Four<T>::type (&dh)[4], float* stage) {
   constexpr bool kFast = !Tile<T>::kFloat;
-  if constexpr (kOp == kGradients) {
-    const int64_t all_rows = w.weights ? p.k : p.m, all_cols = w.weights ? p.f : p.k;
-    if (r0 >= all_rows || c >= all_cols) return;
-    const int rows = int(min(int64_t(32), all_rows - r0)), cols = int(min(int64_t(32), all_cols - c));
-    if (w.weights && p.splits > 1) {
-      store_tile(p.parts + ((int64_t(w.split) * 2 + w.weight) * p.k + r0) * p.f + c, p.f, rows, cols, v, stage);
-    } else {
-      T* to = static_cast<T*>(w.weights ? (w.weight ? p.dwu : p.dwg) : p.out);
-      store_tile(to + r0 * all_cols + c, all_cols, rows, cols, v, stage);
-    }
-  } else {
-    if (r0 >= p.m || c >= p.f) return;
-    const int rows = int(min(int64_t(32), p.m - r0)), cols = int(min(int64_t(32), p.f - c));
+  const int lane = threadIdx.x & 31, col = lane % 4 * 4;
+  const int n = int(min(int64_t(4), p.f - c - col));
+  if (n <= 0) return;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int r = gated_row(lane) + 8 * i;
+    if (r0 + r >= p.m) return;
+    const float4 g = *stage_at(stage, r, lane % 4), u = *stage_at(stage, r, 4 + lane % 4);
+    float4 y, slope;
+    activate<kFast, kAct>(g.x, &y.x, &slope.x);
+    activate<kFast, kAct>(g.y, &y.y, &slope.y);
+    activate<kFast, kAct>(g.z, &y.z, &slope.z);
+    activate<kFast, kAct>(g.w, &y.w, &slope.w);
     if constexpr (kOp == kForward) {
-#pragma unroll
-      for (int i = 0; i < 32; ++i) {
-        float y, slope;
-        activate<kFast>(p.act, v[i], &y, &slope);
-        v[i] = y * u[i];
-      }
-      store_tile(static_cast<T*>(p.out) + r0 * p.f + c, p.f, rows, cols, v, stage);
+      store_four(static_cast<T*>(p.out) + (r0 + r) * p.f + c + col,
+                 make_float4(y.x * u.x, y.y * u.y, y.z * u.z, y.w * u.w), p.wide, n);
     } else {
-      float d[32];
-      load_tile(static_cast<const T*>(p.dh) + r0 * p.f + c, p.f, rows, cols, d, stage);
+      const float4 d = unpack_four(dh[i]);
+      float4 dg = make_float4(d.x * u.x * slope.x, d.y * u.y * slope.y, d.z * u.z * slope.z, d.w * u.w * slope.w);
+      float4 du = make_float4(d.x * y.x, d.y * y.y, d.z * y.z, d.w * y.w);
+      __nv_bfloat16* to = p.gates + (r0 + r) * p.pitch + c + col;  // the pitch holds whole eights
 #pragma unroll
-      for (int i = 0; i < 32; ++i) {
-        float y, slope;
-        activate<kFast>(p.act, v[i], &y, &slope);
-        v[i] = d[i] * u[i] * slope;
-        u[i] = d[i] * y;
-      }
-#pragma unroll 1
-      for (int q = 0; q < Tile<T>::kPlanes; ++q) {
-        __nv_bfloat16* to = p.gates + (2 * q * p.m + r0) * p.pitch + c;
-        store_tile(to, p.pitch, rows, cols, v, stage);
-        store_tile(to + p.m * p.pitch, p.pitch, rows, cols, u, stage);
-        if (Tile<T>::kPlanes > 1) {
-#pragma unroll
-          for (int i = 0; i < 32; ++i) {
-            v[i] -= __bfloat162float(__float2bfloat16_rn(v[i]));
-            u[i] -= __bfloat162float(__float2bfloat16_rn(u[i]));
-          }
-        }
+      for (int q = 0; q < Tile<T>::kPlanes; ++q, to += 2 * p.m * p.pitch) {
+        const uint2 a = pack_four(dg), b = pack_four(du);
+        *reinterpret_cast<uint2*>(to) = a;
+        *reinterpret_cast<uint2*>(to + p.m * p.pitch) = b;
+        const float4 x = unpack_four(a), z = unpack_four(b);
+        dg.x -= x.x, dg.y -= x.y, dg.z -= x.z, dg.w -= x.w, du.x -= z.x, du.y -= z.y, du.z -= z.z, du.w -= z.w;
       }
     }
+  }
+}
+template <typename T>
+RLENV_D void finish_values(T* to, int64_t pitch, int64_t rows, int64_t cols, float* stage) {
+  const int lane = threadIdx.x & 31, col = lane % 8 * 4;
+  const int n = int(min(int64_t(4), cols - col));
+  if (n <= 0) return;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int r = lane / 8 + 4 * i;
+    if (r >= rows) return;
+    store_four(to + r * pitch + col, *stage_at(stage, r, lane % 8), pitch % 4 == 0, n);
+  }
+}
+
+// Rows from r0, columns from c (of h, a weight or dx). v: 16 gates and 16 ups, or 32 values.
+template <typename T, int kOp>
+RLENV_D void finish(const Product& p, const Work& w, int64_t r0, int64_t c, const float (&v)[32],
+                    const typename Four<T>::type (&dh)[4], float* stage) {
+  const int64_t all_rows = kOp == kGradients && w.weights ? p.k : p.m;
+  const int64_t all_cols = kOp == kGradients && !w.weights ? p.k : p.f;
+  if (r0 >= all_rows || c >= all_cols) return;
+  const int lane = threadIdx.x & 31;
+  __syncwarp();
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+    *stage_at(stage, lane, i) = make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+  __syncwarp();
+  if constexpr (kOp == kGradients) {
+    if (w.weights && p.splits > 1)
+      finish_values(p.parts + ((int64_t(w.split) * 2 + w.weight) * p.k + r0) * p.f + c, p.f, all_rows - r0,
+                    all_cols - c, stage);
+    else
+      finish_values(static_cast<T*>(w.weights ? (w.weight ? p.dwu : p.dwg) : p.out) + r0 * all_cols + c, all_cols,
+                    all_rows - r0, all_cols - c, stage);
+  } else if (p.act == kSilu) {
+    finish_gated<T, kOp, kSilu>(p, r0, c, dh, stage);
+  } else {
+    finish_gated<T, kOp, kGelu>(p, r0, c, dh, stage);
   }
 }
 
@@ -331,27 +351,31 @@ product_kernel(const __grid_constant__ Product p, int items) {
       for (int item = first; item < items && ok; item += stride) {
         const Work w = work_of<T, kOp>(p, item);
         const Operands& in = p.in[kOp == kGradients && w.weights];
-        const int r0 = (2 * w.row + rank) * kRows, steps = C::kPairs * w.segs * w.blocks;
-        for (int it = 0; it < steps; ++it) {
-          const Step s = step_of<T>(w, it);
-          const int k0 = s.k * kStep;
-          if (!(ok = bw::barrier_wait(empty + 8 * stage, phase ^ 1, dead))) break;
-          if (rank == 0) bw::barrier_expect(full + 8 * stage, 2 * C::kRingBytes);
-          const uint32_t bar = full_at + 8 * stage, a = ring + stage * C::kRingBytes, b = a + C::kABytes;
-          if (kPaired) {  // A by rows of the contraction's axis; gates in the first block, ups in the second
-            bw::copy_tile(a, &in.a, bar, k0, r0, s.a);
-            for (int i = 0; i < C::kHalf / 64; ++i)
-              bw::copy_tile(b + i * kBox, rank ? &in.b1 : &in.b0, bar, w.c0 + 64 * i, k0, s.b);
-          } else if (w.weights) {
-            for (int i = 0; i < kRows / 64; ++i) bw::copy_tile(a + i * kBox, &in.a, bar, r0 + 64 * i, k0, s.a);
-            for (int i = 0; i < C::kHalf / 64; ++i)
-              bw::copy_tile(b + i * kBox, &in.b0, bar, w.c0 + rank * C::kHalf + 64 * i, k0, 2 * s.b + w.weight);
-          } else {
-            bw::copy_tile(a, &in.a, bar, k0, r0, 2 * s.a + s.seg);
-            bw::copy_tile(b, s.seg ? &in.b1 : &in.b0, bar, k0, w.c0 + rank * C::kHalf, s.b);
+        const int r0 = (2 * w.row + rank) * kRows;
+        for (int pair = 0; pair < C::kPairs && ok; ++pair) {
+          const int pa = plane_a<T>(pair), pb = plane_b<T>(pair);
+          for (int seg = 0; seg < w.segs && ok; ++seg) {
+            for (int k = w.k0; k < w.k0 + w.blocks; ++k) {
+              const int k0 = k * kStep;
+              if (!(ok = bw::barrier_wait(empty + 8 * stage, phase ^ 1, dead))) break;
+              if (rank == 0) bw::barrier_expect(full + 8 * stage, 2 * C::kRingBytes);
+              const uint32_t bar = full_at + 8 * stage, a = ring + stage * C::kRingBytes, b = a + C::kABytes;
+              if (kPaired) {  // gates in the first block, ups in the second
+                bw::copy_tile(a, &in.a, bar, k0, r0, pa);
+                for (int i = 0; i < C::kHalf / 64; ++i)
+                  bw::copy_tile(b + i * kBox, rank ? &in.b1 : &in.b0, bar, w.c0 + 64 * i, k0, pb);
+              } else if (w.weights) {
+                for (int i = 0; i < kRows / 64; ++i) bw::copy_tile(a + i * kBox, &in.a, bar, r0 + 64 * i, k0, pa);
+                for (int i = 0; i < C::kHalf / 64; ++i)
+                  bw::copy_tile(b + i * kBox, &in.b0, bar, w.c0 + rank * C::kHalf + 64 * i, k0, 2 * pb + w.weight);
+              } else {
+                bw::copy_tile(a, &in.a, bar, k0, r0, 2 * pa + seg);
+                bw::copy_tile(b, seg ? &in.b1 : &in.b0, bar, k0, w.c0 + rank * C::kHalf, pb);
+              }
+              used |= 1u << stage;
+              if (++stage == C::kStages) stage = 0, phase ^= 1;
+            }
           }
-          used |= 1u << stage;
-          if (++stage == C::kStages) stage = 0, phase ^= 1;
         }
       }
       if (!ok && rank == 0) {  // the copies in flight land before the blocks may end
@@ -393,7 +417,7 @@ product_kernel(const __grid_constant__ Product p, int items) {
   } else if (warp >= 4) {
     const int quarter = warp & 3, half = (warp - 4) >> 2;
     float* const own_stage = reinterpret_cast<float*>(raw + (ring - bw::shared_at(raw)) + C::kStageAt) +
-                             (warp - 4) * 32 * kStagePitch;
+                             (warp - 4) * kStageFloats;
     constexpr int kMine = C::kCols / 2;  // columns of the accumulator that a thread reads
     int buffer = 0;
     uint32_t buffer_phase = 0;
@@ -405,13 +429,23 @@ product_kernel(const __grid_constant__ Product p, int items) {
       if (lane == 0) bw::barrier_arrive(taken_at + 8 * buffer);
       if (++buffer == 2) buffer = 0, buffer_phase ^= 1;
     };
-    // Run j of 32 columns of this thread's; a paired tile's second half of runs are ups.
-    const auto column = [&](int j) {
-      return kPaired ? (j < kMine / 64 ? 0 : C::kHalf - kMine / 2) + half * (kMine / 2) + 32 * j : half * kMine + 32 * j;
+    // Run j of 32 columns of this thread's, as two of 16: a gated tile's are gates and ups.
+    const auto column = [&](int j) { return kPaired ? half * (C::kHalf / 2) + 16 * j : half * kMine + 32 * j; };
+    const auto load_run = [&](float (&v)[32], int j) {
+      const uint32_t at = tmem + lanes + buffer * C::kCols + column(j);
+      bw::tmem_load16x2(v, at, at + (kPaired ? C::kHalf : 16));
     };
     for (int item = first; item < items; item += stride) {
       const Work w = work_of<T, kOp>(p, item);
       const int64_t r0 = int64_t(2 * w.row + rank) * kRows + 32 * quarter;
+      typename Four<T>::type dh[4], dh_next[4];  // loaded one run ahead, the first under the tile's products
+      if constexpr (kOp == kGates) load_gradient<T>(p, r0, w.c0 + column(0), dh_next);
+      const auto next_gradient = [&](int j) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) dh[i] = dh_next[i];
+        if constexpr (kOp == kGates)
+          if (j + 1 < kMine / 32) load_gradient<T>(p, r0, w.c0 + column(j + 1), dh_next);
+      };
       if constexpr (C::kFloat) {
         const int steps = C::kPairs * w.segs * w.blocks;
         float sum[kMine / 32][32];
@@ -428,40 +462,36 @@ product_kernel(const __grid_constant__ Product p, int items) {
 #pragma unroll
           for (int j = 0; j < kMine / 32; ++j) {
             float v[32];
-            bw::tmem_load32(v, tmem + lanes + buffer * C::kCols + column(j));
+            load_run(v, j);
 #pragma unroll
             for (int i = 0; i < 32; ++i) sum[j][i] += v[i];
           }
           take_next();
         }
-        if (!ok) {  // a wait ran out: the results say so
 #pragma unroll
-          for (int j = 0; j < kMine / 32; ++j)
+        for (int j = 0; j < kMine / 32; ++j) {
+          if (!ok) {  // a wait ran out: the results say so
 #pragma unroll
             for (int i = 0; i < 32; ++i) sum[j][i] = __uint_as_float(0x7fffffffu);
-        }
-        if constexpr (kPaired) {
-          finish<T, kOp>(p, w, r0, w.c0 + column(0), sum[0], sum[1], own_stage);
-        } else {
-#pragma unroll
-          for (int j = 0; j < kMine / 32; ++j)
-            finish<T, kOp>(p, w, r0, w.c0 + column(j), sum[j], sum[j], own_stage);
+          }
+          next_gradient(j);
+          finish<T, kOp>(p, w, r0, w.c0 + column(j), sum[j], dh, own_stage);
         }
       } else {
         ok = ok && bw::barrier_wait(summed + 8 * buffer, buffer_phase, dead);
         ok = __all_sync(0xffffffffu, ok);
         bw::fence_after();
 #pragma unroll 1
-        for (int j = 0; j < (kPaired ? kMine / 64 : kMine / 32); ++j) {
-          float v[32], u[32];
+        for (int j = 0; j < kMine / 32; ++j) {
+          float v[32];
+          next_gradient(j);
           if (ok) {
-            bw::tmem_load32(v, tmem + lanes + buffer * C::kCols + column(j));
-            if (kPaired) bw::tmem_load32(u, tmem + lanes + buffer * C::kCols + column(j + kMine / 64));
+            load_run(v, j);
           } else {
 #pragma unroll
-            for (int i = 0; i < 32; ++i) v[i] = u[i] = __uint_as_float(0x7fffffffu);
+            for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(0x7fffffffu);
           }
-          finish<T, kOp>(p, w, r0, w.c0 + column(j), v, u, own_stage);
+          finish<T, kOp>(p, w, r0, w.c0 + column(j), v, dh, own_stage);
         }
         take_next();
       }
@@ -603,6 +633,7 @@ int ffn(const void* dh, const void* x, const void* wg, const void* wu, int64_t m
   Product p{};
   p.m = m, p.k = k, p.f = f, p.act = act, p.out = out, p.dh = dh;
   p.gates = static_cast<__nv_bfloat16*>(l.gates), p.pitch = round_up(f, 8);
+  p.wide = f % 4 == 0 && reinterpret_cast<uintptr_t>(dh) % (4 * sizeof(T)) == 0;
   p.row_tiles = tile_count(m, 2 * kRows), p.col_tiles = tile_count(f, C::kHalf);
   if (const int rc = X.map(&p.in[0].a, kRows)) return rc;
   if (const int rc = G.map(&p.in[0].b0, 64)) return rc;
@@ -648,7 +679,7 @@ int rlenv_gated_ffn_forward(int dtype, int activation, int64_t m, int64_t k, int
   if (m == 0 || f == 0) return RLENV_OK;
   if (k == 0) return out ? int(cudaMemsetAsync(out, 0, size_t(m) * f * (dtype == RLENV_F32 ? 4 : 2), as_stream(stream)))
                          : RLENV_EINVAL;
-  if (!out || !x || !w_gate || !w_up || off_boundary(x, w_gate, w_up)) return RLENV_EINVAL;
+  if (!out || !x || !w_gate || !w_up || off_boundary(x, w_gate, w_up) || off_boundary(out, out, out)) return RLENV_EINVAL;
   const Layout l = lay_out(dtype, m, k, f, false, scratch);
   if (!scratch_holds(scratch, scratch_bytes, l.bytes)) return RLENV_EINVAL;
   const cudaStream_t s = as_stream(stream);
@@ -663,7 +694,8 @@ int rlenv_gated_ffn_backward(int dtype, int activation, int64_t m, int64_t k, in
   using namespace rlenv;
   if (const int rc = check_ffn(dtype, activation, m, k, f)) return rc;
   if (m == 0 || k == 0 || f == 0) return RLENV_EINVAL;
-  if (!grad_out || !x || !w_gate || !w_up || !grad_x || !grad_w_gate || !grad_w_up || off_boundary(x, w_gate, w_up))
+  if (!grad_out || !x || !w_gate || !w_up || !grad_x || !grad_w_gate || !grad_w_up || off_boundary(x, w_gate, w_up) ||
+      off_boundary(grad_x, grad_w_gate, grad_w_up))
     return RLENV_EINVAL;
   const Layout l = lay_out(dtype, m, k, f, true, scratch);
   if (!scratch_holds(scratch, scratch_bytes, l.bytes)) return RLENV_EINVAL;
