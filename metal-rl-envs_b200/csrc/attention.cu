@@ -20,24 +20,22 @@ struct Split {
 };
 
 template <typename T, int D, bool kLocal>
-__global__ void __launch_bounds__(attn::kThreads)
+__global__ void __launch_bounds__(attn::Shape<T, D>::kThreads, attn::Shape<T, D>::kPerSm)
 chunk_kernel(const __grid_constant__ Problem p, const __grid_constant__ Split split) {
   using namespace attn;
   using C = Shape<T, D>;
   constexpr int DB = C::DB, kTiles = D / DB;
   extern __shared__ __align__(16) unsigned char smem[];
-  __shared__ float left[kChunk];       // l_j
-  __shared__ uint32_t reset_words[2];
-  __nv_bfloat16* const X = reinterpret_cast<__nv_bfloat16*>(smem);
-  __nv_bfloat16* const A = X + C::kIn * C::kX;
-  __nv_bfloat16* const B = A + C::kIn * C::kX;
-  __nv_bfloat16* const S = B + C::kIn * C::kB;
+  __shared__ float decays[kChunk];  // g^(64 - f - j)
+  __nv_bfloat16* const tiles = reinterpret_cast<__nv_bfloat16*>(smem);
+  __nv_bfloat16* const S = tiles + C::kBuffers * C::kTiles;
+  constexpr int kAAt = C::kIn * C::kX, kBAt = 2 * C::kIn * C::kX;  // x, a and b in a buffer
 
   int64_t id = blockIdx.x;
   const int col = int(id % kTiles) * DB;
   id /= kTiles;
-  const Scan& s = p.scan[id % p.scans];
   const int64_t scan = id % p.scans;
+  const Scan& s = p.scan[scan];
   id /= p.scans;
   const int64_t segment = id % split.segments, seq = id / split.segments;
   const int64_t n = seq / p.h, h = seq % p.h;
@@ -47,14 +45,18 @@ chunk_kernel(const __grid_constant__ Problem p, const __grid_constant__ Split sp
   const bool whole = split.segments == 1;
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int gr = lane >> 2, gc = (lane & 3) * 2;  // a fragment's row and column
+  const int rb = warp & 3, oc = (warp >> 2) * C::OC;  // this warp's 16 tokens and output columns
+  const int gr = lane >> 2, gc = (lane & 3) * 2;      // a fragment's row and column
   const float log2_g = log2f(__ldg(p.decay + h));
   const int f = s.reverse ? 0 : 1;
+  if (threadIdx.x < kChunk) decays[threadIdx.x] = power(log2_g, kChunk - f - int(threadIdx.x));
+  const float chunk_decay = power(log2_g, kChunk);
 
   // The carry, float32 in registers: rows srow + 16 m + (gr, gr + 8), columns scol + 8 t + (gc, gc + 1).
   const int rg = warp % C::RG, cg = warp / C::RG;
   const bool holds = cg < C::CG;
   const int srow = rg * 16 * C::MT, scol = cg * 8 * C::NT;
+  const bool fine = kLocal || C::kFloat || s.carry_out;  // a carry that goes out in float32 takes all planes
   float z[C::MT][C::NT][4];
   const float* start = kLocal ? nullptr : whole ? s.carry_in : split.carry + slot * D * D;
   if (!kLocal && whole && start) start += seq * D * D;
@@ -70,29 +72,68 @@ chunk_kernel(const __grid_constant__ Problem p, const __grid_constant__ Split sp
         z[m][t][q] = start && holds ? start_mul * __ldg(start + (turned ? c * D + r : r * D + c)) : 0.0f;
       }
 
-  // The weights between a warp's rows and 16 columns: on the diagonal, and one block to its left.
+  // The weights, `scale` among them, between a warp's rows and 16 columns: on the diagonal, and one block
+  // to its left; and from the carry to its rows.
   float near[8], next[8], row_decay[2];
   if constexpr (!kLocal) {
 #pragma unroll
     for (int q = 0; q < 8; ++q) {
       const int apart = gr + (q & 2) * 4 - (gc + (q & 1) + (q & 4) * 2);
-      near[q] = apart >= 0 ? power(log2_g, apart) : 0.0f;
-      next[q] = power(log2_g, 16 + apart);
+      near[q] = apart >= 0 ? p.scale * power(log2_g, apart) : 0.0f;
+      next[q] = p.scale * power(log2_g, 16 + apart);
     }
-    row_decay[0] = power(log2_g, 16 * warp + gr + f);
-    row_decay[1] = power(log2_g, 16 * warp + gr + 8 + f);
+    row_decay[0] = p.scale * power(log2_g, 16 * rb + gr + f);
+    row_decay[1] = p.scale * power(log2_g, 16 * rb + gr + 8 + f);
   }
+  const float block_decay = power(log2_g, 16);
 
-  const T* const xs = static_cast<const T*>(s.x) + n * s.xs.n + h * s.xs.h;
-  const T* const as = static_cast<const T*>(s.a) + n * s.as.n + h * s.as.h;
-  const T* const bs = static_cast<const T*>(s.b) + n * s.bs.n + h * s.bs.h + col;
+  using LoadX = TileLoader<T, D, C::PX, C::kX, C::kThreads>;
+  using LoadB = TileLoader<T, DB, C::PB, C::kB, C::kThreads>;
+  LoadX load_x(static_cast<const T*>(s.x) + n * s.xs.n + h * s.xs.h, s.xs.t, s.reverse, p.t, first);
+  LoadX load_a(static_cast<const T*>(s.a) + n * s.as.n + h * s.as.h, s.as.t, s.reverse, p.t, first);
+  LoadB load_b(static_cast<const T*>(s.b) + n * s.bs.n + h * s.bs.h + col, s.bs.t, s.reverse, p.t, first);
+  float4 vx[C::kFloat && !kLocal ? LoadX::kCount : 1], va[C::kFloat ? LoadX::kCount : 1], vb[C::kFloat ? LoadB::kCount : 1];
+  // the next chunk's tiles set out, from chunk `i` into buffer `to`
+  const auto set_out = [&](int64_t i, __nv_bfloat16* to) {
+    if constexpr (C::kFloat) {
+      if constexpr (!kLocal) load_x.fetch(vx, last - i);
+      load_a.fetch(va, last - i);
+      load_b.fetch(vb, last - i);
+    } else {
+      if constexpr (!kLocal) load_x.copy(shared_address(to), last - i);
+      load_a.copy(shared_address(to + kAAt), last - i);
+      load_b.copy(shared_address(to + kBAt), last - i);
+      copies_end();
+    }
+    load_x.advance(), load_a.advance(), load_b.advance();
+  };
+  // a lane's two resets of a chunk, as bytes
+  const auto reset_at = [&](int64_t i) -> int {
+    if (i >= last) return 0;
+    return __ldg(p.resets + (s.reverse ? p.t - 1 - i : i) * p.n + n);
+  };
+  int reset0 = 0, reset1 = 0;
+  if (p.resets && first < last) reset0 = reset_at(first + lane), reset1 = reset_at(first + 32 + lane);
+  if (first < last) set_out(first, tiles);
+
   float bad = 0.0f;      // NaN once any value is not finite
   bool cut = false;      // a reset anywhere in the segment
-
+  int buffer = 0;
   for (int64_t i0 = first; i0 < last; i0 += kChunk) {
     const int len = int(last - i0 < kChunk ? last - i0 : kChunk);
+    __nv_bfloat16* const X = tiles + (C::kFloat ? 0 : buffer * C::kTiles);
+    __nv_bfloat16* const A = X + kAAt;
+    __nv_bfloat16* const B = X + kBAt;
+    buffer ^= 1;
+    const uint64_t resets = uint64_t(__ballot_sync(0xffffffffu, reset1 != 0)) << 32 | __ballot_sync(0xffffffffu, reset0 != 0);
+    cut = cut || resets != 0;
+    // The first position that position i (or, for i = 63, the chunk's end) is linked to; `none`: also the carry.
+    const auto linked_from = [&](uint64_t before, bool* none) -> int {
+      const uint64_t m = resets & before;
+      *none = m == 0;
+      return m ? 64 - f - __clzll(m) : 0;
+    };
     if constexpr (!kLocal) {
-      load_tile<T, D, C::PX, C::kX>(xs, s.xs.t, s, p.t, i0, last, X);
       // the carry at the chunk's start as planes
       if (holds) {
 #pragma unroll
@@ -110,38 +151,28 @@ chunk_kernel(const __grid_constant__ Problem p, const __grid_constant__ Split sp
             }
       }
     }
-    load_tile<T, D, C::PX, C::kX>(as, s.as.t, s, p.t, i0, last, A);
-    load_tile<T, DB, C::PB, C::kB>(bs, s.bs.t, s, p.t, i0, last, B);
-    if (threadIdx.x < kChunk) {
-      const int j = threadIdx.x;
-      bool reset = false;
-      if (p.resets && j < len) {
-        const int64_t t = s.reverse ? p.t - 1 - (i0 + j) : i0 + j;
-        reset = __ldg(p.resets + t * p.n + n) != 0;
-      }
-      const uint32_t word = __ballot_sync(0xffffffffu, reset);
-      if (lane == 0) reset_words[warp] = word;
-    }
-    copies_landed();
-    __syncthreads();
-    const uint64_t resets = uint64_t(reset_words[1]) << 32 | reset_words[0];
-    // resets that act before position i is used
-    const auto count = [&](int i) { return __popcll(resets & ((uint64_t(f + 1) << i) - 1)); };
-    if (threadIdx.x < kChunk) {
-      const int j = threadIdx.x;
-      const bool reaches = j < len && (resets == 0 || count(j) == __popcll(resets));
-      left[j] = reaches ? power(log2_g, len - f - j) : 0.0f;
+    if constexpr (C::kFloat) {
+      if constexpr (!kLocal) load_x.put(X, vx);
+      load_a.put(A, va);
+      load_b.put(B, vb);
+    } else {
+      copies_landed<0>();
     }
     __syncthreads();
+    const int64_t next_chunk = i0 + kChunk;
+    if (next_chunk < last) {
+      set_out(next_chunk, tiles + (C::kFloat ? 0 : buffer * C::kTiles));
+      if (p.resets) reset0 = reset_at(next_chunk + lane), reset1 = reset_at(next_chunk + 32 + lane);
+    }
 
     if constexpr (!kLocal) {
-      float o[DB / 8][4];
+      float o[C::OC / 8][4];
 #pragma unroll
-      for (int t = 0; t < DB / 8; ++t)
+      for (int t = 0; t < C::OC / 8; ++t)
 #pragma unroll
         for (int q = 0; q < 4; ++q) o[t][q] = 0.0f;
-      const uint32_t xa = shared_address(X + (16 * warp + (lane & 15)) * C::PX + (lane >> 4) * 8);
-      const uint32_t sa = shared_address(S + (lane & 15) * C::PB + (lane >> 4) * 8);
+      const uint32_t xa = shared_address(X + (16 * rb + (lane & 15)) * C::PX + (lane >> 4) * 8);
+      const uint32_t sa = shared_address(S + (lane & 15) * C::PB + (lane >> 4) * 8 + oc);
       // x Z
 #pragma unroll
       for (int k = 0; k < D / 16; ++k) {
@@ -149,68 +180,71 @@ chunk_kernel(const __grid_constant__ Problem p, const __grid_constant__ Split sp
 #pragma unroll
         for (int q = 0; q < C::kIn; ++q) load_matrices(x[q], xa + 2 * (q * C::kX + 16 * k));
 #pragma unroll
-        for (int t = 0; t < DB / 16; ++t) {
+        for (int t = 0; t < C::OC / 16; ++t) {
           uint32_t v[C::kMid][4];
 #pragma unroll
           for (int q = 0; q < C::kMid; ++q) load_matrices_turned(v[q], sa + 2 * (q * C::kS + 16 * k * C::PB + 16 * t));
           multiply_planes<C::kIn, C::kMid, C::kFloat>(o[2 * t], o[2 * t + 1], x, v);
         }
       }
-      const int row[2] = {16 * warp + gr, 16 * warp + gr + 8};
-      int seen[2] = {0, 0};
-      if (resets) seen[0] = count(row[0]), seen[1] = count(row[1]);
+      const int row[2] = {16 * rb + gr, 16 * rb + gr + 8};
+      int from[2];
+      float keep[2];
 #pragma unroll
-      for (int t = 0; t < DB / 8; ++t)
+      for (int half = 0; half < 2; ++half) {
+        bool none;
+        from[half] = linked_from((uint64_t(f + 1) << row[half]) - 1, &none);
+        keep[half] = none ? row_decay[half] : 0.0f;
+      }
 #pragma unroll
-        for (int q = 0; q < 4; ++q) o[t][q] = seen[q >> 1] == 0 ? row_decay[q >> 1] * o[t][q] : 0.0f;
-      // (W * x a') b, 16 tokens at a time up to the diagonal
+      for (int t = 0; t < C::OC / 8; ++t)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) o[t][q] *= keep[q >> 1];
+      // (W * x a') b, 16 tokens at a time from the diagonal to the left
       const uint32_t aa = shared_address(A + ((lane & 7) + (lane >> 4) * 8) * C::PX + ((lane >> 3) & 1) * 8);
-      const uint32_t ba = shared_address(B + (lane & 15) * C::PB + (lane >> 4) * 8);
-      for (int jb = 0; jb <= warp; ++jb) {
+      const uint32_t ba = shared_address(B + (lane & 15) * C::PB + (lane >> 4) * 8 + oc);
+      float far = 1.0f;
+      for (int jb = rb; jb >= 0; --jb) {
         float w[2][4] = {};
 #pragma unroll
         for (int k = 0; k < D / 16; ++k) {
-          uint32_t x[C::kIn][4];
+          uint32_t x[C::kIn][4], v[C::kIn][4];
 #pragma unroll
           for (int q = 0; q < C::kIn; ++q) load_matrices(x[q], xa + 2 * (q * C::kX + 16 * k));
-          uint32_t v[C::kIn][4];
 #pragma unroll
           for (int q = 0; q < C::kIn; ++q) load_matrices(v[q], aa + 2 * (q * C::kX + 16 * jb * C::PX + 16 * k));
           multiply_planes<C::kIn, C::kIn, C::kFloat>(w[0], w[1], x, v);
         }
-        const float far = jb < warp ? power(log2_g, 16 * (warp - 1 - jb)) : 1.0f;
+        const bool diagonal = jb == rb;
 #pragma unroll
         for (int q = 0; q < 8; ++q) {
-          bool linked = jb < warp || gr + (q & 2) * 4 >= gc + (q & 1) + (q & 4) * 2;
-          if (resets) linked = linked && seen[(q >> 1) & 1] == count(16 * jb + gc + (q & 1) + (q & 4) * 2);
-          const float weight = jb < warp ? next[q] * far : near[q];
-          w[q >> 2][q & 3] = linked ? weight * w[q >> 2][q & 3] : 0.0f;
+          const int j = 16 * jb + gc + (q & 1) + (q & 4) * 2;
+          const float weight = diagonal ? near[q] : next[q] * far;
+          w[q >> 2][q & 3] *= j >= from[(q >> 1) & 1] ? weight : 0.0f;
         }
+        if (!diagonal) far *= block_decay;
         uint32_t wp[C::kMid][4];
         split_pair<C::kMid>(w[0][0], w[0][1], &wp[0][0], 4);
         split_pair<C::kMid>(w[0][2], w[0][3], &wp[0][1], 4);
         split_pair<C::kMid>(w[1][0], w[1][1], &wp[0][2], 4);
         split_pair<C::kMid>(w[1][2], w[1][3], &wp[0][3], 4);
 #pragma unroll
-        for (int t = 0; t < DB / 16; ++t) {
+        for (int t = 0; t < C::OC / 16; ++t) {
           uint32_t v[C::kIn][4];
 #pragma unroll
           for (int q = 0; q < C::kIn; ++q) load_matrices_turned(v[q], ba + 2 * (q * C::kB + 16 * jb * C::PB + 16 * t));
           multiply_planes<C::kMid, C::kIn, C::kFloat>(o[2 * t], o[2 * t + 1], wp, v);
         }
       }
-      T* const out = static_cast<T*>(s.out);
 #pragma unroll
       for (int half = 0; half < 2; ++half) {
         const int64_t i = i0 + row[half];
-        const bool real = row[half] < len;
-        const int64_t t_ = s.reverse ? p.t - 1 - i : i;
-        T* const at = out + ((t_ * p.n + n) * p.h + h) * D + col + gc;
+        T* const at = static_cast<T*>(s.out) + (((s.reverse ? p.t - 1 - i : i) * p.n + n) * p.h + h) * D + col + oc + gc;
+        if (row[half] < len) {
 #pragma unroll
-        for (int t = 0; t < DB / 8; ++t) {
-          const float lo = p.scale * o[t][2 * half], hi = p.scale * o[t][2 * half + 1];
-          bad = fmaf(lo, 0.0f, bad), bad = fmaf(hi, 0.0f, bad);
-          if (real) {
+          for (int t = 0; t < C::OC / 8; ++t) {
+            const float lo = o[t][2 * half], hi = o[t][2 * half + 1];
+            bad = fmaf(lo, 0.0f, bad), bad = fmaf(hi, 0.0f, bad);
             if constexpr (sizeof(T) == 2)
               *reinterpret_cast<uint32_t*>(at + 8 * t) = pack(lo, hi);
             else
@@ -220,21 +254,27 @@ chunk_kernel(const __grid_constant__ Problem p, const __grid_constant__ Split sp
       }
     }
 
-    // Z <- g^L Z + (l * A)' B
+    // Z <- g^L Z + (l * A)' B, l_j = g^(L - f - j) where no reset lies between token j and the end
     if (holds) {
-      const float through = resets ? 0.0f : power(log2_g, len);
+      bool none;
+      const int reached = linked_from(~uint64_t(0), &none);
+      const float through = !none ? 0.0f : len == kChunk ? chunk_decay : power(log2_g, len);
 #pragma unroll
       for (int m = 0; m < C::MT; ++m)
 #pragma unroll
         for (int t = 0; t < C::NT; ++t)
 #pragma unroll
-          for (int q = 0; q < 4; ++q) z[m][t][q] = resets ? 0.0f : through * z[m][t][q];
+          for (int q = 0; q < 4; ++q) z[m][t][q] = none ? through * z[m][t][q] : 0.0f;
       const uint32_t at = shared_address(A + ((lane & 7) + (lane >> 4) * 8) * C::PX + ((lane >> 3) & 1) * 8 + srow);
       const uint32_t bt = shared_address(B + (lane & 15) * C::PB + (lane >> 4) * 8 + scol);
 #pragma unroll
       for (int j = 0; j < kChunk / 16; ++j) {
-        const float l0 = left[16 * j + gc], l1 = left[16 * j + gc + 1];
-        const float l2 = left[16 * j + gc + 8], l3 = left[16 * j + gc + 9];
+        float l[4];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const int i = 16 * j + gc + (q & 1) + (q & 2) * 4;
+          l[q] = i >= reached && i < len ? decays[i + kChunk - len] : 0.0f;
+        }
         uint32_t key[C::MT][C::kKeys][4];
 #pragma unroll
         for (int m = 0; m < C::MT; ++m) {
@@ -247,8 +287,7 @@ chunk_kernel(const __grid_constant__ Problem p, const __grid_constant__ Split sp
             for (int u = 0; u < 4; ++u) lo[u] += low_half(v[u]), hi[u] += high_half(v[u]);
           }
 #pragma unroll
-          for (int u = 0; u < 4; ++u)
-            split_pair<C::kKeys>((u & 2 ? l2 : l0) * lo[u], (u & 2 ? l3 : l1) * hi[u], &key[m][0][u], 4);
+          for (int u = 0; u < 4; ++u) split_pair<C::kKeys>(l[u & 2] * lo[u], l[(u & 2) + 1] * hi[u], &key[m][0][u], 4);
         }
 #pragma unroll
         for (int t = 0; t < C::NT / 2; ++t) {
@@ -257,11 +296,10 @@ chunk_kernel(const __grid_constant__ Problem p, const __grid_constant__ Split sp
           for (int q = 0; q < C::kIn; ++q) load_matrices_turned(v[q], bt + 2 * (q * C::kB + 16 * j * C::PB + 16 * t));
 #pragma unroll
           for (int m = 0; m < C::MT; ++m)
-            multiply_planes<C::kKeys, C::kIn, C::kFloat>(z[m][2 * t], z[m][2 * t + 1], key[m], v);
+            multiply_planes<C::kKeys, C::kIn, C::kFloat>(z[m][2 * t], z[m][2 * t + 1], key[m], v, fine);
         }
       }
     }
-    cut = cut || resets != 0;
     __syncthreads();
   }
 
@@ -277,8 +315,8 @@ chunk_kernel(const __grid_constant__ Problem p, const __grid_constant__ Split sp
   if (kLocal && threadIdx.x == 0 && col == 0) split.through[slot] = cut ? -1.0f : power(log2_g, last - first);
   // A value that is not finite may have met a masked zero on its way: the definition decides.
   if (__syncthreads_or(bad != bad)) {
-    scan_tokens<T, D, DB, attn::kThreads, !kLocal>(s, p, n, h, col, first, last, start, turned, start_mul,
-                                                   reinterpret_cast<float*>(smem), end, end_turned, end_mul);
+    scan_tokens<T, D, DB, C::kThreads, !kLocal>(s, p, n, h, col, first, last, start, turned, start_mul,
+                                                reinterpret_cast<float*>(smem), end, end_turned, end_mul);
     return;
   }
   if (end && holds) {
@@ -305,35 +343,49 @@ join_kernel(const __grid_constant__ Problem p, const __grid_constant__ Split spl
   const Scan& s = p.scan[scan];
   const int64_t outside = seq * size + (s.turned ? at % d * d + at / d : at);
   float z = s.carry_in ? s.in_mul * __ldg(s.carry_in + outside) : 0.0f;
-  for (int64_t g = 0; g < split.segments; ++g) {
-    float* const own = split.carry + (which * split.segments + g) * size + at;
-    const float through = split.through[which * split.segments + g];
-    const float mine = *own;
-    *own = z;
-    z = (through < 0.0f ? 0.0f : through * z) + mine;
+  float* const own = split.carry + which * split.segments * size + at;
+  const float* const through = split.through + which * split.segments;
+  constexpr int kAhead = 8;  // loads in flight: the sums are a chain, the loads are not
+  for (int64_t g0 = 0; g0 < split.segments; g0 += kAhead) {
+    float mine[kAhead], over[kAhead];
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i)
+      if (g0 + i < split.segments) mine[i] = own[(g0 + i) * size], over[i] = through[g0 + i];
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i)
+      if (g0 + i < split.segments) {
+        own[(g0 + i) * size] = z;
+        z = (over[i] < 0.0f ? 0.0f : over[i] * z) + mine[i];
+      }
   }
   if (s.carry_out) s.carry_out[outside] = s.out_mul * z;
 }
 
-// How a call is split over the time axis: not at all where the sequences fill the GPU, else into
-// segments of whole chunks until there are some kBlocksWanted blocks.
-constexpr int64_t kBlocksWanted = 148 * 4;
+// How a call is split over the time axis: not at all where the sequences fill the GPU or nearly so (the
+// segments' own carries cost a second pass over half the products), else into one round of blocks, as
+// many as fit the SMs at once.
+constexpr int64_t kSms = 148;
 
-int64_t split_segments(int64_t t, int64_t blocks, int64_t* per) {
-  const int64_t chunks = (t + attn::kChunk - 1) / attn::kChunk;
-  int64_t want = blocks >= kBlocksWanted / 2 ? 1 : kBlocksWanted / (blocks > 0 ? blocks : 1);
+int64_t split_segments(int64_t t, int64_t blocks, int per_sm, int64_t* per) {
+  const int64_t chunks = (t + attn::kChunk - 1) / attn::kChunk, room = kSms * per_sm;
+  int64_t want = blocks > 0 && 2 * blocks <= room ? room / blocks : 1;
   if (want > chunks) want = chunks;
   if (want < 1) want = 1;
   *per = chunks > 0 ? (chunks + want - 1) / want : 1;
   return chunks > 0 ? (chunks + *per - 1) / *per : 1;
 }
 
-int64_t attention_scratch(int d, int64_t t, int64_t n, int64_t h, int scans) {
-  int64_t per;
-  const int64_t tiles = d > 64 ? d / 64 : 1;
-  const int64_t segments = split_segments(t, n * h * scans * tiles, &per);
-  return segments == 1 ? 0 : scans * n * h * segments * (int64_t(d) * d + 1) * 4;
-}
+struct ScratchSize {
+  int64_t t, n, h;
+  int scans;
+  template <typename T, int D>
+  int64_t operator()() const {
+    int64_t per;
+    const int64_t segments =
+        split_segments(t, n * h * scans * (D / attn::Shape<T, D>::DB), attn::Shape<T, D>::kPerSm, &per);
+    return segments == 1 ? 0 : scans * n * h * segments * (int64_t(D) * D + 1) * 4;
+  }
+};
 
 template <typename T, int D>
 int launch_scan(const Problem& p, void* scratch, cudaStream_t stream) {
@@ -341,7 +393,7 @@ int launch_scan(const Problem& p, void* scratch, cudaStream_t stream) {
   constexpr int kTiles = D / C::DB;
   Split split{};
   const int64_t sequences = p.n * p.h;
-  split.segments = split_segments(p.t, sequences * p.scans * kTiles, &split.per);
+  split.segments = split_segments(p.t, sequences * p.scans * kTiles, C::kPerSm, &split.per);
   const int64_t blocks = sequences * p.scans * kTiles * split.segments;
   if (blocks > 0x7fffffff) return RLENV_EINVAL;
   if (cudaError_t e = cudaFuncSetAttribute(chunk_kernel<T, D, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem))
@@ -351,12 +403,12 @@ int launch_scan(const Problem& p, void* scratch, cudaStream_t stream) {
     split.through = split.carry + p.scans * sequences * split.segments * D * D;
     if (cudaError_t e = cudaFuncSetAttribute(chunk_kernel<T, D, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem))
       return int(e);
-    chunk_kernel<T, D, true><<<unsigned(blocks), attn::kThreads, C::kSmem, stream>>>(p, split);
+    chunk_kernel<T, D, true><<<unsigned(blocks), C::kThreads, C::kSmem, stream>>>(p, split);
     if (const int rc = launch_status()) return rc;
     join_kernel<<<grid_for(p.scans * sequences * D * D, 256), 256, 0, stream>>>(p, split, D);
     if (const int rc = launch_status()) return rc;
   }
-  chunk_kernel<T, D, false><<<unsigned(blocks), attn::kThreads, C::kSmem, stream>>>(p, split);
+  chunk_kernel<T, D, false><<<unsigned(blocks), C::kThreads, C::kSmem, stream>>>(p, split);
   return launch_status();
 }
 
@@ -419,8 +471,8 @@ step_kernel(const T* __restrict__ q, const T* __restrict__ k, const T* __restric
 bool width_built(int d) { return d == 16 || d == 32 || d == 64 || d == 128; }
 
 // Calls fn<T, D>() for the type and width.
-template <typename F>
-int dispatch(int dtype, int d, F&& fn) {
+template <typename R, typename F>
+R dispatch(int dtype, int d, F&& fn) {
   if (dtype == RLENV_F32) {
     switch (d) {
       case 16: return fn.template operator()<float, 16>();
@@ -473,7 +525,7 @@ extern "C" {
 
 int64_t rlenv_linear_attention_scratch_bytes(int dtype, int d, int64_t t, int64_t n, int64_t h, int backward) {
   using namespace rlenv;
-  return check_sizes(dtype, d, t, n, h, 1.0f) == RLENV_OK ? attention_scratch(d, t, n, h, backward ? 3 : 1) : -1;
+  return check_sizes(dtype, d, t, n, h, 1.0f) == RLENV_OK ? dispatch<int64_t>(dtype, d, ScratchSize{t, n, h, backward ? 3 : 1}) : -1;
 }
 
 int rlenv_linear_attention_forward(int dtype, int d, int64_t t, int64_t n, int64_t h, const void* q, const void* k,
@@ -489,12 +541,12 @@ int rlenv_linear_attention_forward(int dtype, int d, int64_t t, int64_t n, int64
   const int64_t* st = t > 0 ? strides : kNone;
   if (!aligned_rows(q, st, dtype, 3) || !aligned_rows(k, st + 3, dtype, 3) || !aligned_rows(v, st + 6, dtype, 3))
     return RLENV_EINVAL;
-  if (!scratch_holds(scratch, scratch_bytes, attention_scratch(d, t, n, h, 1))) return RLENV_EINVAL;
+  if (!scratch_holds(scratch, scratch_bytes, dispatch<int64_t>(dtype, d, ScratchSize{t, n, h, 1}))) return RLENV_EINVAL;
   Problem p{};
   p.t = t, p.n = n, p.h = h, p.decay = decay, p.resets = resets, p.scale = scale, p.scans = 1;
   p.scan[0] = Scan{q, k, v, {st[0], st[1], st[2]}, {st[3], st[4], st[5]}, {st[6], st[7], st[8]},
                    out, state_in, state_out, 1.0f, 1.0f, 0, 0};
-  return dispatch(dtype, d, Runner{p, scratch, as_stream(stream)});
+  return dispatch<int>(dtype, d, Runner{p, scratch, as_stream(stream)});
 }
 
 int rlenv_linear_attention_backward(int dtype, int d, int64_t t, int64_t n, int64_t h, const void* grad_out,
@@ -512,7 +564,7 @@ int rlenv_linear_attention_backward(int dtype, int d, int64_t t, int64_t n, int6
   if (!aligned_rows(grad_out, st, dtype, 3) || !aligned_rows(q, st + 3, dtype, 3) ||
       !aligned_rows(k, st + 6, dtype, 3) || !aligned_rows(v, st + 9, dtype, 3))
     return RLENV_EINVAL;
-  if (!scratch_holds(scratch, scratch_bytes, attention_scratch(d, t, n, h, 3))) return RLENV_EINVAL;
+  if (!scratch_holds(scratch, scratch_bytes, dispatch<int64_t>(dtype, d, ScratchSize{t, n, h, 3}))) return RLENV_EINVAL;
   const Strides ds{st[0], st[1], st[2]}, qs{st[3], st[4], st[5]}, ks{st[6], st[7], st[8]}, vs{st[9], st[10], st[11]};
   Problem p{};
   p.t = t, p.n = n, p.h = h, p.decay = decay, p.resets = resets, p.scale = scale, p.scans = 3;
@@ -521,7 +573,7 @@ int rlenv_linear_attention_backward(int dtype, int d, int64_t t, int64_t n, int6
   p.scan[0] = Scan{grad_out, v, k, ds, vs, ks, grad_q, state_in, nullptr, 1.0f, 1.0f, 1, 0};
   p.scan[1] = Scan{v, grad_out, q, vs, ds, qs, grad_k, grad_state_out, nullptr, inv, scale, 1, 1};
   p.scan[2] = Scan{k, q, grad_out, ks, qs, ds, grad_v, grad_state_out, grad_state_in, inv, scale, 0, 1};
-  return dispatch(dtype, d, Runner{p, scratch, as_stream(stream)});
+  return dispatch<int>(dtype, d, Runner{p, scratch, as_stream(stream)});
 }
 
 }  // extern "C"
@@ -559,7 +611,7 @@ extern "C" int rlenv_linear_attention_step(int dtype, int d, int64_t n, int64_t 
   if (!aligned_rows(q, strides, dtype, 2) || !aligned_rows(k, strides + 2, dtype, 2) ||
       !aligned_rows(v, strides + 4, dtype, 2) || reinterpret_cast<uintptr_t>(state) % 16)
     return RLENV_EINVAL;
-  return dispatch(dtype, d,
+  return dispatch<int>(dtype, d,
                   StepRunner{q, k, v, {0, strides[0], strides[1]}, {0, strides[2], strides[3]},
                              {0, strides[4], strides[5]}, decay, resets, scale, n, h, state, out, as_stream(stream)});
 }

@@ -130,24 +130,33 @@ RLENV_D void scan_tokens(const Scan& s, const Problem& p, int64_t n, int64_t h, 
 // the decayed keys three, since the carry goes out in float32. Of the products of planes those
 // below 2^-24 of the whole are left out.
 constexpr int kChunk = 64;
-constexpr int kThreads = 128;  // four warps, each 16 tokens of the chunk
 
 template <typename T, int D>
 struct Shape {
-  static constexpr int kIn = sizeof(T) == 4 ? 3 : 1;    // planes of x, a, b
-  static constexpr int kMid = sizeof(T) == 4 ? 3 : 2;   // of the weighted products and the carry
-  static constexpr int kKeys = 3;                       // of the decayed keys
   static constexpr bool kFloat = sizeof(T) == 4;
+  static constexpr int kIn = kFloat ? 3 : 1;            // planes of x, a, b
+  static constexpr int kMid = kFloat ? 3 : 2;           // of the weighted products and the carry
+  static constexpr int kKeys = 3;                       // of the decayed keys
   static constexpr int DB = D < 64 ? D : 64;            // columns of the carry that a block owns
   static constexpr int PX = D + 8, PB = DB + 8;         // row pitches: 16 bytes past a multiple of 32,
                                                         // so that eight rows' pieces fall in distinct banks
   static constexpr int kX = kChunk * PX, kB = kChunk * PB, kS = D * PB;  // a plane's elements
-  static constexpr int kSmem = 2 * (kIn * (2 * kX + kB) + kMid * kS);
+  // Four warps with 16 tokens of the chunk each, or eight, two to a row of 16 with half the columns
+  // each, where a block's shared memory leaves room for few of them (float32, and 128 columns).
+  static constexpr int kWarps = D == 128 || (kFloat && D >= 32) ? 8 : 4;
+  static constexpr int kThreads = 32 * kWarps;
+  static constexpr int OC = DB / (kWarps / 4);          // output columns a warp
+  // Tiles come two chunks deep for bfloat16 (cp.async); float32 ones pass through registers, where they
+  // become planes, one chunk ahead.
+  static constexpr int kBuffers = kFloat ? 1 : 2;
+  static constexpr int kTiles = kIn * (2 * kX + kB);    // elements of a buffer
+  static constexpr int kSmem = 2 * (kBuffers * kTiles + kMid * kS);
   // The carry's rows and columns by warp: RG groups of rows, CG of columns.
-  static constexpr int MT = D > 64 ? D / 64 : 1;        // 16-row tiles a warp
+  static constexpr int MT = D / 16 > kWarps ? D / 16 / kWarps : 1;  // 16-row tiles a warp
   static constexpr int RG = D / (16 * MT);
-  static constexpr int CG = 4 / RG < DB / 16 ? 4 / RG : DB / 16;
+  static constexpr int CG = kWarps / RG < DB / 16 ? kWarps / RG : DB / 16;
   static constexpr int NT = DB / CG / 8;                // 8-column tiles a warp
+  static constexpr int kPerSm = kSmem > 113000 ? 1 : kSmem > 75000 ? 2 : kWarps == 8 ? 2 : 3;  // blocks that fit
 };
 
 RLENV_D uint32_t shared_address(const void* p) { return uint32_t(__cvta_generic_to_shared(p)); }
@@ -170,15 +179,17 @@ RLENV_D void multiply(float c[4], const uint32_t a[4], uint32_t b0, uint32_t b1)
 // c0, c1 (two 8-column tiles) += a b over all pairs of planes worth it, the small ones first. The tensor
 // core truncates as it accumulates: for float32 results (three planes of data) the pairs are summed from
 // zero and added to c in a rounded addition, or the error of long sums grows to a few 1e-6.
+// The last plane of a only where `fine`.
 template <int NA, int NB, bool kFloat>
-RLENV_D void multiply_planes(float c0[4], float c1[4], const uint32_t (&a)[NA][4], const uint32_t (&b)[NB][4]) {
+RLENV_D void multiply_planes(float c0[4], float c1[4], const uint32_t (&a)[NA][4], const uint32_t (&b)[NB][4],
+                             bool fine = true) {
   float s0[4] = {}, s1[4] = {};
 #pragma unroll
   for (int order = 2; order >= 0; --order)
 #pragma unroll
     for (int u = 0; u <= order; ++u) {
       const int q = order - u;
-      if (u < NA && q < NB) {
+      if (u < NA && q < NB && (u + 1 < NA || fine)) {
         multiply(kFloat ? s0 : c0, a[u], b[q][0], b[q][1]);
         multiply(kFloat ? s1 : c1, a[u], b[q][2], b[q][3]);
       }
@@ -210,33 +221,55 @@ RLENV_D void split_pair(float lo, float hi, uint32_t* planes, int stride) {
 RLENV_D void copy_async_16(uint32_t to, const void* from, bool real) {  // zeros where not real
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(real ? 16 : 0) : "memory");
 }
-RLENV_D void copies_landed() { asm volatile("cp.async.wait_all;" ::: "memory"); }
+RLENV_D void copies_end() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int kLeft>  // all but the latest kLeft groups have landed
+RLENV_D void copies_landed() { asm volatile("cp.async.wait_group %0;" ::"n"(kLeft) : "memory"); }
 
-// W columns of kChunk rows from token position `first` (positions past `last` are zeros) into planes
-// at `to`, pitch P.
-template <typename T, int W, int P, int kPlane>
-RLENV_D void load_tile(const T* base, int64_t stride, const Scan& s, int64_t tokens, int64_t first, int64_t last,
-                       __nv_bfloat16* to) {
-  constexpr int kPer = 16 / sizeof(T), kPieces = W / kPer;
-  const uint32_t at = shared_address(to);
-#pragma unroll 4
-  for (int e = threadIdx.x; e < kChunk * kPieces; e += kThreads) {
-    const int r = e / kPieces, c = e % kPieces * kPer;
-    const int64_t i = first + r;
-    const bool real = i < last;
-    const T* from = base + (real ? (s.reverse ? tokens - 1 - i : i) : 0) * stride + c;
-    if constexpr (sizeof(T) == 2) {
-      copy_async_16(at + (r * P + c) * 2, from, real);
-    } else {
-      const float4 v = real ? __ldg(reinterpret_cast<const float4*>(from)) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-      uint32_t lo[3], hi[3];
-      split_pair<3>(v.x, v.y, lo, 1);
-      split_pair<3>(v.z, v.w, hi, 1);
+// A thread's share of a tile of kChunk rows and W columns: 16-byte pieces of every kRowStep-th row, at a
+// fixed column. `at` follows the tokens of one chunk after the other.
+template <typename T, int W, int P, int kPlane, int kThreads>
+struct TileLoader {
+  static constexpr int kPer = 16 / sizeof(T), kPieces = W / kPer;
+  static constexpr int kRowStep = kThreads / kPieces;
+  static constexpr int kCount = kChunk / kRowStep;
+  static_assert(kCount >= 1, "every thread has a piece");
+  const T* at;
+  int64_t step;  // kRowStep tokens on
+  int row, col;
+  RLENV_D TileLoader(const T* base, int64_t stride, bool reverse, int64_t tokens, int64_t first) {
+    row = threadIdx.x / kPieces, col = threadIdx.x % kPieces * kPer;
+    const int64_t i = first + row;
+    at = base + (reverse ? tokens - 1 - i : i) * stride + col;
+    step = (reverse ? -stride : stride) * kRowStep;
+  }
+  RLENV_D bool real(int u, int64_t left) const { return row + u * kRowStep < left; }
+  RLENV_D void advance() { at += step * kCount; }
+  // bfloat16: straight to shared memory, zeros past `left` rows
+  RLENV_D void copy(uint32_t to, int64_t left) const {
 #pragma unroll
-      for (int q = 0; q < 3; ++q) *reinterpret_cast<uint2*>(to + q * kPlane + r * P + c) = make_uint2(lo[q], hi[q]);
+    for (int u = 0; u < kCount; ++u) {
+      const bool r = real(u, left);
+      copy_async_16(to + ((row + u * kRowStep) * P + col) * 2, r ? at + u * step : at - row * (step / kRowStep), r);
     }
   }
-}
+  // float32: into registers, and from there as planes
+  RLENV_D void fetch(float4 (&v)[kCount], int64_t left) const {
+#pragma unroll
+    for (int u = 0; u < kCount; ++u)
+      v[u] = real(u, left) ? __ldg(reinterpret_cast<const float4*>(at + u * step)) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  }
+  RLENV_D void put(__nv_bfloat16* to, const float4 (&v)[kCount]) const {
+#pragma unroll
+    for (int u = 0; u < kCount; ++u) {
+      uint32_t lo[3], hi[3];
+      split_pair<3>(v[u].x, v[u].y, lo, 1);
+      split_pair<3>(v[u].z, v[u].w, hi, 1);
+#pragma unroll
+      for (int q = 0; q < 3; ++q)
+        *reinterpret_cast<uint2*>(to + q * kPlane + (row + u * kRowStep) * P + col) = make_uint2(lo[q], hi[q]);
+    }
+  }
+};
 
 }  // namespace attn
 }  // namespace rlenv
