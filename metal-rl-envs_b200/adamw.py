@@ -13,8 +13,10 @@ Gradients are expected to be finite; a value that is not makes its own element's
 NaN or infinite and no other's.
 """
 
-import ctypes
+from array import array
 from dataclasses import dataclass
+from functools import lru_cache
+from operator import attrgetter
 
 import torch
 
@@ -39,6 +41,7 @@ class State:
     seed: int = 0
 
 
+@lru_cache(maxsize=64)
 def _blocks(sizes):
     return sum(-(-n // BLOCK) for n in sizes)
 
@@ -48,7 +51,7 @@ def init_state(params, bits=32, seed=0):
     if bits not in (8, 32):
         raise ValueError(f"moments are held in 8 or 32 bits; got {bits}")
     sizes = tuple(p.numel() for p in params)
-    dev = _rl.same_device(**{f"params[{i}]": p for i, p in enumerate(params)}) if params else _rl.device()
+    dev = params[0].device if params else _rl.device()
     blocks = _blocks(sizes)
 
     def zeros(n, dtype):
@@ -60,18 +63,37 @@ def init_state(params, bits=32, seed=0):
                  zeros(blocks, torch.uint8), zeros(blocks, torch.uint8), seed=seed)
 
 
-def _check_state(state, dev):
-    blocks = _blocks(state.sizes)
+def _check_state(state):
+    """The state's device index; raises where its tensors do not fit its sizes."""
+    blocks = _blocks(tuple(state.sizes))
     if state.bits not in (8, 32):
         raise ValueError(f"moments are held in 8 or 32 bits; got {state.bits}")
-    kinds = [("m", torch.float32 if state.bits == 32 else torch.uint8, blocks * BLOCK)]
-    kinds.append(("v",) + kinds[0][1:])
+    kind = torch.float32 if state.bits == 32 else torch.uint8
+    index = state.m.get_device()
+    _expect("state.m", state.m, kind, blocks * BLOCK, index)
+    _expect("state.v", state.v, kind, blocks * BLOCK, index)
     if state.bits == 8:
-        kinds += [("m_exp", torch.uint8, blocks), ("v_exp", torch.uint8, blocks)]
-    for name, dtype, n in kinds:
-        x = getattr(state, name)
-        if x is None or x.dtype != dtype or x.numel() != n or not x.is_contiguous() or x.device != dev:
-            raise ValueError(f"state.{name} must be {n} contiguous {dtype} elements on {dev}")
+        _expect("state.m_exp", state.m_exp, torch.uint8, blocks, index)
+        _expect("state.v_exp", state.v_exp, torch.uint8, blocks, index)
+    return index
+
+
+def _expect(name, x, dtype, n, index):
+    if x is None or x.dtype is not dtype or x.numel() != n or not x.is_contiguous() or x.get_device() != index \
+            or index < 0:
+        raise ValueError(f"{name} must be {n} contiguous {dtype} elements on the state's CUDA device")
+
+
+_dtype, _numel, _index = attrgetter("dtype"), torch.Tensor.numel, torch.Tensor.get_device
+_dense, _pointer = torch.Tensor.is_contiguous, torch.Tensor.data_ptr
+
+
+def _check_list(name, tensors, dtype, sizes, index):
+    """Every tensor dense, of dtype, on the device, of its size: the whole list in a few passes that run in
+    the interpreter's C loops (a policy has dozens of small tensors and a step of some microseconds)."""
+    if set(map(_dtype, tensors)) != {dtype} or set(map(_index, tensors)) != {index} or not all(map(_dense, tensors)) \
+            or tuple(map(_numel, tensors)) != sizes:
+        raise ValueError(f"{name} must be contiguous {dtype} tensors on cuda:{index} of the state's sizes {sizes}")
 
 
 def step(params, grads, state, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.01, copies=None,
@@ -79,54 +101,41 @@ def step(params, grads, state, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_dec
     """Updates params, state and copies in place. grads: one tensor a parameter, all of one dtype.
     grad_scale, a one-element float32 CUDA tensor, multiplies every gradient (clipping by a norm that
     stays on the device)."""
-    count = len(params)
-    if len(grads) != count or (copies is not None and len(copies) != count) or len(state.sizes) != count:
-        raise ValueError(f"{count} params need as many grads, copies and state.sizes")
+    count, sizes = len(state.sizes), tuple(state.sizes)
+    if len(params) != count or len(grads) != count or (copies is not None and len(copies) != count):
+        raise ValueError(f"{len(params)} params need as many grads, copies and state.sizes")
     if count == 0:
         state.step += 1
         return
-    dev, grad_dtype = params[0].device, grads[0].dtype
+    index, grad_dtype = _check_state(state), grads[0].dtype
     if grad_dtype not in _rl.FLOAT_DTYPES:
         raise ValueError(f"grads must be float32 or bfloat16; got {grad_dtype}")
-    for i, (p, g, n) in enumerate(zip(params, grads, state.sizes)):
-        if p.dtype != torch.float32 or not p.is_contiguous() or p.device != dev or not p.is_cuda or p.numel() != n:
-            raise ValueError(f"params[{i}] must be {n} contiguous float32 elements on one CUDA device")
-        if g.dtype != grad_dtype or g.device != dev or g.shape != p.shape:
-            raise ValueError(f"grads[{i}] must be {grad_dtype} on {dev}, of its parameter's shape")
+    _check_list("params", params, torch.float32, sizes, index)
+    if not all(map(_dense, grads)):
+        grads = [g.contiguous() for g in grads]
+    _check_list("grads", grads, grad_dtype, sizes, index)
     if copies is not None:
-        for i, (p, c) in enumerate(zip(params, copies)):
-            if c.dtype != torch.bfloat16 or not c.is_contiguous() or c.device != dev or c.shape != p.shape:
-                raise ValueError(f"copies[{i}] must be contiguous bfloat16 on {dev}, of its parameter's shape")
+        _check_list("copies", copies, torch.bfloat16, sizes, index)
     if grad_scale is not None:
-        _rl.as_floats("grad_scale", grad_scale, dtype=torch.float32)
-        if grad_scale.numel() != 1 or grad_scale.device != dev:
-            raise ValueError(f"grad_scale must be one float32 on {dev}")
-    _check_state(state, dev)
+        _expect("grad_scale", grad_scale, torch.float32, 1, index)
     b1, b2 = betas
-    grads = [g.contiguous() for g in grads]
-    pointers = ctypes.c_void_p * count
-    with torch.cuda.device(dev):
-        _rl.check(_rl.lib().adamw_step(
-            state.bits, _rl.FLOAT_DTYPES[grad_dtype], count, pointers(*[p.data_ptr() for p in params]),
-            pointers(*[g.data_ptr() for g in grads]),
-            pointers(*[c.data_ptr() for c in copies]) if copies is not None else None,
-            (ctypes.c_int64 * count)(*state.sizes), state.m.data_ptr(), state.v.data_ptr(), _rl.ptr(state.m_exp),
-            _rl.ptr(state.v_exp), lr, b1, b2, eps, weight_decay, _rl.ptr(grad_scale), state.step + 1,
-            state.seed & 0xFFFFFFFF, _rl.stream_ptr(dev)))
+    # the lists of pointers and sizes, alive until the call returns
+    lists = [array("Q", map(_pointer, params)), array("Q", map(_pointer, grads)),
+             array("Q", map(_pointer, copies)) if copies is not None else None, array("q", sizes)]
+    params_at, grads_at, copies_at, sizes_at = (None if x is None else x.buffer_info()[0] for x in lists)
+    _rl.launch(index, _rl.lib().adamw_step, state.bits, _rl.FLOAT_DTYPES[grad_dtype], count, params_at, grads_at,
+               copies_at, sizes_at, state.m.data_ptr(), state.v.data_ptr(), _rl.ptr(state.m_exp), _rl.ptr(state.v_exp),
+               lr, b1, b2, eps, weight_decay, _rl.ptr(grad_scale), state.step + 1, state.seed & 0xFFFFFFFF)
     state.step += 1
 
 
 def moments(state):
     """(m, v), flat float32 tensors laid out as the state's: the state's own where it holds 32 bits, the
     values that its codes stand for where it holds 8."""
-    dev = state.m.device
-    _check_state(state, dev)
     if state.bits == 32:
         return state.m, state.v
-    with torch.cuda.device(dev):
-        m = torch.empty(state.m.numel(), dtype=torch.float32, device=dev)
-        v = torch.empty_like(m)
-        _rl.check(_rl.lib().adamw_moments(state.m_exp.numel(), state.m.data_ptr(), state.v.data_ptr(),
-                                          state.m_exp.data_ptr(), state.v_exp.data_ptr(), m.data_ptr(), v.data_ptr(),
-                                          _rl.stream_ptr(dev)))
+    index = _check_state(state)
+    m, v = (state.m.new_empty(state.m.numel(), dtype=torch.float32) for _ in range(2))
+    _rl.launch(index, _rl.lib().adamw_moments, state.m_exp.numel(), state.m.data_ptr(), state.v.data_ptr(),
+               state.m_exp.data_ptr(), state.v_exp.data_ptr(), m.data_ptr(), v.data_ptr())
     return m, v

@@ -516,6 +516,99 @@ add_parts_kernel(const float* __restrict__ parts, int splits, int64_t size, T* _
   (e < size ? dwg : dwu)[e < size ? e : e - size] = T(sum);
 }
 
+// ---- few rows ----------------------------------------------------------------------------------------
+
+// h for up to kFew rows of x at a time, a policy acting: matrix-vector products, bound by reading the
+// weights. A block owns 32 columns of both weights; its warps split the contraction, each thread reading 16
+// bytes of every kApart-th row, and the sums meet in shared memory in a fixed order.
+constexpr int kFewThreads = 256, kFewCols = 32;
+
+template <typename T, bool kWide>
+RLENV_D void load_columns(const T* p, int n, float (&v)[16 / sizeof(T)]) {
+  constexpr int kPer = 16 / sizeof(T);
+  if constexpr (kWide && sizeof(T) == 2) {
+    const uint4 w = __ldg(reinterpret_cast<const uint4*>(p));
+    const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[2 * i] = __uint_as_float(u[i] << 16), v[2 * i + 1] = __uint_as_float(u[i] & 0xffff0000u);
+  } else if constexpr (kWide) {
+    const float4 w = __ldg(reinterpret_cast<const float4*>(p));
+    v[0] = w.x, v[1] = w.y, v[2] = w.z, v[3] = w.w;
+  } else {
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) v[i] = i < n ? float(p[i]) : 0.0f;
+  }
+}
+
+template <typename T, int kFew, bool kWide>
+__global__ void __launch_bounds__(kFewThreads)
+few_rows_kernel(const T* __restrict__ x, const T* __restrict__ wg, const T* __restrict__ wu, int64_t m, int64_t k,
+                int64_t f, int act, T* __restrict__ out) {
+  constexpr int kPer = 16 / sizeof(T), kAcross = kFewCols / kPer, kApart = kFewThreads / kAcross;
+  constexpr int kUnroll = kFew > 4 ? 4 : 8;
+  __shared__ float parts[kFewThreads / 32][2 * kFew * kFewCols];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, own = lane % kAcross * kPer;
+  const int64_t c = int64_t(blockIdx.x) * kFewCols + own, m0 = int64_t(blockIdx.y) * kFew;
+  const int n = int(min(int64_t(kPer), max(int64_t(0), f - c)));
+  float g[kFew][kPer] = {}, u[kFew][kPer] = {};
+  if (n > 0) {
+#pragma unroll kUnroll
+    for (int64_t i = threadIdx.x / kAcross; i < k; i += kApart) {
+      float a[kPer], b[kPer];
+      load_columns<T, kWide>(wg + i * f + c, n, a);
+      load_columns<T, kWide>(wu + i * f + c, n, b);
+#pragma unroll
+      for (int r = 0; r < kFew; ++r) {
+        const float xr = m0 + r < m ? float(x[(m0 + r) * k + i]) : 0.0f;
+#pragma unroll
+        for (int j = 0; j < kPer; ++j) g[r][j] = fmaf(xr, a[j], g[r][j]), u[r][j] = fmaf(xr, b[j], u[r][j]);
+      }
+    }
+  }
+#pragma unroll
+  for (int r = 0; r < kFew; ++r)
+#pragma unroll
+    for (int j = 0; j < kPer; ++j) {
+#pragma unroll
+      for (int o = 16; o >= kAcross; o >>= 1) {
+        g[r][j] += __shfl_xor_sync(0xffffffffu, g[r][j], o);
+        u[r][j] += __shfl_xor_sync(0xffffffffu, u[r][j], o);
+      }
+      if (lane < kAcross) {
+        parts[warp][r * kFewCols + own + j] = g[r][j];
+        parts[warp][(kFew + r) * kFewCols + own + j] = u[r][j];
+      }
+    }
+  __syncthreads();
+  for (int e = threadIdx.x; e < kFew * kFewCols; e += kFewThreads) {
+    const int64_t r = m0 + e / kFewCols, col = int64_t(blockIdx.x) * kFewCols + e % kFewCols;
+    if (r >= m || col >= f) continue;
+    float sg = 0.0f, su = 0.0f;
+#pragma unroll
+    for (int w = 0; w < kFewThreads / 32; ++w) sg += parts[w][e], su += parts[w][kFew * kFewCols + e];
+    float y, slope;
+    if (act == kSilu) activate<false, kSilu>(sg, &y, &slope);
+    else activate<false, kGelu>(sg, &y, &slope);
+    out[r * f + col] = T(y * su);
+  }
+}
+
+template <typename T, int kFew>
+int few_rows(const void* x, const void* wg, const void* wu, int64_t m, int64_t k, int64_t f, int act, void* out,
+             cudaStream_t s) {
+  const dim3 grid(unsigned((f + kFewCols - 1) / kFewCols), unsigned((m + kFew - 1) / kFew));
+  const T *X = static_cast<const T*>(x), *G = static_cast<const T*>(wg), *U = static_cast<const T*>(wu);
+  if (f * int64_t(sizeof(T)) % 16 == 0)
+    few_rows_kernel<T, kFew, true><<<grid, kFewThreads, 0, s>>>(X, G, U, m, k, f, act, static_cast<T*>(out));
+  else
+    few_rows_kernel<T, kFew, false><<<grid, kFewThreads, 0, s>>>(X, G, U, m, k, f, act, static_cast<T*>(out));
+  return launch_status();
+}
+
+// Up to how many rows the products are formed this way. The tensor-core kernel reads the weights once for
+// all rows, but with a tile's latency (some 10 us), and float32 weights are laid out as planes first.
+constexpr int64_t kFewestRowsTiled[2] = {17, 65};  // bfloat16, float32
+
 // ---- host ------------------------------------------------------------------------------------------
 
 constexpr int64_t kMaxExtent = int64_t(1) << 31;
@@ -580,6 +673,7 @@ Layout lay_out(int dtype, int64_t m, int64_t k, int64_t f, bool backward, void* 
   Scratch s{static_cast<unsigned char*>(scratch), 0};
   Layout l{};
   const int64_t n = planes(dtype);
+  if (!backward && m < kFewestRowsTiled[dtype == RLENV_F32]) return l;
   if (packs(dtype, k)) l.x = s.take(n * m * round_up(k, 8) * 2);
   if (packs(dtype, f)) l.wg = s.take(n * k * round_up(f, 8) * 2), l.wu = s.take(n * k * round_up(f, 8) * 2);
   if (backward) {
@@ -626,6 +720,11 @@ template <typename T>
 int ffn(const void* dh, const void* x, const void* wg, const void* wu, int64_t m, int64_t k, int64_t f, int act,
         void* out, void* dx, void* dwg, void* dwu, const Layout& l, cudaStream_t s) {
   using C = Tile<T>;
+  if (!dh && m < kFewestRowsTiled[C::kFloat])
+    return m == 1   ? few_rows<T, 1>(x, wg, wu, m, k, f, act, out, s)
+           : m == 2 ? few_rows<T, 2>(x, wg, wu, m, k, f, act, out, s)
+           : m <= 4 ? few_rows<T, 4>(x, wg, wu, m, k, f, act, out, s)
+                    : few_rows<T, 8>(x, wg, wu, m, k, f, act, out, s);
   Operand X, G, U;
   if (const int rc = operand<T>(x, m, k, l.x, s, &X)) return rc;
   if (const int rc = operand<T>(wg, k, f, l.wg, s, &G)) return rc;

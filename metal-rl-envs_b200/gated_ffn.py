@@ -25,47 +25,45 @@ def _dense(x):
 
 def _check(x, w_gate, w_up, activation, grad_out=None):
     _rl.as_floats("x", x)
-    if x.dim() < 1:
-        raise ValueError("x must have at least one axis")
-    _rl.as_floats("w_gate", w_gate, (x.shape[-1], None), x.dtype)
+    if x.dim() < 1 or w_gate.dim() != 2 or w_gate.shape[0] != x.shape[-1]:
+        raise ValueError(f"x must be (..., K) and w_gate (K, F); got {tuple(x.shape)} and {tuple(w_gate.shape)}")
+    _rl.as_floats("w_gate", w_gate, None, x.dtype)
     _rl.as_floats("w_up", w_up, w_gate.shape, x.dtype)
     if grad_out is not None:
         _rl.as_floats("grad_out", grad_out, (*x.shape[:-1], w_gate.shape[1]), x.dtype)
     if activation not in ACTIVATIONS:
         raise ValueError(f"activation must be one of {sorted(ACTIVATIONS)}; got {activation!r}")
-    dev = _rl.same_device(x=x, w_gate=w_gate, w_up=w_up, grad_out=grad_out)
-    m = x.numel() // x.shape[-1] if x.shape[-1] else torch.Size(x.shape[:-1]).numel()
-    return m, x.shape[-1], w_gate.shape[1], _rl.FLOAT_DTYPES[x.dtype], dev
+    index = x.get_device()
+    _rl.one_device(index, w_gate=w_gate, w_up=w_up, grad_out=grad_out)
+    k, f = w_gate.shape
+    return x.numel() // k if k else x.shape[:-1].numel(), k, f, _rl.FLOAT_DTYPES[x.dtype], index
 
 
 def forward(x, w_gate, w_up, activation="silu"):
     """act(x w_gate) * (x w_up), (..., F)."""
-    m, k, f, code, dev = _check(x, w_gate, w_up, activation)
+    m, k, f, code, index = _check(x, w_gate, w_up, activation)
     x, w_gate, w_up = _dense(x), _dense(w_gate), _dense(w_up)
     lib = _rl.lib()
-    with torch.cuda.device(dev):
-        out = torch.empty((*x.shape[:-1], f), dtype=x.dtype, device=dev)
-        nbytes = lib.gated_ffn_scratch_bytes(code, m, k, f, 0)
-        tmp = _rl.scratch(nbytes, dev)
-        _rl.check(lib.gated_ffn_forward(code, ACTIVATIONS[activation], m, k, f, x.data_ptr(), w_gate.data_ptr(),
-                                        w_up.data_ptr(), out.data_ptr(), _rl.ptr(tmp), nbytes, _rl.stream_ptr(dev)))
+    out = x.new_empty((*x.shape[:-1], f))
+    nbytes = lib.gated_ffn_scratch_bytes(code, m, k, f, 0)
+    tmp = _rl.scratch(nbytes, x)
+    _rl.launch(index, lib.gated_ffn_forward, code, ACTIVATIONS[activation], m, k, f, x.data_ptr(), w_gate.data_ptr(),
+               w_up.data_ptr(), out.data_ptr(), _rl.ptr(tmp), nbytes)
     return out
 
 
 def backward(grad_out, x, w_gate, w_up, activation="silu"):
     """(dx, dw_gate, dw_up) of `forward` from grad_out (..., F)."""
-    m, k, f, code, dev = _check(x, w_gate, w_up, activation, grad_out)
+    m, k, f, code, index = _check(x, w_gate, w_up, activation, grad_out)
     if 0 in (m, k, f):  # sums over nothing
         return torch.zeros_like(x), torch.zeros_like(w_gate), torch.zeros_like(w_up)
-    grad_out, x, w_gate, w_up = (_dense(y) for y in (grad_out, x, w_gate, w_up))
+    grad_out, x, w_gate, w_up = _dense(grad_out), _dense(x), _dense(w_gate), _dense(w_up)
     lib = _rl.lib()
-    with torch.cuda.device(dev):
-        dx, dwg, dwu = torch.empty_like(x), torch.empty_like(w_gate), torch.empty_like(w_up)
-        nbytes = lib.gated_ffn_scratch_bytes(code, m, k, f, 1)
-        tmp = _rl.scratch(nbytes, dev)
-        _rl.check(lib.gated_ffn_backward(code, ACTIVATIONS[activation], m, k, f, grad_out.data_ptr(), x.data_ptr(),
-                                         w_gate.data_ptr(), w_up.data_ptr(), dx.data_ptr(), dwg.data_ptr(),
-                                         dwu.data_ptr(), _rl.ptr(tmp), nbytes, _rl.stream_ptr(dev)))
+    dx, dwg, dwu = torch.empty_like(x), torch.empty_like(w_gate), torch.empty_like(w_up)
+    nbytes = lib.gated_ffn_scratch_bytes(code, m, k, f, 1)
+    tmp = _rl.scratch(nbytes, x)
+    _rl.launch(index, lib.gated_ffn_backward, code, ACTIVATIONS[activation], m, k, f, grad_out.data_ptr(), x.data_ptr(),
+               w_gate.data_ptr(), w_up.data_ptr(), dx.data_ptr(), dwg.data_ptr(), dwu.data_ptr(), _rl.ptr(tmp), nbytes)
     return dx, dwg, dwu
 
 

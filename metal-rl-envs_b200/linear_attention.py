@@ -20,6 +20,7 @@ where a negative decay is raised to a power.
 """
 
 import ctypes
+from functools import lru_cache
 
 import torch
 
@@ -31,97 +32,104 @@ WIDTHS = (16, 32, 64, 128)
 def _rows(x):
     """(x, its strides without the last) with rows dense and on 16-byte boundaries; anything else is
     copied. Axes of one element have stride 0."""
+    if x.is_contiguous() and x.data_ptr() % 16 == 0:
+        return x, x.stride()[:-1]
     size = x.element_size()
-    strides = [0 if n == 1 else s for s, n in zip(x.stride(), x.shape)]
+    strides = tuple(0 if n == 1 else s for s, n in zip(x.stride(), x.shape))
     if strides[-1] != 1 or x.data_ptr() % 16 or any(s * size % 16 or s < 0 for s in strides[:-1]):
-        x = x.contiguous() if not x.is_contiguous() else x.clone(memory_format=torch.contiguous_format)
-        strides = [0 if n == 1 else s for s, n in zip(x.stride(), x.shape)]
+        x = x.clone(memory_format=torch.contiguous_format)
+        strides = x.stride()
     return x, strides[:-1]
 
 
-def _check(lead, decay, state, resets, grad_state=None, **tokens):
+@lru_cache(maxsize=64)
+def _stride_array(*strides):
+    flat = [s for triple in strides for s in triple]
+    return (ctypes.c_int64 * len(flat))(*flat)
+
+
+def _check(lead, decay, state, resets, grad_state, **tokens):
     """The tokens' common shape, dtype and device, and the resets as bytes. lead: leading axes."""
-    names = list(tokens)
-    first = _rl.as_floats(names[0], tokens[names[0]], (None,) * (lead + 2))
-    for name in names[1:]:
-        _rl.as_floats(name, tokens[name], first.shape, first.dtype)
-    *_, n, h, d = first.shape
+    shape = dtype = None
+    for name, x in tokens.items():
+        if shape is None or x.shape != shape or x.dtype is not dtype or x.get_device() != index:
+            _rl.as_floats(name, x, shape, dtype)
+            if shape is not None:
+                raise ValueError(f"{name} must be on cuda:{index} as the other tensors; got {x.device}")
+            shape, dtype, index = x.shape, x.dtype, x.get_device()
+    if len(shape) != lead + 2:
+        raise ValueError(f"{', '.join(tokens)} must have {lead + 2} axes; got shape {tuple(shape)}")
+    n, h, d = shape[-3:]
     if d not in WIDTHS:
         raise ValueError(f"the heads' width must be one of {WIDTHS}; got {d}")
     _rl.as_floats("decay", decay, (h,), torch.float32)
-    for name, s in (("state", state), ("grad_state", grad_state)):
-        if s is not None:
-            _rl.as_floats(name, s, (n, h, d, d), torch.float32)
+    if state is not None:
+        _rl.as_floats("state", state, (n, h, d, d), torch.float32)
+    if grad_state is not None:
+        _rl.as_floats("grad_state", grad_state, (n, h, d, d), torch.float32)
     if resets is not None:
         if not isinstance(resets, torch.Tensor) or resets.dtype not in (torch.bool, torch.uint8) \
-                or resets.shape != first.shape[:-2]:
-            raise ValueError(f"resets must be a bool or uint8 tensor of shape {tuple(first.shape[:-2])}")
+                or resets.shape != shape[:-2]:
+            raise ValueError(f"resets must be a bool or uint8 tensor of shape {tuple(shape[:-2])}")
         resets = resets.contiguous()
-    dev = _rl.same_device(decay=decay, state=state, resets=resets, grad_state=grad_state, **tokens)
-    return first.shape, first.dtype, dev, resets
+    _rl.one_device(index, decay=decay, state=state, resets=resets, grad_state=grad_state)
+    return shape, dtype, index, resets
 
 
 def _scale(scale, d):
     return d ** -0.5 if scale is None else float(scale)
 
 
-def _strides(rows):
-    flat = [s for _, strides in rows for s in strides]
-    return (ctypes.c_int64 * len(flat))(*flat)
-
-
 def forward(q, k, v, decay, state=None, resets=None, scale=None):
     """(out (T, N, H, D), state after the last token (N, H, D, D)). state None starts from zero; the
     given one is not changed. scale None is D ** -0.5."""
-    (t, n, h, d), dtype, dev, resets = _check(1 + 1, decay, state, resets, q=q, k=k, v=v)
-    rows = [_rows(x) for x in (q, k, v)]
+    shape, dtype, index, resets = _check(2, decay, state, resets, None, q=q, k=k, v=v)
+    t, n, h, d = shape
+    (q, qs), (k, ks), (v, vs) = _rows(q), _rows(k), _rows(v)
     decay, state = decay.contiguous(), None if state is None else state.contiguous()
     lib, code = _rl.lib(), _rl.FLOAT_DTYPES[dtype]
-    with torch.cuda.device(dev):
-        out = torch.empty((t, n, h, d), dtype=dtype, device=dev)
-        new = torch.empty((n, h, d, d), dtype=torch.float32, device=dev)
-        nbytes = lib.linear_attention_scratch_bytes(code, d, t, n, h, 0)
-        tmp = _rl.scratch(nbytes, dev)
-        _rl.check(lib.linear_attention_forward(
-            code, d, t, n, h, *(x.data_ptr() for x, _ in rows), _strides(rows), decay.data_ptr(), _rl.ptr(resets),
-            _scale(scale, d), _rl.ptr(state), out.data_ptr(), new.data_ptr(), _rl.ptr(tmp), nbytes,
-            _rl.stream_ptr(dev)))
+    out = q.new_empty(shape)
+    new = q.new_empty((n, h, d, d), dtype=torch.float32)
+    nbytes = lib.linear_attention_scratch_bytes(code, d, t, n, h, 0)
+    tmp = _rl.scratch(nbytes, q)
+    _rl.launch(index, lib.linear_attention_forward, code, d, t, n, h, q.data_ptr(), k.data_ptr(), v.data_ptr(),
+               _stride_array(qs, ks, vs), decay.data_ptr(), _rl.ptr(resets), _scale(scale, d), _rl.ptr(state),
+               out.data_ptr(), new.data_ptr(), _rl.ptr(tmp), nbytes)
     return out, new
 
 
 def backward(grad_out, q, k, v, decay, state=None, resets=None, scale=None, grad_state=None):
     """Gradients (dq, dk, dv (T, N, H, D), dstate (N, H, D, D)) of `forward` from grad_out and, where the
     final state is used further, grad_state."""
-    (t, n, h, d), dtype, dev, resets = _check(1 + 1, decay, state, resets, grad_state, grad_out=grad_out, q=q, k=k, v=v)
-    rows = [_rows(x) for x in (grad_out, q, k, v)]
+    shape, dtype, index, resets = _check(2, decay, state, resets, grad_state, grad_out=grad_out, q=q, k=k, v=v)
+    t, n, h, d = shape
+    (g, gs), (q, qs), (k, ks), (v, vs) = _rows(grad_out), _rows(q), _rows(k), _rows(v)
     decay = decay.contiguous()
     state, grad_state = (None if s is None else s.contiguous() for s in (state, grad_state))
     lib, code = _rl.lib(), _rl.FLOAT_DTYPES[dtype]
-    with torch.cuda.device(dev):
-        dq, dk, dv = (torch.empty((t, n, h, d), dtype=dtype, device=dev) for _ in range(3))
-        dstate = torch.empty((n, h, d, d), dtype=torch.float32, device=dev)
-        nbytes = lib.linear_attention_scratch_bytes(code, d, t, n, h, 1)
-        tmp = _rl.scratch(nbytes, dev)
-        _rl.check(lib.linear_attention_backward(
-            code, d, t, n, h, *(x.data_ptr() for x, _ in rows), _strides(rows), decay.data_ptr(), _rl.ptr(resets),
-            _scale(scale, d), _rl.ptr(state), _rl.ptr(grad_state), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(),
-            dstate.data_ptr(), _rl.ptr(tmp), nbytes, _rl.stream_ptr(dev)))
+    dq, dk, dv = q.new_empty(shape), q.new_empty(shape), q.new_empty(shape)
+    dstate = q.new_empty((n, h, d, d), dtype=torch.float32)
+    nbytes = lib.linear_attention_scratch_bytes(code, d, t, n, h, 1)
+    tmp = _rl.scratch(nbytes, q)
+    _rl.launch(index, lib.linear_attention_backward, code, d, t, n, h, g.data_ptr(), q.data_ptr(), k.data_ptr(),
+               v.data_ptr(), _stride_array(gs, qs, ks, vs), decay.data_ptr(), _rl.ptr(resets), _scale(scale, d),
+               _rl.ptr(state), _rl.ptr(grad_state), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), dstate.data_ptr(),
+               _rl.ptr(tmp), nbytes)
     return dq, dk, dv, dstate
 
 
 def step(q, k, v, decay, state, resets=None, scale=None):
     """One token for every environment, q, k, v (N, H, D), resets (N,): updates `state` (N, H, D, D) in
     place and returns out (N, H, D)."""
-    (n, h, d), dtype, dev, resets = _check(1, decay, state, resets, q=q, k=k, v=v)
+    shape, dtype, index, resets = _check(1, decay, state, resets, None, q=q, k=k, v=v)
     if state is None or not state.is_contiguous() or state.data_ptr() % 16:
         raise ValueError("state must be contiguous and on a 16-byte boundary: it is updated in place")
-    rows = [_rows(x) for x in (q, k, v)]
-    decay = decay.contiguous()
-    with torch.cuda.device(dev):
-        out = torch.empty((n, h, d), dtype=dtype, device=dev)
-        _rl.check(_rl.lib().linear_attention_step(
-            _rl.FLOAT_DTYPES[dtype], d, n, h, *(x.data_ptr() for x, _ in rows), _strides(rows), decay.data_ptr(),
-            _rl.ptr(resets), _scale(scale, d), state.data_ptr(), out.data_ptr(), _rl.stream_ptr(dev)))
+    n, h, d = shape
+    (q, qs), (k, ks), (v, vs) = _rows(q), _rows(k), _rows(v)
+    out = q.new_empty(shape)
+    _rl.launch(index, _rl.lib().linear_attention_step, _rl.FLOAT_DTYPES[dtype], d, n, h, q.data_ptr(), k.data_ptr(),
+               v.data_ptr(), _stride_array(qs, ks, vs), decay.contiguous().data_ptr(), _rl.ptr(resets),
+               _scale(scale, d), state.data_ptr(), out.data_ptr())
     return out
 
 

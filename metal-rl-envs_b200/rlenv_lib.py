@@ -411,32 +411,49 @@ def as_theta(theta, p, d, dev):
 
 
 # ---- operators of a memory policy --------------------------------------------------------------
+#
+# These calls sit between a program's other GPU work, some of them once per environment step, so the host
+# side is kept to a few microseconds: no copies unless rows need them, checks that compare whole shapes.
 
 
 def as_floats(name, x, shape=None, dtype=None):
-    """x checked as a CUDA tensor of the operators' types (float32, bfloat16), of `shape` (None
-    entries are free) and `dtype` where given. Nothing is copied: these calls sit between a
-    program's other GPU work, and there is no CPU path."""
-    if not isinstance(x, torch.Tensor) or x.device.type != "cuda":
+    """x checked as a CUDA tensor of the operators' types (float32, bfloat16), of `shape` and `dtype`
+    where given. There is no CPU path."""
+    if not isinstance(x, torch.Tensor) or not x.is_cuda:
         raise ValueError(f"{name} must be a CUDA tensor: there is no CPU path")
-    if x.dtype not in FLOAT_DTYPES or (dtype is not None and x.dtype != dtype):
+    if x.dtype not in FLOAT_DTYPES or (dtype is not None and x.dtype is not dtype):
         raise ValueError(f"{name} must be {dtype or 'float32 or bfloat16'}; got {x.dtype}")
-    if shape is not None and (x.dim() != len(shape) or any(w is not None and w != g for w, g in zip(shape, x.shape))):
-        raise ValueError(f"{name} must have shape {tuple('*' if w is None else w for w in shape)}; got {tuple(x.shape)}")
+    if shape is not None and x.shape != shape:
+        raise ValueError(f"{name} must have shape {tuple(shape)}; got {tuple(x.shape)}")
     return x
 
 
-def same_device(**tensors):
-    """The one device of the tensors given (None entries aside); anything else raises."""
-    devs = {x.device for x in tensors.values() if x is not None}
-    if len(devs) != 1:
-        raise ValueError(f"{', '.join(tensors)} must be on one device; got {sorted(map(str, devs))}")
-    return devs.pop()
+def one_device(index, **tensors):
+    """Raises unless every tensor given (None aside) is on CUDA device `index`."""
+    for name, x in tensors.items():
+        if x is not None and x.get_device() != index:
+            raise ValueError(f"{name} must be on cuda:{index} as the other tensors; got {x.device}")
 
 
-def scratch(nbytes, dev):
-    """Working memory for one call, from torch's caching allocator: it belongs to the current
-    stream, which the call's kernels run on."""
+# the current stream's handle without a Stream object around it, where this torch has the call
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or \
+    (lambda index: torch.cuda.current_stream(index).cuda_stream)
+
+
+def launch(index, entry, *args):
+    """entry(*args, stream) on CUDA device `index` and torch's current stream there; the status raises."""
+    if torch.cuda.current_device() == index:
+        rc = entry(*args, _raw_stream(index))
+    else:
+        with torch.cuda.device(index):
+            rc = entry(*args, _raw_stream(index))
+    if rc:
+        check(rc)
+
+
+def scratch(nbytes, like):
+    """Working memory for one call, from torch's caching allocator: it belongs to the current stream of
+    `like`'s device, which the call's kernels run on."""
     if nbytes < 0:
         check(-1)
-    return torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
+    return like.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
