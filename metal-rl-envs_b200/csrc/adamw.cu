@@ -30,7 +30,9 @@ namespace {
 
 constexpr int kStateBlock = 256;
 constexpr int kAdamThreads = 256;
-constexpr int kAdamTensors = 96;  // tensors per launch: their table travels in the launch's parameters
+constexpr int kAdamTensors = 96;    // tensors per launch: their table travels in the launch's parameters
+
+constexpr int kAdamPerSm = 3, kSms = 148;  // blocks of threads
 
 struct AdamTensor {
   float* p;
@@ -54,34 +56,67 @@ struct AdamArgs {
   AdamTensor t[kAdamTensors];
 };
 
-RLENV_D float load_grad(const float* g, int64_t i) { return __ldg(g + i); }
-RLENV_D float load_grad(const __nv_bfloat16* g, int64_t i) { return __bfloat162float(g[i]); }
-RLENV_D void load_grad4(const float* g, int64_t i, float o[4]) {
-  const float4 x = __ldg(reinterpret_cast<const float4*>(g + i));
-  o[0] = x.x, o[1] = x.y, o[2] = x.z, o[3] = x.w;
-}
-RLENV_D void load_grad4(const __nv_bfloat16* g, int64_t i, float o[4]) {
-  const uint2 x = __ldg(reinterpret_cast<const uint2*>(g + i));
-  o[0] = __uint_as_float(x.x << 16), o[1] = __uint_as_float(x.x & 0xffff0000u);
-  o[2] = __uint_as_float(x.y << 16), o[3] = __uint_as_float(x.y & 0xffff0000u);
-}
+// Four gradients as they are stored.
+template <typename G>
+struct FourGrads;
+template <>
+struct FourGrads<float> {
+  float4 raw;
+  RLENV_D void load(const float* g, int64_t i) { raw = __ldg(reinterpret_cast<const float4*>(g + i)); }
+  RLENV_D void load(const float* g, int64_t i, int64_t n) {
+    raw = make_float4(i < n ? g[i] : 0.0f, i + 1 < n ? g[i + 1] : 0.0f, i + 2 < n ? g[i + 2] : 0.0f,
+                      i + 3 < n ? g[i + 3] : 0.0f);
+  }
+  RLENV_D float4 values() const { return raw; }
+};
+template <>
+struct FourGrads<__nv_bfloat16> {
+  uint2 raw;
+  RLENV_D void load(const __nv_bfloat16* g, int64_t i) { raw = __ldg(reinterpret_cast<const uint2*>(g + i)); }
+  RLENV_D void load(const __nv_bfloat16* from, int64_t i, int64_t n) {
+    const unsigned short* g = reinterpret_cast<const unsigned short*>(from);
+    raw = make_uint2((i < n ? g[i] : 0u) | (i + 1 < n ? uint32_t(g[i + 1]) << 16 : 0u),
+                     (i + 2 < n ? g[i + 2] : 0u) | (i + 3 < n ? uint32_t(g[i + 3]) << 16 : 0u));
+  }
+  RLENV_D float4 values() const {
+    return make_float4(__uint_as_float(raw.x << 16), __uint_as_float(raw.x & 0xffff0000u),
+                       __uint_as_float(raw.y << 16), __uint_as_float(raw.y & 0xffff0000u));
+  }
+};
 
-RLENV_D float sqrt_approx(float x) {  // within an ulp; only the update passes through it
+// The update's root and quotient from the special function unit, within 2 ulp; no moment passes through
+// them. Values below 2^-126 count as zero.
+RLENV_D float sqrt_approx(float x) {
   float r;
-  asm("sqrt.approx.f32 %0, %1;" : "=f"(r) : "f"(x));
+  asm("sqrt.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+RLENV_D float quotient_approx(float x, float y) {
+  float r;
+  asm("div.approx.ftz.f32 %0, %1, %2;" : "=f"(r) : "f"(x), "f"(y));
   return r;
 }
 
-constexpr uint32_t kInfBits = 0x7f800000u;
+constexpr uint32_t kInfBits = 0x7f800000u, kNanBits = 0x7fffffffu, kCodeBit = 1u << 20;
 
-// E exponent bits: see the top of the file.
+// E exponent bits (see the top of the file): a code's value is the float whose bits are its magnitude << 20
+// plus base<E>(e), so that both ways are an addition.
 template <int E>
-RLENV_D float decode(uint32_t c, uint32_t e) {
+RLENV_D uint32_t base(uint32_t e) { return (8u * (e - ((1u << E) - 1u))) << 20; }
+
+template <int E, bool kTops>
+RLENV_D float decode(uint32_t c, uint32_t from) {
   constexpr uint32_t kTop = (1u << (E + 3)) - 1;
   const uint32_t mag = c & kTop;
-  const uint32_t bits = (mag + 8u * (e - ((1u << E) - 1u))) << 20;
-  float x = mag == 0 ? 0.0f : mag == kTop ? __uint_as_float(0x7fffffffu) : __uint_as_float(bits);
-  return E == 4 && (c & 128u) ? -x : x;
+  uint32_t bits = mag == 0 ? 0u : (mag << 20) + from;
+  if (kTops && mag == kTop) bits = kNanBits;
+  return __uint_as_float(E == 4 ? bits | (c & 128u) << 24 : bits);
+}
+// Whether any of four codes is the largest, NaN's.
+template <int E>
+RLENV_D uint32_t any_top(uint32_t c) {
+  const uint32_t sevens = (c & 0x7f7f7f7fu) + 0x01010101u;  // the high bit of a byte whose low seven are ones
+  return (E == 4 ? sevens : c & sevens) & 0x80808080u;
 }
 
 // The block's shared exponent from the bits of its largest finite magnitude.
@@ -90,123 +125,191 @@ RLENV_D uint32_t block_exponent(uint32_t bits) {
   return e < 32u ? 32u : e;
 }
 
-template <int E>
-RLENV_D uint32_t encode(float x, uint32_t e, uint32_t rand16) {
-  constexpr int kTop = (1 << (E + 3)) - 1;
+// The code in the top byte. rand4: the random bits at 4..19. kSpecial: x may be infinite or NaN.
+template <int E, bool kSpecial>
+RLENV_D uint32_t encode_high(float x, uint32_t from, uint32_t rand4) {
+  constexpr uint32_t kTop = (1u << (E + 3)) - 1;
   const uint32_t bits = __float_as_uint(x) & 0x7fffffffu;
-  int c = int((bits + (rand16 << 4)) >> 20) - 8 * (int(e) - ((1 << E) - 1));
-  c = max(c, E == 5 && bits > 0 ? 1 : 0);
-  if (bits >= kInfBits) c = kTop;
-  return uint32_t(c) | (E == 4 ? (__float_as_uint(x) >> 31) << 7 : 0u);
+  // negative where x is below the block's range; v > 0 has at least code 1
+  int place = max(int(bits + rand4 - from), E == 5 && bits > 0 ? int(kCodeBit) : 0);
+  if (kSpecial && bits >= kInfBits) place = int(kTop << 20);
+  return (uint32_t(place) << 4 & (E == 4 ? 0x7f000000u : 0xff000000u)) | (E == 4 ? __float_as_uint(x) & 0x80000000u : 0u);
+}
+RLENV_D uint32_t top_bytes(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+  return __byte_perm(__byte_perm(a, b, 0x0073), __byte_perm(c, d, 0x0073), 0x5410);
 }
 
-// A warp owns a state block: lane l elements 4 l .. 4 l + 3 and 128 + 4 l .. + 3.
-template <typename G, bool kEight>
-__global__ void __launch_bounds__(kAdamThreads) adamw_kernel(const __grid_constant__ AdamArgs a) {
-  const uint32_t local = blockIdx.x * (kAdamThreads / 32) + (threadIdx.x >> 5);
-  if (local >= a.blocks) return;
-  const uint32_t block = a.t[0].first + local;
-  const int lane = threadIdx.x & 31;
-  int lo = 0, hi = a.count - 1;  // the last tensor that starts at or before the block
-  while (lo < hi) {
-    const int mid = (lo + hi + 1) >> 1;
-    if (a.t[mid].first <= block) lo = mid; else hi = mid - 1;
+template <bool kSpecial>
+RLENV_D void encode_four(const float* m, const float* v, uint32_t place, uint32_t from_m, uint32_t from_v,
+                         uint32_t* cm, uint32_t* cv) {
+  uint32_t a[4], b[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const uint32_t r = pcg_hash(place ^ j);
+    a[j] = encode_high<4, kSpecial>(m[j], from_m, r << 4 & 0xffff0u);
+    b[j] = encode_high<5, kSpecial>(v[j], from_v, r >> 12 & 0xffff0u);
   }
-  const AdamTensor t = a.t[lo];
-  const G* grad = static_cast<const G*>(t.g);
-  const int64_t base = int64_t(block - t.first) * kStateBlock;  // in the tensor
-  const int64_t flat = int64_t(block) * kStateBlock;            // in the moments
-  const float gs = a.grad_scale ? __ldg(a.grad_scale) : 1.0f;
+  *cm = top_bytes(a[0], a[1], a[2], a[3]);
+  *cv = top_bytes(b[0], b[1], b[2], b[3]);
+}
 
-  float p[8], g[8], m[8], v[8];
-  uint32_t em = 0, ev = 0;
-  if constexpr (kEight) em = a.m_exp[block], ev = a.v_exp[block];
+// What a lane reads of a state block: elements 4 l .. 4 l + 3 and 128 + 4 l .. + 3.
+template <typename G, bool kEight>
+struct Elements {
+  float4 p[2], m[kEight ? 1 : 2], v[kEight ? 1 : 2];
+  FourGrads<G> g[2];
+  uint32_t cm[2], cv[2], em, ev;
+
+  RLENV_D void load(const AdamArgs& a, const AdamTensor& t, uint32_t block, int lane) {
+    const int64_t in = int64_t(block - t.first) * kStateBlock + 4 * lane;  // in the tensor
+    const int64_t flat = int64_t(block) * kStateBlock + 4 * lane;          // in the moments
+    const G* grad = static_cast<const G*>(t.g);
+    if constexpr (kEight) em = a.m_exp[block], ev = a.v_exp[block];
 #pragma unroll
-  for (int u = 0; u < 2; ++u) {
-    const int64_t i = base + 128 * u + 4 * lane;
-    if (t.wide && i + 4 <= t.n) {
-      const float4 x = *reinterpret_cast<const float4*>(t.p + i);
-      p[4 * u] = x.x, p[4 * u + 1] = x.y, p[4 * u + 2] = x.z, p[4 * u + 3] = x.w;
-      load_grad4(grad, i, g + 4 * u);
-    } else {
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const bool in = i + j < t.n;
-        p[4 * u + j] = in ? t.p[i + j] : 0.0f;
-        g[4 * u + j] = in ? load_grad(grad, i + j) : 0.0f;
+    for (int u = 0; u < 2; ++u) {
+      const int64_t i = in + 128 * u, f = flat + 128 * u;
+      if constexpr (kEight) {
+        cm[u] = *reinterpret_cast<const uint32_t*>(static_cast<const uint8_t*>(a.m) + f);
+        cv[u] = *reinterpret_cast<const uint32_t*>(static_cast<const uint8_t*>(a.v) + f);
+      } else {
+        m[u] = *reinterpret_cast<const float4*>(static_cast<const float*>(a.m) + f);
+        v[u] = *reinterpret_cast<const float4*>(static_cast<const float*>(a.v) + f);
+      }
+      if (t.wide && i + 4 <= t.n) {
+        p[u] = *reinterpret_cast<const float4*>(t.p + i);
+        g[u].load(grad, i);
+      } else {
+        p[u] = make_float4(i < t.n ? t.p[i] : 0.0f, i + 1 < t.n ? t.p[i + 1] : 0.0f, i + 2 < t.n ? t.p[i + 2] : 0.0f,
+                           i + 3 < t.n ? t.p[i + 3] : 0.0f);
+        g[u].load(grad, i, t.n);
       }
     }
-    const int64_t f = flat + 128 * u + 4 * lane;
+  }
+};
+
+RLENV_D void unpack(const float4& x, float* to) { to[0] = x.x, to[1] = x.y, to[2] = x.z, to[3] = x.w; }
+
+// A warp takes every stride-th state block and reads one ahead: a block's arithmetic, some 80 instructions an
+// element with 8-bit moments, runs under the next one's loads.
+template <typename G, bool kEight>
+__global__ void __launch_bounds__(kAdamThreads, kAdamPerSm) adamw_kernel(const __grid_constant__ AdamArgs a) {
+  const int lane = threadIdx.x & 31;
+  const uint32_t stride = gridDim.x * (kAdamThreads / 32), end = a.t[0].first + a.blocks;
+  uint32_t block = a.t[0].first + blockIdx.x * (kAdamThreads / 32) + (threadIdx.x >> 5);
+  if (block >= end) return;
+  int at = 0, hi = a.count - 1;  // the last tensor that starts at or before the block
+  while (at < hi) {
+    const int mid = (at + hi + 1) >> 1;
+    if (a.t[mid].first <= block) at = mid; else hi = mid - 1;
+  }
+  const float gs = a.grad_scale ? __ldg(a.grad_scale) : 1.0f;
+  Elements<G, kEight> ahead;
+  ahead.load(a, a.t[at], block, lane);
+  while (true) {
+    const Elements<G, kEight> x = ahead;
+    const AdamTensor& t = a.t[at];
+    const uint32_t next = block + stride;
+    int next_at = at;
+    if (next < end) {
+      while (next_at + 1 < a.count && a.t[next_at + 1].first <= next) ++next_at;
+      ahead.load(a, a.t[next_at], next, lane);
+    }
+    const int64_t in = int64_t(block - t.first) * kStateBlock + 4 * lane, flat = int64_t(block) * kStateBlock + 4 * lane;
+    float p[8], g[8], m[8], v[8];
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      unpack(x.p[u], p + 4 * u);
+      unpack(x.g[u].values(), g + 4 * u);
+      if constexpr (!kEight) unpack(x.m[u], m + 4 * u), unpack(x.v[u], v + 4 * u);
+    }
     if constexpr (kEight) {
-      const uint32_t cm = *reinterpret_cast<const uint32_t*>(static_cast<const uint8_t*>(a.m) + f);
-      const uint32_t cv = *reinterpret_cast<const uint32_t*>(static_cast<const uint8_t*>(a.v) + f);
+      const uint32_t from_m = base<4>(x.em), from_v = base<5>(x.ev);
+      const uint32_t tops = any_top<4>(x.cm[0]) | any_top<4>(x.cm[1]) | any_top<5>(x.cv[0]) | any_top<5>(x.cv[1]);
+      if (__any_sync(0xffffffffu, tops != 0)) {
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        m[4 * u + j] = decode<4>((cm >> (8 * j)) & 255u, em);
-        v[4 * u + j] = decode<5>((cv >> (8 * j)) & 255u, ev);
-      }
-    } else {
-      const float4 x = *reinterpret_cast<const float4*>(static_cast<const float*>(a.m) + f);
-      const float4 y = *reinterpret_cast<const float4*>(static_cast<const float*>(a.v) + f);
-      m[4 * u] = x.x, m[4 * u + 1] = x.y, m[4 * u + 2] = x.z, m[4 * u + 3] = x.w;
-      v[4 * u] = y.x, v[4 * u + 1] = y.y, v[4 * u + 2] = y.z, v[4 * u + 3] = y.w;
-    }
-  }
-  uint32_t top_m = 0, top_v = 0;
-#pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    const float x = __fmul_rn(g[j], gs);
-    m[j] = __fadd_rn(__fmul_rn(m[j], a.b1), __fmul_rn(x, a.c1));
-    v[j] = __fadd_rn(__fmul_rn(v[j], a.b2), __fmul_rn(__fmul_rn(x, x), a.c2));
-    const float denom = sqrt_approx(v[j]) * a.root + a.eps;
-    p[j] = __fsub_rn(__fmul_rn(p[j], a.keep), __fdividef(m[j] * a.rate, denom));
-    if constexpr (kEight) {
-      const uint32_t bm = __float_as_uint(m[j]) & 0x7fffffffu, bv = __float_as_uint(v[j]);
-      if (bm < kInfBits) top_m = max(top_m, bm);
-      if (bv < kInfBits) top_v = max(top_v, bv);
-    }
-  }
-  if constexpr (kEight) {
-    em = block_exponent(__reduce_max_sync(0xffffffffu, top_m));
-    ev = block_exponent(__reduce_max_sync(0xffffffffu, top_v));
-    if (lane == 0) a.m_exp[block] = uint8_t(em), a.v_exp[block] = uint8_t(ev);
-  }
-#pragma unroll
-  for (int u = 0; u < 2; ++u) {
-    const int64_t i = base + 128 * u + 4 * lane;
-    if (t.wide && i + 4 <= t.n) {
-      *reinterpret_cast<float4*>(t.p + i) = make_float4(p[4 * u], p[4 * u + 1], p[4 * u + 2], p[4 * u + 3]);
-      if (t.copy) {
-        const __nv_bfloat162 lo2 = __floats2bfloat162_rn(p[4 * u], p[4 * u + 1]);
-        const __nv_bfloat162 hi2 = __floats2bfloat162_rn(p[4 * u + 2], p[4 * u + 3]);
-        *reinterpret_cast<uint2*>(t.copy + i) =
-            make_uint2(*reinterpret_cast<const uint32_t*>(&lo2), *reinterpret_cast<const uint32_t*>(&hi2));
-      }
-    } else {
-#pragma unroll
-      for (int j = 0; j < 4; ++j)
-        if (i + j < t.n) {
-          t.p[i + j] = p[4 * u + j];
-          if (t.copy) t.copy[i + j] = __float2bfloat16_rn(p[4 * u + j]);
+        for (int j = 0; j < 8; ++j) {
+          m[j] = decode<4, true>(x.cm[j / 4] >> (8 * (j % 4)) & 255u, from_m);
+          v[j] = decode<5, true>(x.cv[j / 4] >> (8 * (j % 4)) & 255u, from_v);
         }
-    }
-    const int64_t f = flat + 128 * u + 4 * lane;
-    if constexpr (kEight) {
-      uint32_t cm = 0, cv = 0;
+      } else {
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const uint32_t r = pcg_hash(uint32_t(f + j) ^ a.key);
-        cm |= encode<4>(m[4 * u + j], em, r & 0xffffu) << (8 * j);
-        cv |= encode<5>(v[4 * u + j], ev, r >> 16) << (8 * j);
+        for (int j = 0; j < 8; ++j) {
+          m[j] = decode<4, false>(x.cm[j / 4] >> (8 * (j % 4)) & 255u, from_m);
+          v[j] = decode<5, false>(x.cv[j / 4] >> (8 * (j % 4)) & 255u, from_v);
+        }
       }
-      *reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(a.m) + f) = cm;
-      *reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(a.v) + f) = cv;
-    } else {
-      *reinterpret_cast<float4*>(static_cast<float*>(a.m) + f) =
-          make_float4(m[4 * u], m[4 * u + 1], m[4 * u + 2], m[4 * u + 3]);
-      *reinterpret_cast<float4*>(static_cast<float*>(a.v) + f) =
-          make_float4(v[4 * u], v[4 * u + 1], v[4 * u + 2], v[4 * u + 3]);
     }
+    uint32_t top_m = 0, top_v = 0;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const float y = __fmul_rn(g[j], gs);
+      m[j] = __fadd_rn(__fmul_rn(m[j], a.b1), __fmul_rn(y, a.c1));
+      v[j] = __fadd_rn(__fmul_rn(v[j], a.b2), __fmul_rn(__fmul_rn(y, y), a.c2));
+      const float denom = fmaf(sqrt_approx(v[j]), a.root, a.eps);
+      p[j] = __fsub_rn(__fmul_rn(p[j], a.keep), quotient_approx(m[j] * a.rate, denom));
+      if constexpr (kEight) {
+        top_m = max(top_m, __float_as_uint(m[j]) & 0x7fffffffu);
+        top_v = max(top_v, __float_as_uint(v[j]) & 0x7fffffffu);
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      const int64_t i = in + 128 * u;
+      if (t.wide && i + 4 <= t.n) {
+        *reinterpret_cast<float4*>(t.p + i) = make_float4(p[4 * u], p[4 * u + 1], p[4 * u + 2], p[4 * u + 3]);
+        if (t.copy) {
+          const __nv_bfloat162 lo2 = __floats2bfloat162_rn(p[4 * u], p[4 * u + 1]);
+          const __nv_bfloat162 hi2 = __floats2bfloat162_rn(p[4 * u + 2], p[4 * u + 3]);
+          *reinterpret_cast<uint2*>(t.copy + i) =
+              make_uint2(*reinterpret_cast<const uint32_t*>(&lo2), *reinterpret_cast<const uint32_t*>(&hi2));
+        }
+      } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (i + j < t.n) {
+            t.p[i + j] = p[4 * u + j];
+            if (t.copy) t.copy[i + j] = __float2bfloat16_rn(p[4 * u + j]);
+          }
+      }
+    }
+    if constexpr (kEight) {
+      top_m = __reduce_max_sync(0xffffffffu, top_m);
+      top_v = __reduce_max_sync(0xffffffffu, top_v);
+      const bool special = max(top_m, top_v) >= kInfBits;
+      if (special) {  // the largest finite ones
+        top_m = top_v = 0;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const uint32_t bm = __float_as_uint(m[j]) & 0x7fffffffu, bv = __float_as_uint(v[j]) & 0x7fffffffu;
+          if (bm < kInfBits) top_m = max(top_m, bm);
+          if (bv < kInfBits) top_v = max(top_v, bv);
+        }
+        top_m = __reduce_max_sync(0xffffffffu, top_m);
+        top_v = __reduce_max_sync(0xffffffffu, top_v);
+      }
+      const uint32_t em = block_exponent(top_m), ev = block_exponent(top_v);
+      if (lane == 0) a.m_exp[block] = uint8_t(em), a.v_exp[block] = uint8_t(ev);
+      const uint32_t from_m = base<4>(em), from_v = base<5>(ev);
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const uint32_t place = uint32_t(flat + 128 * u) ^ a.key;  // a multiple of four before the key
+        uint32_t cm, cv;
+        if (special) encode_four<true>(m + 4 * u, v + 4 * u, place, from_m, from_v, &cm, &cv);
+        else encode_four<false>(m + 4 * u, v + 4 * u, place, from_m, from_v, &cm, &cv);
+        *reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(a.m) + flat + 128 * u) = cm;
+        *reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(a.v) + flat + 128 * u) = cv;
+      }
+    } else {
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        *reinterpret_cast<float4*>(static_cast<float*>(a.m) + flat + 128 * u) =
+            make_float4(m[4 * u], m[4 * u + 1], m[4 * u + 2], m[4 * u + 3]);
+        *reinterpret_cast<float4*>(static_cast<float*>(a.v) + flat + 128 * u) =
+            make_float4(v[4 * u], v[4 * u + 1], v[4 * u + 2], v[4 * u + 3]);
+      }
+    }
+    if (next >= end) return;
+    block = next, at = next_at;
   }
 }
 
@@ -218,18 +321,19 @@ moments_kernel(const uint32_t* __restrict__ m, const uint32_t* __restrict__ v, c
   const int64_t i = int64_t(blockIdx.x) * 256 + threadIdx.x;
   if (i >= quads) return;
   const uint32_t cm = __ldg(m + i), cv = __ldg(v + i);
-  const uint32_t em = __ldg(m_exp + i / (kStateBlock / 4)), ev = __ldg(v_exp + i / (kStateBlock / 4));
-  m_out[i] = make_float4(decode<4>(cm & 255u, em), decode<4>((cm >> 8) & 255u, em), decode<4>((cm >> 16) & 255u, em),
-                         decode<4>(cm >> 24, em));
-  v_out[i] = make_float4(decode<5>(cv & 255u, ev), decode<5>((cv >> 8) & 255u, ev), decode<5>((cv >> 16) & 255u, ev),
-                         decode<5>(cv >> 24, ev));
+  const uint32_t em = base<4>(__ldg(m_exp + i / (kStateBlock / 4))), ev = base<5>(__ldg(v_exp + i / (kStateBlock / 4)));
+  m_out[i] = make_float4(decode<4, true>(cm & 255u, em), decode<4, true>((cm >> 8) & 255u, em), decode<4, true>((cm >> 16) & 255u, em),
+                         decode<4, true>(cm >> 24, em));
+  v_out[i] = make_float4(decode<5, true>(cv & 255u, ev), decode<5, true>((cv >> 8) & 255u, ev), decode<5, true>((cv >> 16) & 255u, ev),
+                         decode<5, true>(cv >> 24, ev));
 }
 
 bool on_boundary(const void* p, int bytes) { return reinterpret_cast<uintptr_t>(p) % bytes == 0; }
 
 template <typename G, bool kEight>
 int adamw_launch(const AdamArgs& a, cudaStream_t stream) {
-  const unsigned grid = (a.blocks + kAdamThreads / 32 - 1) / (kAdamThreads / 32);
+  constexpr uint32_t kWarps = kAdamThreads / 32, kMost = kSms * kAdamPerSm;
+  const uint32_t grid = (a.blocks + kWarps - 1) / kWarps < kMost ? (a.blocks + kWarps - 1) / kWarps : kMost;
   adamw_kernel<G, kEight><<<grid, kAdamThreads, 0, stream>>>(a);
   return launch_status();
 }
