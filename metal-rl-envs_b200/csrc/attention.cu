@@ -45,11 +45,12 @@ chunk_kernel(const __grid_constant__ Problem p, const __grid_constant__ Split sp
   const bool whole = split.segments == 1;
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int rb = warp & 3, oc = (warp >> 2) * C::OC;  // this warp's 16 tokens and output columns
+  const int rb = warp % C::kRowWarps * C::RT;         // this warp's first 16 tokens,
+  const int oc = warp / C::kRowWarps * C::OC;         // and output columns
   const int gr = lane >> 2, gc = (lane & 3) * 2;      // a fragment's row and column
   const float log2_g = log2f(__ldg(p.decay + h));
   const int f = s.reverse ? 0 : 1;
-  if (threadIdx.x < kChunk) decays[threadIdx.x] = power(log2_g, kChunk - f - int(threadIdx.x));
+  for (int j = threadIdx.x; j < kChunk; j += C::kThreads) decays[j] = power(log2_g, kChunk - f - j);
   const float chunk_decay = power(log2_g, kChunk);
 
   // The carry, float32 in registers: rows srow + 16 m + (gr, gr + 8), columns scol + 8 t + (gc, gc + 1).
@@ -72,9 +73,9 @@ chunk_kernel(const __grid_constant__ Problem p, const __grid_constant__ Split sp
         z[m][t][q] = start && holds ? start_mul * __ldg(start + (turned ? c * D + r : r * D + c)) : 0.0f;
       }
 
-  // The weights, `scale` among them, between a warp's rows and 16 columns: on the diagonal, and one block
-  // to its left; and from the carry to its rows.
-  float near[8], next[8], row_decay[2];
+  // The weights, `scale` among them, between 16 tokens and 16 others: on the diagonal, and one block to its
+  // left; and from the carry to this warp's tokens.
+  float near[8], next[8], row_decay[C::RT][2];
   if constexpr (!kLocal) {
 #pragma unroll
     for (int q = 0; q < 8; ++q) {
@@ -82,8 +83,10 @@ chunk_kernel(const __grid_constant__ Problem p, const __grid_constant__ Split sp
       near[q] = apart >= 0 ? p.scale * power(log2_g, apart) : 0.0f;
       next[q] = p.scale * power(log2_g, 16 + apart);
     }
-    row_decay[0] = p.scale * power(log2_g, 16 * rb + gr + f);
-    row_decay[1] = p.scale * power(log2_g, 16 * rb + gr + 8 + f);
+#pragma unroll
+    for (int r = 0; r < C::RT; ++r)
+#pragma unroll
+      for (int half = 0; half < 2; ++half) row_decay[r][half] = p.scale * power(log2_g, 16 * (rb + r) + gr + 8 * half + f);
   }
   const float block_decay = power(log2_g, 16);
 
@@ -108,25 +111,41 @@ chunk_kernel(const __grid_constant__ Problem p, const __grid_constant__ Split sp
     load_x.advance(), load_a.advance(), load_b.advance();
   };
   // a lane's two resets of a chunk, as bytes
-  const auto reset_at = [&](int64_t i) -> int {
-    if (i >= last) return 0;
-    return __ldg(p.resets + (s.reverse ? p.t - 1 - i : i) * p.n + n);
-  };
+  const int64_t reset_step = s.reverse ? -p.n : p.n;
+  const uint8_t* reset_at = p.resets + (s.reverse ? p.t - 1 - (first + lane) : first + lane) * p.n + n;
   int reset0 = 0, reset1 = 0;
-  if (p.resets && first < last) reset0 = reset_at(first + lane), reset1 = reset_at(first + 32 + lane);
-  if (first < last) set_out(first, tiles);
+  const auto read_resets = [&](int64_t i) {
+    reset0 = i + lane < last ? __ldg(reset_at) : 0;
+    reset1 = i + 32 + lane < last ? __ldg(reset_at + 32 * reset_step) : 0;
+    reset_at += kChunk * reset_step;
+  };
+  // results leave as 16-byte pieces: lane l the piece l % kPieces of row l / kPieces of the warp's
+  constexpr int kPer = 16 / sizeof(T), kPieces = C::OC / kPer, kRowsOut = 32 / kPieces;
+  const int64_t token_step = p.n * p.h * D, out_step = s.reverse ? -token_step : token_step;
+  T* out_at;
+  {
+    const int64_t i = first + 16 * rb + lane / kPieces;
+    out_at = static_cast<T*>(s.out) + (s.reverse ? p.t - 1 - i : i) * token_step + seq * D + col + oc + lane % kPieces * kPer;
+  }
+  if (p.resets && first < last) read_resets(first);
+  constexpr bool kAhead = C::kFloat || C::kBuffers == 2;  // tiles set out a chunk ahead
+  if (kAhead && first < last) set_out(first, tiles);
 
   float bad = 0.0f;      // NaN once any value is not finite
   bool cut = false;      // a reset anywhere in the segment
   int buffer = 0;
   for (int64_t i0 = first; i0 < last; i0 += kChunk) {
     const int len = int(last - i0 < kChunk ? last - i0 : kChunk);
-    __nv_bfloat16* const X = tiles + (C::kFloat ? 0 : buffer * C::kTiles);
+    __nv_bfloat16* const X = tiles + buffer * C::kTiles;
     __nv_bfloat16* const A = X + kAAt;
     __nv_bfloat16* const B = X + kBAt;
-    buffer ^= 1;
-    const uint64_t resets = uint64_t(__ballot_sync(0xffffffffu, reset1 != 0)) << 32 | __ballot_sync(0xffffffffu, reset0 != 0);
-    cut = cut || resets != 0;
+    if (C::kBuffers == 2) buffer ^= 1;
+    if (!kAhead) set_out(i0, tiles);
+    uint64_t resets = 0;
+    if (p.resets) {
+      resets = uint64_t(__ballot_sync(0xffffffffu, reset1 != 0)) << 32 | __ballot_sync(0xffffffffu, reset0 != 0);
+      cut = cut || resets != 0;
+    }
     // The first position that position i (or, for i = 63, the chunk's end) is linked to; `none`: also the carry.
     const auto linked_from = [&](uint64_t before, bool* none) -> int {
       const uint64_t m = resets & before;
@@ -161,94 +180,158 @@ chunk_kernel(const __grid_constant__ Problem p, const __grid_constant__ Split sp
     __syncthreads();
     const int64_t next_chunk = i0 + kChunk;
     if (next_chunk < last) {
-      set_out(next_chunk, tiles + (C::kFloat ? 0 : buffer * C::kTiles));
-      if (p.resets) reset0 = reset_at(next_chunk + lane), reset1 = reset_at(next_chunk + 32 + lane);
+      if (kAhead) set_out(next_chunk, tiles + buffer * C::kTiles);
+      if (p.resets) read_resets(next_chunk);
     }
 
     if constexpr (!kLocal) {
-      float o[C::OC / 8][4];
+      float o[C::RT][C::OC / 8][4];
 #pragma unroll
-      for (int t = 0; t < C::OC / 8; ++t)
+      for (int r = 0; r < C::RT; ++r)
 #pragma unroll
-        for (int q = 0; q < 4; ++q) o[t][q] = 0.0f;
+        for (int t = 0; t < C::OC / 8; ++t)
+#pragma unroll
+          for (int q = 0; q < 4; ++q) o[r][t][q] = 0.0f;
       const uint32_t xa = shared_address(X + (16 * rb + (lane & 15)) * C::PX + (lane >> 4) * 8);
       const uint32_t sa = shared_address(S + (lane & 15) * C::PB + (lane >> 4) * 8 + oc);
+      constexpr int kGroup = C::OC >= 32 ? 2 : 1;  // pairs of tiles whose products run side by side
+      const auto load_x_tiles = [&](uint32_t (&x)[C::RT][C::kIn][4], int k) {
+#pragma unroll
+        for (int r = 0; r < C::RT; ++r)
+#pragma unroll
+          for (int q = 0; q < C::kIn; ++q) load_matrices(x[r][q], xa + 2 * (q * C::kX + 16 * r * C::PX + 16 * k));
+      };
       // x Z
 #pragma unroll
       for (int k = 0; k < D / 16; ++k) {
-        uint32_t x[C::kIn][4];
+        uint32_t x[C::RT][C::kIn][4];
+        load_x_tiles(x, k);
 #pragma unroll
-        for (int q = 0; q < C::kIn; ++q) load_matrices(x[q], xa + 2 * (q * C::kX + 16 * k));
+        for (int t = 0; t < C::OC / 16; t += kGroup) {
+          uint32_t v[kGroup][C::kMid][4];
 #pragma unroll
-        for (int t = 0; t < C::OC / 16; ++t) {
-          uint32_t v[C::kMid][4];
+          for (int i = 0; i < kGroup; ++i)
 #pragma unroll
-          for (int q = 0; q < C::kMid; ++q) load_matrices_turned(v[q], sa + 2 * (q * C::kS + 16 * k * C::PB + 16 * t));
-          multiply_planes<C::kIn, C::kMid, C::kFloat>(o[2 * t], o[2 * t + 1], x, v);
+            for (int q = 0; q < C::kMid; ++q)
+              load_matrices_turned(v[i][q], sa + 2 * (q * C::kS + 16 * k * C::PB + 16 * (t + i)));
+#pragma unroll
+          for (int r = 0; r < C::RT; ++r)
+            multiply_planes<C::kIn, C::kMid, kGroup, C::kFloat>(&o[r][2 * t], x[r], v);
         }
       }
-      const int row[2] = {16 * rb + gr, 16 * rb + gr + 8};
-      int from[2];
-      float keep[2];
+      int from[C::RT][2] = {};
 #pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        bool none;
-        from[half] = linked_from((uint64_t(f + 1) << row[half]) - 1, &none);
-        keep[half] = none ? row_decay[half] : 0.0f;
-      }
+      for (int r = 0; r < C::RT; ++r)
 #pragma unroll
-      for (int t = 0; t < C::OC / 8; ++t)
+        for (int half = 0; half < 2; ++half) {
+          bool carry = true;
+          if (resets) from[r][half] = linked_from((uint64_t(f + 1) << (16 * (rb + r) + gr + 8 * half)) - 1, &carry);
+          const float keep = row_decay[r][half];
 #pragma unroll
-        for (int q = 0; q < 4; ++q) o[t][q] *= keep[q >> 1];
+          for (int t = 0; t < C::OC / 8; ++t) {
+            o[r][t][2 * half] = carry ? keep * o[r][t][2 * half] : 0.0f;
+            o[r][t][2 * half + 1] = carry ? keep * o[r][t][2 * half + 1] : 0.0f;
+          }
+        }
       // (W * x a') b, 16 tokens at a time from the diagonal to the left
       const uint32_t aa = shared_address(A + ((lane & 7) + (lane >> 4) * 8) * C::PX + ((lane >> 3) & 1) * 8);
       const uint32_t ba = shared_address(B + (lane & 15) * C::PB + (lane >> 4) * 8 + oc);
-      float far = 1.0f;
-      for (int jb = rb; jb >= 0; --jb) {
-        float w[2][4] = {};
+      float far[C::RT];
+#pragma unroll
+      for (int r = 0; r < C::RT; ++r) far[r] = 1.0f;
+      for (int jb = rb + C::RT - 1; jb >= 0; --jb) {
+        float w[C::RT][2][4] = {}, w_odd[C::RT][2][4] = {};  // even and odd steps of the sum side by side
 #pragma unroll
         for (int k = 0; k < D / 16; ++k) {
-          uint32_t x[C::kIn][4], v[C::kIn][4];
+          uint32_t x[C::RT][C::kIn][4], v[1][C::kIn][4];
+          load_x_tiles(x, k);
 #pragma unroll
-          for (int q = 0; q < C::kIn; ++q) load_matrices(x[q], xa + 2 * (q * C::kX + 16 * k));
+          for (int q = 0; q < C::kIn; ++q) load_matrices(v[0][q], aa + 2 * (q * C::kX + 16 * jb * C::PX + 16 * k));
 #pragma unroll
-          for (int q = 0; q < C::kIn; ++q) load_matrices(v[q], aa + 2 * (q * C::kX + 16 * jb * C::PX + 16 * k));
-          multiply_planes<C::kIn, C::kIn, C::kFloat>(w[0], w[1], x, v);
+          for (int r = 0; r < C::RT; ++r)
+            if (C::RT == 1 || jb <= rb + r)
+              multiply_planes<C::kIn, C::kIn, 1, C::kFloat>(k & 1 ? w_odd[r] : w[r], x[r], v);
         }
-        const bool diagonal = jb == rb;
+        if (D > 16) {
 #pragma unroll
-        for (int q = 0; q < 8; ++q) {
-          const int j = 16 * jb + gc + (q & 1) + (q & 4) * 2;
-          const float weight = diagonal ? near[q] : next[q] * far;
-          w[q >> 2][q & 3] *= j >= from[(q >> 1) & 1] ? weight : 0.0f;
+          for (int r = 0; r < C::RT; ++r)
+#pragma unroll
+            for (int q = 0; q < 8; ++q) w[r][q >> 2][q & 3] += w_odd[r][q >> 2][q & 3];
         }
-        if (!diagonal) far *= block_decay;
-        uint32_t wp[C::kMid][4];
-        split_pair<C::kMid>(w[0][0], w[0][1], &wp[0][0], 4);
-        split_pair<C::kMid>(w[0][2], w[0][3], &wp[0][1], 4);
-        split_pair<C::kMid>(w[1][0], w[1][1], &wp[0][2], 4);
-        split_pair<C::kMid>(w[1][2], w[1][3], &wp[0][3], 4);
+        uint32_t wp[C::RT][C::kMid][4];
 #pragma unroll
-        for (int t = 0; t < C::OC / 16; ++t) {
-          uint32_t v[C::kIn][4];
+        for (int r = 0; r < C::RT; ++r) {
+          if (C::RT > 1 && jb > rb + r) continue;
+          const bool diagonal = jb == rb + r;
 #pragma unroll
-          for (int q = 0; q < C::kIn; ++q) load_matrices_turned(v[q], ba + 2 * (q * C::kB + 16 * jb * C::PB + 16 * t));
-          multiply_planes<C::kMid, C::kIn, C::kFloat>(o[2 * t], o[2 * t + 1], wp, v);
+          for (int q = 0; q < 8; ++q) {
+            const int j = 16 * jb + gc + (q & 1) + (q & 4) * 2;
+            const float weight = diagonal ? near[q] : next[q] * far[r];
+            w[r][q >> 2][q & 3] *= j >= from[r][(q >> 1) & 1] ? weight : 0.0f;
+          }
+          if (!diagonal) far[r] *= block_decay;
+          split_pair<C::kMid>(w[r][0][0], w[r][0][1], &wp[r][0][0], 4);
+          split_pair<C::kMid>(w[r][0][2], w[r][0][3], &wp[r][0][1], 4);
+          split_pair<C::kMid>(w[r][1][0], w[r][1][1], &wp[r][0][2], 4);
+          split_pair<C::kMid>(w[r][1][2], w[r][1][3], &wp[r][0][3], 4);
+        }
+#pragma unroll
+        for (int t = 0; t < C::OC / 16; t += kGroup) {
+          uint32_t v[kGroup][C::kIn][4];
+#pragma unroll
+          for (int i = 0; i < kGroup; ++i)
+#pragma unroll
+            for (int q = 0; q < C::kIn; ++q)
+              load_matrices_turned(v[i][q], ba + 2 * (q * C::kB + 16 * jb * C::PB + 16 * (t + i)));
+#pragma unroll
+          for (int r = 0; r < C::RT; ++r)
+            if (C::RT == 1 || jb <= rb + r)
+              multiply_planes<C::kMid, C::kIn, kGroup, C::kFloat>(&o[r][2 * t], wp[r], v);
         }
       }
 #pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        const int64_t i = i0 + row[half];
-        T* const at = static_cast<T*>(s.out) + (((s.reverse ? p.t - 1 - i : i) * p.n + n) * p.h + h) * D + col + oc + gc;
-        if (row[half] < len) {
+      for (int r = 0; r < C::RT; ++r)
 #pragma unroll
-          for (int t = 0; t < C::OC / 8; ++t) {
-            const float lo = o[t][2 * half], hi = o[t][2 * half + 1];
-            bad = fmaf(lo, 0.0f, bad), bad = fmaf(hi, 0.0f, bad);
-            if constexpr (sizeof(T) == 2)
-              *reinterpret_cast<uint32_t*>(at + 8 * t) = pack(lo, hi);
-            else
-              *reinterpret_cast<float2*>(at + 8 * t) = make_float2(lo, hi);
+        for (int t = 0; t < C::OC / 8; ++t)
+#pragma unroll
+          for (int q = 0; q < 4; ++q)
+            if (16 * (rb + r) + gr + (q & 2) * 4 < len) bad = fmaf(o[r][t][q], 0.0f, bad);
+      if constexpr (C::kColWarps == 1 && sizeof(T) == 2) {
+        // to global memory by whole rows, through this warp's rows of x, which nothing reads any more
+        __syncwarp();
+        __nv_bfloat16* const own = X + 16 * rb * C::PX;
+#pragma unroll
+        for (int r = 0; r < C::RT; ++r)
+#pragma unroll
+          for (int half = 0; half < 2; ++half)
+#pragma unroll
+            for (int t = 0; t < C::OC / 8; ++t)
+              *reinterpret_cast<uint32_t*>(own + (16 * r + gr + 8 * half) * C::PX + 8 * t + gc) =
+                  pack(o[r][t][2 * half], o[r][t][2 * half + 1]);
+        __syncwarp();
+#pragma unroll
+        for (int e = 0; e < 16 * C::RT / kRowsOut; ++e) {
+          const int r = lane / kPieces + e * kRowsOut;
+          if (16 * rb + r < len)
+            *reinterpret_cast<uint4*>(out_at + e * kRowsOut * out_step) =
+                *reinterpret_cast<const uint4*>(own + r * C::PX + lane % kPieces * kPer);
+        }
+        out_at += kChunk * out_step;
+      } else {
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          const int row = 16 * rb + gr + 8 * half;
+          const int64_t i = i0 + row;
+          T* const at = static_cast<T*>(s.out) + (s.reverse ? p.t - 1 - i : i) * token_step + seq * D + col + oc + gc;
+          if (row < len) {
+#pragma unroll
+            for (int t = 0; t < C::OC / 8; ++t) {
+              const float lo = o[0][t][2 * half], hi = o[0][t][2 * half + 1];
+              if constexpr (sizeof(T) == 2)
+                *reinterpret_cast<uint32_t*>(at + 8 * t) = pack(lo, hi);
+              else
+                *reinterpret_cast<float2*>(at + 8 * t) = make_float2(lo, hi);
+            }
           }
         }
       }
@@ -256,9 +339,9 @@ chunk_kernel(const __grid_constant__ Problem p, const __grid_constant__ Split sp
 
     // Z <- g^L Z + (l * A)' B, l_j = g^(L - f - j) where no reset lies between token j and the end
     if (holds) {
-      bool none;
-      const int reached = linked_from(~uint64_t(0), &none);
-      const float through = !none ? 0.0f : len == kChunk ? chunk_decay : power(log2_g, len);
+      bool none = true;
+      const int reached = resets ? linked_from(~uint64_t(0), &none) : 0;
+      const float through = len == kChunk ? chunk_decay : power(log2_g, len);
 #pragma unroll
       for (int m = 0; m < C::MT; ++m)
 #pragma unroll
@@ -289,14 +372,18 @@ chunk_kernel(const __grid_constant__ Problem p, const __grid_constant__ Split sp
 #pragma unroll
           for (int u = 0; u < 4; ++u) split_pair<C::kKeys>(l[u & 2] * lo[u], l[(u & 2) + 1] * hi[u], &key[m][0][u], 4);
         }
+        constexpr int kGroup = C::NT >= 4 ? 2 : 1;
 #pragma unroll
-        for (int t = 0; t < C::NT / 2; ++t) {
-          uint32_t v[C::kIn][4];
+        for (int t = 0; t < C::NT / 2; t += kGroup) {
+          uint32_t v[kGroup][C::kIn][4];
 #pragma unroll
-          for (int q = 0; q < C::kIn; ++q) load_matrices_turned(v[q], bt + 2 * (q * C::kB + 16 * j * C::PB + 16 * t));
+          for (int i = 0; i < kGroup; ++i)
+#pragma unroll
+            for (int q = 0; q < C::kIn; ++q)
+              load_matrices_turned(v[i][q], bt + 2 * (q * C::kB + 16 * j * C::PB + 16 * (t + i)));
 #pragma unroll
           for (int m = 0; m < C::MT; ++m)
-            multiply_planes<C::kKeys, C::kIn, C::kFloat>(z[m][2 * t], z[m][2 * t + 1], key[m], v, fine);
+            multiply_planes<C::kKeys, C::kIn, kGroup, C::kFloat>(&z[m][2 * t], key[m], v, fine);
         }
       }
     }
@@ -491,10 +578,12 @@ R dispatch(int dtype, int d, F&& fn) {
   return RLENV_EUNSUPPORTED;
 }
 
+bool off_boundary(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 != 0; }
+
 // Rows are read as 16-byte pieces: a base and strides off that boundary are rejected.
 bool aligned_rows(const void* p, const int64_t* st, int dtype, int axes) {
   const uint64_t size = dtype == RLENV_F32 ? 4 : 2;
-  if (reinterpret_cast<uintptr_t>(p) % 16) return false;
+  if (off_boundary(p)) return false;
   for (int i = 0; i < axes; ++i)
     if (uint64_t(st[i]) * size % 16) return false;
   return true;
@@ -535,7 +624,7 @@ int rlenv_linear_attention_forward(int dtype, int d, int64_t t, int64_t n, int64
   using namespace rlenv;
   if (const int rc = check_sizes(dtype, d, t, n, h, scale)) return rc;
   if (n == 0 || h == 0) return RLENV_OK;
-  if (t > 0 && (!q || !k || !v || !strides || !out)) return RLENV_EINVAL;
+  if (t > 0 && (!q || !k || !v || !strides || !out || off_boundary(out))) return RLENV_EINVAL;
   if (!decay || !state_out || state_in == state_out) return RLENV_EINVAL;
   static const int64_t kNone[9] = {};
   const int64_t* st = t > 0 ? strides : kNone;
@@ -557,7 +646,9 @@ int rlenv_linear_attention_backward(int dtype, int d, int64_t t, int64_t n, int6
   using namespace rlenv;
   if (const int rc = check_sizes(dtype, d, t, n, h, scale)) return rc;
   if (n == 0 || h == 0) return RLENV_OK;
-  if (t > 0 && (!grad_out || !q || !k || !v || !strides || !grad_q || !grad_k || !grad_v)) return RLENV_EINVAL;
+  if (t > 0 && (!grad_out || !q || !k || !v || !strides || !grad_q || !grad_k || !grad_v ||
+                off_boundary(grad_q) || off_boundary(grad_k) || off_boundary(grad_v)))
+    return RLENV_EINVAL;
   if (!decay || (grad_state_in && grad_state_in == grad_state_out)) return RLENV_EINVAL;
   static const int64_t kNone[12] = {};
   const int64_t* st = t > 0 ? strides : kNone;

@@ -141,14 +141,17 @@ struct Shape {
   static constexpr int PX = D + 8, PB = DB + 8;         // row pitches: 16 bytes past a multiple of 32,
                                                         // so that eight rows' pieces fall in distinct banks
   static constexpr int kX = kChunk * PX, kB = kChunk * PB, kS = D * PB;  // a plane's elements
-  // Four warps with 16 tokens of the chunk each, or eight, two to a row of 16 with half the columns
-  // each, where a block's shared memory leaves room for few of them (float32, and 128 columns).
-  static constexpr int kWarps = D == 128 || (kFloat && D >= 32) ? 8 : 4;
+  // Warps: kRowWarps share the chunk's tokens, kColWarps the output's columns (float32 heads of 128, whose
+  // planes leave room for one block on an SM). Narrow bfloat16 heads give a warp two tiles of 16 tokens (RT): a
+  // fragment of the other operand then serves twice.
+  static constexpr int kRowWarps = !kFloat && D <= 32 ? 2 : 4, kColWarps = kFloat && D == 128 ? 2 : 1;
+  static constexpr int kWarps = kRowWarps * kColWarps;
   static constexpr int kThreads = 32 * kWarps;
-  static constexpr int OC = DB / (kWarps / 4);          // output columns a warp
-  // Tiles come two chunks deep for bfloat16 (cp.async); float32 ones pass through registers, where they
-  // become planes, one chunk ahead.
-  static constexpr int kBuffers = kFloat ? 1 : 2;
+  static constexpr int RT = 4 / kRowWarps;
+  static constexpr int OC = DB / kColWarps;             // output columns a warp
+  // Tiles come a chunk ahead: bfloat16 ones in a second buffer (cp.async), but at 128 columns, where a second
+  // block on the SM is worth more; float32 ones through registers, where they become planes.
+  static constexpr int kBuffers = kFloat || D == 128 ? 1 : 2;
   static constexpr int kTiles = kIn * (2 * kX + kB);    // elements of a buffer
   static constexpr int kSmem = 2 * (kBuffers * kTiles + kMid * kS);
   // The carry's rows and columns by warp: RG groups of rows, CG of columns.
@@ -156,7 +159,9 @@ struct Shape {
   static constexpr int RG = D / (16 * MT);
   static constexpr int CG = kWarps / RG < DB / 16 ? kWarps / RG : DB / 16;
   static constexpr int NT = DB / CG / 8;                // 8-column tiles a warp
-  static constexpr int kPerSm = kSmem > 113000 ? 1 : kSmem > 75000 ? 2 : kWarps == 8 ? 2 : 3;  // blocks that fit
+  // blocks that fit an SM's shared memory and registers
+  static constexpr int kRoom = 227 * 1024 / (kSmem + 2048), kMost = D >= 64 ? 3 : kFloat ? (D == 32 ? 3 : 4) : D == 32 ? 6 : 8;
+  static constexpr int kPerSm = kRoom < kMost ? kRoom : kMost;
 };
 
 RLENV_D uint32_t shared_address(const void* p) { return uint32_t(__cvta_generic_to_shared(p)); }
@@ -176,27 +181,32 @@ RLENV_D void multiply(float c[4], const uint32_t a[4], uint32_t b0, uint32_t b1)
                : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-// c0, c1 (two 8-column tiles) += a b over all pairs of planes worth it, the small ones first. The tensor
-// core truncates as it accumulates: for float32 results (three planes of data) the pairs are summed from
-// zero and added to c in a rounded addition, or the error of long sums grows to a few 1e-6.
-// The last plane of a only where `fine`.
-template <int NA, int NB, bool kFloat>
-RLENV_D void multiply_planes(float c0[4], float c1[4], const uint32_t (&a)[NA][4], const uint32_t (&b)[NB][4],
-                             bool fine = true) {
-  float s0[4] = {}, s1[4] = {};
+// c (2 NT tiles of 8 columns) += a b over all pairs of planes worth it, the small ones first, `a`'s last plane
+// only where `fine`; b holds two tiles a fragment. Planes run outside of tiles, so that products which add to
+// the same tile are 2 NT apart: one's latency is some four others' issue. The tensor core truncates as it
+// accumulates: for float32 results (three planes of data) the pairs are summed from zero and added to c in a
+// rounded addition, or the error of long sums grows to a few 1e-6.
+template <int NA, int NB, int NT, bool kFloat>
+RLENV_D void multiply_planes(float (*c)[4], const uint32_t (&a)[NA][4], const uint32_t (&b)[NT][NB][4], bool fine = true) {
+  float s[2 * NT][4] = {};
 #pragma unroll
   for (int order = 2; order >= 0; --order)
 #pragma unroll
     for (int u = 0; u <= order; ++u) {
       const int q = order - u;
       if (u < NA && q < NB && (u + 1 < NA || fine)) {
-        multiply(kFloat ? s0 : c0, a[u], b[q][0], b[q][1]);
-        multiply(kFloat ? s1 : c1, a[u], b[q][2], b[q][3]);
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+          multiply(kFloat ? s[2 * t] : c[2 * t], a[u], b[t][q][0], b[t][q][1]);
+          multiply(kFloat ? s[2 * t + 1] : c[2 * t + 1], a[u], b[t][q][2], b[t][q][3]);
+        }
       }
     }
   if constexpr (kFloat) {
 #pragma unroll
-    for (int q = 0; q < 4; ++q) c0[q] += s0[q], c1[q] += s1[q];
+    for (int t = 0; t < 2 * NT; ++t)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) c[t][q] += s[t][q];
   }
 }
 

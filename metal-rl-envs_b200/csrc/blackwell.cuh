@@ -37,14 +37,22 @@ RLENV_D bool barrier_try(uint32_t bar, uint32_t parity) {
       : "=r"(done) : "r"(bar), "r"(parity) : "memory");
   return done != 0;
 }
-// Waits for the phase of `parity` to end. Every wait is bounded: past kTries attempts, each of which the
-// hardware suspends for a while, `dead` is set, and from then on every wait of the block gives up at once.
-constexpr int kTries = 1 << 22;
+// Waits for the phase of `parity` to end. Every wait is bounded: after kPatience nanoseconds `dead` is set,
+// and from then on every wait of the block gives up at once.
+constexpr uint64_t kPatience = 2000000000;
+RLENV_D uint64_t nanoseconds() {
+  uint64_t t;
+  asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
+  return t;
+}
 RLENV_D bool barrier_wait(uint32_t bar, uint32_t parity, volatile int* dead) {
-  for (int i = 0; i < kTries; ++i) {
+  for (int i = 0; i < 32; ++i)
+    if (barrier_try(bar, parity)) return true;
+  const uint64_t start = nanoseconds();
+  do {
     if (barrier_try(bar, parity)) return true;
     if (*dead) return false;
-  }
+  } while (nanoseconds() - start < kPatience);
   *dead = 1;
   return false;
 }
