@@ -100,11 +100,16 @@ RLENV_D void commit(uint32_t bar) {
       "h"(uint16_t(3))
       : "memory");
 }
-RLENV_D void multiply(uint32_t d, uint64_t a, uint64_t b, uint32_t kind, bool accumulate) {
+// The high word of every operand's descriptor: eight rows every 1,024 bytes, 128-byte swizzle.
+constexpr uint32_t kOperandHigh = 1024 >> 4 | 1u << 14 | 2u << 29;
+
+// D (+)= A B; a and b are the operands' places (below). One thread issues a product after the other, each
+// waiting for the few instructions before it, so nothing is computed here that can stand outside the loop.
+RLENV_D void multiply(uint32_t d, uint32_t a, uint32_t b, uint32_t kind, bool accumulate) {
   asm volatile(
-      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
-      " tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n}" ::"r"(d),
-      "l"(a), "l"(b), "r"(kind), "r"(uint32_t(accumulate))
+      "{\n .reg .pred p;\n .reg .b64 a, b;\n setp.ne.b32 p, %4, 0;\n mov.b64 a, {%1, %5};\n mov.b64 b, {%2, %5};\n"
+      " tcgen05.mma.cta_group::2.kind::f16 [%0], a, b, %3, p;\n}" ::"r"(d),
+      "r"(a), "r"(b), "r"(kind), "r"(uint32_t(accumulate)), "n"(kOperandHigh)
       : "memory");
 }
 // 16 columns at each of two places, of this warp's 32 lanes: lane l gets its row's columns. The wait
@@ -125,13 +130,13 @@ RLENV_D void tmem_load16x2(float (&v)[32], uint32_t at, uint32_t and_at) {
   for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
 }
 
-// A bfloat16 operand in shared memory, rows of 128 bytes swizzled by eights as the tensor copies write
-// them. K-major: a row is 64 elements of the contraction, eight rows 1,024 bytes apart from the next
-// eight. MN-major: a row is 64 elements of the other axis, eight steps of the contraction 1,024 bytes
+// The place of a bfloat16 operand in shared memory, rows of 128 bytes swizzled by eights as the tensor
+// copies write them: the low word of its descriptor, in 16-byte units, so that `bytes` further on is an
+// addition of bytes / 16. K-major: a row is 64 elements of the contraction, eight rows 1,024 bytes apart from
+// the next eight. MN-major: a row is 64 elements of the other axis, eight steps of the contraction 1,024 bytes
 // apart from the next eight and the next 64 elements `block` bytes away.
-RLENV_D uint64_t operand(uint32_t at, bool mn_major, uint32_t block) {
-  return uint64_t((at & 0x3ffff) >> 4) | uint64_t(mn_major ? block >> 4 : 1) << 16 | uint64_t(1024 >> 4) << 32 |
-         uint64_t(1) << 46 | uint64_t(2) << 61;
+RLENV_D uint32_t operand(uint32_t at, bool mn_major, uint32_t block) {
+  return (at & 0x3ffff) >> 4 | (mn_major ? block >> 4 : 1) << 16;
 }
 // bfloat16 x bfloat16 -> float32, M x N.
 constexpr uint32_t product_kind(int m, int n, bool a_mn, bool b_mn) {

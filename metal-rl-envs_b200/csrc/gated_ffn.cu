@@ -149,14 +149,12 @@ template <typename T>
 RLENV_D int plane_a(int pair) { return Tile<T>::kFloat ? 0x118 >> (2 * pair) & 3 : 0; }  // 0 2 1 0 1 0
 template <typename T>
 RLENV_D int plane_b(int pair) { return Tile<T>::kFloat ? 0x052 >> (2 * pair) & 3 : 0; }  // 2 0 1 1 0 0
-// Whether the accumulator is handed over after step `it` of `steps`.
-template <typename T>
-RLENV_D bool run_ends(int it, int steps) {
-  if (it + 1 == steps) return true;
-  if (!Tile<T>::kFloat) return false;
-  const int small = steps / Tile<T>::kPairs * (Tile<T>::kPairs - 1);
-  if (it + 1 <= small) return it + 1 == small || (it + 1) % Tile<T>::kSmallRun == 0;
-  return (it + 1 - small) % Tile<T>::kRun == 0;
+// How often the accumulator of a float32 tile of `steps` steps is handed over: the small products' runs, and
+// the leading ones'.
+RLENV_D int runs_of(int steps) {
+  constexpr int kPairs = Tile<float>::kPairs, kSmall = Tile<float>::kSmallRun, kRun = Tile<float>::kRun;
+  const int leading = steps / kPairs, small = steps - leading;
+  return (small + kSmall - 1) / kSmall + (leading + kRun - 1) / kRun;
 }
 
 // Four neighbouring values of a row, the first n of them there: in one access where all are and `wide`
@@ -351,26 +349,30 @@ product_kernel(const __grid_constant__ Product p, int items) {
       for (int item = first; item < items && ok; item += stride) {
         const Work w = work_of<T, kOp>(p, item);
         const Operands& in = p.in[kOp == kGradients && w.weights];
-        const int r0 = (2 * w.row + rank) * kRows;
+        const int r0 = (2 * w.row + rank) * kRows, c0 = w.c0 + (kPaired ? 0 : rank * C::kHalf);
+        const CUtensorMap* const map_a = &in.a;
         for (int pair = 0; pair < C::kPairs && ok; ++pair) {
           const int pa = plane_a<T>(pair), pb = plane_b<T>(pair);
           for (int seg = 0; seg < w.segs && ok; ++seg) {
-            for (int k = w.k0; k < w.k0 + w.blocks; ++k) {
-              const int k0 = k * kStep;
+            // slices: planes; of the gates dg's and du's by turns. Gates in the first block, ups in the second.
+            const CUtensorMap* const map_b = (kPaired ? rank : seg) ? &in.b1 : &in.b0;
+            const int slice_a = kPaired || w.weights ? pa : 2 * pa + seg, slice_b = !kPaired && w.weights ? 2 * pb + w.weight : pb;
+            const int k_end = (w.k0 + w.blocks) * kStep;
+            for (int k0 = w.k0 * kStep; k0 < k_end; k0 += kStep) {
+              const uint32_t bar = full_at + 8 * stage, a = ring + stage * C::kRingBytes, b = a + C::kABytes;
               if (!(ok = bw::barrier_wait(empty + 8 * stage, phase ^ 1, dead))) break;
               if (rank == 0) bw::barrier_expect(full + 8 * stage, 2 * C::kRingBytes);
-              const uint32_t bar = full_at + 8 * stage, a = ring + stage * C::kRingBytes, b = a + C::kABytes;
-              if (kPaired) {  // gates in the first block, ups in the second
-                bw::copy_tile(a, &in.a, bar, k0, r0, pa);
-                for (int i = 0; i < C::kHalf / 64; ++i)
-                  bw::copy_tile(b + i * kBox, rank ? &in.b1 : &in.b0, bar, w.c0 + 64 * i, k0, pb);
-              } else if (w.weights) {
-                for (int i = 0; i < kRows / 64; ++i) bw::copy_tile(a + i * kBox, &in.a, bar, r0 + 64 * i, k0, pa);
-                for (int i = 0; i < C::kHalf / 64; ++i)
-                  bw::copy_tile(b + i * kBox, &in.b0, bar, w.c0 + rank * C::kHalf + 64 * i, k0, 2 * pb + w.weight);
+              if (!kPaired && w.weights) {
+#pragma unroll
+                for (int i = 0; i < kRows / 64; ++i) bw::copy_tile(a + i * kBox, map_a, bar, r0 + 64 * i, k0, slice_a);
               } else {
-                bw::copy_tile(a, &in.a, bar, k0, r0, 2 * pa + seg);
-                bw::copy_tile(b, seg ? &in.b1 : &in.b0, bar, k0, w.c0 + rank * C::kHalf, pb);
+                bw::copy_tile(a, map_a, bar, k0, r0, slice_a);
+              }
+              if (kPaired || w.weights) {
+#pragma unroll
+                for (int i = 0; i < C::kHalf / 64; ++i) bw::copy_tile(b + i * kBox, map_b, bar, c0 + 64 * i, k0, slice_b);
+              } else {
+                bw::copy_tile(b, map_b, bar, k0, c0, slice_b);
               }
               used |= 1u << stage;
               if (++stage == C::kStages) stage = 0, phase ^= 1;
@@ -394,21 +396,26 @@ product_kernel(const __grid_constant__ Product p, int items) {
         const int steps = C::kPairs * w.segs * w.blocks;
         const bool mn_a = w.weights, mn_b = kPaired || w.weights;
         const uint32_t kind = bw::product_kind(2 * kRows, C::kCols, mn_a, mn_b);
+        const uint32_t a0 = bw::operand(ring, mn_a, kBox), b0 = bw::operand(ring + C::kABytes, mn_b, kBox);
+        const uint32_t a_step = mn_a ? 2048 / 16 : 32 / 16, b_step = mn_b ? 2048 / 16 : 32 / 16;  // 16 of the contraction
+        const int small = steps / C::kPairs * (C::kPairs - 1);
+        int left = C::kFloat ? min(C::kSmallRun, small) : steps;  // steps to the end of the run
         bool fresh = true;
         for (int it = 0; it < steps; ++it) {
           if (fresh && !(ok = bw::barrier_wait(taken + 8 * buffer, buffer_phase ^ 1, dead))) break;
+          const uint32_t d = tmem + buffer * C::kCols, a = a0 + stage * (C::kRingBytes / 16),
+                         b = b0 + stage * (C::kRingBytes / 16);
           if (!(ok = bw::barrier_wait(full + 8 * stage, phase, dead))) break;
           bw::fence_after();
-          const uint32_t a = ring + stage * C::kRingBytes, b = a + C::kABytes;
+          bw::multiply(d, a, b, kind, !fresh);
 #pragma unroll
-          for (int k = 0; k < kStep / 16; ++k)
-            bw::multiply(tmem + buffer * C::kCols, bw::operand(a + k * (mn_a ? 2048 : 32), mn_a, kBox),
-                         bw::operand(b + k * (mn_b ? 2048 : 32), mn_b, kBox), kind, !(fresh && k == 0));
+          for (int k = 1; k < kStep / 16; ++k) bw::multiply(d, a + k * a_step, b + k * b_step, kind, true);
           bw::commit(empty + 8 * stage);
-          fresh = run_ends<T>(it, steps);
+          fresh = --left == 0;
           if (fresh) {
             bw::commit(summed + 8 * buffer);
             if (++buffer == 2) buffer = 0, buffer_phase ^= 1;
+            left = it + 1 < small ? min(C::kSmallRun, small - it - 1) : min(C::kRun, steps - it - 1);
           }
           if (++stage == C::kStages) stage = 0, phase ^= 1;
         }
@@ -453,8 +460,7 @@ product_kernel(const __grid_constant__ Product p, int items) {
         for (int j = 0; j < kMine / 32; ++j)
 #pragma unroll
           for (int i = 0; i < 32; ++i) sum[j][i] = 0.0f;
-        for (int it = 0; it < steps; ++it) {
-          if (!run_ends<T>(it, steps)) continue;
+        for (int runs = runs_of(steps); runs > 0; --runs) {
           ok = ok && bw::barrier_wait(summed + 8 * buffer, buffer_phase, dead);
           ok = __all_sync(0xffffffffu, ok);
           if (!ok) break;
