@@ -57,6 +57,28 @@ RLENV_D bool barrier_wait(uint32_t bar, uint32_t parity, volatile int* dead) {
   return false;
 }
 
+// The same by a whole warp, all of whose lanes get the same answer, and know it: copies and products take
+// their operands from the warp's uniform registers, and under control flow that may diverge each operand is
+// moved there anew, some 60 cycles a product. So the warps that issue them run as one, and only the
+// instruction itself stands under `elect`.
+RLENV_D bool barrier_wait_warp(uint32_t bar, uint32_t parity, volatile int* dead) {
+  for (int i = 0; i < 32; ++i)
+    if (__all_sync(0xffffffffu, barrier_try(bar, parity))) return true;
+  const uint64_t start = nanoseconds();
+  while (true) {
+    if (__all_sync(0xffffffffu, barrier_try(bar, parity))) return true;
+    if (__any_sync(0xffffffffu, *dead != 0)) return false;
+    if (__any_sync(0xffffffffu, nanoseconds() - start > kPatience)) break;
+  }
+  *dead = 1;
+  return false;
+}
+RLENV_D bool elect() {  // one lane of the warp
+  uint32_t r;
+  asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}" : "=r"(r));
+  return r != 0;
+}
+
 // ---- tensor copies ------------------------------------------------------------------------------
 RLENV_D void prefetch_map(const CUtensorMap* map) {
   asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory");

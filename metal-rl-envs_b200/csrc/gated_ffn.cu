@@ -323,7 +323,7 @@ product_kernel(const __grid_constant__ Product p, int items) {
   const uint32_t ring = (bw::shared_at(raw) + 1023) & ~1023u;
   const uint32_t full = bw::shared_at(bars), empty = full + 8 * C::kStages;
   const uint32_t summed = empty + 8 * C::kStages, taken = summed + 16;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(0xffffffffu, int(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
   const int rank = int(bw::cluster_rank());
   if (threadIdx.x == 0) {
     for (int i = 0; i < C::kStages; ++i) bw::barrier_init(full + 8 * i, 1), bw::barrier_init(empty + 8 * i, 1);
@@ -336,31 +336,31 @@ product_kernel(const __grid_constant__ Product p, int items) {
   __syncthreads();
   bw::cluster_sync();
   bw::fence_after();
-  const uint32_t tmem = tmem_slot;
+  const uint32_t tmem = __shfl_sync(0xffffffffu, tmem_slot, 0);
   const int first = blockIdx.x / 2, stride = gridDim.x / 2;
 
   if (warp == 0) {
-    if (lane == 0) {
-      // Both blocks copy their rows of A and their columns of B; all bytes count at the first block's barrier.
-      int stage = 0;
-      uint32_t phase = 0, used = 0;  // used: stages that have been filled at least once
-      bool ok = true;
-      const uint32_t full_at = bw::in_block(full, 0);
-      for (int item = first; item < items && ok; item += stride) {
-        const Work w = work_of<T, kOp>(p, item);
-        const Operands& in = p.in[kOp == kGradients && w.weights];
-        const int r0 = (2 * w.row + rank) * kRows, c0 = w.c0 + (kPaired ? 0 : rank * C::kHalf);
-        const CUtensorMap* const map_a = &in.a;
-        for (int pair = 0; pair < C::kPairs && ok; ++pair) {
-          const int pa = plane_a<T>(pair), pb = plane_b<T>(pair);
-          for (int seg = 0; seg < w.segs && ok; ++seg) {
-            // slices: planes; of the gates dg's and du's by turns. Gates in the first block, ups in the second.
-            const CUtensorMap* const map_b = (kPaired ? rank : seg) ? &in.b1 : &in.b0;
-            const int slice_a = kPaired || w.weights ? pa : 2 * pa + seg, slice_b = !kPaired && w.weights ? 2 * pb + w.weight : pb;
-            const int k_end = (w.k0 + w.blocks) * kStep;
-            for (int k0 = w.k0 * kStep; k0 < k_end; k0 += kStep) {
-              const uint32_t bar = full_at + 8 * stage, a = ring + stage * C::kRingBytes, b = a + C::kABytes;
-              if (!(ok = bw::barrier_wait(empty + 8 * stage, phase ^ 1, dead))) break;
+    // Both blocks copy their rows of A and their columns of B; all bytes count at the first block's barrier.
+    int stage = 0;
+    uint32_t phase = 0, used = 0;  // used: stages that have been filled at least once
+    bool ok = true;
+    const uint32_t full_at = bw::in_block(full, 0);
+    for (int item = first; item < items && ok; item += stride) {
+      const Work w = work_of<T, kOp>(p, item);
+      const Operands& in = p.in[kOp == kGradients && w.weights];
+      const int r0 = (2 * w.row + rank) * kRows, c0 = w.c0 + (kPaired ? 0 : rank * C::kHalf);
+      const CUtensorMap* const map_a = &in.a;
+      for (int pair = 0; pair < C::kPairs && ok; ++pair) {
+        const int pa = plane_a<T>(pair), pb = plane_b<T>(pair);
+        for (int seg = 0; seg < w.segs && ok; ++seg) {
+          // slices: planes; of the gates dg's and du's by turns. Gates in the first block, ups in the second.
+          const CUtensorMap* const map_b = (kPaired ? rank : seg) ? &in.b1 : &in.b0;
+          const int slice_a = kPaired || w.weights ? pa : 2 * pa + seg, slice_b = !kPaired && w.weights ? 2 * pb + w.weight : pb;
+          const int k_end = (w.k0 + w.blocks) * kStep;
+          for (int k0 = w.k0 * kStep; k0 < k_end; k0 += kStep) {
+            const uint32_t bar = full_at + 8 * stage, a = ring + stage * C::kRingBytes, b = a + C::kABytes;
+            if (!(ok = bw::barrier_wait_warp(empty + 8 * stage, phase ^ 1, dead))) break;
+            if (bw::elect()) {
               if (rank == 0) bw::barrier_expect(full + 8 * stage, 2 * C::kRingBytes);
               if (!kPaired && w.weights) {
 #pragma unroll
@@ -374,20 +374,20 @@ product_kernel(const __grid_constant__ Product p, int items) {
               } else {
                 bw::copy_tile(b, map_b, bar, k0, c0, slice_b);
               }
-              used |= 1u << stage;
-              if (++stage == C::kStages) stage = 0, phase ^= 1;
             }
+            used |= 1u << stage;
+            if (++stage == C::kStages) stage = 0, phase ^= 1;
           }
         }
       }
-      if (!ok && rank == 0) {  // the copies in flight land before the blocks may end
-        int unused = 0;
-        for (int i = 0; i < C::kStages; ++i)
-          if (used >> i & 1) bw::barrier_wait(full + 8 * i, i < stage ? phase : phase ^ 1, &unused), unused = 0;
-      }
+    }
+    if (!ok && rank == 0) {  // the copies in flight land before the blocks may end
+      int unused = 0;
+      for (int i = 0; i < C::kStages; ++i)
+        if (used >> i & 1) bw::barrier_wait(full + 8 * i, i < stage ? phase : phase ^ 1, &unused), unused = 0;
     }
   } else if (warp == 1) {
-    if (lane == 0 && rank == 0) {
+    if (rank == 0) {
       int stage = 0, buffer = 0;
       uint32_t phase = 0, buffer_phase = 0;
       bool ok = true;
@@ -402,18 +402,21 @@ product_kernel(const __grid_constant__ Product p, int items) {
         int left = C::kFloat ? min(C::kSmallRun, small) : steps;  // steps to the end of the run
         bool fresh = true;
         for (int it = 0; it < steps; ++it) {
-          if (fresh && !(ok = bw::barrier_wait(taken + 8 * buffer, buffer_phase ^ 1, dead))) break;
+          if (fresh && !(ok = bw::barrier_wait_warp(taken + 8 * buffer, buffer_phase ^ 1, dead))) break;
           const uint32_t d = tmem + buffer * C::kCols, a = a0 + stage * (C::kRingBytes / 16),
                          b = b0 + stage * (C::kRingBytes / 16);
-          if (!(ok = bw::barrier_wait(full + 8 * stage, phase, dead))) break;
+          if (!(ok = bw::barrier_wait_warp(full + 8 * stage, phase, dead))) break;
           bw::fence_after();
-          bw::multiply(d, a, b, kind, !fresh);
-#pragma unroll
-          for (int k = 1; k < kStep / 16; ++k) bw::multiply(d, a + k * a_step, b + k * b_step, kind, true);
-          bw::commit(empty + 8 * stage);
+          const bool more = !fresh;
           fresh = --left == 0;
+          if (bw::elect()) {
+            bw::multiply(d, a, b, kind, more);
+#pragma unroll
+            for (int k = 1; k < kStep / 16; ++k) bw::multiply(d, a + k * a_step, b + k * b_step, kind, true);
+            bw::commit(empty + 8 * stage);
+            if (fresh) bw::commit(summed + 8 * buffer);
+          }
           if (fresh) {
-            bw::commit(summed + 8 * buffer);
             if (++buffer == 2) buffer = 0, buffer_phase ^= 1;
             left = it + 1 < small ? min(C::kSmallRun, small - it - 1) : min(C::kRun, steps - it - 1);
           }
