@@ -60,7 +60,7 @@ pack_kernel(const T* __restrict__ from, int64_t rows, int64_t cols, int64_t pitc
 enum Op { kForward, kGates, kGradients };  // h; dg and du; dx, dWg and dWu
 
 constexpr int kRows = 128;       // of a tile, in each block of a pair
-constexpr int kStep = 64;        // of the contraction, a ring buffer's
+constexpr int kBlock = 64;       // of the contraction: a tile row's 128 bytes
 constexpr int kProductThreads = 384;  // copies, products, two idle warps, eight warps of epilogue
 constexpr int kEpilogueWarps = 8;
 constexpr int kTmemColumns = 512;
@@ -73,9 +73,14 @@ struct Tile {
   static constexpr int kPairs = kFloat ? 6 : 1;  // products of planes
   static constexpr int kCols = kFloat ? 128 : 256;
   static constexpr int kHalf = kCols / 2;        // columns of B in each block
-  static constexpr int kABytes = kRows * kStep * 2;
-  static constexpr int kRingBytes = kABytes + kHalf * kStep * 2;
-  static constexpr int kStages = kFloat ? 8 : 6;
+  // A ring buffer's blocks: float32's narrower products are over sooner, and two blocks keep the turn of a
+  // step, some 300 cycles of waiting and committing, below the products' time.
+  static constexpr int kBlocks = kFloat ? 2 : 1;
+  static constexpr int kStep = kBlocks * kBlock;
+  static constexpr int kABytes = kRows * kBlock * 2;
+  static constexpr int kBlockBytes = kABytes + kHalf * kBlock * 2;
+  static constexpr int kRingBytes = kBlocks * kBlockBytes;
+  static constexpr int kStages = kFloat ? 4 : 6;
   static constexpr int kStageAt = kStages * kRingBytes;  // the epilogue's 32 x 32 tiles, one a warp
   // the ring starts on a 1,024-byte boundary
   static constexpr int kSmem = kStageAt + kEpilogueWarps * kStageFloats * 4 + 1024;
@@ -83,7 +88,7 @@ struct Tile {
   // (float32 only). The tensor core truncates as it accumulates; rounded additions of short sums keep
   // float32 results at float32's error. Of the products of planes only the leading one, the last to be
   // formed, is large enough to need the short sums.
-  static constexpr int kRun = 4, kSmallRun = 32;
+  static constexpr int kRun = 2, kSmallRun = 16;
 };
 
 struct Operands {
@@ -95,7 +100,7 @@ struct alignas(64) Product {
   int act;
   // Tiles: of h or the gates; of dx and of both weights.
   int row_tiles, col_tiles, weight_rows, weight_cols;
-  int splits, split_blocks;  // of the contraction over tokens in the weights' gradients
+  int splits, split_steps;   // of the contraction over tokens in the weights' gradients
   const void* dh;            // kGates
   void *out, *dwg, *dwu;     // h or dx; the weights' gradients
   float* parts;              // (splits, 2, K, F) where splits > 1
@@ -108,14 +113,15 @@ struct alignas(64) Product {
 // operands that lie in L2.
 constexpr int kBand = 8;
 
-// A tile of work: columns from c0, rows from row tile `row`, a contraction over `blocks` steps of each of
-// `segs` segments from block k0.
+// A tile of work: columns from c0, rows from row tile `row`, a contraction over `steps` ring buffers of each of
+// `segs` segments from the one numbered k0.
 struct Work {
   bool weights;
-  int weight, split, row, c0, k0, blocks, segs;
+  int weight, split, row, c0, k0, steps, segs;
 };
 template <typename T, int kOp>
 RLENV_D Work work_of(const Product& p, int item) {
+  constexpr int kStep = Tile<T>::kStep;
   Work w{};
   int rows = p.row_tiles, cols = p.col_tiles;
   w.segs = 1;
@@ -126,14 +132,14 @@ RLENV_D Work work_of(const Product& p, int item) {
     if (w.weights) {
       w.split = item / per, item %= per;
       rows = p.weight_rows, cols = p.weight_cols;
-      w.k0 = w.split * p.split_blocks;
-      w.blocks = min(p.split_blocks, int((p.m + kStep - 1) / kStep) - w.k0);
+      w.k0 = w.split * p.split_steps;
+      w.steps = min(p.split_steps, int((p.m + kStep - 1) / kStep) - w.k0);
     } else {
       item -= per * p.splits;
-      w.segs = 2, w.blocks = int((p.f + kStep - 1) / kStep);
+      w.segs = 2, w.steps = int((p.f + kStep - 1) / kStep);
     }
   } else {
-    w.blocks = int((p.k + kStep - 1) / kStep);
+    w.steps = int((p.k + kStep - 1) / kStep);
   }
   const int per = kBand * cols, band = item / per, in = item % per;
   const int high = min(kBand, rows - band * kBand);
@@ -282,9 +288,9 @@ RLENV_D void finish_values(T* to, int64_t pitch, int64_t rows, int64_t cols, flo
   }
 }
 
-// Rows from r0, columns from c (of h, a weight or dx). v: 16 gates and 16 ups, or 32 values.
+// Rows from r0, columns from c (of h, a weight or dx). v, as bits: 16 gates and 16 ups, or 32 values.
 template <typename T, int kOp>
-RLENV_D void finish(const Product& p, const Work& w, int64_t r0, int64_t c, const float (&v)[32],
+RLENV_D void finish(const Product& p, const Work& w, int64_t r0, int64_t c, const uint32_t (&v)[32],
                     const typename Four<T>::type (&dh)[4], float* stage) {
   const int64_t all_rows = kOp == kGradients && w.weights ? p.k : p.m;
   const int64_t all_cols = kOp == kGradients && !w.weights ? p.k : p.f;
@@ -293,7 +299,7 @@ RLENV_D void finish(const Product& p, const Work& w, int64_t r0, int64_t c, cons
   __syncwarp();
 #pragma unroll
   for (int i = 0; i < 8; ++i)
-    *stage_at(stage, lane, i) = make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+    *reinterpret_cast<uint4*>(stage_at(stage, lane, i)) = make_uint4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
   __syncwarp();
   if constexpr (kOp == kGradients) {
     if (w.weights && p.splits > 1)
@@ -314,7 +320,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kProductThreads, 1)
 product_kernel(const __grid_constant__ Product p, int items) {
   using C = Tile<T>;
   constexpr bool kPaired = kOp != kGradients;  // half of a tile's columns are gates, half ups
-  constexpr uint32_t kBox = 64 * kStep * 2;
+  constexpr uint32_t kBox = 64 * kBlock * 2;
   extern __shared__ unsigned char raw[];
   __shared__ __align__(8) uint64_t bars[2 * C::kStages + 4];
   __shared__ uint32_t tmem_slot;
@@ -356,23 +362,28 @@ product_kernel(const __grid_constant__ Product p, int items) {
           // slices: planes; of the gates dg's and du's by turns. Gates in the first block, ups in the second.
           const CUtensorMap* const map_b = (kPaired ? rank : seg) ? &in.b1 : &in.b0;
           const int slice_a = kPaired || w.weights ? pa : 2 * pa + seg, slice_b = !kPaired && w.weights ? 2 * pb + w.weight : pb;
-          const int k_end = (w.k0 + w.blocks) * kStep;
-          for (int k0 = w.k0 * kStep; k0 < k_end; k0 += kStep) {
-            const uint32_t bar = full_at + 8 * stage, a = ring + stage * C::kRingBytes, b = a + C::kABytes;
+          const int k_end = (w.k0 + w.steps) * C::kStep;
+          for (int k0 = w.k0 * C::kStep; k0 < k_end; k0 += C::kStep) {
+            const uint32_t bar = full_at + 8 * stage, a0 = ring + stage * C::kRingBytes;
             if (!(ok = bw::barrier_wait_warp(empty + 8 * stage, phase ^ 1, dead))) break;
             if (bw::elect()) {
               if (rank == 0) bw::barrier_expect(full + 8 * stage, 2 * C::kRingBytes);
-              if (!kPaired && w.weights) {
 #pragma unroll
-                for (int i = 0; i < kRows / 64; ++i) bw::copy_tile(a + i * kBox, map_a, bar, r0 + 64 * i, k0, slice_a);
-              } else {
-                bw::copy_tile(a, map_a, bar, k0, r0, slice_a);
-              }
-              if (kPaired || w.weights) {
+              for (int q = 0; q < C::kBlocks; ++q) {  // what lies past the contraction's end reads as zero
+                const uint32_t a = a0 + q * C::kBlockBytes, b = a + C::kABytes;
+                const int k = k0 + q * kBlock;
+                if (!kPaired && w.weights) {
 #pragma unroll
-                for (int i = 0; i < C::kHalf / 64; ++i) bw::copy_tile(b + i * kBox, map_b, bar, c0 + 64 * i, k0, slice_b);
-              } else {
-                bw::copy_tile(b, map_b, bar, k0, c0, slice_b);
+                  for (int i = 0; i < kRows / 64; ++i) bw::copy_tile(a + i * kBox, map_a, bar, r0 + 64 * i, k, slice_a);
+                } else {
+                  bw::copy_tile(a, map_a, bar, k, r0, slice_a);
+                }
+                if (kPaired || w.weights) {
+#pragma unroll
+                  for (int i = 0; i < C::kHalf / 64; ++i) bw::copy_tile(b + i * kBox, map_b, bar, c0 + 64 * i, k, slice_b);
+                } else {
+                  bw::copy_tile(b, map_b, bar, k, c0, slice_b);
+                }
               }
             }
             used |= 1u << stage;
@@ -393,7 +404,7 @@ product_kernel(const __grid_constant__ Product p, int items) {
       bool ok = true;
       for (int item = first; item < items && ok; item += stride) {
         const Work w = work_of<T, kOp>(p, item);
-        const int steps = C::kPairs * w.segs * w.blocks;
+        const int steps = C::kPairs * w.segs * w.steps;
         const bool mn_a = w.weights, mn_b = kPaired || w.weights;
         const uint32_t kind = bw::product_kind(2 * kRows, C::kCols, mn_a, mn_b);
         const uint32_t a0 = bw::operand(ring, mn_a, kBox), b0 = bw::operand(ring + C::kABytes, mn_b, kBox);
@@ -410,9 +421,12 @@ product_kernel(const __grid_constant__ Product p, int items) {
           const bool more = !fresh;
           fresh = --left == 0;
           if (bw::elect()) {
-            bw::multiply(d, a, b, kind, more);
 #pragma unroll
-            for (int k = 1; k < kStep / 16; ++k) bw::multiply(d, a + k * a_step, b + k * b_step, kind, true);
+            for (int q = 0; q < C::kBlocks; ++q)
+#pragma unroll
+              for (int k = 0; k < kBlock / 16; ++k)
+                bw::multiply(d, a + q * (C::kBlockBytes / 16) + k * a_step, b + q * (C::kBlockBytes / 16) + k * b_step,
+                             kind, q + k > 0 || more);
             bw::commit(empty + 8 * stage);
             if (fresh) bw::commit(summed + 8 * buffer);
           }
@@ -441,68 +455,74 @@ product_kernel(const __grid_constant__ Product p, int items) {
     };
     // Run j of 32 columns of this thread's, as two of 16: a gated tile's are gates and ups.
     const auto column = [&](int j) { return kPaired ? half * (C::kHalf / 2) + 16 * j : half * kMine + 32 * j; };
-    const auto load_run = [&](float (&v)[32], int j) {
+    constexpr int kRuns = kMine / 32;
+    const auto load_run = [&](uint32_t (&v)[32], int j) {
       const uint32_t at = tmem + lanes + buffer * C::kCols + column(j);
       bw::tmem_load16x2(v, at, at + (kPaired ? C::kHalf : 16));
     };
     for (int item = first; item < items; item += stride) {
       const Work w = work_of<T, kOp>(p, item);
       const int64_t r0 = int64_t(2 * w.row + rank) * kRows + 32 * quarter;
-      typename Four<T>::type dh[4], dh_next[4];  // loaded one run ahead, the first under the tile's products
-      if constexpr (kOp == kGates) load_gradient<T>(p, r0, w.c0 + column(0), dh_next);
-      const auto next_gradient = [&](int j) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) dh[i] = dh_next[i];
+      // A run of results goes out while the next one's accumulators and gradients are on their way, the first
+      // gradients under the tile's products.
+      typename Four<T>::type dh[2][4];
+      const auto load_dh = [&](int j) {
         if constexpr (kOp == kGates)
-          if (j + 1 < kMine / 32) load_gradient<T>(p, r0, w.c0 + column(j + 1), dh_next);
+          if (j < kRuns) load_gradient<T>(p, r0, w.c0 + column(j), dh[j & 1]);
       };
-      if constexpr (C::kFloat) {
-        const int steps = C::kPairs * w.segs * w.blocks;
-        float sum[kMine / 32][32];
+      const auto finish_run = [&](uint32_t (&v)[32], int j) {
+        if (!ok) {  // a wait ran out: the results say so
 #pragma unroll
-        for (int j = 0; j < kMine / 32; ++j)
+          for (int i = 0; i < 32; ++i) v[i] = 0x7fffffffu;
+        }
+        finish<T, kOp>(p, w, r0, w.c0 + column(j), v, dh[j & 1], own_stage);
+      };
+      load_dh(0);
+      if constexpr (C::kFloat) {
+        float sum[kRuns][32];
+#pragma unroll
+        for (int j = 0; j < kRuns; ++j)
 #pragma unroll
           for (int i = 0; i < 32; ++i) sum[j][i] = 0.0f;
-        for (int runs = runs_of(steps); runs > 0; --runs) {
-          ok = ok && bw::barrier_wait(summed + 8 * buffer, buffer_phase, dead);
-          ok = __all_sync(0xffffffffu, ok);
+        for (int runs = runs_of(C::kPairs * w.segs * w.steps); runs > 0; --runs) {
+          ok = bw::barrier_wait_warp(summed + 8 * buffer, buffer_phase, dead) && ok;
           if (!ok) break;
           bw::fence_after();
 #pragma unroll
-          for (int j = 0; j < kMine / 32; ++j) {
-            float v[32];
+          for (int j = 0; j < kRuns; ++j) {
+            uint32_t v[32];
             load_run(v, j);
+            bw::tmem_ready(v);
 #pragma unroll
-            for (int i = 0; i < 32; ++i) sum[j][i] += v[i];
+            for (int i = 0; i < 32; ++i) sum[j][i] += __uint_as_float(v[i]);
           }
           take_next();
         }
 #pragma unroll
-        for (int j = 0; j < kMine / 32; ++j) {
-          if (!ok) {  // a wait ran out: the results say so
+        for (int j = 0; j < kRuns; ++j) {
+          load_dh(j + 1);
+          uint32_t v[32];
 #pragma unroll
-            for (int i = 0; i < 32; ++i) sum[j][i] = __uint_as_float(0x7fffffffu);
-          }
-          next_gradient(j);
-          finish<T, kOp>(p, w, r0, w.c0 + column(j), sum[j], dh, own_stage);
+          for (int i = 0; i < 32; ++i) v[i] = __float_as_uint(sum[j][i]);
+          finish_run(v, j);
         }
       } else {
-        ok = ok && bw::barrier_wait(summed + 8 * buffer, buffer_phase, dead);
-        ok = __all_sync(0xffffffffu, ok);
+        ok = bw::barrier_wait_warp(summed + 8 * buffer, buffer_phase, dead) && ok;
         bw::fence_after();
+        uint32_t even[32], odd[32];
+        load_run(even, 0);
 #pragma unroll 1
-        for (int j = 0; j < kMine / 32; ++j) {
-          float v[32];
-          next_gradient(j);
-          if (ok) {
-            load_run(v, j);
-          } else {
-#pragma unroll
-            for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(0x7fffffffu);
-          }
-          finish<T, kOp>(p, w, r0, w.c0 + column(j), v, dh, own_stage);
+        for (int j = 0; j < kRuns; j += 2) {
+          bw::tmem_ready(even);
+          load_run(odd, j + 1);
+          load_dh(j + 1);
+          finish_run(even, j);
+          bw::tmem_ready(odd);
+          if (j + 2 < kRuns) load_run(even, j + 2);
+          else take_next();  // all of the accumulator is read
+          load_dh(j + 2);
+          finish_run(odd, j + 1);
         }
-        take_next();
       }
     }
   }
@@ -657,26 +677,27 @@ int64_t planes(int dtype) { return dtype == RLENV_F32 ? 3 : 1; }
 struct Layout {  // scratch of a call
   void *x, *wg, *wu, *gates;
   float* parts;
-  int splits, split_blocks;
+  int splits, split_steps;
   int64_t bytes;
 };
 
 constexpr int kPairsOfSms = 74;
-constexpr int64_t kFewestBlocks = 8;
+constexpr int64_t kFewestSteps = 8;
 
 // The contraction over tokens of the weights' gradients is split where a tile of them would take longer
 // than a pair of SMs' share of all the work: a small block's weights are a few tiles, each a sum over every
 // token. The sums of each run of tokens are kept in float32 and added up in order.
 void split_tokens(int dtype, int64_t m, int64_t k, int64_t f, Layout* l) {
-  const int64_t wide = dtype == RLENV_F32 ? 128 : 256, high = 2 * kRows;
-  const int64_t blocks = (m + kStep - 1) / kStep, tiles = (k + high - 1) / high * ((f + wide - 1) / wide) * 2;
-  const int64_t dx = (m + high - 1) / high * ((k + wide - 1) / wide) * 2 * ((f + kStep - 1) / kStep);
-  int64_t share = (tiles * blocks + dx) / kPairsOfSms;
-  if (share < kFewestBlocks) share = kFewestBlocks;
-  int64_t splits = (blocks + share - 1) / share;
+  const int64_t wide = dtype == RLENV_F32 ? Tile<float>::kCols : Tile<__nv_bfloat16>::kCols, high = 2 * kRows;
+  const int64_t step = dtype == RLENV_F32 ? Tile<float>::kStep : Tile<__nv_bfloat16>::kStep;
+  const int64_t steps = (m + step - 1) / step, tiles = (k + high - 1) / high * ((f + wide - 1) / wide) * 2;
+  const int64_t dx = (m + high - 1) / high * ((k + wide - 1) / wide) * 2 * ((f + step - 1) / step);
+  int64_t share = (tiles * steps + dx) / kPairsOfSms;
+  if (share < kFewestSteps) share = kFewestSteps;
+  int64_t splits = (steps + share - 1) / share;
   if (splits < 1) splits = 1;
-  l->split_blocks = int((blocks + splits - 1) / splits);
-  l->splits = int((blocks + l->split_blocks - 1) / l->split_blocks);
+  l->split_steps = int((steps + splits - 1) / splits);
+  l->splits = int((steps + l->split_steps - 1) / l->split_steps);
 }
 Layout lay_out(int dtype, int64_t m, int64_t k, int64_t f, bool backward, void* scratch) {
   Scratch s{static_cast<unsigned char*>(scratch), 0};
@@ -749,7 +770,7 @@ int ffn(const void* dh, const void* x, const void* wg, const void* wu, int64_t m
   if (!dh) return run_product<T, kForward>(p, s);
   if (const int rc = run_product<T, kGates>(p, s)) return rc;
   const Operand D{p.gates, m, f, p.pitch, 2 * C::kPlanes};
-  p.out = dx, p.dwg = dwg, p.dwu = dwu, p.parts = l.parts, p.splits = l.splits, p.split_blocks = l.split_blocks;
+  p.out = dx, p.dwg = dwg, p.dwu = dwu, p.parts = l.parts, p.splits = l.splits, p.split_steps = l.split_steps;
   p.col_tiles = tile_count(k, C::kCols);
   p.weight_rows = tile_count(k, 2 * kRows), p.weight_cols = 2 * tile_count(f, C::kCols);
   if (const int rc = D.map(&p.in[0].a, kRows)) return rc;
