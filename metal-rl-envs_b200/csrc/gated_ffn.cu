@@ -38,19 +38,27 @@ RLENV_D void activate(float g, float* y, float* slope) {
 
 // ---- operands ------------------------------------------------------------------------------------
 
-// Planes of a (rows, cols) array as bfloat16 (planes, rows, pitch), pitch a multiple of 8: for float32
-// the three whose sum it is, for bfloat16 a copy (rows that are not on 16-byte boundaries).
+// Planes of up to three (rows, cols) arrays as bfloat16 (planes, rows, pitch), pitch a multiple of 8: for
+// float32 the three whose sum it is, for bfloat16 a copy (rows that are not on 16-byte boundaries).
+struct Packing {
+  const void* from[3];
+  __nv_bfloat16* to[3];
+  int64_t rows[3], cols[3], pairs[4];  // pairs: of elements, running
+};
 template <typename T, int kPlanes>
-__global__ void __launch_bounds__(256)
-pack_kernel(const T* __restrict__ from, int64_t rows, int64_t cols, int64_t pitch, __nv_bfloat16* __restrict__ to) {
-  const int64_t pairs = pitch / 2, e = int64_t(blockIdx.x) * 256 + threadIdx.x;
-  if (e >= rows * pairs) return;
-  const int64_t r = e / pairs, c = e % pairs * 2;
-  float lo = c < cols ? float(from[r * cols + c]) : 0.0f, hi = c + 1 < cols ? float(from[r * cols + c + 1]) : 0.0f;
+__global__ void __launch_bounds__(256) pack_kernel(const __grid_constant__ Packing p) {
+  const int64_t i = int64_t(blockIdx.x) * 256 + threadIdx.x;
+  if (i >= p.pairs[3]) return;
+  const int a = i < p.pairs[1] ? 0 : i < p.pairs[2] ? 1 : 2;
+  const int64_t rows = p.rows[a], cols = p.cols[a], pitch = (cols + 7) / 8 * 8, e = i - p.pairs[a];
+  const int64_t r = e / (pitch / 2), c = e % (pitch / 2) * 2;
+  const T* from = static_cast<const T*>(p.from[a]) + r * cols + c;
+  __nv_bfloat16* to = p.to[a] + r * pitch + c;
+  float lo = c < cols ? float(from[0]) : 0.0f, hi = c + 1 < cols ? float(from[1]) : 0.0f;
 #pragma unroll
   for (int q = 0; q < kPlanes; ++q) {
     const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
-    *reinterpret_cast<__nv_bfloat162*>(to + (q * rows + r) * pitch + c) = v;
+    *reinterpret_cast<__nv_bfloat162*>(to + q * rows * pitch) = v;
     lo -= __low2float(v), hi -= __high2float(v);
   }
 }
@@ -61,8 +69,6 @@ enum Op { kForward, kGates, kGradients };  // h; dg and du; dx, dWg and dWu
 
 constexpr int kRows = 128;       // of a tile, in each block of a pair
 constexpr int kBlock = 64;       // of the contraction: a tile row's 128 bytes
-constexpr int kProductThreads = 384;  // copies, products, two idle warps, eight warps of epilogue
-constexpr int kEpilogueWarps = 8;
 constexpr int kTmemColumns = 512;
 constexpr int kStageFloats = 32 * 32;  // the epilogue's tile of a warp
 
@@ -73,6 +79,11 @@ struct Tile {
   static constexpr int kPairs = kFloat ? 6 : 1;  // products of planes
   static constexpr int kCols = kFloat ? 128 : 256;
   static constexpr int kHalf = kCols / 2;        // columns of B in each block
+  // Warps: copies, products, two idle ones, and those of the epilogue. float32's, with the exact exponential
+  // and error function and three planes to store, needs twice as many to hide its latencies.
+  static constexpr int kEpilogue = kFloat ? 16 : 8;
+  static constexpr int kThreads = 128 + 32 * kEpilogue;
+  static constexpr int kMine = kCols / (kEpilogue / 4);  // columns of the accumulator that a thread reads
   // A ring buffer's blocks: float32's narrower products are over sooner, and two blocks keep the turn of a
   // step, some 300 cycles of waiting and committing, below the products' time.
   static constexpr int kBlocks = kFloat ? 2 : 1;
@@ -80,10 +91,10 @@ struct Tile {
   static constexpr int kABytes = kRows * kBlock * 2;
   static constexpr int kBlockBytes = kABytes + kHalf * kBlock * 2;
   static constexpr int kRingBytes = kBlocks * kBlockBytes;
-  static constexpr int kStages = kFloat ? 4 : 6;
+  static constexpr int kStages = kFloat ? 3 : 6;
   static constexpr int kStageAt = kStages * kRingBytes;  // the epilogue's 32 x 32 tiles, one a warp
   // the ring starts on a 1,024-byte boundary
-  static constexpr int kSmem = kStageAt + kEpilogueWarps * kStageFloats * 4 + 1024;
+  static constexpr int kSmem = kStageAt + kEpilogue * kStageFloats * 4 + 1024;
   // Steps of the contraction summed in tensor memory before the epilogue takes them out into registers
   // (float32 only). The tensor core truncates as it accumulates; rounded additions of short sums keep
   // float32 results at float32's error. Of the products of planes only the leading one, the last to be
@@ -316,7 +327,7 @@ RLENV_D void finish(const Product& p, const Work& w, int64_t r0, int64_t c, cons
 }
 
 template <typename T, int kOp>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kProductThreads, 1)
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Tile<T>::kThreads, 1)
 product_kernel(const __grid_constant__ Product p, int items) {
   using C = Tile<T>;
   constexpr bool kPaired = kOp != kGradients;  // half of a tile's columns are gates, half ups
@@ -333,7 +344,7 @@ product_kernel(const __grid_constant__ Product p, int items) {
   const int rank = int(bw::cluster_rank());
   if (threadIdx.x == 0) {
     for (int i = 0; i < C::kStages; ++i) bw::barrier_init(full + 8 * i, 1), bw::barrier_init(empty + 8 * i, 1);
-    for (int i = 0; i < 2; ++i) bw::barrier_init(summed + 8 * i, 1), bw::barrier_init(taken + 8 * i, 2 * kEpilogueWarps);
+    for (int i = 0; i < 2; ++i) bw::barrier_init(summed + 8 * i, 1), bw::barrier_init(taken + 8 * i, 2 * C::kEpilogue);
     dead_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -439,10 +450,9 @@ product_kernel(const __grid_constant__ Product p, int items) {
       }
     }
   } else if (warp >= 4) {
-    const int quarter = warp & 3, half = (warp - 4) >> 2;
+    const int quarter = warp & 3, part = (warp - 4) >> 2;
     float* const own_stage = reinterpret_cast<float*>(raw + (ring - bw::shared_at(raw)) + C::kStageAt) +
                              (warp - 4) * kStageFloats;
-    constexpr int kMine = C::kCols / 2;  // columns of the accumulator that a thread reads
     int buffer = 0;
     uint32_t buffer_phase = 0;
     bool ok = true;
@@ -454,8 +464,8 @@ product_kernel(const __grid_constant__ Product p, int items) {
       if (++buffer == 2) buffer = 0, buffer_phase ^= 1;
     };
     // Run j of 32 columns of this thread's, as two of 16: a gated tile's are gates and ups.
-    const auto column = [&](int j) { return kPaired ? half * (C::kHalf / 2) + 16 * j : half * kMine + 32 * j; };
-    constexpr int kRuns = kMine / 32;
+    const auto column = [&](int j) { return kPaired ? part * (C::kMine / 2) + 16 * j : part * C::kMine + 32 * j; };
+    constexpr int kRuns = C::kMine / 32;
     const auto load_run = [&](uint32_t (&v)[32], int j) {
       const uint32_t at = tmem + lanes + buffer * C::kCols + column(j);
       bw::tmem_load16x2(v, at, at + (kPaired ? C::kHalf : 16));
@@ -715,17 +725,26 @@ Layout lay_out(int dtype, int64_t m, int64_t k, int64_t f, bool backward, void* 
   return l;
 }
 
+// The operands of the caller's arrays, the ones that need it packed in one launch.
 template <typename T>
-int operand(const void* from, int64_t rows, int64_t cols, void* packed, cudaStream_t s, Operand* o) {
+int operands(const void* const (&from)[3], const int64_t (&rows)[3], const int64_t (&cols)[3], void* const (&packed)[3],
+             cudaStream_t s, Operand (&o)[3]) {
   constexpr int kPlanes = Tile<T>::kPlanes;
-  if (!packed) {
-    *o = {static_cast<const __nv_bfloat16*>(from), rows, cols, cols, 1};
-    return RLENV_OK;
+  Packing p{};
+  for (int i = 0; i < 3; ++i) {
+    p.pairs[i + 1] = p.pairs[i];
+    if (!packed[i]) {
+      o[i] = {static_cast<const __nv_bfloat16*>(from[i]), rows[i], cols[i], cols[i], 1};
+      continue;
+    }
+    const int64_t pitch = round_up(cols[i], 8);
+    p.from[i] = from[i], p.to[i] = static_cast<__nv_bfloat16*>(packed[i]);
+    p.rows[i] = rows[i], p.cols[i] = cols[i], p.pairs[i + 1] += rows[i] * (pitch / 2);
+    o[i] = {p.to[i], rows[i], cols[i], pitch, kPlanes};
   }
-  const int64_t pitch = round_up(cols, 8), pairs = rows * (pitch / 2);
-  pack_kernel<T, kPlanes><<<unsigned((pairs + 255) / 256), 256, 0, s>>>(static_cast<const T*>(from), rows, cols, pitch,
-                                                                       static_cast<__nv_bfloat16*>(packed));
-  *o = {static_cast<const __nv_bfloat16*>(packed), rows, cols, pitch, kPlanes};
+  if (p.pairs[3] == 0) return RLENV_OK;
+  if ((p.pairs[3] + 255) / 256 > 0x7fffffff) return RLENV_EINVAL;
+  pack_kernel<T, kPlanes><<<grid_for(p.pairs[3], 256), 256, 0, s>>>(p);
   return launch_status();
 }
 
@@ -740,7 +759,7 @@ int run_product(const Product& p, cudaStream_t s) {
   if (cudaError_t e = cudaFuncSetAttribute(product_kernel<T, kOp>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem))
     return int(e);
   const int grid = 2 * int(items < sms / 2 ? items : sms / 2);
-  product_kernel<T, kOp><<<grid, kProductThreads, C::kSmem, s>>>(p, int(items));
+  product_kernel<T, kOp><<<grid, C::kThreads, C::kSmem, s>>>(p, int(items));
   return launch_status();
 }
 
@@ -755,10 +774,9 @@ int ffn(const void* dh, const void* x, const void* wg, const void* wu, int64_t m
            : m == 2 ? few_rows<T, 2>(x, wg, wu, m, k, f, act, out, s)
            : m <= 4 ? few_rows<T, 4>(x, wg, wu, m, k, f, act, out, s)
                     : few_rows<T, 8>(x, wg, wu, m, k, f, act, out, s);
-  Operand X, G, U;
-  if (const int rc = operand<T>(x, m, k, l.x, s, &X)) return rc;
-  if (const int rc = operand<T>(wg, k, f, l.wg, s, &G)) return rc;
-  if (const int rc = operand<T>(wu, k, f, l.wu, s, &U)) return rc;
+  Operand in[3];
+  if (const int rc = operands<T>({x, wg, wu}, {m, k, k}, {k, f, f}, {l.x, l.wg, l.wu}, s, in)) return rc;
+  const Operand &X = in[0], &G = in[1], &U = in[2];
   Product p{};
   p.m = m, p.k = k, p.f = f, p.act = act, p.out = out, p.dh = dh;
   p.gates = static_cast<__nv_bfloat16*>(l.gates), p.pitch = round_up(f, 8);
