@@ -39,27 +39,34 @@ RLENV_D void activate(float g, float* y, float* slope) {
 // ---- operands ------------------------------------------------------------------------------------
 
 // Planes of up to three (rows, cols) arrays as bfloat16 (planes, rows, pitch), pitch a multiple of 8: for
-// float32 the three whose sum it is, for bfloat16 a copy (rows that are not on 16-byte boundaries).
+// float32 the three whose sum it is, for bfloat16 a copy (rows that are not on 16-byte boundaries). A warp takes
+// a run of kPackRun columns of a row, a lane pairs of its elements.
+constexpr int kPackRun = 512;
 struct Packing {
   const void* from[3];
   __nv_bfloat16* to[3];
-  int64_t rows[3], cols[3], pairs[4];  // pairs: of elements, running
+  int64_t rows[3], cols[3], runs[4];  // runs: running
 };
 template <typename T, int kPlanes>
 __global__ void __launch_bounds__(256) pack_kernel(const __grid_constant__ Packing p) {
-  const int64_t i = int64_t(blockIdx.x) * 256 + threadIdx.x;
-  if (i >= p.pairs[3]) return;
-  const int a = i < p.pairs[1] ? 0 : i < p.pairs[2] ? 1 : 2;
-  const int64_t rows = p.rows[a], cols = p.cols[a], pitch = (cols + 7) / 8 * 8, e = i - p.pairs[a];
-  const int64_t r = e / (pitch / 2), c = e % (pitch / 2) * 2;
-  const T* from = static_cast<const T*>(p.from[a]) + r * cols + c;
-  __nv_bfloat16* to = p.to[a] + r * pitch + c;
-  float lo = c < cols ? float(from[0]) : 0.0f, hi = c + 1 < cols ? float(from[1]) : 0.0f;
+  const int64_t i = int64_t(blockIdx.x) * 8 + (threadIdx.x >> 5);
+  if (i >= p.runs[3]) return;
+  const int a = i < p.runs[1] ? 0 : i < p.runs[2] ? 1 : 2;
+  const int64_t rows = p.rows[a], cols = p.cols[a], pitch = (cols + 7) / 8 * 8;
+  const uint32_t a_row = uint32_t((pitch + kPackRun - 1) / kPackRun);
+  const int64_t run = i - p.runs[a], r = a_row == 1 ? run : run / a_row, c0 = a_row == 1 ? 0 : run % a_row * kPackRun;
+  const T* from = static_cast<const T*>(p.from[a]) + r * cols;
+  __nv_bfloat16* to = p.to[a] + r * pitch;
+  const int64_t end = c0 + kPackRun < pitch ? c0 + kPackRun : pitch;
+#pragma unroll 4
+  for (int64_t c = c0 + 2 * (threadIdx.x & 31); c < end; c += 64) {
+    float lo = c < cols ? float(from[c]) : 0.0f, hi = c + 1 < cols ? float(from[c + 1]) : 0.0f;
 #pragma unroll
-  for (int q = 0; q < kPlanes; ++q) {
-    const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
-    *reinterpret_cast<__nv_bfloat162*>(to + q * rows * pitch) = v;
-    lo -= __low2float(v), hi -= __high2float(v);
+    for (int q = 0; q < kPlanes; ++q) {
+      const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+      *reinterpret_cast<__nv_bfloat162*>(to + q * rows * pitch + c) = v;
+      lo -= __low2float(v), hi -= __high2float(v);
+    }
   }
 }
 
@@ -112,9 +119,10 @@ struct alignas(64) Product {
   // Tiles: of h or the gates; of dx and of both weights.
   int row_tiles, col_tiles, weight_rows, weight_cols;
   int splits, split_steps;   // of the contraction over tokens in the weights' gradients
+  int dx_splits, dx_split_steps;  // of that over F in dx
   const void* dh;            // kGates
   void *out, *dwg, *dwu;     // h or dx; the weights' gradients
-  float* parts;              // (splits, 2, K, F) where splits > 1
+  float *parts, *dx_parts;   // (splits, 2, K, F) where splits > 1, (dx_splits, M, K) where dx_splits > 1
   __nv_bfloat16* gates;      // (plane, dg or du, M, pitch)
   int64_t pitch;
   bool wide;                 // rows of h and dh start on the boundaries of fours
@@ -147,7 +155,10 @@ RLENV_D Work work_of(const Product& p, int item) {
       w.steps = min(p.split_steps, int((p.m + kStep - 1) / kStep) - w.k0);
     } else {
       item -= per * p.splits;
-      w.segs = 2, w.steps = int((p.f + kStep - 1) / kStep);
+      const int tiles = rows * cols;
+      w.split = item / tiles, item %= tiles;
+      w.k0 = w.split * p.dx_split_steps;
+      w.segs = 2, w.steps = min(p.dx_split_steps, int((p.f + kStep - 1) / kStep) - w.k0);
     }
   } else {
     w.steps = int((p.k + kStep - 1) / kStep);
@@ -236,66 +247,130 @@ RLENV_D float4* stage_at(float* stage, int row, int four) {
   return reinterpret_cast<float4*>(stage) + row * 8 + (four ^ (row & 7));
 }
 // A gated tile is 16 columns of gates and their 16 ups: lane l has columns 4 (l % 4) .. + 3 of rows
-// gated_row(l) + 8 i.
+// gated_row(l) + 8 i. Where the caller's rows do not start on the boundaries of fours, its values pass through
+// the tile once more, so that a row's accesses are neighbours still: column l % 16 of rows lone_row(l, i).
 RLENV_D int gated_row(int lane) { return (lane >> 2 & 1) * 4 + (lane >> 3); }
+RLENV_D int lone_row(int lane, int i) { return (lane >> 4) * 4 + (i & 3) + (i >> 2) * 8; }
+RLENV_D float& stage_one(float* stage, int row, int col) {
+  return reinterpret_cast<float*>(stage_at(stage, row, col >> 2))[col & 3];
+}
 
-// The gradient dh of a gated tile.
+// The gradient dh of a gated tile, in a lane's order.
 template <typename T>
 RLENV_D void load_gradient(const Product& p, int64_t r0, int64_t c, typename Four<T>::type (&d)[4]) {
-  const int lane = threadIdx.x & 31, col = lane % 4 * 4;
-  const int n = int(min(int64_t(4), max(int64_t(0), p.f - c - col)));
+  const int lane = threadIdx.x & 31;
+  const T* dh = static_cast<const T*>(p.dh) + r0 * p.f + c;
+  const int rows = int(min(int64_t(32), p.m - r0)), cols = int(min(int64_t(16), p.f - c));
+  if (p.wide) {
+    const int col = lane % 4 * 4;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int64_t r = r0 + gated_row(lane) + 8 * i;
-    load_four(static_cast<const T*>(p.dh) + r * p.f + c + col, &d[i], p.wide, r < p.m ? n : 0);
+    for (int i = 0; i < 4; ++i) {
+      const int r = gated_row(lane) + 8 * i;
+      load_four(dh + r * p.f + col, &d[i], true, r < rows ? cols - col : 0);
+    }
+  } else {
+    const int col = lane % 16;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      T v[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int r = lone_row(lane, 4 * i + j);
+        v[j] = r < rows && col < cols ? dh[r * p.f + col] : T(0.0f);
+      }
+      if constexpr (sizeof(T) == 4) {
+        d[i] = make_float4(v[0], v[1], v[2], v[3]);
+      } else {
+        const __nv_bfloat162 lo = __halves2bfloat162(v[0], v[1]), hi = __halves2bfloat162(v[2], v[3]);
+        d[i] = make_uint2(*reinterpret_cast<const uint32_t*>(&lo), *reinterpret_cast<const uint32_t*>(&hi));
+      }
+    }
   }
 }
 
 template <typename T, int kOp, int kAct>
 RLENV_D void finish_gated(const Product& p, int64_t r0, int64_t c, const typename Four<T>::type (&dh)[4], float* stage) {
   constexpr bool kFast = !Tile<T>::kFloat;
-  const int lane = threadIdx.x & 31, col = lane % 4 * 4;
-  const int n = int(min(int64_t(4), p.f - c - col));
-  if (n <= 0) return;
+  const int lane = threadIdx.x & 31, col = lane % 4 * 4, lone = lane % 16;
+  const int rows = int(min(int64_t(32), p.m - r0)), cols = int(min(int64_t(16), p.f - c));
+  const int64_t plane = p.m * p.pitch;
+  float4 g[4], u[4], d[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    g[i] = *stage_at(stage, gated_row(lane) + 8 * i, lane % 4);
+    u[i] = *stage_at(stage, gated_row(lane) + 8 * i, 4 + lane % 4);
+    if constexpr (kOp == kGates) d[i] = unpack_four(dh[i]);
+  }
+  if (kOp == kGates && !p.wide) {
+    __syncwarp();
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      stage_one(stage, lone_row(lane, 4 * i), lone) = d[i].x;
+      stage_one(stage, lone_row(lane, 4 * i + 1), lone) = d[i].y;
+      stage_one(stage, lone_row(lane, 4 * i + 2), lone) = d[i].z;
+      stage_one(stage, lone_row(lane, 4 * i + 3), lone) = d[i].w;
+    }
+    __syncwarp();
+#pragma unroll
+    for (int i = 0; i < 4; ++i) d[i] = *stage_at(stage, gated_row(lane) + 8 * i, lane % 4);
+  }
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const int r = gated_row(lane) + 8 * i;
-    if (r0 + r >= p.m) return;
-    const float4 g = *stage_at(stage, r, lane % 4), u = *stage_at(stage, r, 4 + lane % 4);
     float4 y, slope;
-    activate<kFast, kAct>(g.x, &y.x, &slope.x);
-    activate<kFast, kAct>(g.y, &y.y, &slope.y);
-    activate<kFast, kAct>(g.z, &y.z, &slope.z);
-    activate<kFast, kAct>(g.w, &y.w, &slope.w);
+    activate<kFast, kAct>(g[i].x, &y.x, &slope.x);
+    activate<kFast, kAct>(g[i].y, &y.y, &slope.y);
+    activate<kFast, kAct>(g[i].z, &y.z, &slope.z);
+    activate<kFast, kAct>(g[i].w, &y.w, &slope.w);
     if constexpr (kOp == kForward) {
-      store_four(static_cast<T*>(p.out) + (r0 + r) * p.f + c + col,
-                 make_float4(y.x * u.x, y.y * u.y, y.z * u.z, y.w * u.w), p.wide, n);
-    } else {
-      const float4 d = unpack_four(dh[i]);
-      float4 dg = make_float4(d.x * u.x * slope.x, d.y * u.y * slope.y, d.z * u.z * slope.z, d.w * u.w * slope.w);
-      float4 du = make_float4(d.x * y.x, d.y * y.y, d.z * y.z, d.w * y.w);
+      g[i] = make_float4(y.x * u[i].x, y.y * u[i].y, y.z * u[i].z, y.w * u[i].w);
+      if (p.wide && r < rows) store_four(static_cast<T*>(p.out) + (r0 + r) * p.f + c + col, g[i], true, cols - col);
+    } else if (r < rows && col < cols) {
+      float4 dg = make_float4(d[i].x * u[i].x * slope.x, d[i].y * u[i].y * slope.y, d[i].z * u[i].z * slope.z,
+                              d[i].w * u[i].w * slope.w);
+      float4 du = make_float4(d[i].x * y.x, d[i].y * y.y, d[i].z * y.z, d[i].w * y.w);
       __nv_bfloat16* to = p.gates + (r0 + r) * p.pitch + c + col;  // the pitch holds whole eights
 #pragma unroll
-      for (int q = 0; q < Tile<T>::kPlanes; ++q, to += 2 * p.m * p.pitch) {
+      for (int q = 0; q < Tile<T>::kPlanes; ++q, to += 2 * plane) {
         const uint2 a = pack_four(dg), b = pack_four(du);
         *reinterpret_cast<uint2*>(to) = a;
-        *reinterpret_cast<uint2*>(to + p.m * p.pitch) = b;
+        *reinterpret_cast<uint2*>(to + plane) = b;
         const float4 x = unpack_four(a), z = unpack_four(b);
         dg.x -= x.x, dg.y -= x.y, dg.z -= x.z, dg.w -= x.w, du.x -= z.x, du.y -= z.y, du.z -= z.z, du.w -= z.w;
       }
     }
   }
+  if (kOp == kForward && !p.wide) {
+    __syncwarp();
+#pragma unroll
+    for (int i = 0; i < 4; ++i) *stage_at(stage, gated_row(lane) + 8 * i, lane % 4) = g[i];
+    __syncwarp();
+    T* const out = static_cast<T*>(p.out) + r0 * p.f + c + lone;
+#pragma unroll 8
+    for (int i = 0; i < 16; ++i) {
+      const int r = lone_row(lane, i);
+      if (r < rows && lone < cols) out[r * p.f] = T(stage_one(stage, r, lone));
+    }
+  }
 }
 template <typename T>
 RLENV_D void finish_values(T* to, int64_t pitch, int64_t rows, int64_t cols, float* stage) {
-  const int lane = threadIdx.x & 31, col = lane % 8 * 4;
-  const int n = int(min(int64_t(4), cols - col));
-  if (n <= 0) return;
+  const int lane = threadIdx.x & 31;
+  if (pitch % 4 == 0) {
+    const int col = lane % 8 * 4, n = int(min(int64_t(4), cols - col));
+    if (n <= 0) return;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const int r = lane / 8 + 4 * i;
-    if (r >= rows) return;
-    store_four(to + r * pitch + col, *stage_at(stage, r, lane % 8), pitch % 4 == 0, n);
+    for (int i = 0; i < 8; ++i) {
+      const int r = lane / 8 + 4 * i;
+      if (r >= rows) return;
+      store_four(to + r * pitch + col, *stage_at(stage, r, lane % 8), true, n);
+    }
+  } else if (lane < cols) {
+#pragma unroll 8
+    for (int r = 0; r < 32; ++r) {
+      if (r >= rows) return;
+      to[r * pitch + lane] = T(stage_one(stage, r, lane));
+    }
   }
 }
 
@@ -316,6 +391,8 @@ RLENV_D void finish(const Product& p, const Work& w, int64_t r0, int64_t c, cons
     if (w.weights && p.splits > 1)
       finish_values(p.parts + ((int64_t(w.split) * 2 + w.weight) * p.k + r0) * p.f + c, p.f, all_rows - r0,
                     all_cols - c, stage);
+    else if (!w.weights && p.dx_splits > 1)
+      finish_values(p.dx_parts + (int64_t(w.split) * p.m + r0) * p.k + c, p.k, all_rows - r0, all_cols - c, stage);
     else
       finish_values(static_cast<T*>(w.weights ? (w.weight ? p.dwu : p.dwg) : p.out) + r0 * all_cols + c, all_cols,
                     all_rows - r0, all_cols - c, stage);
@@ -544,15 +621,25 @@ product_kernel(const __grid_constant__ Product p, int items) {
   if (warp == 2) bw::tmem_free<kTmemColumns>(tmem);
 }
 
-// The weights' gradients from the sums over runs of tokens.
+// The gradients from the sums over parts of their contractions: both weights' from `splits` parts of tokens,
+// dx's from `dx_splits` parts of F (0: it is whole already).
 template <typename T>
 __global__ void __launch_bounds__(256)
-add_parts_kernel(const float* __restrict__ parts, int splits, int64_t size, T* __restrict__ dwg, T* __restrict__ dwu) {
-  const int64_t e = int64_t(blockIdx.x) * 256 + threadIdx.x;
-  if (e >= 2 * size) return;
+add_parts_kernel(const float* __restrict__ parts, int splits, int64_t size, T* __restrict__ dwg, T* __restrict__ dwu,
+                 const float* __restrict__ dx_parts, int dx_splits, int64_t dx_size, T* __restrict__ dx) {
+  int64_t e = int64_t(blockIdx.x) * 256 + threadIdx.x;
+  const int64_t weights = splits > 1 ? 2 * size : 0;
+  const bool of_dx = e >= weights;
+  if (of_dx) e -= weights;
+  if (of_dx && (dx_splits <= 1 || e >= dx_size)) return;
+  const float* from = of_dx ? dx_parts : parts;
+  const int64_t stride = of_dx ? dx_size : 2 * size;
+  const int count = of_dx ? dx_splits : splits;
   float sum = 0.0f;
-  for (int s = 0; s < splits; ++s) sum += __ldg(parts + s * 2 * size + e);
-  (e < size ? dwg : dwu)[e < size ? e : e - size] = T(sum);
+#pragma unroll 4
+  for (int s = 0; s < count; ++s) sum += __ldg(from + s * stride + e);
+  T* to = of_dx ? dx : e < size ? dwg : dwu;
+  to[!of_dx && e >= size ? e - size : e] = T(sum);
 }
 
 // ---- few rows ----------------------------------------------------------------------------------------
@@ -686,28 +773,31 @@ int64_t planes(int dtype) { return dtype == RLENV_F32 ? 3 : 1; }
 
 struct Layout {  // scratch of a call
   void *x, *wg, *wu, *gates;
-  float* parts;
-  int splits, split_steps;
+  float *parts, *dx_parts;
+  int splits, split_steps, dx_splits, dx_split_steps;
   int64_t bytes;
 };
 
 constexpr int kPairsOfSms = 74;
 constexpr int64_t kFewestSteps = 8;
 
-// The contraction over tokens of the weights' gradients is split where a tile of them would take longer
-// than a pair of SMs' share of all the work: a small block's weights are a few tiles, each a sum over every
-// token. The sums of each run of tokens are kept in float32 and added up in order.
-void split_tokens(int dtype, int64_t m, int64_t k, int64_t f, Layout* l) {
+// The gradients' contractions are split where a tile would take longer than a pair of SMs' share of all the
+// work: a small block's weights are a few tiles, each a sum over every token; few tokens' dx a few, each a sum
+// over all of F. The parts' sums are kept in float32 and added up in order.
+void split_gradients(int dtype, int64_t m, int64_t k, int64_t f, Layout* l) {
   const int64_t wide = dtype == RLENV_F32 ? Tile<float>::kCols : Tile<__nv_bfloat16>::kCols, high = 2 * kRows;
   const int64_t step = dtype == RLENV_F32 ? Tile<float>::kStep : Tile<__nv_bfloat16>::kStep;
   const int64_t steps = (m + step - 1) / step, tiles = (k + high - 1) / high * ((f + wide - 1) / wide) * 2;
-  const int64_t dx = (m + high - 1) / high * ((k + wide - 1) / wide) * 2 * ((f + step - 1) / step);
-  int64_t share = (tiles * steps + dx) / kPairsOfSms;
+  const int64_t dx_steps = (f + step - 1) / step, dx_tiles = (m + high - 1) / high * ((k + wide - 1) / wide);
+  int64_t share = (tiles * steps + 2 * dx_tiles * dx_steps) / kPairsOfSms;
   if (share < kFewestSteps) share = kFewestSteps;
-  int64_t splits = (steps + share - 1) / share;
-  if (splits < 1) splits = 1;
-  l->split_steps = int((steps + splits - 1) / splits);
-  l->splits = int((steps + l->split_steps - 1) / l->split_steps);
+  const auto split = [](int64_t all, int64_t most, int* count, int* each) {
+    const int64_t parts = (all + most - 1) / most;
+    *each = int((all + parts - 1) / parts);
+    *count = int((all + *each - 1) / *each);
+  };
+  split(steps, share, &l->splits, &l->split_steps);
+  split(dx_steps, (share + 1) / 2, &l->dx_splits, &l->dx_split_steps);
 }
 Layout lay_out(int dtype, int64_t m, int64_t k, int64_t f, bool backward, void* scratch) {
   Scratch s{static_cast<unsigned char*>(scratch), 0};
@@ -718,8 +808,9 @@ Layout lay_out(int dtype, int64_t m, int64_t k, int64_t f, bool backward, void* 
   if (packs(dtype, f)) l.wg = s.take(n * k * round_up(f, 8) * 2), l.wu = s.take(n * k * round_up(f, 8) * 2);
   if (backward) {
     l.gates = s.take(2 * n * m * round_up(f, 8) * 2);
-    if (m > 0 && k > 0 && f > 0) split_tokens(dtype, m, k, f, &l);
+    if (m > 0 && k > 0 && f > 0) split_gradients(dtype, m, k, f, &l);
     if (l.splits > 1) l.parts = static_cast<float*>(s.take(int64_t(l.splits) * 2 * k * f * 4));
+    if (l.dx_splits > 1) l.dx_parts = static_cast<float*>(s.take(int64_t(l.dx_splits) * m * k * 4));
   }
   l.bytes = s.used;
   return l;
@@ -732,26 +823,27 @@ int operands(const void* const (&from)[3], const int64_t (&rows)[3], const int64
   constexpr int kPlanes = Tile<T>::kPlanes;
   Packing p{};
   for (int i = 0; i < 3; ++i) {
-    p.pairs[i + 1] = p.pairs[i];
+    p.runs[i + 1] = p.runs[i];
     if (!packed[i]) {
       o[i] = {static_cast<const __nv_bfloat16*>(from[i]), rows[i], cols[i], cols[i], 1};
       continue;
     }
     const int64_t pitch = round_up(cols[i], 8);
     p.from[i] = from[i], p.to[i] = static_cast<__nv_bfloat16*>(packed[i]);
-    p.rows[i] = rows[i], p.cols[i] = cols[i], p.pairs[i + 1] += rows[i] * (pitch / 2);
+    p.rows[i] = rows[i], p.cols[i] = cols[i], p.runs[i + 1] += rows[i] * ((pitch + kPackRun - 1) / kPackRun);
     o[i] = {p.to[i], rows[i], cols[i], pitch, kPlanes};
   }
-  if (p.pairs[3] == 0) return RLENV_OK;
-  if ((p.pairs[3] + 255) / 256 > 0x7fffffff) return RLENV_EINVAL;
-  pack_kernel<T, kPlanes><<<grid_for(p.pairs[3], 256), 256, 0, s>>>(p);
+  if (p.runs[3] == 0) return RLENV_OK;
+  if ((p.runs[3] + 7) / 8 > 0x7fffffff) return RLENV_EINVAL;
+  pack_kernel<T, kPlanes><<<grid_for(p.runs[3], 8), 256, 0, s>>>(p);
   return launch_status();
 }
 
 template <typename T, int kOp>
 int run_product(const Product& p, cudaStream_t s) {
   using C = Tile<T>;
-  const int64_t items = int64_t(p.row_tiles) * p.col_tiles + int64_t(p.weight_rows) * p.weight_cols * p.splits;
+  const int64_t items = int64_t(p.row_tiles) * p.col_tiles * (kOp == kGradients ? p.dx_splits : 1) +
+                        int64_t(p.weight_rows) * p.weight_cols * p.splits;
   if (items > 0x7fffffff) return RLENV_EINVAL;
   int dev = 0, sms = 0;
   if (cudaError_t e = cudaGetDevice(&dev)) return int(e);
@@ -789,6 +881,7 @@ int ffn(const void* dh, const void* x, const void* wg, const void* wu, int64_t m
   if (const int rc = run_product<T, kGates>(p, s)) return rc;
   const Operand D{p.gates, m, f, p.pitch, 2 * C::kPlanes};
   p.out = dx, p.dwg = dwg, p.dwu = dwu, p.parts = l.parts, p.splits = l.splits, p.split_steps = l.split_steps;
+  p.dx_parts = l.dx_parts, p.dx_splits = l.dx_splits, p.dx_split_steps = l.dx_split_steps;
   p.col_tiles = tile_count(k, C::kCols);
   p.weight_rows = tile_count(k, 2 * kRows), p.weight_cols = 2 * tile_count(f, C::kCols);
   if (const int rc = D.map(&p.in[0].a, kRows)) return rc;
@@ -797,9 +890,10 @@ int ffn(const void* dh, const void* x, const void* wg, const void* wu, int64_t m
   if (const int rc = X.map(&p.in[1].a, 64)) return rc;
   if (const int rc = D.map(&p.in[1].b0, 64)) return rc;
   if (const int rc = run_product<T, kGradients>(p, s)) return rc;
-  if (l.splits == 1) return RLENV_OK;
-  add_parts_kernel<T><<<grid_for(2 * k * f, 256), 256, 0, s>>>(l.parts, l.splits, k * f, static_cast<T*>(dwg),
-                                                               static_cast<T*>(dwu));
+  const int64_t sums = (l.splits > 1 ? 2 * k * f : 0) + (l.dx_splits > 1 ? m * k : 0);
+  if (sums == 0) return RLENV_OK;
+  add_parts_kernel<T><<<grid_for(sums, 256), 256, 0, s>>>(l.parts, l.splits, k * f, static_cast<T*>(dwg), static_cast<T*>(dwu),
+                                                         l.dx_parts, l.dx_splits, m * k, static_cast<T*>(dx));
   return launch_status();
 }
 
