@@ -26,23 +26,24 @@ chunk_kernel(const __grid_constant__ Problem p, const __grid_constant__ Split sp
   using C = Shape<T, D>;
   constexpr int DB = C::DB, kTiles = D / DB;
   extern __shared__ __align__(16) unsigned char smem[];
-  __shared__ float decays[kChunk];  // g^(64 - f - j)
+  __shared__ float powers[kChunk + 17];  // of the decay
   __nv_bfloat16* const tiles = reinterpret_cast<__nv_bfloat16*>(smem);
   __nv_bfloat16* const S = tiles + C::kBuffers * C::kTiles;
   constexpr int kAAt = C::kIn * C::kX, kBAt = 2 * C::kIn * C::kX;  // x, a and b in a buffer
 
-  int64_t id = blockIdx.x;
+  uint32_t id = blockIdx.x;  // the counts that make it up are below 2^31 as it is
   const int col = int(id % kTiles) * DB;
   id /= kTiles;
-  const int64_t scan = id % p.scans;
+  const uint32_t scan = p.scans == 1 ? 0 : id % p.scans;
   const Scan& s = p.scan[scan];
   id /= p.scans;
-  const int64_t segment = id % split.segments, seq = id / split.segments;
-  const int64_t n = seq / p.h, h = seq % p.h;
-  const int64_t slot = (scan * p.n * p.h + seq) * split.segments + segment;
+  const uint32_t segments = uint32_t(split.segments), seq = segments == 1 ? id : id / segments;
+  const int64_t segment = id - seq * segments;
+  const int64_t n = seq / uint32_t(p.h), h = seq % uint32_t(p.h);
+  const int64_t slot = (scan * p.n * p.h + seq) * segments + segment;
   const int64_t first = segment * split.per * kChunk;
   const int64_t last = first + split.per * kChunk < p.t ? first + split.per * kChunk : p.t;
-  const bool whole = split.segments == 1;
+  const bool whole = segments == 1;
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int rb = warp % C::kRowWarps * C::RT;         // this warp's first 16 tokens,
@@ -50,8 +51,7 @@ chunk_kernel(const __grid_constant__ Problem p, const __grid_constant__ Split sp
   const int gr = lane >> 2, gc = (lane & 3) * 2;      // a fragment's row and column
   const float log2_g = log2f(__ldg(p.decay + h));
   const int f = s.reverse ? 0 : 1;
-  for (int j = threadIdx.x; j < kChunk; j += C::kThreads) decays[j] = power(log2_g, kChunk - f - j);
-  const float chunk_decay = power(log2_g, kChunk);
+  for (int j = threadIdx.x; j < kChunk + 17; j += C::kThreads) powers[j] = power(log2_g, j);
 
   // The carry, float32 in registers: rows srow + 16 m + (gr, gr + 8), columns scol + 8 t + (gc, gc + 1).
   const int rg = warp % C::RG, cg = warp / C::RG;
@@ -60,7 +60,7 @@ chunk_kernel(const __grid_constant__ Problem p, const __grid_constant__ Split sp
   const bool fine = kLocal || C::kFloat || s.carry_out;  // a carry that goes out in float32 takes all planes
   float z[C::MT][C::NT][4];
   const float* start = kLocal ? nullptr : whole ? s.carry_in : split.carry + slot * D * D;
-  if (!kLocal && whole && start) start += seq * D * D;
+  if (!kLocal && whole && start) start += int64_t(seq) * D * D;
   const bool turned = whole && s.turned;
   const float start_mul = whole ? s.in_mul : 1.0f;
 #pragma unroll
@@ -72,23 +72,6 @@ chunk_kernel(const __grid_constant__ Problem p, const __grid_constant__ Split sp
         const int r = srow + 16 * m + gr + (q & 2) * 4, c = col + scol + 8 * t + gc + (q & 1);
         z[m][t][q] = start && holds ? start_mul * __ldg(start + (turned ? c * D + r : r * D + c)) : 0.0f;
       }
-
-  // The weights, `scale` among them, between 16 tokens and 16 others: on the diagonal, and one block to its
-  // left; and from the carry to this warp's tokens.
-  float near[8], next[8], row_decay[C::RT][2];
-  if constexpr (!kLocal) {
-#pragma unroll
-    for (int q = 0; q < 8; ++q) {
-      const int apart = gr + (q & 2) * 4 - (gc + (q & 1) + (q & 4) * 2);
-      near[q] = apart >= 0 ? p.scale * power(log2_g, apart) : 0.0f;
-      next[q] = p.scale * power(log2_g, 16 + apart);
-    }
-#pragma unroll
-    for (int r = 0; r < C::RT; ++r)
-#pragma unroll
-      for (int half = 0; half < 2; ++half) row_decay[r][half] = p.scale * power(log2_g, 16 * (rb + r) + gr + 8 * half + f);
-  }
-  const float block_decay = power(log2_g, 16);
 
   using LoadX = TileLoader<T, D, C::PX, C::kX, C::kThreads>;
   using LoadB = TileLoader<T, DB, C::PB, C::kB, C::kThreads>;
@@ -125,17 +108,39 @@ chunk_kernel(const __grid_constant__ Problem p, const __grid_constant__ Split sp
   T* out_at;
   {
     const int64_t i = first + 16 * rb + lane / kPieces;
-    out_at = static_cast<T*>(s.out) + (s.reverse ? p.t - 1 - i : i) * token_step + seq * D + col + oc + lane % kPieces * kPer;
+    out_at = static_cast<T*>(s.out) + (s.reverse ? p.t - 1 - i : i) * token_step + int64_t(seq) * D + col + oc + lane % kPieces * kPer;
   }
   if (p.resets && first < last) read_resets(first);
   constexpr bool kAhead = C::kFloat || C::kBuffers == 2;  // tiles set out a chunk ahead
   if (kAhead && first < last) set_out(first, tiles);
+  __syncthreads();  // the powers are there
+
+  // The weights, `scale` among them, between 16 tokens and 16 others: on the diagonal, and one block to its
+  // left; and from the carry to this warp's tokens.
+  float near[8], next[8], row_decay[C::RT][2];
+  if constexpr (!kLocal) {
+#pragma unroll
+    for (int q = 0; q < 8; ++q) {
+      const int apart = gr + (q & 2) * 4 - (gc + (q & 1) + (q & 4) * 2);
+      near[q] = apart >= 0 ? p.scale * powers[apart] : 0.0f;
+      next[q] = p.scale * powers[16 + apart];
+    }
+#pragma unroll
+    for (int r = 0; r < C::RT; ++r)
+#pragma unroll
+      for (int half = 0; half < 2; ++half) row_decay[r][half] = p.scale * powers[16 * (rb + r) + gr + 8 * half + f];
+  }
+  const float block_decay = powers[16];
+
 
   float bad = 0.0f;      // NaN once any value is not finite
   bool cut = false;      // a reset anywhere in the segment
   int buffer = 0;
   for (int64_t i0 = first; i0 < last; i0 += kChunk) {
     const int len = int(last - i0 < kChunk ? last - i0 : kChunk);
+    // Blocks of 16 tokens that hold any; wide heads, whose time goes with the carry, work on all four and keep
+    // their loops straight.
+    const int live = D <= 32 || (C::kFloat && D == 64) ? (len + 15) / 16 : kChunk / 16;
     __nv_bfloat16* const X = tiles + buffer * C::kTiles;
     __nv_bfloat16* const A = X + kAAt;
     __nv_bfloat16* const B = X + kBAt;
@@ -184,7 +189,7 @@ chunk_kernel(const __grid_constant__ Problem p, const __grid_constant__ Split sp
       if (p.resets) read_resets(next_chunk);
     }
 
-    if constexpr (!kLocal) {
+    if (!kLocal && rb < live) {
       float o[C::RT][C::OC / 8][4];
 #pragma unroll
       for (int r = 0; r < C::RT; ++r)
@@ -239,7 +244,7 @@ chunk_kernel(const __grid_constant__ Problem p, const __grid_constant__ Split sp
       float far[C::RT];
 #pragma unroll
       for (int r = 0; r < C::RT; ++r) far[r] = 1.0f;
-      for (int jb = rb + C::RT - 1; jb >= 0; --jb) {
+      for (int jb = min(rb + C::RT, live) - 1; jb >= 0; --jb) {
         float w[C::RT][2][4] = {}, w_odd[C::RT][2][4] = {};  // even and odd steps of the sum side by side
 #pragma unroll
         for (int k = 0; k < D / 16; ++k) {
@@ -316,13 +321,12 @@ chunk_kernel(const __grid_constant__ Problem p, const __grid_constant__ Split sp
             *reinterpret_cast<uint4*>(out_at + e * kRowsOut * out_step) =
                 *reinterpret_cast<const uint4*>(own + r * C::PX + lane % kPieces * kPer);
         }
-        out_at += kChunk * out_step;
       } else {
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
           const int row = 16 * rb + gr + 8 * half;
           const int64_t i = i0 + row;
-          T* const at = static_cast<T*>(s.out) + (s.reverse ? p.t - 1 - i : i) * token_step + seq * D + col + oc + gc;
+          T* const at = static_cast<T*>(s.out) + (s.reverse ? p.t - 1 - i : i) * token_step + int64_t(seq) * D + col + oc + gc;
           if (row < len) {
 #pragma unroll
             for (int t = 0; t < C::OC / 8; ++t) {
@@ -337,11 +341,13 @@ chunk_kernel(const __grid_constant__ Problem p, const __grid_constant__ Split sp
       }
     }
 
+    out_at += kChunk * out_step;
+
     // Z <- g^L Z + (l * A)' B, l_j = g^(L - f - j) where no reset lies between token j and the end
     if (holds) {
       bool none = true;
       const int reached = resets ? linked_from(~uint64_t(0), &none) : 0;
-      const float through = len == kChunk ? chunk_decay : power(log2_g, len);
+      const float through = powers[len];
 #pragma unroll
       for (int m = 0; m < C::MT; ++m)
 #pragma unroll
@@ -352,11 +358,12 @@ chunk_kernel(const __grid_constant__ Problem p, const __grid_constant__ Split sp
       const uint32_t bt = shared_address(B + (lane & 15) * C::PB + (lane >> 4) * 8 + scol);
 #pragma unroll
       for (int j = 0; j < kChunk / 16; ++j) {
+        if (j >= live) break;
         float l[4];
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
           const int i = 16 * j + gc + (q & 1) + (q & 2) * 4;
-          l[q] = i >= reached && i < len ? decays[i + kChunk - len] : 0.0f;
+          l[q] = i >= reached && i < len ? powers[len - f - i] : 0.0f;
         }
         uint32_t key[C::MT][C::kKeys][4];
 #pragma unroll
@@ -396,7 +403,7 @@ chunk_kernel(const __grid_constant__ Problem p, const __grid_constant__ Split sp
     for (int t = 0; t < C::NT; ++t)
 #pragma unroll
       for (int q = 0; q < 4; ++q) bad = fmaf(z[m][t][q], 0.0f, bad);
-  float* const end = kLocal ? split.carry + slot * D * D : whole && s.carry_out ? s.carry_out + seq * D * D : nullptr;
+  float* const end = kLocal ? split.carry + slot * D * D : whole && s.carry_out ? s.carry_out + int64_t(seq) * D * D : nullptr;
   const bool end_turned = !kLocal && s.turned;
   const float end_mul = kLocal ? 1.0f : s.out_mul;
   if (kLocal && threadIdx.x == 0 && col == 0) split.through[slot] = cut ? -1.0f : power(log2_g, last - first);
