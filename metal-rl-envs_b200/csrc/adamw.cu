@@ -32,7 +32,10 @@ constexpr int kStateBlock = 256;
 constexpr int kAdamThreads = 256;
 constexpr int kAdamTensors = 96;    // tensors per launch: their table travels in the launch's parameters
 
-constexpr int kAdamPerSm = 3, kSms = 148;  // blocks of threads
+// Blocks of threads on an SM: 8-bit moments, bound by instructions, want as many as their registers allow (213 us
+// against 217 with three, 228 with two, for 60 M parameters); 32-bit ones, bound by memory, two, with more in
+// flight each (277 us against 289 with three, 314 with four).
+constexpr int kPerSm[2] = {2, 4}, kSms = 148;  // 32 bits, 8 bits
 
 struct AdamTensor {
   float* p;
@@ -192,7 +195,7 @@ RLENV_D void unpack(const float4& x, float* to) { to[0] = x.x, to[1] = x.y, to[2
 // A warp takes every stride-th state block and reads one ahead: a block's arithmetic, some 80 instructions an
 // element with 8-bit moments, runs under the next one's loads.
 template <typename G, bool kEight>
-__global__ void __launch_bounds__(kAdamThreads, kAdamPerSm) adamw_kernel(const __grid_constant__ AdamArgs a) {
+__global__ void __launch_bounds__(kAdamThreads, kPerSm[kEight]) adamw_kernel(const __grid_constant__ AdamArgs a) {
   const int lane = threadIdx.x & 31;
   const uint32_t stride = gridDim.x * (kAdamThreads / 32), end = a.t[0].first + a.blocks;
   uint32_t block = a.t[0].first + blockIdx.x * (kAdamThreads / 32) + (threadIdx.x >> 5);
@@ -332,7 +335,7 @@ bool on_boundary(const void* p, int bytes) { return reinterpret_cast<uintptr_t>(
 
 template <typename G, bool kEight>
 int adamw_launch(const AdamArgs& a, cudaStream_t stream) {
-  constexpr uint32_t kWarps = kAdamThreads / 32, kMost = kSms * kAdamPerSm;
+  constexpr uint32_t kWarps = kAdamThreads / 32, kMost = kSms * kPerSm[kEight];
   const uint32_t grid = (a.blocks + kWarps - 1) / kWarps < kMost ? (a.blocks + kWarps - 1) / kWarps : kMost;
   adamw_kernel<G, kEight><<<grid, kAdamThreads, 0, stream>>>(a);
   return launch_status();
