@@ -111,9 +111,11 @@ def step(params, grads, state, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_dec
     if grad_dtype not in _rl.FLOAT_DTYPES:
         raise ValueError(f"grads must be float32 or bfloat16; got {grad_dtype}")
     _check_list("params", params, torch.float32, sizes, index)
-    if not all(map(_dense, grads)):
+    try:
+        _check_list("grads", grads, grad_dtype, sizes, index)
+    except ValueError:  # a gradient with strides is copied; anything else raises here
         grads = [g.contiguous() for g in grads]
-    _check_list("grads", grads, grad_dtype, sizes, index)
+        _check_list("grads", grads, grad_dtype, sizes, index)
     if copies is not None:
         _check_list("copies", copies, torch.bfloat16, sizes, index)
     if grad_scale is not None:

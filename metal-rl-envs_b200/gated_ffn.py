@@ -24,19 +24,23 @@ def _dense(x):
 
 
 def _check(x, w_gate, w_up, activation, grad_out=None):
+    """(M, K, F, the type's code, the device's index). What fits passes on a few comparisons; what does not is
+    looked at again for the message."""
     _rl.as_floats("x", x)
+    index, dtype = x.get_device(), x.dtype
     if x.dim() < 1 or w_gate.dim() != 2 or w_gate.shape[0] != x.shape[-1]:
         raise ValueError(f"x must be (..., K) and w_gate (K, F); got {tuple(x.shape)} and {tuple(w_gate.shape)}")
-    _rl.as_floats("w_gate", w_gate, None, x.dtype)
-    _rl.as_floats("w_up", w_up, w_gate.shape, x.dtype)
+    k, f = w_gate.shape
+    for name, w in (("w_gate", w_gate), ("w_up", w_up)):
+        if w.get_device() != index or w.dtype is not dtype or w.shape != (k, f):
+            _rl.as_floats(name, w, (k, f), dtype)
+            _rl.one_device(index, **{name: w})
     if grad_out is not None:
-        _rl.as_floats("grad_out", grad_out, (*x.shape[:-1], w_gate.shape[1]), x.dtype)
+        _rl.as_floats("grad_out", grad_out, (*x.shape[:-1], f), dtype)
+        _rl.one_device(index, grad_out=grad_out)
     if activation not in ACTIVATIONS:
         raise ValueError(f"activation must be one of {sorted(ACTIVATIONS)}; got {activation!r}")
-    index = x.get_device()
-    _rl.one_device(index, w_gate=w_gate, w_up=w_up, grad_out=grad_out)
-    k, f = w_gate.shape
-    return x.numel() // k if k else x.shape[:-1].numel(), k, f, _rl.FLOAT_DTYPES[x.dtype], index
+    return x.numel() // k if k else x.shape[:-1].numel(), k, f, _rl.FLOAT_DTYPES[dtype], index
 
 
 def forward(x, w_gate, w_up, activation="silu"):

@@ -48,31 +48,36 @@ def _stride_array(*strides):
     return (ctypes.c_int64 * len(flat))(*flat)
 
 
-def _check(lead, decay, state, resets, grad_state, **tokens):
-    """The tokens' common shape, dtype and device, and the resets as bytes. lead: leading axes."""
-    shape = dtype = None
-    for name, x in tokens.items():
-        if shape is None or x.shape != shape or x.dtype is not dtype or x.get_device() != index:
+def _check(lead, decay, state, resets, grad_state, names, tokens):
+    """The tokens' common shape, dtype and device, and the resets as bytes. lead: leading axes. What fits passes
+    on a few comparisons; what does not is looked at again for the message."""
+    first = tokens[0]
+    if not isinstance(first, torch.Tensor) or not first.is_cuda or first.dtype not in _rl.FLOAT_DTYPES:
+        _rl.as_floats(names[0], first)
+    shape, dtype, index = first.shape, first.dtype, first.get_device()
+    for name, x in zip(names[1:], tokens[1:]):
+        if x.get_device() != index or x.dtype is not dtype or x.shape != shape:
             _rl.as_floats(name, x, shape, dtype)
-            if shape is not None:
-                raise ValueError(f"{name} must be on cuda:{index} as the other tensors; got {x.device}")
-            shape, dtype, index = x.shape, x.dtype, x.get_device()
+            _rl.one_device(index, **{name: x})
     if len(shape) != lead + 2:
-        raise ValueError(f"{', '.join(tokens)} must have {lead + 2} axes; got shape {tuple(shape)}")
+        raise ValueError(f"{', '.join(names)} must have {lead + 2} axes; got shape {tuple(shape)}")
     n, h, d = shape[-3:]
     if d not in WIDTHS:
         raise ValueError(f"the heads' width must be one of {WIDTHS}; got {d}")
-    _rl.as_floats("decay", decay, (h,), torch.float32)
-    if state is not None:
-        _rl.as_floats("state", state, (n, h, d, d), torch.float32)
-    if grad_state is not None:
-        _rl.as_floats("grad_state", grad_state, (n, h, d, d), torch.float32)
+    if decay.get_device() != index or decay.dtype is not torch.float32 or decay.shape != (h,):
+        _rl.as_floats("decay", decay, (h,), torch.float32)
+        _rl.one_device(index, decay=decay)
+    for s in (state, grad_state):
+        if s is not None and (s.get_device() != index or s.dtype is not torch.float32 or s.shape != (n, h, d, d)):
+            name = "state" if s is state else "grad_state"
+            _rl.as_floats(name, s, (n, h, d, d), torch.float32)
+            _rl.one_device(index, **{name: s})
     if resets is not None:
         if not isinstance(resets, torch.Tensor) or resets.dtype not in (torch.bool, torch.uint8) \
                 or resets.shape != shape[:-2]:
             raise ValueError(f"resets must be a bool or uint8 tensor of shape {tuple(shape[:-2])}")
+        _rl.one_device(index, resets=resets)
         resets = resets.contiguous()
-    _rl.one_device(index, decay=decay, state=state, resets=resets, grad_state=grad_state)
     return shape, dtype, index, resets
 
 
@@ -83,7 +88,7 @@ def _scale(scale, d):
 def forward(q, k, v, decay, state=None, resets=None, scale=None):
     """(out (T, N, H, D), state after the last token (N, H, D, D)). state None starts from zero; the
     given one is not changed. scale None is D ** -0.5."""
-    shape, dtype, index, resets = _check(2, decay, state, resets, None, q=q, k=k, v=v)
+    shape, dtype, index, resets = _check(2, decay, state, resets, None, ("q", "k", "v"), (q, k, v))
     t, n, h, d = shape
     (q, qs), (k, ks), (v, vs) = _rows(q), _rows(k), _rows(v)
     decay, state = decay.contiguous(), None if state is None else state.contiguous()
@@ -101,7 +106,8 @@ def forward(q, k, v, decay, state=None, resets=None, scale=None):
 def backward(grad_out, q, k, v, decay, state=None, resets=None, scale=None, grad_state=None):
     """Gradients (dq, dk, dv (T, N, H, D), dstate (N, H, D, D)) of `forward` from grad_out and, where the
     final state is used further, grad_state."""
-    shape, dtype, index, resets = _check(2, decay, state, resets, grad_state, grad_out=grad_out, q=q, k=k, v=v)
+    shape, dtype, index, resets = _check(2, decay, state, resets, grad_state, ("grad_out", "q", "k", "v"),
+                                         (grad_out, q, k, v))
     t, n, h, d = shape
     (g, gs), (q, qs), (k, ks), (v, vs) = _rows(grad_out), _rows(q), _rows(k), _rows(v)
     decay = decay.contiguous()
@@ -121,7 +127,7 @@ def backward(grad_out, q, k, v, decay, state=None, resets=None, scale=None, grad
 def step(q, k, v, decay, state, resets=None, scale=None):
     """One token for every environment, q, k, v (N, H, D), resets (N,): updates `state` (N, H, D, D) in
     place and returns out (N, H, D)."""
-    shape, dtype, index, resets = _check(1, decay, state, resets, None, q=q, k=k, v=v)
+    shape, dtype, index, resets = _check(1, decay, state, resets, None, ("q", "k", "v"), (q, k, v))
     if state is None or not state.is_contiguous() or state.data_ptr() % 16:
         raise ValueError("state must be contiguous and on a 16-byte boundary: it is updated in place")
     n, h, d = shape
