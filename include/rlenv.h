@@ -386,7 +386,7 @@ RLENV_API int rlenv_linear_attention_step(int dtype, int d, int64_t n, int64_t h
 /* Gated feed-forward block: out = act(x w_gate) * (x w_up), x (m, k), weights (k, f), out (m, f),
  * all dense row-major of one dtype (RLENV_F32 or RLENV_BF16), x, the weights and the
  * results on 16-byte boundaries, products summed in 32 bits. float32 operands pass the tensor cores as sums of three
- * bfloat16 terms (an infinity comes out as NaN). A launch takes all tensor-memory columns of its
+ * bfloat16 terms (an infinity may come out as NaN). A launch takes all tensor-memory columns of its
  * SMs and frees them before it ends.
  * activation: RLENV_SILU, or RLENV_GELU with the exact normal distribution. scratch: device
  * memory of at least rlenv_gated_ffn_scratch_bytes bytes, 256-byte aligned (NULL when that is 0). */

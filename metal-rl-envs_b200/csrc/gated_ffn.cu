@@ -653,7 +653,8 @@ add_parts_kernel(const float* __restrict__ parts, int splits, int64_t size, T* _
 // weights (1,024 x 4,096 in bfloat16, one row: 5.1 us with the weights in L2, 3.3 TB/s; eight rows, 11.4 us, are
 // bound by the products). A block owns 32 columns of both weights, so that 148 blocks read at once; its warps
 // split the contraction, each thread reading 16 bytes of every kApart-th row, and the sums meet in shared memory
-// in a fixed order.
+// in a fixed order. kGrad: with dh, the gates' gradients dg and du in float32, (2, m, pitch) with pitch f rounded
+// up to four and zeros there.
 constexpr int kFewThreads = 256, kFewCols = 32;
 
 template <typename T, bool kWide>
@@ -673,10 +674,10 @@ RLENV_D void load_columns(const T* p, int n, float (&v)[16 / sizeof(T)]) {
   }
 }
 
-template <typename T, int kFew, bool kWide>
+template <typename T, int kFew, bool kWide, bool kGrad>
 __global__ void __launch_bounds__(kFewThreads)
 few_rows_kernel(const T* __restrict__ x, const T* __restrict__ wg, const T* __restrict__ wu, int64_t m, int64_t k,
-                int64_t f, int act, T* __restrict__ out) {
+                int64_t f, int act, T* __restrict__ out, const T* __restrict__ dh, float* __restrict__ gates) {
   constexpr int kPer = 16 / sizeof(T), kAcross = kFewCols / kPer, kApart = kFewThreads / kAcross;
   constexpr int kUnroll = kFew > 4 ? 4 : 8;
   __shared__ float parts[kFewThreads / 32][2 * kFew * kFewCols];
@@ -715,6 +716,8 @@ few_rows_kernel(const T* __restrict__ x, const T* __restrict__ wg, const T* __re
   __syncthreads();
   for (int e = threadIdx.x; e < kFew * kFewCols; e += kFewThreads) {
     const int64_t r = m0 + e / kFewCols, col = int64_t(blockIdx.x) * kFewCols + e % kFewCols;
+    const int64_t pitch = (f + 3) / 4 * 4;
+    if (kGrad && r < m && col >= f && col < pitch) gates[r * pitch + col] = gates[(m + r) * pitch + col] = 0.0f;
     if (r >= m || col >= f) continue;
     float sg = 0.0f, su = 0.0f;
 #pragma unroll
@@ -722,19 +725,168 @@ few_rows_kernel(const T* __restrict__ x, const T* __restrict__ wg, const T* __re
     float y, slope;
     if (act == kSilu) activate<false, kSilu>(sg, &y, &slope);
     else activate<false, kGelu>(sg, &y, &slope);
-    out[r * f + col] = T(y * su);
+    if constexpr (kGrad) {
+      const float d = float(dh[r * f + col]);
+      gates[r * pitch + col] = d * su * slope;
+      gates[(m + r) * pitch + col] = d * y;
+    } else {
+      out[r * f + col] = T(y * su);
+    }
   }
+}
+
+// Four neighbours of a row, those from n on as zeros and not written.
+template <typename T, bool kWide>
+RLENV_D float4 load_four(const T* p, int64_t n) {
+  if constexpr (kWide && sizeof(T) == 2) {
+    const uint2 w = __ldg(reinterpret_cast<const uint2*>(p));
+    return make_float4(__uint_as_float(w.x << 16), __uint_as_float(w.x & 0xffff0000u), __uint_as_float(w.y << 16),
+                       __uint_as_float(w.y & 0xffff0000u));
+  } else if constexpr (kWide) {
+    return __ldg(reinterpret_cast<const float4*>(p));
+  } else {
+    return make_float4(n > 0 ? float(p[0]) : 0.0f, n > 1 ? float(p[1]) : 0.0f, n > 2 ? float(p[2]) : 0.0f,
+                       n > 3 ? float(p[3]) : 0.0f);
+  }
+}
+template <typename T, bool kWide>
+RLENV_D void store_four(T* p, const float (&v)[4], int64_t n) {
+  if constexpr (kWide && sizeof(T) == 2) {
+    const __nv_bfloat162 lo = __floats2bfloat162_rn(v[0], v[1]), hi = __floats2bfloat162_rn(v[2], v[3]);
+    *reinterpret_cast<uint2*>(p) =
+        make_uint2(*reinterpret_cast<const uint32_t*>(&lo), *reinterpret_cast<const uint32_t*>(&hi));
+  } else if constexpr (kWide) {
+    *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (i < n) p[i] = T(v[i]);
+  }
+}
+RLENV_D float dot_four(const float4& a, const float4& b, float sum) {
+  return fmaf(a.x, b.x, fmaf(a.y, b.y, fmaf(a.z, b.z, fmaf(a.w, b.w, sum))));
+}
+
+// The gradients of few rows from dg and du (`gates`, as above). Bound by writing both weights' gradients and
+// reading the weights: a float32 row of 1,024 x 4,096 20 us with the gates' launch, 100 MB in all, 5 TB/s (in turns
+// that find the weights in L2); from some eight rows on by the products. The first blocks form a 64 x 64 tile of
+// both weights' gradients each, sums over the tokens in registers; the others dx of kFew tokens at four columns, dot
+// products of whole rows of the weights, whose sums meet in shared memory in a fixed order.
+constexpr int kFewTile = 64, kFewTokens = 8, kFewDx = 4;
+struct FewGradients {
+  const void *x, *wg, *wu;
+  const float* gates;
+  void *dx, *dwg, *dwu;
+  int64_t m, k, f;
+  uint32_t across, weight_blocks, dx_across;
+};
+
+template <typename T, int kFew, bool kWide>
+__global__ void __launch_bounds__(kFewThreads) few_gradients_kernel(const FewGradients p) {
+  const int64_t pitch = (p.f + 3) / 4 * 4;
+  const float *const dg = p.gates, *const du = p.gates + p.m * pitch;
+  if (blockIdx.x < p.weight_blocks) {
+    __shared__ __align__(16) float d[2][kFewTokens][kFewTile], x[kFewTokens][kFewTile];
+    const int64_t c0 = int64_t(blockIdx.x % p.across) * kFewTile, r0 = int64_t(blockIdx.x / p.across) * kFewTile;
+    const int own_c = threadIdx.x % 16 * 4, own_r = threadIdx.x / 16 * 4;
+    float g[4][4] = {}, u[4][4] = {};
+    for (int64_t m0 = 0; m0 < p.m; m0 += kFewTokens) {
+      const int which = threadIdx.x / 128, token = threadIdx.x / 16 % kFewTokens;
+      *reinterpret_cast<float4*>(&d[which][token][own_c]) =
+          m0 + token < p.m && c0 + own_c < pitch
+              ? __ldg(reinterpret_cast<const float4*>((which ? du : dg) + (m0 + token) * pitch + c0 + own_c))
+              : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      for (int e = threadIdx.x; e < kFewTokens * kFewTile; e += kFewThreads) {
+        const int64_t t = m0 + e / kFewTile, r = r0 + e % kFewTile;
+        x[e / kFewTile][e % kFewTile] = t < p.m && r < p.k ? float(static_cast<const T*>(p.x)[t * p.k + r]) : 0.0f;
+      }
+      __syncthreads();
+#pragma unroll
+      for (int t = 0; t < kFewTokens; ++t) {
+        const float4 a = *reinterpret_cast<const float4*>(&x[t][own_r]);
+        const float4 b = *reinterpret_cast<const float4*>(&d[0][t][own_c]);
+        const float4 c = *reinterpret_cast<const float4*>(&d[1][t][own_c]);
+        const float av[4] = {a.x, a.y, a.z, a.w}, bv[4] = {b.x, b.y, b.z, b.w}, cv[4] = {c.x, c.y, c.z, c.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) g[i][j] = fmaf(av[i], bv[j], g[i][j]), u[i][j] = fmaf(av[i], cv[j], u[i][j]);
+      }
+      __syncthreads();
+    }
+    const int64_t c = c0 + own_c;
+    if (c >= p.f) return;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int64_t r = r0 + own_r + i;
+      if (r >= p.k) return;
+      store_four<T, kWide>(static_cast<T*>(p.dwg) + r * p.f + c, g[i], p.f - c);
+      store_four<T, kWide>(static_cast<T*>(p.dwu) + r * p.f + c, u[i], p.f - c);
+    }
+    return;
+  }
+  __shared__ float parts[kFewThreads / 32][kFewDx * kFew];
+  const uint32_t id = blockIdx.x - p.weight_blocks;
+  const int64_t k0 = int64_t(id % p.dx_across) * kFewDx, m0 = int64_t(id / p.dx_across) * kFew;
+  float sum[kFewDx][kFew] = {};
+  for (int64_t c = 4 * threadIdx.x; c < p.f; c += 4 * kFewThreads) {
+    float4 g[kFewDx], u[kFewDx];
+#pragma unroll
+    for (int i = 0; i < kFewDx; ++i) {
+      const int64_t at = (k0 + i < p.k ? k0 + i : p.k - 1) * p.f + c;
+      g[i] = load_four<T, kWide>(static_cast<const T*>(p.wg) + at, p.f - c);
+      u[i] = load_four<T, kWide>(static_cast<const T*>(p.wu) + at, p.f - c);
+    }
+#pragma unroll
+    for (int t = 0; t < kFew; ++t) {
+      const int64_t at = (m0 + t < p.m ? m0 + t : p.m - 1) * pitch + c;
+      const float4 b = __ldg(reinterpret_cast<const float4*>(dg + at)), w = __ldg(reinterpret_cast<const float4*>(du + at));
+#pragma unroll
+      for (int i = 0; i < kFewDx; ++i) sum[i][t] = dot_four(u[i], w, dot_four(g[i], b, sum[i][t]));
+    }
+  }
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+#pragma unroll
+  for (int i = 0; i < kFewDx; ++i)
+#pragma unroll
+    for (int t = 0; t < kFew; ++t) {
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) sum[i][t] += __shfl_xor_sync(0xffffffffu, sum[i][t], o);
+      if (lane == 0) parts[warp][t * kFewDx + i] = sum[i][t];
+    }
+  __syncthreads();
+  const int t = threadIdx.x / kFewDx, i = threadIdx.x % kFewDx;
+  if (t >= kFew || m0 + t >= p.m || k0 + i >= p.k) return;
+  float whole = 0.0f;
+#pragma unroll
+  for (int w = 0; w < kFewThreads / 32; ++w) whole += parts[w][threadIdx.x];
+  static_cast<T*>(p.dx)[(m0 + t) * p.k + k0 + i] = T(whole);
 }
 
 template <typename T, int kFew>
 int few_rows(const void* x, const void* wg, const void* wu, int64_t m, int64_t k, int64_t f, int act, void* out,
-             cudaStream_t s) {
+             const void* dh, void* gates, void* dx, void* dwg, void* dwu, cudaStream_t s) {
   const dim3 grid(unsigned((f + kFewCols - 1) / kFewCols), unsigned((m + kFew - 1) / kFew));
   const T *X = static_cast<const T*>(x), *G = static_cast<const T*>(wg), *U = static_cast<const T*>(wu);
-  if (f * int64_t(sizeof(T)) % 16 == 0)
-    few_rows_kernel<T, kFew, true><<<grid, kFewThreads, 0, s>>>(X, G, U, m, k, f, act, static_cast<T*>(out));
-  else
-    few_rows_kernel<T, kFew, false><<<grid, kFewThreads, 0, s>>>(X, G, U, m, k, f, act, static_cast<T*>(out));
+  const T* const D = static_cast<const T*>(dh);
+  T* const to = static_cast<T*>(out);
+  float* const own = static_cast<float*>(gates);
+  const bool wide = f * int64_t(sizeof(T)) % 16 == 0;
+  if (!dh) {
+    if (wide) few_rows_kernel<T, kFew, true, false><<<grid, kFewThreads, 0, s>>>(X, G, U, m, k, f, act, to, D, own);
+    else few_rows_kernel<T, kFew, false, false><<<grid, kFewThreads, 0, s>>>(X, G, U, m, k, f, act, to, D, own);
+    return launch_status();
+  }
+  FewGradients p{x, wg, wu, own, dx, dwg, dwu, m, k, f};
+  const int64_t across = (f + kFewTile - 1) / kFewTile, weight_blocks = across * ((k + kFewTile - 1) / kFewTile);
+  const int64_t dx_across = (k + kFewDx - 1) / kFewDx, blocks = weight_blocks + dx_across * ((m + kFew - 1) / kFew);
+  if (blocks > 0x7fffffff) return RLENV_EINVAL;
+  p.across = uint32_t(across), p.weight_blocks = uint32_t(weight_blocks), p.dx_across = uint32_t(dx_across);
+  if (wide) few_rows_kernel<T, kFew, true, true><<<grid, kFewThreads, 0, s>>>(X, G, U, m, k, f, act, to, D, own);
+  else few_rows_kernel<T, kFew, false, true><<<grid, kFewThreads, 0, s>>>(X, G, U, m, k, f, act, to, D, own);
+  if (const int rc = launch_status()) return rc;
+  if (f % 4 == 0) few_gradients_kernel<T, kFew, true><<<unsigned(blocks), kFewThreads, 0, s>>>(p);
+  else few_gradients_kernel<T, kFew, false><<<unsigned(blocks), kFewThreads, 0, s>>>(p);
   return launch_status();
 }
 
@@ -749,6 +901,16 @@ bool few_rows_fit(int dtype, int64_t m, int64_t f) {
   const bool wide = dtype == RLENV_F32;
   const int64_t blocks = (m + 7) / 8 * ((f + kFewCols - 1) / kFewCols);
   return m <= (wide ? 24 : 4) || blocks <= 148 * (wide ? 3 : 1);
+}
+// The same for the gradient, whose tiles cost two launches more and work on 256 rows however few there are; this
+// way takes longer by the row. Measured in us, this way and by tiles: float32 1,024 x 4,096, 1 row 20 and 143, 32
+// rows 91 and 94, 64 rows 166 and 96; 1,024 x 1,024, 64 rows 53.5 and 54.2; 97 x 250, 128 rows 26.3 and 27.8;
+// bfloat16 922 x 5,556, 4 rows 39 and 44, 8 rows 51 and 45; 1,024 x 1,024, 16 rows 22.2 and 22.7, 24 rows 25.9 and
+// 23.2; 97 x 250, 32 rows 14.5 and 21.0, 128 rows 28.1 and 21.9; 512 x 512, 64 rows 21.4 and 21.0.
+bool few_gradients_fit(int dtype, int64_t m, int64_t k, int64_t f) {
+  const double products = double(m) * double(k) * double(f);
+  return dtype == RLENV_F32 ? m <= 32 || (m <= 128 && products <= 67108864.0)
+                            : m <= 4 || (m <= 32 && products <= 16777216.0);
 }
 
 // ---- host ------------------------------------------------------------------------------------------
@@ -820,6 +982,11 @@ Layout lay_out(int dtype, int64_t m, int64_t k, int64_t f, bool backward, void* 
   Layout l{};
   const int64_t n = planes(dtype);
   if (!backward && few_rows_fit(dtype, m, f)) return l;
+  if (backward && few_gradients_fit(dtype, m, k, f)) {
+    l.gates = s.take(2 * m * round_up(f, 4) * 4);
+    l.bytes = s.used;
+    return l;
+  }
   if (packs(dtype, k)) l.x = s.take(n * m * round_up(k, 8) * 2);
   if (packs(dtype, f)) l.wg = s.take(n * k * round_up(f, 8) * 2), l.wu = s.take(n * k * round_up(f, 8) * 2);
   if (backward) {
@@ -877,11 +1044,12 @@ template <typename T>
 int ffn(const void* dh, const void* x, const void* wg, const void* wu, int64_t m, int64_t k, int64_t f, int act,
         void* out, void* dx, void* dwg, void* dwu, const Layout& l, cudaStream_t s) {
   using C = Tile<T>;
-  if (!dh && few_rows_fit(C::kFloat ? RLENV_F32 : RLENV_BF16, m, f))
-    return m == 1   ? few_rows<T, 1>(x, wg, wu, m, k, f, act, out, s)
-           : m == 2 ? few_rows<T, 2>(x, wg, wu, m, k, f, act, out, s)
-           : m <= 4 ? few_rows<T, 4>(x, wg, wu, m, k, f, act, out, s)
-                    : few_rows<T, 8>(x, wg, wu, m, k, f, act, out, s);
+  constexpr int kDtype = C::kFloat ? RLENV_F32 : RLENV_BF16;
+  if (dh ? few_gradients_fit(kDtype, m, k, f) : few_rows_fit(kDtype, m, f))
+    return m == 1   ? few_rows<T, 1>(x, wg, wu, m, k, f, act, out, dh, l.gates, dx, dwg, dwu, s)
+           : m == 2 ? few_rows<T, 2>(x, wg, wu, m, k, f, act, out, dh, l.gates, dx, dwg, dwu, s)
+           : m <= 4 ? few_rows<T, 4>(x, wg, wu, m, k, f, act, out, dh, l.gates, dx, dwg, dwu, s)
+                    : few_rows<T, 8>(x, wg, wu, m, k, f, act, out, dh, l.gates, dx, dwg, dwu, s);
   Operand in[3];
   if (const int rc = operands<T>({x, wg, wu}, {m, k, k}, {k, f, f}, {l.x, l.wg, l.wu}, s, in)) return rc;
   const Operand &X = in[0], &G = in[1], &U = in[2];

@@ -5,9 +5,9 @@ x is (..., K), the weights (K, F) as es.unflatten's (in, out) layout, out (..., 
 float32 or bfloat16; sums are in 32 bits. activation is "silu" or "gelu" (the exact normal
 distribution). `backward` forms both products again instead of keeping them. `apply` is the
 differentiable form. The projection back to K is a plain matrix product and is left to the caller.
-float32 operands
-go through the tensor cores as sums of three bfloat16 terms: results have float32's precision, but an
-infinity, or a magnitude above bfloat16's 3.39e38, comes out as NaN. The reference's policies are tanh MLPs (es.py:156-164); there is no counterpart there.
+float32 operands go through the tensor cores as sums of three bfloat16 terms, but for few rows: results
+have float32's precision, but an infinity, or a magnitude above bfloat16's 3.39e38, may come out as NaN.
+The reference's policies are tanh MLPs (es.py:156-164); there is no counterpart there.
 """
 
 import torch

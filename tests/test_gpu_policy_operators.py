@@ -331,6 +331,27 @@ def test_ffn_backward(cuda, m, k, f, act, dtype):
         close(a, w, tol + low * abs(w), name)
 
 
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("m,k,f", [(1, 97, 250), (2, 300, 77), (3, 64, 256), (5, 1, 5), (9, 129, 131), (32, 65, 1030),
+                                   (33, 70, 68), (77, 31, 36), (128, 97, 250), (129, 97, 250)])
+def test_ffn_backward_of_few_rows(cuda, m, k, f, dtype):
+    test_ffn_backward(cuda, m, k, f, "gelu", dtype)
+
+
+def test_ffn_gradient_of_few_rows_with_infinities(cuda):
+    """Sums of products as the formula has them: what is not finite stays with its own token and column."""
+    import gated_ffn
+
+    x, wg, wu, dh = ffn_inputs(cuda, 3, 20, 23, "f32")
+    want = gated_ffn.backward(dh, x, wg, wu)
+    bad = dh.clone()
+    bad[1, 22] = float("inf")
+    dx, dwg, dwu = gated_ffn.backward(bad, x, wg, wu)
+    assert not torch.isfinite(dx[1]).any() and torch.equal(dx[[0, 2]], want[0][[0, 2]])
+    for got, w in ((dwg, want[1]), (dwu, want[2])):
+        assert not torch.isfinite(got[:, 22]).any() and torch.equal(got[:, :22], w[:, :22])
+
+
 def test_ffn_shapes_strides_and_empties(cuda):
     import gated_ffn
 
