@@ -43,9 +43,14 @@ RLENV_D void activate(float g, float* y, float* slope) {
 
 // ---- operands ------------------------------------------------------------------------------------
 
-// Planes of up to three (rows, cols) arrays as bfloat16 (planes, rows, pitch), pitch a multiple of 8: for
+// The pitch of rows in scratch: whole lines of 128 bytes, so that a tensor copy's row of a tile lies in one
+// (float32 4,330 x 881 x 1,780: 124 us against 184 with rows on 16 bytes, the gradient 502 against 698).
+__host__ __device__ constexpr int64_t pitch_of(int64_t cols) { return (cols + 63) / 64 * 64; }
+
+// Planes of up to three (rows, cols) arrays as bfloat16 (planes, rows, pitch_of(cols)): for
 // float32 the three whose sum it is, for bfloat16 a copy (rows that are not on 16-byte boundaries). A warp takes
-// a run of kPackRun columns of a row, a lane pairs of its elements.
+// a run of kPackRun columns of a row, a lane pairs of its elements. Bound by memory: 4,330 x 881 and twice 881 x
+// 1,780 in float32, 69 MB, 10 us.
 constexpr int kPackRun = 512;
 struct Packing {
   const void* from[3];
@@ -57,20 +62,28 @@ __global__ void __launch_bounds__(256) pack_kernel(const __grid_constant__ Packi
   const int64_t i = int64_t(blockIdx.x) * 8 + (threadIdx.x >> 5);
   if (i >= p.runs[3]) return;
   const int a = i < p.runs[1] ? 0 : i < p.runs[2] ? 1 : 2;
-  const int64_t rows = p.rows[a], cols = p.cols[a], pitch = (cols + 7) / 8 * 8;
-  const uint32_t a_row = uint32_t((pitch + kPackRun - 1) / kPackRun);
+  const int64_t rows = p.rows[a], cols = p.cols[a], pitch = pitch_of(cols);
+  const uint32_t a_row = uint32_t((cols + kPackRun - 1) / kPackRun);
   const int64_t run = i - p.runs[a], r = a_row == 1 ? run : run / a_row, c0 = a_row == 1 ? 0 : run % a_row * kPackRun;
   const T* from = static_cast<const T*>(p.from[a]) + r * cols;
   __nv_bfloat16* to = p.to[a] + r * pitch;
-  const int64_t end = c0 + kPackRun < pitch ? c0 + kPackRun : pitch;
-#pragma unroll 4
-  for (int64_t c = c0 + 2 * (threadIdx.x & 31); c < end; c += 64) {
-    float lo = c < cols ? float(from[c]) : 0.0f, hi = c + 1 < cols ? float(from[c + 1]) : 0.0f;
+  const int64_t first = c0 + 2 * (threadIdx.x & 31);
+  float lo[kPackRun / 64], hi[kPackRun / 64];  // all loads before the first store
+#pragma unroll
+  for (int u = 0; u < kPackRun / 64; ++u) {
+    if (c0 + 64 * u >= cols) break;
+    const int64_t c = first + 64 * u;
+    lo[u] = c < cols ? float(__ldg(from + c)) : 0.0f, hi[u] = c + 1 < cols ? float(__ldg(from + c + 1)) : 0.0f;
+  }
+#pragma unroll
+  for (int u = 0; u < kPackRun / 64; ++u) {
+    const int64_t c = first + 64 * u;
+    if (c >= cols) break;
 #pragma unroll
     for (int q = 0; q < kPlanes; ++q) {
-      const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+      const __nv_bfloat162 v = __floats2bfloat162_rn(lo[u], hi[u]);
       *reinterpret_cast<__nv_bfloat162*>(to + q * rows * pitch + c) = v;
-      lo -= __low2float(v), hi -= __high2float(v);
+      lo[u] -= __low2float(v), hi[u] -= __high2float(v);
     }
   }
 }
@@ -987,10 +1000,10 @@ Layout lay_out(int dtype, int64_t m, int64_t k, int64_t f, bool backward, void* 
     l.bytes = s.used;
     return l;
   }
-  if (packs(dtype, k)) l.x = s.take(n * m * round_up(k, 8) * 2);
-  if (packs(dtype, f)) l.wg = s.take(n * k * round_up(f, 8) * 2), l.wu = s.take(n * k * round_up(f, 8) * 2);
+  if (packs(dtype, k)) l.x = s.take(n * m * pitch_of(k) * 2);
+  if (packs(dtype, f)) l.wg = s.take(n * k * pitch_of(f) * 2), l.wu = s.take(n * k * pitch_of(f) * 2);
   if (backward) {
-    l.gates = s.take(2 * n * m * round_up(f, 8) * 2);
+    l.gates = s.take(2 * n * m * pitch_of(f) * 2);
     if (m > 0 && k > 0 && f > 0) split_gradients(dtype, m, k, f, &l);
     if (l.splits > 1) l.parts = static_cast<float*>(s.take(int64_t(l.splits) * 2 * k * f * 4));
     if (l.dx_splits > 1) l.dx_parts = static_cast<float*>(s.take(int64_t(l.dx_splits) * m * k * 4));
@@ -1011,10 +1024,9 @@ int operands(const void* const (&from)[3], const int64_t (&rows)[3], const int64
       o[i] = {static_cast<const __nv_bfloat16*>(from[i]), rows[i], cols[i], cols[i], 1};
       continue;
     }
-    const int64_t pitch = round_up(cols[i], 8);
     p.from[i] = from[i], p.to[i] = static_cast<__nv_bfloat16*>(packed[i]);
-    p.rows[i] = rows[i], p.cols[i] = cols[i], p.runs[i + 1] += rows[i] * ((pitch + kPackRun - 1) / kPackRun);
-    o[i] = {p.to[i], rows[i], cols[i], pitch, kPlanes};
+    p.rows[i] = rows[i], p.cols[i] = cols[i], p.runs[i + 1] += rows[i] * ((cols[i] + kPackRun - 1) / kPackRun);
+    o[i] = {p.to[i], rows[i], cols[i], pitch_of(cols[i]), kPlanes};
   }
   if (p.runs[3] == 0) return RLENV_OK;
   if ((p.runs[3] + 7) / 8 > 0x7fffffff) return RLENV_EINVAL;
@@ -1055,7 +1067,7 @@ int ffn(const void* dh, const void* x, const void* wg, const void* wu, int64_t m
   const Operand &X = in[0], &G = in[1], &U = in[2];
   Product p{};
   p.m = m, p.k = k, p.f = f, p.act = act, p.out = out, p.dh = dh;
-  p.gates = static_cast<__nv_bfloat16*>(l.gates), p.pitch = round_up(f, 8);
+  p.gates = static_cast<__nv_bfloat16*>(l.gates), p.pitch = pitch_of(f);
   p.wide = f % 4 == 0 && reinterpret_cast<uintptr_t>(dh) % (4 * sizeof(T)) == 0;
   p.row_tiles = tile_count(m, 2 * kRows), p.col_tiles = tile_count(f, C::kHalf);
   if (const int rc = X.map(&p.in[0].a, kRows)) return rc;
