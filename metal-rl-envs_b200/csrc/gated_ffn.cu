@@ -68,23 +68,24 @@ __global__ void __launch_bounds__(256) pack_kernel(const __grid_constant__ Packi
   const T* from = static_cast<const T*>(p.from[a]) + r * cols;
   __nv_bfloat16* to = p.to[a] + r * pitch;
   const int64_t first = c0 + 2 * (threadIdx.x & 31);
-  float lo[kPackRun / 64], hi[kPackRun / 64];  // all loads before the first store
-#pragma unroll
-  for (int u = 0; u < kPackRun / 64; ++u) {
-    if (c0 + 64 * u >= cols) break;
-    const int64_t c = first + 64 * u;
-    lo[u] = c < cols ? float(__ldg(from + c)) : 0.0f, hi[u] = c + 1 < cols ? float(__ldg(from + c + 1)) : 0.0f;
-  }
-#pragma unroll
-  for (int u = 0; u < kPackRun / 64; ++u) {
-    const int64_t c = first + 64 * u;
-    if (c >= cols) break;
+  const auto store = [&](int64_t c, float lo, float hi) {
 #pragma unroll
     for (int q = 0; q < kPlanes; ++q) {
-      const __nv_bfloat162 v = __floats2bfloat162_rn(lo[u], hi[u]);
+      const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
       *reinterpret_cast<__nv_bfloat162*>(to + q * rows * pitch + c) = v;
-      lo[u] -= __low2float(v), hi[u] -= __high2float(v);
+      lo -= __low2float(v), hi -= __high2float(v);
     }
+  };
+  if (c0 + kPackRun <= cols) {
+    float lo[kPackRun / 64], hi[kPackRun / 64];  // all loads before the first store
+#pragma unroll
+    for (int u = 0; u < kPackRun / 64; ++u)
+      lo[u] = float(__ldg(from + first + 64 * u)), hi[u] = float(__ldg(from + first + 64 * u + 1));
+#pragma unroll
+    for (int u = 0; u < kPackRun / 64; ++u) store(first + 64 * u, lo[u], hi[u]);
+  } else {
+#pragma unroll 4
+    for (int64_t c = first; c < cols; c += 64) store(c, float(__ldg(from + c)), c + 1 < cols ? float(__ldg(from + c + 1)) : 0.0f);
   }
 }
 
@@ -94,14 +95,13 @@ enum Op { kForward, kGates, kGradients };  // h; dg and du; dx, dWg and dWu
 
 constexpr int kRows = 128;       // of a tile, in each block of a pair
 constexpr int kBlock = 64;       // of the contraction: a tile row's 128 bytes
-constexpr int kTmemColumns = 512;
+constexpr int kTmemColumns = 512, kBufferColumns = 256;
 constexpr int kStageFloats = 32 * 32;  // the epilogue's tile of a warp
 
 template <typename T>
 struct Tile {
   static constexpr bool kFloat = sizeof(T) == 4;
   static constexpr int kPlanes = kFloat ? 3 : 1;
-  static constexpr int kPairs = kFloat ? 6 : 1;  // products of planes
   static constexpr int kCols = kFloat ? 128 : 256;
   static constexpr int kHalf = kCols / 2;        // columns of B in each block
   // Warps: copies, products, two idle ones, and those of the epilogue. float32's, with the exact exponential
@@ -109,22 +109,18 @@ struct Tile {
   static constexpr int kEpilogue = kFloat ? 16 : 8;
   static constexpr int kThreads = 128 + 32 * kEpilogue;
   static constexpr int kMine = kCols / (kEpilogue / 4);  // columns of the accumulator that a thread reads
-  // A ring buffer's blocks: float32's narrower products are over sooner, and two blocks keep the turn of a
-  // step, some 300 cycles of waiting and committing, below the products' time.
-  static constexpr int kBlocks = kFloat ? 2 : 1;
-  static constexpr int kStep = kBlocks * kBlock;
+  static constexpr int kStep = kBlock;
   static constexpr int kABytes = kRows * kBlock * 2;
-  static constexpr int kBlockBytes = kABytes + kHalf * kBlock * 2;
-  static constexpr int kRingBytes = kBlocks * kBlockBytes;
-  static constexpr int kStages = kFloat ? 3 : 6;
+  static constexpr int kRingBytes = kABytes + kHalf * kBlock * 2;  // a ring buffer: a plane of both operands
+  static constexpr int kStages = 6;
   static constexpr int kStageAt = kStages * kRingBytes;  // the epilogue's 32 x 32 tiles, one a warp
   // the ring starts on a 1,024-byte boundary
   static constexpr int kSmem = kStageAt + kEpilogue * kStageFloats * 4 + 1024;
   // Steps of the contraction summed in tensor memory before the epilogue takes them out into registers
   // (float32 only). The tensor core truncates as it accumulates; rounded additions of short sums keep
-  // float32 results at float32's error. Of the products of planes only the leading one, the last to be
-  // formed, is large enough to need the short sums.
-  static constexpr int kRun = 2, kSmallRun = 16;
+  // float32 results at float32's error. The leading planes' product and the five small ones have an
+  // accumulator each: what is truncated of the small sums is small.
+  static constexpr int kRun = 4;
 };
 
 struct Operands {
@@ -190,18 +186,12 @@ RLENV_D Work work_of(const Product& p, int item) {
   return w;
 }
 
-// The pairs of planes, the small products first: a's and b's, two bits each.
+// A step's planes in the order in which they are copied. A plane's products with those before it follow its
+// arrival: 1 1, then 0 1, 1 0 and 0 0, then 0 2 and 2 0. Each is read from L2 once for all of its products
+// (measured against a pass over the contraction for each product, 96 bytes a clock and SM: TODO), and the first
+// buffer is free again halfway through.
 template <typename T>
-RLENV_D int plane_a(int pair) { return Tile<T>::kFloat ? 0x118 >> (2 * pair) & 3 : 0; }  // 0 2 1 0 1 0
-template <typename T>
-RLENV_D int plane_b(int pair) { return Tile<T>::kFloat ? 0x052 >> (2 * pair) & 3 : 0; }  // 2 0 1 1 0 0
-// How often the accumulator of a float32 tile of `steps` steps is handed over: the small products' runs, and
-// the leading ones'.
-RLENV_D int runs_of(int steps) {
-  constexpr int kPairs = Tile<float>::kPairs, kSmall = Tile<float>::kSmallRun, kRun = Tile<float>::kRun;
-  const int leading = steps / kPairs, small = steps - leading;
-  return (small + kSmall - 1) / kSmall + (leading + kRun - 1) / kRun;
-}
+RLENV_D int plane_of(int turn) { return Tile<T>::kFloat ? 0x21 >> (2 * turn) & 3 : 0; }
 
 // Four neighbouring values of a row, the first n of them there: in one access where all are and `wide`
 // says that rows start on the boundaries of fours.
@@ -462,34 +452,30 @@ product_kernel(const __grid_constant__ Product p, int items) {
       const Operands& in = p.in[kOp == kGradients && w.weights];
       const int r0 = (2 * w.row + rank) * kRows, c0 = w.c0 + (kPaired ? 0 : rank * C::kHalf);
       const CUtensorMap* const map_a = &in.a;
-      for (int pair = 0; pair < C::kPairs && ok; ++pair) {
-        const int pa = plane_a<T>(pair), pb = plane_b<T>(pair);
-        for (int seg = 0; seg < w.segs && ok; ++seg) {
-          // slices: planes; of the gates dg's and du's by turns. Gates in the first block, ups in the second.
-          const CUtensorMap* const map_b = (kPaired ? rank : seg) ? &in.b1 : &in.b0;
-          const int slice_a = kPaired || w.weights ? pa : 2 * pa + seg, slice_b = !kPaired && w.weights ? 2 * pb + w.weight : pb;
-          const int k_end = (w.k0 + w.steps) * C::kStep;
-          for (int k0 = w.k0 * C::kStep; k0 < k_end; k0 += C::kStep) {
-            const uint32_t bar = full_at + 8 * stage, a0 = ring + stage * C::kRingBytes;
+      for (int seg = 0; seg < w.segs && ok; ++seg) {
+        // slices: planes; of the gates dg's and du's by turns. Gates in the first block, ups in the second.
+        const CUtensorMap* const map_b = (kPaired ? rank : seg) ? &in.b1 : &in.b0;
+        const int k_end = (w.k0 + w.steps) * C::kStep;
+        for (int k = w.k0 * C::kStep; k < k_end && ok; k += C::kStep) {  // what lies past the contraction reads as zero
+          for (int turn = 0; turn < C::kPlanes; ++turn) {
+            const int plane = plane_of<T>(turn);
+            const int slice_a = kPaired || w.weights ? plane : 2 * plane + seg;
+            const int slice_b = !kPaired && w.weights ? 2 * plane + w.weight : plane;
+            const uint32_t bar = full_at + 8 * stage, a = ring + stage * C::kRingBytes, b = a + C::kABytes;
             if (!(ok = bw::barrier_wait_warp(empty + 8 * stage, phase ^ 1, dead))) break;
             if (bw::elect()) {
               if (rank == 0) bw::barrier_expect(full + 8 * stage, 2 * C::kRingBytes);
+              if (!kPaired && w.weights) {
 #pragma unroll
-              for (int q = 0; q < C::kBlocks; ++q) {  // what lies past the contraction's end reads as zero
-                const uint32_t a = a0 + q * C::kBlockBytes, b = a + C::kABytes;
-                const int k = k0 + q * kBlock;
-                if (!kPaired && w.weights) {
+                for (int i = 0; i < kRows / 64; ++i) bw::copy_tile(a + i * kBox, map_a, bar, r0 + 64 * i, k, slice_a);
+              } else {
+                bw::copy_tile(a, map_a, bar, k, r0, slice_a);
+              }
+              if (kPaired || w.weights) {
 #pragma unroll
-                  for (int i = 0; i < kRows / 64; ++i) bw::copy_tile(a + i * kBox, map_a, bar, r0 + 64 * i, k, slice_a);
-                } else {
-                  bw::copy_tile(a, map_a, bar, k, r0, slice_a);
-                }
-                if (kPaired || w.weights) {
-#pragma unroll
-                  for (int i = 0; i < C::kHalf / 64; ++i) bw::copy_tile(b + i * kBox, map_b, bar, c0 + 64 * i, k, slice_b);
-                } else {
-                  bw::copy_tile(b, map_b, bar, k, c0, slice_b);
-                }
+                for (int i = 0; i < C::kHalf / 64; ++i) bw::copy_tile(b + i * kBox, map_b, bar, c0 + 64 * i, k, slice_b);
+              } else {
+                bw::copy_tile(b, map_b, bar, k, c0, slice_b);
               }
             }
             used |= 1u << stage;
@@ -510,37 +496,55 @@ product_kernel(const __grid_constant__ Product p, int items) {
       bool ok = true;
       for (int item = first; item < items && ok; item += stride) {
         const Work w = work_of<T, kOp>(p, item);
-        const int steps = C::kPairs * w.segs * w.steps;
+        const int steps = w.segs * w.steps;
         const bool mn_a = w.weights, mn_b = kPaired || w.weights;
         const uint32_t kind = bw::product_kind(2 * kRows, C::kCols, mn_a, mn_b);
         const uint32_t a0 = bw::operand(ring, mn_a, kBox), b0 = bw::operand(ring + C::kABytes, mn_b, kBox);
         const uint32_t a_step = mn_a ? 2048 / 16 : 32 / 16, b_step = mn_b ? 2048 / 16 : 32 / 16;  // 16 of the contraction
-        const int small = steps / C::kPairs * (C::kPairs - 1);
-        int left = C::kFloat ? min(C::kSmallRun, small) : steps;  // steps to the end of the run
-        bool fresh = true;
+        int left = C::kFloat ? min(C::kRun, steps) : steps;  // steps to the end of the run
+        bool more = false;                                   // the run has begun
         for (int it = 0; it < steps; ++it) {
-          if (fresh && !(ok = bw::barrier_wait_warp(taken + 8 * buffer, buffer_phase ^ 1, dead))) break;
-          const uint32_t d = tmem + buffer * C::kCols, a = a0 + stage * (C::kRingBytes / 16),
+          if (!more && !(ok = bw::barrier_wait_warp(taken + 8 * buffer, buffer_phase ^ 1, dead))) break;
+          const uint32_t d = tmem + buffer * kBufferColumns, a = a0 + stage * (C::kRingBytes / 16),
                          b = b0 + stage * (C::kRingBytes / 16);
-          if (!(ok = bw::barrier_wait_warp(full + 8 * stage, phase, dead))) break;
-          bw::fence_after();
-          const bool more = !fresh;
-          fresh = --left == 0;
-          if (bw::elect()) {
+          const auto add = [&](uint32_t to, int of_a, int of_b, bool accumulate) {
 #pragma unroll
-            for (int q = 0; q < C::kBlocks; ++q)
+            for (int k = 0; k < kBlock / 16; ++k)
+              bw::multiply(to, a + of_a * (C::kRingBytes / 16) + k * a_step, b + of_b * (C::kRingBytes / 16) + k * b_step,
+                           kind, k > 0 || accumulate);
+          };
+          const bool last = --left == 0;
 #pragma unroll
-              for (int k = 0; k < kBlock / 16; ++k)
-                bw::multiply(d, a + q * (C::kBlockBytes / 16) + k * a_step, b + q * (C::kBlockBytes / 16) + k * b_step,
-                             kind, q + k > 0 || more);
-            bw::commit(empty + 8 * stage);
-            if (fresh) bw::commit(summed + 8 * buffer);
+          for (int turn = 0; turn < C::kPlanes; ++turn) {
+            if (!(ok = bw::barrier_wait_warp(full + 8 * (stage + turn), phase, dead))) break;
+            bw::fence_after();
+            if (bw::elect()) {
+              if (!C::kFloat) {
+                add(d, 0, 0, more);
+                bw::commit(empty + 8 * stage);
+              } else if (turn == 0) {
+                add(d + C::kCols, 0, 0, more);
+              } else if (turn == 1) {
+                add(d + C::kCols, 1, 0, true);
+                add(d + C::kCols, 0, 1, true);
+                bw::commit(empty + 8 * stage);
+                add(d, 1, 1, more);
+              } else {
+                add(d + C::kCols, 1, 2, true);
+                add(d + C::kCols, 2, 1, true);
+                bw::commit(empty + 8 * (stage + 1));
+                bw::commit(empty + 8 * (stage + 2));
+              }
+              if (last && turn == C::kPlanes - 1) bw::commit(summed + 8 * buffer);
+            }
           }
-          if (fresh) {
+          if (!ok) break;
+          more = !last;
+          if (last) {
             if (++buffer == 2) buffer = 0, buffer_phase ^= 1;
-            left = it + 1 < small ? min(C::kSmallRun, small - it - 1) : min(C::kRun, steps - it - 1);
+            left = min(C::kRun, steps - it - 1);
           }
-          if (++stage == C::kStages) stage = 0, phase ^= 1;
+          if ((stage += C::kPlanes) == C::kStages) stage = 0, phase ^= 1;
         }
       }
     }
@@ -561,8 +565,8 @@ product_kernel(const __grid_constant__ Product p, int items) {
     // Run j of 32 columns of this thread's, as two of 16: a gated tile's are gates and ups.
     const auto column = [&](int j) { return kPaired ? part * (C::kMine / 2) + 16 * j : part * C::kMine + 32 * j; };
     constexpr int kRuns = C::kMine / 32;
-    const auto load_run = [&](uint32_t (&v)[32], int j) {
-      const uint32_t at = tmem + lanes + buffer * C::kCols + column(j);
+    const auto load_run = [&](uint32_t (&v)[32], int j, int from = 0) {
+      const uint32_t at = tmem + lanes + buffer * kBufferColumns + from + column(j);
       bw::tmem_load16x2(v, at, at + (kPaired ? C::kHalf : 16));
     };
     for (int item = first; item < items; item += stride) {
@@ -589,18 +593,20 @@ product_kernel(const __grid_constant__ Product p, int items) {
         for (int j = 0; j < kRuns; ++j)
 #pragma unroll
           for (int i = 0; i < 32; ++i) sum[j][i] = 0.0f;
-        for (int runs = runs_of(C::kPairs * w.segs * w.steps); runs > 0; --runs) {
+        for (int left = w.segs * w.steps; left > 0; left -= C::kRun) {
           ok = bw::barrier_wait_warp(summed + 8 * buffer, buffer_phase, dead) && ok;
           if (!ok) break;
           bw::fence_after();
 #pragma unroll
-          for (int j = 0; j < kRuns; ++j) {
-            uint32_t v[32];
-            load_run(v, j);
-            bw::tmem_ready(v);
+          for (int j = 0; j < kRuns; ++j)
 #pragma unroll
-            for (int i = 0; i < 32; ++i) sum[j][i] += __uint_as_float(v[i]);
-          }
+            for (int from = 0; from <= C::kCols; from += C::kCols) {
+              uint32_t v[32];
+              load_run(v, j, from);
+              bw::tmem_ready(v);
+#pragma unroll
+              for (int i = 0; i < 32; ++i) sum[j][i] += __uint_as_float(v[i]);
+            }
           take_next();
         }
 #pragma unroll
