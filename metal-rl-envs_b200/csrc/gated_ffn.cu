@@ -76,16 +76,19 @@ __global__ void __launch_bounds__(256) pack_kernel(const __grid_constant__ Packi
       lo -= __low2float(v), hi -= __high2float(v);
     }
   };
-  if (c0 + kPackRun <= cols) {
-    float lo[kPackRun / 64], hi[kPackRun / 64];  // all loads before the first store
+  constexpr int kAhead = kPlanes > 1 ? 8 : 4;  // pairs a lane loads before it stores any
 #pragma unroll
-    for (int u = 0; u < kPackRun / 64; ++u)
-      lo[u] = float(__ldg(from + first + 64 * u)), hi[u] = float(__ldg(from + first + 64 * u + 1));
+  for (int u0 = 0; u0 < kPackRun / 64; u0 += kAhead) {
+    if (c0 + 64 * u0 >= cols) break;
+    float lo[kAhead], hi[kAhead];
 #pragma unroll
-    for (int u = 0; u < kPackRun / 64; ++u) store(first + 64 * u, lo[u], hi[u]);
-  } else {
-#pragma unroll 4
-    for (int64_t c = first; c < cols; c += 64) store(c, float(__ldg(from + c)), c + 1 < cols ? float(__ldg(from + c + 1)) : 0.0f);
+    for (int u = 0; u < kAhead; ++u) {
+      const int64_t c = first + 64 * (u0 + u);
+      lo[u] = c < cols ? float(__ldg(from + c)) : 0.0f, hi[u] = c + 1 < cols ? float(__ldg(from + c + 1)) : 0.0f;
+    }
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u)
+      if (first + 64 * (u0 + u) < cols) store(first + 64 * (u0 + u), lo[u], hi[u]);
   }
 }
 
@@ -134,12 +137,36 @@ struct alignas(64) Product {
   int row_tiles, col_tiles, weight_rows, weight_cols;
   int splits, split_steps;   // of the contraction over tokens in the weights' gradients
   int dx_splits, dx_split_steps;  // of that over F in dx
+  int extra;                      // rounds of dx's tiles for the pairs with fewer of the weights'
   const void* dh;            // kGates
   void *out, *dwg, *dwu;     // h or dx; the weights' gradients
   float *parts, *dx_parts;   // (splits, 2, K, F) where splits > 1, (dx_splits, M, K) where dx_splits > 1
   __nv_bfloat16* gates;      // (plane, dg or du, M, pitch)
   int64_t pitch;
   bool wide;                 // rows of h and dh start on the boundaries of fours
+};
+
+// What pair `pair` of SMs works on, one item after the other: its share of the weights' tiles, then of dx's. The
+// pairs with one of the weights' tiles fewer take kGradients' first `extra` rounds of dx's among themselves, and
+// come first in the others.
+struct Turn {
+  int pairs, items, weights, mine, light, order, extra, at;
+  RLENV_D Turn(const Product& p, int items, bool gradients) : items(items), at(0) {
+    const int pair = blockIdx.x / 2;
+    pairs = gridDim.x / 2;
+    weights = gradients ? p.weight_rows * p.weight_cols * p.splits : 0;
+    const int heavy = weights % pairs;  // pairs with a tile of the weights more
+    mine = weights / pairs + (pair < heavy), light = pairs - heavy;
+    order = pair < heavy ? light + pair : pair - heavy;
+    extra = gradients ? p.extra : 0;
+  }
+  RLENV_D int next() {  // an item, or -1 after the last
+    const int turn = at++, round = turn - mine;
+    if (round < 0) return (order < light ? order + pairs - light : order - light) + turn * pairs;
+    const bool early = order < light && round < extra;
+    const int item = weights + (early ? round * light : extra * light + (order < light ? round - extra : round) * pairs) + order;
+    return item < items ? item : -1;
+  }
 };
 
 // Tiles are taken in bands of kBand rows of tiles, column by column, so that those in flight share
@@ -439,7 +466,7 @@ product_kernel(const __grid_constant__ Product p, int items) {
   bw::cluster_sync();
   bw::fence_after();
   const uint32_t tmem = __shfl_sync(0xffffffffu, tmem_slot, 0);
-  const int first = blockIdx.x / 2, stride = gridDim.x / 2;
+  Turn turns(p, items, kOp == kGradients);
 
   if (warp == 0) {
     // Both blocks copy their rows of A and their columns of B; all bytes count at the first block's barrier.
@@ -447,7 +474,7 @@ product_kernel(const __grid_constant__ Product p, int items) {
     uint32_t phase = 0, used = 0;  // used: stages that have been filled at least once
     bool ok = true;
     const uint32_t full_at = bw::in_block(full, 0);
-    for (int item = first; item < items && ok; item += stride) {
+    for (int item = turns.next(); item >= 0 && ok; item = turns.next()) {
       const Work w = work_of<T, kOp>(p, item);
       const Operands& in = p.in[kOp == kGradients && w.weights];
       const int r0 = (2 * w.row + rank) * kRows, c0 = w.c0 + (kPaired ? 0 : rank * C::kHalf);
@@ -494,7 +521,7 @@ product_kernel(const __grid_constant__ Product p, int items) {
       int stage = 0, buffer = 0;
       uint32_t phase = 0, buffer_phase = 0;
       bool ok = true;
-      for (int item = first; item < items && ok; item += stride) {
+      for (int item = turns.next(); item >= 0 && ok; item = turns.next()) {
         const Work w = work_of<T, kOp>(p, item);
         const int steps = w.segs * w.steps;
         const bool mn_a = w.weights, mn_b = kPaired || w.weights;
@@ -569,24 +596,29 @@ product_kernel(const __grid_constant__ Product p, int items) {
       const uint32_t at = tmem + lanes + buffer * kBufferColumns + from + column(j);
       bw::tmem_load16x2(v, at, at + (kPaired ? C::kHalf : 16));
     };
-    for (int item = first; item < items; item += stride) {
-      const Work w = work_of<T, kOp>(p, item);
-      const int64_t r0 = int64_t(2 * w.row + rank) * kRows + 32 * quarter;
-      // A run of results goes out while the next one's accumulators and gradients are on their way, the first
-      // gradients under the tile's products.
-      typename Four<T>::type dh[2][4];
-      const auto load_dh = [&](int j) {
-        if constexpr (kOp == kGates)
-          if (j < kRuns) load_gradient<T>(p, r0, w.c0 + column(j), dh[j & 1]);
-      };
-      const auto finish_run = [&](uint32_t (&v)[32], int j) {
+    // A run of results goes out while the next one's accumulators and gradients are on their way, the next tile's
+    // first gradients among them.
+    typename Four<T>::type dh[2][4];
+    const auto rows_of = [&](const Work& w) { return int64_t(2 * w.row + rank) * kRows + 32 * quarter; };
+    int item = turns.next();
+    Work next = item >= 0 ? work_of<T, kOp>(p, item) : Work{};
+    const auto load_dh = [&](const Work& w, int j) {
+      if constexpr (kOp == kGates) load_gradient<T>(p, rows_of(w), w.c0 + column(j), dh[j & 1]);
+    };
+    if (item >= 0) load_dh(next, 0);
+    while (item >= 0) {
+      const Work w = next;
+      item = turns.next();
+      const bool another = item >= 0;
+      if (another) next = work_of<T, kOp>(p, item);
+      const int64_t r0 = rows_of(w);
+      const auto finish_run = [&](uint32_t (&v)[32], int j, const typename Four<T>::type (&d)[4]) {
         if (!ok) {  // a wait ran out: the results say so
 #pragma unroll
           for (int i = 0; i < 32; ++i) v[i] = 0x7fffffffu;
         }
-        finish<T, kOp>(p, w, r0, w.c0 + column(j), v, dh[j & 1], own_stage);
+        finish<T, kOp>(p, w, r0, w.c0 + column(j), v, d, own_stage);
       };
-      load_dh(0);
       if constexpr (C::kFloat) {
         float sum[kRuns][32];
 #pragma unroll
@@ -609,14 +641,13 @@ product_kernel(const __grid_constant__ Product p, int items) {
             }
           take_next();
         }
+        static_assert(kRuns == 1, "a float32 tile's columns are one run a thread");
+        uint32_t v[32];
 #pragma unroll
-        for (int j = 0; j < kRuns; ++j) {
-          load_dh(j + 1);
-          uint32_t v[32];
-#pragma unroll
-          for (int i = 0; i < 32; ++i) v[i] = __float_as_uint(sum[j][i]);
-          finish_run(v, j);
-        }
+        for (int i = 0; i < 32; ++i) v[i] = __float_as_uint(sum[0][i]);
+        typename Four<T>::type d[4] = {dh[0][0], dh[0][1], dh[0][2], dh[0][3]};
+        if (another) load_dh(next, 0);
+        finish_run(v, 0, d);
       } else {
         ok = bw::barrier_wait_warp(summed + 8 * buffer, buffer_phase, dead) && ok;
         bw::fence_after();
@@ -626,13 +657,14 @@ product_kernel(const __grid_constant__ Product p, int items) {
         for (int j = 0; j < kRuns; j += 2) {
           bw::tmem_ready(even);
           load_run(odd, j + 1);
-          load_dh(j + 1);
-          finish_run(even, j);
+          load_dh(w, j + 1);
+          finish_run(even, j, dh[0]);
           bw::tmem_ready(odd);
           if (j + 2 < kRuns) load_run(even, j + 2);
           else take_next();  // all of the accumulator is read
-          load_dh(j + 2);
-          finish_run(odd, j + 1);
+          if (j + 2 < kRuns) load_dh(w, j + 2);
+          else if (another) load_dh(next, 0);
+          finish_run(odd, j + 1, dh[1]);
         }
       }
     }
@@ -971,30 +1003,55 @@ int64_t planes(int dtype) { return dtype == RLENV_F32 ? 3 : 1; }
 struct Layout {  // scratch of a call
   void *x, *wg, *wu, *gates;
   float *parts, *dx_parts;
-  int splits, split_steps, dx_splits, dx_split_steps;
+  int splits, split_steps, dx_splits, dx_split_steps, extra;
   int64_t bytes;
 };
 
 constexpr int kPairsOfSms = 74;
 constexpr int64_t kFewestSteps = 8;
 
+// The longest share of a pair of SMs, in steps, when the weights' tiles of Lw steps and dx's of Ld are dealt as
+// Turn does, with `extra` rounds of dx's for the pairs that have a tile of the weights fewer.
+double longest_share(int64_t weights, double lw, int64_t dx, double ld, int64_t extra) {
+  const int64_t pairs = weights + dx < kPairsOfSms ? weights + dx : kPairsOfSms;
+  const int64_t each = weights / pairs, heavy = weights % pairs, light = pairs - heavy;
+  const int64_t rest = dx > extra * light ? dx - extra * light : 0, rounds = rest / pairs, left = rest % pairs;
+  const double a = heavy ? (each + 1) * lw + (rounds + (left > light)) * ld : 0.0;
+  const double b = each * lw + (extra + rounds + (left > 0)) * ld;
+  return a > b ? a : b;
+}
+
 // The gradients' contractions are split where a tile would take longer than a pair of SMs' share of all the
-// work: a small block's weights are a few tiles, each a sum over every token; few tokens' dx a few, each a sum
-// over all of F. The parts' sums are kept in float32 and added up in order.
+// work, or the shares would be uneven: a small block's weights are a few tiles, each a sum over every token; few
+// tokens' dx a few, each a sum over all of F. The parts' sums are kept in float32 and added up in order, which
+// costs their writing and reading, at some 5 TB/s, and a launch, 4 us. Of the numbers of parts from the least
+// that keeps a tile within the share to three more, the ones with the shortest longest share, plus that cost.
 void split_gradients(int dtype, int64_t m, int64_t k, int64_t f, Layout* l) {
-  const int64_t wide = dtype == RLENV_F32 ? Tile<float>::kCols : Tile<__nv_bfloat16>::kCols, high = 2 * kRows;
-  const int64_t step = dtype == RLENV_F32 ? Tile<float>::kStep : Tile<__nv_bfloat16>::kStep;
-  const int64_t steps = (m + step - 1) / step, tiles = (k + high - 1) / high * ((f + wide - 1) / wide) * 2;
-  const int64_t dx_steps = (f + step - 1) / step, dx_tiles = (m + high - 1) / high * ((k + wide - 1) / wide);
+  const bool is_float = dtype == RLENV_F32;
+  const int64_t wide = is_float ? Tile<float>::kCols : Tile<__nv_bfloat16>::kCols, high = 2 * kRows;
+  const int64_t steps = (m + kBlock - 1) / kBlock, tiles = (k + high - 1) / high * ((f + wide - 1) / wide) * 2;
+  const int64_t dx_steps = (f + kBlock - 1) / kBlock, dx_tiles = (m + high - 1) / high * ((k + wide - 1) / wide);
+  // A step's time; what a tile takes besides its steps, and at the least (its epilogue), in steps. As measured.
+  const double step_us = is_float ? 1.06 : 0.36, turn = 0.5, least = is_float ? 2.0 : 10.0;
+  const auto length = [&](int64_t n) { return turn + (n > least ? n : least); };
   int64_t share = (tiles * steps + 2 * dx_tiles * dx_steps) / kPairsOfSms;
   if (share < kFewestSteps) share = kFewestSteps;
-  const auto split = [](int64_t all, int64_t most, int* count, int* each) {
-    const int64_t parts = (all + most - 1) / most;
-    *each = int((all + parts - 1) / parts);
-    *count = int((all + *each - 1) / *each);
-  };
-  split(steps, share, &l->splits, &l->split_steps);
-  split(dx_steps, (share + 1) / 2, &l->dx_splits, &l->dx_split_steps);
+  double best = 0.0;
+  const int64_t a0 = (steps + share - 1) / share, b0 = (2 * dx_steps + share - 1) / share;
+  for (int64_t i = 0; i < 4; ++i)
+    for (int64_t j = 0; j < 4; ++j) {
+      const int64_t each = (steps + a0 + i - 1) / (a0 + i), dx_each = (dx_steps + b0 + j - 1) / (b0 + j);
+      const int64_t a = (steps + each - 1) / each, b = (dx_steps + dx_each - 1) / dx_each;
+      const double bytes = (a > 1 ? 16.0 * a * k * f : 0.0) + (b > 1 ? 8.0 * b * m * k : 0.0);
+      const double cost = bytes > 0.0 ? (4.0 + bytes / 5e6) / step_us : 0.0, lw = length(each), ld = length(2 * dx_each);
+      for (int64_t extra = int64_t(lw / ld); extra <= int64_t(lw / ld) + 1; ++extra) {
+        const double all = cost + longest_share(tiles * a, lw, dx_tiles * b, ld, extra);
+        if (best > 0.0 && all >= best) continue;
+        best = all;
+        l->splits = int(a), l->split_steps = int(each), l->dx_splits = int(b), l->dx_split_steps = int(dx_each);
+        l->extra = int(extra);
+      }
+    }
 }
 Layout lay_out(int dtype, int64_t m, int64_t k, int64_t f, bool backward, void* scratch) {
   Scratch s{static_cast<unsigned char*>(scratch), 0};
@@ -1045,7 +1102,7 @@ int run_product(const Product& p, cudaStream_t s) {
   using C = Tile<T>;
   const int64_t items = int64_t(p.row_tiles) * p.col_tiles * (kOp == kGradients ? p.dx_splits : 1) +
                         int64_t(p.weight_rows) * p.weight_cols * p.splits;
-  if (items > 0x7fffffff) return RLENV_EINVAL;
+  if (items > 0x7fff0000) return RLENV_EINVAL;
   int dev = 0, sms = 0;
   if (cudaError_t e = cudaGetDevice(&dev)) return int(e);
   if (cudaError_t e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev)) return int(e);
@@ -1083,7 +1140,7 @@ int ffn(const void* dh, const void* x, const void* wg, const void* wu, int64_t m
   if (const int rc = run_product<T, kGates>(p, s)) return rc;
   const Operand D{p.gates, m, f, p.pitch, 2 * C::kPlanes};
   p.out = dx, p.dwg = dwg, p.dwu = dwu, p.parts = l.parts, p.splits = l.splits, p.split_steps = l.split_steps;
-  p.dx_parts = l.dx_parts, p.dx_splits = l.dx_splits, p.dx_split_steps = l.dx_split_steps;
+  p.dx_parts = l.dx_parts, p.dx_splits = l.dx_splits, p.dx_split_steps = l.dx_split_steps, p.extra = l.extra;
   p.col_tiles = tile_count(k, C::kCols);
   p.weight_rows = tile_count(k, 2 * kRows), p.weight_cols = 2 * tile_count(f, C::kCols);
   if (const int rc = D.map(&p.in[0].a, kRows)) return rc;
