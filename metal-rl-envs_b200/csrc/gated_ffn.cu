@@ -101,21 +101,22 @@ constexpr int kBlock = 64;       // of the contraction: a tile row's 128 bytes
 constexpr int kTmemColumns = 512, kBufferColumns = 256;
 constexpr int kStageFloats = 32 * 32;  // the epilogue's tile of a warp
 
-template <typename T>
+template <typename T, int kOp = kForward>
 struct Tile {
   static constexpr bool kFloat = sizeof(T) == 4;
   static constexpr int kPlanes = kFloat ? 3 : 1;
   static constexpr int kCols = kFloat ? 128 : 256;
   static constexpr int kHalf = kCols / 2;        // columns of B in each block
-  // Warps: copies, products, two idle ones, and those of the epilogue. float32's, with the exact exponential
-  // and error function and three planes to store, needs twice as many to hide its latencies.
-  static constexpr int kEpilogue = kFloat ? 16 : 8;
+  // Warps: copies, products, two idle ones, and those of the epilogue: sixteen where it computes (16,384 x 512 x
+  // 1,376 in bfloat16, 34 us forward against 41 with eight, the gates 60 against 70). bfloat16's plain results want
+  // the shared memory of the other eight as a sixth ring buffer (8,192 x 1,024 x 2,720, 125 us against 131).
+  static constexpr int kEpilogue = kFloat || kOp != kGradients ? 16 : 8;
   static constexpr int kThreads = 128 + 32 * kEpilogue;
   static constexpr int kMine = kCols / (kEpilogue / 4);  // columns of the accumulator that a thread reads
   static constexpr int kStep = kBlock;
   static constexpr int kABytes = kRows * kBlock * 2;
   static constexpr int kRingBytes = kABytes + kHalf * kBlock * 2;  // a ring buffer: a plane of both operands
-  static constexpr int kStages = 6;
+  static constexpr int kStages = kFloat || kOp == kGradients ? 6 : 5;
   static constexpr int kStageAt = kStages * kRingBytes;  // the epilogue's 32 x 32 tiles, one a warp
   // the ring starts on a 1,024-byte boundary
   static constexpr int kSmem = kStageAt + kEpilogue * kStageFloats * 4 + 1024;
@@ -439,9 +440,9 @@ RLENV_D void finish(const Product& p, const Work& w, int64_t r0, int64_t c, cons
 }
 
 template <typename T, int kOp>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Tile<T>::kThreads, 1)
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Tile<T, kOp>::kThreads, 1)
 product_kernel(const __grid_constant__ Product p, int items) {
-  using C = Tile<T>;
+  using C = Tile<T, kOp>;
   constexpr bool kPaired = kOp != kGradients;  // half of a tile's columns are gates, half ups
   constexpr uint32_t kBox = 64 * kBlock * 2;
   extern __shared__ unsigned char raw[];
@@ -651,20 +652,19 @@ product_kernel(const __grid_constant__ Product p, int items) {
       } else {
         ok = bw::barrier_wait_warp(summed + 8 * buffer, buffer_phase, dead) && ok;
         bw::fence_after();
-        uint32_t even[32], odd[32];
-        load_run(even, 0);
-#pragma unroll 1
-        for (int j = 0; j < kRuns; j += 2) {
-          bw::tmem_ready(even);
-          load_run(odd, j + 1);
-          load_dh(w, j + 1);
-          finish_run(even, j, dh[0]);
-          bw::tmem_ready(odd);
-          if (j + 2 < kRuns) load_run(even, j + 2);
-          else take_next();  // all of the accumulator is read
-          if (j + 2 < kRuns) load_dh(w, j + 2);
+        // Where the registers allow, the next run is read while this one goes out.
+        constexpr int kAhead = kOp == kGradients;
+        uint32_t v[1 + kAhead][32];
+        load_run(v[0], 0);
+#pragma unroll
+        for (int j = 0; j < kRuns; ++j) {
+          bw::tmem_ready(v[j & kAhead]);
+          if (kAhead && j + 1 < kRuns) load_run(v[(j + 1) & kAhead], j + 1);
+          if (j + 1 == kRuns) take_next();  // all of the accumulator is read
+          if (j + 1 < kRuns) load_dh(w, j + 1);
           else if (another) load_dh(next, 0);
-          finish_run(odd, j + 1, dh[1]);
+          finish_run(v[j & kAhead], j, dh[j & 1]);
+          if (!kAhead && j + 1 < kRuns) load_run(v[0], j + 1);
         }
       }
     }
@@ -1099,7 +1099,7 @@ int operands(const void* const (&from)[3], const int64_t (&rows)[3], const int64
 
 template <typename T, int kOp>
 int run_product(const Product& p, cudaStream_t s) {
-  using C = Tile<T>;
+  using C = Tile<T, kOp>;
   const int64_t items = int64_t(p.row_tiles) * p.col_tiles * (kOp == kGradients ? p.dx_splits : 1) +
                         int64_t(p.weight_rows) * p.weight_cols * p.splits;
   if (items > 0x7fff0000) return RLENV_EINVAL;
