@@ -11,10 +11,12 @@
 // A pair reads a 256 x 256 tile's operands once between its two SMs, 64 bytes a clock for each, where single
 // SMs with tiles of 128 x 256 read 96.
 //
-// Measured, bfloat16: a step of 64 of the contraction takes a pair 515 cycles of at least 512, so that the
-// clock under the power limit is what is left: 16,384 x 1,024 x 4,096 forward 172 us in a short run (1.60
-// PFLOP/s), 211 us sustained; the gates' epilogue, with dh to read and two results, 643 cycles a step at 1,024
-// deep. float32: 4,096 x 1,024 x 1,024 forward 91 us (188 TFLOP/s of float32 products, six times that formed).
+// Measured: a step of 64 of the contraction takes a pair 515 cycles of at least 512 in bfloat16, and three such in
+// float32 (six products of half as wide a tile), so that the clock under the power limit is what is left of
+// long contractions: 16,384 x 1,024 x 4,096 forward 171 us in a short run (1.61 PFLOP/s), 211 us sustained;
+// float32 4,330 x 881 x 1,780 forward 104 us. Where the contraction is short the epilogues bound, by their
+// instructions and the latency of their few turns: 16,384 x 512 x 1,376 34 us, its gates 60 us, float32's of
+// 18,500 x 97 x 250 30 us.
 // float32 operands are sums of three bfloat16 planes (8 + 8 + 8 bits of mantissa), laid out by
 // pack_kernel; a product of two is six products of planes, the three below 2^-24 left out.
 #include <cuda_bf16.h>
@@ -145,6 +147,7 @@ struct alignas(64) Product {
   __nv_bfloat16* gates;      // (plane, dg or du, M, pitch)
   int64_t pitch;
   bool wide;                 // rows of h and dh start on the boundaries of fours
+  bool turned;               // the weights' gradients are formed as their transposes, dg' x and du' x
 };
 
 // What pair `pair` of SMs works on, one item after the other: its share of the weights' tiles, then of dx's. The
@@ -216,8 +219,8 @@ RLENV_D Work work_of(const Product& p, int item) {
 
 // A step's planes in the order in which they are copied. A plane's products with those before it follow its
 // arrival: 1 1, then 0 1, 1 0 and 0 0, then 0 2 and 2 0. Each is read from L2 once for all of its products
-// (measured against a pass over the contraction for each product, 96 bytes a clock and SM: TODO), and the first
-// buffer is free again halfway through.
+// (48 bytes a clock and SM; with a pass over the contraction for each product it was 96, more than L2 gives, and
+// 4,330 x 881 x 1,780 forward took 125 us instead of 104), and the first buffer is free again halfway through.
 template <typename T>
 RLENV_D int plane_of(int turn) { return Tile<T>::kFloat ? 0x21 >> (2 * turn) & 3 : 0; }
 
@@ -414,10 +417,25 @@ RLENV_D void finish_values(T* to, int64_t pitch, int64_t rows, int64_t cols, flo
 template <typename T, int kOp>
 RLENV_D void finish(const Product& p, const Work& w, int64_t r0, int64_t c, const uint32_t (&v)[32],
                     const typename Four<T>::type (&dh)[4], float* stage) {
-  const int64_t all_rows = kOp == kGradients && w.weights ? p.k : p.m;
-  const int64_t all_cols = kOp == kGradients && !w.weights ? p.k : p.f;
+  const bool turned = kOp == kGradients && w.weights && p.turned;
+  const int64_t all_rows = kOp != kGradients || !w.weights ? p.m : turned ? p.f : p.k;
+  const int64_t all_cols = kOp == kGradients && (turned || !w.weights) ? p.k : p.f;
   if (r0 >= all_rows || c >= all_cols) return;
   const int lane = threadIdx.x & 31;
+  if constexpr (kOp == kGradients && Tile<T>::kFloat) {
+    if (turned) {  // a column of the tile lies in a row of the gradient
+      float* to = p.splits > 1 ? p.parts + (int64_t(w.split) * 2 + w.weight) * p.k * p.f
+                               : static_cast<float*>(w.weight ? p.dwu : p.dwg);
+      to += c * p.f + r0 + lane;
+      const int cols = int(min(int64_t(32), p.k - c));
+      if (r0 + lane < p.f) {
+#pragma unroll
+        for (int i = 0; i < 32; ++i)
+          if (i < cols) to[i * p.f] = __uint_as_float(v[i]);
+      }
+      return;
+    }
+  }
   __syncwarp();
 #pragma unroll
   for (int i = 0; i < 8; ++i)
@@ -487,8 +505,9 @@ product_kernel(const __grid_constant__ Product p, int items) {
         for (int k = w.k0 * C::kStep; k < k_end && ok; k += C::kStep) {  // what lies past the contraction reads as zero
           for (int turn = 0; turn < C::kPlanes; ++turn) {
             const int plane = plane_of<T>(turn);
-            const int slice_a = kPaired || w.weights ? plane : 2 * plane + seg;
-            const int slice_b = !kPaired && w.weights ? 2 * plane + w.weight : plane;
+            const int of_gates = 2 * plane + (!kPaired && w.weights ? w.weight : seg);
+            const int slice_a = !kPaired && (!w.weights || p.turned) ? of_gates : plane;
+            const int slice_b = !kPaired && w.weights && !p.turned ? of_gates : plane;
             const uint32_t bar = full_at + 8 * stage, a = ring + stage * C::kRingBytes, b = a + C::kABytes;
             if (!(ok = bw::barrier_wait_warp(empty + 8 * stage, phase ^ 1, dead))) break;
             if (bw::elect()) {
@@ -692,7 +711,7 @@ add_parts_kernel(const float* __restrict__ parts, int splits, int64_t size, T* _
   const int64_t stride = of_dx ? dx_size : 2 * size;
   const int count = of_dx ? dx_splits : splits;
   float sum = 0.0f;
-#pragma unroll 4
+#pragma unroll 8
   for (int s = 0; s < count; ++s) sum += __ldg(from + s * stride + e);
   T* to = of_dx ? dx : e < size ? dwg : dwu;
   to[!of_dx && e >= size ? e - size : e] = T(sum);
@@ -943,25 +962,26 @@ int few_rows(const void* x, const void* wg, const void* wu, int64_t m, int64_t k
 
 // Whether the products are formed this way: a few rows in any case, more where the blocks of 8 rows and 32
 // columns are one round on the SMs (bfloat16) or three (float32, whose tiles have the weights laid out as planes
-// first). Measured in us, this way and by tiles: bfloat16 1,024 x 4,096, 1 row 5.1 and 12.2, 8 rows 11.4 and 11.2,
-// 16 rows 21.0 and 11.2; 1,024 x 16,384, 4 rows 21.9 and 21.3, 8 rows 38.8 and 21.1; 512 x 512, 72 rows 8.1 and
-// 8.7, 96 rows 14.7 and 8.8; 4,096 x 1,024, 16 rows 29.2 and 24.3 (the rule's worst); float32 1,024 x 4,096, 24
-// rows 26.5 and 41.2, 48 rows 50.7 and 41.4; 1,024 x 16,384, 24 rows 165 and 166; 512 x 512, 216 rows 16.5 and
-// 17.5, 256 rows 21.1 and 17.6.
+// first). Measured in us, this way and by tiles: bfloat16 1,024 x 4,096, 1 row 5.0 and 12.9, 8 rows 11.3 and 10.7,
+// 16 rows 21.0 and 10.6; 1,024 x 16,384, 4 rows 21.8 and 21.1, 8 rows 38.7 and 20.9; 512 x 512, 72 rows 8.0 and
+// 8.3, 96 rows 14.6 and 8.4; 4,096 x 1,024, 16 rows 29.2 and 23.8 (the rule's worst); float32 1,024 x 4,096, 24
+// rows 26.4 and 31.4, 32 rows 34.5 and 31.4; 1,024 x 16,384, 16 rows 108 and 125, 24 rows 165 and 121; 512 x 512,
+// 192 rows 16.3 and 15.9, 256 rows 21.1 and 16.0; 97 x 250, 256 rows 7.5 and 10.7, 448 rows 13.4 and 10.9.
 bool few_rows_fit(int dtype, int64_t m, int64_t f) {
   const bool wide = dtype == RLENV_F32;
   const int64_t blocks = (m + 7) / 8 * ((f + kFewCols - 1) / kFewCols);
-  return m <= (wide ? 24 : 4) || blocks <= 148 * (wide ? 3 : 1);
+  return m <= (wide ? 16 : 4) || blocks <= 148 * (wide ? 3 : 1);
 }
-// The same for the gradient, whose tiles cost two launches more and work on 256 rows however few there are; this
-// way takes longer by the row. Measured in us, this way and by tiles: float32 1,024 x 4,096, 1 row 20 and 143, 32
-// rows 91 and 94, 64 rows 166 and 96; 1,024 x 1,024, 64 rows 53.5 and 54.2; 97 x 250, 128 rows 26.3 and 27.8;
-// bfloat16 922 x 5,556, 4 rows 39 and 44, 8 rows 51 and 45; 1,024 x 1,024, 16 rows 22.2 and 22.7, 24 rows 25.9 and
-// 23.2; 97 x 250, 32 rows 14.5 and 21.0, 128 rows 28.1 and 21.9; 512 x 512, 64 rows 21.4 and 21.0.
+// The same for the gradient, whose tiles cost a launch or two more and work on 256 rows however few there are; this
+// way takes longer by the row. Measured in us, this way and by tiles: float32 1,024 x 4,096, 1 row 20 and 73, 16
+// rows 53 and 67, 24 rows 73 and 67; 1,024 x 1,024, 32 rows 29.5 and 39.9, 48 rows 45 and 40; 83 x 3,683, 48 rows
+// 28.1 and 29.6, 64 rows 35.6 and 29.7; 512 x 512, 64 rows 20 and 28. bfloat16 922 x 5,556, 4 rows 39 and 43, 8
+// rows 52 and 40; 1,024 x 4,096, 8 rows 28.3 and 30.3; 97 x 250, 32 rows 14 and 20; 512 x 512, 8 rows 11 and 20, 32
+// rows 16 and 21; 83 x 3,683, 16 rows 26 and 23; 2,000 x 100, 4 rows 24 and 25.5, 8 rows 32 and 25.5.
 bool few_gradients_fit(int dtype, int64_t m, int64_t k, int64_t f) {
   const double products = double(m) * double(k) * double(f);
-  return dtype == RLENV_F32 ? m <= 32 || (m <= 128 && products <= 67108864.0)
-                            : m <= 4 || (m <= 32 && products <= 16777216.0);
+  return dtype == RLENV_F32 ? m <= 16 || (m <= 48 && products <= 33554432.0)
+                            : m <= 4 || (m <= 32 && products <= 2097152.0);
 }
 
 // ---- host ------------------------------------------------------------------------------------------
@@ -1010,6 +1030,13 @@ struct Layout {  // scratch of a call
 constexpr int kPairsOfSms = 74;
 constexpr int64_t kFewestSteps = 8;
 
+// Whether the weights' gradients take fewer tiles as their transposes: a tile of float32 values is twice as high as
+// wide (18,500 x 97 x 250: both gradients 29 us against 35).
+bool turns(int dtype, int64_t k, int64_t f) {
+  constexpr int64_t kHigh = 2 * kRows, kWide = Tile<float>::kCols;
+  return dtype == RLENV_F32 && round_up(f, kHigh) * round_up(k, kWide) < round_up(k, kHigh) * round_up(f, kWide);
+}
+
 // The longest share of a pair of SMs, in steps, when the weights' tiles of Lw steps and dx's of Ld are dealt as
 // Turn does, with `extra` rounds of dx's for the pairs that have a tile of the weights fewer.
 double longest_share(int64_t weights, double lw, int64_t dx, double ld, int64_t extra) {
@@ -1029,7 +1056,8 @@ double longest_share(int64_t weights, double lw, int64_t dx, double ld, int64_t 
 void split_gradients(int dtype, int64_t m, int64_t k, int64_t f, Layout* l) {
   const bool is_float = dtype == RLENV_F32;
   const int64_t wide = is_float ? Tile<float>::kCols : Tile<__nv_bfloat16>::kCols, high = 2 * kRows;
-  const int64_t steps = (m + kBlock - 1) / kBlock, tiles = (k + high - 1) / high * ((f + wide - 1) / wide) * 2;
+  const int64_t rows = turns(dtype, k, f) ? f : k, cols = turns(dtype, k, f) ? k : f;
+  const int64_t steps = (m + kBlock - 1) / kBlock, tiles = (rows + high - 1) / high * ((cols + wide - 1) / wide) * 2;
   const int64_t dx_steps = (f + kBlock - 1) / kBlock, dx_tiles = (m + high - 1) / high * ((k + wide - 1) / wide);
   // A step's time; what a tile takes besides its steps, and at the least (its epilogue), in steps. As measured.
   const double step_us = is_float ? 1.06 : 0.36, turn = 0.5, least = is_float ? 2.0 : 10.0;
@@ -1142,12 +1170,13 @@ int ffn(const void* dh, const void* x, const void* wg, const void* wu, int64_t m
   p.out = dx, p.dwg = dwg, p.dwu = dwu, p.parts = l.parts, p.splits = l.splits, p.split_steps = l.split_steps;
   p.dx_parts = l.dx_parts, p.dx_splits = l.dx_splits, p.dx_split_steps = l.dx_split_steps, p.extra = l.extra;
   p.col_tiles = tile_count(k, C::kCols);
-  p.weight_rows = tile_count(k, 2 * kRows), p.weight_cols = 2 * tile_count(f, C::kCols);
+  p.turned = turns(kDtype, k, f);
+  p.weight_rows = tile_count(p.turned ? f : k, 2 * kRows), p.weight_cols = 2 * tile_count(p.turned ? k : f, C::kCols);
   if (const int rc = D.map(&p.in[0].a, kRows)) return rc;
   if (const int rc = G.map(&p.in[0].b0, C::kHalf)) return rc;
   if (const int rc = U.map(&p.in[0].b1, C::kHalf)) return rc;
-  if (const int rc = X.map(&p.in[1].a, 64)) return rc;
-  if (const int rc = D.map(&p.in[1].b0, 64)) return rc;
+  if (const int rc = (p.turned ? D : X).map(&p.in[1].a, 64)) return rc;
+  if (const int rc = (p.turned ? X : D).map(&p.in[1].b0, 64)) return rc;
   if (const int rc = run_product<T, kGradients>(p, s)) return rc;
   const int64_t sums = (l.splits > 1 ? 2 * k * f : 0) + (l.dx_splits > 1 ? m * k : 0);
   if (sums == 0) return RLENV_OK;

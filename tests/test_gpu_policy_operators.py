@@ -338,6 +338,19 @@ def test_ffn_backward_of_few_rows(cuda, m, k, f, dtype):
     test_ffn_backward(cuda, m, k, f, "gelu", dtype)
 
 
+@pytest.mark.parametrize("m,k,f", [(300, 40, 200), (1500, 97, 250), (6000, 17, 129), (700, 128, 511), (2100, 250, 97)])
+def test_ffn_backward_of_narrow_weights(cuda, m, k, f):
+    """float32 weights' gradients formed as their transposes, whole and in parts, and a shape that is not."""
+    test_ffn_backward(cuda, m, k, f, "silu", "f32")
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("m,k,f", [(5000, 300, 520), (9000, 130, 70), (2600, 600, 260)])
+def test_ffn_backward_dealt_unevenly(cuda, m, k, f, dtype):
+    """Several tiles a pair of SMs, of both kinds and of unequal lengths."""
+    test_ffn_backward(cuda, m, k, f, "gelu", dtype)
+
+
 def test_ffn_gradient_of_few_rows_with_infinities(cuda):
     """Sums of products as the formula has them: what is not finite stays with its own token and column."""
     import gated_ffn
