@@ -51,8 +51,12 @@ chunk_kernel(const __grid_constant__ Problem p, const __grid_constant__ Split sp
   const bool whole = segments == 1;
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int rb = warp % C::kRowWarps * C::RT;         // this warp's first 16 tokens,
-  const int oc = warp / C::kRowWarps * C::OC;         // and output columns
+  // This warp's first 16 tokens and output columns. Later tokens have more before them, and a scheduler has the same
+  // warps of every block: the warps of the other columns stand the other way round (float32 heads of 128, 16,384
+  // tokens: 311 us against 356), and those of Shape::kTurning change places from chunk to chunk.
+  int rb = warp % C::kRowWarps * C::RT;
+  if (warp >= C::kRowWarps) rb = (C::kRowWarps - 1) * C::RT - rb;
+  const int oc = warp / C::kRowWarps * C::OC;
   const int gr = lane >> 2, gc = (lane & 3) * 2;      // a fragment's row and column
   const float log2_g = log2f(__ldg(p.decay + h));
   const int f = s.reverse ? 0 : 1;
@@ -112,7 +116,7 @@ chunk_kernel(const __grid_constant__ Problem p, const __grid_constant__ Split sp
   const int64_t token_step = p.n * p.h * D, out_step = s.reverse ? -token_step : token_step;
   T* out_at;
   {
-    const int64_t i = first + 16 * rb + lane / kPieces;
+    const int64_t i = first + (C::kTurning ? 0 : 16 * rb) + lane / kPieces;
     out_at = static_cast<T*>(s.out) + (s.reverse ? p.t - 1 - i : i) * token_step + int64_t(seq) * D + col + oc + lane % kPieces * kPer;
   }
   if (p.resets && first < last) read_resets(first);
@@ -123,6 +127,12 @@ chunk_kernel(const __grid_constant__ Problem p, const __grid_constant__ Split sp
   // The weights, `scale` among them, between 16 tokens and 16 others: on the diagonal, and one block to its
   // left; and from the carry to this warp's tokens.
   float near[8], next[8], row_decay[C::RT][2];
+  const auto decay_rows = [&] {
+#pragma unroll
+    for (int r = 0; r < C::RT; ++r)
+#pragma unroll
+      for (int half = 0; half < 2; ++half) row_decay[r][half] = p.scale * powers[16 * (rb + r) + gr + 8 * half + f];
+  };
   if constexpr (!kLocal) {
 #pragma unroll
     for (int q = 0; q < 8; ++q) {
@@ -130,13 +140,9 @@ chunk_kernel(const __grid_constant__ Problem p, const __grid_constant__ Split sp
       near[q] = apart >= 0 ? p.scale * powers[apart] : 0.0f;
       next[q] = p.scale * powers[16 + apart];
     }
-#pragma unroll
-    for (int r = 0; r < C::RT; ++r)
-#pragma unroll
-      for (int half = 0; half < 2; ++half) row_decay[r][half] = p.scale * powers[16 * (rb + r) + gr + 8 * half + f];
+    decay_rows();
   }
   const float block_decay = powers[16];
-
 
   float bad = 0.0f;      // NaN once any value is not finite
   bool cut = false;      // a reset anywhere in the segment
@@ -323,7 +329,7 @@ chunk_kernel(const __grid_constant__ Problem p, const __grid_constant__ Split sp
         for (int e = 0; e < 16 * C::RT / kRowsOut; ++e) {
           const int r = lane / kPieces + e * kRowsOut;
           if (16 * rb + r < len)
-            *reinterpret_cast<uint4*>(out_at + e * kRowsOut * out_step) =
+            *reinterpret_cast<uint4*>(out_at + ((C::kTurning ? 16 * rb : 0) + e * kRowsOut) * out_step) =
                 *reinterpret_cast<const uint4*>(own + r * C::PX + lane % kPieces * kPer);
         }
       } else {
@@ -347,6 +353,10 @@ chunk_kernel(const __grid_constant__ Problem p, const __grid_constant__ Split sp
     }
 
     out_at += kChunk * out_step;
+    if (!kLocal && C::kTurning) {
+      rb = rb + C::RT < C::kRowWarps * C::RT ? rb + C::RT : 0;
+      decay_rows();
+    }
 
     // Z <- g^L Z + (l * A)' B, l_j = g^(L - f - j) where no reset lies between token j and the end
     if (holds) {

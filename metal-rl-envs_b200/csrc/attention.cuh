@@ -149,6 +149,9 @@ struct Shape {
   static constexpr int kThreads = 32 * kWarps;
   static constexpr int RT = 4 / kRowWarps;
   static constexpr int OC = DB / kColWarps;             // output columns a warp
+  // Warps change places from chunk to chunk (500 steps of 1,024 float32 heads of 64: 351 us against 386; bfloat16 heads
+  // of 32: 114 against 121), but where the arithmetic of it costs as much (bfloat16 heads of 64: 243 against 233).
+  static constexpr bool kTurning = kColWarps == 1 && (kFloat ? D >= 32 : D == 32);
   // Tiles come a chunk ahead: bfloat16 ones in a second buffer (cp.async), but at 128 columns, where a second
   // block on the SM is worth more; float32 ones through registers, where they become planes.
   static constexpr int kBuffers = kFloat || D == 128 ? 1 : 2;
