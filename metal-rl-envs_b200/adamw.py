@@ -79,7 +79,7 @@ def _check_state(state):
 
 
 def _expect(name, x, dtype, n, index):
-    if x is None or x.dtype is not dtype or x.numel() != n or not x.is_contiguous() or x.get_device() != index \
+    if not isinstance(x, torch.Tensor) or x.dtype is not dtype or x.numel() != n or not x.is_contiguous() or x.get_device() != index \
             or index < 0:
         raise ValueError(f"{name} must be {n} contiguous {dtype} elements on the state's CUDA device")
 
@@ -91,8 +91,12 @@ _dense, _pointer = torch.Tensor.is_contiguous, torch.Tensor.data_ptr
 def _check_list(name, tensors, dtype, sizes, index):
     """Every tensor dense, of dtype, on the device, of its size: the whole list in a few passes that run in
     the interpreter's C loops (a policy has dozens of small tensors and a step of some microseconds)."""
-    if set(map(_dtype, tensors)) != {dtype} or set(map(_index, tensors)) != {index} or not all(map(_dense, tensors)) \
-            or tuple(map(_numel, tensors)) != sizes:
+    try:
+        fit = set(map(_dtype, tensors)) == {dtype} and set(map(_index, tensors)) == {index} \
+            and all(map(_dense, tensors)) and tuple(map(_numel, tensors)) == sizes
+    except (AttributeError, TypeError):  # None, say: a parameter without a gradient
+        fit = False
+    if not fit:
         raise ValueError(f"{name} must be contiguous {dtype} tensors on cuda:{index} of the state's sizes {sizes}")
 
 
@@ -107,14 +111,14 @@ def step(params, grads, state, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_dec
     if count == 0:
         state.step += 1
         return
-    index, grad_dtype = _check_state(state), grads[0].dtype
+    index, grad_dtype = _check_state(state), getattr(grads[0], "dtype", None)
     if grad_dtype not in _rl.FLOAT_DTYPES:
         raise ValueError(f"grads must be float32 or bfloat16; got {grad_dtype}")
     _check_list("params", params, torch.float32, sizes, index)
     try:
         _check_list("grads", grads, grad_dtype, sizes, index)
     except ValueError:  # a gradient with strides is copied; anything else raises here
-        grads = [g.contiguous() for g in grads]
+        grads = [g.contiguous() if isinstance(g, torch.Tensor) else g for g in grads]
         _check_list("grads", grads, grad_dtype, sizes, index)
     if copies is not None:
         _check_list("copies", copies, torch.bfloat16, sizes, index)

@@ -11,6 +11,7 @@ The reference's policies are tanh MLPs (es.py:156-164); there is no counterpart 
 """
 
 import torch
+from torch.autograd.function import once_differentiable
 
 import rlenv_lib as _rl
 
@@ -23,21 +24,23 @@ def _dense(x):
     return x if x.data_ptr() % 16 == 0 else x.clone()
 
 
-def _check(x, w_gate, w_up, activation, grad_out=None):
+def _check(x, w_gate, w_up, activation, *grad_out):
     """(M, K, F, the type's code, the device's index). What fits passes on a few comparisons; what does not is
     looked at again for the message."""
     _rl.as_floats("x", x)
+    if not isinstance(w_gate, torch.Tensor):
+        _rl.as_floats("w_gate", w_gate)
     index, dtype = x.get_device(), x.dtype
     if x.dim() < 1 or w_gate.dim() != 2 or w_gate.shape[0] != x.shape[-1]:
         raise ValueError(f"x must be (..., K) and w_gate (K, F); got {tuple(x.shape)} and {tuple(w_gate.shape)}")
     k, f = w_gate.shape
     for name, w in (("w_gate", w_gate), ("w_up", w_up)):
-        if w.get_device() != index or w.dtype is not dtype or w.shape != (k, f):
+        if not isinstance(w, torch.Tensor) or w.get_device() != index or w.dtype is not dtype or w.shape != (k, f):
             _rl.as_floats(name, w, (k, f), dtype)
             _rl.one_device(index, **{name: w})
-    if grad_out is not None:
-        _rl.as_floats("grad_out", grad_out, (*x.shape[:-1], f), dtype)
-        _rl.one_device(index, grad_out=grad_out)
+    for g in grad_out:
+        _rl.as_floats("grad_out", g, (*x.shape[:-1], f), dtype)
+        _rl.one_device(index, grad_out=g)
     if activation not in ACTIVATIONS:
         raise ValueError(f"activation must be one of {sorted(ACTIVATIONS)}; got {activation!r}")
     return x.numel() // k if k else x.shape[:-1].numel(), k, f, _rl.FLOAT_DTYPES[dtype], index
@@ -79,6 +82,7 @@ class _Apply(torch.autograd.Function):
         return forward(x, w_gate, w_up, activation)
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, grad_out):
         x, w_gate, w_up = ctx.saved_tensors
         return (*backward(grad_out, x, w_gate, w_up, ctx.activation), None)

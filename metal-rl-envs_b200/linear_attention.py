@@ -23,6 +23,7 @@ import ctypes
 from functools import lru_cache
 
 import torch
+from torch.autograd.function import once_differentiable
 
 import rlenv_lib as _rl
 
@@ -56,7 +57,7 @@ def _check(lead, decay, state, resets, grad_state, names, tokens):
         _rl.as_floats(names[0], first)
     shape, dtype, index = first.shape, first.dtype, first.get_device()
     for name, x in zip(names[1:], tokens[1:]):
-        if x.get_device() != index or x.dtype is not dtype or x.shape != shape:
+        if not isinstance(x, torch.Tensor) or x.get_device() != index or x.dtype is not dtype or x.shape != shape:
             _rl.as_floats(name, x, shape, dtype)
             _rl.one_device(index, **{name: x})
     if len(shape) != lead + 2:
@@ -64,11 +65,13 @@ def _check(lead, decay, state, resets, grad_state, names, tokens):
     n, h, d = shape[-3:]
     if d not in WIDTHS:
         raise ValueError(f"the heads' width must be one of {WIDTHS}; got {d}")
-    if decay.get_device() != index or decay.dtype is not torch.float32 or decay.shape != (h,):
+    if not isinstance(decay, torch.Tensor) or decay.get_device() != index or decay.dtype is not torch.float32 \
+            or decay.shape != (h,):
         _rl.as_floats("decay", decay, (h,), torch.float32)
         _rl.one_device(index, decay=decay)
     for s in (state, grad_state):
-        if s is not None and (s.get_device() != index or s.dtype is not torch.float32 or s.shape != (n, h, d, d)):
+        if s is not None and (not isinstance(s, torch.Tensor) or s.get_device() != index
+                              or s.dtype is not torch.float32 or s.shape != (n, h, d, d)):
             name = "state" if s is state else "grad_state"
             _rl.as_floats(name, s, (n, h, d, d), torch.float32)
             _rl.one_device(index, **{name: s})
@@ -157,6 +160,7 @@ class _Attend(torch.autograd.Function):
         return forward(q, k, v, decay, state, resets, scale)
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, grad_out, grad_state):
         q, k, v, decay, state, resets = ctx.saved_tensors
         dq, dk, dv, dstate = backward(grad_out.contiguous(), q, k, v, decay, state, resets, ctx.scale, grad_state)

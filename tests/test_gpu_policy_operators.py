@@ -555,3 +555,42 @@ def test_adamw_refusals(cuda):
     with pytest.raises(ValueError):
         adamw.step(p, g, bad)
     assert s.step == 0 and p[0].abs().sum() == 0
+
+
+def test_what_is_no_tensor_is_refused(cuda):
+    import adamw
+    import gated_ffn
+    import linear_attention as la
+
+    (q, k, v, g), decay, state, _, _ = inputs(cuda, 4, 1, 2, 16, "f32")
+    for args in ((q, k, None, decay), (q, None, v, decay), (None, k, v, decay), (q, k, v, 0.9), (q, k, v, None),
+                 (q, k, v, decay, 1.0), (q, k, v, decay, None, [True])):
+        with pytest.raises(ValueError):
+            la.forward(*args)
+    with pytest.raises(ValueError):
+        la.backward(None, q, k, v, decay)
+    x, wg, wu, dh = ffn_inputs(cuda, 4, 8, 16, "f32")
+    for args in ((None, wg, wu), (x, None, wu), (x, wg, None), (x, wg.cpu(), wu)):
+        with pytest.raises(ValueError):
+            gated_ffn.forward(*args)
+    with pytest.raises(ValueError):
+        gated_ffn.backward(None, x, wg, wu)
+    params = [torch.zeros(4, device=cuda), torch.zeros(3, device=cuda)]
+    grads, opt = [torch.ones_like(p) for p in params], adamw.init_state(params)
+    for a, b, more in ((params, [grads[0], None], {}), (params, [None, None], {}), ([None, params[1]], grads, {}),
+                       (params, grads, {"grad_scale": 0.5}), (params, grads, {"copies": [None, None]})):
+        with pytest.raises(ValueError):
+            adamw.step(a, b, opt, **more)
+    assert opt.step == 0 and not params[0].any()
+
+
+def test_second_derivatives_are_refused(cuda):
+    import gated_ffn
+    import linear_attention as la
+
+    (q, k, v, _), decay, _, _, _ = inputs(cuda, 4, 1, 2, 16, "f32")
+    x, wg, wu, _ = ffn_inputs(cuda, 4, 8, 16, "f32")
+    for leaf, y in ((q.requires_grad_(), la.attend(q, k, v, decay)[0]), (x.requires_grad_(), gated_ffn.apply(x, wg, wu))):
+        grad, = torch.autograd.grad(y.sum(), leaf, create_graph=True)
+        with pytest.raises(RuntimeError):
+            grad.sum().backward()
