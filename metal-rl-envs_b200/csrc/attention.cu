@@ -17,7 +17,7 @@ using attn::Strides;
 // Measured: bfloat16 heads of 64, 500 steps x 256 x 8, 232 us (2.5 TB/s of the tensors; the tensor pipe 45% busy,
 // shared memory 60%, issue 44%: a warp's fragments come from shared memory, and what a warp waits for next is
 // hidden by two other warps of its scheduler only); gradient of half as many 330 us. float32 heads of 128, 16,384
-// steps x 8, 468 us, of which 100 us are the segments' own carries and 8 us the joining.
+// steps x 8, 420 us, of which 101 us are the segments' own carries and 8 us the joining.
 struct Split {
   int64_t segments, per;
   float* carry;    // (scans, sequences, segments, D, D): a segment's own, then the one at its start
