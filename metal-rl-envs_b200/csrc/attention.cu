@@ -14,9 +14,9 @@ using attn::Strides;
 // segment's own carry from zero, join_kernel the carry at each segment's start, and
 // chunk_kernel<whole> the outputs.
 //
-// Measured: bfloat16 heads of 64, 500 steps x 256 x 8, 232 us (2.5 TB/s of the tensors; the tensor pipe 45% busy,
+// Measured: bfloat16 heads of 64, 500 steps x 256 x 8, 230 us (2.6 TB/s of the tensors; the tensor pipe 45% busy,
 // shared memory 60%, issue 44%: a warp's fragments come from shared memory, and what a warp waits for next is
-// hidden by two other warps of its scheduler only); gradient of half as many 330 us. float32 heads of 128, 16,384
+// hidden by two other warps of its scheduler only); gradient of half as many 328 us. float32 heads of 128, 16,384
 // steps x 8, 420 us, of which 101 us are the segments' own carries and 8 us the joining.
 struct Split {
   int64_t segments, per;
@@ -217,11 +217,18 @@ chunk_kernel(const __grid_constant__ Problem p, const __grid_constant__ Split sp
 #pragma unroll
           for (int q = 0; q < C::kIn; ++q) load_matrices(x[r][q], xa + 2 * (q * C::kX + 16 * r * C::PX + 16 * k));
       };
+      // Tokens of bfloat16 heads of 64 stay in registers for all of their products (the rollouts 230 us against 233;
+      // wider heads have no registers left, narrower ones no use for it).
+      constexpr int kKept = !C::kFloat && D == 64 ? D / 16 : 0;
+      uint32_t kept[kKept ? kKept : 1][C::RT][C::kIn][4];
+#pragma unroll
+      for (int k = 0; k < kKept; ++k) load_x_tiles(kept[k], k);
       // x Z
 #pragma unroll
       for (int k = 0; k < D / 16; ++k) {
-        uint32_t x[C::RT][C::kIn][4];
-        load_x_tiles(x, k);
+        uint32_t fresh[C::RT][C::kIn][4];
+        if (!kKept) load_x_tiles(fresh, k);
+        const auto& x = kKept ? kept[kKept ? k : 0] : fresh;
 #pragma unroll
         for (int t = 0; t < C::OC / 16; t += kGroup) {
           uint32_t v[kGroup][C::kMid][4];
@@ -259,8 +266,9 @@ chunk_kernel(const __grid_constant__ Problem p, const __grid_constant__ Split sp
         float w[C::RT][2][4] = {}, w_odd[C::RT][2][4] = {};  // even and odd steps of the sum side by side
 #pragma unroll
         for (int k = 0; k < D / 16; ++k) {
-          uint32_t x[C::RT][C::kIn][4], v[1][C::kIn][4];
-          load_x_tiles(x, k);
+          uint32_t fresh[C::RT][C::kIn][4], v[1][C::kIn][4];
+          if (!kKept) load_x_tiles(fresh, k);
+          const auto& x = kKept ? kept[kKept ? k : 0] : fresh;
 #pragma unroll
           for (int q = 0; q < C::kIn; ++q) load_matrices(v[0][q], aa + 2 * (q * C::kX + 16 * jb * C::PX + 16 * k));
 #pragma unroll
