@@ -586,6 +586,151 @@ step_kernel(const T* __restrict__ q, const T* __restrict__ k, const T* __restric
   }
 }
 
+// A few tokens of many sequences, with the state in registers as `step` has it, token after token: bound by reading
+// and writing the states (8,000 bfloat16 heads of 64, one token: 55 us, 4.8 TB/s), where a chunk would be mostly
+// padding. A state's element (r, c) grows by left_r right_c; a token's results are across_r = scale sum_c (r, c)
+// along_c and down_c = scale sum_r (r, c) head_r. Forward, down of k, v and q; dq, across of k, v and do; dk and dv
+// from one pass of the adjoint state, across and down of q, do and v, k, last token first. A block is one sequence:
+// thread t holds four columns of D / 8 rows. Sums along a row go through the lanes that hold it, half of the values a
+// step; those down a column meet in shared memory.
+struct Tokens {
+  const void *left, *right, *along, *head;
+  Strides ls, rs, as, hs;
+  const float* decay;
+  const uint8_t* resets;
+  const float* in;
+  float* end;
+  void *across, *down;
+  float scale, in_mul, out_mul;
+  int t, reverse;
+  int64_t n, h;
+};
+constexpr int kMostTokens = 16;
+
+template <int D, bool kAcross, bool kDown>
+constexpr int tokens_smem(int t) {
+  return t * D * 4 * (2 + (kAcross ? 2 : 0) + (kDown ? 1 + D / 16 : 0));
+}
+
+template <typename T, int D, bool kAcross, bool kDown>
+__global__ void __launch_bounds__(2 * D) tokens_kernel(const __grid_constant__ Tokens p) {
+  constexpr int kLanes = D / 4, kRows = D / 8, kThreads = 2 * D, kWarps = D / 16;
+  extern __shared__ __align__(16) unsigned char smem[];
+  __shared__ int cut[kMostTokens];
+  const int size = p.t * D;
+  float* const left = reinterpret_cast<float*>(smem);
+  float *const right = left + size, *const along = right + size, *const across = along + size;
+  float *const head = right + size + (kAcross ? 2 * size : 0), *const parts = head + size;  // parts: (token, warp, D)
+  const int64_t seq = blockIdx.x, n = seq / p.h, h = seq % p.h;
+  const int row = threadIdx.x / kLanes * kRows, c = threadIdx.x % kLanes * 4, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  float4 z[kRows];
+#pragma unroll
+  for (int k = 0; k < kRows; ++k) {
+    z[k] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    if (p.in) {
+      z[k] = __ldg(reinterpret_cast<const float4*>(p.in + (seq * D + row + k) * D + c));
+      z[k].x *= p.in_mul, z[k].y *= p.in_mul, z[k].z *= p.in_mul, z[k].w *= p.in_mul;
+    }
+  }
+  const auto fetch = [&](float* to, const void* from, const Strides& s) {
+    const T* at = static_cast<const T*>(from) + n * s.n + h * s.h;
+    for (int e = threadIdx.x; e < size; e += kThreads) to[e] = attn::to_float(at[e / D * s.t + e % D]);
+  };
+  fetch(left, p.left, p.ls);
+  fetch(right, p.right, p.rs);
+  if (kAcross) fetch(along, p.along, p.as);
+  if (kDown) fetch(head, p.head, p.hs);
+  if (threadIdx.x < p.t) cut[threadIdx.x] = p.resets ? __ldg(p.resets + threadIdx.x * p.n + n) : 0;
+  const float g = __ldg(p.decay + h);
+  __syncthreads();
+  const auto decay = [&](bool reset) {
+#pragma unroll
+    for (int k = 0; k < kRows; ++k) {
+      z[k].x = reset ? 0.0f : g * z[k].x, z[k].y = reset ? 0.0f : g * z[k].y;
+      z[k].z = reset ? 0.0f : g * z[k].z, z[k].w = reset ? 0.0f : g * z[k].w;
+    }
+  };
+  for (int j = 0; j < p.t; ++j) {
+    const int i = p.reverse ? p.t - 1 - j : j;
+    const bool reset = cut[i] != 0;
+    if (!p.reverse) decay(reset);
+    const float4 r = *reinterpret_cast<const float4*>(right + i * D + c);
+    float4 y = make_float4(0.0f, 0.0f, 0.0f, 0.0f), o = y;
+    if (kAcross) y = *reinterpret_cast<const float4*>(along + i * D + c);
+    float s[kRows];
+#pragma unroll
+    for (int k = 0; k < kRows; k += 2) {
+      const float2 l = *reinterpret_cast<const float2*>(left + i * D + row + k);
+      float2 w = make_float2(0.0f, 0.0f);
+      if (kDown) w = *reinterpret_cast<const float2*>(head + i * D + row + k);
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const float lu = u ? l.y : l.x, wu = u ? w.y : w.x;
+        float4& v = z[k + u];
+        v.x = fmaf(lu, r.x, v.x), v.y = fmaf(lu, r.y, v.y), v.z = fmaf(lu, r.z, v.z), v.w = fmaf(lu, r.w, v.w);
+        if (kDown) o.x = fmaf(wu, v.x, o.x), o.y = fmaf(wu, v.y, o.y), o.z = fmaf(wu, v.z, o.z), o.w = fmaf(wu, v.w, o.w);
+        if (kAcross) s[k + u] = fmaf(y.x, v.x, fmaf(y.y, v.y, fmaf(y.z, v.z, y.w * v.w)));
+      }
+    }
+    if constexpr (kAcross) {
+#pragma unroll
+      for (int m = kRows / 2; m >= 1; m /= 2) {  // lanes 2 m apart share their values out
+        const bool upper = lane & 2 * m;
+#pragma unroll
+        for (int k = 0; k < m; ++k) {
+          const float give = upper ? s[k] : s[k + m], keep = upper ? s[k + m] : s[k];
+          s[k] = keep + __shfl_xor_sync(0xffffffffu, give, 2 * m);
+        }
+      }
+      s[0] += __shfl_xor_sync(0xffffffffu, s[0], 1);
+      if (lane % 2 == 0) across[i * D + row + lane % kLanes / 2] = s[0];
+    }
+    if constexpr (kDown) {
+#pragma unroll
+      for (int m = kLanes; m < 32; m *= 2) {
+        o.x += __shfl_xor_sync(0xffffffffu, o.x, m), o.y += __shfl_xor_sync(0xffffffffu, o.y, m);
+        o.z += __shfl_xor_sync(0xffffffffu, o.z, m), o.w += __shfl_xor_sync(0xffffffffu, o.w, m);
+      }
+      if (lane < kLanes) *reinterpret_cast<float4*>(parts + (i * kWarps + warp) * D + c) = o;
+    }
+    if (p.reverse) decay(reset);
+  }
+  if (p.end) {
+#pragma unroll
+    for (int k = 0; k < kRows; ++k)
+      *reinterpret_cast<float4*>(p.end + (seq * D + row + k) * D + c) =
+          make_float4(p.out_mul * z[k].x, p.out_mul * z[k].y, p.out_mul * z[k].z, p.out_mul * z[k].w);
+  }
+  __syncthreads();
+  for (int e = threadIdx.x; e < size; e += kThreads) {
+    const int64_t at = (e / D * p.n * p.h + seq) * D + e % D;
+    if (kAcross) static_cast<T*>(p.across)[at] = attn::from_float<T>(p.scale * across[e]);
+    if (kDown) {
+      float sum = 0.0f;
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) sum += parts[(e / D * kWarps + w) * D + e % D];
+      static_cast<T*>(p.down)[at] = attn::from_float<T>(p.scale * sum);
+    }
+  }
+}
+
+template <bool kAcross, bool kDown>
+struct TokensRunner {
+  const Tokens& p;
+  cudaStream_t stream;
+  template <typename T, int D>
+  int operator()() const {
+    constexpr int kMost = tokens_smem<D, kAcross, kDown>(kMostTokens);
+    if (kMost > 40 * 1024)
+      if (cudaError_t e = cudaFuncSetAttribute(tokens_kernel<T, D, kAcross, kDown>,
+                                               cudaFuncAttributeMaxDynamicSharedMemorySize, kMost))
+        return int(e);
+    tokens_kernel<T, D, kAcross, kDown>
+        <<<unsigned(p.n * p.h), 2 * D, tokens_smem<D, kAcross, kDown>(p.t), stream>>>(p);
+    return launch_status();
+  }
+};
+
 bool width_built(int d) { return d == 16 || d == 32 || d == 64 || d == 128; }
 
 // Calls fn<T, D>() for the type and width.
@@ -618,6 +763,16 @@ bool aligned_rows(const void* p, const int64_t* st, int dtype, int axes) {
   for (int i = 0; i < axes; ++i)
     if (uint64_t(st[i]) * size % 16) return false;
   return true;
+}
+
+// Whether tokens are taken one after the other: few of them, in as many sequences as give each SM 256 threads.
+// Measured in us, this way and by chunks, forward and gradient: bfloat16, 8,000 heads of 64, 1 token 55 and 170, 103
+// and 421, 8 tokens 99 and 173, 211 and 427; 2,400 of 128, 8 tokens 175 and 205, 370 and 499; 1,200 of 128, 12
+// tokens 137 and 108, 302 and 254; 16,000 of 32, 16 tokens 108 and 99; float32 2,400 heads of 128, 1 token 99
+// and 465, 183 and 1,251, 16 tokens 256 and 474, 575 and 1,272; 24,000 of 16, 16 tokens 63 and 153; few sequences,
+// 15 of 64, 8 tokens, 5 and 8, 13 and 8; 296 of 16, 8 tokens, 4.4 and 3.8, 9.9 and 7.6.
+bool few_tokens(int dtype, int d, int64_t t, int64_t n, int64_t h) {
+  return t > 0 && t <= (dtype == RLENV_F32 ? kMostTokens : kMostTokens / 2) && n * h * d >= 128 * 148;
 }
 
 struct Runner {
@@ -662,6 +817,11 @@ int rlenv_linear_attention_forward(int dtype, int d, int64_t t, int64_t n, int64
   if (!aligned_rows(q, st, dtype, 3) || !aligned_rows(k, st + 3, dtype, 3) || !aligned_rows(v, st + 6, dtype, 3))
     return RLENV_EINVAL;
   if (!scratch_holds(scratch, scratch_bytes, dispatch<int64_t>(dtype, d, ScratchSize{t, n, h, 1}))) return RLENV_EINVAL;
+  if (few_tokens(dtype, d, t, n, h) && !off_boundary(state_in) && !off_boundary(state_out)) {
+    const Tokens f{k, v, nullptr, q, {st[3], st[4], st[5]}, {st[6], st[7], st[8]}, {}, {st[0], st[1], st[2]}, decay,
+                   resets, state_in, state_out, nullptr, out, scale, 1.0f, 1.0f, int(t), 0, n, h};
+    return dispatch<int>(dtype, d, TokensRunner<false, true>{f, as_stream(stream)});
+  }
   Problem p{};
   p.t = t, p.n = n, p.h = h, p.decay = decay, p.resets = resets, p.scale = scale, p.scans = 1;
   p.scan[0] = Scan{q, k, v, {st[0], st[1], st[2]}, {st[3], st[4], st[5]}, {st[6], st[7], st[8]},
@@ -688,10 +848,18 @@ int rlenv_linear_attention_backward(int dtype, int d, int64_t t, int64_t n, int6
     return RLENV_EINVAL;
   if (!scratch_holds(scratch, scratch_bytes, dispatch<int64_t>(dtype, d, ScratchSize{t, n, h, 3}))) return RLENV_EINVAL;
   const Strides ds{st[0], st[1], st[2]}, qs{st[3], st[4], st[5]}, ks{st[6], st[7], st[8]}, vs{st[9], st[10], st[11]};
-  Problem p{};
-  p.t = t, p.n = n, p.h = h, p.decay = decay, p.resets = resets, p.scale = scale, p.scans = 3;
   // The reverse scans carry R / scale, so that the common factor stays outside.
   const float inv = 1.0f / scale;
+  if (few_tokens(dtype, d, t, n, h) && !off_boundary(state_in) && !off_boundary(grad_state_out) && !off_boundary(grad_state_in)) {
+    const Tokens f{k, v, grad_out, nullptr, ks, vs, ds, {}, decay, resets, state_in, nullptr, grad_q, nullptr, scale,
+                   1.0f, 1.0f, int(t), 0, n, h};
+    if (const int rc = dispatch<int>(dtype, d, TokensRunner<true, false>{f, as_stream(stream)})) return rc;
+    const Tokens r{q, grad_out, v, k, qs, ds, vs, ks, decay, resets, grad_state_out, grad_state_in, grad_k, grad_v,
+                   scale, inv, scale, int(t), 1, n, h};
+    return dispatch<int>(dtype, d, TokensRunner<true, true>{r, as_stream(stream)});
+  }
+  Problem p{};
+  p.t = t, p.n = n, p.h = h, p.decay = decay, p.resets = resets, p.scale = scale, p.scans = 3;
   p.scan[0] = Scan{grad_out, v, k, ds, vs, ks, grad_q, state_in, nullptr, 1.0f, 1.0f, 1, 0};
   p.scan[1] = Scan{v, grad_out, q, vs, ds, qs, grad_k, grad_state_out, nullptr, inv, scale, 1, 1};
   p.scan[2] = Scan{k, q, grad_out, ks, qs, ds, grad_v, grad_state_out, grad_state_in, inv, scale, 0, 1};

@@ -332,6 +332,51 @@ def test_ffn_backward(cuda, m, k, f, act, dtype):
 
 
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("t,n,h,d", [(1, 200, 6, 16), (3, 200, 6, 16), (8, 100, 6, 32), (16, 75, 4, 64), (7, 50, 3, 128),
+                                     (9, 50, 3, 128), (17, 200, 6, 16), (16, 200, 6, 16), (5, 20, 5, 64)])
+def test_attention_of_few_tokens(cuda, t, n, h, d, dtype):
+    test_attention_forward(cuda, t, n, h, d, dtype)
+    test_attention_backward(cuda, t, n, h, d, dtype)
+
+
+def test_attention_of_few_tokens_with_infinities(cuda):
+    """What a reset cuts off is dropped, an infinity too, and other sequences see nothing of it."""
+    import linear_attention as la
+
+    (q, k, v, g), decay, state, gstate, resets = inputs(cuda, 6, 300, 2, 32, "f32", p_reset=0.0)
+    resets[3, 1] = True
+    bad = [x.clone() for x in (q, k, v, g)]
+    for x in bad[1:3]:
+        x[2, 1, 0] = float("inf")
+    out, end = la.forward(bad[0], bad[1], bad[2], decay, state, resets)
+    want, wend = la.forward(q, k, v, decay, state, resets)
+    assert not torch.isfinite(out[2, 1, 0]).any()
+    assert torch.equal(out[3:], want[3:]) and torch.equal(end, wend)
+    assert torch.equal(out[:, [0, 2]], want[:, [0, 2]]) and torch.equal(out[:2], want[:2])
+    bad = g.clone()
+    bad[4, 1, 0] = float("inf")  # of the second episode: the first one's gradients do not see it
+    got, want = la.backward(bad, q, k, v, decay, state, resets, None, gstate), la.backward(g, q, k, v, decay, state,
+                                                                                       resets, None, gstate)
+    for a, b in zip(got[:3], want[:3]):
+        assert torch.equal(a[:3], b[:3]) and torch.equal(a[:, [0, 2]], b[:, [0, 2]])
+    assert torch.equal(got[3], want[3]) and not torch.isfinite(got[0][4, 1, 0]).all()
+
+
+def test_attention_states_off_the_vector_boundary(cuda):
+    import linear_attention as la
+
+    (q, k, v, g), decay, state, gstate, resets = inputs(cuda, 4, 600, 2, 16, "f32")
+    flat = torch.empty(2 * state.numel() + 1, device=cuda)
+    off, goff = (flat[1 + i * state.numel():][:state.numel()].view(state.shape) for i in (0, 1))
+    off.copy_(state), goff.copy_(gstate)
+    for a, b in zip(la.forward(q, k, v, decay, off, resets), la.forward(q, k, v, decay, state, resets)):
+        assert torch.allclose(a, b, rtol=1e-5, atol=1e-5)
+    for a, b in zip(la.backward(g, q, k, v, decay, off, resets, None, goff),
+                    la.backward(g, q, k, v, decay, state, resets, None, gstate)):
+        assert torch.allclose(a, b, rtol=1e-5, atol=1e-5)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
 @pytest.mark.parametrize("m,k,f", [(1, 97, 250), (2, 300, 77), (3, 64, 256), (5, 1, 5), (9, 129, 131), (32, 65, 1030),
                                    (33, 70, 68), (77, 31, 36), (128, 97, 250), (129, 97, 250)])
 def test_ffn_backward_of_few_rows(cuda, m, k, f, dtype):
