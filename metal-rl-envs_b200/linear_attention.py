@@ -84,6 +84,15 @@ def _check(lead, decay, state, resets, grad_state, names, tokens):
     return shape, dtype, index, resets
 
 
+def _like(x):
+    """A dense tensor of x's shape and type (empty_like is the quicker call, but keeps x's strides)."""
+    return torch.empty_like(x) if x.is_contiguous() else x.new_empty(x.shape)
+
+
+def _state_like(state, q, n, h, d):
+    return _like(state) if state is not None else q.new_empty((n, h, d, d), dtype=torch.float32)
+
+
 def _scale(scale, d):
     return d ** -0.5 if scale is None else float(scale)
 
@@ -96,8 +105,7 @@ def forward(q, k, v, decay, state=None, resets=None, scale=None):
     (q, qs), (k, ks), (v, vs) = _rows(q), _rows(k), _rows(v)
     decay, state = decay.contiguous(), None if state is None else state.contiguous()
     lib, code = _rl.lib(), _rl.FLOAT_DTYPES[dtype]
-    out = q.new_empty(shape)
-    new = q.new_empty((n, h, d, d), dtype=torch.float32)
+    out, new = _like(q), _state_like(state, q, n, h, d)
     nbytes = lib.linear_attention_scratch_bytes(code, d, t, n, h, 0)
     tmp = _rl.scratch(nbytes, q)
     _rl.launch(index, lib.linear_attention_forward, code, d, t, n, h, q.data_ptr(), k.data_ptr(), v.data_ptr(),
@@ -116,8 +124,7 @@ def backward(grad_out, q, k, v, decay, state=None, resets=None, scale=None, grad
     decay = decay.contiguous()
     state, grad_state = (None if s is None else s.contiguous() for s in (state, grad_state))
     lib, code = _rl.lib(), _rl.FLOAT_DTYPES[dtype]
-    dq, dk, dv = q.new_empty(shape), q.new_empty(shape), q.new_empty(shape)
-    dstate = q.new_empty((n, h, d, d), dtype=torch.float32)
+    dq, dk, dv, dstate = _like(q), _like(q), _like(q), _state_like(state, q, n, h, d)
     nbytes = lib.linear_attention_scratch_bytes(code, d, t, n, h, 1)
     tmp = _rl.scratch(nbytes, q)
     _rl.launch(index, lib.linear_attention_backward, code, d, t, n, h, g.data_ptr(), q.data_ptr(), k.data_ptr(),
@@ -135,7 +142,7 @@ def step(q, k, v, decay, state, resets=None, scale=None):
         raise ValueError("state must be contiguous and on a 16-byte boundary: it is updated in place")
     n, h, d = shape
     (q, qs), (k, ks), (v, vs) = _rows(q), _rows(k), _rows(v)
-    out = q.new_empty(shape)
+    out = _like(q)
     _rl.launch(index, _rl.lib().linear_attention_step, _rl.FLOAT_DTYPES[dtype], d, n, h, q.data_ptr(), k.data_ptr(),
                v.data_ptr(), _stride_array(qs, ks, vs), decay.contiguous().data_ptr(), _rl.ptr(resets),
                _scale(scale, d), state.data_ptr(), out.data_ptr())
