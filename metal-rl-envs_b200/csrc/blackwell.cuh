@@ -80,9 +80,6 @@ RLENV_D bool elect() {  // one lane of the warp
 }
 
 // ---- tensor copies ------------------------------------------------------------------------------
-RLENV_D void prefetch_map(const CUtensorMap* map) {
-  asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory");
-}
 // Into this block's shared memory; the bytes are counted at a barrier of either block of the pair.
 RLENV_D void copy_tile(uint32_t to, const CUtensorMap* map, uint32_t cluster_bar, int x, int y, int z) {
   asm volatile(

@@ -969,7 +969,7 @@ int few_rows(const void* x, const void* wg, const void* wu, int64_t m, int64_t k
     else few_rows_kernel<T, kFew, false, false><<<grid, kFewThreads, 0, s>>>(X, G, U, m, k, f, act, to, D, own);
     return launch_status();
   }
-  FewGradients p{x, wg, wu, own, dx, dwg, dwu, m, k, f};
+  FewGradients p{x, wg, wu, own, dx, dwg, dwu, m, k, f, 0, 0, 0};
   const int64_t across = (f + kFewTile - 1) / kFewTile, weight_blocks = across * ((k + kFewTile - 1) / kFewTile);
   const int64_t dx_across = (k + kFewDx - 1) / kFewDx, blocks = weight_blocks + dx_across * ((m + kFew - 1) / kFew);
   if (blocks > 0x7fffffff) return RLENV_EINVAL;
