@@ -553,6 +553,10 @@ product_kernel(const __grid_constant__ Product p, int items) {
         }
       }
     }
+    // Both blocks' buffers are released by the first block's commits: each block waits for the last release of every
+    // buffer, so that no arrival is on its way to a block that has ended. (A release's parity is its round's.)
+    for (int i = 0; i < C::kStages && ok; ++i)
+      if (used >> i & 1) ok = bw::barrier_wait_warp(empty + 8 * i, i < stage ? phase : phase ^ 1, dead);
     if (!ok && rank == 0) {  // the copies in flight land before the blocks may end
       int unused = 0;
       for (int i = 0; i < C::kStages; ++i)

@@ -639,3 +639,12 @@ def test_second_derivatives_are_refused(cuda):
         grad, = torch.autograd.grad(y.sum(), leaf, create_graph=True)
         with pytest.raises(RuntimeError):
             grad.sum().backward()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("blocks", [1, 2, 3, 5, 6, 7, 11, 12, 13])
+def test_ffn_rings_filled_any_number_of_times(cuda, blocks, dtype):
+    """A pair of SMs whose only tile fills its ring of five or six buffers less than once, exactly, once more, twice;
+    the blocks of the pair end behind the last release of every buffer."""
+    test_ffn_forward(cuda, 1200, 64 * blocks - 3, 520, "silu", dtype)
+    test_ffn_backward(cuda, 257, 64 * blocks - 3, 264, "silu", dtype)
