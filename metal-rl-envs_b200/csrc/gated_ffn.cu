@@ -664,6 +664,7 @@ product_kernel(const __grid_constant__ Product p, int items) {
           for (int i = 0; i < 32; ++i) v[i] = 0x7fffffffu;
         }
         finish<T, kOp>(p, w, r0, w.c0 + column(j), v, d, own_stage);
+        __syncwarp();  // lanes part over rows and columns that are not there; what follows is the whole warp's
       };
       if constexpr (C::kFloat) {
         float sum[kRuns][32];
