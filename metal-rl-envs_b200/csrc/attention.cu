@@ -199,6 +199,7 @@ chunk_kernel(const __grid_constant__ Problem p, const __grid_constant__ Split sp
       if (kAhead) set_out(next_chunk, tiles + buffer * C::kTiles);
       if (p.resets) read_resets(next_chunk);
     }
+    __syncwarp();  // lanes part where a tile's rows end; the matrix instructions are the whole warp's
 
     if (!kLocal && rb < live) {
       float o[C::RT][C::OC / 8][4];
@@ -360,6 +361,7 @@ chunk_kernel(const __grid_constant__ Problem p, const __grid_constant__ Split sp
       }
     }
 
+    __syncwarp();  // behind the stores of a chunk's last rows
     out_at += kChunk * out_step;
     if (!kLocal && C::kTurning) {
       rb = rb + C::RT < C::kRowWarps * C::RT ? rb + C::RT : 0;

@@ -648,3 +648,20 @@ def test_ffn_rings_filled_any_number_of_times(cuda, blocks, dtype):
     the blocks of the pair end behind the last release of every buffer."""
     test_ffn_forward(cuda, 1200, 64 * blocks - 3, 520, "silu", dtype)
     test_ffn_backward(cuda, 257, 64 * blocks - 3, 264, "silu", dtype)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("d", [16, 32, 64, 128])
+def test_attention_of_chunks_that_end_anywhere(cuda, d, dtype):
+    """Rows and columns of a warp's tiles that are partly there, in the last of two chunks."""
+    for t in (66, 71, 73, 80, 97, 111, 127):
+        test_attention_forward(cuda, t, 1, 3, d, dtype)
+    test_attention_backward(cuda, 75, 1, 3, d, dtype)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("m,k,f", [(450, 70, 530), (513, 64, 519), (700, 90, 390)])
+def test_ffn_tiles_that_end_anywhere(cuda, m, k, f, dtype):
+    """Tiles of which a warp's lanes have some rows and columns and not others."""
+    test_ffn_forward(cuda, m, k, f, "gelu", dtype)
+    test_ffn_backward(cuda, m, k, f, "gelu", dtype)
