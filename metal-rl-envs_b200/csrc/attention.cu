@@ -546,7 +546,7 @@ step_kernel(const T* __restrict__ q, const T* __restrict__ k, const T* __restric
   constexpr int kThreads = D * D / 4 < kStepThreads ? D * D / 4 : kStepThreads;
   constexpr int kRows = kThreads / kQuads;          // rows in flight
   constexpr int kPer = D / kRows;                   // rows a thread holds
-  __shared__ float part[kRows][D];
+  __shared__ __align__(16) float part[kRows][D];  // read and written by fours
   const int64_t seq = blockIdx.x, n = seq / heads, h = seq % heads;
   const int c = (threadIdx.x % kQuads) * 4, r0 = threadIdx.x / kQuads;
   float4* S = reinterpret_cast<float4*>(state + seq * D * D);
