@@ -30,6 +30,13 @@ RLENV_D void barrier_arrive(uint32_t cluster_bar) {
 RLENV_D void barrier_expect(uint32_t bar, uint32_t bytes) {
   asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
 }
+// Bytes that will not come count as come.
+RLENV_D void barrier_strike(uint32_t bar, uint32_t bytes) {
+  asm volatile("mbarrier.complete_tx.relaxed.cluster.shared::cluster.b64 [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
+}
+RLENV_D void store_in_block(uint32_t cluster_at, int x) {
+  asm volatile("st.shared::cluster.b32 [%0], %1;" ::"r"(cluster_at), "r"(x) : "memory");
+}
 RLENV_D bool barrier_try(uint32_t bar, uint32_t parity) {
   uint32_t done;
   asm volatile(
@@ -45,22 +52,10 @@ RLENV_D uint64_t nanoseconds() {
   asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
   return t;
 }
-RLENV_D bool barrier_wait(uint32_t bar, uint32_t parity, volatile int* dead) {
-  for (int i = 0; i < 32; ++i)
-    if (barrier_try(bar, parity)) return true;
-  const uint64_t start = nanoseconds();
-  do {
-    if (barrier_try(bar, parity)) return true;
-    if (*dead) return false;
-  } while (nanoseconds() - start < kPatience);
-  *dead = 1;
-  return false;
-}
-
-// The same by a whole warp, all of whose lanes get the same answer, and know it: copies and products take
-// their operands from the warp's uniform registers, and under control flow that may diverge each operand is
-// moved there anew, some 60 cycles a product. So the warps that issue them run as one, and only the
-// instruction itself stands under `elect`.
+// A whole warp waits, all of whose lanes get the same answer, and know it: copies and products take their
+// operands from the warp's uniform registers, and under control flow that may diverge each operand is moved there
+// anew, some 60 cycles a product. So the warps that issue them run as one, and only the instruction itself stands
+// under `elect`.
 RLENV_D bool barrier_wait_warp(uint32_t bar, uint32_t parity, volatile int* dead) {
   for (int i = 0; i < 32; ++i)
     if (__all_sync(0xffffffffu, barrier_try(bar, parity))) return true;

@@ -479,6 +479,54 @@ RLENV_D void finish(const Product& p, const Work& w, int64_t r0, int64_t c, cons
   }
 }
 
+// What a block has done by its end, for the other one of the pair.
+struct Ending {
+  int filled;          // ring buffers that its copying warp has filled
+  int released, runs;  // the first block's: releases of ring buffers and sums that its issuing warp has committed
+  int gave_up;         // whether a wait ran out
+};
+RLENV_D void tell(const Ending* e, uint32_t rank) {  // the same place in the other block's shared memory
+  bw::store_in_block(bw::in_block(bw::shared_at(&e->filled), rank), e->filled);
+  bw::store_in_block(bw::in_block(bw::shared_at(&e->released), rank), e->released);
+  bw::store_in_block(bw::in_block(bw::shared_at(&e->runs), rank), e->runs);
+  bw::store_in_block(bw::in_block(bw::shared_at(&e->gave_up), rank), e->gave_up);
+}
+
+// After a wait that ran out: what is under way lands before the pair may end and tensor memory is freed, each with
+// a wait of its own, up to one that runs out too. Products behind the last commit get one. A buffer's bytes all count at the first block: where
+// one block has filled it and the other has not, the other's are struck off, or its own alone expected (the blocks
+// are less than a round of the ring apart). Then every barrier's last phase, by the number of its rounds.
+template <int kStages>
+__device__ __noinline__ void drain(const Ending* endings, int rank, int warp, uint32_t full, uint32_t bytes, uint32_t empty,
+                                   uint32_t summed, uint32_t drained) {
+  int late = 0;  // a flag of its own: not cut short by the wait that ran out before
+  const auto last_of = [&](uint32_t bar, int turns, int slot, int slots) {
+    const int rounds = (turns - slot + slots - 1) / slots;
+    if (turns > slot) bw::barrier_wait_warp(bar + 8 * slot, (rounds - 1) & 1, &late);
+  };
+  if (warp == 1) {
+    if (rank == 0 && bw::elect()) bw::commit(drained);
+    __syncwarp();
+    bw::barrier_wait_warp(drained, 0, &late);
+  } else if (warp == 0) {
+    if (rank == 0) {
+      const int own = endings[0].filled, other = endings[1].filled;
+      if (bw::elect()) {
+        for (int i = own; i < other; ++i) bw::barrier_expect(full + 8 * (i % kStages), bytes);
+        for (int i = other; i < own; ++i) bw::barrier_strike(full + 8 * (i % kStages), bytes);
+      }
+      __syncwarp();
+      for (int i = 0; i < kStages; ++i) last_of(full, own > other ? own : other, i, kStages);
+    }
+    for (int i = 0; i < kStages; ++i) last_of(empty, endings[0].released, i, kStages);
+    for (int i = 0; i < 2; ++i) last_of(summed, endings[0].runs, i, 2);
+  }
+  __syncwarp();
+  bw::fence_before();
+  bw::cluster_sync();
+  bw::fence_after();
+}
+
 template <typename T, int kOp>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Tile<T, kOp>::kThreads, 1)
 product_kernel(const __grid_constant__ Product p, int items) {
@@ -486,19 +534,21 @@ product_kernel(const __grid_constant__ Product p, int items) {
   constexpr bool kPaired = kOp != kGradients;  // half of a tile's columns are gates, half ups
   constexpr uint32_t kBox = 64 * kBlock * 2;
   extern __shared__ unsigned char raw[];
-  __shared__ __align__(8) uint64_t bars[2 * C::kStages + 4];
+  __shared__ __align__(8) uint64_t bars[2 * C::kStages + 5];
   __shared__ uint32_t tmem_slot;
   __shared__ int dead_flag;
+  __shared__ Ending endings[2];  // of the pair's first block, and of its second
   volatile int* const dead = &dead_flag;
   const uint32_t ring = (bw::shared_at(raw) + 1023) & ~1023u;
   const uint32_t full = bw::shared_at(bars), empty = full + 8 * C::kStages;
-  const uint32_t summed = empty + 8 * C::kStages, taken = summed + 16;
+  const uint32_t summed = empty + 8 * C::kStages, taken = summed + 16, drained = taken + 16;
   const int warp = __shfl_sync(0xffffffffu, int(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
   const int rank = int(bw::cluster_rank());
   if (threadIdx.x == 0) {
     for (int i = 0; i < C::kStages; ++i) bw::barrier_init(full + 8 * i, 1), bw::barrier_init(empty + 8 * i, 1);
     for (int i = 0; i < 2; ++i) bw::barrier_init(summed + 8 * i, 1), bw::barrier_init(taken + 8 * i, 2 * C::kEpilogue);
-    dead_flag = 0;
+    bw::barrier_init(drained, 1);
+    dead_flag = 0, endings[rank] = Ending{};
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (warp == 2) bw::tmem_alloc<kTmemColumns>(bw::shared_at(&tmem_slot));
@@ -511,8 +561,8 @@ product_kernel(const __grid_constant__ Product p, int items) {
 
   if (warp == 0) {
     // Both blocks copy their rows of A and their columns of B; all bytes count at the first block's barrier.
-    int stage = 0;
-    uint32_t phase = 0, used = 0;  // used: stages that have been filled at least once
+    int stage = 0, filled = 0;
+    uint32_t phase = 0;
     bool ok = true;
     const uint32_t full_at = bw::in_block(full, 0);
     for (int item = turns.next(); item >= 0 && ok; item = turns.next()) {
@@ -547,7 +597,7 @@ product_kernel(const __grid_constant__ Product p, int items) {
                 bw::copy_tile(b, map_b, bar, k, c0, slice_b);
               }
             }
-            used |= 1u << stage;
+            ++filled;
             if (++stage == C::kStages) stage = 0, phase ^= 1;
           }
         }
@@ -556,15 +606,11 @@ product_kernel(const __grid_constant__ Product p, int items) {
     // Both blocks' buffers are released by the first block's commits: each block waits for the last release of every
     // buffer, so that no arrival is on its way to a block that has ended. (A release's parity is its round's.)
     for (int i = 0; i < C::kStages && ok; ++i)
-      if (used >> i & 1) ok = bw::barrier_wait_warp(empty + 8 * i, i < stage ? phase : phase ^ 1, dead);
-    if (!ok && rank == 0) {  // the copies in flight land before the blocks may end
-      int unused = 0;
-      for (int i = 0; i < C::kStages; ++i)
-        if (used >> i & 1) bw::barrier_wait(full + 8 * i, i < stage ? phase : phase ^ 1, &unused), unused = 0;
-    }
+      if (i < filled) ok = bw::barrier_wait_warp(empty + 8 * i, i < stage ? phase : phase ^ 1, dead);
+    if (lane == 0) endings[rank].filled = filled;
   } else if (warp == 1) {
     if (rank == 0) {
-      int stage = 0, buffer = 0;
+      int stage = 0, buffer = 0, released = 0, runs = 0;
       uint32_t phase = 0, buffer_phase = 0;
       bool ok = true;
       for (int item = turns.next(); item >= 0 && ok; item = turns.next()) {
@@ -610,8 +656,10 @@ product_kernel(const __grid_constant__ Product p, int items) {
               }
               if (last && turn == C::kPlanes - 1) bw::commit(summed + 8 * buffer);
             }
+            released += C::kFloat ? turn : 1;  // none, one and two of a step's three
           }
           if (!ok) break;
+          runs += last;
           more = !last;
           if (last) {
             if (++buffer == 2) buffer = 0, buffer_phase ^= 1;
@@ -620,6 +668,7 @@ product_kernel(const __grid_constant__ Product p, int items) {
           if ((stage += C::kPlanes) == C::kStages) stage = 0, phase ^= 1;
         }
       }
+      if (lane == 0) endings[0].released = released, endings[0].runs = runs;
     }
   } else if (warp >= 4) {
     const int quarter = warp & 3, part = (warp - 4) >> 2;
@@ -673,8 +722,7 @@ product_kernel(const __grid_constant__ Product p, int items) {
 #pragma unroll
           for (int i = 0; i < 32; ++i) sum[j][i] = 0.0f;
         for (int left = w.segs * w.steps; left > 0; left -= C::kRun) {
-          ok = bw::barrier_wait_warp(summed + 8 * buffer, buffer_phase, dead) && ok;
-          if (!ok) break;
+          if (!(ok = ok && bw::barrier_wait_warp(summed + 8 * buffer, buffer_phase, dead))) break;
           bw::fence_after();
 #pragma unroll
           for (int j = 0; j < kRuns; ++j)
@@ -696,7 +744,7 @@ product_kernel(const __grid_constant__ Product p, int items) {
         if (another) load_dh(next, 0);
         finish_run(v, 0, d);
       } else {
-        ok = bw::barrier_wait_warp(summed + 8 * buffer, buffer_phase, dead) && ok;
+        ok = ok && bw::barrier_wait_warp(summed + 8 * buffer, buffer_phase, dead);
         bw::fence_after();
         // Where the registers allow, the next run is read while this one goes out.
         constexpr int kAhead = kOp == kGradients;
@@ -706,7 +754,7 @@ product_kernel(const __grid_constant__ Product p, int items) {
         for (int j = 0; j < kRuns; ++j) {
           bw::tmem_ready(v[j & kAhead]);
           if (kAhead && j + 1 < kRuns) load_run(v[(j + 1) & kAhead], j + 1);
-          if (j + 1 == kRuns) take_next();  // all of the accumulator is read
+          if (ok && j + 1 == kRuns) take_next();  // all of the accumulator is read
           if (j + 1 < kRuns) load_dh(w, j + 1);
           else if (another) load_dh(next, 0);
           finish_run(v[j & kAhead], j, dh[j & 1]);
@@ -718,8 +766,14 @@ product_kernel(const __grid_constant__ Product p, int items) {
   __syncwarp();
   bw::fence_before();
   __syncthreads();
+  if (threadIdx.x == 0) {
+    endings[rank].gave_up = dead_flag;
+    tell(&endings[rank], rank ^ 1);
+  }
   bw::cluster_sync();
   bw::fence_after();
+  if (endings[0].gave_up || endings[1].gave_up)
+    drain<C::kStages>(endings, rank, warp, full, C::kRingBytes, empty, summed, drained);
   if (warp == 2) bw::tmem_free<kTmemColumns>(tmem);
 }
 
