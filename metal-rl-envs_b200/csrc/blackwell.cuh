@@ -45,8 +45,20 @@ RLENV_D bool barrier_try(uint32_t bar, uint32_t parity) {
   return done != 0;
 }
 // Waits for the phase of `parity` to end. Every wait is bounded: after kPatience nanoseconds `dead` is set,
-// and from then on every wait of the block gives up at once.
-constexpr uint64_t kPatience = 2000000000;
+// and from then on every wait of the block gives up at once. What counts is time between looks at the barrier, of
+// each pause kLongestPause at most: while the GPU runs another process's kernels, the clock goes on and the block
+// does not, nor what it waits for.
+constexpr uint64_t kPatience = 2000000000, kLongestPause = 10000000;
+struct Patience {
+  uint64_t limit, last, waited;
+  RLENV_HD Patience(uint64_t limit, uint64_t now) : limit(limit), last(now), waited(0) {}
+  RLENV_HD bool over(uint64_t now) {
+    const uint64_t pause = now - last;
+    waited += pause < kLongestPause ? pause : kLongestPause;
+    last = now;
+    return waited > limit;
+  }
+};
 RLENV_D uint64_t nanoseconds() {
   uint64_t t;
   asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
@@ -56,14 +68,14 @@ RLENV_D uint64_t nanoseconds() {
 // operands from the warp's uniform registers, and under control flow that may diverge each operand is moved there
 // anew, some 60 cycles a product. So the warps that issue them run as one, and only the instruction itself stands
 // under `elect`.
-RLENV_D bool barrier_wait_warp(uint32_t bar, uint32_t parity, volatile int* dead) {
+RLENV_D bool barrier_wait_warp(uint32_t bar, uint32_t parity, volatile int* dead, uint64_t limit = kPatience) {
   for (int i = 0; i < 32; ++i)
     if (__all_sync(0xffffffffu, barrier_try(bar, parity))) return true;
-  const uint64_t start = nanoseconds();
+  Patience patience(limit, nanoseconds());
   while (true) {
     if (__all_sync(0xffffffffu, barrier_try(bar, parity))) return true;
     if (__any_sync(0xffffffffu, *dead != 0)) return false;
-    if (__any_sync(0xffffffffu, nanoseconds() - start > kPatience)) break;
+    if (__any_sync(0xffffffffu, patience.over(nanoseconds()))) break;
   }
   *dead = 1;
   return false;
