@@ -405,6 +405,12 @@ RLENV_API int rlenv_gated_ffn_backward(int dtype, int activation, int64_t m, int
                                        void* grad_x, void* grad_w_gate, void* grad_w_up, void* scratch,
                                        int64_t scratch_bytes, void* stream);
 
+/* The block's kernels wait on barriers of their own, each wait for two seconds at most. One that runs out (it
+ * never has) leaves NaN in the results that it was for, and is counted: *gave_up is the number of thread
+ * blocks on the current device that ended so since the library was loaded or the count last cleared. Waits for
+ * the device. */
+RLENV_API int rlenv_gated_ffn_status(unsigned int* gave_up, int clear);
+
 /* One AdamW step over many tensors, in place:
  *     m <- beta1 m + (1 - beta1) g,  v <- beta2 v + (1 - beta2) g^2,
  *     p <- p (1 - lr weight_decay) - lr (m / (1 - beta1^step)) / (sqrt(v / (1 - beta2^step)) + eps).

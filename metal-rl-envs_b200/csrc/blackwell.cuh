@@ -80,6 +80,17 @@ RLENV_D bool barrier_wait_warp(uint32_t bar, uint32_t parity, volatile int* dead
   *dead = 1;
   return false;
 }
+// Blocks that have ended with a wait that ran out, of this source file's kernels and on this device. The reader
+// waits for the device: streams that do not wait for the default one hold launches too.
+static __device__ unsigned int g_given_up;
+RLENV_D void note_given_up() { atomicAdd(&g_given_up, 1u); }
+static inline int read_given_up(unsigned int* count, bool clear) {
+  const unsigned int zero = 0;
+  if (cudaError_t e = cudaDeviceSynchronize()) return int(e);
+  if (cudaError_t e = cudaMemcpyFromSymbol(count, g_given_up, sizeof zero)) return int(e);
+  return clear ? int(cudaMemcpyToSymbol(g_given_up, &zero, sizeof zero)) : RLENV_OK;
+}
+
 RLENV_D bool elect() {  // one lane of the warp
   uint32_t r;
   asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}" : "=r"(r));

@@ -768,6 +768,7 @@ product_kernel(const __grid_constant__ Product p, int items) {
   __syncthreads();
   if (threadIdx.x == 0) {
     endings[rank].gave_up = dead_flag;
+    if (dead_flag) bw::note_given_up();
     tell(&endings[rank], rank ^ 1);
   }
   bw::cluster_sync();
@@ -1314,6 +1315,12 @@ int rlenv_gated_ffn_backward(int dtype, int activation, int64_t m, int64_t k, in
                                          grad_w_up, l, s)
                             : ffn<__nv_bfloat16>(grad_out, x, w_gate, w_up, m, k, f, activation, nullptr, grad_x,
                                                  grad_w_gate, grad_w_up, l, s);
+}
+
+int rlenv_gated_ffn_status(unsigned int* gave_up, int clear) {
+  if (!gave_up) return RLENV_EINVAL;
+  *gave_up = 0;
+  return rlenv::bw::read_given_up(gave_up, clear != 0);
 }
 
 }  // extern "C"

@@ -10,6 +10,8 @@ have float32's precision, but an infinity, or a magnitude above bfloat16's 3.39e
 The reference's policies are tanh MLPs (es.py:156-164); there is no counterpart there.
 """
 
+import ctypes
+
 import torch
 from torch.autograd.function import once_differentiable
 
@@ -72,6 +74,16 @@ def backward(grad_out, x, w_gate, w_up, activation="silu"):
     _rl.launch(index, lib.gated_ffn_backward, code, ACTIVATIONS[activation], m, k, f, grad_out.data_ptr(), x.data_ptr(),
                w_gate.data_ptr(), w_up.data_ptr(), dx.data_ptr(), dwg.data_ptr(), dwu.data_ptr(), _rl.ptr(tmp), nbytes)
     return dx, dwg, dwu
+
+
+def gave_up(device=None, clear=True):
+    """How many thread blocks on `device` (None: the current one) ended with a wait that ran out since the last
+    clear: zero unless something is wrong with the machine. Results of such a call hold NaN. Waits for the
+    device."""
+    count = ctypes.c_uint(0)
+    with torch.cuda.device(device):
+        _rl.check(_rl.lib().gated_ffn_status(ctypes.byref(count), int(clear)))
+    return count.value
 
 
 class _Apply(torch.autograd.Function):

@@ -89,6 +89,7 @@ _SIGNATURES = {
                                 c_void_p, c_int64, c_void_p],
     "rlenv_gated_ffn_backward": [c_int, c_int, c_int64, c_int64, c_int64, c_void_p, c_void_p, c_void_p, c_void_p,
                                  c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_void_p],
+    "rlenv_gated_ffn_status": [c_void_p, c_int],
     "rlenv_adamw_step": [c_int, c_int, c_int64, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
                          c_void_p, c_double, c_double, c_double, c_double, c_double, c_void_p, c_int64, c_uint32,
                          c_void_p],

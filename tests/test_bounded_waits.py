@@ -49,6 +49,18 @@ def test_time_without_looks_does_not_count(probe):
     assert over(probe, np.arange(1, 400) * 100 * MS) == 200
 
 
+def test_the_status_is_an_error_code_without_a_device():
+    import torch
+
+    import rlenv_lib
+
+    if torch.cuda.is_available():
+        pytest.skip("this is the no-device path")
+    lib, count = rlenv_lib.load(), ctypes.c_uint(7)
+    assert lib.gated_ffn_status(None, 1) == -1
+    assert lib.gated_ffn_status(ctypes.byref(count), 1) > 0 and count.value == 0
+
+
 @pytest.mark.gpu
 def test_a_wait_gives_up(cuda, probe):
     import torch
@@ -60,3 +72,29 @@ def test_a_wait_gives_up(cuda, probe):
     assert (took >= 20 * MS).all() and (took < 2000 * MS).all()
     assert not second.any() and (after < 1000 * MS).all(), "the next wait, of up to 20 s, gives up at the flag"
     assert third.all(), "an arrival ends a wait"
+
+
+@pytest.mark.gpu
+def test_a_wait_that_ran_out_is_counted(cuda, probe):
+    import torch
+
+    out, count = torch.zeros((32, 6), dtype=torch.int64, device=cuda), ctypes.c_uint(7)
+    assert probe.wait_probe_status(ctypes.byref(count), 1) == 0
+    for runs in (1, 2):
+        assert probe.wait_probe(MS, out.data_ptr()) == 0
+        assert probe.wait_probe_status(ctypes.byref(count), 0) == 0 and count.value == runs
+    assert probe.wait_probe_status(ctypes.byref(count), 1) == 0 and count.value == 2
+    assert probe.wait_probe_status(ctypes.byref(count), 0) == 0 and count.value == 0
+
+
+@pytest.mark.gpu
+def test_the_blocks_calls_report_no_wait_that_ran_out(cuda):
+    import torch
+
+    import gated_ffn
+
+    gated_ffn.gave_up()
+    x, w = torch.randn((700, 96), device=cuda), torch.randn((96, 200), device=cuda)
+    y = gated_ffn.forward(x, w, w)
+    gated_ffn.backward(y, x, w, w)
+    assert gated_ffn.gave_up() == 0 and gated_ffn.gave_up(cuda, clear=False) == 0

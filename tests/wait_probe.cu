@@ -28,6 +28,7 @@ __global__ void wait_probe_kernel(unsigned long long limit, long long* out) {
   }
   __syncwarp();
   const bool third = rlenv::bw::barrier_wait_warp(at, 0, &dead, limit);
+  if (threadIdx.x == 0 && flag) rlenv::bw::note_given_up();
   long long* const mine = out + 6 * threadIdx.x;
   mine[0] = first, mine[1] = second, mine[2] = third, mine[3] = flag, mine[4] = t1 - t0, mine[5] = t2 - t1;
 }
@@ -37,6 +38,8 @@ extern "C" int wait_probe(unsigned long long limit, long long* out) {  // out: 3
   wait_probe_kernel<<<1, 32>>>(limit, out);
   return int(cudaDeviceSynchronize());
 }
+
+extern "C" int wait_probe_status(unsigned int* count, int clear) { return rlenv::bw::read_given_up(count, clear); }
 
 // On the host: the first of n looks at the clock, from `start` on, at which a wait of `limit` is over, or -1.
 extern "C" int patience_probe(unsigned long long limit, unsigned long long start, const unsigned long long* looks, int n) {
