@@ -24,6 +24,7 @@ from functools import lru_cache
 
 import torch
 from torch.autograd.function import once_differentiable
+from torch.autograd.graph import increment_version
 
 import rlenv_lib as _rl
 
@@ -136,7 +137,8 @@ def backward(grad_out, q, k, v, decay, state=None, resets=None, scale=None, grad
 
 def step(q, k, v, decay, state, resets=None, scale=None):
     """One token for every environment, q, k, v (N, H, D), resets (N,): updates `state` (N, H, D, D) in
-    place and returns out (N, H, D)."""
+    place and returns out (N, H, D). For acting: out carries no gradient, whatever its inputs do (`attend` is the
+    differentiable form), and a graph that saved `state` before its update raises in its backward pass."""
     shape, dtype, index, resets = _check(1, decay, state, resets, None, ("q", "k", "v"), (q, k, v))
     if state is None or not state.is_contiguous() or state.data_ptr() % 16:
         raise ValueError("state must be contiguous and on a 16-byte boundary: it is updated in place")
@@ -146,6 +148,7 @@ def step(q, k, v, decay, state, resets=None, scale=None):
     _rl.launch(index, _rl.lib().linear_attention_step, _rl.FLOAT_DTYPES[dtype], d, n, h, q.data_ptr(), k.data_ptr(),
                v.data_ptr(), _stride_array(qs, ks, vs), decay.contiguous().data_ptr(), _rl.ptr(resets),
                _scale(scale, d), state.data_ptr(), out.data_ptr())
+    increment_version(state)
     return out
 
 

@@ -665,3 +665,23 @@ def test_ffn_tiles_that_end_anywhere(cuda, m, k, f, dtype):
     """Tiles of which a warp's lanes have some rows and columns and not others."""
     test_ffn_forward(cuda, m, k, f, "gelu", dtype)
     test_ffn_backward(cuda, m, k, f, "gelu", dtype)
+
+
+def test_a_state_stepped_before_the_backward_pass_is_noticed(cuda):
+    """`attend` saves its state; `step` writes it in place, as autograd has to see."""
+    import linear_attention as la
+
+    (q, k, v, _), decay, state, _, _ = inputs(cuda, 5, 2, 2, 16, "f32")
+    leaf = q.clone().requires_grad_()
+    out, _ = la.attend(leaf, k, v, decay, state)
+    version = state._version
+    stepped = la.step(leaf[0], k[0], v[0], decay, state)
+    assert state._version == version + 1 and not stepped.requires_grad
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        out.sum().backward()
+    out, _ = la.attend(leaf, k, v, decay, state.clone())
+    la.step(q[1], k[1], v[1], decay, state)
+    out.sum().backward()
+    assert leaf.grad is not None
+    with torch.inference_mode():  # such tensors keep no versions
+        la.step(q[0], k[0], v[0], decay, torch.zeros_like(state))
