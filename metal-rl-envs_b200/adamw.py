@@ -19,6 +19,7 @@ from functools import lru_cache
 from operator import attrgetter
 
 import torch
+from torch.autograd.graph import increment_version
 
 import rlenv_lib as _rl
 
@@ -104,7 +105,8 @@ def step(params, grads, state, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_dec
          grad_scale=None):
     """Updates params, state and copies in place. grads: one tensor a parameter, all of one dtype.
     grad_scale, a one-element float32 CUDA tensor, multiplies every gradient (clipping by a norm that
-    stays on the device)."""
+    stays on the device). Autograd sees the tensors as written in place: a graph that saved one of them raises in
+    its backward pass."""
     count, sizes = len(state.sizes), tuple(state.sizes)
     if len(params) != count or len(grads) != count or (copies is not None and len(copies) != count):
         raise ValueError(f"{len(params)} params need as many grads, copies and state.sizes")
@@ -132,6 +134,7 @@ def step(params, grads, state, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_dec
     _rl.launch(index, _rl.lib().adamw_step, state.bits, _rl.FLOAT_DTYPES[grad_dtype], count, params_at, grads_at,
                copies_at, sizes_at, state.m.data_ptr(), state.v.data_ptr(), _rl.ptr(state.m_exp), _rl.ptr(state.v_exp),
                lr, b1, b2, eps, weight_decay, _rl.ptr(grad_scale), state.step + 1, state.seed & 0xFFFFFFFF)
+    increment_version([*params, *(copies or ()), state.m, state.v])
     state.step += 1
 
 

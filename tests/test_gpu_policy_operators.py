@@ -685,3 +685,26 @@ def test_a_state_stepped_before_the_backward_pass_is_noticed(cuda):
     assert leaf.grad is not None
     with torch.inference_mode():  # such tensors keep no versions
         la.step(q[0], k[0], v[0], decay, torch.zeros_like(state))
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_weights_stepped_before_the_backward_pass_are_noticed(cuda, bits):
+    """`apply` saves the weights; `adamw.step` writes them and their copies in place, as autograd has to see."""
+    import adamw
+    import gated_ffn
+
+    x, wg, wu, dh = ffn_inputs(cuda, 9, 16, 24, "f32")
+    low = [w.to(torch.bfloat16).requires_grad_() for w in (wg, wu)]
+    weights = [wg.requires_grad_(), wu.requires_grad_()]
+    state = adamw.init_state(weights, bits)
+    for used, inputs_ in ((weights, x), (low, x.to(torch.bfloat16))):
+        out = gated_ffn.apply(inputs_, *used)
+        versions = [w._version for w in weights + low + [state.m, state.v]]
+        adamw.step(weights, [torch.ones_like(w) for w in weights], state, copies=[w.detach() for w in low])
+        assert [w._version for w in weights + low + [state.m, state.v]] == [v + 1 for v in versions]
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            out.sum().backward()
+    gated_ffn.apply(x, *weights).sum().backward()
+    assert all(w.grad is not None for w in weights)
+    with torch.no_grad():
+        adamw.step([w.detach() for w in weights], [w.grad for w in weights], state)
