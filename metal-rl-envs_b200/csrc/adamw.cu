@@ -356,8 +356,7 @@ int rlenv_adamw_step(int state_bits, int grad_dtype, int64_t tensors, float* con
   if (tensors < 0 || step < 1 || !(beta1 >= 0.0 && beta1 < 1.0) || !(beta2 >= 0.0 && beta2 < 1.0) || !(eps >= 0.0))
     return RLENV_EINVAL;
   if (tensors == 0) return RLENV_OK;
-  if (!params || !grads || !sizes || !m || !v || (state_bits == 8 && (!m_exp || !v_exp))) return RLENV_EINVAL;
-  if (!on_boundary(m, state_bits == 8 ? 4 : 16) || !on_boundary(v, state_bits == 8 ? 4 : 16)) return RLENV_EINVAL;
+  if (!params || !grads || !sizes) return RLENV_EINVAL;
   int64_t total = 0;
   for (int64_t i = 0; i < tensors; ++i) {
     if (sizes[i] < 0 || sizes[i] > (int64_t(1) << 40)) return RLENV_EINVAL;
@@ -365,6 +364,9 @@ int rlenv_adamw_step(int state_bits, int grad_dtype, int64_t tensors, float* con
     total += (sizes[i] + kStateBlock - 1) / kStateBlock;
     if (total > (int64_t(1) << 32) / kStateBlock) return RLENV_EINVAL;  // places are hashed as 32-bit words
   }
+  if (total == 0) return RLENV_OK;  // moments of no elements may be NULL
+  if (!m || !v || (state_bits == 8 && (!m_exp || !v_exp))) return RLENV_EINVAL;
+  if (!on_boundary(m, state_bits == 8 ? 4 : 16) || !on_boundary(v, state_bits == 8 ? 4 : 16)) return RLENV_EINVAL;
   AdamArgs a;
   a.b1 = float(beta1), a.c1 = float(1.0 - beta1), a.b2 = float(beta2), a.c2 = float(1.0 - beta2);
   a.rate = float(lr / (1.0 - pow(beta1, double(step))));

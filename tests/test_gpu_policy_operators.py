@@ -708,3 +708,15 @@ def test_weights_stepped_before_the_backward_pass_are_noticed(cuda, bits):
     assert all(w.grad is not None for w in weights)
     with torch.no_grad():
         adamw.step([w.detach() for w in weights], [w.grad for w in weights], state)
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_adamw_of_empty_tensors(cuda, bits):
+    import adamw
+
+    for sizes in ((0,), (0, 0), (0, 7)):
+        params = [torch.ones(n, device=cuda) for n in sizes]
+        state = adamw.init_state(params, bits)
+        adamw.step(params, [torch.ones_like(p) for p in params], state)
+        assert state.step == 1 and [x.numel() for x in adamw.moments(state)] == [256 * any(sizes)] * 2
+        assert (params[-1] < 1).all()

@@ -203,3 +203,19 @@ def test_episode_starts():
     assert linear_attention.episode_starts(dones).tolist() == want
     assert linear_attention.episode_starts(dones, torch.tensor([True, False]))[0].tolist() == [True, False]
     assert linear_attention.episode_starts(dones[:0]).shape == (0, 2)
+
+
+@pytest.mark.parametrize("bits", [8, 32])
+def test_adamw_of_empty_tensors_needs_no_moments(bits):
+    """A tensor without elements has no moments: their pointers may be NULL, as torch's empty tensors' are."""
+    import rlenv_lib
+
+    lib = rlenv_lib.load()
+
+    def step(sizes, at=None, m=None):
+        n = len(sizes)
+        return lib.adamw_step(bits, rlenv_lib.F32, n, (ctypes.c_void_p * n)(*[at] * n), (ctypes.c_void_p * n)(*[at] * n),
+                              None, (ctypes.c_int64 * n)(*sizes), m, m, m, m, 1e-3, 0.9, 0.999, 1e-8, 0.0, None, 1, 0, None)
+
+    assert step([0]) == 0 and step([0, 0, 0]) == 0
+    assert step([0, 5], 0x1000) == -1 and step([5], None, FAKE) == -1 and step([0, -1]) == -1
