@@ -33,11 +33,13 @@ WIDTHS = (16, 32, 64, 128)
 
 def _rows(x):
     """(x, its strides without the last) with rows dense and on 16-byte boundaries; anything else is
-    copied. Axes of one element have stride 0."""
+    copied. Axes of one element have stride 0: torch's is any number, in a contiguous tensor too."""
+    strides = x.stride()
+    if 1 in x.shape:
+        strides = tuple(0 if n == 1 else s for s, n in zip(strides, x.shape))
     if x.is_contiguous() and x.data_ptr() % 16 == 0:
-        return x, x.stride()[:-1]
+        return x, strides[:-1]
     size = x.element_size()
-    strides = tuple(0 if n == 1 else s for s, n in zip(x.stride(), x.shape))
     if strides[-1] != 1 or x.data_ptr() % 16 or any(s * size % 16 or s < 0 for s in strides[:-1]):
         x = x.clone(memory_format=torch.contiguous_format)
         strides = x.stride()

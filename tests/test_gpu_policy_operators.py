@@ -720,3 +720,26 @@ def test_adamw_of_empty_tensors(cuda, bits):
         adamw.step(params, [torch.ones_like(p) for p in params], state)
         assert state.step == 1 and [x.numel() for x in adamw.moments(state)] == [256 * any(sizes)] * 2
         assert (params[-1] < 1).all()
+
+
+def test_attention_takes_any_stride_of_an_axis_of_one(cuda):
+    """One step, environment or head out of a tensor whose rows lie an odd number of elements apart."""
+    import linear_attention as la
+
+    decay = torch.tensor([0.9, 0.5, 0.7], device=cuda)
+    for axis in range(3):
+        shape = [1 if i == axis else n for i, n in enumerate((5, 4, 3))] + [16]
+        strides = [0, 0, 0, 1]
+        for i in range(2, -1, -1):
+            strides[i] = strides[i + 1] * shape[i + 1]
+        strides[axis] = 4097
+        flat = torch.randn(8000, device=cuda)
+        x = flat.as_strided(shape, strides)
+        assert x.is_contiguous()
+        y, g = torch.empty(shape, device=cuda).copy_(x), decay[:shape[2]]
+        for a, b in zip(la.forward(x, x, x, g), la.forward(y, y, y, g)):
+            assert torch.equal(a, b)
+        for a, b in zip(la.backward(x, x, x, x, g), la.backward(y, y, y, y, g)):
+            assert torch.equal(a, b)
+        s, z = torch.ones((2, *shape[1:], 16), device=cuda)
+        assert torch.equal(la.step(x[0], x[0], x[0], g, s), la.step(y[0], y[0], y[0], g, z)) and torch.equal(s, z)

@@ -219,3 +219,21 @@ def test_adamw_of_empty_tensors_needs_no_moments(bits):
 
     assert step([0]) == 0 and step([0, 0, 0]) == 0
     assert step([0, 5], 0x1000) == -1 and step([5], None, FAKE) == -1 and step([0, -1]) == -1
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_rows_have_strides_that_the_kernels_take(dtype):
+    """Bases and strides on 16-byte boundaries, and the same values through them: axes of one element may have any
+    stride in torch, a contiguous tensor's among them."""
+    import linear_attention
+
+    flat = torch.arange(4000, dtype=torch.float32).to(dtype)
+    views = [flat.as_strided((1, 3, 2, 16), (97, 32, 16, 1)), flat.as_strided((3, 1, 2, 16), (32, 7, 16, 1)),
+             flat.as_strided((5, 3, 1, 16), (48, 16, 3, 1)), flat.as_strided((1, 1, 1, 32), (1, 3, 5, 1)),
+             flat.as_strided((4, 3, 2, 16), (97, 32, 16, 1)), flat.as_strided((4, 3, 2, 16), (0, 32, 16, 1)),
+             flat.as_strided((4, 3, 2, 16), (32, 128, 16, 1)), flat[1:97].view(1, 3, 2, 16)]
+    for x in views:
+        y, strides = linear_attention._rows(x)
+        assert len(strides) == 3 and y.data_ptr() % 16 == 0, x.stride()
+        assert all(s * x.element_size() % 16 == 0 for s in strides), (x.stride(), strides)
+        assert torch.equal(y.as_strided(x.shape, (*strides, 1)), x)
