@@ -146,9 +146,9 @@ def step(q, k, v, decay, state, resets=None, scale=None):
         raise ValueError("state must be contiguous and on a 16-byte boundary: it is updated in place")
     n, h, d = shape
     (q, qs), (k, ks), (v, vs) = _rows(q), _rows(k), _rows(v)
-    out = _like(q)
+    decay, out = decay.contiguous(), _like(q)
     _rl.launch(index, _rl.lib().linear_attention_step, _rl.FLOAT_DTYPES[dtype], d, n, h, q.data_ptr(), k.data_ptr(),
-               v.data_ptr(), _stride_array(qs, ks, vs), decay.contiguous().data_ptr(), _rl.ptr(resets),
+               v.data_ptr(), _stride_array(qs, ks, vs), decay.data_ptr(), _rl.ptr(resets),
                _scale(scale, d), state.data_ptr(), out.data_ptr())
     increment_version(state)
     return out

@@ -743,3 +743,24 @@ def test_attention_takes_any_stride_of_an_axis_of_one(cuda):
             assert torch.equal(a, b)
         s, z = torch.ones((2, *shape[1:], 16), device=cuda)
         assert torch.equal(la.step(x[0], x[0], x[0], g, s), la.step(y[0], y[0], y[0], g, z)) and torch.equal(s, z)
+
+
+def test_copies_that_a_call_makes_live_until_its_launch(cuda, monkeypatch):
+    """A decay with strides is copied: memory taken from torch between the checks and the launch is not the copy's."""
+    import linear_attention as la
+    import rlenv_lib
+
+    (q, k, v, g), _, state, _, _ = inputs(cuda, 3, 2, 4, 16, "f32")
+    decay = torch.tensor([[0.9, 0.0], [0.5, 0.0], [0.7, 0.0], [0.1, 0.0]], device=cuda)[:, 0]
+    states = [state.clone() for _ in range(2)]
+    want = [la.step(q[0], k[0], v[0], decay.contiguous(), states[0]), *la.forward(q, k, v, decay.contiguous()),
+            *la.backward(g, q, k, v, decay.contiguous())]
+    launch, taken = rlenv_lib.launch, []
+
+    def launch_late(index, entry, *args):
+        taken.extend(torch.full((n,), 7.0, device=cuda) for n in (4, 4, 4, q.numel(), q[0].numel()))
+        launch(index, entry, *args)
+
+    monkeypatch.setattr(rlenv_lib, "launch", launch_late)
+    got = [la.step(q[0], k[0], v[0], decay, states[1]), *la.forward(q, k, v, decay), *la.backward(g, q, k, v, decay)]
+    assert all(torch.equal(a, b) for a, b in zip(got, want)) and torch.equal(*states)
