@@ -89,7 +89,8 @@ struct FourGrads<__nv_bfloat16> {
 };
 
 // The update's root and quotient from the special function unit, within 2 ulp; no moment passes through
-// them. Values below 2^-126 count as zero.
+// them. Values below 2^-126 count as zero, so that sqrt(v) is off by up to 2^-63: nothing beside an epsilon of
+// 2^-40 and more (times `root`). A smaller one, zero among them, takes the exactly rounded functions (kExact).
 RLENV_D float sqrt_approx(float x) {
   float r;
   asm("sqrt.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
@@ -195,7 +196,7 @@ RLENV_D void unpack(const float4& x, float* to) { to[0] = x.x, to[1] = x.y, to[2
 
 // A warp takes every stride-th state block and reads one ahead: a block's arithmetic, some 80 instructions an
 // element with 8-bit moments, runs under the next one's loads.
-template <typename G, bool kEight>
+template <typename G, bool kEight, bool kExact>
 __global__ void __launch_bounds__(kAdamThreads, kPerSm[kEight]) adamw_kernel(const __grid_constant__ AdamArgs a) {
   const int lane = threadIdx.x & 31;
   const uint32_t stride = gridDim.x * (kAdamThreads / 32), end = a.t[0].first + a.blocks;
@@ -249,8 +250,8 @@ __global__ void __launch_bounds__(kAdamThreads, kPerSm[kEight]) adamw_kernel(con
       const float y = __fmul_rn(g[j], gs);
       m[j] = __fadd_rn(__fmul_rn(m[j], a.b1), __fmul_rn(y, a.c1));
       v[j] = __fadd_rn(__fmul_rn(v[j], a.b2), __fmul_rn(__fmul_rn(y, y), a.c2));
-      const float denom = fmaf(sqrt_approx(v[j]), a.root, a.eps);
-      p[j] = __fsub_rn(__fmul_rn(p[j], a.keep), quotient_approx(m[j] * a.rate, denom));
+      const float denom = fmaf(kExact ? __fsqrt_rn(v[j]) : sqrt_approx(v[j]), a.root, a.eps), top = m[j] * a.rate;
+      p[j] = __fsub_rn(__fmul_rn(p[j], a.keep), kExact ? __fdiv_rn(top, denom) : quotient_approx(top, denom));
       if constexpr (kEight) {
         top_m = max(top_m, __float_as_uint(m[j]) & 0x7fffffffu);
         top_v = max(top_v, __float_as_uint(v[j]) & 0x7fffffffu);
@@ -338,7 +339,9 @@ template <typename G, bool kEight>
 int adamw_launch(const AdamArgs& a, cudaStream_t stream) {
   constexpr uint32_t kWarps = kAdamThreads / 32, kMost = kSms * kPerSm[kEight];
   const uint32_t grid = (a.blocks + kWarps - 1) / kWarps < kMost ? (a.blocks + kWarps - 1) / kWarps : kMost;
-  adamw_kernel<G, kEight><<<grid, kAdamThreads, 0, stream>>>(a);
+  constexpr float kApproxEps = 0x1p-40f;
+  if (a.eps >= kApproxEps * a.root) adamw_kernel<G, kEight, false><<<grid, kAdamThreads, 0, stream>>>(a);
+  else adamw_kernel<G, kEight, true><<<grid, kAdamThreads, 0, stream>>>(a);
   return launch_status();
 }
 

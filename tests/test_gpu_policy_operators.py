@@ -764,3 +764,21 @@ def test_copies_that_a_call_makes_live_until_its_launch(cuda, monkeypatch):
     monkeypatch.setattr(rlenv_lib, "launch", launch_late)
     got = [la.step(q[0], k[0], v[0], decay, states[1]), *la.forward(q, k, v, decay), *la.backward(g, q, k, v, decay)]
     assert all(torch.equal(a, b) for a, b in zip(got, want)) and torch.equal(*states)
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("eps", [0.0, 1e-16, 1e-13, 1e-8])
+def test_adamw_of_tiny_gradients(cuda, bits, eps):
+    """Gradients down to 1e-20, whose second moments lie below float32's smallest normal number: the update is the
+    formula's for every epsilon, some lr without one. From parameters of zero, so that the update alone counts; its
+    roundings, of root, product, sum and quotient, are some ulps of 2^-23 each."""
+    import adamw
+
+    f, n = np.float32, 1000
+    g = np.geomspace(1e-20, 1e-16, n).astype(f) * np.where(np.arange(n) % 2, f(1), f(-1))
+    params, lr, (b1, b2) = [torch.zeros(n, device=cuda)], 1e-3, (0.9, 0.999)
+    adamw.step(params, [torch.from_numpy(g).to(cuda)], adamw.init_state(params, bits), lr, (b1, b2), eps, 0.0)
+    m, v = (g * f(1 - b1)).astype(float), ((g * g) * f(1 - b2)).astype(float)
+    assert (v > 0).all() and (v < 2.0 ** -126).any()
+    want = -lr / (1 - b1) * m / (np.sqrt(v / (1 - b2)) + eps)
+    assert (abs(to64(params[0]) - want) <= 2.0 ** -20 * abs(want)).all()
