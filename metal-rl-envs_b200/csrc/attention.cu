@@ -464,6 +464,7 @@ join_kernel(const __grid_constant__ Problem p, const __grid_constant__ Split spl
   float z = s.carry_in ? s.in_mul * __ldg(s.carry_in + outside) : 0.0f;
   float* const own = split.carry + which * split.segments * size + at;
   const float* const through = split.through + which * split.segments;
+  const float g = __ldg(p.decay + seq % p.h);
   constexpr int kAhead = 8;  // loads in flight: the sums are a chain, the loads are not
   for (int64_t g0 = 0; g0 < split.segments; g0 += kAhead) {
     float mine[kAhead], over[kAhead];
@@ -474,7 +475,9 @@ join_kernel(const __grid_constant__ Problem p, const __grid_constant__ Split spl
     for (int i = 0; i < kAhead; ++i)
       if (g0 + i < split.segments) {
         own[(g0 + i) * size] = z;
-        z = (over[i] < 0.0f ? 0.0f : over[i] * z) + mine[i];
+        // A power of a positive decay that has underflowed leaves an infinity one, as token by token.
+        const float kept = over[i] * z;
+        z = (over[i] < 0.0f ? 0.0f : kept != kept && z == z && g > 0.0f ? z : kept) + mine[i];
       }
   }
   if (s.carry_out) s.carry_out[outside] = s.out_mul * z;

@@ -782,3 +782,32 @@ def test_adamw_of_tiny_gradients(cuda, bits, eps):
     assert (v > 0).all() and (v < 2.0 ** -126).any()
     want = -lr / (1 - b1) * m / (np.sqrt(v / (1 - b2)) + eps)
     assert (abs(to64(params[0]) - want) <= 2.0 ** -20 * abs(want)).all()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_infinities_of_long_sequences_are_the_definitions(cuda, dtype):
+    """Without resets an infinity stays one, however long it decays, and is NaN where the decay is zero: in
+    sequences that are split over the time axis too."""
+    import linear_attention as la
+
+    t, d = 4000, 16
+    (q, k, v, do), _, state, gstate, _ = inputs(cuda, t, 1, 3, d, dtype, seed=9)
+    q, k, v, do = (x.abs() for x in (q, k, v, do))
+    decay = torch.tensor([0.9, 0.5, 0.0], device=cuda)
+    for at in (3, 2000):
+        bad = k.clone()
+        bad[at, :, :, 1] = np.inf
+        with np.errstate(invalid="ignore"):
+            want, wend = policy.scan(to64(q), to64(bad), to64(v), to64(decay), None, None, d ** -0.5)
+        out, end = la.forward(q, bad, v, decay)
+        for got, w in ((out, want), (end, wend)):
+            got = to64(got)
+            assert (np.isposinf(got) == np.isposinf(w)).all() and (np.isnan(got) == np.isnan(w)).all()
+        assert np.isposinf(wend[0, :2, 1]).all() and np.isnan(wend[0, 2, 1]).all()
+    bad = do.clone()  # and from the last token to the first
+    bad[t - 3, :, :, 2] = np.inf
+    with np.errstate(invalid="ignore"):
+        wants = policy.attention_grad(to64(bad), to64(q), to64(k), to64(v), to64(decay), None, None, d ** -0.5, None)
+    for got, w in zip(la.backward(bad, q, k, v, decay), wants):
+        got = to64(got)
+        assert (np.isposinf(got) == np.isposinf(w)).all() and (np.isnan(got) == np.isnan(w)).all()
