@@ -33,3 +33,24 @@ def test_training_makes_episodes_longer(cuda, bits):
     _, lengths = mp.train(mp.Config(envs=512, updates=80, state_bits=bits))
     early, late = sum(lengths[:5]) / 5, sum(lengths[-5:]) / 5
     assert late > 2 * early, (early, late)
+
+
+def test_training_uses_the_memory(cuda, monkeypatch):
+    """The same policy with every token marked as an episode's first sees one frame. Without the velocities no
+    action drawn from one frame keeps the pole up for long: a search over logistic policies of position and angle, on
+    4,000 environments in numpy, ends at 53.5 steps an episode. With its memory the policy passes that by far."""
+    import linear_attention as la
+    import memory_policy as mp
+
+    def late(cfg):
+        return sum(mp.train(cfg)[1][-5:]) / 5
+
+    cfg = mp.Config(envs=512, updates=100)
+    with_memory = late(cfg)
+    for name in ("step", "attend"):
+        def always_first(q, k, v, decay, state, resets, call=getattr(la, name)):
+            return call(q, k, v, decay, state, torch.ones_like(resets))
+
+        monkeypatch.setattr(la, name, always_first)
+    without = late(cfg)
+    assert without < 60 and with_memory > 75, (without, with_memory)

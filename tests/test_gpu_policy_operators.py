@@ -811,3 +811,93 @@ def test_infinities_of_long_sequences_are_the_definitions(cuda, dtype):
     for got, w in zip(la.backward(bad, q, k, v, decay), wants):
         got = to64(got)
         assert (np.isposinf(got) == np.isposinf(w)).all() and (np.isnan(got) == np.isnan(w)).all()
+
+
+# ---- what the larger sizes reach ---------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("sizes", [(700_001, 255, 1_300_007, 0, 3, 1_000_000, 77),
+                                   (9, 300_000) * 20 + (1,)])
+def test_adamw_of_more_blocks_than_warps(cuda, sizes, dtype, bits):
+    """Warps that take several blocks of 256 elements, read ahead and cross from tensor to tensor: two steps against
+    the definition in 64 bits, moments as in the small cases exactly."""
+    import adamw
+
+    f, lr, betas, eps, wd = np.float32, 1e-2, (0.9, 0.999), 1e-8, 0.1
+    params, _ = adam_inputs(cuda, sizes, dtype, 0, True)
+    copies = [torch.zeros_like(p, dtype=torch.bfloat16) for p in params]
+    state = adamw.init_state(params, bits, seed=5)
+    p = padded([x.cpu().numpy() for x in params]).astype(np.float64)
+    assert p.size // 256 > 4736 and all(x.is_contiguous() for x in params)
+    m, v = np.zeros(p.size, f), np.zeros(p.size, f)
+    for t in (1, 2):
+        _, grads = adam_inputs(cuda, sizes, dtype, t, True)
+        adamw.step(params, grads, state, lr, betas, eps, wd, copies)
+        g = padded([x.float().cpu().numpy() for x in grads])
+        before = p
+        p, m64, v64 = policy.adamw(p, g.astype(float), m.astype(float), v.astype(float), t, lr, betas, eps, wd)
+        m = m * f(betas[0]) + g * f(1 - betas[0])
+        v = v * f(betas[1]) + (g * g) * f(1 - betas[1])
+        assert np.allclose(m, m64, rtol=1e-6, atol=1e-9) and np.allclose(v, v64, rtol=1e-6, atol=1e-12)
+        if bits == 8:
+            words = policy.rounding_words(p.size, 5, t)
+            (cm, em), (cv, ev) = policy.encode(m, words & 0xFFFF, 4), policy.encode(v, words >> 16, 5)
+            for name, want in (("m", cm), ("m_exp", em), ("v", cv), ("v_exp", ev)):
+                assert (getattr(state, name).cpu().numpy() == want).all(), name
+            m, v = policy.decode(cm, em, 4), policy.decode(cv, ev, 5)
+        gm, gv = (x.cpu().numpy() for x in adamw.moments(state))
+        assert (gm == m).all() and (gv == v).all()
+        # the update is at most some lr large: 16 roundings of it, and two of the parameter, a step
+        off = abs(padded([to64(x) for x in params]) - p)
+        assert (off <= t * (2.0 ** -20 * (abs(p - before) + lr) + 2.0 ** -22 * abs(p))).all(), off.max()
+    for c, x in zip(copies, params):
+        assert torch.equal(c, x.to(torch.bfloat16))
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("m,k,f", [(5000, 300, 520), (2100, 70, 2300), (20_000, 61, 173)])
+def test_ffn_forward_of_several_tiles_a_pair(cuda, m, k, f, dtype):
+    """More tiles than pairs of SMs: accumulators, rings and epilogues go on from tile to tile."""
+    test_ffn_forward(cuda, m, k, f, "gelu", dtype)
+
+
+@pytest.mark.parametrize("rows", [2, 700])
+def test_ffn_of_large_bfloat16_values(cuda, rows):
+    """By matrix-vector products and by tiles: 6400 x 6400 to half an ulp of bfloat16, 2^-8 of it at most."""
+    import gated_ffn
+
+    big = torch.full((rows, 32), 200.0, device=cuda, dtype=torch.bfloat16)
+    w = torch.ones((32, 264), device=cuda, dtype=torch.bfloat16)
+    for act in ("silu", "gelu"):
+        out = gated_ffn.forward(big, w, w, act).double()
+        assert ((out - 6400.0 ** 2).abs() <= 2.0 ** -8 * 6400.0 ** 2).all()
+        assert not gated_ffn.forward(big, -w, w, act).any()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_attention_of_few_tokens_takes_any_strides(cuda, dtype):
+    """Tokens one after the other, every operand with strides of its own: the bits of dense copies."""
+    import linear_attention as la
+
+    t, n, h, d = 5, 150, 4, 32
+    g = torch.Generator(device=cuda).manual_seed(15)
+
+    def draw(*shape):
+        return torch.randn(shape, generator=g, device=cuda).to(TYPES[dtype])
+
+    fused = draw(n, t, 3, h, d).transpose(0, 1)
+    q, k = fused[:, :, 0], draw(h, t, n, d).permute(1, 2, 0, 3)
+    v, do = draw(t, n, 1, d).expand(t, n, h, d), draw(t, h, n, d + 16)[..., 16:].transpose(1, 2)
+    assert len({x.stride() for x in (q, k, v, do)}) == 4
+    decay = torch.tensor([0.9, 0.99, 0.5, 0.0], device=cuda)
+    state, gstate = torch.randn((2, n, h, d, d), generator=g, device=cuda)
+    resets = (torch.rand((n, t), generator=g, device=cuda) < 0.1).t()
+    for order in ((q, k, v, do), (k, v, do, q), (v, do, q, k), (do, q, k, v)):
+        dense = [x.contiguous() for x in order]
+        for a, b in zip(la.forward(*order[:3], decay, state, resets), la.forward(*dense[:3], decay, state, resets)):
+            assert torch.equal(a, b)
+        for a, b in zip(la.backward(*order, decay, state, resets, None, gstate),
+                        la.backward(*dense, decay, state, resets, None, gstate)):
+            assert torch.equal(a, b)
