@@ -21,6 +21,7 @@ where a negative decay is raised to a power.
 
 import ctypes
 from functools import lru_cache
+from math import gcd
 
 import torch
 from torch.autograd.function import once_differentiable
@@ -33,11 +34,12 @@ WIDTHS = (16, 32, 64, 128)
 
 def _rows(x):
     """(x, its strides without the last) with rows dense and on 16-byte boundaries; anything else is
-    copied. Axes of one element have stride 0: torch's is any number, in a contiguous tensor too."""
-    strides = x.stride()
-    if 1 in x.shape:
-        strides = tuple(0 if n == 1 else s for s, n in zip(strides, x.shape))
-    if x.is_contiguous() and x.data_ptr() % 16 == 0:
+    copied. Axes of one element get stride 0 where torch's, which is any number, would not do."""
+    strides, dense = x.stride(), x.is_contiguous() and x.data_ptr() % 16 == 0
+    if dense and gcd(*strides[:-1]) % 16 == 0:
+        return x, strides[:-1]
+    strides = tuple(0 if n == 1 else s for s, n in zip(strides, x.shape))
+    if dense:
         return x, strides[:-1]
     size = x.element_size()
     if strides[-1] != 1 or x.data_ptr() % 16 or any(s * size % 16 or s < 0 for s in strides[:-1]):
