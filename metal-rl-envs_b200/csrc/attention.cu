@@ -15,7 +15,7 @@ using attn::Strides;
 // chunk_kernel<whole> the outputs.
 //
 // Measured: bfloat16 heads of 64, 500 steps x 256 x 8, 230 us (2.6 TB/s of the tensors; the tensor pipe 45% busy,
-// shared memory 60%, issue 44%: a warp's fragments come from shared memory, and what a warp waits for next is
+// shared memory 61%, issue 42%: a warp's fragments come from shared memory, and what a warp waits for next is
 // hidden by two other warps of its scheduler only); gradient of half as many 328 us. float32 heads of 128, 16,384
 // steps x 8, 420 us, of which 101 us are the segments' own carries and 8 us the joining.
 struct Split {

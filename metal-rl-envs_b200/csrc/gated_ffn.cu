@@ -2,6 +2,9 @@
 // gradient. With g = x Wg, u = x Wu and the gradient dh of h,
 //     dg = dh u act'(g),   du = dh act(g),
 //     dx = dg Wg' + du Wu',   dWg = x' dg,   dWu = x' du.
+// dg and du pass through the inputs' type on their way into the last three products, for bfloat16 through its 8 bits, as
+// in a program that keeps them as tensors: a second plane would double those products' time. Against 64 bits the
+// gradients of 8,192 x 1,024 x 2,720 are off by 0.0023, with 32-bit dg and du by 0.0017. (Few rows keep them in 32.)
 // The backward pass forms g and u again from x instead of keeping them: 2 M F values less to
 // store and read, and no rounding of g and u to the inputs' type.
 //
@@ -35,10 +38,12 @@ RLENV_D float reciprocal_approx(float x) {
 }
 
 // act(g) and act'(g): silu g / (1 + e^-g), or gelu g Phi(g) with the exact normal distribution. For bfloat16 results
-// the fast exponential and reciprocal, good to 2^-20, are enough, and so is a polynomial for Phi: with z = |g| /
-// sqrt 2 and t = 1 / (1 + 0.46 z), erfc(z) = e^(-z^2) t p(t), p of degree 7 fitted to erfc by least squares weighted
-// towards the smallest largest relative error, 6.8e-7 (2^-20); e^(-z^2) serves the density too. The epilogue's
-// instructions bound short contractions: gelu's gates of 16,384 x 512 x 1,376 take 68 us, with erfcf 97.
+// (half an ulp is 2^-9) the fast exponential and reciprocal are enough: __expf(x) is within 2 + 1.173 |x| ulp, 2^-20
+// of its value where |x| < 5 and 2^-16 where it underflows, far out in silu's and gelu's negative tails. So is a
+// polynomial for Phi: with z = |g| / sqrt 2 and t = 1 / (1 + 0.46 z), erfc(z) = e^(-z^2) t p(t), p of degree 7 fitted to
+// erfc by least squares weighted towards the smallest largest relative error, 7.1e-7 with the coefficients as printed;
+// e^(-z^2) serves the density too. The epilogue's instructions bound short contractions: gelu's gates of 16,384 x
+// 512 x 1,376 take 68 us, with erfcf 97.
 template <bool kFast, int kAct>
 RLENV_D void activate(float g, float* y, float* slope) {
   if constexpr (kAct == kSilu) {

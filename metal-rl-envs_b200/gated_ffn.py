@@ -6,7 +6,10 @@ float32 or bfloat16; sums are in 32 bits. activation is "silu" or "gelu" (the ex
 distribution). `backward` forms both products again instead of keeping them. `apply` is the
 differentiable form. The projection back to K is a plain matrix product and is left to the caller.
 float32 operands go through the tensor cores as sums of three bfloat16 terms, but for few rows: results
-have float32's precision, but an infinity, or a magnitude above bfloat16's 3.39e38, may come out as NaN.
+have float32's precision, but an infinity, or a magnitude above bfloat16's 3.39e38, may come out as NaN, and of
+operands below 2^-110 (8e-34) the lower terms are lost. bfloat16 gradients: the two products' own gradients,
+grad_out act'(x w_gate) (x w_up) and grad_out act(x w_gate), are rounded to bfloat16 before the products that
+follow.
 The reference's policies are tanh MLPs (es.py:156-164); there is no counterpart there.
 """
 
