@@ -349,8 +349,9 @@ RLENV_API int rlenv_reset_uniform(float* out, int rows, int64_t n, const float* 
  * byte each, or NULL; decay (h) float32 in [0, 1]. strides (host) holds the elements between
  * steps, environments and heads of q, then of k, then of v; the last axis is dense. Bases and
  * strides must keep rows on 16-byte boundaries. state_in (n, h, d, d) may be NULL for zero.
- * scale is finite and not zero (the gradient divides by it: grad_state_out / scale has to be a float32). Sums and states are held in 32 bits or more. Products of bf16
- * values that pass through 16 bits keep a second 16-bit term.
+ * scale is finite and not zero (the gradient divides by it: grad_state_out / scale has to be a
+ * float32). Sums and states are held in 32 bits or more. Products of bf16 values that pass
+ * through 16 bits keep a second 16-bit term.
  *
  * forward: out (t, n, h, d) dense and state_out, the state after the last token; state_out
  * must not alias state_in. t = 0 copies the state. scratch: device memory of at least
@@ -386,8 +387,8 @@ RLENV_API int rlenv_linear_attention_step(int dtype, int d, int64_t n, int64_t h
 /* Gated feed-forward block: out = act(x w_gate) * (x w_up), x (m, k), weights (k, f), out (m, f),
  * all dense row-major of one dtype (RLENV_F32 or RLENV_BF16), x, the weights and the
  * results on 16-byte boundaries, products summed in 32 bits. float32 operands pass the tensor cores as sums of three
- * bfloat16 terms (an infinity may come out as NaN; of operands below 2^-110 the lower terms are lost). A launch takes all tensor-memory columns of its
- * SMs and frees them before it ends.
+ * bfloat16 terms (an infinity may come out as NaN; of operands below 2^-110 the lower terms are
+ * lost). A launch takes all tensor-memory columns of its SMs and frees them before it ends.
  * activation: RLENV_SILU, or RLENV_GELU with the exact normal distribution. scratch: device
  * memory of at least rlenv_gated_ffn_scratch_bytes bytes, 256-byte aligned (NULL when that is 0). */
 #define RLENV_SILU 0
@@ -406,10 +407,10 @@ RLENV_API int rlenv_gated_ffn_backward(int dtype, int activation, int64_t m, int
                                        void* grad_x, void* grad_w_gate, void* grad_w_up, void* scratch,
                                        int64_t scratch_bytes, void* stream);
 
-/* The block's kernels wait on barriers of their own, each wait for two seconds at most. One that runs out (it
- * never has) leaves NaN in the results that it was for, and is counted: *gave_up is the number of thread
- * blocks on the current device that ended so since the library was loaded or the count last cleared. Waits for
- * the device. */
+/* The block's kernels wait on barriers of their own, each wait for two seconds at most (of the GPU's time on
+ * them). One that runs out leaves NaN in the results that it was for, and is counted: *gave_up is the number of
+ * thread blocks on the current device that ended so since the library was loaded or the count last cleared.
+ * Waits for the device. */
 RLENV_API int rlenv_gated_ffn_status(unsigned int* gave_up, int clear);
 
 /* One AdamW step over many tensors, in place:

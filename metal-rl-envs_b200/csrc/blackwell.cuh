@@ -80,6 +80,7 @@ RLENV_D bool barrier_wait_warp(uint32_t bar, uint32_t parity, volatile int* dead
   *dead = 1;
   return false;
 }
+
 // Blocks that have ended with a wait that ran out, of this source file's kernels and on this device. The reader
 // waits for the device: streams that do not wait for the default one hold launches too.
 static __device__ unsigned int g_given_up;

@@ -2,9 +2,10 @@
 // gradient. With g = x Wg, u = x Wu and the gradient dh of h,
 //     dg = dh u act'(g),   du = dh act(g),
 //     dx = dg Wg' + du Wu',   dWg = x' dg,   dWu = x' du.
-// dg and du pass through the inputs' type on their way into the last three products, for bfloat16 through its 8 bits, as
-// in a program that keeps them as tensors: a second plane would double those products' time. Against 64 bits the
-// gradients of 8,192 x 1,024 x 2,720 are off by 0.0023, with 32-bit dg and du by 0.0017. (Few rows keep them in 32.)
+// dg and du pass through the inputs' type on their way into the last three products, for bfloat16 through its 8
+// bits, as in a program that keeps them as tensors: a second plane would double those products' time. Against 64
+// bits the gradients of 8,192 x 1,024 x 2,720 are off by 0.0023, with 32-bit dg and du by 0.0017. (Few rows keep
+// them in 32.)
 // The backward pass forms g and u again from x instead of keeping them: 2 M F values less to
 // store and read, and no rounding of g and u to the inputs' type.
 //
@@ -498,9 +499,10 @@ RLENV_D void tell(const Ending* e, uint32_t rank) {  // the same place in the ot
 }
 
 // After a wait that ran out: what is under way lands before the pair may end and tensor memory is freed, each with
-// a wait of its own, up to one that runs out too. Products behind the last commit get one. A buffer's bytes all count at the first block: where
-// one block has filled it and the other has not, the other's are struck off, or its own alone expected (the blocks
-// are less than a round of the ring apart). Then every barrier's last phase, by the number of its rounds.
+// a wait of its own, up to one that runs out too. Products behind the last commit get one. A buffer's bytes all
+// count at the first block: where one block has filled it and the other has not, the other's are struck off, or its
+// own alone expected (the blocks are a round of the ring apart at most). Then every barrier's last phase, by the
+// number of its rounds.
 template <int kStages>
 __device__ __noinline__ void drain(const Ending* endings, int rank, int warp, uint32_t full, uint32_t bytes, uint32_t empty,
                                    uint32_t summed, uint32_t drained) {
