@@ -434,6 +434,76 @@ RLENV_API int rlenv_adamw_step(int state_bits, int grad_dtype, int64_t tensors, 
 RLENV_API int rlenv_adamw_moments(int64_t blocks, const uint8_t* m, const uint8_t* v, const uint8_t* m_exp,
                                   const uint8_t* v_exp, float* m_out, float* v_out, void* stream);
 
+/* Root-mean-square norm with the residual's addition: t = x + residual (residual NULL: t = x),
+ * r = (t't / k + eps)^(-1/2), out = t r weight (weight NULL: 1). Rows of k values of dtype
+ * RLENV_F32 or RLENV_BF16; x_stride and residual_stride are the values between rows (0: the
+ * same row again), the last axis is dense, out and total (t rounded to dtype; may be NULL) are
+ * dense (m, k). Sums in 32 bits; out is formed from t before its rounding. eps >= 0. Rows may
+ * start anywhere; where everything is on 16-byte boundaries accesses are 16 bytes wide. */
+RLENV_API int rlenv_rms_norm_forward(int dtype, int64_t m, int64_t k, const void* x, int64_t x_stride,
+                                     const void* residual, int64_t residual_stride, const void* weight, float eps,
+                                     void* out, void* total, void* stream);
+
+/* The same in 8-bit integers: codes row i holds round(out 127 / a) and scale[i] a / 127, a the
+ * row's largest magnitude. normalise 0: of t weight instead of the norm. Rows of codes are
+ * `pitch` >= k bytes apart, bytes past k are left as they are. A row whose a is below 2^-100 is
+ * zeros with scale 0; one that holds a value that is not finite is zeros with scale NaN. */
+RLENV_API int rlenv_rms_norm_codes(int dtype, int64_t m, int64_t k, const void* x, int64_t x_stride,
+                                   const void* residual, int64_t residual_stride, const void* weight, float eps,
+                                   int normalise, int8_t* codes, int64_t pitch, float* scale, void* total,
+                                   void* stream);
+
+/* The norm's gradient: from grad_out and, where t is used further, grad_total (or NULL) the gradient
+ * grad (m, k) of t, which x's and the residual's both are, and the weight's, grad_weight (k) of
+ * dtype (NULL: not wanted). total is t. With grad_weight, scratch is device memory of at least
+ * rlenv_rms_norm_scratch_bytes bytes, 256-byte aligned, and m >= 1. */
+RLENV_API int64_t rlenv_rms_norm_scratch_bytes(int64_t m, int64_t k);
+
+RLENV_API int rlenv_rms_norm_backward(int dtype, int64_t m, int64_t k, const void* grad_out, int64_t grad_out_stride,
+                                      const void* total, int64_t total_stride, const void* weight, float eps,
+                                      const void* grad_total, int64_t grad_total_stride, void* grad,
+                                      void* grad_weight, void* scratch, int64_t scratch_bytes, void* stream);
+
+/* Product of 8-bit integers with scales: out (m, f) of dtype RLENV_F32 or RLENV_BF16, dense,
+ *     out[i][j] = (sum over k of a[i][k] w[j][k]) a_scale[i] w_scale[j],
+ * the sums exact in 32-bit integers (1 <= k <= 131071). a (m, k) and w (f, k): signed bytes, rows
+ * a_pitch and w_pitch bytes apart (multiples of 16, bases on 16-byte boundaries; bytes past k are
+ * not looked at). scratch: device memory of at least rlenv_int8_linear_scratch_bytes bytes,
+ * 256-byte aligned (NULL when that is 0). */
+RLENV_API int64_t rlenv_int8_linear_scratch_bytes(int64_t m, int64_t k, int64_t f);
+
+RLENV_API int rlenv_int8_linear_forward(int dtype, int64_t m, int64_t k, int64_t f, const int8_t* a, int64_t a_pitch,
+                                        const float* a_scale, const int8_t* w, int64_t w_pitch, const float* w_scale,
+                                        void* out, void* scratch, int64_t scratch_bytes, void* stream);
+
+/* Scores of actions: for each of m rows of v logits l (dtype RLENV_F32 or RLENV_BF16, `stride` values
+ * between rows, last axis dense), over the actions that `allowed` admits (one byte each, rows
+ * allowed_stride apart; NULL: all),
+ *     normalizer = log sum exp(l),   log_prob = l[action] - normalizer,
+ *     entropy = - sum p log p,   p = exp(l - normalizer),
+ * float32 (m) each, and the `top` <= 32 largest l in falling order, ties to the lowest action:
+ * top_actions int64 and top_log_probs float32, (m, top) each. actions: int32, int64 or uint8 (m). A
+ * negative action marks a row without one: log_prob is 0. One of v or above: NaN. An action that is
+ * not allowed counts as a logit of -infinity; what is in its place is not looked at. Rows that
+ * allow nothing: normalizer and log-probabilities -infinity, entropy 0. Rows with a NaN or
+ * +infinity among the logits allowed: NaN, a NaN counting as the largest among top_actions. top
+ * <= v. */
+RLENV_API int rlenv_log_probs_forward(int dtype, int64_t m, int64_t v, const void* logits, int64_t stride,
+                                      const void* actions, int action_dtype, const uint8_t* allowed,
+                                      int64_t allowed_stride, float* log_prob, float* entropy, float* normalizer,
+                                      int top, int64_t* top_actions, float* top_log_probs, void* stream);
+
+/* Their gradient: grad (m, v) of dtype, dense, from grad_log_prob (m) and grad_entropy (m) (either may be
+ * NULL for zero), the forward pass's normalizer and entropy:
+ *     grad_j = grad_log_prob ([j = action] - p_j) - grad_entropy p_j (log p_j + entropy),
+ * zero where an action is not allowed or its logit is -infinity, and in rows that allow nothing. Rows
+ * with a negative action have no first term; with one of v or above they are NaN elsewhere. */
+RLENV_API int rlenv_log_probs_backward(int dtype, int64_t m, int64_t v, const float* grad_log_prob,
+                                       const float* grad_entropy, const void* logits, int64_t stride,
+                                       const void* actions, int action_dtype, const float* normalizer,
+                                       const float* entropy, const uint8_t* allowed, int64_t allowed_stride,
+                                       void* grad, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,120 @@
+"""Scores of actions from a policy's logits, as sm_100a kernels: the log-probability of each token's chosen action, the
+entropy of its distribution and its best alternatives, and their gradient.
+
+    normalizer = log sum exp(logits),   log_prob = logits[action] - normalizer,   entropy = - sum p log p
+
+logits (..., A) are float32 or bfloat16, actions (...) integers, `allowed` (..., A) bool says which actions there are in
+a token (None: all; what stands in the others' places is not looked at). Results are float32. Everything is formed in
+one reading of the logits; the gradient is one reading and one writing.
+
+- A negative action marks a token without one (padding): its log_prob is 0 and has no gradient. One of A or above gives
+  NaN, in the gradient too.
+- A token that allows nothing has normalizer and log_prob -infinity, entropy 0 and no gradient; an action that is not
+  allowed, or whose logit is -infinity, has log_prob -infinity and no gradient of its own place.
+- A NaN or +infinity among a token's allowed logits makes its results NaN.
+
+The reference's policies act greedily and have no gradient (es.py:156-175); there is no counterpart there.
+"""
+
+from typing import NamedTuple
+
+import torch
+from torch.autograd.function import once_differentiable
+
+import rlenv_lib as _rl
+
+MOST_ALTERNATIVES = 32
+
+
+class Scores(NamedTuple):
+    """Of logits (..., A): log_prob, entropy and normalizer (...) float32; of the alternatives asked for, best first
+    (ties: the lower action), top_log_probs (..., n) float32 and top_actions (..., n) int64, None without."""
+    log_prob: torch.Tensor
+    entropy: torch.Tensor
+    normalizer: torch.Tensor
+    top_log_probs: torch.Tensor | None = None
+    top_actions: torch.Tensor | None = None
+
+
+def _check(logits, actions, allowed):
+    """(rows, A, the type's code, the actions' code, the device's index)"""
+    if not isinstance(logits, torch.Tensor) or not logits.is_cuda or logits.dtype not in _rl.FLOAT_DTYPES:
+        _rl.as_floats("logits", logits)
+    shape, index = logits.shape, logits.get_device()
+    if not shape or shape[-1] == 0:
+        raise ValueError(f"logits must be (..., A) with A of at least 1; got shape {tuple(shape)}")
+    if not isinstance(actions, torch.Tensor) or actions.dtype not in _ACTIONS or actions.shape != shape[:-1]:
+        raise ValueError(f"actions must be an int64, int32 or uint8 tensor of shape {tuple(shape[:-1])}")
+    if allowed is not None and (not isinstance(allowed, torch.Tensor) or allowed.dtype not in (torch.bool, torch.uint8)
+                                or allowed.shape != shape):
+        raise ValueError(f"allowed must be a bool or uint8 tensor of shape {tuple(shape)}")
+    if actions.get_device() != index or (allowed is not None and allowed.get_device() != index):
+        _rl.one_device(index, actions=actions, allowed=allowed)
+    return shape[:-1].numel(), shape[-1], _rl.FLOAT_DTYPES[logits.dtype], _ACTIONS[actions.dtype], index
+
+
+_ACTIONS = {torch.int64: _rl.I64, torch.int32: _rl.I32, torch.uint8: _rl.U8}
+
+
+def forward(logits, actions, allowed=None, alternatives=0):
+    """Scores of the actions, and of the `alternatives` (up to 32) best ones."""
+    m, v, code, action_code, index = _check(logits, actions, allowed)
+    if not 0 <= alternatives <= min(v, MOST_ALTERNATIVES):
+        raise ValueError(f"alternatives must be from 0 to {min(v, MOST_ALTERNATIVES)}; got {alternatives}")
+    lead = logits.shape[:-1]
+    logits, stride = _rl.as_rows(logits)
+    allowed, allowed_stride = (None, 0) if allowed is None else _rl.as_rows(allowed)
+    actions = actions.contiguous()
+    log_prob, entropy, normalizer = (logits.new_empty(lead, dtype=torch.float32) for _ in range(3))
+    top, best = None, None
+    if alternatives:
+        top = logits.new_empty((*lead, alternatives), dtype=torch.float32)
+        best = logits.new_empty((*lead, alternatives), dtype=torch.int64)
+    _rl.launch(index, _rl.lib().log_probs_forward, code, m, v, logits.data_ptr(), stride, actions.data_ptr(), action_code,
+               _rl.ptr(allowed), allowed_stride, log_prob.data_ptr(), entropy.data_ptr(), normalizer.data_ptr(), alternatives,
+               _rl.ptr(best), _rl.ptr(top))
+    return Scores(log_prob, entropy, normalizer, top, best)
+
+
+def backward(grad_log_prob, grad_entropy, logits, actions, normalizer, entropy, allowed=None):
+    """The gradient (..., A) of the logits from those of log_prob and entropy (either may be None), with `forward`'s
+    normalizer and entropy."""
+    m, v, code, action_code, index = _check(logits, actions, allowed)
+    lead = logits.shape[:-1]
+    rows = []
+    for name, x in (("grad_log_prob", grad_log_prob), ("grad_entropy", grad_entropy), ("normalizer", normalizer),
+                    ("entropy", entropy)):
+        if x is None and name.startswith("grad"):
+            rows.append(None)
+            continue
+        if not isinstance(x, torch.Tensor) or x.get_device() != index or x.dtype is not torch.float32 or x.shape != lead:
+            _rl.as_floats(name, x, lead, torch.float32)
+            _rl.one_device(index, **{name: x})
+        rows.append(x.contiguous())
+    grad_log_prob, grad_entropy, normalizer, entropy = rows
+    logits, stride = _rl.as_rows(logits)
+    allowed, allowed_stride = (None, 0) if allowed is None else _rl.as_rows(allowed)
+    actions, grad = actions.contiguous(), _rl.empty_rows(logits, v, logits.dtype)
+    _rl.launch(index, _rl.lib().log_probs_backward, code, m, v, _rl.ptr(grad_log_prob), _rl.ptr(grad_entropy),
+               logits.data_ptr(), stride, actions.data_ptr(), action_code, normalizer.data_ptr(), entropy.data_ptr(),
+               _rl.ptr(allowed), allowed_stride, grad.data_ptr())
+    return grad
+
+
+class _Apply(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, actions, allowed):
+        scores = forward(logits, actions, allowed)
+        ctx.save_for_backward(logits, actions, allowed, scores.normalizer, scores.entropy)
+        return scores.log_prob, scores.entropy
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad_log_prob, grad_entropy):
+        logits, actions, allowed, normalizer, entropy = ctx.saved_tensors
+        return backward(grad_log_prob, grad_entropy, logits, actions, normalizer, entropy, allowed), None, None
+
+
+def apply(logits, actions, allowed=None):
+    """(log_prob, entropy) as differentiable operations of the logits."""
+    return _Apply.apply(logits, actions, allowed)

@@ -30,7 +30,8 @@ _DTYPES = {torch.int32: I32, torch.int64: I64, torch.uint8: U8, torch.bool: U8}
 
 # name -> argument types; every function returns int except those in _RESTYPES
 _RESTYPES = {"rlenv_es_ranks_scratch_bytes": c_int64, "rlenv_linear_attention_scratch_bytes": c_int64,
-             "rlenv_gated_ffn_scratch_bytes": c_int64}
+             "rlenv_gated_ffn_scratch_bytes": c_int64, "rlenv_rms_norm_scratch_bytes": c_int64,
+             "rlenv_int8_linear_scratch_bytes": c_int64}
 _SIGNATURES = {
     "rlenv_abi_version": [],
     "rlenv_checks_status": [c_void_p, c_int],
@@ -94,6 +95,20 @@ _SIGNATURES = {
                          c_void_p, c_double, c_double, c_double, c_double, c_double, c_void_p, c_int64, c_uint32,
                          c_void_p],
     "rlenv_adamw_moments": [c_int64, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p],
+    "rlenv_rms_norm_forward": [c_int, c_int64, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_float, c_void_p,
+                               c_void_p, c_void_p],
+    "rlenv_rms_norm_codes": [c_int, c_int64, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_float, c_int,
+                             c_void_p, c_int64, c_void_p, c_void_p, c_void_p],
+    "rlenv_rms_norm_scratch_bytes": [c_int64, c_int64],
+    "rlenv_rms_norm_backward": [c_int, c_int64, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_float,
+                                c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_int64, c_void_p],
+    "rlenv_int8_linear_scratch_bytes": [c_int64, c_int64, c_int64],
+    "rlenv_int8_linear_forward": [c_int, c_int64, c_int64, c_int64, c_void_p, c_int64, c_void_p, c_void_p, c_int64,
+                                  c_void_p, c_void_p, c_void_p, c_int64, c_void_p],
+    "rlenv_log_probs_forward": [c_int, c_int64, c_int64, c_void_p, c_int64, c_void_p, c_int, c_void_p, c_int64,
+                                c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_void_p],
+    "rlenv_log_probs_backward": [c_int, c_int64, c_int64, c_void_p, c_void_p, c_void_p, c_int64, c_void_p, c_int,
+                                 c_void_p, c_void_p, c_void_p, c_int64, c_void_p, c_void_p],
     "rlenv_reset_uniform": [c_void_p, c_int, c_int64, c_void_p, c_float, c_uint32, c_int64, c_void_p],
 }
 
@@ -458,3 +473,28 @@ def scratch(nbytes, like):
     if nbytes < 0:
         check(-1)
     return like.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
+
+
+def as_rows(x):
+    """(x, the elements between its rows) of x (..., K) with its last axis dense and its leading axes one even step
+    apart; anything else is copied."""
+    if x.is_contiguous():
+        return x, x.shape[-1]
+    step, count = None, 1  # the leading axes' step, and how many rows the axes seen so far hold
+    if x.stride(-1) == 1 or x.shape[-1] == 1:
+        for n, s in zip(reversed(x.shape[:-1]), reversed(x.stride()[:-1])):
+            if n == 1:
+                continue
+            if step is None:
+                step = s
+            elif s != step * count:
+                break
+            count *= n
+        else:
+            return x, step or 0
+    return x.contiguous(), x.shape[-1]
+
+
+def empty_rows(x, k, dtype):
+    """A dense tensor of x's leading axes with rows of k."""
+    return x.new_empty((*x.shape[:-1], k), dtype=dtype)

@@ -1,0 +1,123 @@
+"""Root-mean-square norm with the residual's addition, as sm_100a kernels:
+
+    total = x + residual,   out = total / sqrt(mean(total^2) + eps) * weight
+
+x and residual are (..., K), weight (K,), all of one type, float32 or bfloat16; sums are in 32 bits. `total` is the
+residual stream that the next layer adds to; out is formed from it before it is rounded to the tensors' type.
+
+- `forward` and `backward`, and `apply`, forward with its gradient through torch.autograd;
+- `forward8` gives out in 8-bit integers with a scale for each token, for int8_linear's products.
+
+Rows may be any even step apart (slices of wider rows, expanded ones); other strides are copied. Squares are summed
+in float32: magnitudes above 1.8e19 overflow to a norm of zeros. The reference's policies are tanh MLPs
+(es.py:156-164); there is no counterpart there.
+"""
+
+import torch
+from torch.autograd.function import once_differentiable
+
+import rlenv_lib as _rl
+
+
+def _check(first, weight, eps, **others):
+    """(rows, K, the type's code, the device's index); first is (name, tensor). What fits passes on a few
+    comparisons; what does not is looked at again for the message."""
+    name, x = first
+    if not isinstance(x, torch.Tensor) or not x.is_cuda or x.dtype not in _rl.FLOAT_DTYPES:
+        _rl.as_floats(name, x)
+    shape, dtype, index = x.shape, x.dtype, x.get_device()
+    if not shape or shape[-1] == 0:
+        raise ValueError(f"{name} must be (..., K) with K of at least 1; got shape {tuple(shape)}")
+    for other, y in others.items():
+        if y is not None and (not isinstance(y, torch.Tensor) or y.get_device() != index or y.dtype is not dtype
+                              or y.shape != shape):
+            _rl.as_floats(other, y, shape, dtype)
+            _rl.one_device(index, **{other: y})
+    k = shape[-1]
+    if weight is not None and (not isinstance(weight, torch.Tensor) or weight.get_device() != index
+                               or weight.dtype is not dtype or weight.shape != (k,)):
+        _rl.as_floats("weight", weight, (k,), dtype)
+        _rl.one_device(index, weight=weight)
+    if not eps >= 0.0:
+        raise ValueError(f"eps must not be negative; got {eps}")
+    return x.numel() // k, k, _rl.FLOAT_DTYPES[dtype], index
+
+
+def _rows(x):
+    return (None, 0) if x is None else _rl.as_rows(x)
+
+
+def forward(x, weight=None, residual=None, eps=1e-6):
+    """(out, total), both (..., K). residual None: total is x itself; weight None: ones."""
+    m, k, code, index = _check(("x", x), weight, eps, residual=residual)
+    (x, xs), (residual, rs) = _rl.as_rows(x), _rows(residual)
+    weight = None if weight is None else weight.contiguous()
+    out = _rl.empty_rows(x, k, x.dtype)
+    total = x if residual is None else torch.empty_like(out)
+    _rl.launch(index, _rl.lib().rms_norm_forward, code, m, k, x.data_ptr(), xs, _rl.ptr(residual), rs, _rl.ptr(weight),
+               eps, out.data_ptr(), 0 if residual is None else total.data_ptr())
+    return out, total
+
+
+def codes_like(x, k):
+    """Room for 8-bit rows of k as int8_linear takes them: (..., K) int8, rows on 16-byte boundaries."""
+    pitch = (k + 15) // 16 * 16
+    codes = _rl.empty_rows(x, pitch, torch.int8)
+    return codes if pitch == k else codes[..., :k]
+
+
+def forward8(x, weight=None, residual=None, eps=1e-6):
+    """(codes (..., K) int8, scale (...) float32, total): out = codes * scale, each token's scale its largest magnitude
+    over 127, rounded to the nearest. Rows of codes start on 16-byte boundaries. A token whose out is below 2^-100 is
+    zeros with scale 0; one that holds a value that is not finite is zeros with scale NaN."""
+    m, k, code, index = _check(("x", x), weight, eps, residual=residual)
+    (x, xs), (residual, rs) = _rl.as_rows(x), _rows(residual)
+    weight = None if weight is None else weight.contiguous()
+    codes, scale = codes_like(x, k), x.new_empty(x.shape[:-1], dtype=torch.float32)
+    total = x if residual is None else _rl.empty_rows(x, k, x.dtype)
+    _rl.launch(index, _rl.lib().rms_norm_codes, code, m, k, x.data_ptr(), xs, _rl.ptr(residual), rs, _rl.ptr(weight), eps,
+               1, codes.data_ptr(), (k + 15) // 16 * 16, scale.data_ptr(), 0 if residual is None else total.data_ptr())
+    return codes, scale, total
+
+
+def backward(grad_out, total, weight=None, eps=1e-6, grad_total=None):
+    """(grad, grad_weight) from grad_out and, where the total is used further, grad_total: grad (..., K) is the
+    gradient of x and of the residual alike, grad_weight (K,) or None without a weight."""
+    m, k, code, index = _check(("total", total), weight, eps, grad_out=grad_out, grad_total=grad_total)
+    lib = _rl.lib()
+    if m == 0:
+        return torch.empty_like(total), None if weight is None else torch.zeros_like(weight)
+    (g, gs), (t, ts), (s, ss) = _rl.as_rows(grad_out), _rl.as_rows(total), _rows(grad_total)
+    grad = _rl.empty_rows(t, k, t.dtype)
+    grad_weight, tmp, nbytes = None, None, 0
+    if weight is not None:
+        weight = weight.contiguous()
+        grad_weight, nbytes = torch.empty_like(weight), lib.rms_norm_scratch_bytes(m, k)
+        tmp = _rl.scratch(nbytes, t)
+    _rl.launch(index, lib.rms_norm_backward, code, m, k, g.data_ptr(), gs, t.data_ptr(), ts, _rl.ptr(weight), eps,
+               _rl.ptr(s), ss, grad.data_ptr(), _rl.ptr(grad_weight), _rl.ptr(tmp), nbytes)
+    return grad, grad_weight
+
+
+class _Apply(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, residual, eps):
+        out, total = forward(x, weight, residual, eps)
+        ctx.save_for_backward(total, weight)
+        ctx.eps, ctx.with_residual = eps, residual is not None
+        return (out, total) if ctx.with_residual else out
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad_out, grad_total=None):
+        total, weight = ctx.saved_tensors
+        grad, grad_weight = backward(grad_out, total, weight, ctx.eps, grad_total)
+        return grad, grad_weight, grad if ctx.with_residual else None, None
+
+
+def apply(x, weight=None, residual=None, eps=1e-6):
+    """`forward` as a differentiable operation of x, weight and residual: (out, total). The gradient is taken at the
+    total as it is stored."""
+    if residual is not None:
+        return _Apply.apply(x, weight, residual, eps)
+    return _Apply.apply(x, weight, None, eps), x

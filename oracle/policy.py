@@ -4,6 +4,8 @@
   summed instead (what rounding errors are measured against);
 - `attention_grad`: its gradient, by the adjoint recurrence;
 - `ffn`, `ffn_grad`: the gated feed-forward block;
+- `norm`, `norm_grad`: the root-mean-square norm; `quantise`: rows in 8-bit integers;
+- `scores`, `scores_grad`, `best`: log-probabilities of actions, entropy, alternatives;
 - `adamw`: one step of AdamW; `encode`, `decode`: the 8-bit moments in float32, bit for bit.
 """
 
@@ -78,6 +80,61 @@ def ffn_grad(dh, x, wg, wu, act):
     y, slope = activation(x @ wg, act)
     dg, du = dh * (x @ wu) * slope, dh * y
     return dg @ wg.T + du @ wu.T, x.T @ dg, x.T @ du, dg, du
+
+
+def norm(t, w, eps):
+    """t / sqrt(mean(t^2) + eps) * w over the last axis; w None: ones."""
+    out = t / np.sqrt((t * t).mean(-1, keepdims=True) + eps)
+    return out if w is None else out * w
+
+
+def norm_grad(g, t, w, eps, gt=None, absolute=False):
+    """(dt, dw) of sum(g * norm(t, w)) + sum(gt * t); with `absolute` the sums of their terms' magnitudes."""
+    if absolute:
+        g, t, w, gt = (None if x is None else abs(x) for x in (g, t, w, gt))
+    k = t.shape[-1]
+    r = 1.0 / np.sqrt((t * t).mean(-1, keepdims=True) + eps)
+    gw = g if w is None else g * w
+    along = r ** 3 * (gw * t).sum(-1, keepdims=True) / k * t
+    dt = r * gw + along if absolute else r * gw - along
+    return dt if gt is None else dt + gt, (g * t * r).reshape(-1, k).sum(0)
+
+
+def quantise(y):
+    """(whole numbers, scale) of rows: the largest magnitude is 127 steps."""
+    top = abs(y).max(-1, keepdims=True)
+    some = top >= 2.0 ** -100
+    return np.where(some, np.rint(y * 127 / np.where(some, top, 1.0)), 0.0), np.where(some, top / 127, 0.0)[..., 0]
+
+
+def scores(l, actions, allowed=None):
+    """(log_prob, entropy, normalizer, log-probabilities (..., A)) of logits l (..., A)."""
+    l = l if allowed is None else np.where(allowed, l, -np.inf)
+    with np.errstate(divide="ignore", invalid="ignore"):
+        top = l.max(-1, keepdims=True)
+        base = np.where(top == -np.inf, 0.0, top)
+        e = np.exp(l - base)
+        s = e.sum(-1, keepdims=True)
+        normalizer = base + np.log(s)
+        lp = np.where(l == -np.inf, -np.inf, l - normalizer)
+        entropy = np.where(s > 0, np.log(s) - np.where(e > 0, e * (l - base), 0.0).sum(-1, keepdims=True) / s, 0.0)
+    chosen = np.take_along_axis(lp, np.maximum(actions, 0)[..., None], -1)[..., 0]
+    return np.where(actions < 0, 0.0, chosen), entropy[..., 0], normalizer[..., 0], lp
+
+
+def scores_grad(g, h, l, actions, allowed=None):
+    """The gradient of sum(g * log_prob) + sum(h * entropy)."""
+    _, entropy, _, lp = scores(l, actions, allowed)
+    p, lp = np.exp(lp), np.where(lp == -np.inf, 0.0, lp)
+    chosen = np.arange(l.shape[-1]) == actions[..., None]
+    grad = np.where(actions < 0, 0.0, g)[..., None] * (chosen - p) - h[..., None] * p * (lp + entropy[..., None])
+    return np.where(p > 0, grad, 0.0)
+
+
+def best(l, n, allowed=None):
+    """Places (..., n) of the largest logits, ties to the lower place."""
+    l = l if allowed is None else np.where(allowed, l, -np.inf)
+    return np.argsort(-l, -1, kind="stable")[..., :n]
 
 
 def adamw(p, g, m, v, step, lr, betas, eps, weight_decay):

@@ -1,0 +1,597 @@
+"""The norm, the 8-bit products and the scores of actions on the GPU against the oracle in 64 bits.
+
+Tolerances are bounds on rounding, element by element. A float32 sum whose longest chain of additions is n is within
+(n + the roundings of a term) 2^-24 of the same sum of magnitudes; a team of threads adds up to 128 terms a thread and
+then in a tree, longer rows K / 512 a thread. rsqrtf errs by 2^-22, expf's fast form by (2 + 1.2 |x|) 2^-23, a product or
+quotient by 2^-24. Results of type t are rounded by at most finfo(t).eps / 2 of their value."""
+
+import numpy as np
+import pytest
+import torch
+
+import rlenv_lib
+from oracle import policy
+
+pytestmark = pytest.mark.gpu
+
+TYPES = {"f32": torch.float32, "bf16": torch.bfloat16}
+HALF = 2.0 ** -24
+
+
+def to64(x):
+    return x.detach().double().cpu().numpy()
+
+
+def half(dtype):
+    return torch.finfo(TYPES[dtype]).eps / 2
+
+
+def close(got, want, tol, what):
+    got = to64(got)
+    assert got.shape == want.shape, what
+    bad = ~np.isfinite(want)
+    assert np.array_equal(got[bad], want[bad], equal_nan=True), f"{what}: values that are not finite"
+    off = np.abs(np.where(bad, 0.0, got) - np.where(bad, 0.0, want)) - np.where(bad, 0.0, tol)
+    assert (off <= 0).all(), f"{what}: {(~(off <= 0)).sum()} of {off.size} outside, worst by {np.nanmax(off):.3g} at " \
+                             f"{np.unravel_index(np.nanargmax(off), off.shape)}"
+
+
+def chain(k):
+    return min(k, 128) + k / 512 + 12
+
+
+def normal(cuda, *shape, seed=0, scale=1.0, dtype="f32"):
+    g = torch.Generator(device=cuda).manual_seed(seed)
+    return (torch.randn(shape, generator=g, device=cuda) * scale).to(TYPES[dtype])
+
+
+# ---- the norm ------------------------------------------------------------------------------------------
+
+NORM_SIZES = [(1, 1), (3, 7), (1, 8), (9, 96), (18, 97), (5, 256), (2, 257), (33, 512), (7, 513), (300, 40), (4, 1000),
+              (3, 1024), (2, 1032), (2, 2047), (3, 4096), (2, 4097), (1, 8200), (2, 16384), (1, 16383), (2, 20001),
+              (1, 40000), (700, 128)]
+
+
+def norm_tol(k, want, dtype):
+    # t is exact to half a step, its square's sum to chain(k) halves, r to half of that and rsqrtf's, two products
+    return ((chain(k) + 4) / 2 + 10) * HALF * abs(want) + half(dtype) * abs(want) + 1e-37
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("m,k", NORM_SIZES)
+def test_norm_forward(cuda, m, k, dtype):
+    import rms_norm
+
+    x, y = normal(cuda, m, k, dtype=dtype), normal(cuda, m, k, seed=1, scale=3.0, dtype=dtype)
+    w = (1 + 0.2 * normal(cuda, k, seed=2)).to(TYPES[dtype])
+    for weight, residual in ((w, y), (None, None), (w, None), (None, y)):
+        out, total = rms_norm.forward(x, weight, residual, 1e-5)
+        t = to64(x) if residual is None else to64(x) + to64(residual)
+        assert out.dtype == total.dtype == x.dtype and out.is_contiguous()
+        close(total, t, (HALF + half(dtype)) * abs(t), "total")
+        assert residual is not None or total is x
+        want = policy.norm(t, None if weight is None else to64(weight), 1e-5)
+        close(out, want, norm_tol(k, want, dtype), "out")
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("m,k", NORM_SIZES)
+def test_norm_in_8_bits(cuda, m, k, dtype):
+    import int8_linear
+    import rms_norm
+
+    x, y = normal(cuda, m, k, dtype=dtype), normal(cuda, m, k, seed=1, scale=3.0, dtype=dtype)
+    w = (1 + 0.2 * normal(cuda, k, seed=2)).to(TYPES[dtype])
+    codes, scale, total = rms_norm.forward8(x, w, y, 1e-5)
+    t = to64(x) + to64(y)
+    want = policy.norm(t, to64(w), 1e-5)
+    close(total, t, (HALF + half(dtype)) * abs(t), "total")
+    off = norm_tol(k, want, "f32")  # of the values before their codes
+    top = abs(want).max(-1, keepdims=True)
+    rel = off.max(-1, keepdims=True) / np.where(top > 0, top, 1) + 3 * HALF
+    close(scale, top[:, 0] / 127, rel[:, 0] * top[:, 0] / 127, "scale")
+    # a code is the nearest whole number to the value over the scale, each a little off
+    close(codes, want / np.where(top > 0, top / 127, 1.0), 0.5 + 127 * 2 * rel, "codes")
+    assert codes.dtype == torch.int8 and scale.dtype == torch.float32
+    assert codes.data_ptr() % 16 == 0 and (m == 1 or codes.stride(0) % 16 == 0)
+    # without a norm: the values themselves, whose scale and codes are known but for ties' neighbours
+    codes, scale = int8_linear.quantise(x)
+    want = to64(x)
+    top = abs(want).max(-1, keepdims=True)
+    close(scale, top[:, 0] / 127, HALF * top[:, 0] / 127, "scale of rows")
+    close(codes, want * 127 / np.where(top > 0, top, 1.0), 0.5 + 127 * 3 * HALF, "codes of rows")
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("m,k", NORM_SIZES + [(5000, 72), (4999, 33)])
+def test_norm_backward(cuda, m, k, dtype):
+    import rms_norm
+
+    t, g = normal(cuda, m, k, scale=3.0, dtype=dtype), normal(cuda, m, k, seed=1, dtype=dtype)
+    s, w = normal(cuda, m, k, seed=2, dtype=dtype), (1 + 0.2 * normal(cuda, k, seed=3)).to(TYPES[dtype])
+    for weight, stream in ((w, s), (None, None), (w, None), (None, s)):
+        grad, grad_weight = rms_norm.backward(g, t, weight, 1e-5, stream)
+        args = (to64(g), to64(t), None if weight is None else to64(weight), 1e-5, None if stream is None else to64(stream))
+        want, want_w = policy.norm_grad(*args)
+        mag, mag_w = policy.norm_grad(*args, absolute=True)
+        n = 2.5 * chain(k) + 24  # the two sums, r to the third power, some products
+        close(grad, want, n * HALF * mag + half(dtype) * abs(want), "grad")
+        assert (grad_weight is None) == (weight is None)
+        if weight is not None:
+            rows = min(m, m / 296 + 60)  # a team's rows, a block's teams, the blocks' sums
+            close(grad_weight, want_w, (rows + chain(k) / 2 + 16) * HALF * mag_w + half(dtype) * abs(want_w), "grad_weight")
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_norm_takes_rows_of_any_layout(cuda, dtype):
+    """Slices, expanded rows, strides that are copied and bases off every boundary."""
+    import int8_linear
+    import rms_norm
+
+    wide = normal(cuda, 6, 5, 136, dtype=dtype)
+    views = [wide[..., :128], wide[..., 8:], wide[..., 1:129], wide[:, 2, 3:100], wide[0, :1, :128].expand(7, 128),
+             wide.transpose(0, 1)[..., :64], wide[..., ::2], wide[0, 0, 5:69], wide[:1, :1, :64]]
+    for x in views:
+        k, y = x.shape[-1], torch.flip(x, (0,))
+        w = normal(cuda, k, seed=5, dtype=dtype)
+        t = to64(x) + to64(y)
+        want = policy.norm(t, to64(w), 1e-6)
+        out, total = rms_norm.forward(x, w, y)
+        close(out, want, norm_tol(k, want, dtype), "out")
+        close(total, t, (HALF + half(dtype)) * abs(t), "total")
+        codes, scale, total = rms_norm.forward8(x, w, y)
+        close(total, t, (HALF + half(dtype)) * abs(t), "total of codes")
+        close(codes * scale[..., None], want, 0.501 * abs(want).max(-1, keepdims=True) / 127, "codes")
+        dense = x.clone(memory_format=torch.contiguous_format)
+        assert all(torch.equal(a, b) for a, b in zip(int8_linear.quantise(x), int8_linear.quantise(dense)))
+        grad, grad_weight = rms_norm.backward(x, x, w, 1e-6, x)
+        args = (to64(x), to64(x), to64(w), 1e-6, to64(x))
+        (want, want_w), (mag, mag_w) = policy.norm_grad(*args), policy.norm_grad(*args, absolute=True)
+        n = 2.5 * chain(k) + 24
+        close(grad, want, n * HALF * mag + half(dtype) * abs(want), "grad")
+        close(grad_weight, want_w, (60 + n) * HALF * mag_w + half(dtype) * abs(want_w), "grad_weight")
+
+
+def test_norm_of_rows_that_are_zero_or_not_finite(cuda):
+    """A row that holds an infinity or a NaN changes no other row, and says so; a row of zeros is zeros."""
+    import int8_linear
+    import rms_norm
+
+    for k in (40, 97, 2000, 40000):
+        x = normal(cuda, 6, k)
+        want, want8 = rms_norm.forward(x)[0], rms_norm.forward8(x)
+        bad = x.clone()
+        bad[1, k // 2], bad[2, 0], bad[3, k - 1], bad[4] = float("inf"), float("nan"), -float("inf"), 0.0
+        out, _ = rms_norm.forward(bad)
+        assert torch.equal(out[0], want[0]) and torch.equal(out[5], want[5]) and not out[4].any()
+        assert torch.isnan(out[2]).all() and torch.isnan(out[1, k // 2]) and torch.isnan(out[3, k - 1])
+        codes, scale, _ = rms_norm.forward8(bad)
+        for i in (0, 5):
+            assert torch.equal(codes[i], want8[0][i]) and scale[i] == want8[1][i]
+        assert torch.isnan(scale[1:4]).all() and scale[4] == 0 and not codes[1:5].any()
+        bad[5] *= 2.0 ** -110  # too small for codes of their own
+        codes, scale = int8_linear.quantise(bad)
+        assert torch.isnan(scale[1:4]).all() and not scale[4:].any() and not codes[1:].any() and scale[0] > 0
+
+
+def test_codes_leave_the_bytes_past_a_row(cuda):
+    x = normal(cuda, 5, 21)
+    room, scale = torch.full((5, 32), 99, dtype=torch.int8, device=cuda), torch.empty(5, device=cuda)
+    rlenv_lib.launch(0, rlenv_lib.lib().rms_norm_codes, rlenv_lib.F32, 5, 21, x.data_ptr(), 21, 0, 0, 0, 0.0, 0,
+                     room.data_ptr(), 32, scale.data_ptr(), 0)
+    assert (room[:, 21:] == 99).all() and (room[:, :21].abs().amax(1) == 127).all()
+
+
+def test_norm_of_no_rows(cuda):
+    import int8_linear
+    import rms_norm
+
+    x, w = torch.zeros((0, 3, 8), device=cuda), torch.ones(8, device=cuda)
+    out, total = rms_norm.forward(x, w, x)
+    codes, scale, _ = rms_norm.forward8(x, w)
+    grad, grad_weight = rms_norm.backward(x, x, w)
+    assert out.shape == total.shape == grad.shape == codes.shape == (0, 3, 8) and scale.shape == (0, 3)
+    assert grad_weight.shape == (8,) and not grad_weight.any()
+    weight = int8_linear.quantise_weight(torch.ones((8, 5), device=cuda))
+    assert int8_linear.forward(codes, scale, weight).shape == (0, 3, 5)
+
+
+@pytest.mark.parametrize("with_residual", [True, False])
+def test_norm_through_autograd(cuda, with_residual):
+    import rms_norm
+
+    x, y, g, gt = (normal(cuda, 5, 3, 40, seed=i) for i in range(4))
+    w = 1 + 0.2 * normal(cuda, 40, seed=9)
+    leaves = [v.clone().requires_grad_() for v in ((x, w, y) if with_residual else (x, w))]
+    out, total = rms_norm.apply(leaves[0], leaves[1], leaves[2] if with_residual else None, 1e-5)
+    grads = torch.autograd.grad((out * g).sum() + (total * gt).sum(), leaves)
+    t = to64(x) + to64(y) if with_residual else to64(x)
+    args = [v.reshape(15, 40) if v.size > 40 else v for v in (to64(g), t, to64(w))] + [1e-5, to64(gt).reshape(15, 40)]
+    want, want_w = policy.norm_grad(*args)
+    mag, mag_w = policy.norm_grad(*args, absolute=True)
+    n = 2.5 * chain(40) + 28
+    close(grads[0].reshape(15, 40), want, n * HALF * mag, "x")
+    close(grads[1], want_w, n * HALF * mag_w, "weight")
+    if with_residual:
+        assert torch.equal(grads[0], grads[2])
+    only = torch.autograd.grad(rms_norm.apply(*leaves)[1].sum() if with_residual else rms_norm.apply(*leaves)[0].sum(),
+                               leaves[0])[0]
+    assert torch.isfinite(only).all()
+    with pytest.raises(RuntimeError):
+        again = torch.autograd.grad(rms_norm.apply(*leaves)[0].square().sum(), leaves[0], create_graph=True)[0]
+        torch.autograd.grad(again.sum(), leaves[0])
+
+
+# ---- products of 8-bit integers ----------------------------------------------------------------------------
+
+def codes(cuda, rows, cols, seed):
+    import rms_norm
+
+    g = torch.Generator(device=cuda).manual_seed(seed)
+    room = rms_norm.codes_like(torch.empty((rows, cols), device=cuda), cols)
+    return room.copy_(torch.randint(-128, 128, (rows, cols), generator=g, device=cuda))
+
+
+def product_want(a, sa, w, sw):
+    # whole numbers below 2^53 / 128^2 terms: exact in 64 bits
+    return (to64(a) @ to64(w).T) * to64(sa)[..., None] * to64(sw)
+
+
+PRODUCT_SIZES = [(1, 1, 1), (1, 15, 3), (1, 16, 8), (2, 17, 9), (1, 1024, 4096), (3, 1000, 100), (7, 33, 257), (8, 64, 64),
+                 (9, 4097, 31), (16, 256, 512), (17, 640, 96), (33, 100, 130), (64, 2048, 100), (100, 97, 2720),
+                 (128, 128, 128), (129, 129, 129), (256, 512, 256), (257, 1000, 300), (300, 1000, 2720), (511, 96, 1040),
+                 (1000, 64, 17), (2050, 200, 264)]
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("m,k,f", PRODUCT_SIZES)
+def test_int8_product(cuda, m, k, f, dtype):
+    import int8_linear
+
+    a, w = codes(cuda, m, k, 0), codes(cuda, f, k, 1)
+    sa, sw = normal(cuda, m, seed=2).abs() + 0.1, normal(cuda, f, seed=3).abs() + 0.1
+    out = int8_linear.forward(a, sa, int8_linear.Weight(w, sw), TYPES[dtype])
+    want = product_want(a, sa, w, sw)
+    # the sum exact, its conversion and two products
+    close(out, want, 3.1 * HALF * abs(want) + half(dtype) * abs(want), "out")
+    assert out.dtype == TYPES[dtype] and out.shape == (m, f)
+    assert torch.equal(out, int8_linear.forward(a, sa, int8_linear.Weight(w, sw), TYPES[dtype]))
+
+
+@pytest.mark.parametrize("m", [1, 8, 40, 300])
+def test_int8_sums_reach_the_ends_of_32_bits(cuda, m):
+    import int8_linear
+
+    k, f = int8_linear.MOST_TERMS, 5
+    pitch = k + 1
+    low, high = (torch.full((r, pitch), v, dtype=torch.int8, device=cuda)[:, :k] for r, v in ((m, -128), (f, 127)))
+    one = torch.ones(max(m, f), device=cuda)
+    assert (int8_linear.forward(low, one[:m], int8_linear.Weight(high, one[:f]), torch.float32) == -128 * 127 * k).all()
+    low_w = int8_linear.Weight(torch.full((f, pitch), -128, dtype=torch.int8, device=cuda)[:, :k], one[:f])
+    assert (int8_linear.forward(low, one[:m], low_w, torch.float32) == float(128 * 128 * k)).all()
+
+
+@pytest.mark.parametrize("m", [1, 5, 200])
+def test_int8_product_of_other_layouts(cuda, m):
+    """Rows off the boundaries, expanded and transposed ones, leading axes: the results of their copies."""
+    import int8_linear
+
+    g = torch.Generator(device=cuda).manual_seed(0)
+    a = torch.randint(-128, 128, (m, 3, 50), generator=g, device=cuda).to(torch.int8)
+    w = torch.randint(-128, 128, (40, 70), generator=g, device=cuda).to(torch.int8)
+    sa, sw = normal(cuda, m, 6, seed=1)[:, ::2], normal(cuda, 40, seed=2)
+    for x, y in ((a, w[:, :50]), (a, w[:, 7:57]), (a[:, :1].expand(m, 3, 50), w.t()[:50].t()), (a[..., 1:34], w[:, 16:49]),
+                 (a.flip(0), w[:, :50].contiguous())):
+        out = int8_linear.forward(x, sa, int8_linear.Weight(y, sw), torch.float32)
+        want = product_want(x, sa, y, sw)
+        close(out, want, 3.1 * HALF * abs(want), "out")
+
+
+def test_a_layer_in_8_bits(cuda):
+    """Norm, codes and product as a policy that acts in 8 bits runs them, against the same from the definitions: the
+    codes' rounding is the largest error, half a step of each term."""
+    import int8_linear
+    import rms_norm
+
+    for m, k, f in ((1, 64, 192), (33, 100, 70), (500, 1000, 2720)):
+        x, y, w = normal(cuda, m, k), normal(cuda, m, k, seed=1), normal(cuda, k, f, seed=2, scale=k ** -0.5)
+        weight = int8_linear.quantise_weight(w)
+        assert weight.codes.shape == (f, k) and weight.scale.shape == (f,)
+        w64 = to64(w)
+        close(weight.codes * weight.scale[:, None], w64.T, (0.5 + 1e-4) * abs(w64).max(0)[:, None] / 127, "weight")
+        got = int8_linear.forward(*rms_norm.forward8(x, None, y)[:2], weight, torch.float32)
+        v = policy.norm(to64(x) + to64(y), None, 1e-6)
+        step, wstep = abs(v).max(1, keepdims=True) / 127, abs(w64).max(0) / 127
+        # |v w - v' w'| <= |v - v'| |w| + |v'| |w - w'|
+        tol = 0.5 * step * abs(w64).sum(0) + 0.5 * (abs(v) + 0.5 * step).sum(1, keepdims=True) * wstep
+        close(got, v @ w64, 1.001 * tol, "layer")
+        assert torch.equal(int8_linear.product(x, weight), int8_linear.forward(*int8_linear.quantise(x), weight, x.dtype))
+
+
+def test_int8_refusals(cuda):
+    import int8_linear
+
+    a, w, one = codes(cuda, 4, 20, 0), codes(cuda, 6, 20, 1), torch.ones(6, device=cuda)
+    fine = int8_linear.Weight(w, one)
+    for args in ((a.float(), one[:4], fine), (a, one[:3], fine), (a[:, :19], one[:4], fine), (a, one[:4].double(), fine),
+                 (a, one[:4], int8_linear.Weight(w, one[:5])), (a, one[:4], int8_linear.Weight(w.float(), one)),
+                 (a, one[:4], fine, torch.float16), (a, one[:4].cpu(), fine), (a[:, :0], one[:4], int8_linear.Weight(w[:, :0], one))):
+        with pytest.raises(ValueError):
+            int8_linear.forward(*args)
+    with pytest.raises(ValueError):
+        int8_linear.quantise_weight(torch.ones(3, device=cuda))
+    with pytest.raises(ValueError, match="K must be"):
+        big = torch.zeros((1, 131072), dtype=torch.int8, device=cuda)
+        int8_linear.forward(big, one[:1], int8_linear.Weight(big, one[:1]))
+
+
+# ---- scores -------------------------------------------------------------------------------------------------
+
+def score_inputs(cuda, m, v, dtype, beside=0, masked=False, seed=0):
+    l = normal(cuda, m, v + beside, seed=seed, scale=2.0, dtype=dtype)[:, :v]
+    g = torch.Generator(device=cuda).manual_seed(seed + 1)
+    allowed = torch.rand((m, v), generator=g, device=cuda) < 0.6 if masked else None
+    actions = torch.randint(0, v, (m,), generator=g, device=cuda)
+    if masked:
+        allowed[torch.arange(m, device=cuda), actions] = True
+        if m > 2:
+            allowed[1] = False
+    return l, actions, allowed
+
+
+def score_bounds(l, allowed, v):
+    """Of (log_prob's and the normalizer's, the entropy's) errors, but for log_prob's last subtraction."""
+    e64 = np.where(allowed, l, -np.inf) if allowed is not None else l
+    with np.errstate(all="ignore"):
+        _, h, z, lp = policy.scores(l, np.zeros(l.shape[0], np.int64), allowed)
+        top = e64.max(-1, keepdims=True)
+        p, d = np.exp(lp), np.where(e64 > -np.inf, e64 - np.where(top > -np.inf, top, 0), 0)
+        one, two = (p * -d).sum(-1), (p * d * d).sum(-1)  # means of |d| and d^2
+        n = chain(v)
+        sums = (n + 6) * 2 ** -23 + (2.4 * one) * 2 ** -23       # of log S
+        z_off = sums + 2 ** -23 * (abs(z) + abs(np.log(v)))
+        h_off = sums * (1 + one) + ((n + 8) * one + 2.4 * two) * 2 ** -23 + 2 ** -22 * (one + np.log(v) + 1)
+    return np.where(np.isfinite(z), z_off, 0), np.where(np.isfinite(z), h_off, 0)
+
+
+def check_scores(got, l, actions, allowed, top):
+    l64, a = to64(l), actions.cpu().numpy().astype(np.int64)
+    al = None if allowed is None else allowed.cpu().numpy() != 0
+    lp, h, z, every = policy.scores(l64, a, al)
+    z_off, h_off = score_bounds(l64, al, l64.shape[1])
+    close(got.normalizer, z, z_off, "normalizer")
+    close(got.entropy, h, h_off, "entropy")
+    last = HALF * abs(np.where(np.isfinite(lp), lp, 0)) + 2 ** -23
+    close(got.log_prob, lp, z_off + last, "log_prob")
+    if top:
+        best = policy.best(l64, top, al)
+        assert got.top_actions.dtype == torch.int64
+        assert np.array_equal(got.top_actions.cpu().numpy(), best), "top_actions"
+        want = np.take_along_axis(every, best, -1)
+        close(got.top_log_probs, want, z_off[:, None] + HALF * abs(np.where(np.isfinite(want), want, 0)) + 2 ** -23, "top_log_probs")
+    else:
+        assert got.top_actions is None and got.top_log_probs is None
+
+
+SCORE_SIZES = [(1, 1), (5, 2), (300, 3), (7, 8), (5, 9), (4, 16), (9, 17), (6, 33), (5, 64), (3, 65), (4, 255), (3, 256),
+               (9, 257), (5, 300), (3, 513), (4, 1000), (9, 1025), (3, 2047), (2, 2049), (3, 5000), (2, 8193), (1, 9001),
+               (2, 32768), (1, 50021), (400, 4100), (1, 131071)]
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("m,v", SCORE_SIZES)
+def test_scores(cuda, m, v, dtype):
+    import log_probs
+
+    for beside, masked, top in ((0, False, min(v, 8)), (1, True, min(v, 32)), (0, True, 0), (3, False, 1)):
+        l, actions, allowed = score_inputs(cuda, m, v, dtype, beside, masked, seed=beside)
+        check_scores(log_probs.forward(l, actions, allowed, top), l, actions, allowed, top)
+
+
+@pytest.mark.parametrize("m,v,dtype", [(1, 300_001, "bf16"), (2, 150_001, "f32"), (200, 40_000, "f32"), (700, 70_000, "bf16")])
+def test_scores_of_long_rows(cuda, m, v, dtype):
+    """Rows that registers do not hold, alone and with their clusters over all of the GPU."""
+    import log_probs
+
+    l, actions, allowed = score_inputs(cuda, m, v, dtype, masked=m < 10)
+    check_scores(log_probs.forward(l, actions, allowed, 20), l, actions, allowed, 20)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("v", [5, 40, 200, 700, 1500, 6000, 20_000, 60_000, 140_000])
+def test_alternatives_of_equal_logits(cuda, v, dtype):
+    """Rows of one value, of two, of steps up and down, of both zeros, and the largest all in one thread's reach: ties go
+    to the lower action however many there are."""
+    import log_probs
+
+    top = min(v, 32)
+    l = torch.zeros((9, v), device=cuda)
+    l[1] = torch.arange(v, device=cuda) % 2
+    l[2] = torch.arange(v, device=cuda) // 100
+    l[3] = -l[2]
+    l[4, ::2] = -0.0
+    l[5, v // 2:] = 3.0
+    l[6, ::512 * 8] = 5.0
+    l[7, -1] = 1.0
+    l[8] = -torch.inf
+    l[8, v // 3] = -4.0
+    l = l.to(TYPES[dtype])
+    actions = torch.zeros(9, dtype=torch.int32, device=cuda)
+    check_scores(log_probs.forward(l, actions, None, top), l, actions, None, top)
+    allowed = torch.ones((9, v), dtype=torch.uint8, device=cuda) * 3
+    allowed[:, 1::3] = 0
+    check_scores(log_probs.forward(l, actions, allowed, top), l, actions, allowed, top)
+
+
+@pytest.mark.parametrize("v", [2, 30, 100, 400, 1200, 3000, 20_000, 70_000])
+def test_scores_where_rows_are_odd(cuda, v):
+    """Padding, actions outside, rows that allow nothing, logits that are not finite in and out of masked places: each
+    row as documented and no other changed."""
+    import log_probs
+
+    l, actions, _ = score_inputs(cuda, 12, v, "f32")
+    clean = log_probs.forward(l, actions, None, 2)
+    allowed = torch.ones((12, v), dtype=torch.bool, device=cuda)
+    bad, a = l.clone(), actions.clone()
+    a[1], a[2] = -1, v
+    allowed[3] = False
+    bad[4, v // 2] = torch.nan
+    bad[5, 0] = torch.inf
+    bad[6, v - 1], allowed[6, v - 1], a[6] = torch.nan, False, 0
+    bad[7, v - 1], allowed[7, v - 1], a[7] = torch.inf, False, v - 1
+    bad[8, v - 1], a[8] = -torch.inf, v - 1
+    bad[9] = torch.finfo(torch.float32).min
+    got = log_probs.forward(bad, a, allowed, 2)
+    for i in (0, 10, 11):
+        assert all(x[i].equal(y[i]) for x, y in zip(got, clean))
+    assert got.log_prob[1] == 0 and torch.isnan(got.log_prob[2])
+    assert got.entropy[1] == clean.entropy[1] and got.entropy[2] == clean.entropy[2]
+    assert got.normalizer[3] == -torch.inf and got.log_prob[3] == -torch.inf and got.entropy[3] == 0
+    assert got.top_actions[3].tolist() == [0, 1] and (got.top_log_probs[3] == -torch.inf).all()
+    for i in (4, 5):
+        assert all(torch.isnan(x[i]) for x in (got.log_prob, got.entropy, got.normalizer))
+    assert got.top_actions[4, 0] == v // 2 and got.top_actions[5, 0] == 0
+    rest = l[6:8].clone()
+    rest[:, v - 1] = -torch.inf
+    check_scores(log_probs.Scores(*(x[6:9] for x in got)), torch.cat([rest, bad[8:9]]), a[6:9], None, 2)
+    want = -np.log(v)
+    assert abs(got.log_prob[9].item() - want) <= 2.0 ** 104 and abs(got.entropy[9].item() + want) < 1e-4
+    g, h = normal(cuda, 12, seed=5), normal(cuda, 12, seed=6)
+    grad = log_probs.backward(g, h, bad, a, got.normalizer, got.entropy, allowed)
+    ref = log_probs.backward(g, h, l, actions, clean.normalizer, clean.entropy)
+    for i in (0, 10, 11):
+        assert torch.equal(grad[i], ref[i])
+    assert torch.equal(grad[1], log_probs.backward(None, h, l, actions, clean.normalizer, clean.entropy)[1])
+    assert torch.isnan(grad[2]).all() and not grad[3].any()
+    assert torch.isnan(grad[4]).any() and torch.isnan(grad[5]).any()
+    assert not grad[6:9, v - 1].any() and torch.isfinite(grad[6:9]).all()
+
+
+def grad_tol(g, h, l, actions, allowed, dtype):
+    lp, entropy, z, every = policy.scores(l, actions, allowed)
+    z_off, h_off = score_bounds(l, allowed, l.shape[1])
+    with np.errstate(all="ignore"):
+        some = every > -np.inf
+        p, lp = np.where(some, np.exp(every), 0), np.where(some, every, 0)
+        lp_off = z_off[:, None] + HALF * abs(lp) + 2 ** -23
+        rel = lp_off + (2 + 1.2 * abs(lp)) * 2 ** -23  # of p
+        far = abs(lp) > 80  # e^-87 is below float32's normal numbers
+    want = policy.scores_grad(g, h, l, actions, allowed)
+    inner = abs(lp + entropy[:, None])
+    tol = abs(g)[:, None] * (p * rel + HALF * (p + (p > 0.1)) + 2 * HALF * abs(1 - p) * (p > 0.5)) \
+        + abs(h)[:, None] * p * (inner * (rel + 4 * HALF) + lp_off + h_off[:, None]) + 4 * HALF * abs(want) \
+        + (abs(g) + 90 * abs(h))[:, None] * (far * 2.0 ** -110 + 2.0 ** -125)
+    chosen = np.arange(l.shape[1]) == actions[:, None]
+    return want, tol + chosen * abs(g)[:, None] * 2 * HALF + half(dtype) * abs(want)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("m,v", SCORE_SIZES)
+def test_scores_gradient(cuda, m, v, dtype):
+    import log_probs
+
+    for beside, masked in ((0, False), (1, True), (0, True), (3, False)):
+        l, actions, allowed = score_inputs(cuda, m, v, dtype, beside, masked, seed=7 + beside)
+        if m > 3:
+            actions[3] = -1
+        s = log_probs.forward(l, actions, allowed)
+        g, h = normal(cuda, m, seed=5), normal(cuda, m, seed=6)
+        a, al = actions.cpu().numpy(), None if allowed is None else allowed.cpu().numpy()
+        for gg, hh in ((g, h), (None, h), (g, None), (None, None)):
+            grad = log_probs.backward(gg, hh, l, actions, s.normalizer, s.entropy, allowed)
+            zero = np.zeros(m)
+            want, tol = grad_tol(zero if gg is None else to64(gg), zero if hh is None else to64(hh), to64(l), a, al, dtype)
+            close(grad, want, tol, "grad")
+            assert grad.dtype == l.dtype and grad.is_contiguous()
+
+
+@pytest.mark.parametrize("kind", [torch.int64, torch.int32, torch.uint8])
+def test_scores_through_autograd(cuda, kind):
+    """The loss of an actor: log_prob and entropy, their gradient against the oracle's; leading axes, a slice."""
+    import log_probs
+
+    l = normal(cuda, 6, 5, 10, scale=2.0).requires_grad_()
+    actions = torch.randint(0, 9, (6, 5), device=cuda).to(kind)
+    allowed = torch.rand((6, 1, 9), device=cuda) < 0.8
+    allowed[..., 0] = True
+    allowed = allowed.expand(6, 5, 9)
+    g = normal(cuda, 6, 5, seed=3)
+    lp, entropy = log_probs.apply(l[..., :9], actions, allowed)
+    chosen = allowed.gather(-1, actions.long()[..., None])[..., 0]
+    loss = (g * torch.where(chosen, lp, 0.0)).sum() + 0.3 * entropy.sum()
+    grad, = torch.autograd.grad(loss, l)
+    assert not grad[..., 9].any()
+    g64 = np.where(chosen.cpu().numpy(), to64(g), 0.0).reshape(30)
+    want, tol = grad_tol(g64, np.full(30, 0.3), to64(l)[..., :9].reshape(30, 9), actions.long().cpu().numpy().reshape(30),
+                         allowed.cpu().numpy().reshape(30, 9), "f32")
+    close(grad[..., :9].reshape(30, 9), want, tol, "grad")
+
+
+def test_scores_of_no_rows_and_refusals(cuda):
+    import log_probs
+
+    l, a = torch.zeros((0, 4, 7), device=cuda), torch.zeros((0, 4), dtype=torch.int64, device=cuda)
+    s = log_probs.forward(l, a, None, 3)
+    assert s.log_prob.shape == (0, 4) and s.top_actions.shape == (0, 4, 3)
+    assert log_probs.backward(s.log_prob, None, l, a, s.normalizer, s.entropy).shape == l.shape
+    l, a = torch.zeros((3, 7), device=cuda), torch.zeros(3, dtype=torch.int64, device=cuda)
+    for args in ((l, a.float()), (l, a[:2]), (l.double(), a), (l, a, torch.ones((3, 6), dtype=torch.bool, device=cuda)),
+                 (l, a, l), (l, a, None, 8), (l, a, None, -1), (l[:, :0], a), (l, a.cpu()), (l, None), (l.half(), a),
+                 (torch.zeros((3, 99), device=cuda), a, None, 33)):
+        with pytest.raises(ValueError):
+            log_probs.forward(*args)
+    s = log_probs.forward(l, a)
+    for args in ((s.log_prob.double(), None, l, a, s.normalizer, s.entropy), (None, None, l, a, None, s.entropy),
+                 (None, None, l, a, s.normalizer[:2], s.entropy), (s.log_prob.cpu(), None, l, a, s.normalizer, s.entropy)):
+        with pytest.raises(ValueError):
+            log_probs.backward(*args)
+
+
+# ---- streams and graphs ---------------------------------------------------------------------------------------
+
+def test_operators_in_a_captured_graph_and_on_other_streams(cuda):
+    """Everything once eagerly, then on a side stream, then captured and replayed on new inputs, two graphs' replays
+    interleaved: the same bits."""
+    import int8_linear
+    import log_probs
+    import rms_norm
+
+    def inputs(seed):
+        return [normal(cuda, 300, 96, seed=seed), normal(cuda, 300, 96, seed=seed + 1), normal(cuda, 300, 700, seed=seed + 2)]
+
+    w, weight = 1 + 0.1 * normal(cuda, 96, seed=50), int8_linear.quantise_weight(normal(cuda, 96, 300, seed=51))
+    actions = torch.arange(300, device=cuda)
+
+    def everything(x, y, l):
+        out, total = rms_norm.forward(x, w, y)
+        c, s, _ = rms_norm.forward8(x, w, y)
+        got = log_probs.forward(l, actions, None, 4)
+        return [out, total, c, s, *rms_norm.backward(x, total, w, 1e-6, y), int8_linear.forward(c, s, weight),
+                int8_linear.forward(c[:3], s[:3], weight), *got,
+                log_probs.backward(got.log_prob, got.entropy, l, actions, got.normalizer, got.entropy)]
+
+    first, second = inputs(0), inputs(10)
+    want = [everything(*first), everything(*second)]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        other = everything(*first)
+    torch.cuda.current_stream().wait_stream(side)
+    assert all(torch.equal(a, b) for a, b in zip(other, want[0]))
+    graphs, outs, rooms = [], [], []
+    for _ in range(2):
+        room = [x.clone() for x in first]
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs.append(everything(*room))
+        graphs.append(graph)
+        rooms.append(room)
+    for order in ((0, 1), (1, 0)):
+        for which in (0, 1):
+            for to, x in zip(rooms[which], (first, second)[order[which]]):
+                to.copy_(x)
+        graphs[0].replay()
+        graphs[1].replay()
+        torch.cuda.synchronize()
+        for which in (0, 1):
+            assert all(torch.equal(a, b) for a, b in zip(outs[which], want[order[which]]))
