@@ -469,12 +469,16 @@ RLENV_API int rlenv_rms_norm_backward(int dtype, int64_t m, int64_t k, const voi
  * the sums exact in 32-bit integers (1 <= k <= 131071). a (m, k) and w (f, k): signed bytes, rows
  * a_pitch and w_pitch bytes apart (multiples of 16, bases on 16-byte boundaries; bytes past k are
  * not looked at). scratch: device memory of at least rlenv_int8_linear_scratch_bytes bytes,
- * 256-byte aligned (NULL when that is 0). */
+ * 256-byte aligned (NULL when that is 0). More than a few rows go over the tensor cores: a launch takes
+ * tensor memory of its SMs and frees it before it ends. */
 RLENV_API int64_t rlenv_int8_linear_scratch_bytes(int64_t m, int64_t k, int64_t f);
 
 RLENV_API int rlenv_int8_linear_forward(int dtype, int64_t m, int64_t k, int64_t f, const int8_t* a, int64_t a_pitch,
                                         const float* a_scale, const int8_t* w, int64_t w_pitch, const float* w_scale,
                                         void* out, void* scratch, int64_t scratch_bytes, void* stream);
+
+/* As rlenv_gated_ffn_status, for the waits of these products' kernels. */
+RLENV_API int rlenv_int8_linear_status(unsigned int* gave_up, int clear);
 
 /* Scores of actions: for each of m rows of v logits l (dtype RLENV_F32 or RLENV_BF16, `stride` values
  * between rows, last axis dense), over the actions that `allowed` admits (one byte each, rows

@@ -181,10 +181,71 @@ RLENV_D void tmem_ready(uint32_t (&r)[32]) {
 RLENV_D uint32_t operand(uint32_t at, bool mn_major, uint32_t block) {
   return (at & 0x3ffff) >> 4 | (mn_major ? block >> 4 : 1) << 16;
 }
+// The same with signed 8-bit integers, K-major, sums in 32-bit ones.
+RLENV_D void multiply_int8(uint32_t d, uint32_t a, uint32_t b, uint32_t kind, bool accumulate) {
+  asm volatile(
+      "{\n .reg .pred p;\n .reg .b64 a, b;\n setp.ne.b32 p, %4, 0;\n mov.b64 a, {%1, %5};\n mov.b64 b, {%2, %5};\n"
+      " tcgen05.mma.cta_group::2.kind::i8 [%0], a, b, %3, p;\n}" ::"r"(d),
+      "r"(a), "r"(b), "r"(kind), "r"(uint32_t(accumulate)), "n"(kOperandHigh)
+      : "memory");
+}
+constexpr uint32_t product_kind_int8(int m, int n) {
+  return 2u << 4 | 1u << 7 | 1u << 10 | uint32_t(n >> 3) << 17 | uint32_t(m >> 4) << 24;
+}
 // bfloat16 x bfloat16 -> float32, M x N.
 constexpr uint32_t product_kind(int m, int n, bool a_mn, bool b_mn) {
   return 1u << 4 | 1u << 7 | 1u << 10 | uint32_t(a_mn) << 15 | uint32_t(b_mn) << 16 | uint32_t(n >> 3) << 17 |
          uint32_t(m >> 4) << 24;
+}
+
+// ---- the end of a pair whose wait ran out --------------------------------------------------
+// What a block has done by its end, for the other one of the pair.
+struct Ending {
+  int filled;          // ring buffers that its copying warp has filled
+  int released, runs;  // the first block's: releases of ring buffers and sums that its issuing warp has committed
+  int gave_up;         // whether a wait ran out
+};
+RLENV_D void tell(const Ending* e, uint32_t rank) {  // the same place in the other block's shared memory
+  store_in_block(in_block(shared_at(&e->filled), rank), e->filled);
+  store_in_block(in_block(shared_at(&e->released), rank), e->released);
+  store_in_block(in_block(shared_at(&e->runs), rank), e->runs);
+  store_in_block(in_block(shared_at(&e->gave_up), rank), e->gave_up);
+}
+
+// After a wait that ran out: what is under way lands before the pair may end and tensor memory is freed, each with
+// a wait of its own, up to one that runs out too. Products behind the last commit get one. A buffer's bytes all
+// count at the first block: where one block has filled it and the other has not, the other's are struck off, or its
+// own alone expected (the blocks are a round of the ring apart at most). Then every barrier's last phase, by the
+// number of its rounds.
+template <int kStages>
+__device__ __noinline__ void drain(const Ending* endings, int rank, int warp, uint32_t full, uint32_t bytes, uint32_t empty,
+                                   uint32_t summed, uint32_t drained) {
+  int late = 0;  // a flag of its own: not cut short by the wait that ran out before
+  const auto last_of = [&](uint32_t bar, int turns, int slot, int slots) {
+    const int rounds = (turns - slot + slots - 1) / slots;
+    if (turns > slot) barrier_wait_warp(bar + 8 * slot, (rounds - 1) & 1, &late);
+  };
+  if (warp == 1) {
+    if (rank == 0 && elect()) commit(drained);
+    __syncwarp();
+    barrier_wait_warp(drained, 0, &late);
+  } else if (warp == 0) {
+    if (rank == 0) {
+      const int own = endings[0].filled, other = endings[1].filled;
+      if (elect()) {
+        for (int i = own; i < other; ++i) barrier_expect(full + 8 * (i % kStages), bytes);
+        for (int i = other; i < own; ++i) barrier_strike(full + 8 * (i % kStages), bytes);
+      }
+      __syncwarp();
+      for (int i = 0; i < kStages; ++i) last_of(full, own > other ? own : other, i, kStages);
+    }
+    for (int i = 0; i < kStages; ++i) last_of(empty, endings[0].released, i, kStages);
+    for (int i = 0; i < 2; ++i) last_of(summed, endings[0].runs, i, 2);
+  }
+  __syncwarp();
+  fence_before();
+  cluster_sync();
+  fence_after();
 }
 
 // ---- host: tensor maps -----------------------------------------------------------------------------
@@ -205,15 +266,17 @@ inline EncodeTiled encode_tiled() {  // the driver's function, looked up once
 }
 
 // A (slices, rows, cols) bfloat16 array with `pitch` elements between rows, copied in boxes of 64
-// columns and box_rows rows; what lies past cols or rows reads as zero. 0 or a cudaError_t.
+// columns and box_rows rows; `bytes`: of bytes, 128 columns a box. What lies past cols or rows reads as zero.
+// 0 or a cudaError_t.
 inline int tile_map(CUtensorMap* map, const void* base, int64_t cols, int64_t rows, int64_t slices, int64_t pitch,
-                    int box_rows) {
+                    int box_rows, bool bytes = false) {
   const EncodeTiled encode = encode_tiled();
   if (!encode) return int(cudaErrorNotSupported);
   const cuuint64_t dims[3] = {cuuint64_t(cols), cuuint64_t(rows), cuuint64_t(slices)};
-  const cuuint64_t strides[2] = {cuuint64_t(pitch) * 2, cuuint64_t(pitch) * 2 * cuuint64_t(rows)};
-  const cuuint32_t box[3] = {64, cuuint32_t(box_rows), 1}, steps[3] = {1, 1, 1};
-  const CUresult rc = encode(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(base), dims, strides, box,
+  const cuuint64_t row = cuuint64_t(pitch) * (bytes ? 1 : 2);
+  const cuuint64_t strides[2] = {row, row * cuuint64_t(rows)};
+  const cuuint32_t box[3] = {bytes ? 128u : 64u, cuuint32_t(box_rows), 1}, steps[3] = {1, 1, 1};
+  const CUresult rc = encode(map, bytes ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(base), dims, strides, box,
                              steps, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
                              CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   return rc == CUDA_SUCCESS ? 0 : int(cudaErrorInvalidValue);

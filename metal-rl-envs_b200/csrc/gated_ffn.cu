@@ -485,55 +485,6 @@ RLENV_D void finish(const Product& p, const Work& w, int64_t r0, int64_t c, cons
   }
 }
 
-// What a block has done by its end, for the other one of the pair.
-struct Ending {
-  int filled;          // ring buffers that its copying warp has filled
-  int released, runs;  // the first block's: releases of ring buffers and sums that its issuing warp has committed
-  int gave_up;         // whether a wait ran out
-};
-RLENV_D void tell(const Ending* e, uint32_t rank) {  // the same place in the other block's shared memory
-  bw::store_in_block(bw::in_block(bw::shared_at(&e->filled), rank), e->filled);
-  bw::store_in_block(bw::in_block(bw::shared_at(&e->released), rank), e->released);
-  bw::store_in_block(bw::in_block(bw::shared_at(&e->runs), rank), e->runs);
-  bw::store_in_block(bw::in_block(bw::shared_at(&e->gave_up), rank), e->gave_up);
-}
-
-// After a wait that ran out: what is under way lands before the pair may end and tensor memory is freed, each with
-// a wait of its own, up to one that runs out too. Products behind the last commit get one. A buffer's bytes all
-// count at the first block: where one block has filled it and the other has not, the other's are struck off, or its
-// own alone expected (the blocks are a round of the ring apart at most). Then every barrier's last phase, by the
-// number of its rounds.
-template <int kStages>
-__device__ __noinline__ void drain(const Ending* endings, int rank, int warp, uint32_t full, uint32_t bytes, uint32_t empty,
-                                   uint32_t summed, uint32_t drained) {
-  int late = 0;  // a flag of its own: not cut short by the wait that ran out before
-  const auto last_of = [&](uint32_t bar, int turns, int slot, int slots) {
-    const int rounds = (turns - slot + slots - 1) / slots;
-    if (turns > slot) bw::barrier_wait_warp(bar + 8 * slot, (rounds - 1) & 1, &late);
-  };
-  if (warp == 1) {
-    if (rank == 0 && bw::elect()) bw::commit(drained);
-    __syncwarp();
-    bw::barrier_wait_warp(drained, 0, &late);
-  } else if (warp == 0) {
-    if (rank == 0) {
-      const int own = endings[0].filled, other = endings[1].filled;
-      if (bw::elect()) {
-        for (int i = own; i < other; ++i) bw::barrier_expect(full + 8 * (i % kStages), bytes);
-        for (int i = other; i < own; ++i) bw::barrier_strike(full + 8 * (i % kStages), bytes);
-      }
-      __syncwarp();
-      for (int i = 0; i < kStages; ++i) last_of(full, own > other ? own : other, i, kStages);
-    }
-    for (int i = 0; i < kStages; ++i) last_of(empty, endings[0].released, i, kStages);
-    for (int i = 0; i < 2; ++i) last_of(summed, endings[0].runs, i, 2);
-  }
-  __syncwarp();
-  bw::fence_before();
-  bw::cluster_sync();
-  bw::fence_after();
-}
-
 template <typename T, int kOp>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Tile<T, kOp>::kThreads, 1)
 product_kernel(const __grid_constant__ Product p, int items) {
@@ -544,7 +495,7 @@ product_kernel(const __grid_constant__ Product p, int items) {
   __shared__ __align__(8) uint64_t bars[2 * C::kStages + 5];
   __shared__ uint32_t tmem_slot;
   __shared__ int dead_flag;
-  __shared__ Ending endings[2];  // of the pair's first block, and of its second
+  __shared__ bw::Ending endings[2];  // of the pair's first block, and of its second
   volatile int* const dead = &dead_flag;
   const uint32_t ring = (bw::shared_at(raw) + 1023) & ~1023u;
   const uint32_t full = bw::shared_at(bars), empty = full + 8 * C::kStages;
@@ -555,7 +506,7 @@ product_kernel(const __grid_constant__ Product p, int items) {
     for (int i = 0; i < C::kStages; ++i) bw::barrier_init(full + 8 * i, 1), bw::barrier_init(empty + 8 * i, 1);
     for (int i = 0; i < 2; ++i) bw::barrier_init(summed + 8 * i, 1), bw::barrier_init(taken + 8 * i, 2 * C::kEpilogue);
     bw::barrier_init(drained, 1);
-    dead_flag = 0, endings[rank] = Ending{};
+    dead_flag = 0, endings[rank] = bw::Ending{};
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (warp == 2) bw::tmem_alloc<kTmemColumns>(bw::shared_at(&tmem_slot));
@@ -776,12 +727,12 @@ product_kernel(const __grid_constant__ Product p, int items) {
   if (threadIdx.x == 0) {
     endings[rank].gave_up = dead_flag;
     if (dead_flag) bw::note_given_up();
-    tell(&endings[rank], rank ^ 1);
+    bw::tell(&endings[rank], rank ^ 1);
   }
   bw::cluster_sync();
   bw::fence_after();
   if (endings[0].gave_up || endings[1].gave_up)
-    drain<C::kStages>(endings, rank, warp, full, C::kRingBytes, empty, summed, drained);
+    bw::drain<C::kStages>(endings, rank, warp, full, C::kRingBytes, empty, summed, drained);
   if (warp == 2) bw::tmem_free<kTmemColumns>(tmem);
 }
 

@@ -8,6 +8,7 @@ int8 with a scale for each of its F channels (`quantise_weight`, once). Sums are
 acting. The reference's policies are float32 MLPs (es.py:156-164); there is no counterpart there.
 """
 
+import ctypes
 from dataclasses import dataclass
 
 import torch
@@ -92,3 +93,12 @@ def forward(codes, scale, weight, dtype=torch.bfloat16):
 def product(x, weight, dtype=None):
     """`forward` of x (..., K) in 8 bits, (..., F) of dtype (None: x's)."""
     return forward(*quantise(x), weight, dtype or x.dtype)
+
+
+def gave_up(device=None, clear=True):
+    """As gated_ffn.gave_up, for this module's kernels: how many thread blocks on `device` ended with a wait that ran
+    out. Zero unless something is wrong with the machine. Waits for the device."""
+    count = ctypes.c_uint(0)
+    with torch.cuda.device(device):
+        _rl.check(_rl.lib().int8_linear_status(ctypes.byref(count), int(clear)))
+    return count.value

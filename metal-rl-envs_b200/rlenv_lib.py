@@ -105,6 +105,7 @@ _SIGNATURES = {
     "rlenv_int8_linear_scratch_bytes": [c_int64, c_int64, c_int64],
     "rlenv_int8_linear_forward": [c_int, c_int64, c_int64, c_int64, c_void_p, c_int64, c_void_p, c_void_p, c_int64,
                                   c_void_p, c_void_p, c_void_p, c_int64, c_void_p],
+    "rlenv_int8_linear_status": [c_void_p, c_int],
     "rlenv_log_probs_forward": [c_int, c_int64, c_int64, c_void_p, c_int64, c_void_p, c_int, c_void_p, c_int64,
                                 c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_void_p],
     "rlenv_log_probs_backward": [c_int, c_int64, c_int64, c_void_p, c_void_p, c_void_p, c_int64, c_void_p, c_int,
