@@ -501,7 +501,7 @@ RLENV_API int rlenv_log_probs_forward(int dtype, int64_t m, int64_t v, const voi
  * NULL for zero), the forward pass's normalizer and entropy:
  *     grad_j = grad_log_prob ([j = action] - p_j) - grad_entropy p_j (log p_j + entropy),
  * zero where an action is not allowed or its logit is -infinity, and in rows that allow nothing. Rows
- * with a negative action have no first term; with one of v or above they are NaN elsewhere. */
+ * with a negative action have no first term; with one of v or above they are NaN. */
 RLENV_API int rlenv_log_probs_backward(int dtype, int64_t m, int64_t v, const float* grad_log_prob,
                                        const float* grad_entropy, const void* logits, int64_t stride,
                                        const void* actions, int action_dtype, const float* normalizer,

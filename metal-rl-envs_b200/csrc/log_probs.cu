@@ -52,6 +52,39 @@ RLENV_D float value_at(const __nv_bfloat16* from) {
   return __uint_as_float(uint32_t(__ldg(reinterpret_cast<const unsigned short*>(from))) << 16);
 }
 
+// Two float32 values side by side: sm_100 adds and multiplies them in one instruction.
+RLENV_D uint64_t pair_of(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+RLENV_D float2 values_of(uint64_t p) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(p));
+  return r;
+}
+RLENV_D uint64_t add_pairs(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+RLENV_D uint64_t multiply_pairs(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+RLENV_D uint64_t multiply_add_pairs(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+RLENV_D float exp2_fast(float x) {  // within 2 ulp, 0 where float32's normal numbers end
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+constexpr float kLog2E = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+
 // Logits are ordered by value, ties by the lower place: as one whole number, larger first. 0 stands below all, NaN
 // above.
 RLENV_D uint32_t order_of(float x) {
@@ -175,13 +208,46 @@ struct Grid {
   RLENV_D int64_t place(int64_t i) const { return i * kValues - skip; }
 };
 
-// The words of 32 bits of a vector, and its values.
+// A vector is four words of 32 bits, each one float32 or two bfloat16 logits.
 template <typename T>
 RLENV_D float word_value(const uint32_t (&w)[4], int j) {
   if constexpr (sizeof(T) == 4)
     return __uint_as_float(w[j]);
   else
     return __uint_as_float(j % 2 ? w[j / 2] & 0xffff0000u : w[j / 2] << 16);
+}
+template <typename T>
+RLENV_D uint64_t word_pair(const uint32_t (&w)[4], int i) {  // values 2 i and 2 i + 1
+  return pair_of(word_value<T>(w, 2 * i), word_value<T>(w, 2 * i + 1));
+}
+template <typename T>
+RLENV_D uint32_t word_of(float x) {  // x in each place
+  if constexpr (sizeof(T) == 4) return __float_as_uint(x);
+  const __nv_bfloat162 p = __float2bfloat162_rn(x);
+  return *reinterpret_cast<const uint32_t*>(&p);
+}
+RLENV_D __nv_bfloat162 as_bf162(uint32_t w) { return *reinterpret_cast<const __nv_bfloat162*>(&w); }
+template <typename T>
+RLENV_D uint32_t larger_words(uint32_t a, uint32_t b) {  // place by place, or NaN
+  if constexpr (sizeof(T) == 4) return __float_as_uint(larger(__uint_as_float(a), __uint_as_float(b)));
+  const __nv_bfloat162 p = __hmax2_nan(as_bf162(a), as_bf162(b));
+  return *reinterpret_cast<const uint32_t*>(&p);
+}
+template <typename T>
+RLENV_D float largest_of(uint32_t w) {
+  if constexpr (sizeof(T) == 4) return __uint_as_float(w);
+  return larger(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+}
+template <typename T>
+RLENV_D bool any_reaches(uint32_t w, uint32_t least) {  // a place that is not below least's
+  if constexpr (sizeof(T) == 4) return !(__uint_as_float(w) < __uint_as_float(least));
+  return __hgeu2_mask(as_bf162(w), as_bf162(least)) != 0;
+}
+// log2 e^(l - base) of two logits. What lies further below than kFar counts as that: it adds nothing, and -infinity times
+// nothing would be NaN.
+RLENV_D uint64_t powers_of(uint64_t l, uint64_t minus_base) {
+  const float2 d = values_of(add_pairs(l, minus_base));
+  return multiply_pairs(pair_of(larger(d.x, kFar), larger(d.y, kFar)), pair_of(kLog2E, kLog2E));
 }
 template <typename T>
 RLENV_D constexpr uint32_t empty_word() {  // -infinity
@@ -246,17 +312,16 @@ RLENV_D void load_vector(const Grid<T>& grid, const uint8_t* allowed, int64_t i,
   }
 }
 
-// A team of kThreads threads, a warp or a block.
+// A team of kThreads threads, a warp or a block, in 32 groups of neighbours.
 template <int kThreads>
 struct Team {
   static constexpr int kWarps = kThreads / 32, kBlock = kThreads == 32 ? 256 : kThreads, kRows = kBlock / kThreads;
-  static constexpr int kRoom = kThreads >= 512 ? 1024 : kThreads == 32 ? 96 : 512;  // alternatives looked at
+  static constexpr int kRoom = kThreads == 32 ? 128 : 4 * kThreads;  // alternatives looked at
   struct Shared {
-    float sums[2 * kWarps];
-    uint32_t orders[kThreads];
+    float groups[32], sums[2 * kWarps];
     uint64_t keys[kRoom], top[kMostTop];
-    uint32_t count, threshold;
-    Sums of_block;
+    uint32_t count;
+    float of_block[3];
   };
   static RLENV_D void sync() {
     if constexpr (kWarps == 1)
@@ -264,35 +329,7 @@ struct Team {
     else
       __syncthreads();
   }
-  static RLENV_D float most(float x, float* room) {
-#pragma unroll
-    for (int d = 16; d > 0; d /= 2) x = larger(x, __shfl_xor_sync(0xffffffffu, x, d));
-    if constexpr (kWarps > 1) {
-      const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-      if (lane == 0) room[warp] = x;
-      __syncthreads();
-      x = room[lane % kWarps];
-#pragma unroll
-      for (int d = kWarps / 2; d > 0; d /= 2) x = larger(x, __shfl_xor_sync(0xffffffffu, x, d));
-      __syncthreads();
-    }
-    return x;
-  }
-  // The sums of a and b, known to all.
-  static RLENV_D void sum(float& a, float& b, float* room) {
-#pragma unroll
-    for (int d = 16; d > 0; d /= 2) a += __shfl_xor_sync(0xffffffffu, a, d), b += __shfl_xor_sync(0xffffffffu, b, d);
-    if constexpr (kWarps > 1) {
-      const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-      if (lane == 0) room[warp] = a, room[kWarps + warp] = b;
-      __syncthreads();
-      a = room[lane % kWarps], b = room[kWarps + lane % kWarps];
-#pragma unroll
-      for (int d = kWarps / 2; d > 0; d /= 2)
-        a += __shfl_xor_sync(0xffffffffu, a, d), b += __shfl_xor_sync(0xffffffffu, b, d);
-      __syncthreads();
-    }
-  }
+  // The team's largest key; room holds kWarps of them.
   static RLENV_D uint64_t most(uint64_t x, uint64_t* room) {
 #pragma unroll
     for (int d = 16; d > 0; d /= 2) {
@@ -300,10 +337,9 @@ struct Team {
       x = y > x ? y : x;
     }
     if constexpr (kWarps > 1) {
-      const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-      if (lane == 0) room[warp] = x;
+      if (threadIdx.x % 32 == 0) room[threadIdx.x / 32] = x;
       __syncthreads();
-      x = room[lane % kWarps];
+      x = room[threadIdx.x % kWarps];
 #pragma unroll
       for (int d = kWarps / 2; d > 0; d /= 2) {
         const uint64_t y = __shfl_xor_sync(0xffffffffu, x, d);
@@ -313,64 +349,51 @@ struct Team {
     }
     return x;
   }
-  // The top-th largest of the threads' orders, 0 standing for none, known to all. Warp 0 takes the largest out, one
-  // after the other.
-  static RLENV_D uint32_t threshold(Shared& sh, uint32_t order, int top) {
-    const int lane = threadIdx.x % 32;
-    uint32_t result = 0;
-    if constexpr (kWarps > 1) {
-      sh.orders[threadIdx.x] = order;
-      __syncthreads();
-    }
-    if (kWarps == 1 || threadIdx.x < 32) {
-      uint32_t mine[kWarps];
-#pragma unroll
-      for (int i = 0; i < kWarps; ++i) mine[i] = kWarps == 1 ? order : sh.orders[lane + 32 * i];
-      for (int r = 0; r < top; ++r) {
-        uint32_t best = 0;
-#pragma unroll
-        for (int i = 0; i < kWarps; ++i) best = max(best, mine[i]);
-        result = __reduce_max_sync(0xffffffffu, best);
-        if (lane == __ffs(__ballot_sync(0xffffffffu, best == result)) - 1) {
-          bool out = false;
-#pragma unroll
-          for (int i = 0; i < kWarps; ++i) {
-            const bool it = !out && mine[i] == result;
-            mine[i] = it ? 0 : mine[i];
-            out |= it;
-          }
-        }
-      }
-      if (lane == 0) sh.threshold = result, sh.count = 0;
-    }
-    sync();
-    return sh.threshold;
-  }
 };
 
+// The n-th largest of a warp's values, known to all lanes: sorted by exchanges with lanes at growing distances
+// (Batcher 1968).
+RLENV_D float nth_largest(float x, int n) {
+  const int lane = threadIdx.x % 32;
+  uint32_t v = order_of(x);
+#pragma unroll
+  for (int size = 2; size <= 32; size *= 2)
+#pragma unroll
+    for (int d = size / 2; d > 0; d /= 2) {
+      const uint32_t other = __shfl_xor_sync(0xffffffffu, v, d);
+      v = ((lane & d) == 0) == ((lane & size) == 0) ? max(v, other) : min(v, other);
+    }
+  return value_of(__shfl_sync(0xffffffffu, v, n - 1));
+}
+
 // kThreads threads with room for kVectors vectors each; longer parts of a row go tile by tile, and are read again for
-// their alternatives. A cluster's blocks have a part of the row each.
+// their sums. A cluster's blocks have a part of the row each.
+//
+// The alternatives: the n-th largest of the 32 groups' largest logits has n logits at least that are not below it, and as
+// a rule few more. These are collected and their ranks counted; where they are too many (a row of equal logits, or all
+// large ones in one group) they are found one after the other.
 template <typename T, int kThreads, int kVectors>
 __global__ void __launch_bounds__(Team<kThreads>::kBlock) scores_kernel(const __grid_constant__ Scores p) {
   using G = Team<kThreads>;
-  constexpr int kValues = Grid<T>::kValues;
+  constexpr int kValues = Grid<T>::kValues, kTile = kThreads * kVectors;
   __shared__ typename G::Shared shared[G::kRows];
   auto& sh = shared[threadIdx.x / kThreads];
   cg::cluster_group cluster = cg::this_cluster();
   const int blocks = kThreads == 32 ? 1 : int(cluster.num_blocks()), rank = blocks > 1 ? int(cluster.block_rank()) : 0;
-  const int at = threadIdx.x % kThreads;
+  const int at = threadIdx.x % kThreads, lane = threadIdx.x % 32;
   const int64_t row = kThreads == 32 ? int64_t(blockIdx.x) * G::kRows + threadIdx.x / 32 : blockIdx.x / blocks;
   if (row >= p.m) return;  // a warp
   const Grid<T> grid(static_cast<const T*>(p.logits) + row * p.stride, p.v);
   const uint8_t* const allowed = p.allowed ? p.allowed + row * p.allowed_stride : nullptr;
-  const int64_t part = (grid.vectors() + blocks - 1) / blocks, begin = rank * part,
-                end = begin + part < grid.vectors() ? begin + part : grid.vectors();
+  const int vectors = int(grid.vectors()), part = (vectors + blocks - 1) / blocks, begin = min(rank * part, vectors),
+            end = min(begin + part, vectors);
+  const bool one_tile = end - begin <= kTile;
 
   uint32_t w[kVectors][4];
-  const auto load_tile = [&](int64_t from) {
+  const auto load_tile = [&](int from) {
 #pragma unroll
     for (int r = 0; r < kVectors; ++r) {
-      const int64_t i = from + r * kThreads + at;
+      const int i = from + r * kThreads + at;
       if (i < end) {
         load_vector(grid, allowed, i, w[r]);
       } else {
@@ -379,115 +402,152 @@ __global__ void __launch_bounds__(Team<kThreads>::kBlock) scores_kernel(const __
       }
     }
   };
-  Sums sums{-infinity(), 0.0f, 0.0f};
-  for (int64_t from = begin; from < end; from += kThreads * kVectors) {
-    load_tile(from);
-    float most = -infinity();
-    if constexpr (sizeof(T) == 4) {
-#pragma unroll
-      for (int r = 0; r < kVectors; ++r)
-#pragma unroll
-        for (int k = 0; k < 4; ++k) most = larger(most, __uint_as_float(w[r][k]));
-    } else {
-      __nv_bfloat162 pairs = *reinterpret_cast<const __nv_bfloat162*>(&w[0][0]);
-#pragma unroll
-      for (int r = 0; r < kVectors; ++r)
-#pragma unroll
-        for (int k = 0; k < 4; ++k) pairs = __hmax2_nan(pairs, *reinterpret_cast<const __nv_bfloat162*>(&w[r][k]));
-      most = larger(__low2float(pairs), __high2float(pairs));
-    }
-    if (from > begin) {
-      most = larger(most, sums.m);
-      sums = moved(sums, most);
-    }
-    sums.m = most;
-    const float base = base_of(most);
+  // f(r) for the tile's vectors of this thread; the same ones are left out by all threads.
+  const auto each_vector = [&](int from, auto&& f) {
 #pragma unroll
     for (int r = 0; r < kVectors; ++r)
-#pragma unroll
-      for (int j = 0; j < kValues; ++j) add(sums, word_value<T>(w[r], j), base);
+      if (from + r * kThreads < end) f(r);
+  };
+  uint32_t most = empty_word<T>();
+  for (int from = begin; from < end; from += kTile) {
+    load_tile(from);
+    each_vector(from, [&](int r) {
+      most = larger_words<T>(most, larger_words<T>(larger_words<T>(w[r][0], w[r][1]), larger_words<T>(w[r][2], w[r][3])));
+    });
   }
-  const float own_most = sums.m;
-  sums = moved(sums, G::most(sums.m, sh.sums));
-  G::sum(sums.s, sums.w, sh.sums);
+  const float own_most = largest_of<T>(most);
+  float group = own_most;
+  if constexpr (kThreads > 32) {
+#pragma unroll
+    for (int d = (kThreads / 32) / 2; d > 0; d /= 2) group = larger(group, __shfl_xor_sync(0xffffffffu, group, d));
+    if (at % (kThreads / 32) == 0) sh.groups[at / (kThreads / 32)] = group;
+  }
+  if (at == 0) sh.count = 0;
+  G::sync();
+  if constexpr (kThreads > 32) group = sh.groups[lane];
+  Sums sums{group, 0.0f, 0.0f};
+#pragma unroll
+  for (int d = 16; d > 0; d /= 2) sums.m = larger(sums.m, __shfl_xor_sync(0xffffffffu, sums.m, d));
+  const float base = base_of(sums.m);
+  const float least = p.top > 0 ? nth_largest(group, p.top) : 0.0f;
+
+  const uint32_t reach = word_of<T>(least);
+  const uint64_t minus_base = pair_of(-base, -base);
+  const bool mine = p.top > 0 && !(own_most < least);
+  uint64_t s2 = 0, w2 = 0;
+  for (int from = begin; from < end; from += kTile) {
+    if (!one_tile) load_tile(from);
+    if (mine)
+      each_vector(from, [&](int r) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          if (any_reaches<T>(w[r][k], reach)) {
+#pragma unroll
+            for (int h = 0; h < kValues / 4; ++h) {
+              const int j = k * (kValues / 4) + h;
+              const float x = word_value<T>(w[r], j);
+              const int64_t place = grid.place(from + r * kThreads + at) + j;
+              if (x < least || place < 0 || place >= p.v || from + r * kThreads + at >= end) continue;
+              const uint32_t slot = atomicAdd(&sh.count, 1u);
+              if (slot < G::kRoom) sh.keys[slot] = key_of(x, uint32_t(place));
+            }
+          }
+      });
+    each_vector(from, [&](int r) {
+#pragma unroll
+      for (int i = 0; i < kValues / 2; ++i) {
+        const uint64_t y = powers_of(word_pair<T>(w[r], i), minus_base);
+        const float2 of = values_of(y);
+        const uint64_t e = pair_of(exp2_fast(of.x), exp2_fast(of.y));
+        s2 = add_pairs(s2, e), w2 = multiply_add_pairs(e, y, w2);
+      }
+    });
+  }
+  const float2 s_own = values_of(s2), w_own = values_of(w2);
+  sums.s = s_own.x + s_own.y, sums.w = (w_own.x + w_own.y) * kLn2;
+#pragma unroll
+  for (int d = 16; d > 0; d /= 2) {
+    sums.s += __shfl_xor_sync(0xffffffffu, sums.s, d);
+    sums.w += __shfl_xor_sync(0xffffffffu, sums.w, d);
+  }
+  if (kThreads > 32 && lane == 0) sh.sums[at / 32] = sums.s, sh.sums[G::kWarps + at / 32] = sums.w;
+  G::sync();
+  if constexpr (kThreads > 32) {
+    sums.s = sh.sums[lane % G::kWarps], sums.w = sh.sums[G::kWarps + lane % G::kWarps];
+#pragma unroll
+    for (int d = G::kWarps / 2; d > 0; d /= 2) {
+      sums.s += __shfl_xor_sync(0xffffffffu, sums.s, d);
+      sums.w += __shfl_xor_sync(0xffffffffu, sums.w, d);
+    }
+  }
+  const bool alone = kThreads == 32 || blocks == 1;
+  if (alone && at == 0) write_scores<T>(p, row, sums);
 
   if (p.top > 0) {
-    // What is at least as large as the top-th largest of the threads' own largest ones holds the alternatives: no
-    // more than top - 1 threads' logits and those equal to it. Their ranks are counted.
-    const bool some = begin + at < end;
-    const uint32_t least = G::threshold(sh, some ? order_of(own_most) : 0u, p.top);
-    const auto each = [&](auto&& f) {  // f(key) for this thread's logits
-      for (int64_t from = begin; from < end; from += kThreads * kVectors) {
-        if (end - begin > kThreads * kVectors) load_tile(from);
-#pragma unroll
-        for (int r = 0; r < kVectors; ++r) {
-          const int64_t i = from + r * kThreads + at;
-          if (i >= end) continue;
-#pragma unroll
-          for (int j = 0; j < kValues; ++j) {
-            const int64_t place = grid.place(i) + j;
-            if (place >= 0 && place < p.v) f(key_of(word_value<T>(w[r], j), uint32_t(place)));
-          }
-        }
-      }
+    const float normalizer = normalizer_of(sums);  // of the row, where the block has all of it
+    const auto found = [&](int r, uint64_t key) {
+      if (alone)
+        write_top(p, row, r, key, normalizer);
+      else
+        sh.top[r] = key;
     };
-    if (some && order_of(own_most) >= least)
-      each([&](uint64_t key) {
-        if (uint32_t(key >> 32) >= least) {
-          const uint32_t slot = atomicAdd(&sh.count, 1u);
-          if (slot < G::kRoom) sh.keys[slot] = key;
-        }
-      });
-    if (at < kMostTop) sh.top[at] = 0;
-    G::sync();
     const int count = int(sh.count);
     if (count <= G::kRoom) {
+      if (!alone && at >= count && at < p.top) sh.top[at] = 0;  // a part of fewer logits
       for (int i = at; i < count; i += kThreads) {
         const uint64_t key = sh.keys[i];
         int above = 0;
         for (int k = 0; k < count; ++k) above += sh.keys[k] > key;
-        if (above < p.top) sh.top[above] = key;
+        if (above < p.top) found(above, key);
       }
-    } else {  // many equal ones, or all in few threads' parts: one after the other
+    } else {
       uint64_t last = ~uint64_t(0);
-      for (int r = 0; r < p.top; ++r) {
+      G::sync();  // the keys' room is free
+      for (int n = 0; n < p.top; ++n) {
         uint64_t best = 0;
-        each([&](uint64_t key) {
-          if (key < last && key > best) best = key;
-        });
+        for (int from = begin; from < end; from += kTile) {
+          if (!one_tile) load_tile(from);
+#pragma unroll
+          for (int r = 0; r < kVectors; ++r) {
+            const int i = from + r * kThreads + at;
+            if (i >= end) continue;
+#pragma unroll
+            for (int j = 0; j < kValues; ++j) {
+              const int64_t place = grid.place(i) + j;
+              const uint64_t key = key_of(word_value<T>(w[r], j), uint32_t(place));
+              if (place >= 0 && place < p.v && key < last && key > best) best = key;
+            }
+          }
+        }
         last = G::most(best, sh.keys);
-        if (at == 0) sh.top[r] = last;
+        if (at == 0) found(n, last);
       }
     }
-    G::sync();
   }
+  if (alone) return;
 
-  if (kThreads == 32 || blocks == 1) {
-    if (at == 0) write_scores<T>(p, row, sums);
-    if (at < p.top) write_top(p, row, at, sh.top[at], normalizer_of(sums));
-    return;
-  }
   // The cluster's first block joins the parts: their sums in order, and their alternatives by their ranks.
-  if (at == 0) sh.of_block = sums;
+  if (at == 0) sh.of_block[0] = sums.m, sh.of_block[1] = sums.s, sh.of_block[2] = sums.w;
   cluster.sync();
   if (rank == 0) {
-    Sums all = sums;
-    for (int b = 1; b < blocks; ++b) all.m = larger(all.m, cluster.map_shared_rank(&sh.of_block, b)->m);
-    Sums joined{all.m, 0.0f, 0.0f};
+    Sums all{sums.m, 0.0f, 0.0f};
+    for (int b = 1; b < blocks; ++b) all.m = larger(all.m, cluster.map_shared_rank(sh.of_block, b)[0]);
     for (int b = 0; b < blocks; ++b) {
-      const Sums one = moved(*cluster.map_shared_rank(&sh.of_block, b), all.m);
-      joined.s += one.s, joined.w += one.w;
+      const float* const of = cluster.map_shared_rank(sh.of_block, b);
+      const Sums one = moved(Sums{of[0], of[1], of[2]}, all.m);
+      all.s += one.s, all.w += one.w;
     }
-    if (at == 0) write_scores<T>(p, row, joined);
+    if (at == 0) write_scores<T>(p, row, all);
     if (p.top > 0) {
       const int count = blocks * p.top;
-      for (int i = at; i < count; i += kThreads) sh.keys[i] = cluster.map_shared_rank(&sh.top[i % p.top], i / p.top)[0];
+      for (int i = at; i < count; i += kThreads) sh.keys[i] = cluster.map_shared_rank(sh.top, i / p.top)[i % p.top];
       __syncthreads();
+      const float normalizer = normalizer_of(all);
       for (int i = at; i < count; i += kThreads) {
         const uint64_t key = sh.keys[i];
         int above = 0;
         for (int k = 0; k < count; ++k) above += sh.keys[k] > key;
-        if (key && above < p.top) write_top(p, row, above, key, normalizer_of(joined));
+        if (key && above < p.top) write_top(p, row, above, key, normalizer);
       }
     }
   }
@@ -550,43 +610,65 @@ __global__ void __launch_bounds__(256) few_scores_grad_kernel(const __grid_const
   }
 }
 
-// A warp a run of kRun vectors of a row of the gradient, on its 16-byte boundaries.
+// A warp a run of kRun vectors of a row of the gradient, on its 16-byte boundaries. With y = log2 p the gradient of what
+// was not chosen is - p (g + h entropy + h ln 2 y): two values an instruction but for the power.
 constexpr int kRun = 128;
 template <typename T>
 __global__ void __launch_bounds__(256) scores_grad_kernel(const __grid_constant__ ScoresGrad p, int64_t runs) {
-  constexpr int kValues = Grid<T>::kValues;
+  constexpr int kValues = Grid<T>::kValues, kVectors = kRun / 32;
   const int64_t warp = int64_t(blockIdx.x) * 8 + threadIdx.x / 32, row = warp / runs;
   if (row >= p.m) return;
-  const int64_t run = warp - row * runs;
-  const int lane = threadIdx.x % 32;
-  const RowGrad of_row(p, row);
+  const int lane = threadIdx.x % 32, first = int(warp - row * runs) * kRun + lane;
   const T* const logits = static_cast<const T*>(p.logits) + row * p.stride;
   const uint8_t* const allowed = p.allowed ? p.allowed + row * p.allowed_stride : nullptr;
   T* const grad = static_cast<T*>(p.grad) + row * p.v;
   const Grid<T> to(grad, p.v), from(logits, p.v);
-  uint32_t w[kRun / 32][4];
-  if (to.skip == from.skip) {
+  const int vectors = int(to.vectors());
+  uint32_t w[kVectors][4];
 #pragma unroll
-    for (int r = 0; r < kRun / 32; ++r) {
-      const int64_t i = run * kRun + lane + 32 * r;
-      if (i < to.vectors()) load_vector(from, allowed, i, w[r]);
+  for (int r = 0; r < kVectors; ++r) {
+    const int i = first + 32 * r;
+    if (i >= vectors) continue;
+    if (to.skip == from.skip) {
+      load_vector(from, allowed, i, w[r]);
+    } else {
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        w[r][k] = 0;
+#pragma unroll
+        for (int h = 0; h < kValues / 4; ++h) {
+          const int64_t place = to.place(i) + k * (kValues / 4) + h;
+          const bool open = place >= 0 && place < p.v && (!allowed || allowed[place]);
+          const uint32_t x = __float_as_uint(open ? value_at(logits + place) : -infinity());
+          w[r][k] |= sizeof(T) == 4 ? x : x >> 16 << 16 * h;
+        }
+      }
     }
   }
+  const RowGrad of(p, row);
+  const bool none = of.normalizer == -infinity();
+  const float base = none ? 0.0f : of.normalizer;
+  const float a = none ? 0.0f : -(of.g + of.h * of.entropy), b = none ? 0.0f : -of.h * kLn2;
+  const uint64_t minus_base = pair_of(-base, -base), a2 = pair_of(a, a), b2 = pair_of(b, b);
 #pragma unroll
-  for (int r = 0; r < kRun / 32; ++r) {
-    const int64_t i = run * kRun + lane + 32 * r, j0 = to.place(i);
-    if (i >= to.vectors()) continue;
+  for (int r = 0; r < kVectors; ++r) {
+    const int i = first + 32 * r;
+    if (i >= vectors) continue;
+    const int64_t j0 = to.place(i);
     float x[kValues];
 #pragma unroll
-    for (int j = 0; j < kValues; ++j) {
-      const int64_t place = j0 + j;
-      if (to.skip == from.skip) {
-        x[j] = word_value<T>(w[r], j);
-      } else {
-        const bool open = place >= 0 && place < p.v && (!allowed || allowed[place]);
-        x[j] = open ? value_at(logits + place) : -infinity();
-      }
-      x[j] = of_row.at(x[j], place);
+    for (int k = 0; k < kValues / 2; ++k) {
+      const uint64_t y = powers_of(word_pair<T>(w[r], k), minus_base);
+      const float2 q = values_of(y);
+      const uint64_t prob = pair_of(exp2_fast(q.x), exp2_fast(q.y));
+      const float2 v = values_of(multiply_pairs(prob, multiply_add_pairs(b2, y, a2)));
+      x[2 * k] = v.x, x[2 * k + 1] = v.y;
+    }
+    const int64_t chosen = of.action - j0;
+    if (chosen >= 0 && chosen < kValues && !none) {
+#pragma unroll
+      for (int j = 0; j < kValues; ++j)
+        if (j == chosen && word_value<T>(w[r], j) != -infinity()) x[j] += of.g;
     }
     if (j0 >= 0 && j0 + kValues <= p.v) {
       if constexpr (sizeof(T) == 4) {
@@ -609,6 +691,8 @@ __global__ void __launch_bounds__(256) scores_grad_kernel(const __grid_constant_
 }
 
 // ---- host -----------------------------------------------------------------------------------------------
+
+bool at_multiple(const void* p, int size) { return reinterpret_cast<uintptr_t>(p) % size == 0; }
 
 template <typename T, int kLanes>
 int few_scores(const Scores& p, cudaStream_t s) {
@@ -638,7 +722,8 @@ int scores_of(const Scores& p, cudaStream_t s) {
   if (p.v <= 4 * kEach) return few_scores<T, 4>(p, s);
   if (p.v <= 8 * kEach) return few_scores<T, 8>(p, s);
   if (p.v <= 32 * kEach) return few_scores<T, 32>(p, s);
-  const int64_t vectors = (p.v + 2 * kValues - 2) / kValues;  // at most, wherever rows start
+  const bool on_lines = at_multiple(p.logits, 16) && p.stride % kValues == 0;
+  const int64_t vectors = (p.v + (on_lines ? kValues - 1 : 2 * kValues - 2)) / kValues;  // at most
   if (vectors <= 64) return scores<T, 32, 2>(p, 1, s);
   if (vectors <= 128) return scores<T, 32, 4>(p, 1, s);
   if (vectors <= 256) return scores<T, 32, 8>(p, 1, s);
@@ -648,6 +733,7 @@ int scores_of(const Scores& p, cudaStream_t s) {
   int blocks = 1;
   while (blocks < 8 && (vectors > 512 * 8 * blocks || (p.m * blocks < 296 && vectors > 512 * blocks))) blocks *= 2;
   if (vectors <= 512 * 2 * blocks) return scores<T, 512, 2>(p, blocks, s);
+  if (vectors <= 512 * 4 * blocks) return scores<T, 512, 4>(p, blocks, s);
   return scores<T, 512, 8>(p, blocks, s);
 }
 
@@ -668,7 +754,6 @@ bool scores_sizes(int dtype, int64_t m, int64_t v, int64_t stride, int action_dt
          m < (int64_t(1) << 26) && m * v < (int64_t(1) << 40) && stride >= 0 && allowed_stride >= 0 &&
          valid_dtype(action_dtype);
 }
-bool at_multiple(const void* p, int size) { return reinterpret_cast<uintptr_t>(p) % size == 0; }
 int action_size(int dtype) { return dtype == RLENV_I64 ? 8 : dtype == RLENV_I32 ? 4 : 1; }
 
 }  // namespace
