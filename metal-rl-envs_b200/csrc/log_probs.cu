@@ -112,6 +112,18 @@ RLENV_D Sums moved(const Sums& a, float m) {  // against m >= a.m
   const float d = larger(a.m - m, kFar), e = __expf(d);
   return {m, e * a.s, e * fmaf(a.s, d, a.w)};
 }
+// Of kLanes neighbouring lanes, known to all of them.
+template <int kLanes>
+RLENV_D Sums of_team(const Sums& a) {
+  float m = a.m;
+#pragma unroll
+  for (int d = kLanes / 2; d > 0; d /= 2) m = larger(m, __shfl_xor_sync(0xffffffffu, m, d));
+  Sums r = moved(a, m);
+#pragma unroll
+  for (int d = kLanes / 2; d > 0; d /= 2)
+    r.s += __shfl_xor_sync(0xffffffffu, r.s, d), r.w += __shfl_xor_sync(0xffffffffu, r.w, d);
+  return r;
+}
 RLENV_D void add(Sums& a, float l, float base) {
   const float d = larger(l - base, kFar), e = __expf(d);
   a.s += e;
@@ -254,21 +266,22 @@ RLENV_D constexpr uint32_t empty_word() {  // -infinity
   return sizeof(T) == 4 ? 0xff800000u : 0xff80ff80u;
 }
 
-// The kValues bytes of `allowed` from place j0 on, all of them in the row, as two words.
+// The kValues bytes of `allowed` from place j0 on, all of them in the row of v, as words.
 template <int kValues>
 RLENV_D uint2 bytes_at(const uint8_t* allowed, int64_t j0, int64_t v) {
   const uint8_t* const at = allowed + j0;
-  const unsigned off = unsigned(reinterpret_cast<uintptr_t>(at) % 4);
+  const unsigned off = unsigned(reinterpret_cast<uintptr_t>(at) % kValues);
   uint2 b = make_uint2(0, 0);
   if (off == 0) {
-    const uint32_t* const words = reinterpret_cast<const uint32_t*>(at);
-    b.x = __ldg(words);
-    if (kValues == 8) b.y = __ldg(words + 1);
+    if constexpr (kValues == 8)
+      b = __ldg(reinterpret_cast<const uint2*>(at));
+    else
+      b.x = __ldg(reinterpret_cast<const uint32_t*>(at));
   } else if (j0 >= 4 && j0 + kValues + 4 <= v) {  // the words around them are in the row too
-    const uint32_t* const words = reinterpret_cast<const uint32_t*>(at - off);
-    const uint32_t w0 = __ldg(words), w1 = __ldg(words + 1);
-    b.x = __funnelshift_r(w0, w1, 8 * off);
-    if (kValues == 8) b.y = __funnelshift_r(w1, __ldg(words + 2), 8 * off);
+    const uint32_t* const words = reinterpret_cast<const uint32_t*>(at - off % 4);
+    const uint32_t w1 = __ldg(words + 1);
+    b.x = __funnelshift_r(__ldg(words), w1, 8 * (off % 4));
+    if (kValues == 8) b.y = __funnelshift_r(w1, off % 4 ? __ldg(words + 2) : 0u, 8 * (off % 4));
   } else {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -278,277 +291,295 @@ RLENV_D uint2 bytes_at(const uint8_t* allowed, int64_t j0, int64_t v) {
   }
   return b;
 }
-
-// Vector i of a row in 32-bit words, -infinity where a place is not allowed or not in the row.
+// kValues logits from place j0 on, which need not be a boundary; the places before and after them are in the row too.
 template <typename T>
-RLENV_D void load_vector(const Grid<T>& grid, const uint8_t* allowed, int64_t i, uint32_t (&w)[4]) {
-  constexpr int kValues = Grid<T>::kValues;
-  const int64_t j0 = grid.place(i);
-  if (j0 >= 0 && j0 + kValues <= grid.v) {
-    const uint4 q = __ldg(reinterpret_cast<const uint4*>(grid.row + j0));
-    w[0] = q.x, w[1] = q.y, w[2] = q.z, w[3] = q.w;
-    if (allowed) {
-      const uint2 b = bytes_at<kValues>(allowed, j0, grid.v);
-      const uint32_t none[2] = {__vcmpeq4(b.x, 0), __vcmpeq4(b.y, 0)};  // 0xff for what is not allowed
+RLENV_D uint4 words_between(const T* row, int64_t j0) {
+  const T* const at = row + j0;
+  const bool between = sizeof(T) == 2 && reinterpret_cast<uintptr_t>(at) % 4;
+  const uint32_t* const words = reinterpret_cast<const uint32_t*>(between ? at - 1 : at);
+  uint32_t w[5];
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const uint32_t mask = kValues == 8 ? __byte_perm(none[k / 2], 0, k % 2 ? 0x3322 : 0x1100)
-                                           : __byte_perm(none[0], 0, 0x1111 * k);
-        w[k] = (w[k] & ~mask) | (empty_word<T>() & mask);
-      }
-    }
-  } else {
+  for (int i = 0; i < 4; ++i) w[i] = __ldg(words + i);
+  if (!between) return make_uint4(w[0], w[1], w[2], w[3]);
+  w[4] = __ldg(words + 4);
+  return make_uint4(__funnelshift_r(w[0], w[1], 16), __funnelshift_r(w[1], w[2], 16), __funnelshift_r(w[2], w[3], 16),
+                    __funnelshift_r(w[3], w[4], 16));
+}
+// Bytes that hold bit 7 of a byte of x eight times over: of byte n where the selector's digit is 8 + n.
+RLENV_D uint32_t repeat_signs(uint32_t x, uint32_t selector) {
+  uint32_t r;
+  asm("prmt.b32 %0, %1, 0, %2;" : "=r"(r) : "r"(x), "r"(selector));
+  return r;
+}
+// A vector's words with -infinity in the places whose bytes are zero.
+template <typename T>
+RLENV_D void cut_out(uint32_t (&w)[4], uint2 bytes) {
+  // bit 7 of each byte that is not zero, then all bits of the values' places
+  const auto marked = [](uint32_t b) { return (((b & 0x7f7f7f7fu) + 0x7f7f7f7fu) | b) & 0x80808080u; };
+  const uint32_t of[2] = {marked(bytes.x), marked(bytes.y)};
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      w[k] = 0;
-#pragma unroll
-      for (int h = 0; h < kValues / 4; ++h) {
-        const int64_t j = j0 + k * (kValues / 4) + h;
-        const bool open = j >= 0 && j < grid.v && (!allowed || allowed[j]);
-        const float x = open ? value_at(grid.row + j) : -infinity();
-        w[k] |= sizeof(T) == 4 ? __float_as_uint(x) : __float_as_uint(x) >> 16 << 16 * h;
-      }
-    }
+  for (int k = 0; k < 4; ++k) {
+    const uint32_t open = Grid<T>::kValues == 8 ? repeat_signs(of[k / 2], k % 2 ? 0xbbaa : 0x9988)
+                                                : repeat_signs(of[0], 0x8888 + 0x1111 * k);
+    w[k] = (w[k] & open) | (empty_word<T>() & ~open);
   }
 }
-
-// A team of kThreads threads, a warp or a block, in 32 groups of neighbours.
-template <int kThreads>
-struct Team {
-  static constexpr int kWarps = kThreads / 32, kBlock = kThreads == 32 ? 256 : kThreads, kRows = kBlock / kThreads;
-  static constexpr int kRoom = kThreads == 32 ? 128 : 4 * kThreads;  // alternatives looked at
-  struct Shared {
-    float groups[32], sums[2 * kWarps];
-    uint64_t keys[kRoom], top[kMostTop];
-    uint32_t count;
-    float of_block[3];
-  };
-  static RLENV_D void sync() {
-    if constexpr (kWarps == 1)
-      __syncwarp();
+// A vector that a row's end cuts: -infinity where a place is not in the row or not allowed.
+template <typename T>
+__device__ __noinline__ uint4 edge_vector(const T* row, const uint8_t* allowed, int64_t v, int64_t j0) {
+  constexpr int kValues = 16 / int(sizeof(T));
+  uint32_t w[4] = {0, 0, 0, 0};
+#pragma unroll
+  for (int j = 0; j < kValues; ++j) {
+    const int64_t place = j0 + j;
+    const bool open = place >= 0 && place < v && (!allowed || allowed[place]);
+    const uint32_t x = __float_as_uint(open ? value_at(row + place) : -infinity());
+    if constexpr (sizeof(T) == 4)
+      w[j] = x;
     else
-      __syncthreads();
+      w[j / 2] |= x >> 16 << 16 * (j % 2);
   }
-  // The team's largest key; room holds kWarps of them.
-  static RLENV_D uint64_t most(uint64_t x, uint64_t* room) {
-#pragma unroll
-    for (int d = 16; d > 0; d /= 2) {
-      const uint64_t y = __shfl_xor_sync(0xffffffffu, x, d);
-      x = y > x ? y : x;
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+// A warp's search for its best logits. Its part of a row is 32 lanes' vectors of up to kEpochs epochs, each of which leaves
+// its largest logit behind. The top-th largest of these has `top` logits at least that are not below it, and the groups
+// which reach it, `top` of them where none are equal, are looked through again.
+constexpr int kEpochs = 4;
+struct Best {
+  static constexpr int kMany = 64, kRoom = kMany + 256;  // a step adds one vector a lane, 256 logits at most
+  union {
+    uint32_t largest[kEpochs][32];  // orders; 0: none. Until the groups are chosen
+    uint64_t keys[kRoom];
+  };
+  uint64_t kept[kMostTop];
+  uint8_t groups[32 * kEpochs];
+  int count;
+  RLENV_D void add(uint64_t key) { keys[atomicAdd(&count, 1)] = key; }
+  // Keeps the best `top` keys, in order. The smallest of them, or 0 where there are fewer. For the whole warp.
+  RLENV_D uint64_t keep(int top) {
+    __syncwarp();
+    const int lane = threadIdx.x % 32, n = count;
+    for (int i = lane; i < n; i += 32) {
+      const uint64_t key = keys[i];
+      int above = 0;
+#pragma unroll 4
+      for (int k = 0; k < n; ++k) above += keys[k] > key;
+      if (above < top) kept[above] = key;
     }
-    if constexpr (kWarps > 1) {
-      if (threadIdx.x % 32 == 0) room[threadIdx.x / 32] = x;
-      __syncthreads();
-      x = room[threadIdx.x % kWarps];
+    __syncwarp();
+    if (lane < top && lane < n) keys[lane] = kept[lane];
+    if (lane == 0) count = n < top ? n : top;
+    const uint64_t least = n < top ? 0 : kept[top - 1];
+    __syncwarp();
+    return least;
+  }
+  // Lists the groups that reach the top-th largest of all, and that as `least`; returns their number.
+  RLENV_D int choose(int top, int epochs, uint32_t& least) {
+    const int lane = threadIdx.x % 32;
+    uint32_t of[kEpochs], rest[kEpochs];
 #pragma unroll
-      for (int d = kWarps / 2; d > 0; d /= 2) {
-        const uint64_t y = __shfl_xor_sync(0xffffffffu, x, d);
-        x = y > x ? y : x;
+    for (int e = 0; e < kEpochs; ++e) of[e] = rest[e] = e < epochs ? largest[e][lane] : 0;
+    for (int r = 0; r < top; ++r) {  // takes the largest out, one after the other
+      uint32_t own = 0;
+#pragma unroll
+      for (int e = 0; e < kEpochs; ++e) own = max(own, rest[e]);
+      least = __reduce_max_sync(0xffffffffu, own);
+      if (lane == __ffs(__ballot_sync(0xffffffffu, own == least)) - 1) {
+        bool out = false;
+#pragma unroll
+        for (int e = 0; e < kEpochs; ++e)
+          if (!out && rest[e] == least) rest[e] = 0, out = true;
       }
-      __syncthreads();
     }
-    return x;
+    int n = 0;
+#pragma unroll
+    for (int e = 0; e < kEpochs; ++e) {
+      const bool in = of[e] != 0 && of[e] >= least;
+      const uint32_t all = __ballot_sync(0xffffffffu, in);
+      if (in) groups[n + __popc(all & ((1u << lane) - 1))] = uint8_t(32 * e + lane);
+      n += __popc(all);
+    }
+    __syncwarp();
+    return n;
   }
 };
 
-// The n-th largest of a warp's values, known to all lanes: sorted by exchanges with lanes at growing distances
-// (Batcher 1968).
-RLENV_D float nth_largest(float x, int n) {
-  const int lane = threadIdx.x % 32;
-  uint32_t v = order_of(x);
-#pragma unroll
-  for (int size = 2; size <= 32; size *= 2)
-#pragma unroll
-    for (int d = size / 2; d > 0; d /= 2) {
-      const uint32_t other = __shfl_xor_sync(0xffffffffu, v, d);
-      v = ((lane & d) == 0) == ((lane & size) == 0) ? max(v, other) : min(v, other);
-    }
-  return value_of(__shfl_sync(0xffffffffu, v, n - 1));
-}
-
-// kThreads threads with room for kVectors vectors each; longer parts of a row go tile by tile, and are read again for
-// their sums. A cluster's blocks have a part of the row each.
-//
-// The alternatives: the n-th largest of the 32 groups' largest logits has n logits at least that are not below it, and as
-// a rule few more. These are collected and their ranks counted; where they are too many (a row of equal logits, or all
-// large ones in one group) they are found one after the other.
-template <typename T, int kThreads, int kVectors>
-__global__ void __launch_bounds__(Team<kThreads>::kBlock) scores_kernel(const __grid_constant__ Scores p) {
-  using G = Team<kThreads>;
-  constexpr int kValues = Grid<T>::kValues, kTile = kThreads * kVectors;
-  __shared__ typename G::Shared shared[G::kRows];
-  auto& sh = shared[threadIdx.x / kThreads];
+// kWarps warps read a row in steps of kSteps vectors a lane, and a cluster's blocks a part of it each: no lane waits for
+// another before the row's end. A lane's sums stand against a base of its own, which moves only where a logit is so far
+// above that powers would grow too large.
+constexpr int kSteps = 4;
+constexpr float kAbove = 20.0f;
+template <int kWarps>
+struct Team {
+  static constexpr int kThreads = kWarps == 1 ? 128 : 32 * kWarps, kRows = kThreads / (32 * kWarps);
+};
+template <typename T, int kWarps>
+__global__ void __launch_bounds__(Team<kWarps>::kThreads, 1024 / Team<kWarps>::kThreads)
+scores_kernel(const __grid_constant__ Scores p) {
+  constexpr int kValues = Grid<T>::kValues, kStride = 32 * kWarps, kBlockWarps = Team<kWarps>::kThreads / 32;
+  __shared__ Best bests[kBlockWarps];
+  __shared__ Sums of_warps[kBlockWarps];
+  __shared__ Sums of_block;
+  __shared__ uint64_t top_of_block[kMostTop];
   cg::cluster_group cluster = cg::this_cluster();
-  const int blocks = kThreads == 32 ? 1 : int(cluster.num_blocks()), rank = blocks > 1 ? int(cluster.block_rank()) : 0;
-  const int at = threadIdx.x % kThreads, lane = threadIdx.x % 32;
-  const int64_t row = kThreads == 32 ? int64_t(blockIdx.x) * G::kRows + threadIdx.x / 32 : blockIdx.x / blocks;
+  const int blocks = kWarps == 16 ? int(cluster.num_blocks()) : 1, rank = blocks > 1 ? int(cluster.block_rank()) : 0;
+  const int lane = threadIdx.x % 32, warp = threadIdx.x / 32 % kWarps;
+  const int64_t row = kWarps == 1 ? int64_t(blockIdx.x) * kBlockWarps + threadIdx.x / 32 : blockIdx.x / blocks;
   if (row >= p.m) return;  // a warp
   const Grid<T> grid(static_cast<const T*>(p.logits) + row * p.stride, p.v);
   const uint8_t* const allowed = p.allowed ? p.allowed + row * p.allowed_stride : nullptr;
   const int vectors = int(grid.vectors()), part = (vectors + blocks - 1) / blocks, begin = min(rank * part, vectors),
             end = min(begin + part, vectors);
-  const bool one_tile = end - begin <= kTile;
+  // The row's first and last vectors, where they are not whole.
+  const int first_whole = grid.skip > 0, last_whole = (grid.skip + p.v) % kValues ? vectors - 1 : vectors;
+  Best& best = bests[threadIdx.x / 32];
 
-  uint32_t w[kVectors][4];
-  const auto load_tile = [&](int from) {
+  const auto load = [&](int i, uint32_t (&w)[4], uint2& bytes) {
+    if (i >= first_whole && i < last_whole && i < end) {
+      const uint4 q = __ldg(reinterpret_cast<const uint4*>(grid.row + grid.place(i)));
+      w[0] = q.x, w[1] = q.y, w[2] = q.z, w[3] = q.w;
+      if (allowed) bytes = bytes_at<kValues>(allowed, grid.place(i), p.v);
+    } else {
 #pragma unroll
-    for (int r = 0; r < kVectors; ++r) {
-      const int i = from + r * kThreads + at;
-      if (i < end) {
-        load_vector(grid, allowed, i, w[r]);
-      } else {
-#pragma unroll
-        for (int k = 0; k < 4; ++k) w[r][k] = empty_word<T>();
-      }
+      for (int k = 0; k < 4; ++k) w[k] = empty_word<T>();
     }
   };
-  // f(r) for the tile's vectors of this thread; the same ones are left out by all threads.
-  const auto each_vector = [&](int from, auto&& f) {
-#pragma unroll
-    for (int r = 0; r < kVectors; ++r)
-      if (from + r * kThreads < end) f(r);
+  const auto finish = [&](int i, uint32_t (&w)[4], uint2 bytes) {
+    if (i >= first_whole && i < last_whole && i < end) {
+      if (allowed) cut_out<T>(w, bytes);
+    } else if (i < end) {
+      const uint4 q = edge_vector(grid.row, allowed, p.v, grid.place(i));
+      w[0] = q.x, w[1] = q.y, w[2] = q.z, w[3] = q.w;
+    }
   };
-  uint32_t most = empty_word<T>();
-  for (int from = begin; from < end; from += kTile) {
-    load_tile(from);
-    each_vector(from, [&](int r) {
-      most = larger_words<T>(most, larger_words<T>(larger_words<T>(w[r][0], w[r][1]), larger_words<T>(w[r][2], w[r][3])));
-    });
-  }
-  const float own_most = largest_of<T>(most);
-  float group = own_most;
-  if constexpr (kThreads > 32) {
-#pragma unroll
-    for (int d = (kThreads / 32) / 2; d > 0; d /= 2) group = larger(group, __shfl_xor_sync(0xffffffffu, group, d));
-    if (at % (kThreads / 32) == 0) sh.groups[at / (kThreads / 32)] = group;
-  }
-  if (at == 0) sh.count = 0;
-  G::sync();
-  if constexpr (kThreads > 32) group = sh.groups[lane];
-  Sums sums{group, 0.0f, 0.0f};
-#pragma unroll
-  for (int d = 16; d > 0; d /= 2) sums.m = larger(sums.m, __shfl_xor_sync(0xffffffffu, sums.m, d));
-  const float base = base_of(sums.m);
-  const float least = p.top > 0 ? nth_largest(group, p.top) : 0.0f;
+  const auto largest_word = [](const uint32_t (&w)[4]) {
+    return larger_words<T>(larger_words<T>(w[0], w[1]), larger_words<T>(w[2], w[3]));
+  };
 
-  const uint32_t reach = word_of<T>(least);
-  const uint64_t minus_base = pair_of(-base, -base);
-  const bool mine = p.top > 0 && !(own_most < least);
+  float base = -infinity(), of_epoch = -infinity();
   uint64_t s2 = 0, w2 = 0;
-  for (int from = begin; from < end; from += kTile) {
-    if (!one_tile) load_tile(from);
-    if (mine)
-      each_vector(from, [&](int r) {
+  const auto own_sums = [&] {
+    const float2 s = values_of(s2), w = values_of(w2);
+    return Sums{base, s.x + s.y, (w.x + w.y) * kLn2};
+  };
+  const int warp_begin = begin + 32 * warp, turns = warp_begin < end ? (end - warp_begin + kSteps * kStride - 1) / (kSteps * kStride) : 0,
+            epoch = (turns + kEpochs - 1) / kEpochs;  // turns of one
+  for (int turn = 0, left = epoch; turn < turns; ++turn) {
+    const int from = warp_begin + turn * kSteps * kStride;
+    uint32_t w[kSteps][4];
+    uint2 bytes[kSteps];
 #pragma unroll
-        for (int k = 0; k < 4; ++k)
-          if (any_reaches<T>(w[r][k], reach)) {
+    for (int u = 0; u < kSteps; ++u) load(from + u * kStride + lane, w[u], bytes[u]);
 #pragma unroll
-            for (int h = 0; h < kValues / 4; ++h) {
-              const int j = k * (kValues / 4) + h;
-              const float x = word_value<T>(w[r], j);
-              const int64_t place = grid.place(from + r * kThreads + at) + j;
-              if (x < least || place < 0 || place >= p.v || from + r * kThreads + at >= end) continue;
-              const uint32_t slot = atomicAdd(&sh.count, 1u);
-              if (slot < G::kRoom) sh.keys[slot] = key_of(x, uint32_t(place));
-            }
-          }
-      });
-    each_vector(from, [&](int r) {
+    for (int u = 0; u < kSteps; ++u) finish(from + u * kStride + lane, w[u], bytes[u]);
+    uint32_t all = largest_word(w[0]);
+#pragma unroll
+    for (int u = 1; u < kSteps; ++u) all = larger_words<T>(all, largest_word(w[u]));
+    const float most = largest_of<T>(all);
+    if (most > base + kAbove) {
+      const Sums now = moved(own_sums(), most);
+      base = most, s2 = pair_of(now.s, 0.0f), w2 = pair_of(now.w * kLog2E, 0.0f);
+    }
+    const float against = base_of(base);
+    const uint64_t minus_base = pair_of(-against, -against);
+#pragma unroll
+    for (int u = 0; u < kSteps; ++u) {
+      if (from + u * kStride >= end) break;
 #pragma unroll
       for (int i = 0; i < kValues / 2; ++i) {
-        const uint64_t y = powers_of(word_pair<T>(w[r], i), minus_base);
+        const uint64_t y = powers_of(word_pair<T>(w[u], i), minus_base);
         const float2 of = values_of(y);
         const uint64_t e = pair_of(exp2_fast(of.x), exp2_fast(of.y));
         s2 = add_pairs(s2, e), w2 = multiply_add_pairs(e, y, w2);
       }
-    });
-  }
-  const float2 s_own = values_of(s2), w_own = values_of(w2);
-  sums.s = s_own.x + s_own.y, sums.w = (w_own.x + w_own.y) * kLn2;
-#pragma unroll
-  for (int d = 16; d > 0; d /= 2) {
-    sums.s += __shfl_xor_sync(0xffffffffu, sums.s, d);
-    sums.w += __shfl_xor_sync(0xffffffffu, sums.w, d);
-  }
-  if (kThreads > 32 && lane == 0) sh.sums[at / 32] = sums.s, sh.sums[G::kWarps + at / 32] = sums.w;
-  G::sync();
-  if constexpr (kThreads > 32) {
-    sums.s = sh.sums[lane % G::kWarps], sums.w = sh.sums[G::kWarps + lane % G::kWarps];
-#pragma unroll
-    for (int d = G::kWarps / 2; d > 0; d /= 2) {
-      sums.s += __shfl_xor_sync(0xffffffffu, sums.s, d);
-      sums.w += __shfl_xor_sync(0xffffffffu, sums.w, d);
+    }
+    if (p.top > 0) {
+      of_epoch = larger(of_epoch, most);
+      if (--left == 0 || turn == turns - 1) {
+        best.largest[turn / epoch][lane] = warp_begin + turn / epoch * epoch * kSteps * kStride + lane < end ? order_of(of_epoch) : 0;
+        of_epoch = -infinity(), left = epoch;
+      }
     }
   }
-  const bool alone = kThreads == 32 || blocks == 1;
-  if (alone && at == 0) write_scores<T>(p, row, sums);
+  Sums sums = of_team<32>(own_sums());
 
   if (p.top > 0) {
-    const float normalizer = normalizer_of(sums);  // of the row, where the block has all of it
-    const auto found = [&](int r, uint64_t key) {
-      if (alone)
-        write_top(p, row, r, key, normalizer);
-      else
-        sh.top[r] = key;
-    };
-    const int count = int(sh.count);
-    if (count <= G::kRoom) {
-      if (!alone && at >= count && at < p.top) sh.top[at] = 0;  // a part of fewer logits
-      for (int i = at; i < count; i += kThreads) {
-        const uint64_t key = sh.keys[i];
-        int above = 0;
-        for (int k = 0; k < count; ++k) above += sh.keys[k] > key;
-        if (above < p.top) found(above, key);
-      }
-    } else {
-      uint64_t last = ~uint64_t(0);
-      G::sync();  // the keys' room is free
-      for (int n = 0; n < p.top; ++n) {
-        uint64_t best = 0;
-        for (int from = begin; from < end; from += kTile) {
-          if (!one_tile) load_tile(from);
-#pragma unroll
-          for (int r = 0; r < kVectors; ++r) {
-            const int i = from + r * kThreads + at;
-            if (i >= end) continue;
+    if (lane == 0) best.count = 0;
+    __syncwarp();
+    uint32_t least = 0;
+    const int each = kSteps * epoch, chosen = turns ? best.choose(p.top, (turns + epoch - 1) / epoch, least) : 0;
+    uint64_t least_key = uint64_t(least) << 32;
+    for (int at = 0; at < chosen * each; at += 32) {
+      const int t = at + lane;
+      if (t < chosen * each) {
+        const int group = best.groups[t / each], i = warp_begin + (group / 32 * each + t % each) * kStride + group % 32;
+        if (i < end) {
+          uint32_t w[4];
+          uint2 bytes;
+          load(i, w, bytes);
+          finish(i, w, bytes);
+          if (order_of(largest_of<T>(largest_word(w))) >= uint32_t(least_key >> 32)) {
 #pragma unroll
             for (int j = 0; j < kValues; ++j) {
               const int64_t place = grid.place(i) + j;
-              const uint64_t key = key_of(word_value<T>(w[r], j), uint32_t(place));
-              if (place >= 0 && place < p.v && key < last && key > best) best = key;
+              const uint64_t key = key_of(word_value<T>(w, j), uint32_t(place));
+              if (key > least_key && place >= 0 && place < p.v) best.add(key);
             }
           }
         }
-        last = G::most(best, sh.keys);
-        if (at == 0) found(n, last);
       }
+      __syncwarp();
+      if (best.count > Best::kMany)
+        if (const uint64_t now = best.keep(p.top)) least_key = now;
     }
+    best.keep(p.top);
   }
-  if (alone) return;
+  if constexpr (kWarps == 1) {
+    if (lane == 0) write_scores<T>(p, row, sums);
+    if (lane < p.top) write_top(p, row, lane, best.kept[lane], normalizer_of(sums));
+    return;
+  }
 
-  // The cluster's first block joins the parts: their sums in order, and their alternatives by their ranks.
-  if (at == 0) sh.of_block[0] = sums.m, sh.of_block[1] = sums.s, sh.of_block[2] = sums.w;
+  // The warps' sums and alternatives, these by their ranks among all.
+  const auto rank_all = [&](int lists, auto&& key_at, auto&& found) {
+    for (int i = threadIdx.x; i < lists * p.top; i += kStride) {
+      const uint64_t key = key_at(i);
+      if (key == 0) continue;  // a part of fewer logits
+      int above = 0;
+      for (int k = 0; k < lists * p.top; ++k) above += key_at(k) > key;
+      if (above < p.top) found(above, key);
+    }
+  };
+  if (lane == 0) of_warps[warp] = sums;
+  if (lane < p.top && lane >= best.count) best.kept[lane] = 0;
+  if (threadIdx.x < kMostTop) top_of_block[threadIdx.x] = 0;
+  __syncthreads();
+  sums = of_team<kWarps>(of_warps[lane % kWarps]);
+  if (blocks == 1 && threadIdx.x == 0) write_scores<T>(p, row, sums);
+  if (p.top > 0) {
+    const float normalizer = normalizer_of(sums);
+    rank_all(kWarps, [&](int i) { return bests[i / p.top].kept[i % p.top]; }, [&](int r, uint64_t key) {
+      if (blocks == 1)
+        write_top(p, row, r, key, normalizer);
+      else
+        top_of_block[r] = key;
+    });
+  }
+  if (blocks == 1) return;
+
+  // The cluster's first block does the same with the blocks'.
+  if (threadIdx.x == 0) of_block = sums;
   cluster.sync();
   if (rank == 0) {
-    Sums all{sums.m, 0.0f, 0.0f};
-    for (int b = 1; b < blocks; ++b) all.m = larger(all.m, cluster.map_shared_rank(sh.of_block, b)[0]);
-    for (int b = 0; b < blocks; ++b) {
-      const float* const of = cluster.map_shared_rank(sh.of_block, b);
-      const Sums one = moved(Sums{of[0], of[1], of[2]}, all.m);
-      all.s += one.s, all.w += one.w;
-    }
-    if (at == 0) write_scores<T>(p, row, all);
+    sums = of_team<8>(lane % 8 < blocks ? *cluster.map_shared_rank(&of_block, lane % 8) : Sums{-infinity(), 0.0f, 0.0f});
+    if (threadIdx.x == 0) write_scores<T>(p, row, sums);
     if (p.top > 0) {
-      const int count = blocks * p.top;
-      for (int i = at; i < count; i += kThreads) sh.keys[i] = cluster.map_shared_rank(sh.top, i / p.top)[i % p.top];
+      const float normalizer = normalizer_of(sums);
+      for (int i = threadIdx.x; i < blocks * p.top; i += kStride)
+        bests[0].keys[i] = cluster.map_shared_rank(top_of_block, i / p.top)[i % p.top];
       __syncthreads();
-      const float normalizer = normalizer_of(all);
-      for (int i = at; i < count; i += kThreads) {
-        const uint64_t key = sh.keys[i];
-        int above = 0;
-        for (int k = 0; k < count; ++k) above += sh.keys[k] > key;
-        if (key && above < p.top) write_top(p, row, above, key, normalizer);
-      }
+      rank_all(blocks, [&](int i) { return bests[0].keys[i]; }, [&](int r, uint64_t key) { write_top(p, row, r, key, normalizer); });
     }
   }
   cluster.sync();  // no block ends while its shared memory is read
@@ -611,50 +642,51 @@ __global__ void __launch_bounds__(256) few_scores_grad_kernel(const __grid_const
 }
 
 // A warp a run of kRun vectors of a row of the gradient, on its 16-byte boundaries. With y = log2 p the gradient of what
-// was not chosen is - p (g + h entropy + h ln 2 y): two values an instruction but for the power.
+// was not chosen is - p (g + h entropy + h ln 2 y): two values an instruction but for the power. kAlike: the logits' rows
+// lie on the boundaries as the gradient's do.
 constexpr int kRun = 128;
-template <typename T>
-__global__ void __launch_bounds__(256) scores_grad_kernel(const __grid_constant__ ScoresGrad p, int64_t runs) {
+template <typename T, bool kAlike>
+__global__ void __launch_bounds__(256) scores_grad_kernel(const __grid_constant__ ScoresGrad p, uint32_t runs) {
   constexpr int kValues = Grid<T>::kValues, kVectors = kRun / 32;
-  const int64_t warp = int64_t(blockIdx.x) * 8 + threadIdx.x / 32, row = warp / runs;
+  const uint32_t warp = blockIdx.x * 8 + threadIdx.x / 32, of_row = warp / runs;
+  const int64_t row = of_row;
   if (row >= p.m) return;
-  const int lane = threadIdx.x % 32, first = int(warp - row * runs) * kRun + lane;
+  const int lane = threadIdx.x % 32, first = int(warp - of_row * runs) * kRun + lane;
   const T* const logits = static_cast<const T*>(p.logits) + row * p.stride;
   const uint8_t* const allowed = p.allowed ? p.allowed + row * p.allowed_stride : nullptr;
   T* const grad = static_cast<T*>(p.grad) + row * p.v;
-  const Grid<T> to(grad, p.v), from(logits, p.v);
+  const Grid<T> to(grad, p.v);
   const int vectors = int(to.vectors());
+  const int first_whole = to.skip > 0, last_whole = (to.skip + p.v) % kValues ? vectors - 1 : vectors;
   uint32_t w[kVectors][4];
+  uint2 bytes[kVectors];
 #pragma unroll
   for (int r = 0; r < kVectors; ++r) {
     const int i = first + 32 * r;
-    if (i >= vectors) continue;
-    if (to.skip == from.skip) {
-      load_vector(from, allowed, i, w[r]);
-    } else {
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        w[r][k] = 0;
-#pragma unroll
-        for (int h = 0; h < kValues / 4; ++h) {
-          const int64_t place = to.place(i) + k * (kValues / 4) + h;
-          const bool open = place >= 0 && place < p.v && (!allowed || allowed[place]);
-          const uint32_t x = __float_as_uint(open ? value_at(logits + place) : -infinity());
-          w[r][k] |= sizeof(T) == 4 ? x : x >> 16 << 16 * h;
-        }
-      }
+    const int64_t j0 = to.place(i);
+    const bool inside = i >= first_whole && i < last_whole && (kAlike || (j0 > 0 && j0 + kValues < p.v));
+    if (inside) {
+      const uint4 q = kAlike ? __ldg(reinterpret_cast<const uint4*>(logits + j0)) : words_between(logits, j0);
+      w[r][0] = q.x, w[r][1] = q.y, w[r][2] = q.z, w[r][3] = q.w;
+      if (allowed) bytes[r] = bytes_at<kValues>(allowed, j0, p.v);
     }
   }
   const RowGrad of(p, row);
   const bool none = of.normalizer == -infinity();
-  const float base = none ? 0.0f : of.normalizer;
-  const float a = none ? 0.0f : -(of.g + of.h * of.entropy), b = none ? 0.0f : -of.h * kLn2;
+  const float base = none ? 0.0f : of.normalizer, a = none ? 0.0f : -(of.g + of.h * of.entropy), b = none ? 0.0f : -of.h * kLn2;
   const uint64_t minus_base = pair_of(-base, -base), a2 = pair_of(a, a), b2 = pair_of(b, b);
 #pragma unroll
   for (int r = 0; r < kVectors; ++r) {
     const int i = first + 32 * r;
-    if (i >= vectors) continue;
+    if (i >= vectors) break;
     const int64_t j0 = to.place(i);
+    const bool whole = i >= first_whole && i < last_whole;
+    if (whole && (kAlike || (j0 > 0 && j0 + kValues < p.v))) {
+      if (allowed) cut_out<T>(w[r], bytes[r]);
+    } else {
+      const uint4 q = edge_vector(logits, allowed, p.v, j0);
+      w[r][0] = q.x, w[r][1] = q.y, w[r][2] = q.z, w[r][3] = q.w;
+    }
     float x[kValues];
 #pragma unroll
     for (int k = 0; k < kValues / 2; ++k) {
@@ -670,7 +702,7 @@ __global__ void __launch_bounds__(256) scores_grad_kernel(const __grid_constant_
       for (int j = 0; j < kValues; ++j)
         if (j == chosen && word_value<T>(w[r], j) != -infinity()) x[j] += of.g;
     }
-    if (j0 >= 0 && j0 + kValues <= p.v) {
+    if (whole) {
       if constexpr (sizeof(T) == 4) {
         *reinterpret_cast<float4*>(grad + j0) = make_float4(x[0], x[1], x[2], x[3]);
       } else {
@@ -699,18 +731,18 @@ int few_scores(const Scores& p, cudaStream_t s) {
   few_scores_kernel<T, kLanes><<<unsigned((p.m * kLanes + 255) / 256), 256, 0, s>>>(p);
   return launch_status();
 }
-template <typename T, int kThreads, int kVectors>
+template <typename T, int kWarps>
 int scores(const Scores& p, int blocks, cudaStream_t s) {
-  using G = Team<kThreads>;
+  using G = Team<kWarps>;
   cudaLaunchConfig_t config{};
-  config.gridDim = dim3(unsigned(kThreads == 32 ? (p.m + G::kRows - 1) / G::kRows : p.m * blocks));
-  config.blockDim = dim3(G::kBlock);
+  config.gridDim = dim3(unsigned((p.m + G::kRows - 1) / G::kRows * blocks));
+  config.blockDim = dim3(G::kThreads);
   config.stream = s;
   cudaLaunchAttribute cluster{};
   cluster.id = cudaLaunchAttributeClusterDimension;
   cluster.val.clusterDim.x = unsigned(blocks), cluster.val.clusterDim.y = cluster.val.clusterDim.z = 1;
   config.attrs = &cluster, config.numAttrs = blocks > 1 ? 1 : 0;
-  const cudaError_t e = cudaLaunchKernelEx(&config, scores_kernel<T, kThreads, kVectors>, p);
+  const cudaError_t e = cudaLaunchKernelEx(&config, scores_kernel<T, kWarps>, p);
   return e == cudaSuccess ? launch_status() : int(e);
 }
 
@@ -722,19 +754,13 @@ int scores_of(const Scores& p, cudaStream_t s) {
   if (p.v <= 4 * kEach) return few_scores<T, 4>(p, s);
   if (p.v <= 8 * kEach) return few_scores<T, 8>(p, s);
   if (p.v <= 32 * kEach) return few_scores<T, 32>(p, s);
-  const bool on_lines = at_multiple(p.logits, 16) && p.stride % kValues == 0;
-  const int64_t vectors = (p.v + (on_lines ? kValues - 1 : 2 * kValues - 2)) / kValues;  // at most
-  if (vectors <= 64) return scores<T, 32, 2>(p, 1, s);
-  if (vectors <= 128) return scores<T, 32, 4>(p, 1, s);
-  if (vectors <= 256) return scores<T, 32, 8>(p, 1, s);
-  if (vectors <= 1024) return scores<T, 128, 8>(p, 1, s);
-  // A part of a row for each block of a cluster: until it fits into the registers, and while blocks are few and a part
-  // has a vector for each thread.
+  // As few warps a row as fill the GPU, 16 an SM, with a vector a lane at least.
+  const int64_t vectors = p.v / kValues, enough = 16 * 148;
+  if (p.m >= enough || vectors <= 64) return scores<T, 1>(p, 1, s);
+  if (p.m * 4 >= enough || vectors <= 256) return scores<T, 4>(p, 1, s);
   int blocks = 1;
-  while (blocks < 8 && (vectors > 512 * 8 * blocks || (p.m * blocks < 296 && vectors > 512 * blocks))) blocks *= 2;
-  if (vectors <= 512 * 2 * blocks) return scores<T, 512, 2>(p, blocks, s);
-  if (vectors <= 512 * 4 * blocks) return scores<T, 512, 4>(p, blocks, s);
-  return scores<T, 512, 8>(p, blocks, s);
+  while (blocks < 8 && p.m * 16 * blocks < enough && vectors > 512 * blocks) blocks *= 2;
+  return scores<T, 16>(p, blocks, s);
 }
 
 template <typename T>
@@ -744,7 +770,13 @@ int scores_grad_of(const ScoresGrad& p, cudaStream_t s) {
     few_scores_grad_kernel<T><<<unsigned((p.m * p.v + 256 * kFlat - 1) / (256 * kFlat)), 256, 0, s>>>(p);
   } else {
     const int64_t vectors = (p.v + 2 * kValues - 2) / kValues, runs = (vectors + kRun - 1) / kRun;
-    scores_grad_kernel<T><<<unsigned((p.m * runs + 7) / 8), 256, 0, s>>>(p, runs);
+    const bool alike = p.stride % kValues == p.v % kValues && reinterpret_cast<uintptr_t>(p.logits) % 16 ==
+                       reinterpret_cast<uintptr_t>(p.grad) % 16;
+    const unsigned grid = unsigned((p.m * runs + 7) / 8);
+    if (alike)
+      scores_grad_kernel<T, true><<<grid, 256, 0, s>>>(p, uint32_t(runs));
+    else
+      scores_grad_kernel<T, false><<<grid, 256, 0, s>>>(p, uint32_t(runs));
   }
   return launch_status();
 }
