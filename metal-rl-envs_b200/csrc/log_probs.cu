@@ -348,12 +348,14 @@ __device__ __noinline__ uint4 edge_vector(const T* row, const uint8_t* allowed, 
 constexpr int kEpochs = 4;
 struct Best {
   static constexpr int kMany = 64, kRoom = kMany + 256;  // a step adds one vector a lane, 256 logits at most
+  uint64_t* keys;  // kRoom
   union {
     uint32_t largest[kEpochs][32];  // orders; 0: none. Until the groups are chosen
-    uint64_t keys[kRoom];
+    struct {
+      uint64_t kept[kMostTop];
+      uint8_t groups[32 * kEpochs];
+    };
   };
-  uint64_t kept[kMostTop];
-  uint8_t groups[32 * kEpochs];
   int count;
   RLENV_D void add(uint64_t key) { keys[atomicAdd(&count, 1)] = key; }
   // Keeps the best `top` keys, in order. The smallest of them, or 0 where there are fewer. For the whole warp.
@@ -405,19 +407,27 @@ struct Best {
   }
 };
 
-// kWarps warps read a row in steps of kSteps vectors a lane, and a cluster's blocks a part of it each: no lane waits for
-// another before the row's end. A lane's sums stand against a base of its own, which moves only where a logit is so far
-// above that powers would grow too large.
-constexpr int kSteps = 4;
+// kWarps warps read a row in turns of kSteps vectors a lane, and a cluster's blocks a part of it each: no lane waits for
+// another before the row's end. Each lane's next turns are on their way into its own places of shared memory meanwhile. A
+// lane's sums stand against a base of its own, which moves only where a logit is so far above that powers would grow too
+// large.
+constexpr int kSteps = 4, kAhead = 3;  // kAhead: turns in shared memory, the one at work among them
 constexpr float kAbove = 20.0f;
 template <int kWarps>
 struct Team {
   static constexpr int kThreads = kWarps == 1 ? 128 : 32 * kWarps, kRows = kThreads / (32 * kWarps);
+  static constexpr int kRing = kAhead * kSteps * 32;  // vectors of a warp
+  static constexpr int kShared = kThreads / 32 * kRing * 16;
+  static constexpr int kBlocks = 896 / kThreads < 2 ? 2 : 896 / kThreads;  // an SM's: what shared memory holds
 };
+static_assert(Team<1>::kRing * 16 >= Best::kRoom * 8, "the keys lie in the ring's place");
+
 template <typename T, int kWarps>
-__global__ void __launch_bounds__(Team<kWarps>::kThreads, 1024 / Team<kWarps>::kThreads)
+__global__ void __launch_bounds__(Team<kWarps>::kThreads, Team<kWarps>::kBlocks)
 scores_kernel(const __grid_constant__ Scores p) {
-  constexpr int kValues = Grid<T>::kValues, kStride = 32 * kWarps, kBlockWarps = Team<kWarps>::kThreads / 32;
+  using G = Team<kWarps>;
+  constexpr int kValues = Grid<T>::kValues, kStride = 32 * kWarps, kTurn = kSteps * kStride, kBlockWarps = G::kThreads / 32;
+  extern __shared__ __align__(16) uint4 rings[];
   __shared__ Best bests[kBlockWarps];
   __shared__ Sums of_warps[kBlockWarps];
   __shared__ Sums of_block;
@@ -432,29 +442,51 @@ scores_kernel(const __grid_constant__ Scores p) {
   const int vectors = int(grid.vectors()), part = (vectors + blocks - 1) / blocks, begin = min(rank * part, vectors),
             end = min(begin + part, vectors);
   // The row's first and last vectors, where they are not whole.
-  const int first_whole = grid.skip > 0, last_whole = (grid.skip + p.v) % kValues ? vectors - 1 : vectors;
+  const int first_whole = grid.skip > 0, last_whole = min((grid.skip + p.v) % kValues ? vectors - 1 : vectors, end);
+  const auto whole = [&](int i) { return i >= first_whole && i < last_whole; };
   Best& best = bests[threadIdx.x / 32];
+  uint4* const ring = rings + threadIdx.x / 32 * G::kRing;
+  const int warp_begin = begin + 32 * warp, turns = warp_begin < end ? (end - warp_begin + kTurn - 1) / kTurn : 0;
 
-  const auto load = [&](int i, uint32_t (&w)[4], uint2& bytes) {
-    if (i >= first_whole && i < last_whole && i < end) {
-      const uint4 q = __ldg(reinterpret_cast<const uint4*>(grid.row + grid.place(i)));
-      w[0] = q.x, w[1] = q.y, w[2] = q.z, w[3] = q.w;
-      if (allowed) bytes = bytes_at<kValues>(allowed, grid.place(i), p.v);
-    } else {
-#pragma unroll
-      for (int k = 0; k < 4; ++k) w[k] = empty_word<T>();
-    }
-  };
-  const auto finish = [&](int i, uint32_t (&w)[4], uint2 bytes) {
-    if (i >= first_whole && i < last_whole && i < end) {
-      if (allowed) cut_out<T>(w, bytes);
-    } else if (i < end) {
-      const uint4 q = edge_vector(grid.row, allowed, p.v, grid.place(i));
-      w[0] = q.x, w[1] = q.y, w[2] = q.z, w[3] = q.w;
-    }
-  };
   const auto largest_word = [](const uint32_t (&w)[4]) {
     return larger_words<T>(larger_words<T>(w[0], w[1]), larger_words<T>(w[2], w[3]));
+  };
+  const auto words = [](uint4 q, uint32_t (&w)[4]) { w[0] = q.x, w[1] = q.y, w[2] = q.z, w[3] = q.w; };
+  // Whether all of a warp's vectors of a turn are whole ones.
+  const auto inside = [&](int from) { return from >= first_whole && from + kTurn - kStride + 32 <= last_whole; };
+  const auto issue = [&](int turn, int slot) {
+    if (turn < turns) {
+      const int from = warp_begin + turn * kTurn;
+      uint4* const to = ring + slot * (kSteps * 32) + lane;
+      const uint32_t to_at = uint32_t(__cvta_generic_to_shared(to));
+      const T* const at = grid.row + grid.place(from + lane);
+      if (inside(from)) {
+#pragma unroll
+        for (int u = 0; u < kSteps; ++u)
+          asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to_at + u * 512), "l"(at + u * kStride * kValues) : "memory");
+      } else {
+#pragma unroll 1
+        for (int u = 0; u < kSteps; ++u) {
+          const int i = from + u * kStride + lane;
+          if (whole(i))
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to_at + u * 512), "l"(at + u * kStride * kValues) : "memory");
+          else if (i < end)
+            to[u * 32] = edge_vector(grid.row, allowed, p.v, grid.place(i));
+          else
+            to[u * 32] = make_uint4(empty_word<T>(), empty_word<T>(), empty_word<T>(), empty_word<T>());
+        }
+      }
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+  uint2 bytes[kSteps];  // of the turn at work, read a turn ahead
+  const auto load_bytes = [&](int turn) {
+    const int from = warp_begin + turn * kTurn + lane;
+#pragma unroll
+    for (int u = 0; u < kSteps; ++u) {
+      bytes[u] = make_uint2(~0u, ~0u);
+      if (turn < turns && whole(from + u * kStride)) bytes[u] = bytes_at<kValues>(allowed, grid.place(from + u * kStride), p.v);
+    }
   };
 
   float base = -infinity(), of_epoch = -infinity();
@@ -463,16 +495,25 @@ scores_kernel(const __grid_constant__ Scores p) {
     const float2 s = values_of(s2), w = values_of(w2);
     return Sums{base, s.x + s.y, (w.x + w.y) * kLn2};
   };
-  const int warp_begin = begin + 32 * warp, turns = warp_begin < end ? (end - warp_begin + kSteps * kStride - 1) / (kSteps * kStride) : 0,
-            epoch = (turns + kEpochs - 1) / kEpochs;  // turns of one
-  for (int turn = 0, left = epoch; turn < turns; ++turn) {
-    const int from = warp_begin + turn * kSteps * kStride;
+  const int epoch = (turns + kEpochs - 1) / kEpochs;  // turns of one
+#pragma unroll
+  for (int t = 0; t < kAhead - 1; ++t) issue(t, t);
+  if (allowed) load_bytes(0);
+  int slot = 0, next = kAhead - 1, left = epoch, at_epoch = 0;
+  for (int turn = 0; turn < turns; ++turn) {
+    const int from = warp_begin + turn * kTurn;
+    issue(turn + kAhead - 1, next);
+    next = next == kAhead - 1 ? 0 : next + 1;
+    asm volatile("cp.async.wait_group %0;" ::"n"(kAhead - 1) : "memory");
     uint32_t w[kSteps][4];
-    uint2 bytes[kSteps];
 #pragma unroll
-    for (int u = 0; u < kSteps; ++u) load(from + u * kStride + lane, w[u], bytes[u]);
+    for (int u = 0; u < kSteps; ++u) words(ring[(slot * kSteps + u) * 32 + lane], w[u]);
+    slot = slot == kAhead - 1 ? 0 : slot + 1;
+    if (allowed) {
 #pragma unroll
-    for (int u = 0; u < kSteps; ++u) finish(from + u * kStride + lane, w[u], bytes[u]);
+      for (int u = 0; u < kSteps; ++u) cut_out<T>(w[u], bytes[u]);
+      load_bytes(turn + 1);
+    }
     uint32_t all = largest_word(w[0]);
 #pragma unroll
     for (int u = 1; u < kSteps; ++u) all = larger_words<T>(all, largest_word(w[u]));
@@ -497,41 +538,49 @@ scores_kernel(const __grid_constant__ Scores p) {
     if (p.top > 0) {
       of_epoch = larger(of_epoch, most);
       if (--left == 0 || turn == turns - 1) {
-        best.largest[turn / epoch][lane] = warp_begin + turn / epoch * epoch * kSteps * kStride + lane < end ? order_of(of_epoch) : 0;
-        of_epoch = -infinity(), left = epoch;
+        best.largest[at_epoch][lane] = warp_begin + at_epoch * epoch * kTurn + lane < end ? order_of(of_epoch) : 0;
+        of_epoch = -infinity(), left = epoch, ++at_epoch;
       }
     }
   }
   Sums sums = of_team<32>(own_sums());
 
   if (p.top > 0) {
-    if (lane == 0) best.count = 0;
+    if (lane == 0) best.count = 0, best.keys = reinterpret_cast<uint64_t*>(ring);
     __syncwarp();
     uint32_t least = 0;
-    const int each = kSteps * epoch, chosen = turns ? best.choose(p.top, (turns + epoch - 1) / epoch, least) : 0;
+    const int each = kSteps * epoch, chosen = best.choose(p.top, at_epoch, least), total = chosen * each;
     uint64_t least_key = uint64_t(least) << 32;
-    for (int at = 0; at < chosen * each; at += 32) {
-      const int t = at + lane;
-      if (t < chosen * each) {
-        const int group = best.groups[t / each], i = warp_begin + (group / 32 * each + t % each) * kStride + group % 32;
-        if (i < end) {
+    for (int first = 0; first < total; first += 32 * kSteps) {  // kSteps vectors of a lane on their way together
+      uint4 q[kSteps];
+      int at[kSteps];
+#pragma unroll
+      for (int u = 0; u < kSteps; ++u) {
+        const int t = first + 32 * u + lane, group = t < total ? best.groups[t / each] : 0;
+        at[u] = t < total ? warp_begin + (group / 32 * each + t % each) * kStride + group % 32 : end;
+        if (whole(at[u]) && at[u] < end) q[u] = __ldg(reinterpret_cast<const uint4*>(grid.row + grid.place(at[u])));
+      }
+#pragma unroll
+      for (int u = 0; u < kSteps; ++u) {
+        if (at[u] < end) {
           uint32_t w[4];
-          uint2 bytes;
-          load(i, w, bytes);
-          finish(i, w, bytes);
+          if (!whole(at[u]))
+            q[u] = edge_vector(grid.row, allowed, p.v, grid.place(at[u]));
+          words(q[u], w);
+          if (allowed && whole(at[u])) cut_out<T>(w, bytes_at<kValues>(allowed, grid.place(at[u]), p.v));
           if (order_of(largest_of<T>(largest_word(w))) >= uint32_t(least_key >> 32)) {
 #pragma unroll
             for (int j = 0; j < kValues; ++j) {
-              const int64_t place = grid.place(i) + j;
+              const int64_t place = grid.place(at[u]) + j;
               const uint64_t key = key_of(word_value<T>(w, j), uint32_t(place));
               if (key > least_key && place >= 0 && place < p.v) best.add(key);
             }
           }
         }
+        __syncwarp();
+        if (best.count > Best::kMany)
+          if (const uint64_t now = best.keep(p.top)) least_key = now;
       }
-      __syncwarp();
-      if (best.count > Best::kMany)
-        if (const uint64_t now = best.keep(p.top)) least_key = now;
     }
     best.keep(p.top);
   }
@@ -737,11 +786,15 @@ int scores(const Scores& p, int blocks, cudaStream_t s) {
   cudaLaunchConfig_t config{};
   config.gridDim = dim3(unsigned((p.m + G::kRows - 1) / G::kRows * blocks));
   config.blockDim = dim3(G::kThreads);
+  config.dynamicSmemBytes = G::kShared;
   config.stream = s;
   cudaLaunchAttribute cluster{};
   cluster.id = cudaLaunchAttributeClusterDimension;
   cluster.val.clusterDim.x = unsigned(blocks), cluster.val.clusterDim.y = cluster.val.clusterDim.z = 1;
   config.attrs = &cluster, config.numAttrs = blocks > 1 ? 1 : 0;
+  if (G::kShared > 32 * 1024)
+    if (cudaError_t e = cudaFuncSetAttribute(scores_kernel<T, kWarps>, cudaFuncAttributeMaxDynamicSharedMemorySize, G::kShared))
+      return int(e);
   const cudaError_t e = cudaLaunchKernelEx(&config, scores_kernel<T, kWarps>, p);
   return e == cudaSuccess ? launch_status() : int(e);
 }
