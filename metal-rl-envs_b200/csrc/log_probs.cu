@@ -8,6 +8,8 @@
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
 
+#include <type_traits>
+
 #include "common.cuh"
 
 namespace rlenv {
@@ -85,6 +87,13 @@ RLENV_D float exp2_fast(float x) {  // within 2 ulp, 0 where float32's normal nu
 }
 constexpr float kLog2E = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
+// log2 e^(l - base) of two logits. What lies further below than kFar counts as that: it adds nothing, and -infinity times
+// nothing would be NaN.
+RLENV_D uint64_t powers_of(uint64_t l, uint64_t minus_base) {
+  const float2 d = values_of(add_pairs(l, minus_base));
+  return multiply_pairs(pair_of(larger(d.x, kFar), larger(d.y, kFar)), pair_of(kLog2E, kLog2E));
+}
+
 // Logits are ordered by value, ties by the lower place: as one whole number, larger first. 0 stands below all, NaN
 // above.
 RLENV_D uint32_t order_of(float x) {
@@ -124,29 +133,25 @@ RLENV_D Sums of_team(const Sums& a) {
     r.s += __shfl_xor_sync(0xffffffffu, r.s, d), r.w += __shfl_xor_sync(0xffffffffu, r.w, d);
   return r;
 }
-RLENV_D void add(Sums& a, float l, float base) {
-  const float d = larger(l - base, kFar), e = __expf(d);
-  a.s += e;
-  a.w = fmaf(e, d, a.w);
-}
-
 RLENV_D float normalizer_of(const Sums& a) { return base_of(a.m) + logf(a.s); }
 
-template <typename T>
-RLENV_D void write_scores(const Scores& p, int64_t row, const Sums& sums) {
-  const float normalizer = normalizer_of(sums);
-  p.normalizer[row] = normalizer;
-  p.entropy[row] = sums.s == 0.0f ? 0.0f : logf(sums.s) - sums.w / sums.s;
-  const int64_t a = action_of(p.actions, p.action_dtype, row);
-  check_flag(a >= p.v, kCheckActionRange);
-  float lp = 0.0f;
-  if (a >= p.v) {
-    lp = not_a_number();
-  } else if (a >= 0) {
-    const bool open = !p.allowed || p.allowed[row * p.allowed_stride + a];
-    lp = log_prob_of(open ? value_at(static_cast<const T*>(p.logits) + row * p.stride + a) : -infinity(), normalizer);
+// A row's action and its logit, read before the row so that nothing waits for them after it.
+struct Chosen {
+  int64_t action;
+  float l;
+  template <typename T>
+  static RLENV_D Chosen of(const Scores& p, int64_t row, const T* logits, const uint8_t* allowed) {
+    const int64_t a = action_of(p.actions, p.action_dtype, row);
+    return {a, a >= 0 && a < p.v && (!allowed || allowed[a]) ? value_at(logits + a) : -infinity()};
   }
-  p.log_prob[row] = lp;
+};
+
+RLENV_D void write_scores(const Scores& p, int64_t row, const Sums& sums, const Chosen& chosen) {
+  const float log_s = logf(sums.s), normalizer = base_of(sums.m) + log_s;
+  p.normalizer[row] = normalizer;
+  p.entropy[row] = sums.s == 0.0f ? 0.0f : log_s - sums.w / sums.s;
+  check_flag(chosen.action >= p.v, kCheckActionRange);
+  p.log_prob[row] = chosen.action < 0 ? 0.0f : chosen.action >= p.v ? not_a_number() : log_prob_of(chosen.l, normalizer);
 }
 RLENV_D void write_top(const Scores& p, int64_t row, int rank, uint64_t key, float normalizer) {
   p.top_actions[row * p.top + rank] = int64_t(uint32_t(~uint32_t(key)));
@@ -164,24 +169,42 @@ __global__ void __launch_bounds__(256) few_scores_kernel(const __grid_constant__
   const uint8_t* const allowed = p.allowed ? p.allowed + row * p.allowed_stride : nullptr;
   const int v = int(p.v);
   float x[kEach];
-  Sums sums{-infinity(), 0.0f, 0.0f};
 #pragma unroll
   for (int i = 0; i < kEach; ++i) {
     const int j = sub + kLanes * i;
-    x[i] = j < v && (!allowed || allowed[j]) ? value_at(logits + j) : -infinity();
+    x[i] = j < v ? value_at(logits + j) : -infinity();
   }
+  if (allowed) {
 #pragma unroll
-  for (int i = 0; i < kEach; ++i) sums.m = larger(sums.m, x[i]);
+    for (int i = 0; i < kEach; ++i) {
+      const int j = sub + kLanes * i;
+      if (j < v && !allowed[j]) x[i] = -infinity();
+    }
+  }
+  const Chosen chosen = Chosen::of(p, row, logits, allowed);
+  Sums sums{x[0], 0.0f, 0.0f};
+#pragma unroll
+  for (int i = 1; i < kEach; ++i) sums.m = larger(sums.m, x[i]);
 #pragma unroll
   for (int d = kLanes / 2; d > 0; d /= 2) sums.m = larger(sums.m, __shfl_xor_sync(0xffffffffu, sums.m, d));
+  const float base = base_of(sums.m);
+  const uint64_t minus_base = pair_of(-base, -base);
+  uint64_t s2 = 0, w2 = 0;
 #pragma unroll
-  for (int i = 0; i < kEach; ++i) add(sums, x[i], base_of(sums.m));
+  for (int i = 0; i < kEach; i += 2) {
+    const uint64_t y = powers_of(pair_of(x[i], x[i + 1]), minus_base);
+    const float2 of = values_of(y);
+    const uint64_t e = pair_of(exp2_fast(of.x), exp2_fast(of.y));
+    s2 = add_pairs(s2, e), w2 = multiply_add_pairs(e, y, w2);
+  }
+  const float2 s_own = values_of(s2), w_own = values_of(w2);
+  sums.s = s_own.x + s_own.y, sums.w = (w_own.x + w_own.y) * kLn2;
 #pragma unroll
   for (int d = kLanes / 2; d > 0; d /= 2) {
     sums.s += __shfl_xor_sync(0xffffffffu, sums.s, d);
     sums.w += __shfl_xor_sync(0xffffffffu, sums.w, d);
   }
-  if (sub == 0 && at < p.m) write_scores<T>(p, row, sums);
+  if (sub == 0 && at < p.m) write_scores(p, row, sums, chosen);
   if (p.top == 0) return;
   const float normalizer = normalizer_of(sums);
   uint32_t taken = 0;
@@ -254,12 +277,6 @@ template <typename T>
 RLENV_D bool any_reaches(uint32_t w, uint32_t least) {  // a place that is not below least's
   if constexpr (sizeof(T) == 4) return !(__uint_as_float(w) < __uint_as_float(least));
   return __hgeu2_mask(as_bf162(w), as_bf162(least)) != 0;
-}
-// log2 e^(l - base) of two logits. What lies further below than kFar counts as that: it adds nothing, and -infinity times
-// nothing would be NaN.
-RLENV_D uint64_t powers_of(uint64_t l, uint64_t minus_base) {
-  const float2 d = values_of(add_pairs(l, minus_base));
-  return multiply_pairs(pair_of(larger(d.x, kFar), larger(d.y, kFar)), pair_of(kLog2E, kLog2E));
 }
 template <typename T>
 RLENV_D constexpr uint32_t empty_word() {  // -infinity
@@ -379,20 +396,19 @@ struct Best {
   // Lists the groups that reach the top-th largest of all, and that as `least`; returns their number.
   RLENV_D int choose(int top, int epochs, uint32_t& least) {
     const int lane = threadIdx.x % 32;
-    uint32_t of[kEpochs], rest[kEpochs];
+    uint32_t of[kEpochs], rest[kEpochs];  // rest: in falling order
 #pragma unroll
     for (int e = 0; e < kEpochs; ++e) of[e] = rest[e] = e < epochs ? largest[e][lane] : 0;
+    const auto order = [&](int i, int j) {
+      const uint32_t high = max(rest[i], rest[j]);
+      rest[j] = min(rest[i], rest[j]), rest[i] = high;
+    };
+    static_assert(kEpochs == 4, "four values are put in order");
+    order(0, 1), order(2, 3), order(0, 2), order(1, 3), order(1, 2);
     for (int r = 0; r < top; ++r) {  // takes the largest out, one after the other
-      uint32_t own = 0;
-#pragma unroll
-      for (int e = 0; e < kEpochs; ++e) own = max(own, rest[e]);
-      least = __reduce_max_sync(0xffffffffu, own);
-      if (lane == __ffs(__ballot_sync(0xffffffffu, own == least)) - 1) {
-        bool out = false;
-#pragma unroll
-        for (int e = 0; e < kEpochs; ++e)
-          if (!out && rest[e] == least) rest[e] = 0, out = true;
-      }
+      least = __reduce_max_sync(0xffffffffu, rest[0]);
+      if (lane == __ffs(__ballot_sync(0xffffffffu, rest[0] == least)) - 1)
+        rest[0] = rest[1], rest[1] = rest[2], rest[2] = rest[3], rest[3] = 0;
     }
     int n = 0;
 #pragma unroll
@@ -495,10 +511,12 @@ scores_kernel(const __grid_constant__ Scores p) {
     const float2 s = values_of(s2), w = values_of(w2);
     return Sums{base, s.x + s.y, (w.x + w.y) * kLn2};
   };
-  const int epoch = (turns + kEpochs - 1) / kEpochs;  // turns of one
+  // An epoch's turns, a power of two.
+  const int epoch_bits = turns <= kEpochs ? 0 : 32 - __clz((turns - 1) / kEpochs), epoch = 1 << epoch_bits;
 #pragma unroll
   for (int t = 0; t < kAhead - 1; ++t) issue(t, t);
   if (allowed) load_bytes(0);
+  const Chosen chosen = Chosen::of(p, row, grid.row, allowed);
   int slot = 0, next = kAhead - 1, left = epoch, at_epoch = 0;
   for (int turn = 0; turn < turns; ++turn) {
     const int from = warp_begin + turn * kTurn;
@@ -549,30 +567,42 @@ scores_kernel(const __grid_constant__ Scores p) {
     if (lane == 0) best.count = 0, best.keys = reinterpret_cast<uint64_t*>(ring);
     __syncwarp();
     uint32_t least = 0;
-    const int each = kSteps * epoch, chosen = best.choose(p.top, at_epoch, least), total = chosen * each;
+    const int each_bits = 2 + epoch_bits, total = best.choose(p.top, at_epoch, least) << each_bits;
+    static_assert(kSteps == 4, "a group's vectors are 4 a turn");
     uint64_t least_key = uint64_t(least) << 32;
     for (int first = 0; first < total; first += 32 * kSteps) {  // kSteps vectors of a lane on their way together
       uint4 q[kSteps];
       int at[kSteps];
 #pragma unroll
       for (int u = 0; u < kSteps; ++u) {
-        const int t = first + 32 * u + lane, group = t < total ? best.groups[t / each] : 0;
-        at[u] = t < total ? warp_begin + (group / 32 * each + t % each) * kStride + group % 32 : end;
-        if (whole(at[u]) && at[u] < end) q[u] = __ldg(reinterpret_cast<const uint4*>(grid.row + grid.place(at[u])));
+        const int t = first + 32 * u + lane;
+        at[u] = end;
+        if (t < total) {
+          const int group = best.groups[t >> each_bits];
+          at[u] = warp_begin + ((group / 32 << each_bits) + (t & ((1 << each_bits) - 1))) * kStride + group % 32;
+        }
+        if (whole(at[u])) q[u] = __ldg(reinterpret_cast<const uint4*>(grid.row + grid.place(at[u])));
       }
 #pragma unroll
       for (int u = 0; u < kSteps; ++u) {
+        if (first + 32 * u >= total) break;
         if (at[u] < end) {
           uint32_t w[4];
-          if (!whole(at[u]))
-            q[u] = edge_vector(grid.row, allowed, p.v, grid.place(at[u]));
+          if (!whole(at[u])) q[u] = edge_vector(grid.row, allowed, p.v, grid.place(at[u]));
           words(q[u], w);
           if (allowed && whole(at[u])) cut_out<T>(w, bytes_at<kValues>(allowed, grid.place(at[u]), p.v));
-          if (order_of(largest_of<T>(largest_word(w))) >= uint32_t(least_key >> 32)) {
+          const float bar = value_of(uint32_t(least_key >> 32));
+          if (!(largest_of<T>(largest_word(w)) < bar)) {
+            uint32_t reach = 0;
 #pragma unroll
-            for (int j = 0; j < kValues; ++j) {
-              const int64_t place = grid.place(at[u]) + j;
-              const uint64_t key = key_of(word_value<T>(w, j), uint32_t(place));
+            for (int j = 0; j < kValues; ++j) reach |= !(word_value<T>(w, j) < bar) ? 1u << j : 0u;
+            const int place0 = int(grid.place(at[u]));
+            for (; reach; reach &= reach - 1) {
+              const int j = __ffs(reach) - 1, place = place0 + j;
+              const uint32_t word = kValues == 4 ? (j < 2 ? (j < 1 ? w[0] : w[1]) : (j < 3 ? w[2] : w[3]))
+                                                 : (j < 4 ? (j < 2 ? w[0] : w[1]) : (j < 6 ? w[2] : w[3]));
+              const float x = __uint_as_float(kValues == 4 ? word : j % 2 ? word & 0xffff0000u : word << 16);
+              const uint64_t key = key_of(x, uint32_t(place));
               if (key > least_key && place >= 0 && place < p.v) best.add(key);
             }
           }
@@ -585,7 +615,7 @@ scores_kernel(const __grid_constant__ Scores p) {
     best.keep(p.top);
   }
   if constexpr (kWarps == 1) {
-    if (lane == 0) write_scores<T>(p, row, sums);
+    if (lane == 0) write_scores(p, row, sums, chosen);
     if (lane < p.top) write_top(p, row, lane, best.kept[lane], normalizer_of(sums));
     return;
   }
@@ -605,7 +635,7 @@ scores_kernel(const __grid_constant__ Scores p) {
   if (threadIdx.x < kMostTop) top_of_block[threadIdx.x] = 0;
   __syncthreads();
   sums = of_team<kWarps>(of_warps[lane % kWarps]);
-  if (blocks == 1 && threadIdx.x == 0) write_scores<T>(p, row, sums);
+  if (blocks == 1 && threadIdx.x == 0) write_scores(p, row, sums, chosen);
   if (p.top > 0) {
     const float normalizer = normalizer_of(sums);
     rank_all(kWarps, [&](int i) { return bests[i / p.top].kept[i % p.top]; }, [&](int r, uint64_t key) {
@@ -622,7 +652,7 @@ scores_kernel(const __grid_constant__ Scores p) {
   cluster.sync();
   if (rank == 0) {
     sums = of_team<8>(lane % 8 < blocks ? *cluster.map_shared_rank(&of_block, lane % 8) : Sums{-infinity(), 0.0f, 0.0f});
-    if (threadIdx.x == 0) write_scores<T>(p, row, sums);
+    if (threadIdx.x == 0) write_scores(p, row, sums, chosen);
     if (p.top > 0) {
       const float normalizer = normalizer_of(sums);
       for (int i = threadIdx.x; i < blocks * p.top; i += kStride)
@@ -649,50 +679,76 @@ struct ScoresGrad {
   void* grad;
 };
 
-// What a row's gradients have in common.
+// What a row's gradients have in common. With y = log2 p the gradient of what was not chosen is
+// - p (g + h entropy + h ln 2 y): two values an instruction but for the power.
 struct RowGrad {
-  float g, h, normalizer, entropy;
-  int64_t action;
+  int64_t action;  // negative: none whose gradient differs
+  float g;
+  uint64_t minus_base, a, b;
   RLENV_D RowGrad(const ScoresGrad& p, int64_t row) {
     action = action_of(p.actions, p.action_dtype, row);
     check_flag(action >= p.v, kCheckActionRange);
+    const float normalizer = __ldg(p.normalizer + row), entropy = __ldg(p.entropy + row);
+    const float h = p.grad_entropy ? __ldg(p.grad_entropy + row) : 0.0f;
     g = p.grad_log_prob && action >= 0 ? __ldg(p.grad_log_prob + row) : 0.0f;
     if (action >= p.v) g = not_a_number();
-    h = p.grad_entropy ? __ldg(p.grad_entropy + row) : 0.0f;
-    normalizer = __ldg(p.normalizer + row), entropy = __ldg(p.entropy + row);
+    const bool none = normalizer == -infinity();
+    if (none) action = -1;
+    const float base = none ? 0.0f : normalizer, of_p = none ? 0.0f : -(g + h * entropy), of_y = none ? 0.0f : -h * kLn2;
+    minus_base = pair_of(-base, -base), a = pair_of(of_p, of_p), b = pair_of(of_y, of_y);
   }
-  RLENV_D float at(float l, int64_t place) const {
-    if (l == -infinity() || normalizer == -infinity()) return 0.0f;
-    const float lp = larger(l - normalizer, kFar), prob = __expf(lp);
-    return g * ((place == action ? 1.0f : 0.0f) - prob) - h * prob * (lp + entropy);
+  RLENV_D float2 without_choice(uint64_t l) const {
+    const uint64_t y = powers_of(l, minus_base);
+    const float2 of = values_of(y);
+    return values_of(multiply_pairs(pair_of(exp2_fast(of.x), exp2_fast(of.y)), multiply_add_pairs(b, y, a)));
+  }
+  RLENV_D float of_choice(float l) const { return l == -infinity() ? 0.0f : g; }
+  RLENV_D float2 at(float l0, float l1, int j0, int j1) const {
+    float2 r = without_choice(pair_of(l0, l1));
+    if (j0 == action) r.x += of_choice(l0);
+    if (j1 == action) r.y += of_choice(l1);
+    return r;
   }
 };
 
 RLENV_D void store_value(float* to, float x) { *to = x; }
 RLENV_D void store_value(__nv_bfloat16* to, float x) { *to = __float2bfloat16_rn(x); }
 
-// Rows of few actions: a thread an element.
-constexpr int kFlat = 4;
-template <typename T>
+// Rows of few actions: kLanes neighbouring lanes a row, as in the forward pass.
+template <typename T, int kLanes>
 __global__ void __launch_bounds__(256) few_scores_grad_kernel(const __grid_constant__ ScoresGrad p) {
-  const int64_t first = int64_t(blockIdx.x) * 256 * kFlat, row0 = first / p.v;
-  const uint32_t in = uint32_t(first - row0 * p.v), v = uint32_t(p.v);
+  const int sub = threadIdx.x % kLanes;
+  const int64_t row = (int64_t(blockIdx.x) * 256 + threadIdx.x) / kLanes;
+  if (row >= p.m) return;
+  const T* const logits = static_cast<const T*>(p.logits) + row * p.stride;
+  const uint8_t* const allowed = p.allowed ? p.allowed + row * p.allowed_stride : nullptr;
+  T* const grad = static_cast<T*>(p.grad) + row * p.v;
+  const int v = int(p.v);
+  float x[kEach];
 #pragma unroll
-  for (int i = 0; i < kFlat; ++i) {
-    const uint32_t off = in + threadIdx.x + 256 * i;
-    const int64_t row = row0 + off / v;
-    if (row >= p.m) return;
-    const uint32_t j = off % v;
-    const RowGrad grad(p, row);
-    const bool open = !p.allowed || p.allowed[row * p.allowed_stride + j];
-    const float l = open ? value_at(static_cast<const T*>(p.logits) + row * p.stride + j) : -infinity();
-    store_value(static_cast<T*>(p.grad) + row * p.v + j, grad.at(l, j));
+  for (int i = 0; i < kEach; ++i) {
+    const int j = sub + kLanes * i;
+    x[i] = j < v ? value_at(logits + j) : -infinity();
+  }
+  if (allowed) {
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) {
+      const int j = sub + kLanes * i;
+      if (j < v && !allowed[j]) x[i] = -infinity();
+    }
+  }
+  const RowGrad of(p, row);
+#pragma unroll
+  for (int i = 0; i < kEach; i += 2) {
+    const int j = sub + kLanes * i;
+    const float2 g = of.at(x[i], x[i + 1], j, j + kLanes);
+    if (j < v) store_value(grad + j, g.x);
+    if (j + kLanes < v) store_value(grad + j + kLanes, g.y);
   }
 }
 
-// A warp a run of kRun vectors of a row of the gradient, on its 16-byte boundaries. With y = log2 p the gradient of what
-// was not chosen is - p (g + h entropy + h ln 2 y): two values an instruction but for the power. kAlike: the logits' rows
-// lie on the boundaries as the gradient's do.
+// A warp a run of kRun vectors of a row of the gradient, on its 16-byte boundaries. kAlike: the logits' rows lie on the
+// boundaries as the gradient's do.
 constexpr int kRun = 128;
 template <typename T, bool kAlike>
 __global__ void __launch_bounds__(256) scores_grad_kernel(const __grid_constant__ ScoresGrad p, uint32_t runs) {
@@ -721,9 +777,6 @@ __global__ void __launch_bounds__(256) scores_grad_kernel(const __grid_constant_
     }
   }
   const RowGrad of(p, row);
-  const bool none = of.normalizer == -infinity();
-  const float base = none ? 0.0f : of.normalizer, a = none ? 0.0f : -(of.g + of.h * of.entropy), b = none ? 0.0f : -of.h * kLn2;
-  const uint64_t minus_base = pair_of(-base, -base), a2 = pair_of(a, a), b2 = pair_of(b, b);
 #pragma unroll
   for (int r = 0; r < kVectors; ++r) {
     const int i = first + 32 * r;
@@ -739,17 +792,14 @@ __global__ void __launch_bounds__(256) scores_grad_kernel(const __grid_constant_
     float x[kValues];
 #pragma unroll
     for (int k = 0; k < kValues / 2; ++k) {
-      const uint64_t y = powers_of(word_pair<T>(w[r], k), minus_base);
-      const float2 q = values_of(y);
-      const uint64_t prob = pair_of(exp2_fast(q.x), exp2_fast(q.y));
-      const float2 v = values_of(multiply_pairs(prob, multiply_add_pairs(b2, y, a2)));
+      const float2 v = of.without_choice(word_pair<T>(w[r], k));
       x[2 * k] = v.x, x[2 * k + 1] = v.y;
     }
     const int64_t chosen = of.action - j0;
-    if (chosen >= 0 && chosen < kValues && !none) {
+    if (chosen >= 0 && chosen < kValues) {
 #pragma unroll
       for (int j = 0; j < kValues; ++j)
-        if (j == chosen && word_value<T>(w[r], j) != -infinity()) x[j] += of.g;
+        if (j == chosen) x[j] += of.of_choice(word_value<T>(w[r], j));
     }
     if (whole) {
       if constexpr (sizeof(T) == 4) {
@@ -819,8 +869,19 @@ int scores_of(const Scores& p, cudaStream_t s) {
 template <typename T>
 int scores_grad_of(const ScoresGrad& p, cudaStream_t s) {
   constexpr int kValues = Grid<T>::kValues;
-  if (p.v < 64) {
-    few_scores_grad_kernel<T><<<unsigned((p.m * p.v + 256 * kFlat - 1) / (256 * kFlat)), 256, 0, s>>>(p);
+  const auto few = [&](auto lanes) {
+    few_scores_grad_kernel<T, lanes.value><<<unsigned((p.m * lanes.value + 255) / 256), 256, 0, s>>>(p);
+  };
+  if (p.v <= kEach) {
+    few(std::integral_constant<int, 1>());
+  } else if (p.v <= 2 * kEach) {
+    few(std::integral_constant<int, 2>());
+  } else if (p.v <= 4 * kEach) {
+    few(std::integral_constant<int, 4>());
+  } else if (p.v <= 8 * kEach) {
+    few(std::integral_constant<int, 8>());
+  } else if (p.v <= 32 * kEach) {
+    few(std::integral_constant<int, 32>());
   } else {
     const int64_t vectors = (p.v + 2 * kValues - 2) / kValues, runs = (vectors + kRun - 1) / kRun;
     const bool alike = p.stride % kValues == p.v % kValues && reinterpret_cast<uintptr_t>(p.logits) % 16 ==
