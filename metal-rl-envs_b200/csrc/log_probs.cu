@@ -620,25 +620,29 @@ scores_kernel(const __grid_constant__ Scores p) {
     return;
   }
 
-  // The warps' sums and alternatives, these by their ranks among all.
-  const auto rank_all = [&](int lists, auto&& key_at, auto&& found) {
-    for (int i = threadIdx.x; i < lists * p.top; i += kStride) {
-      const uint64_t key = key_at(i);
-      if (key == 0) continue;  // a part of fewer logits
+  // The warps' sums and alternatives, these by their ranks among all: lists of `top` side by side, zeros where a part has
+  // fewer logits. The first warp's ring and the second's have room for them.
+  uint64_t* const lists = reinterpret_cast<uint64_t*>(rings);
+  const auto rank_all = [&](int count, auto&& found) {
+    __syncthreads();
+    for (int i = threadIdx.x; i < count; i += kStride) {
+      const uint64_t key = lists[i];
       int above = 0;
-      for (int k = 0; k < lists * p.top; ++k) above += key_at(k) > key;
-      if (above < p.top) found(above, key);
+#pragma unroll 8
+      for (int k = 0; k < count; ++k) above += lists[k] > key;
+      if (key != 0 && above < p.top) found(above, key);
     }
   };
+  static_assert(kWarps == 1 || (kWarps * kMostTop * 8 <= 2 * G::kRing * 16 && 8 * kMostTop * 8 <= G::kRing * 16), "lists fit");
   if (lane == 0) of_warps[warp] = sums;
-  if (lane < p.top && lane >= best.count) best.kept[lane] = 0;
   if (threadIdx.x < kMostTop) top_of_block[threadIdx.x] = 0;
-  __syncthreads();
+  __syncthreads();  // the rings are free
   sums = of_team<kWarps>(of_warps[lane % kWarps]);
   if (blocks == 1 && threadIdx.x == 0) write_scores(p, row, sums, chosen);
   if (p.top > 0) {
+    if (lane < p.top) lists[warp * p.top + lane] = lane < best.count ? best.kept[lane] : 0;
     const float normalizer = normalizer_of(sums);
-    rank_all(kWarps, [&](int i) { return bests[i / p.top].kept[i % p.top]; }, [&](int r, uint64_t key) {
+    rank_all(kWarps * p.top, [&](int r, uint64_t key) {
       if (blocks == 1)
         write_top(p, row, r, key, normalizer);
       else
@@ -655,10 +659,10 @@ scores_kernel(const __grid_constant__ Scores p) {
     if (threadIdx.x == 0) write_scores(p, row, sums, chosen);
     if (p.top > 0) {
       const float normalizer = normalizer_of(sums);
-      for (int i = threadIdx.x; i < blocks * p.top; i += kStride)
-        bests[0].keys[i] = cluster.map_shared_rank(top_of_block, i / p.top)[i % p.top];
-      __syncthreads();
-      rank_all(blocks, [&](int i) { return bests[0].keys[i]; }, [&](int r, uint64_t key) { write_top(p, row, r, key, normalizer); });
+      for (int i = threadIdx.x; i < 8 * kMostTop; i += kStride)
+        if (i / kMostTop < blocks && i % kMostTop < p.top)
+          lists[i / kMostTop * p.top + i % kMostTop] = cluster.map_shared_rank(top_of_block, i / kMostTop)[i % kMostTop];
+      rank_all(blocks * p.top, [&](int r, uint64_t key) { write_top(p, row, r, key, normalizer); });
     }
   }
   cluster.sync();  // no block ends while its shared memory is read
@@ -747,12 +751,18 @@ __global__ void __launch_bounds__(256) few_scores_grad_kernel(const __grid_const
   }
 }
 
-// A warp a run of kRun vectors of a row of the gradient, on its 16-byte boundaries. kAlike: the logits' rows lie on the
-// boundaries as the gradient's do.
-constexpr int kRun = 128;
-template <typename T, bool kAlike>
-__global__ void __launch_bounds__(256) scores_grad_kernel(const __grid_constant__ ScoresGrad p, uint32_t runs) {
-  constexpr int kValues = Grid<T>::kValues, kVectors = kRun / 32;
+// A warp a run of a row of the gradient, kVectors a lane on 16-byte boundaries. kAlike: the logits' rows lie on the
+// boundaries as the gradient's do. What counts is bytes on their way: 4 vectors with 40 warps an SM (4,096 x 16,384 bf16 48
+// us; 2 vectors with 56 warps 51), with masks, whose bytes take registers too, 2 with 48 (4,096 x 32,771 120 us; 4 with 40
+// warps 139, 2 with 56 warps 143), and rows between the boundaries 2 with 56 (60 us; 4 with 40 warps 68).
+template <bool kAlike, bool kMasked>
+struct Run {
+  static constexpr int kVectors = kAlike && !kMasked ? 4 : 2, kBlocks = kMasked ? 6 : kAlike ? 5 : 7;  // of 8 warps, an SM's
+};
+template <typename T, bool kAlike, bool kMasked>
+__global__ void __launch_bounds__(256, Run<kAlike, kMasked>::kBlocks)
+scores_grad_kernel(const __grid_constant__ ScoresGrad p, uint32_t runs) {
+  constexpr int kValues = Grid<T>::kValues, kVectors = Run<kAlike, kMasked>::kVectors, kRun = 32 * kVectors;
   const uint32_t warp = blockIdx.x * 8 + threadIdx.x / 32, of_row = warp / runs;
   const int64_t row = of_row;
   if (row >= p.m) return;
@@ -773,7 +783,7 @@ __global__ void __launch_bounds__(256) scores_grad_kernel(const __grid_constant_
     if (inside) {
       const uint4 q = kAlike ? __ldg(reinterpret_cast<const uint4*>(logits + j0)) : words_between(logits, j0);
       w[r][0] = q.x, w[r][1] = q.y, w[r][2] = q.z, w[r][3] = q.w;
-      if (allowed) bytes[r] = bytes_at<kValues>(allowed, j0, p.v);
+      if (kMasked) bytes[r] = bytes_at<kValues>(allowed, j0, p.v);
     }
   }
   const RowGrad of(p, row);
@@ -784,7 +794,7 @@ __global__ void __launch_bounds__(256) scores_grad_kernel(const __grid_constant_
     const int64_t j0 = to.place(i);
     const bool whole = i >= first_whole && i < last_whole;
     if (whole && (kAlike || (j0 > 0 && j0 + kValues < p.v))) {
-      if (allowed) cut_out<T>(w[r], bytes[r]);
+      if (kMasked) cut_out<T>(w[r], bytes[r]);
     } else {
       const uint4 q = edge_vector(logits, allowed, p.v, j0);
       w[r][0] = q.x, w[r][1] = q.y, w[r][2] = q.z, w[r][3] = q.w;
@@ -857,12 +867,13 @@ int scores_of(const Scores& p, cudaStream_t s) {
   if (p.v <= 4 * kEach) return few_scores<T, 4>(p, s);
   if (p.v <= 8 * kEach) return few_scores<T, 8>(p, s);
   if (p.v <= 32 * kEach) return few_scores<T, 32>(p, s);
-  // As few warps a row as fill the GPU, 16 an SM, with a vector a lane at least.
+  // As few warps a row as fill the GPU, 16 an SM, with a vector a lane at least; of few rows a cluster of blocks that have a
+  // turn each (one row of 50,021 bf16 5.0 us, one block 6.7; 20 of 30,000 float32 8.2, with a vector a thread 11.0).
   const int64_t vectors = p.v / kValues, enough = 16 * 148;
   if (p.m >= enough || vectors <= 64) return scores<T, 1>(p, 1, s);
   if (p.m * 4 >= enough || vectors <= 256) return scores<T, 4>(p, 1, s);
   int blocks = 1;
-  while (blocks < 8 && p.m * 16 * blocks < enough && vectors > 512 * blocks) blocks *= 2;
+  while (blocks < 8 && p.m * 16 * blocks < enough && vectors > 2048 * blocks) blocks *= 2;
   return scores<T, 16>(p, blocks, s);
 }
 
@@ -883,14 +894,23 @@ int scores_grad_of(const ScoresGrad& p, cudaStream_t s) {
   } else if (p.v <= 32 * kEach) {
     few(std::integral_constant<int, 32>());
   } else {
-    const int64_t vectors = (p.v + 2 * kValues - 2) / kValues, runs = (vectors + kRun - 1) / kRun;
+    const int64_t vectors = (p.v + 2 * kValues - 2) / kValues;
     const bool alike = p.stride % kValues == p.v % kValues && reinterpret_cast<uintptr_t>(p.logits) % 16 ==
                        reinterpret_cast<uintptr_t>(p.grad) % 16;
-    const unsigned grid = unsigned((p.m * runs + 7) / 8);
-    if (alike)
-      scores_grad_kernel<T, true><<<grid, 256, 0, s>>>(p, uint32_t(runs));
+    const auto run = [&](auto is_alike, auto is_masked) {
+      constexpr bool kAlike = decltype(is_alike)::value, kMasked = decltype(is_masked)::value;
+      constexpr int kRun = 32 * Run<kAlike, kMasked>::kVectors;
+      const int64_t runs = (vectors + kRun - 1) / kRun;
+      scores_grad_kernel<T, kAlike, kMasked><<<unsigned((p.m * runs + 7) / 8), 256, 0, s>>>(p, uint32_t(runs));
+    };
+    if (alike && p.allowed)
+      run(std::true_type(), std::true_type());
+    else if (alike)
+      run(std::true_type(), std::false_type());
+    else if (p.allowed)
+      run(std::false_type(), std::true_type());
     else
-      scores_grad_kernel<T, false><<<grid, 256, 0, s>>>(p, uint32_t(runs));
+      run(std::false_type(), std::false_type());
   }
   return launch_status();
 }
