@@ -107,6 +107,16 @@ RLENV_D void copy_tile(uint32_t to, const CUtensorMap* map, uint32_t cluster_bar
       "l"(map), "r"(cluster_bar), "r"(x), "r"(y), "r"(z)
       : "memory");
 }
+// Back from shared memory: what a thread has written there is fenced for the copy, a thread issues it and closes a group,
+// and waits until its groups have read what they copy, or written it.
+RLENV_D void fence_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+RLENV_D void store_tile(const CUtensorMap* map, uint32_t from, int x, int y) {
+  asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%2, %3}], [%1];" ::"l"(map), "r"(from), "r"(x), "r"(y)
+               : "memory");
+}
+RLENV_D void store_commit() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
+RLENV_D void store_wait_read() { asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); }
+RLENV_D void store_wait() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
 RLENV_D uint32_t cluster_rank() {
   uint32_t r;
   asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
@@ -279,6 +289,19 @@ inline int tile_map(CUtensorMap* map, const void* base, int64_t cols, int64_t ro
   const CUresult rc = encode(map, bytes ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(base), dims, strides, box,
                              steps, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
                              CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return rc == CUDA_SUCCESS ? 0 : int(cudaErrorInvalidValue);
+}
+
+// A dense (rows, cols) result of bfloat16 or float32, written in boxes of 32 rows of 128 bytes; what lies past its ends is
+// not written.
+inline int result_map(CUtensorMap* map, void* base, int64_t cols, int64_t rows, bool floats) {
+  const EncodeTiled encode = encode_tiled();
+  if (!encode) return int(cudaErrorNotSupported);
+  const cuuint64_t dims[2] = {cuuint64_t(cols), cuuint64_t(rows)}, strides[1] = {cuuint64_t(cols) * (floats ? 4 : 2)};
+  const cuuint32_t box[2] = {floats ? 32u : 64u, 32}, steps[2] = {1, 1};
+  const CUresult rc = encode(map, floats ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, base, dims,
+                             strides, box, steps, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                             CU_TENSOR_MAP_L2_PROMOTION_NONE, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   return rc == CUDA_SUCCESS ? 0 : int(cudaErrorInvalidValue);
 }
 

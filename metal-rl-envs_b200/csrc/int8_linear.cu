@@ -60,24 +60,31 @@ __global__ void __launch_bounds__(256) few_rows_kernel(const __grid_constant__ I
 // ---- many rows: tensor cores ---------------------------------------------------------------------------
 //
 // Pairs of SMs (tcgen05, cta_group::2) multiply tiles of 256 channels by kTokens tokens, 128 terms a step: a tensor copy's
-// row of 128 bytes is a step of a row. Channels are the accumulator's lanes and tokens its columns, so that a warp's lanes
-// hold neighbouring channels of a token and store them as they are, wherever a row of the result starts.
+// row of 128 bytes is a step of a row. Two forms:
+// - channels are the accumulator's lanes and tokens its columns: a warp's lanes hold neighbouring channels of a token and
+//   store them as they are, wherever a row of the result starts. Tiles of few tokens are possible.
+// - kWide: tokens are its lanes, 256 of them, and channels its columns: a lane holds neighbouring channels of its token,
+//   and a warp's 32 rows of 128 bytes go out through shared memory as one tensor copy. For rows of the result on 16-byte
+//   boundaries. An element costs 3 instructions instead of 7 (8,192 x 256 x 4,096 bf16, all epilogue: 35 us with the other).
 
 constexpr int kChannelsEach = 128, kStepBytes = 128;  // of a tile, in each block of a pair
-template <int kTokens>
+template <int kTokens, bool kWide>
 struct Int8Tile {
-  static constexpr int kHalf = kTokens / 2;  // tokens whose rows each block copies
+  static_assert(!kWide || kTokens == 256, "wide tiles are 256 x 256");
+  static constexpr int kHalf = kTokens / 2;  // rows of the second operand that each block copies
   static constexpr int kABytes = kChannelsEach * kStepBytes, kRingBytes = kABytes + kHalf * kStepBytes;
-  static constexpr int kStages = 6 * 32768 / kRingBytes < 10 ? 6 * 32768 / kRingBytes : 10;
-  static constexpr int kEpilogue = kTokens >= 64 ? 8 : 4;         // warps
+  static constexpr int kStages = kWide ? 4 : 6 * 32768 / kRingBytes < 10 ? 6 * 32768 / kRingBytes : 10;
+  static constexpr int kEpilogue = kTokens >= 128 ? 16 : kTokens >= 64 ? 8 : 4;  // warps
   static constexpr int kMine = kTokens / (kEpilogue / 4);         // columns of a thread
   static constexpr int kThreads = 128 + 32 * kEpilogue;
   static constexpr int kColumns = 2 * kTokens;                    // two accumulators
-  static constexpr int kSmem = kStages * kRingBytes + 1024;       // the ring starts on a 1,024-byte boundary
+  static constexpr int kStageBytes = kWide ? 32 * 128 : 0;        // of a warp, for its rows' way out
+  // the ring starts on a 1,024-byte boundary
+  static constexpr int kSmem = kStages * kRingBytes + kEpilogue * kStageBytes + 1024;
 };
 
 struct alignas(64) Int8Tiles {
-  CUtensorMap a, w;
+  CUtensorMap a, w, result;  // result: wide tiles only
   int64_t m, f;
   const float *a_scale, *w_scale;
   void* out;
@@ -102,16 +109,16 @@ struct Int8Work {
   }
 };
 
-template <typename T, int kTokens>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Int8Tile<kTokens>::kThreads, 1)
+template <typename T, int kTokens, bool kWide>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Int8Tile<kTokens, kWide>::kThreads, 1)
 tile_kernel(const __grid_constant__ Int8Tiles p, int items) {
-  using C = Int8Tile<kTokens>;
+  using C = Int8Tile<kTokens, kWide>;
   extern __shared__ unsigned char raw[];
   __shared__ __align__(8) uint64_t bars[2 * C::kStages + 5];
   __shared__ uint32_t tmem_slot;
   __shared__ int dead_flag;
   __shared__ bw::Ending endings[2];  // of the pair's first block, and of its second
-  __shared__ __align__(16) float scales[C::kEpilogue][32];
+  __shared__ __align__(16) float scales[C::kEpilogue][kWide ? 64 : 32];
   volatile int* const dead = &dead_flag;
   const uint32_t ring = (bw::shared_at(raw) + 1023) & ~1023u;
   const uint32_t full = bw::shared_at(bars), empty = full + 8 * C::kStages;
@@ -133,22 +140,24 @@ tile_kernel(const __grid_constant__ Int8Tiles p, int items) {
   const uint32_t tmem = __shfl_sync(0xffffffffu, tmem_slot, 0);
 
   if (warp == 0) {
-    // Both blocks copy their channels and their half of the tokens; all bytes count at the first block's barrier.
+    // Both blocks copy their half of the lanes' rows and of the columns'; all bytes count at the first block's barrier.
     int stage = 0, filled = 0;
     uint32_t phase = 0;
     bool ok = true;
     const uint32_t full_at = bw::in_block(full, 0);
     for (int item = blockIdx.x / 2; item < items && ok; item += pairs) {
       const Int8Work w(p, item);
-      const int channel = (2 * w.channel + rank) * kChannelsEach, token = w.token * kTokens + rank * C::kHalf;
+      const CUtensorMap *const lanes = kWide ? &p.a : &p.w, *const columns = kWide ? &p.w : &p.a;
+      const int lane0 = (2 * (kWide ? w.token : w.channel) + rank) * kChannelsEach,
+                column0 = (kWide ? w.channel : w.token) * kTokens + rank * C::kHalf;
       for (int it = 0; it < w.steps; ++it) {
         const int k = (w.k0 + it) * kStepBytes;
         const uint32_t bar = full_at + 8 * stage, a = ring + stage * C::kRingBytes;
         if (!(ok = bw::barrier_wait_warp(empty + 8 * stage, phase ^ 1, dead))) break;
         if (bw::elect()) {
           if (rank == 0) bw::barrier_expect(full + 8 * stage, 2 * C::kRingBytes);
-          bw::copy_tile(a, &p.w, bar, k, channel, 0);
-          bw::copy_tile(a + C::kABytes, &p.a, bar, k, token, 0);
+          bw::copy_tile(a, lanes, bar, k, lane0, 0);
+          bw::copy_tile(a + C::kABytes, columns, bar, k, column0, 0);
         }
         ++filled;
         if (++stage == C::kStages) stage = 0, phase ^= 1;
@@ -190,53 +199,105 @@ tile_kernel(const __grid_constant__ Int8Tiles p, int items) {
   } else if (warp >= 4) {
     const int quarter = warp & 3, part = (warp - 4) >> 2;
     float* const own_scales = scales[warp - 4];
+    unsigned char* const own_stage = raw + (ring - bw::shared_at(raw)) + C::kStages * C::kRingBytes + (warp - 4) * C::kStageBytes;
     int buffer = 0;
     uint32_t buffer_phase = 0;
     bool ok = true;
     const uint32_t taken_at = bw::in_block(taken, 0), lanes = uint32_t(32 * quarter) << 16;
     for (int item = blockIdx.x / 2; item < items; item += pairs) {
       const Int8Work w(p, item);
-      const int64_t channel = int64_t(2 * w.channel + rank) * kChannelsEach + 32 * quarter + lane;
-      const bool there = channel < p.f;
-      const float w_scale = there && p.splits == 1 ? __ldg(p.w_scale + channel) : 0.0f;
-      ok = ok && bw::barrier_wait_warp(summed + 8 * buffer, buffer_phase, dead);
-      bw::fence_after();
+      if constexpr (kWide) {
+        constexpr int kValues = 128 / int(sizeof(T));  // of a row in a copy
+        const int64_t token = int64_t(2 * w.token + rank) * kChannelsEach + 32 * quarter;
+        const int64_t channel0 = int64_t(w.channel) * kTokens + part * C::kMine;
+        float a_scale = token + lane < p.m ? __ldg(p.a_scale + token + lane) : 0.0f;
 #pragma unroll
-      for (int run = 0; run < C::kMine / 32; ++run) {
-        const int column = part * C::kMine + 32 * run;
-        const int64_t t0 = int64_t(w.token) * kTokens + column;
-        const int count = int(min(int64_t(32), p.m - t0));
-        if (count <= 0) break;
-        uint32_t v[32];
-        const uint32_t at = tmem + lanes + buffer * kTokens + column;
-        bw::tmem_load16x2(v, at, at + 16);
+        for (int i = 0; i < C::kMine; i += 32)
+          own_scales[i + lane] = channel0 + i + lane < p.f ? __ldg(p.w_scale + channel0 + i + lane) : 0.0f;
+        ok = ok && bw::barrier_wait_warp(summed + 8 * buffer, buffer_phase, dead);
+        if (!ok) a_scale = __uint_as_float(0x7fffffffu);
+        bw::fence_after();
         __syncwarp();
-        own_scales[lane] = !ok ? __uint_as_float(0x7fffffffu) : lane < count ? __ldg(p.a_scale + t0 + lane) : 0.0f;
-        __syncwarp();
-        bw::tmem_ready(v);
-        if (p.splits == 1) {
-          T* const to = static_cast<T*>(p.out) + t0 * p.f + channel;
+        const uint64_t of_row = pair_of(a_scale, a_scale);
 #pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const float4 s = reinterpret_cast<const float4*>(own_scales)[i];
-            const float of[4] = {s.x, s.y, s.z, s.w};
+        for (int run = 0; run < C::kMine / 32; ++run) {
+          const uint32_t at = tmem + lanes + buffer * kTokens + part * C::kMine + 32 * run;
+          uint32_t v[32];
+          bw::tmem_load16x2(v, at, at + 16);
+          bw::tmem_ready(v);
+          if (32 * run % kValues == 0) bw::store_wait_read();  // the last copy has read its rows
+          __syncwarp();
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
-              if (there && 4 * i + j < count) put(to + (4 * i + j) * p.f, float(int(v[4 * i + j])) * of[j] * w_scale);
+          for (int i = 0; i < 32; i += 16 / int(sizeof(T))) {  // 16 bytes of a row
+            uint32_t out[4];
+#pragma unroll
+            for (int j = 0; j < 16 / int(sizeof(T)); j += 2) {
+              const float2 s = *reinterpret_cast<const float2*>(own_scales + 32 * run + i + j);
+              const float2 x = values_of(multiply_pairs(
+                  multiply_pairs(pair_of(float(int(v[i + j])), float(int(v[i + j + 1]))), of_row), pair_of(s.x, s.y)));
+              if constexpr (sizeof(T) == 4) {
+                out[j] = __float_as_uint(x.x), out[j + 1] = __float_as_uint(x.y);
+              } else {
+                const __nv_bfloat162 pair = __floats2bfloat162_rn(x.x, x.y);
+                out[j / 2] = *reinterpret_cast<const uint32_t*>(&pair);
+              }
+            }
+            // 16-byte pieces of a row are exchanged by the row's low three bits, as the copy takes them
+            const int piece = (32 * run % kValues + i) * int(sizeof(T)) / 16;
+            *reinterpret_cast<uint4*>(own_stage + lane * 128 + ((piece ^ (lane & 7)) << 4)) = make_uint4(out[0], out[1], out[2], out[3]);
           }
-        } else {
-          int* const to = p.parts + (int64_t(w.split) * p.m + t0) * p.f + channel;
-#pragma unroll
-          for (int i = 0; i < 32; ++i)
-            if (there && i < count) to[i * p.f] = ok ? int(v[i]) : kLost;
+          if ((32 * run + 32) % kValues == 0) {
+            bw::fence_async();
+            __syncwarp();
+            const int64_t channel = channel0 + 32 * run + 32 - kValues;
+            if (lane == 0 && token < p.m && channel < p.f) bw::store_tile(&p.result, bw::shared_at(own_stage), int(channel), int(token));
+            bw::store_commit();
+          }
         }
-        __syncwarp();
+      } else {
+        const int64_t channel = int64_t(2 * w.channel + rank) * kChannelsEach + 32 * quarter + lane;
+        const bool there = channel < p.f;
+        const float w_scale = there && p.splits == 1 ? __ldg(p.w_scale + channel) : 0.0f;
+        ok = ok && bw::barrier_wait_warp(summed + 8 * buffer, buffer_phase, dead);
+        bw::fence_after();
+#pragma unroll
+        for (int run = 0; run < C::kMine / 32; ++run) {
+          const int column = part * C::kMine + 32 * run;
+          const int64_t t0 = int64_t(w.token) * kTokens + column;
+          const int count = int(min(int64_t(32), p.m - t0));
+          if (count <= 0) break;
+          uint32_t v[32];
+          const uint32_t at = tmem + lanes + buffer * kTokens + column;
+          bw::tmem_load16x2(v, at, at + 16);
+          __syncwarp();
+          own_scales[lane] = !ok ? __uint_as_float(0x7fffffffu) : lane < count ? __ldg(p.a_scale + t0 + lane) : 0.0f;
+          __syncwarp();
+          bw::tmem_ready(v);
+          if (p.splits == 1) {
+            T* const to = static_cast<T*>(p.out) + t0 * p.f + channel;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              const float4 s = reinterpret_cast<const float4*>(own_scales)[i];
+              const float of[4] = {s.x, s.y, s.z, s.w};
+#pragma unroll
+              for (int j = 0; j < 4; ++j)
+                if (there && 4 * i + j < count) put(to + (4 * i + j) * p.f, float(int(v[4 * i + j])) * of[j] * w_scale);
+            }
+          } else {
+            int* const to = p.parts + (int64_t(w.split) * p.m + t0) * p.f + channel;
+#pragma unroll
+            for (int i = 0; i < 32; ++i)
+              if (there && i < count) to[i * p.f] = ok ? int(v[i]) : kLost;
+          }
+          __syncwarp();
+        }
       }
       bw::fence_before();
       __syncwarp();
       if (ok && lane == 0) bw::barrier_arrive(taken_at + 8 * buffer);
       if (++buffer == 2) buffer = 0, buffer_phase ^= 1;
     }
+    if constexpr (kWide) bw::store_wait();
   }
   __syncwarp();
   bw::fence_before();
@@ -299,9 +360,9 @@ Cut cut_of(int64_t m, int64_t k, int64_t f) {
   return best;
 }
 
-template <typename T, int kTokens>
+template <typename T, int kTokens, bool kWide = false>
 int tiles(const Int8Product& q, int splits, void* scratch, cudaStream_t s) {
-  using C = Int8Tile<kTokens>;
+  using C = Int8Tile<kTokens, kWide>;
   Int8Tiles p{};
   p.m = q.m, p.f = q.f, p.a_scale = q.a_scale, p.w_scale = q.w_scale, p.out = q.out;
   p.splits = splits, p.parts = splits > 1 ? static_cast<int*>(scratch) : nullptr;
@@ -311,13 +372,15 @@ int tiles(const Int8Product& q, int splits, void* scratch, cudaStream_t s) {
   p.steps = int(tiles_of(q.k, kStepBytes)), p.split_steps = int(tiles_of(p.steps, splits));
   if (const int rc = bw::tile_map(&p.a, q.a, q.k, q.m, 1, q.a_pitch, C::kHalf, true)) return rc;
   if (const int rc = bw::tile_map(&p.w, q.w, q.k, q.f, 1, q.w_pitch, kChannelsEach, true)) return rc;
+  if constexpr (kWide)
+    if (const int rc = bw::result_map(&p.result, q.out, q.f, q.m, sizeof(T) == 4)) return rc;
   int dev = 0, sms = 0;
   if (cudaError_t e = cudaGetDevice(&dev)) return int(e);
   if (cudaError_t e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev)) return int(e);
-  if (cudaError_t e = cudaFuncSetAttribute(tile_kernel<T, kTokens>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem))
+  if (cudaError_t e = cudaFuncSetAttribute(tile_kernel<T, kTokens, kWide>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem))
     return int(e);
   const int grid = 2 * int(items < sms / 2 ? items : sms / 2);
-  tile_kernel<T, kTokens><<<grid, C::kThreads, C::kSmem, s>>>(p, int(items));
+  tile_kernel<T, kTokens, kWide><<<grid, C::kThreads, C::kSmem, s>>>(p, int(items));
   if (const int rc = launch_status(); rc || splits == 1) return rc;
   add_parts_kernel<T><<<grid_for(q.m * q.f, 256), 256, 0, s>>>(p.parts, splits, q.m, q.f, q.a_scale, q.w_scale,
                                                                static_cast<T*>(q.out));
@@ -327,6 +390,8 @@ int tiles(const Int8Product& q, int splits, void* scratch, cudaStream_t s) {
 template <typename T>
 int product(const Int8Product& p, void* scratch, cudaStream_t s) {
   const Cut cut = cut_of(p.m, p.k, p.f);
+  const bool on_lines = p.f * sizeof(T) % 16 == 0 && reinterpret_cast<uintptr_t>(p.out) % 16 == 0;
+  if (cut.tokens == 256 && cut.splits == 1 && on_lines) return tiles<T, 256, true>(p, 1, scratch, s);
   if (cut.tokens == 256) return tiles<T, 256>(p, cut.splits, scratch, s);
   if (cut.tokens == 128) return tiles<T, 128>(p, cut.splits, scratch, s);
   if (cut.tokens == 64) return tiles<T, 64>(p, cut.splits, scratch, s);
