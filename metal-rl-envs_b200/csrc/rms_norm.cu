@@ -23,7 +23,9 @@ struct Vec {
   static constexpr int kValues = kWide ? 16 / int(sizeof(T)) : 1;
 };
 
-// A vector as it lies in memory, and its values. Rows wait in registers in this form: half the room for bfloat16.
+// A vector as it lies in memory, and its values. Rows wait in registers in this form: half the room for bfloat16, and
+// nothing that waits for a load while others are to be issued (bfloat16 rows of 333 by single values, the gradient of
+// 100,000: 658 us when each was converted as it came).
 template <typename T, bool kWide>
 struct Raw {
   uint4 bits;
@@ -40,15 +42,19 @@ struct Raw {
     }
   }
 };
-template <typename T>
-struct Raw<T, false> {
-  float value;
-  RLENV_D void load(const float* from) { value = __ldg(from); }
-  RLENV_D void load(const __nv_bfloat16* from) {
-    value = __uint_as_float(uint32_t(__ldg(reinterpret_cast<const unsigned short*>(from))) << 16);
-  }
-  RLENV_D void clear() { value = 0.0f; }
-  RLENV_D void values(float (&v)[1]) const { v[0] = value; }
+template <>
+struct Raw<float, false> {
+  float bits;
+  RLENV_D void load(const float* from) { bits = __ldg(from); }
+  RLENV_D void clear() { bits = 0.0f; }
+  RLENV_D void values(float (&v)[1]) const { v[0] = bits; }
+};
+template <>
+struct Raw<__nv_bfloat16, false> {
+  unsigned short bits;
+  RLENV_D void load(const __nv_bfloat16* from) { bits = __ldg(reinterpret_cast<const unsigned short*>(from)); }
+  RLENV_D void clear() { bits = 0; }
+  RLENV_D void values(float (&v)[1]) const { v[0] = __uint_as_float(uint32_t(bits) << 16); }
 };
 template <typename T, int kValues>
 RLENV_D void load(const T* from, float (&v)[kValues]) {
@@ -93,44 +99,54 @@ RLENV_D void store_codes(int8_t* to, const float (&v)[kValues]) {
   }
 }
 
-// The threads that share a row: a warp (several rows a block), or a block.
+// The threads that share a row: some of a warp, a warp, some warps of a block, or a block.
 template <int kThreads>
 struct Team {
-  static constexpr int kBlock = kThreads == 32 ? 256 : kThreads;  // threads of a block
+  static constexpr int kBlock = kThreads < 256 ? 256 : kThreads;  // threads of a block
   static constexpr int kRows = kBlock / kThreads;                 // rows it works on at a time
-  static constexpr int kWarps = kThreads / 32;
+  static constexpr int kWarps = kThreads < 32 ? 1 : kThreads / 32;
+  static constexpr int kSpan = kThreads < 32 ? kThreads : 32;     // its lanes in a warp
 
-  // The sum over the team of each of kN values, in a fixed order; `room` holds kN kWarps of them.
+  static RLENV_D void sync() {  // of more than a warp
+    if constexpr (kRows == 1)
+      __syncthreads();
+    else
+      asm volatile("bar.sync %0, %1;" ::"r"(int(threadIdx.x) / kThreads + 1), "n"(kThreads) : "memory");
+  }
+  // The sum over the team of each of kN values, in a fixed order; `room` holds kN kWarps of them for each team.
   template <int kN>
   static RLENV_D void sum(float (&v)[kN], float* room) {
 #pragma unroll
     for (int i = 0; i < kN; ++i)
 #pragma unroll
-      for (int d = 16; d > 0; d /= 2) v[i] += __shfl_xor_sync(0xffffffffu, v[i], d);
+      for (int d = kSpan / 2; d > 0; d /= 2) v[i] += __shfl_xor_sync(0xffffffffu, v[i], d);
     if constexpr (kWarps > 1) {
-      const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-      __syncthreads();  // the room's last values are read
+      room += threadIdx.x / kThreads * (kN * kWarps);
+      const int warp = threadIdx.x % kThreads / 32, lane = threadIdx.x % 32;
+      sync();  // the room's last values are read
       if (lane == 0)
 #pragma unroll
         for (int i = 0; i < kN; ++i) room[i * kWarps + warp] = v[i];
-      __syncthreads();
+      sync();
 #pragma unroll
       for (int i = 0; i < kN; ++i) {
-        v[i] = lane < kWarps ? room[i * kWarps + lane] : 0.0f;
+        v[i] = room[i * kWarps + lane % kWarps];
 #pragma unroll
-        for (int d = 16; d > 0; d /= 2) v[i] += __shfl_xor_sync(0xffffffffu, v[i], d);
+        for (int d = kWarps / 2; d > 0; d /= 2) v[i] += __shfl_xor_sync(0xffffffffu, v[i], d);
       }
     }
   }
   // The largest of the team's whole numbers.
   static RLENV_D uint32_t largest(uint32_t v, uint32_t* room) {
-    v = __reduce_max_sync(0xffffffffu, v);
+#pragma unroll
+    for (int d = kSpan / 2; d > 0; d /= 2) v = max(v, __shfl_xor_sync(0xffffffffu, v, d));
     if constexpr (kWarps > 1) {
-      const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-      __syncthreads();
+      room += threadIdx.x / kThreads * kWarps;
+      const int warp = threadIdx.x % kThreads / 32, lane = threadIdx.x % 32;
+      sync();
       if (lane == 0) room[warp] = v;
-      __syncthreads();
-      v = __reduce_max_sync(0xffffffffu, lane < kWarps ? room[lane] : 0u);
+      sync();
+      v = __reduce_max_sync(0xffffffffu, room[lane % kWarps]);
     }
     return v;
   }
@@ -156,92 +172,88 @@ template <typename T, bool kWide, int kThreads, int kVectors, bool kCodes>
 __global__ void __launch_bounds__(Team<kThreads>::kBlock) norm_kernel(const __grid_constant__ Norm p) {
   using G = Team<kThreads>;
   constexpr int kN = Vec<T, kWide>::kValues;
-  __shared__ float room[G::kWarps];
-  const int at = threadIdx.x % kThreads;
+  __shared__ float room[G::kWarps * G::kRows];
+  const int at = threadIdx.x % kThreads, k = int(p.k);
   const int64_t row = int64_t(blockIdx.x) * G::kRows + threadIdx.x / kThreads;
-  if (row >= p.m) return;  // a warp, or the whole block
+  const bool there = row < p.m;
   const T *x = static_cast<const T*>(p.x) + row * p.x_stride,
           *residual = p.residual ? static_cast<const T*>(p.residual) + row * p.residual_stride : nullptr,
           *weight = static_cast<const T*>(p.weight);
+  const auto column = [&](int i) { return (at + i * kThreads) * kN; };
+  const auto in = [&](int i) { return there && column(i) < k; };
   float t[kVectors][kN];
+  Raw<T, kWide> from[kVectors], other[kVectors];
 #pragma unroll
   for (int i = 0; i < kVectors; ++i) {
-    const int64_t c = int64_t(at + i * kThreads) * kN;
-    if (c < p.k) {
-      load(x + c, t[i]);
-    } else {
-#pragma unroll
-      for (int j = 0; j < kN; ++j) t[i][j] = 0.0f;
-    }
+    from[i].clear();
+    if (in(i)) from[i].load(x + column(i));
   }
   if (residual) {
 #pragma unroll
     for (int i = 0; i < kVectors; ++i) {
-      const int64_t c = int64_t(at + i * kThreads) * kN;
-      if (c < p.k) {
-        float y[kN];
-        load(residual + c, y);
-#pragma unroll
-        for (int j = 0; j < kN; ++j) t[i][j] += y[j];
-      }
+      other[i].clear();
+      if (in(i)) other[i].load(residual + column(i));
     }
   }
   float sum[1] = {0.0f};
 #pragma unroll
-  for (int i = 0; i < kVectors; ++i)
+  for (int i = 0; i < kVectors; ++i) {
+    from[i].values(t[i]);
+    if (residual) {
+      float y[kN];
+      other[i].values(y);
+#pragma unroll
+      for (int j = 0; j < kN; ++j) t[i][j] += y[j];
+    }
 #pragma unroll
     for (int j = 0; j < kN; ++j) sum[0] = fmaf(t[i][j], t[i][j], sum[0]);
+  }
+  if (weight) {  // on its way while the sum is formed
+#pragma unroll
+    for (int i = 0; i < kVectors; ++i)
+      if (column(i) < k) other[i].load(weight + column(i));
+  }
   if (p.total) {
     T* const total = static_cast<T*>(p.total) + row * p.k;
 #pragma unroll
-    for (int i = 0; i < kVectors; ++i) {
-      const int64_t c = int64_t(at + i * kThreads) * kN;
-      if (c < p.k) store(total + c, t[i]);
-    }
+    for (int i = 0; i < kVectors; ++i)
+      if (in(i)) store(total + column(i), t[i]);
   }
   float r = 1.0f;
   if (!kCodes || p.normalise) {
     G::sum(sum, room);
-    r = rsqrtf(sum[0] / float(p.k) + p.eps);
+    r = rsqrtf(sum[0] / float(k) + p.eps);
   }
 #pragma unroll
   for (int i = 0; i < kVectors; ++i) {
-    const int64_t c = int64_t(at + i * kThreads) * kN;
-    if (c < p.k) {
-      float w[kN];
-      if (weight) load(weight + c, w);
+    float w[kN];
+    if (weight && column(i) < k) other[i].values(w);
 #pragma unroll
-      for (int j = 0; j < kN; ++j) t[i][j] = weight ? t[i][j] * r * w[j] : t[i][j] * r;
-    }
+    for (int j = 0; j < kN; ++j) t[i][j] = weight && column(i) < k ? t[i][j] * r * w[j] : t[i][j] * r;
   }
   if constexpr (!kCodes) {
     T* const out = static_cast<T*>(p.out) + row * p.k;
 #pragma unroll
-    for (int i = 0; i < kVectors; ++i) {
-      const int64_t c = int64_t(at + i * kThreads) * kN;
-      if (c < p.k) store(out + c, t[i]);
-    }
+    for (int i = 0; i < kVectors; ++i)
+      if (in(i)) store(out + column(i), t[i]);
   } else {
     // As bits, magnitudes are ordered with infinity and NaN above all numbers.
     uint32_t most = 0;
 #pragma unroll
     for (int i = 0; i < kVectors; ++i)
 #pragma unroll
-      for (int j = 0; j < kN; ++j) most = max(most, __float_as_uint(t[i][j]) & 0x7fffffffu);
+      for (int j = 0; j < kN; ++j) most = max(most, in(i) ? __float_as_uint(t[i][j]) & 0x7fffffffu : 0u);
     most = G::largest(most, reinterpret_cast<uint32_t*>(room));
     const float top = __uint_as_float(most);
     const bool some = top >= kTiny && most < 0x7f800000u;
     const float to_codes = some ? 127.0f / top : 0.0f;
-    if (at == 0) p.scale[row] = some ? top / 127.0f : top < kTiny ? 0.0f : __uint_as_float(0x7fffffffu);
+    if (at == 0 && there) p.scale[row] = some ? top / 127.0f : top < kTiny ? 0.0f : __uint_as_float(0x7fffffffu);
     int8_t* const codes = p.codes + row * p.pitch;
 #pragma unroll
     for (int i = 0; i < kVectors; ++i) {
-      const int64_t c = int64_t(at + i * kThreads) * kN;
-      if (c < p.k) {
 #pragma unroll
-        for (int j = 0; j < kN; ++j) t[i][j] = some ? t[i][j] * to_codes : 0.0f;
-        store_codes(codes + c, t[i]);
-      }
+      for (int j = 0; j < kN; ++j) t[i][j] = some ? t[i][j] * to_codes : 0.0f;
+      if (in(i)) store_codes(codes + column(i), t[i]);
     }
   }
 }
@@ -313,19 +325,22 @@ struct NormGrad {
   float* parts;  // (blocks, K): each block's sums over its rows of the weight's gradient; null: none asked for
 };
 
+// A team's next row is on its way while it works on one (kAhead: where registers allow).
 template <typename T, bool kWide, int kThreads, int kVectors>
 __global__ void __launch_bounds__(Team<kThreads>::kBlock) norm_grad_kernel(const __grid_constant__ NormGrad p) {
   using G = Team<kThreads>;
+  using R = Raw<T, kWide>;
   constexpr int kN = Vec<T, kWide>::kValues;
-  __shared__ float room[2 * G::kWarps];
-  const int at = threadIdx.x % kThreads;
-  const auto column = [&](int i) { return int64_t(at + i * kThreads) * kN; };
+  constexpr bool kAhead = kVectors * int(sizeof(R)) <= 32;
+  __shared__ float room[2 * G::kWarps * G::kRows];
+  const int at = threadIdx.x % kThreads, k = int(p.k);
+  const auto column = [&](int i) { return (at + i * kThreads) * kN; };
   float dw[kVectors][kN];
-  Raw<T, kWide> w[kVectors];
+  R w[kVectors];
 #pragma unroll
   for (int i = 0; i < kVectors; ++i) {
     w[i].clear();
-    if (p.weight && column(i) < p.k) w[i].load(static_cast<const T*>(p.weight) + column(i));
+    if (p.weight && column(i) < k) w[i].load(static_cast<const T*>(p.weight) + column(i));
 #pragma unroll
     for (int j = 0; j < kN; ++j) dw[i][j] = 0.0f;
   }
@@ -336,19 +351,32 @@ __global__ void __launch_bounds__(Team<kThreads>::kBlock) norm_grad_kernel(const
 #pragma unroll
     for (int j = 0; j < kN; ++j) g[j] *= v[j];
   };
-  for (int64_t row = int64_t(blockIdx.x) * G::kRows + threadIdx.x / kThreads; row < p.m;
-       row += int64_t(gridDim.x) * G::kRows) {
+  R t[kVectors], g[kVectors], s[kVectors];
+  const auto load_row = [&](int64_t row, R (&t)[kVectors], R (&g)[kVectors], R (&s)[kVectors]) {
     const T *total = static_cast<const T*>(p.total) + row * p.total_stride,
-            *grad_out = static_cast<const T*>(p.grad_out) + row * p.grad_out_stride;
-    Raw<T, kWide> t[kVectors], g[kVectors], s[kVectors];
+            *grad_out = static_cast<const T*>(p.grad_out) + row * p.grad_out_stride,
+            *grad_total = static_cast<const T*>(p.grad_total) + row * p.grad_total_stride;
 #pragma unroll
     for (int i = 0; i < kVectors; ++i) {
       t[i].clear(), g[i].clear(), s[i].clear();
-      if (column(i) >= p.k) continue;
-      t[i].load(total + column(i));
-      g[i].load(grad_out + column(i));
-      if (p.grad_total) s[i].load(static_cast<const T*>(p.grad_total) + row * p.grad_total_stride + column(i));
+      if (row < p.m && column(i) < k) {
+        t[i].load(total + column(i));
+        g[i].load(grad_out + column(i));
+        if (p.grad_total) s[i].load(grad_total + column(i));
+      }
     }
+  };
+  const int64_t step = int64_t(gridDim.x) * G::kRows;
+  int64_t row = int64_t(blockIdx.x) * G::kRows + threadIdx.x / kThreads;
+  // A warp's teams make as many turns as its first.
+  const int64_t turns = (p.m - (int64_t(blockIdx.x) * G::kRows + threadIdx.x / 32 * 32 / kThreads) + step - 1) / step;
+  if (kAhead) load_row(row, t, g, s);
+  for (int64_t turn = 0; turn < turns; ++turn, row += step) {
+    R next_t[kVectors], next_g[kVectors], next_s[kVectors];
+    if (kAhead)
+      load_row(row + step, next_t, next_g, next_s);
+    else
+      load_row(row, t, g, s);
     float sums[2] = {0.0f, 0.0f};
 #pragma unroll
     for (int i = 0; i < kVectors; ++i) {
@@ -359,7 +387,7 @@ __global__ void __launch_bounds__(Team<kThreads>::kBlock) norm_grad_kernel(const
       for (int j = 0; j < kN; ++j) sums[0] = fmaf(tv[j], tv[j], sums[0]), sums[1] = fmaf(gv[j], tv[j], sums[1]);
     }
     G::sum(sums, room);
-    const float r = rsqrtf(sums[0] / float(p.k) + p.eps), along = r * (r * sums[1] / float(p.k));
+    const float r = rsqrtf(sums[0] / float(k) + p.eps), along = r * (r * sums[1] / float(k));
     T* const grad = static_cast<T*>(p.grad) + row * p.k;
 #pragma unroll
     for (int i = 0; i < kVectors; ++i) {
@@ -370,40 +398,42 @@ __global__ void __launch_bounds__(Team<kThreads>::kBlock) norm_grad_kernel(const
       weighed(i, gv);
 #pragma unroll
       for (int j = 0; j < kN; ++j) v[j] += r * (gv[j] - tv[j] * along);
-      if (column(i) < p.k) store(grad + column(i), v);
+      if (row < p.m && column(i) < k) store(grad + column(i), v);
+    }
+    if (kAhead) {
+#pragma unroll
+      for (int i = 0; i < kVectors; ++i) t[i] = next_t[i], g[i] = next_g[i], s[i] = next_s[i];
     }
   }
   if (!p.parts) return;
-  // A block's rows: its warps' sums one after the other.
+  // A block's sums: the teams' of a warp, then the warps' one after the other, those of the same columns.
+  if constexpr (kThreads < 32) {
+#pragma unroll
+    for (int i = 0; i < kVectors; ++i)
+#pragma unroll
+      for (int j = 0; j < kN; ++j)
+#pragma unroll
+        for (int d = kThreads; d < 32; d *= 2) dw[i][j] += __shfl_xor_sync(0xffffffffu, dw[i][j], d);
+  }
   extern __shared__ float shared_dw[];
-  if constexpr (G::kRows > 1) {
-    for (int w = 0; w < G::kRows; ++w) {
-      if (int(threadIdx.x) / kThreads == w) {
+  constexpr int kSets = kThreads < 32 ? G::kBlock / 32 : G::kRows;  // of threads that share columns
+  const int set = kThreads < 32 ? threadIdx.x / 32 : threadIdx.x / kThreads;
+  for (int n = 0; n < kSets; ++n) {
+    if (set == n && (kThreads >= 32 || threadIdx.x % 32 < kThreads)) {
 #pragma unroll
-        for (int i = 0; i < kVectors; ++i) {
-          const int64_t c = int64_t(at + i * kThreads) * kN;
+      for (int i = 0; i < kVectors; ++i) {
 #pragma unroll
-          for (int j = 0; j < kN; ++j) {
-            float* const to = shared_dw + (j * kVectors + i) * kThreads + at;
-            if (w > 0) dw[i][j] += *to;
-            if (w + 1 < G::kRows)
-              *to = dw[i][j];
-            else if (c < p.k)
-              p.parts[int64_t(blockIdx.x) * p.k + c + j] = dw[i][j];
-          }
+        for (int j = 0; j < kN; ++j) {
+          float* const to = shared_dw + (j * kVectors + i) * kThreads + at;
+          if (n > 0) dw[i][j] += *to;
+          if (n + 1 < kSets)
+            *to = dw[i][j];
+          else if (column(i) < k)
+            p.parts[int64_t(blockIdx.x) * p.k + column(i) + j] = dw[i][j];
         }
       }
-      __syncthreads();
     }
-  } else {
-#pragma unroll
-    for (int i = 0; i < kVectors; ++i) {
-      const int64_t c = int64_t(at + i * kThreads) * kN;
-      if (c < p.k) {
-#pragma unroll
-        for (int j = 0; j < kN; ++j) p.parts[int64_t(blockIdx.x) * p.k + c + j] = dw[i][j];
-      }
-    }
+    if (kSets > 1) __syncthreads();
   }
 }
 
@@ -438,24 +468,26 @@ __global__ void __launch_bounds__(kLong) long_norm_grad_kernel(const __grid_cons
   }
 }
 
-// The weight's gradient: the blocks' sums added up, a column by 8 threads in a fixed order.
+// The weight's gradient: the blocks' sums added up, a column by 32 threads in a fixed order.
 template <typename T>
 __global__ void __launch_bounds__(256) add_rows_kernel(const float* __restrict__ parts, int count, int64_t k,
                                                        T* __restrict__ grad_weight) {
   __shared__ float room[8][33];
-  const int lane = threadIdx.x % 32, part = threadIdx.x / 32;
-  const int64_t c = int64_t(blockIdx.x) * 32 + lane;
+  const int part = threadIdx.x / 8, column = threadIdx.x / 32;
+  const int64_t c = int64_t(blockIdx.x) * 8 + threadIdx.x % 8, first = int64_t(blockIdx.x) * 8;
   float sum = 0.0f;
   if (c < k) {
 #pragma unroll 8
-    for (int i = part; i < count; i += 8) sum += parts[i * k + c];
+    for (int i = part; i < count; i += 32) sum += __ldg(parts + i * k + c);
   }
-  room[part][lane] = sum;
+  room[threadIdx.x % 8][part] = sum;
   __syncthreads();
-  if (part == 0 && c < k) {
-    for (int i = 1; i < 8; ++i) sum += room[i][lane];
+  sum = room[column][threadIdx.x % 32];
+#pragma unroll
+  for (int d = 16; d > 0; d /= 2) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+  if (threadIdx.x % 32 == 0 && first + column < k) {
     const float v[1] = {sum};
-    store(grad_weight + c, v);
+    store(grad_weight + first + column, v);
   }
 }
 
@@ -468,26 +500,49 @@ struct Form {
 // Calls f with the form for rows of `vectors` vectors; false where none holds them.
 template <bool kWide, typename F>
 bool with_form(int64_t vectors, F&& f) {
-  constexpr int kMost = kWide ? 4 : 16;  // vectors that a thread of the larger teams holds
-  if (vectors <= 32) return f(Form<32, 1>()), true;
-  if (vectors <= 64) return f(Form<32, 2>()), true;
-  if (vectors <= 128) return f(Form<32, 4>()), true;
-  if (!kWide && vectors <= 512) return f(Form<32, 16>()), true;
-  if (vectors <= 128 * kMost) return f(Form<128, kMost>()), true;
-  if (vectors <= 512 * kMost) return f(Form<512, kMost>()), true;
-  if (vectors <= 1024 * kMost) return f(Form<1024, kMost>()), true;
+  if constexpr (kWide) {
+    if (vectors <= 8) return f(Form<8, 1>()), true;
+    if (vectors <= 16) return f(Form<16, 1>()), true;
+    if (vectors <= 32) return f(Form<32, 1>()), true;
+    if (vectors <= 64) return f(Form<32, 2>()), true;
+    if (vectors <= 128) return f(Form<32, 4>()), true;
+    if (vectors <= 512) return f(Form<128, 4>()), true;
+    if (vectors <= 2048) return f(Form<512, 4>()), true;
+    if (vectors <= 4096) return f(Form<512, 8>()), true;
+  } else {
+    if (vectors <= 32) return f(Form<32, 1>()), true;
+    if (vectors <= 128) return f(Form<32, 4>()), true;
+    if (vectors <= 256) return f(Form<32, 8>()), true;
+    if (vectors <= 1024) return f(Form<128, 8>()), true;
+    if (vectors <= 4096) return f(Form<512, 8>()), true;
+    if (vectors <= 16384) return f(Form<1024, 16>()), true;
+  }
   return false;
 }
-// The gradient holds three rows and the weight's gradient.
+// The gradient holds three rows, the next three and the weight's gradient.
 template <typename T, bool kWide, typename F>
 bool with_grad_form(int64_t vectors, F&& f) {
-  constexpr int kMost = !kWide ? 16 : sizeof(T) == 4 ? 8 : 4;
-  if (vectors <= 32) return f(Form<32, 1>()), true;
-  if (vectors <= 64) return f(Form<32, 2>()), true;
-  if (vectors <= 128) return f(Form<32, 4>()), true;
-  if (vectors <= 128 * 4) return f(Form<128, 4>()), true;
-  if (vectors <= 512 * 4) return f(Form<512, 4>()), true;
-  if (kMost > 4 && vectors <= 512 * kMost) return f(Form<512, kMost>()), true;
+  if constexpr (kWide) {
+    if (vectors <= 8) return f(Form<8, 1>()), true;
+    if (vectors <= 16) return f(Form<16, 1>()), true;
+    if (vectors <= 32) return f(Form<32, 1>()), true;
+    if (vectors <= 64) return f(Form<32, 2>()), true;
+    if (vectors <= 128) return f(Form<64, 2>()), true;
+    if (vectors <= 256) return f(Form<128, 2>()), true;
+    if (vectors <= 512) return f(Form<256, 2>()), true;
+    if (vectors <= 1024) return f(Form<512, 2>()), true;
+    if (vectors <= 2048) return f(Form<512, 4>()), true;
+    if (sizeof(T) == 4 && vectors <= 4096) return f(Form<512, 8>()), true;
+  } else {
+    if (vectors <= 32) return f(Form<32, 1>()), true;
+    if (vectors <= 128) return f(Form<32, 4>()), true;
+    if (vectors <= 256) return f(Form<32, 8>()), true;
+    if (vectors <= 512) return f(Form<64, 8>()), true;
+    if (vectors <= 1024) return f(Form<128, 8>()), true;
+    if (vectors <= 2048) return f(Form<256, 8>()), true;
+    if (vectors <= 4096) return f(Form<512, 8>()), true;
+    if (vectors <= 8192) return f(Form<512, 16>()), true;
+  }
   return false;
 }
 
@@ -526,7 +581,7 @@ int norm_grad(const NormGrad& p, void* grad_weight, cudaStream_t s) {
     constexpr bool kWide = decltype(is_wide)::value;
     using G = Team<form.kThreads>;
     blocks = grad_blocks((p.m + G::kRows - 1) / G::kRows);
-    const size_t shared = G::kRows > 1 ? form.kThreads * form.kVectors * Vec<T, kWide>::kValues * sizeof(float) : 0;
+    const size_t shared = G::kRows > 1 ? form.kThreads * form.kVectors * Vec<T, kWide>::kValues * sizeof(float) : 0;  // the warps' sums
     norm_grad_kernel<T, kWide, form.kThreads, form.kVectors><<<unsigned(blocks), G::kBlock, shared, s>>>(p);
   };
   if (wide)
@@ -535,7 +590,7 @@ int norm_grad(const NormGrad& p, void* grad_weight, cudaStream_t s) {
     held = with_grad_form<T, false>(p.k, [&](auto form) { launch(form, std::false_type()); });
   if (!held) long_norm_grad_kernel<T><<<unsigned(blocks), kLong, 0, s>>>(p);
   if (int rc = launch_status(); rc || !p.parts) return rc;
-  add_rows_kernel<T><<<unsigned((p.k + 31) / 32), 256, 0, s>>>(p.parts, int(blocks), p.k, static_cast<T*>(grad_weight));
+  add_rows_kernel<T><<<unsigned((p.k + 7) / 8), 256, 0, s>>>(p.parts, int(blocks), p.k, static_cast<T*>(grad_weight));
   return launch_status();
 }
 

@@ -31,9 +31,9 @@ def quantise(x):
     """(codes (..., K) int8, scale (...) float32) of x (..., K), float32 or bfloat16: each row's largest magnitude
     over 127 is its scale. Rows of codes start on 16-byte boundaries; tokens that are zero or not finite are as
     rms_norm.forward8's."""
-    m, k, code, index = rms_norm._check(("x", x), None, 0.0)
+    m, k, code, index = rms_norm._check("x", x, None, 0.0)
     x, xs = _rl.as_rows(x)
-    codes, scale = rms_norm.codes_like(x, k), x.new_empty(x.shape[:-1], dtype=torch.float32)
+    codes, scale = rms_norm.codes_like(x, k), _rl.empty_lead(x, torch.float32)
     _rl.launch(index, _rl.lib().rms_norm_codes, code, m, k, x.data_ptr(), xs, 0, 0, 0, 0.0, 0, codes.data_ptr(),
                (k + 15) // 16 * 16, scale.data_ptr(), 0)
     return codes, scale
@@ -47,11 +47,11 @@ def quantise_weight(w):
     return Weight(*quantise(w.detach().t().contiguous()))
 
 
-def _on_boundaries(codes):
+def _on_boundaries(codes, rows):
     """(codes, bytes between rows) with rows on 16-byte boundaries; anything else is copied."""
     k = codes.shape[-1]
     codes, pitch = _rl.as_rows(codes)
-    if codes.shape[:-1].numel() <= 1:
+    if rows <= 1:
         pitch = (k + 15) // 16 * 16  # of one row, any
     if pitch % 16 or pitch < k or codes.data_ptr() % 16:
         room = rms_norm.codes_like(codes, k)
@@ -65,24 +65,23 @@ def forward(codes, scale, weight, dtype=torch.bfloat16):
     w, ws = weight.codes, weight.scale
     for name, x, kind in (("codes", codes, torch.int8), ("scale", scale, torch.float32), ("weight.codes", w, torch.int8),
                           ("weight.scale", ws, torch.float32)):
-        if not isinstance(x, torch.Tensor) or not x.is_cuda or x.dtype is not kind:
+        if not isinstance(x, torch.Tensor) or x.dtype is not kind or not x.is_cuda:
             raise ValueError(f"{name} must be a CUDA tensor of {kind}: there is no CPU path")
-    index = codes.get_device()
+    index, lead, of_w = codes.get_device(), scale.shape, w.shape
     if scale.get_device() != index or w.get_device() != index or ws.get_device() != index:
         _rl.one_device(index, scale=scale, **{"weight.codes": w, "weight.scale": ws})
-    if w.dim() != 2 or not codes.dim() or codes.shape[-1] != w.shape[1] or ws.shape != w.shape[:1] \
-            or scale.shape != codes.shape[:-1]:
+    if len(of_w) != 2 or codes.shape != (*lead, of_w[1]) or ws.shape != of_w[:1]:
         raise ValueError(f"codes (..., K), scale (...), weight.codes (F, K) and weight.scale (F,) do not fit: got "
-                         f"{tuple(codes.shape)}, {tuple(scale.shape)}, {tuple(w.shape)} and {tuple(ws.shape)}")
-    f, k = w.shape
+                         f"{tuple(codes.shape)}, {tuple(lead)}, {tuple(of_w)} and {tuple(ws.shape)}")
+    f, k = of_w
     if not 1 <= k <= MOST_TERMS:
         raise ValueError(f"K must be from 1 to {MOST_TERMS}, so that sums fit 32 bits; got {k}")
     if dtype not in _rl.FLOAT_DTYPES:
         raise ValueError(f"dtype must be float32 or bfloat16; got {dtype}")
     m = scale.numel()
-    (codes, pitch), (w, w_pitch) = _on_boundaries(codes), _on_boundaries(w)
+    (codes, pitch), (w, w_pitch) = _on_boundaries(codes, m), _on_boundaries(w, f)
     scale, ws, lib = scale.contiguous(), ws.contiguous(), _rl.lib()
-    out = codes.new_empty((*codes.shape[:-1], f), dtype=dtype)
+    out = _rl.empty_rows(codes, f, dtype)
     nbytes = lib.int8_linear_scratch_bytes(m, k, f)
     tmp = _rl.scratch(nbytes, codes)
     _rl.launch(index, lib.int8_linear_forward, _rl.FLOAT_DTYPES[dtype], m, k, f, codes.data_ptr(), pitch, scale.data_ptr(),

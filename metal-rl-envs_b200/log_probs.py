@@ -61,15 +61,15 @@ def forward(logits, actions, allowed=None, alternatives=0):
     m, v, code, action_code, index = _check(logits, actions, allowed)
     if not 0 <= alternatives <= min(v, MOST_ALTERNATIVES):
         raise ValueError(f"alternatives must be from 0 to {min(v, MOST_ALTERNATIVES)}; got {alternatives}")
-    lead = logits.shape[:-1]
     logits, stride = _rl.as_rows(logits)
     allowed, allowed_stride = (None, 0) if allowed is None else _rl.as_rows(allowed)
     actions = actions.contiguous()
-    log_prob, entropy, normalizer = (logits.new_empty(lead, dtype=torch.float32) for _ in range(3))
+    log_prob = _rl.empty_lead(logits, torch.float32)
+    entropy, normalizer = torch.empty_like(log_prob), torch.empty_like(log_prob)
     top, best = None, None
     if alternatives:
-        top = logits.new_empty((*lead, alternatives), dtype=torch.float32)
-        best = logits.new_empty((*lead, alternatives), dtype=torch.int64)
+        top = _rl.empty_rows(logits, alternatives, torch.float32)
+        best = _rl.empty_rows(logits, alternatives, torch.int64)
     _rl.launch(index, _rl.lib().log_probs_forward, code, m, v, logits.data_ptr(), stride, actions.data_ptr(), action_code,
                _rl.ptr(allowed), allowed_stride, log_prob.data_ptr(), entropy.data_ptr(), normalizer.data_ptr(), alternatives,
                _rl.ptr(best), _rl.ptr(top))

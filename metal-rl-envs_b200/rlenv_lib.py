@@ -15,6 +15,7 @@ There is no CPU path: a missing library or a missing CUDA device raises.
 import ctypes
 import os
 from ctypes import c_double, c_float, c_int, c_int64, c_uint32, c_uint64, c_void_p
+from functools import lru_cache
 from pathlib import Path
 
 import numpy as np
@@ -481,9 +482,12 @@ def as_rows(x):
     apart; anything else is copied."""
     if x.is_contiguous():
         return x, x.shape[-1]
+    strides = x.stride()
+    if len(strides) == 2 and strides[1] == 1:
+        return x, strides[0]
     step, count = None, 1  # the leading axes' step, and how many rows the axes seen so far hold
-    if x.stride(-1) == 1 or x.shape[-1] == 1:
-        for n, s in zip(reversed(x.shape[:-1]), reversed(x.stride()[:-1])):
+    if strides[-1] == 1 or x.shape[-1] == 1:
+        for n, s in zip(reversed(x.shape[:-1]), reversed(strides[:-1])):
             if n == 1:
                 continue
             if step is None:
@@ -496,6 +500,25 @@ def as_rows(x):
     return x.contiguous(), x.shape[-1]
 
 
-def empty_rows(x, k, dtype):
-    """A dense tensor of x's leading axes with rows of k."""
-    return x.new_empty((*x.shape[:-1], k), dtype=dtype)
+@lru_cache(maxsize=None)
+def _cuda(index):
+    return torch.device("cuda", index)
+
+
+def empty_rows(x, k, dtype, pitch=None):
+    """A tensor of x's leading axes with dense rows of k, `pitch` elements apart (None: k). Two axes take the quickest of
+    torch's calls, at 1.5 us against new_empty's 2.5."""
+    shape = x.shape
+    if len(shape) == 2:
+        return torch.empty_strided((shape[0], k), (pitch or k, 1), dtype=dtype, device=_cuda(x.get_device()))
+    if pitch is None or pitch == k:
+        return x.new_empty((*shape[:-1], k), dtype=dtype)
+    return x.new_empty((*shape[:-1], pitch), dtype=dtype)[..., :k]
+
+
+def empty_lead(x, dtype):
+    """A dense tensor of x's leading axes."""
+    shape = x.shape
+    if len(shape) == 2:
+        return torch.empty_strided(shape[:1], (1,), dtype=dtype, device=_cuda(x.get_device()))
+    return x.new_empty(shape[:-1], dtype=dtype)

@@ -19,16 +19,15 @@ from torch.autograd.function import once_differentiable
 import rlenv_lib as _rl
 
 
-def _check(first, weight, eps, **others):
-    """(rows, K, the type's code, the device's index); first is (name, tensor). What fits passes on a few
-    comparisons; what does not is looked at again for the message."""
-    name, x = first
+def _check(name, x, weight, eps, others=()):
+    """(rows, K, the type's code, the device's index); others are (name, tensor) of x's kind or None. What fits passes on
+    a few comparisons; what does not is looked at again for the message."""
     if not isinstance(x, torch.Tensor) or not x.is_cuda or x.dtype not in _rl.FLOAT_DTYPES:
         _rl.as_floats(name, x)
     shape, dtype, index = x.shape, x.dtype, x.get_device()
     if not shape or shape[-1] == 0:
         raise ValueError(f"{name} must be (..., K) with K of at least 1; got shape {tuple(shape)}")
-    for other, y in others.items():
+    for other, y in others:
         if y is not None and (not isinstance(y, torch.Tensor) or y.get_device() != index or y.dtype is not dtype
                               or y.shape != shape):
             _rl.as_floats(other, y, shape, dtype)
@@ -43,52 +42,64 @@ def _check(first, weight, eps, **others):
     return x.numel() // k, k, _rl.FLOAT_DTYPES[dtype], index
 
 
-def _rows(x):
-    return (None, 0) if x is None else _rl.as_rows(x)
+def _like(x):
+    """A dense tensor of x's shape and type."""
+    return torch.empty_like(x) if x.is_contiguous() else x.new_empty(x.shape)
 
 
 def forward(x, weight=None, residual=None, eps=1e-6):
     """(out, total), both (..., K). residual None: total is x itself; weight None: ones."""
-    m, k, code, index = _check(("x", x), weight, eps, residual=residual)
-    (x, xs), (residual, rs) = _rl.as_rows(x), _rows(residual)
-    weight = None if weight is None else weight.contiguous()
-    out = _rl.empty_rows(x, k, x.dtype)
-    total = x if residual is None else torch.empty_like(out)
-    _rl.launch(index, _rl.lib().rms_norm_forward, code, m, k, x.data_ptr(), xs, _rl.ptr(residual), rs, _rl.ptr(weight),
-               eps, out.data_ptr(), 0 if residual is None else total.data_ptr())
+    m, k, code, index = _check("x", x, weight, eps, (("residual", residual),))
+    if weight is not None:
+        weight = weight.contiguous()
+    x, xs = _rl.as_rows(x)
+    out = _like(x)
+    if residual is None:
+        total, res_at, rs, total_at = x, 0, 0, 0
+    else:
+        residual, rs = _rl.as_rows(residual)
+        total = torch.empty_like(out)
+        res_at, total_at = residual.data_ptr(), total.data_ptr()
+    _rl.launch(index, _rl.lib().rms_norm_forward, code, m, k, x.data_ptr(), xs, res_at, rs, _rl.ptr(weight), eps,
+               out.data_ptr(), total_at)
     return out, total
 
 
 def codes_like(x, k):
     """Room for 8-bit rows of k as int8_linear takes them: (..., K) int8, rows on 16-byte boundaries."""
-    pitch = (k + 15) // 16 * 16
-    codes = _rl.empty_rows(x, pitch, torch.int8)
-    return codes if pitch == k else codes[..., :k]
+    return _rl.empty_rows(x, k, torch.int8, (k + 15) // 16 * 16)
 
 
 def forward8(x, weight=None, residual=None, eps=1e-6):
     """(codes (..., K) int8, scale (...) float32, total): out = codes * scale, each token's scale its largest magnitude
     over 127, rounded to the nearest. Rows of codes start on 16-byte boundaries. A token whose out is below 2^-100 is
     zeros with scale 0; one that holds a value that is not finite is zeros with scale NaN."""
-    m, k, code, index = _check(("x", x), weight, eps, residual=residual)
-    (x, xs), (residual, rs) = _rl.as_rows(x), _rows(residual)
-    weight = None if weight is None else weight.contiguous()
-    codes, scale = codes_like(x, k), x.new_empty(x.shape[:-1], dtype=torch.float32)
-    total = x if residual is None else _rl.empty_rows(x, k, x.dtype)
-    _rl.launch(index, _rl.lib().rms_norm_codes, code, m, k, x.data_ptr(), xs, _rl.ptr(residual), rs, _rl.ptr(weight), eps,
-               1, codes.data_ptr(), (k + 15) // 16 * 16, scale.data_ptr(), 0 if residual is None else total.data_ptr())
+    m, k, code, index = _check("x", x, weight, eps, (("residual", residual),))
+    if weight is not None:
+        weight = weight.contiguous()
+    x, xs = _rl.as_rows(x)
+    if residual is None:
+        total, res_at, rs, total_at = x, 0, 0, 0
+    else:
+        residual, rs = _rl.as_rows(residual)
+        total = _like(x)
+        res_at, total_at = residual.data_ptr(), total.data_ptr()
+    codes, scale = codes_like(x, k), _rl.empty_lead(x, torch.float32)
+    _rl.launch(index, _rl.lib().rms_norm_codes, code, m, k, x.data_ptr(), xs, res_at, rs, _rl.ptr(weight), eps, 1,
+               codes.data_ptr(), (k + 15) // 16 * 16, scale.data_ptr(), total_at)
     return codes, scale, total
 
 
 def backward(grad_out, total, weight=None, eps=1e-6, grad_total=None):
     """(grad, grad_weight) from grad_out and, where the total is used further, grad_total: grad (..., K) is the
     gradient of x and of the residual alike, grad_weight (K,) or None without a weight."""
-    m, k, code, index = _check(("total", total), weight, eps, grad_out=grad_out, grad_total=grad_total)
+    m, k, code, index = _check("total", total, weight, eps, (("grad_out", grad_out), ("grad_total", grad_total)))
     lib = _rl.lib()
     if m == 0:
         return torch.empty_like(total), None if weight is None else torch.zeros_like(weight)
-    (g, gs), (t, ts), (s, ss) = _rl.as_rows(grad_out), _rl.as_rows(total), _rows(grad_total)
-    grad = _rl.empty_rows(t, k, t.dtype)
+    (g, gs), (t, ts) = _rl.as_rows(grad_out), _rl.as_rows(total)
+    s, ss = (None, 0) if grad_total is None else _rl.as_rows(grad_total)
+    grad = _like(t)
     grad_weight, tmp, nbytes = None, None, 0
     if weight is not None:
         weight = weight.contiguous()
