@@ -9,6 +9,7 @@
 // results. A row is a warp's or a block's: `Team`.
 #include <cuda_bf16.h>
 
+#include <initializer_list>
 #include <type_traits>
 
 #include "common.cuh"
@@ -16,22 +17,42 @@
 namespace rlenv {
 namespace {
 
-// Values a thread moves at once: 16 bytes where every row starts on a 16-byte boundary and holds whole vectors, else
-// one value (kWide false).
-template <typename T, bool kWide>
+// How a row is moved. kWhole: vectors of 16 bytes, where every row starts on a 16-byte boundary and holds whole ones.
+// kSkewed: rows of any length whose tensors all lie alike on the boundaries: vectors between the first boundary in the row
+// and the last, and the up to 14 values before and after them by a lane each (bfloat16 rows of 333, 100,000 forward 60 us,
+// by single values 182). kSingle: one value at a time.
+enum Way { kWhole, kSkewed, kSingle };
+template <typename T, Way kWay>
 struct Vec {
-  static constexpr int kValues = kWide ? 16 / int(sizeof(T)) : 1;
+  static constexpr int kValues = kWay == kSingle ? 1 : 16 / int(sizeof(T));
 };
 
 // A vector as it lies in memory, and its values. Rows wait in registers in this form: half the room for bfloat16, and
-// nothing that waits for a load while others are to be issued (bfloat16 rows of 333 by single values, the gradient of
-// 100,000: 658 us when each was converted as it came).
-template <typename T, bool kWide>
+// nothing that waits for a load while others are to be issued.
+template <typename T, int kValues>
 struct Raw {
   uint4 bits;
   RLENV_D void load(const T* from) { bits = __ldg(reinterpret_cast<const uint4*>(from)); }
   RLENV_D void clear() { bits = make_uint4(0, 0, 0, 0); }
-  RLENV_D void values(float (&v)[16 / sizeof(T)]) const {
+  // From any place: `before` and `after` it there are that many values of the same array.
+  RLENV_D void load_between(const T* from, int before, int after) {
+    const bool between = sizeof(T) == 2 && reinterpret_cast<uintptr_t>(from) % 4;
+    if (between && (before < 1 || after < 1)) {
+      uint32_t w[4] = {0, 0, 0, 0};
+#pragma unroll
+      for (int i = 0; i < kValues; ++i)
+        w[i * int(sizeof(T)) / 4] |= uint32_t(__ldg(reinterpret_cast<const unsigned short*>(from) + i)) << 16 * (i % 2);
+      bits = make_uint4(w[0], w[1], w[2], w[3]);
+      return;
+    }
+    const uint32_t* const words = reinterpret_cast<const uint32_t*>(between ? from - 1 : from);
+    const uint32_t w0 = __ldg(words), w1 = __ldg(words + 1), w2 = __ldg(words + 2), w3 = __ldg(words + 3);
+    bits = make_uint4(w0, w1, w2, w3);
+    if (between)
+      bits = make_uint4(__funnelshift_r(w0, w1, 16), __funnelshift_r(w1, w2, 16), __funnelshift_r(w2, w3, 16),
+                        __funnelshift_r(w3, __ldg(words + 4), 16));
+  }
+  RLENV_D void values(float* v) const {
     const uint32_t w[4] = {bits.x, bits.y, bits.z, bits.w};
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -43,61 +64,147 @@ struct Raw {
   }
 };
 template <>
-struct Raw<float, false> {
+struct Raw<float, 1> {
   float bits;
   RLENV_D void load(const float* from) { bits = __ldg(from); }
+  RLENV_D void load_between(const float* from, int, int) { load(from); }
   RLENV_D void clear() { bits = 0.0f; }
-  RLENV_D void values(float (&v)[1]) const { v[0] = bits; }
+  RLENV_D void values(float* v) const { v[0] = bits; }
 };
 template <>
-struct Raw<__nv_bfloat16, false> {
+struct Raw<__nv_bfloat16, 1> {
   unsigned short bits;
   RLENV_D void load(const __nv_bfloat16* from) { bits = __ldg(reinterpret_cast<const unsigned short*>(from)); }
+  RLENV_D void load_between(const __nv_bfloat16* from, int, int) { load(from); }
   RLENV_D void clear() { bits = 0; }
-  RLENV_D void values(float (&v)[1]) const { v[0] = __uint_as_float(uint32_t(bits) << 16); }
+  RLENV_D void values(float* v) const { v[0] = __uint_as_float(uint32_t(bits) << 16); }
 };
-template <typename T, int kValues>
-RLENV_D void load(const T* from, float (&v)[kValues]) {
-  Raw<T, (kValues > 1)> raw;
+template <typename T>
+RLENV_D float load(const T* from) {
+  Raw<T, 1> raw;
+  float v;
   raw.load(from);
-  raw.values(v);
-}
-template <int kValues>
-RLENV_D void store(float* to, const float (&v)[kValues]) {
-  if constexpr (kValues == 1)
-    to[0] = v[0];
-  else
-    *reinterpret_cast<float4*>(to) = make_float4(v[0], v[1], v[2], v[3]);
+  raw.values(&v);
+  return v;
 }
 RLENV_D uint32_t pair_bits(float lo, float hi) {
   const __nv_bfloat162 p = __floats2bfloat162_rn(lo, hi);
   return *reinterpret_cast<const uint32_t*>(&p);
 }
-template <int kValues>
-RLENV_D void store(__nv_bfloat16* to, const float (&v)[kValues]) {
-  if constexpr (kValues == 1)
-    to[0] = __float2bfloat16_rn(v[0]);
-  else
-    *reinterpret_cast<uint4*>(to) = make_uint4(pair_bits(v[0], v[1]), pair_bits(v[2], v[3]), pair_bits(v[4], v[5]),
-                                               pair_bits(v[6], v[7]));
+RLENV_D void store(float* to, float v) { *to = v; }
+RLENV_D void store(__nv_bfloat16* to, float v) { *to = __float2bfloat16_rn(v); }
+RLENV_D void store(int8_t* to, float v) { *to = int8_t(__float2int_rn(v)); }  // a whole number of at most 127
+RLENV_D void store_vector(float* to, const float* v) { *reinterpret_cast<float4*>(to) = make_float4(v[0], v[1], v[2], v[3]); }
+RLENV_D void store_vector(__nv_bfloat16* to, const float* v) {
+  *reinterpret_cast<uint4*>(to) =
+      make_uint4(pair_bits(v[0], v[1]), pair_bits(v[2], v[3]), pair_bits(v[4], v[5]), pair_bits(v[6], v[7]));
 }
-// Whole numbers of at most 127 in magnitude, as bytes.
 RLENV_D uint32_t byte_of(float x) { return uint32_t(__float2int_rn(x)) & 0xffu; }
 template <int kValues>
-RLENV_D void store_codes(int8_t* to, const float (&v)[kValues]) {
-  if constexpr (kValues == 1) {
-    to[0] = int8_t(__float2int_rn(v[0]));
-  } else {
-    uint32_t w[kValues / 4];
+RLENV_D void store_bytes(int8_t* to, const float* v) {  // on a boundary of kValues bytes
+  uint32_t w[kValues / 4];
 #pragma unroll
-    for (int i = 0; i < kValues / 4; ++i)
-      w[i] = byte_of(v[4 * i]) | byte_of(v[4 * i + 1]) << 8 | byte_of(v[4 * i + 2]) << 16 | byte_of(v[4 * i + 3]) << 24;
-    if constexpr (kValues == 4)
-      *reinterpret_cast<uint32_t*>(to) = w[0];
-    else
-      *reinterpret_cast<uint2*>(to) = make_uint2(w[0], w[1]);
-  }
+  for (int i = 0; i < kValues / 4; ++i)
+    w[i] = byte_of(v[4 * i]) | byte_of(v[4 * i + 1]) << 8 | byte_of(v[4 * i + 2]) << 16 | byte_of(v[4 * i + 3]) << 24;
+  if constexpr (kValues == 4)
+    *reinterpret_cast<uint32_t*>(to) = w[0];
+  else
+    *reinterpret_cast<uint2*>(to) = make_uint2(w[0], w[1]);
 }
+
+// A thread's part of a row of k values: kVectors vectors, kThreads vectors apart, and with kSkewed one value more. All its
+// values lie side by side in arrays of kCount.
+template <typename T, Way kWay, int kThreads, int kVectors>
+struct Part {
+  static constexpr int kN = Vec<T, kWay>::kValues, kEdge = kWay == kSkewed, kCount = kVectors * kN + kEdge;
+  struct Row {
+    Raw<T, kN> vectors[kVectors];
+    Raw<T, 1> edge;
+    RLENV_D void values(float (&v)[kCount]) const {
+#pragma unroll
+      for (int i = 0; i < kVectors; ++i) vectors[i].values(v + i * kN);
+      if constexpr (kEdge) edge.values(v + kVectors * kN);
+    }
+  };
+  int k, first, count, edge;  // the first vector's place, how many this thread has, the single value's place or -1
+  // of a row at `row`, as far as that lies on the boundaries
+  RLENV_D Part(const void* row, int k, int at) : k(k), edge(-1) {
+    int head = 0;
+    if constexpr (kEdge) head = min(k, (16 - int(reinterpret_cast<uintptr_t>(row) % 16)) % 16 / int(sizeof(T)));
+    const int vectors = (k - head) / kN, tail = k - head - vectors * kN;
+    first = head + at * kN;
+    count = at < vectors ? (vectors - at + kThreads - 1) / kThreads : 0;
+    if constexpr (kEdge) edge = at < head ? at : at >= kN && at - kN < tail ? head + vectors * kN + at - kN : -1;
+  }
+  RLENV_D int place(int i) const { return first + i * kThreads * kN; }
+  RLENV_D void load(const T* row, Row& r) const {
+#pragma unroll
+    for (int i = 0; i < kVectors; ++i) {
+      r.vectors[i].clear();
+      if (i < count) r.vectors[i].load(row + place(i));
+    }
+    if constexpr (kEdge) {
+      r.edge.clear();
+      if (edge >= 0) r.edge.load(row + edge);
+    }
+  }
+  RLENV_D void clear(Row& r) const {
+#pragma unroll
+    for (int i = 0; i < kVectors; ++i) r.vectors[i].clear();
+    r.edge.clear();
+  }
+  RLENV_D void load_weight(const T* weight, Row& r) const {  // which lies on a boundary by itself
+    if constexpr (!kEdge) {
+      load(weight, r);
+    } else {
+#pragma unroll
+      for (int i = 0; i < kVectors; ++i) {
+        r.vectors[i].clear();
+        if (i < count) r.vectors[i].load_between(weight + place(i), place(i), k - place(i) - kN);
+      }
+      r.edge.clear();
+      if (edge >= 0) r.edge.load(weight + edge);
+    }
+  }
+  RLENV_D void store_row(T* row, const float (&v)[kCount]) const {
+#pragma unroll
+    for (int i = 0; i < kVectors; ++i)
+      if (i < count) {
+        if constexpr (kN == 1)
+          store(row + place(i), v[i]);
+        else
+          store_vector(row + place(i), v + i * kN);
+      }
+    if constexpr (kEdge)
+      if (edge >= 0) store(row + edge, v[kVectors * kN]);
+  }
+  RLENV_D void store_codes(int8_t* row, const float (&v)[kCount]) const {
+#pragma unroll
+    for (int i = 0; i < kVectors; ++i)
+      if (i < count) {
+        if constexpr (kWay == kWhole) {
+          store_bytes<kN>(row + place(i), v + i * kN);
+        } else {
+#pragma unroll
+          for (int j = 0; j < kN; ++j) store(row + place(i) + j, v[i * kN + j]);
+        }
+      }
+    if constexpr (kEdge)
+      if (edge >= 0) store(row + edge, v[kVectors * kN]);
+  }
+  // f(place, value) for what is there.
+  template <typename F>
+  RLENV_D void each(float (&v)[kCount], F&& f) const {
+#pragma unroll
+    for (int i = 0; i < kVectors; ++i)
+      if (i < count) {
+#pragma unroll
+        for (int j = 0; j < kN; ++j) f(place(i) + j, v[i * kN + j]);
+      }
+    if constexpr (kEdge)
+      if (edge >= 0) f(edge, v[kVectors * kN]);
+  }
+};
 
 // The threads that share a row: some of a warp, a warp, some warps of a block, or a block.
 template <int kThreads>
@@ -168,93 +275,61 @@ struct Norm {
 constexpr float kTiny = 0x1p-100f;
 
 // Rows of at most kThreads kVectors vectors: kCodes false, out; true, codes and scale.
-template <typename T, bool kWide, int kThreads, int kVectors, bool kCodes>
+template <typename T, Way kWay, int kThreads, int kVectors, bool kCodes>
 __global__ void __launch_bounds__(Team<kThreads>::kBlock) norm_kernel(const __grid_constant__ Norm p) {
   using G = Team<kThreads>;
-  constexpr int kN = Vec<T, kWide>::kValues;
+  using P = Part<T, kWay, kThreads, kVectors>;
+  constexpr int kCount = P::kCount;
   __shared__ float room[G::kWarps * G::kRows];
-  const int at = threadIdx.x % kThreads, k = int(p.k);
+  const int at = threadIdx.x % kThreads;
   const int64_t row = int64_t(blockIdx.x) * G::kRows + threadIdx.x / kThreads;
   const bool there = row < p.m;
   const T *x = static_cast<const T*>(p.x) + row * p.x_stride,
           *residual = p.residual ? static_cast<const T*>(p.residual) + row * p.residual_stride : nullptr,
           *weight = static_cast<const T*>(p.weight);
-  const auto column = [&](int i) { return (at + i * kThreads) * kN; };
-  const auto in = [&](int i) { return there && column(i) < k; };
-  float t[kVectors][kN];
-  Raw<T, kWide> from[kVectors], other[kVectors];
-#pragma unroll
-  for (int i = 0; i < kVectors; ++i) {
-    from[i].clear();
-    if (in(i)) from[i].load(x + column(i));
-  }
+  const P part(x, there ? int(p.k) : 0, at);
+  typename P::Row from, other;
+  part.load(x, from);
+  if (residual) part.load(residual, other);
+  float t[kCount], sum[1] = {0.0f};
+  from.values(t);
   if (residual) {
+    float y[kCount];
+    other.values(y);
 #pragma unroll
-    for (int i = 0; i < kVectors; ++i) {
-      other[i].clear();
-      if (in(i)) other[i].load(residual + column(i));
-    }
+    for (int i = 0; i < kCount; ++i) t[i] += y[i];
   }
-  float sum[1] = {0.0f};
 #pragma unroll
-  for (int i = 0; i < kVectors; ++i) {
-    from[i].values(t[i]);
-    if (residual) {
-      float y[kN];
-      other[i].values(y);
-#pragma unroll
-      for (int j = 0; j < kN; ++j) t[i][j] += y[j];
-    }
-#pragma unroll
-    for (int j = 0; j < kN; ++j) sum[0] = fmaf(t[i][j], t[i][j], sum[0]);
-  }
-  if (weight) {  // on its way while the sum is formed
-#pragma unroll
-    for (int i = 0; i < kVectors; ++i)
-      if (column(i) < k) other[i].load(weight + column(i));
-  }
-  if (p.total) {
-    T* const total = static_cast<T*>(p.total) + row * p.k;
-#pragma unroll
-    for (int i = 0; i < kVectors; ++i)
-      if (in(i)) store(total + column(i), t[i]);
-  }
+  for (int i = 0; i < kCount; ++i) sum[0] = fmaf(t[i], t[i], sum[0]);
+  if (weight) part.load_weight(weight, other);  // on its way while the sum is formed
+  if (p.total && there) part.store_row(static_cast<T*>(p.total) + row * p.k, t);
   float r = 1.0f;
   if (!kCodes || p.normalise) {
     G::sum(sum, room);
-    r = rsqrtf(sum[0] / float(k) + p.eps);
+    r = rsqrtf(sum[0] / float(p.k) + p.eps);
   }
 #pragma unroll
-  for (int i = 0; i < kVectors; ++i) {
-    float w[kN];
-    if (weight && column(i) < k) other[i].values(w);
+  for (int i = 0; i < kCount; ++i) t[i] *= r;
+  if (weight) {
+    float w[kCount];
+    other.values(w);
 #pragma unroll
-    for (int j = 0; j < kN; ++j) t[i][j] = weight && column(i) < k ? t[i][j] * r * w[j] : t[i][j] * r;
+    for (int i = 0; i < kCount; ++i) t[i] *= w[i];
   }
   if constexpr (!kCodes) {
-    T* const out = static_cast<T*>(p.out) + row * p.k;
-#pragma unroll
-    for (int i = 0; i < kVectors; ++i)
-      if (in(i)) store(out + column(i), t[i]);
+    if (there) part.store_row(static_cast<T*>(p.out) + row * p.k, t);
   } else {
     // As bits, magnitudes are ordered with infinity and NaN above all numbers.
     uint32_t most = 0;
-#pragma unroll
-    for (int i = 0; i < kVectors; ++i)
-#pragma unroll
-      for (int j = 0; j < kN; ++j) most = max(most, in(i) ? __float_as_uint(t[i][j]) & 0x7fffffffu : 0u);
+    part.each(t, [&](int, float v) { most = max(most, __float_as_uint(v) & 0x7fffffffu); });
     most = G::largest(most, reinterpret_cast<uint32_t*>(room));
     const float top = __uint_as_float(most);
     const bool some = top >= kTiny && most < 0x7f800000u;
     const float to_codes = some ? 127.0f / top : 0.0f;
     if (at == 0 && there) p.scale[row] = some ? top / 127.0f : top < kTiny ? 0.0f : __uint_as_float(0x7fffffffu);
-    int8_t* const codes = p.codes + row * p.pitch;
 #pragma unroll
-    for (int i = 0; i < kVectors; ++i) {
-#pragma unroll
-      for (int j = 0; j < kN; ++j) t[i][j] = some ? t[i][j] * to_codes : 0.0f;
-      if (in(i)) store_codes(codes + column(i), t[i]);
-    }
+    for (int i = 0; i < kCount; ++i) t[i] = some ? t[i] * to_codes : 0.0f;
+    if (there) part.store_codes(p.codes + row * p.pitch, t);
   }
 }
 
@@ -268,12 +343,7 @@ __global__ void __launch_bounds__(kLong) long_norm_kernel(const __grid_constant_
   const T *x = static_cast<const T*>(p.x) + row * p.x_stride,
           *residual = p.residual ? static_cast<const T*>(p.residual) + row * p.residual_stride : nullptr,
           *weight = static_cast<const T*>(p.weight);
-  const auto total_at = [&](int64_t c) {
-    float t[1], y[1];
-    load(x + c, t);
-    if (residual) load(residual + c, y), t[0] += y[0];
-    return t[0];
-  };
+  const auto total_at = [&](int64_t c) { return residual ? load(x + c) + load(residual + c) : load(x + c); };
   float r = 1.0f;
   if (!kCodes || p.normalise) {
     float sum[1] = {0.0f};
@@ -284,13 +354,7 @@ __global__ void __launch_bounds__(kLong) long_norm_kernel(const __grid_constant_
     G::sum(sum, room);
     r = rsqrtf(sum[0] / float(p.k) + p.eps);
   }
-  const auto out_at = [&](int64_t c) {
-    float w[1];
-    const float v = total_at(c) * r;
-    if (!weight) return v;
-    load(weight + c, w);
-    return v * w[0];
-  };
+  const auto out_at = [&](int64_t c) { return weight ? total_at(c) * r * load(weight + c) : total_at(c) * r; };
   if constexpr (kCodes) {
     uint32_t most = 0;
     for (int64_t c = threadIdx.x; c < p.k; c += kLong) most = max(most, __float_as_uint(out_at(c)) & 0x7fffffffu);
@@ -299,20 +363,11 @@ __global__ void __launch_bounds__(kLong) long_norm_kernel(const __grid_constant_
     const bool some = top >= kTiny && most < 0x7f800000u;
     const float to_codes = some ? 127.0f / top : 0.0f;
     if (threadIdx.x == 0) p.scale[row] = some ? top / 127.0f : top < kTiny ? 0.0f : __uint_as_float(0x7fffffffu);
-    for (int64_t c = threadIdx.x; c < p.k; c += kLong) {
-      const float v[1] = {some ? out_at(c) * to_codes : 0.0f};
-      store_codes(p.codes + row * p.pitch + c, v);
-    }
+    for (int64_t c = threadIdx.x; c < p.k; c += kLong) store(p.codes + row * p.pitch + c, some ? out_at(c) * to_codes : 0.0f);
   }
   for (int64_t c = threadIdx.x; c < p.k; c += kLong) {
-    if constexpr (!kCodes) {
-      const float v[1] = {out_at(c)};
-      store(static_cast<T*>(p.out) + row * p.k + c, v);
-    }
-    if (p.total) {
-      const float v[1] = {total_at(c)};
-      store(static_cast<T*>(p.total) + row * p.k + c, v);
-    }
+    if constexpr (!kCodes) store(static_cast<T*>(p.out) + row * p.k + c, out_at(c));
+    if (p.total) store(static_cast<T*>(p.total) + row * p.k + c, total_at(c));
   }
 }
 
@@ -325,112 +380,95 @@ struct NormGrad {
   float* parts;  // (blocks, K): each block's sums over its rows of the weight's gradient; null: none asked for
 };
 
-// A team's next row is on its way while it works on one (kAhead: where registers allow).
-template <typename T, bool kWide, int kThreads, int kVectors>
+// A team's next row is on its way while it works on one (kAhead: where registers allow). Its rows are a multiple of 8
+// apart, so that they all lie alike on the boundaries.
+template <typename T, Way kWay, int kThreads, int kVectors>
 __global__ void __launch_bounds__(Team<kThreads>::kBlock) norm_grad_kernel(const __grid_constant__ NormGrad p) {
   using G = Team<kThreads>;
-  using R = Raw<T, kWide>;
-  constexpr int kN = Vec<T, kWide>::kValues;
-  constexpr bool kAhead = kVectors * int(sizeof(R)) <= 32;
+  using P = Part<T, kWay, kThreads, kVectors>;
+  using Row = typename P::Row;
+  constexpr int kCount = P::kCount;
+  constexpr bool kAhead = kVectors * int(sizeof(Raw<T, P::kN>)) <= 32;
   __shared__ float room[2 * G::kWarps * G::kRows];
   const int at = threadIdx.x % kThreads, k = int(p.k);
-  const auto column = [&](int i) { return (at + i * kThreads) * kN; };
-  float dw[kVectors][kN];
-  R w[kVectors];
-#pragma unroll
-  for (int i = 0; i < kVectors; ++i) {
-    w[i].clear();
-    if (p.weight && column(i) < k) w[i].load(static_cast<const T*>(p.weight) + column(i));
-#pragma unroll
-    for (int j = 0; j < kN; ++j) dw[i][j] = 0.0f;
-  }
-  const auto weighed = [&](int i, float (&g)[kN]) {
-    if (!p.weight) return;
-    float v[kN];
-    w[i].values(v);
-#pragma unroll
-    for (int j = 0; j < kN; ++j) g[j] *= v[j];
-  };
-  R t[kVectors], g[kVectors], s[kVectors];
-  const auto load_row = [&](int64_t row, R (&t)[kVectors], R (&g)[kVectors], R (&s)[kVectors]) {
-    const T *total = static_cast<const T*>(p.total) + row * p.total_stride,
-            *grad_out = static_cast<const T*>(p.grad_out) + row * p.grad_out_stride,
-            *grad_total = static_cast<const T*>(p.grad_total) + row * p.grad_total_stride;
-#pragma unroll
-    for (int i = 0; i < kVectors; ++i) {
-      t[i].clear(), g[i].clear(), s[i].clear();
-      if (row < p.m && column(i) < k) {
-        t[i].load(total + column(i));
-        g[i].load(grad_out + column(i));
-        if (p.grad_total) s[i].load(grad_total + column(i));
-      }
-    }
-  };
   const int64_t step = int64_t(gridDim.x) * G::kRows;
   int64_t row = int64_t(blockIdx.x) * G::kRows + threadIdx.x / kThreads;
   // A warp's teams make as many turns as its first.
   const int64_t turns = (p.m - (int64_t(blockIdx.x) * G::kRows + threadIdx.x / 32 * 32 / kThreads) + step - 1) / step;
+  const P part(static_cast<const T*>(p.total) + row * p.total_stride, k, at);
+  float dw[kCount];
+#pragma unroll
+  for (int i = 0; i < kCount; ++i) dw[i] = 0.0f;
+  Row w, t, g, s;
+  if (p.weight) part.load_weight(static_cast<const T*>(p.weight), w);
+  const auto weighed = [&](float (&v)[kCount]) {
+    if (!p.weight) return;
+    float of[kCount];
+    w.values(of);
+#pragma unroll
+    for (int i = 0; i < kCount; ++i) v[i] *= of[i];
+  };
+  const auto load_row = [&](int64_t row, Row& t, Row& g, Row& s) {
+    if (row < p.m) {
+      part.load(static_cast<const T*>(p.total) + row * p.total_stride, t);
+      part.load(static_cast<const T*>(p.grad_out) + row * p.grad_out_stride, g);
+      if (p.grad_total)
+        part.load(static_cast<const T*>(p.grad_total) + row * p.grad_total_stride, s);
+      else
+        part.clear(s);
+    } else {
+      part.clear(t), part.clear(g), part.clear(s);
+    }
+  };
   if (kAhead) load_row(row, t, g, s);
   for (int64_t turn = 0; turn < turns; ++turn, row += step) {
-    R next_t[kVectors], next_g[kVectors], next_s[kVectors];
+    Row next_t, next_g, next_s;
     if (kAhead)
       load_row(row + step, next_t, next_g, next_s);
     else
       load_row(row, t, g, s);
-    float sums[2] = {0.0f, 0.0f};
+    float tv[kCount], gv[kCount], sums[2] = {0.0f, 0.0f};
+    t.values(tv), g.values(gv);
+    weighed(gv);
 #pragma unroll
-    for (int i = 0; i < kVectors; ++i) {
-      float tv[kN], gv[kN];
-      t[i].values(tv), g[i].values(gv);
-      weighed(i, gv);
-#pragma unroll
-      for (int j = 0; j < kN; ++j) sums[0] = fmaf(tv[j], tv[j], sums[0]), sums[1] = fmaf(gv[j], tv[j], sums[1]);
-    }
+    for (int i = 0; i < kCount; ++i) sums[0] = fmaf(tv[i], tv[i], sums[0]), sums[1] = fmaf(gv[i], tv[i], sums[1]);
     G::sum(sums, room);
-    const float r = rsqrtf(sums[0] / float(k) + p.eps), along = r * (r * sums[1] / float(k));
-    T* const grad = static_cast<T*>(p.grad) + row * p.k;
+    const float r = row < p.m ? rsqrtf(sums[0] / float(k) + p.eps) : 0.0f, along = r * (r * sums[1] / float(k));
+    float v[kCount];
+    t.values(tv), g.values(gv), s.values(v);
 #pragma unroll
-    for (int i = 0; i < kVectors; ++i) {
-      float tv[kN], gv[kN], v[kN];
-      t[i].values(tv), g[i].values(gv), s[i].values(v);
+    for (int i = 0; i < kCount; ++i) dw[i] = fmaf(gv[i], tv[i] * r, dw[i]);
+    weighed(gv);
 #pragma unroll
-      for (int j = 0; j < kN; ++j) dw[i][j] = fmaf(gv[j], tv[j] * r, dw[i][j]);
-      weighed(i, gv);
-#pragma unroll
-      for (int j = 0; j < kN; ++j) v[j] += r * (gv[j] - tv[j] * along);
-      if (row < p.m && column(i) < k) store(grad + column(i), v);
-    }
-    if (kAhead) {
-#pragma unroll
-      for (int i = 0; i < kVectors; ++i) t[i] = next_t[i], g[i] = next_g[i], s[i] = next_s[i];
-    }
+    for (int i = 0; i < kCount; ++i) v[i] += r * (gv[i] - tv[i] * along);
+    if (row < p.m) part.store_row(static_cast<T*>(p.grad) + row * p.k, v);
+    if (kAhead) t = next_t, g = next_g, s = next_s;
   }
   if (!p.parts) return;
-  // A block's sums: the teams' of a warp, then the warps' one after the other, those of the same columns.
+  // A block's sums: the teams' of a warp, then the warps' one after the other.
   if constexpr (kThreads < 32) {
 #pragma unroll
-    for (int i = 0; i < kVectors; ++i)
+    for (int i = 0; i < kCount; ++i)
 #pragma unroll
-      for (int j = 0; j < kN; ++j)
-#pragma unroll
-        for (int d = kThreads; d < 32; d *= 2) dw[i][j] += __shfl_xor_sync(0xffffffffu, dw[i][j], d);
+      for (int d = kThreads; d < 32; d *= 2) dw[i] += __shfl_xor_sync(0xffffffffu, dw[i], d);
   }
-  extern __shared__ float shared_dw[];
-  constexpr int kSets = kThreads < 32 ? G::kBlock / 32 : G::kRows;  // of threads that share columns
+  extern __shared__ __align__(16) float columns[];  // k, where there are more sets than one
+  constexpr int kSets = kThreads < 32 ? G::kBlock / 32 : G::kRows;  // of threads with all of the columns
   const int set = kThreads < 32 ? threadIdx.x / 32 : threadIdx.x / kThreads;
+  float* const block_part = p.parts + int64_t(blockIdx.x) * p.k;
   for (int n = 0; n < kSets; ++n) {
     if (set == n && (kThreads >= 32 || threadIdx.x % 32 < kThreads)) {
+      if (n > 0) part.each(dw, [&](int c, float& v) { v += columns[c]; });
+      float* const to = n + 1 < kSets ? columns : block_part;
+      if constexpr (kWay == kWhole) {
 #pragma unroll
-      for (int i = 0; i < kVectors; ++i) {
+        for (int i = 0; i < kVectors; ++i)
+          if (i < part.count) {
 #pragma unroll
-        for (int j = 0; j < kN; ++j) {
-          float* const to = shared_dw + (j * kVectors + i) * kThreads + at;
-          if (n > 0) dw[i][j] += *to;
-          if (n + 1 < kSets)
-            *to = dw[i][j];
-          else if (column(i) < k)
-            p.parts[int64_t(blockIdx.x) * p.k + column(i) + j] = dw[i][j];
-        }
+            for (int j = 0; j < P::kN; j += 4) store_vector(to + part.place(i) + j, dw + i * P::kN + j);
+          }
+      } else {
+        part.each(dw, [&](int c, float v) { to[c] = v; });
       }
     }
     if (kSets > 1) __syncthreads();
@@ -445,25 +483,20 @@ __global__ void __launch_bounds__(kLong) long_norm_grad_kernel(const __grid_cons
   float* const part = p.parts ? p.parts + int64_t(blockIdx.x) * p.k : nullptr;
   for (int64_t row = blockIdx.x; row < p.m; row += gridDim.x) {
     const T *total = static_cast<const T*>(p.total) + row * p.total_stride,
-            *grad_out = static_cast<const T*>(p.grad_out) + row * p.grad_out_stride;
-    float sums[2] = {0.0f, 0.0f}, t[1], g[1], w[1] = {1.0f};
+            *grad_out = static_cast<const T*>(p.grad_out) + row * p.grad_out_stride,
+            *grad_total = p.grad_total ? static_cast<const T*>(p.grad_total) + row * p.grad_total_stride : nullptr;
+    const auto weighed_at = [&](int64_t c) { return weight ? load(grad_out + c) * load(weight + c) : load(grad_out + c); };
+    float sums[2] = {0.0f, 0.0f};
     for (int64_t c = threadIdx.x; c < p.k; c += kLong) {
-      load(total + c, t), load(grad_out + c, g);
-      if (weight) load(weight + c, w);
-      sums[0] = fmaf(t[0], t[0], sums[0]), sums[1] = fmaf(g[0] * w[0], t[0], sums[1]);
+      const float t = load(total + c);
+      sums[0] = fmaf(t, t, sums[0]), sums[1] = fmaf(weighed_at(c), t, sums[1]);
     }
     G::sum(sums, room);
     const float r = rsqrtf(sums[0] / float(p.k) + p.eps), along = r * (r * sums[1] / float(p.k));
     for (int64_t c = threadIdx.x; c < p.k; c += kLong) {
-      load(total + c, t), load(grad_out + c, g);
-      if (weight) load(weight + c, w);
-      float v[1] = {r * (g[0] * w[0] - t[0] * along)}, s[1];
-      if (p.grad_total) {
-        load(static_cast<const T*>(p.grad_total) + row * p.grad_total_stride + c, s);
-        v[0] += s[0];
-      }
-      store(static_cast<T*>(p.grad) + row * p.k + c, v);
-      if (part) part[c] = fmaf(g[0], t[0] * r, row == blockIdx.x ? 0.0f : part[c]);
+      const float t = load(total + c), v = r * (weighed_at(c) - t * along);
+      store(static_cast<T*>(p.grad) + row * p.k + c, grad_total ? v + load(grad_total + c) : v);
+      if (part) part[c] = fmaf(load(grad_out + c), t * r, row == blockIdx.x ? 0.0f : part[c]);
     }
   }
 }
@@ -485,109 +518,135 @@ __global__ void __launch_bounds__(256) add_rows_kernel(const float* __restrict__
   sum = room[column][threadIdx.x % 32];
 #pragma unroll
   for (int d = 16; d > 0; d /= 2) sum += __shfl_xor_sync(0xffffffffu, sum, d);
-  if (threadIdx.x % 32 == 0 && first + column < k) {
-    const float v[1] = {sum};
-    store(grad_weight + first + column, v);
-  }
+  if (threadIdx.x % 32 == 0 && first + column < k) store(grad_weight + first + column, sum);
 }
 
-bool on16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
+// Which way rows of k are moved: `rows` are the tensors and the values between their rows.
+struct Rows {
+  const void* at;
+  int64_t stride;
+};
+template <typename T>
+Way way_of(int64_t k, std::initializer_list<Rows> rows) {
+  constexpr int kN = 16 / int(sizeof(T));
+  bool whole = k % kN == 0, alike = k >= 8 * kN;
+  for (const Rows& r : rows) {
+    if (!r.at) continue;
+    const bool on_boundary = reinterpret_cast<uintptr_t>(r.at) % 16 == 0;
+    whole = whole && on_boundary && r.stride % kN == 0;
+    alike = alike && on_boundary && r.stride % kN == k % kN;
+  }
+  return whole ? kWhole : alike ? kSkewed : kSingle;
+}
 
 template <int kTeam, int kCount>
 struct Form {
   static constexpr int kThreads = kTeam, kVectors = kCount;
 };
-// Calls f with the form for rows of `vectors` vectors; false where none holds them.
-template <bool kWide, typename F>
-bool with_form(int64_t vectors, F&& f) {
-  if constexpr (kWide) {
-    if (vectors <= 8) return f(Form<8, 1>()), true;
-    if (vectors <= 16) return f(Form<16, 1>()), true;
-    if (vectors <= 32) return f(Form<32, 1>()), true;
-    if (vectors <= 64) return f(Form<32, 2>()), true;
-    if (vectors <= 128) return f(Form<32, 4>()), true;
-    if (vectors <= 512) return f(Form<128, 4>()), true;
-    if (vectors <= 2048) return f(Form<512, 4>()), true;
-    if (vectors <= 4096) return f(Form<512, 8>()), true;
-  } else {
-    if (vectors <= 32) return f(Form<32, 1>()), true;
-    if (vectors <= 128) return f(Form<32, 4>()), true;
-    if (vectors <= 256) return f(Form<32, 8>()), true;
-    if (vectors <= 1024) return f(Form<128, 8>()), true;
-    if (vectors <= 4096) return f(Form<512, 8>()), true;
-    if (vectors <= 16384) return f(Form<1024, 16>()), true;
+// Calls f with the way and the form for rows of k; false where none holds them.
+template <typename T, typename F>
+bool with_form(Way way, int64_t k, F&& f) {
+  constexpr int kN = 16 / int(sizeof(T));
+  const int64_t vectors = k / kN;
+  if (way == kWhole) {
+    const auto g = [&](auto form) { return f(std::integral_constant<Way, kWhole>(), form), true; };
+    if (vectors <= 8) return g(Form<8, 1>());
+    if (vectors <= 16) return g(Form<16, 1>());
+    if (vectors <= 32) return g(Form<32, 1>());
+    if (vectors <= 64) return g(Form<32, 2>());
+    if (vectors <= 128) return g(Form<32, 4>());
+    if (vectors <= 512) return g(Form<128, 4>());
+    if (vectors <= 2048) return g(Form<512, 4>());
+    if (vectors <= 4096) return g(Form<512, 8>());
+  } else if (way == kSkewed) {
+    const auto g = [&](auto form) { return f(std::integral_constant<Way, kSkewed>(), form), true; };
+    if (vectors <= 32) return g(Form<32, 1>());
+    if (vectors <= 64) return g(Form<32, 2>());
+    if (vectors <= 128) return g(Form<32, 4>());
+    if (vectors <= 512) return g(Form<128, 4>());
+    if (vectors <= 2048) return g(Form<512, 4>());
   }
+  const auto g = [&](auto form) { return f(std::integral_constant<Way, kSingle>(), form), true; };
+  if (k <= 32) return g(Form<32, 1>());
+  if (k <= 128) return g(Form<32, 4>());
+  if (k <= 256) return g(Form<32, 8>());
+  if (k <= 512) return g(Form<64, 8>());
+  if (k <= 1024) return g(Form<128, 8>());
+  if (k <= 4096) return g(Form<512, 8>());
+  if (k <= 16384) return g(Form<1024, 16>());
   return false;
 }
 // The gradient holds three rows, the next three and the weight's gradient.
-template <typename T, bool kWide, typename F>
-bool with_grad_form(int64_t vectors, F&& f) {
-  if constexpr (kWide) {
-    if (vectors <= 8) return f(Form<8, 1>()), true;
-    if (vectors <= 16) return f(Form<16, 1>()), true;
-    if (vectors <= 32) return f(Form<32, 1>()), true;
-    if (vectors <= 64) return f(Form<32, 2>()), true;
-    if (vectors <= 128) return f(Form<64, 2>()), true;
-    if (vectors <= 256) return f(Form<128, 2>()), true;
-    if (vectors <= 512) return f(Form<256, 2>()), true;
-    if (vectors <= 1024) return f(Form<512, 2>()), true;
-    if (vectors <= 2048) return f(Form<512, 4>()), true;
-    if (sizeof(T) == 4 && vectors <= 4096) return f(Form<512, 8>()), true;
-  } else {
-    if (vectors <= 32) return f(Form<32, 1>()), true;
-    if (vectors <= 128) return f(Form<32, 4>()), true;
-    if (vectors <= 256) return f(Form<32, 8>()), true;
-    if (vectors <= 512) return f(Form<64, 8>()), true;
-    if (vectors <= 1024) return f(Form<128, 8>()), true;
-    if (vectors <= 2048) return f(Form<256, 8>()), true;
-    if (vectors <= 4096) return f(Form<512, 8>()), true;
-    if (vectors <= 8192) return f(Form<512, 16>()), true;
+template <typename T, typename F>
+bool with_grad_form(Way way, int64_t k, F&& f) {
+  constexpr int kN = 16 / int(sizeof(T));
+  const int64_t vectors = k / kN;
+  if (way == kWhole) {
+    const auto g = [&](auto form) { return f(std::integral_constant<Way, kWhole>(), form), true; };
+    if (vectors <= 8) return g(Form<8, 1>());
+    if (vectors <= 16) return g(Form<16, 1>());
+    if (vectors <= 32) return g(Form<32, 1>());
+    if (vectors <= 64) return g(Form<32, 2>());
+    if (vectors <= 128) return g(Form<64, 2>());
+    if (vectors <= 256) return g(Form<128, 2>());
+    if (vectors <= 512) return g(Form<256, 2>());
+    if (vectors <= 1024) return g(Form<512, 2>());
+    if (vectors <= 2048) return g(Form<512, 4>());
+    if constexpr (sizeof(T) == 4)
+      if (vectors <= 4096) return g(Form<512, 8>());
+  } else if (way == kSkewed) {
+    const auto g = [&](auto form) { return f(std::integral_constant<Way, kSkewed>(), form), true; };
+    if (vectors <= 32) return g(Form<32, 1>());
+    if (vectors <= 64) return g(Form<32, 2>());
+    if (vectors <= 128) return g(Form<64, 2>());
+    if (vectors <= 256) return g(Form<128, 2>());
+    if (vectors <= 512) return g(Form<256, 2>());
+    if (vectors <= 1024) return g(Form<512, 2>());
+    if (vectors <= 2048) return g(Form<512, 4>());
   }
+  const auto g = [&](auto form) { return f(std::integral_constant<Way, kSingle>(), form), true; };
+  if (k <= 32) return g(Form<32, 1>());
+  if (k <= 128) return g(Form<32, 4>());
+  if (k <= 256) return g(Form<32, 8>());
+  if (k <= 512) return g(Form<64, 8>());
+  if (k <= 1024) return g(Form<128, 8>());
+  if (k <= 4096) return g(Form<512, 8>());
+  if (k <= 8192) return g(Form<512, 16>());
   return false;
 }
 
 template <typename T, bool kCodes>
 int norm(const Norm& p, cudaStream_t s) {
-  constexpr int kN = 16 / int(sizeof(T));
-  const bool wide = p.k % kN == 0 && on16(p.x) && on16(p.residual) && on16(p.weight) && on16(p.out) && on16(p.total) &&
-                    p.x_stride % kN == 0 && p.residual_stride % kN == 0 && (!kCodes || (on16(p.codes) && p.pitch % 16 == 0));
-  bool held;
-  if (wide)
-    held = with_form<true>(p.k / kN, [&](auto form) {
-      using G = Team<form.kThreads>;
-      norm_kernel<T, true, form.kThreads, form.kVectors, kCodes><<<unsigned((p.m + G::kRows - 1) / G::kRows), G::kBlock, 0, s>>>(p);
-    });
-  else
-    held = with_form<false>(p.k, [&](auto form) {
-      using G = Team<form.kThreads>;
-      norm_kernel<T, false, form.kThreads, form.kVectors, kCodes><<<unsigned((p.m + G::kRows - 1) / G::kRows), G::kBlock, 0, s>>>(p);
-    });
+  // codes start on boundaries of a vector's values where whole rows do
+  const Way way = way_of<T>(p.k, {{p.x, p.x_stride}, {p.residual, p.residual_stride}, {p.out, p.k}, {p.total, p.k}, {p.weight, p.k}});
+  const bool held = with_form<T>(kCodes && way == kWhole && (reinterpret_cast<uintptr_t>(p.codes) | p.pitch) % 16 ? kSingle : way,
+                                 p.k, [&](auto of_way, auto form) {
+    using G = Team<form.kThreads>;
+    norm_kernel<T, of_way.value, form.kThreads, form.kVectors, kCodes>
+        <<<unsigned((p.m + G::kRows - 1) / G::kRows), G::kBlock, 0, s>>>(p);
+  });
   if (!held) long_norm_kernel<T, kCodes><<<unsigned(p.m), kLong, 0, s>>>(p);
   return launch_status();
 }
 
+// Blocks of the gradient's kernel, each with a row of the weight's gradient in scratch: two an SM (128,000 x 512 bf16 87 us;
+// one 114, three 106, four 95), and of few rows fewer, so that a team has some. Multiples of 8 where it has more than one.
 constexpr int kGradBlocks = 2 * 148;
-// Blocks of the gradient's kernel, each with a row of the weight's gradient in scratch.
-int64_t grad_blocks(int64_t m) { return m < kGradBlocks ? m : kGradBlocks; }
+int64_t grad_blocks(int64_t rows) {
+  return rows <= 144 ? rows : rows < 4 * 144 ? 144 : rows < 4 * kGradBlocks ? rows / 4 / 8 * 8 : kGradBlocks;
+}
 
 template <typename T>
 int norm_grad(const NormGrad& p, void* grad_weight, cudaStream_t s) {
-  constexpr int kN = 16 / int(sizeof(T));
-  const bool wide = p.k % kN == 0 && on16(p.grad_out) && on16(p.total) && on16(p.weight) && on16(p.grad_total) &&
-                    on16(p.grad) && p.grad_out_stride % kN == 0 && p.total_stride % kN == 0 && p.grad_total_stride % kN == 0;
+  const Way way = way_of<T>(p.k, {{p.grad_out, p.grad_out_stride}, {p.total, p.total_stride}, {p.grad_total, p.grad_total_stride},
+                                  {p.grad, p.k}, {p.weight, p.k}});
   int64_t blocks = grad_blocks(p.m);
-  bool held;
-  const auto launch = [&](auto form, auto is_wide) {
-    constexpr bool kWide = decltype(is_wide)::value;
+  const bool held = with_grad_form<T>(way, p.k, [&](auto of_way, auto form) {
     using G = Team<form.kThreads>;
     blocks = grad_blocks((p.m + G::kRows - 1) / G::kRows);
-    const size_t shared = G::kRows > 1 ? form.kThreads * form.kVectors * Vec<T, kWide>::kValues * sizeof(float) : 0;  // the warps' sums
-    norm_grad_kernel<T, kWide, form.kThreads, form.kVectors><<<unsigned(blocks), G::kBlock, shared, s>>>(p);
-  };
-  if (wide)
-    held = with_grad_form<T, true>(p.k / kN, [&](auto form) { launch(form, std::true_type()); });
-  else
-    held = with_grad_form<T, false>(p.k, [&](auto form) { launch(form, std::false_type()); });
+    const size_t shared = G::kRows > 1 ? p.k * sizeof(float) : 0;
+    norm_grad_kernel<T, of_way.value, form.kThreads, form.kVectors><<<unsigned(blocks), G::kBlock, shared, s>>>(p);
+  });
   if (!held) long_norm_grad_kernel<T><<<unsigned(blocks), kLong, 0, s>>>(p);
   if (int rc = launch_status(); rc || !p.parts) return rc;
   add_rows_kernel<T><<<unsigned((p.k + 7) / 8), 256, 0, s>>>(p.parts, int(blocks), p.k, static_cast<T*>(grad_weight));
@@ -638,7 +697,7 @@ int rlenv_rms_norm_codes(int dtype, int64_t m, int64_t k, const void* x, int64_t
 int64_t rlenv_rms_norm_scratch_bytes(int64_t m, int64_t k) {
   using namespace rlenv;
   if (!norm_sizes(RLENV_F32, m, k)) return RLENV_EINVAL;
-  return grad_blocks(m) * k * 4;
+  return (m < kGradBlocks ? m : kGradBlocks) * k * 4;
 }
 
 int rlenv_rms_norm_backward(int dtype, int64_t m, int64_t k, const void* grad_out, int64_t grad_out_stride, const void* total,

@@ -103,7 +103,8 @@ def test_norm_in_8_bits(cuda, m, k, dtype):
 
 
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
-@pytest.mark.parametrize("m,k", NORM_SIZES + [(5000, 72), (4999, 33)])
+@pytest.mark.parametrize("m,k", NORM_SIZES + [(5000, 72), (4999, 33), (3000, 333), (701, 2049), (1300, 1001), (700, 4096),
+                                              (333, 8193)])
 def test_norm_backward(cuda, m, k, dtype):
     import rms_norm
 
@@ -172,6 +173,22 @@ def test_norm_of_rows_that_are_zero_or_not_finite(cuda):
         bad[5] *= 2.0 ** -110  # too small for codes of their own
         codes, scale = int8_linear.quantise(bad)
         assert torch.isnan(scale[1:4]).all() and not scale[4:].any() and not codes[1:].any() and scale[0] > 0
+
+
+@pytest.mark.parametrize("k", [8, 64, 100, 1000, 1001])
+def test_norm_without_epsilon(cuda, k):
+    """eps 0 is the formula too: rows that share a warp with rows past the last one are not touched by those."""
+    import rms_norm
+
+    t, g, w = normal(cuda, 1501, k), normal(cuda, 1501, k, seed=1), 1 + 0.2 * normal(cuda, k, seed=2)
+    want = policy.norm(to64(t), to64(w), 0.0)
+    close(rms_norm.forward(t, w, None, 0.0)[0], want, norm_tol(k, want, "f32"), "out")
+    grad, grad_weight = rms_norm.backward(g, t, w, 0.0)
+    args = (to64(g), to64(t), to64(w), 0.0)
+    (want, want_w), (mag, mag_w) = policy.norm_grad(*args), policy.norm_grad(*args, absolute=True)
+    n = 2.5 * chain(k) + 24
+    close(grad, want, n * HALF * mag, "grad")
+    close(grad_weight, want_w, (80 + n) * HALF * mag_w, "grad_weight")
 
 
 def test_codes_leave_the_bytes_past_a_row(cuda):
