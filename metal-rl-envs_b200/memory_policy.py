@@ -8,6 +8,11 @@ environments T times (cartpole_metal.step), keeping each environment's attention
 update, then runs the same T x N tokens through the trajectory form and takes one actor-critic step
 (Williams 1992's REINFORCE with a learned baseline). The environments' `dones` cut the memory at episode ends.
 
+With `fused` the norms and the loss's log-probabilities and entropy are kernels of this package too (rms_norm.apply,
+log_probs.apply): the same formulas, rounded in other places. With `act_bits` 8 the policy acts in 8-bit integers
+(rms_norm.forward8, int8_linear), its weights brought into 8 bits once an update; it trains in float32 as before, on
+what it did.
+
     python memory_policy.py --envs 1024 --steps 64 --updates 150
 
 The reference trains memoryless MLPs (es.py) and has no counterpart of this module.
@@ -21,8 +26,11 @@ import torch
 import adamw
 import cartpole_metal
 import gated_ffn
+import int8_linear
 import linear_attention
+import log_probs
 import rlenv_lib as _rl
+import rms_norm
 
 OBSERVED = (0, 2)  # cart position and pole angle; the velocities stay hidden
 
@@ -40,6 +48,8 @@ class Config:
     entropy: float = 0.01
     max_norm: float = 1.0    # of the gradient
     state_bits: int = 32     # of the optimizer's moments
+    act_bits: int = 32       # of the weights and activations while acting: 32 or 8
+    fused: int = 0           # 1: norms and scores by this package's kernels
     seed: int = 0
 
 
@@ -47,6 +57,8 @@ class MemoryPolicy:
     """tokens (..., features) -> action logits and value. Parameters are float32 leaves in `parameters`."""
 
     def __init__(self, cfg, features=len(OBSERVED) + 1, actions=2):
+        if cfg.act_bits not in (8, 32):
+            raise ValueError(f"act_bits must be 8 or 32; got {cfg.act_bits}")
         self.cfg = cfg
         dev, model = _rl.device(), cfg.heads * cfg.width
         g = torch.Generator(device=dev).manual_seed(cfg.seed)
@@ -68,21 +80,51 @@ class MemoryPolicy:
         c = self.cfg
         return torch.zeros((n, c.heads, c.width, c.width), device=self.decay.device)
 
+    def _normal(self, x):
+        return rms_norm.apply(x, eps=_EPS)[0] if self.cfg.fused else _normal(x)
+
     def _split(self, x):
         """q, k, v (..., H, D) as views of one product."""
-        qkv = (_normal(x) @ self.qkv).unflatten(-1, (3, self.cfg.heads, self.cfg.width))
+        qkv = (self._normal(x) @ self.qkv).unflatten(-1, (3, self.cfg.heads, self.cfg.width))
         return qkv.unbind(-3)
 
     def _rest(self, x, out):
-        x = x + out.flatten(-2) @ self.mix
-        x = x + gated_ffn.apply(_normal(x), self.gate, self.up, "silu") @ self.down
-        y = _normal(x) @ self.head
+        if self.cfg.fused:
+            y, x = rms_norm.apply(out.flatten(-2) @ self.mix, None, x, _EPS)
+            y, _ = rms_norm.apply(gated_ffn.apply(y, self.gate, self.up, "silu") @ self.down, None, x, _EPS)
+            y = y @ self.head
+        else:
+            x = x + out.flatten(-2) @ self.mix
+            x = x + gated_ffn.apply(_normal(x), self.gate, self.up, "silu") @ self.down
+            y = _normal(x) @ self.head
         return y[..., :-1], y[..., -1]
 
     @torch.no_grad()
-    def act(self, tokens, state, resets):
-        """One token for every environment, tokens (N, features); state (N, H, D, D) is updated in place."""
+    def quantised(self):
+        """The weights in 8 bits, for `act`."""
+        whole = {"qkv": self.qkv, "mix": self.mix, "gates": torch.cat([self.gate, self.up], 1), "down": self.down,
+                 "head": self.head}
+        return {name: int8_linear.quantise_weight(w) for name, w in whole.items()}
+
+    def _act_in_8_bits(self, x, state, resets, w):
+        """`act` after the embedding, x (N, model) float32, with the weights of `quantised`."""
+        f32 = torch.float32
+        codes, scale, _ = rms_norm.forward8(x, eps=_EPS)
+        qkv = int8_linear.forward(codes, scale, w["qkv"], f32).unflatten(-1, (3, self.cfg.heads, self.cfg.width))
+        out = linear_attention.step(*qkv.unbind(-3), self.decay, state, resets)
+        codes, scale, x = rms_norm.forward8(int8_linear.product(out.flatten(-2), w["mix"]), None, x, _EPS)
+        gate, up = int8_linear.forward(codes, scale, w["gates"], f32).chunk(2, -1)
+        codes, scale, _ = rms_norm.forward8(int8_linear.product(torch.nn.functional.silu(gate) * up, w["down"]), None, x, _EPS)
+        y = int8_linear.forward(codes, scale, w["head"], f32)
+        return y[..., :-1], y[..., -1]
+
+    @torch.no_grad()
+    def act(self, tokens, state, resets, weights=None):
+        """One token for every environment, tokens (N, features); state (N, H, D, D) is updated in place. weights: those of
+        `quantised`, to act in 8 bits."""
         x = tokens @ self.embed
+        if weights is not None:
+            return self._act_in_8_bits(x, state, resets, weights)
         return self._rest(x, linear_attention.step(*self._split(x), self.decay, state, resets))
 
     def trajectory(self, tokens, state, resets):
@@ -92,9 +134,12 @@ class MemoryPolicy:
         return self._rest(x, out)
 
 
+_EPS = 1e-6
+
+
 def _normal(x):
     """Root-mean-square normalisation."""
-    return x * torch.rsqrt(x.square().mean(-1, keepdim=True) + 1e-6)
+    return x * torch.rsqrt(x.square().mean(-1, keepdim=True) + _EPS)
 
 
 def observe(state):
@@ -117,10 +162,11 @@ class Rollout:
 def collect(policy, env_state, memory, resets, steps, generator):
     """(Rollout, env_state, memory, resets) after `steps` steps of every environment."""
     start = memory.clone()
+    weights = policy.quantised() if policy.cfg.act_bits == 8 else None
     tokens, actions, rewards, dones, first, logits = [], [], [], [], resets, []
     for _ in range(steps):
         x = observe(env_state)
-        y, _ = policy.act(x, memory, resets)
+        y, _ = policy.act(x, memory, resets, weights)
         a = torch.multinomial(torch.softmax(y, -1), 1, generator=generator)[:, 0]
         env_state, reward, done = cartpole_metal.step(env_state, a)
         for kept, new in ((tokens, x), (actions, a), (rewards, reward), (dones, done), (logits, y)):
@@ -140,17 +186,27 @@ def returns_of(rewards, dones, values, discount):
     return out
 
 
-def update(policy, optimizer, rollout):
-    """One actor-critic step on a rollout; returns the loss."""
+def loss_of(policy, rollout):
+    """The actor-critic loss of a rollout, differentiable in the parameters."""
     cfg = policy.cfg
     logits, values = policy.trajectory(rollout.tokens, rollout.memory, rollout.resets)
     returns = returns_of(rollout.rewards, rollout.dones, values.detach(), cfg.discount)
     gain = returns - values.detach()
     gain = (gain - gain.mean()) / (gain.std() + 1e-6)
-    logp = torch.log_softmax(logits, -1)
-    chosen = logp.gather(-1, rollout.actions[..., None].long())[..., 0]
-    entropy = -(logp.exp() * logp).sum(-1).mean()
-    loss = -(gain * chosen).mean() + 0.5 * torch.nn.functional.smooth_l1_loss(values, returns) - cfg.entropy * entropy
+    if cfg.fused:
+        chosen, entropy = log_probs.apply(logits, rollout.actions)
+        entropy = entropy.mean()
+    else:
+        logp = torch.log_softmax(logits, -1)
+        chosen = logp.gather(-1, rollout.actions[..., None].long())[..., 0]
+        entropy = -(logp.exp() * logp).sum(-1).mean()
+    return -(gain * chosen).mean() + 0.5 * torch.nn.functional.smooth_l1_loss(values, returns) - cfg.entropy * entropy
+
+
+def update(policy, optimizer, rollout):
+    """One actor-critic step on a rollout; returns the loss."""
+    cfg = policy.cfg
+    loss = loss_of(policy, rollout)
     grads = torch.autograd.grad(loss, policy.parameters)
     norm = torch.stack([g.square().sum() for g in grads]).sum().sqrt()
     with torch.no_grad():

@@ -612,3 +612,59 @@ def test_operators_in_a_captured_graph_and_on_other_streams(cuda):
         torch.cuda.synchronize()
         for which in (0, 1):
             assert all(torch.equal(a, b) for a, b in zip(outs[which], want[order[which]]))
+
+
+# ---- the policy that runs them together ------------------------------------------------------------------------
+
+def rollout_of(cfg):
+    import cartpole_metal
+    import memory_policy as mp
+
+    policy = mp.MemoryPolicy(cfg)
+    g = torch.Generator(device=policy.decay.device).manual_seed(0)
+    cartpole_metal.reseed(5)
+    state, memory = cartpole_metal.reset(cfg.envs), policy.fresh_state(cfg.envs)
+    resets = torch.ones(cfg.envs, dtype=torch.bool, device=policy.decay.device)
+    return policy, mp.collect(policy, state, memory, resets, cfg.steps, g)[0]
+
+
+def test_the_policys_gradients_with_and_without_the_fused_operators(cuda):
+    """The same rollout's loss and gradients, norms and scores by torch and by the kernels: some twenty chained float32
+    operations of up to 2,000 terms, each within 2^-16 of the sum of its terms' magnitudes."""
+    import memory_policy as mp
+
+    cfg = mp.Config(envs=33, steps=40)
+    policy, rollout = rollout_of(cfg)
+    found = []
+    for fused in (0, 1):
+        cfg.fused = fused
+        loss = mp.loss_of(policy, rollout)
+        found.append((loss, torch.autograd.grad(loss, policy.parameters)))
+    (loss, grads), (loss1, grads1) = found
+    assert abs(loss.item() - loss1.item()) <= 1e-3 * (1 + abs(loss.item()))
+    for a, b in zip(grads, grads1):
+        assert torch.isfinite(b).all() and (a - b).abs().max() <= 2e-3 * a.abs().max()
+
+
+def test_the_policy_acts_in_8_bits(cuda):
+    """Logits acted on in 8 bits against the trajectory form's in float32. A code is off by half of a 127th of its row's
+    largest magnitude at most, which is below five times the root mean square of rows of 64 to 128 such values: 2% of that
+    for a token's codes and for a channel's, as many independent errors as terms, so below 3% a product; five in a row
+    below 7%, and a norm keeps a relative error."""
+    import memory_policy as mp
+
+    cfg = mp.Config(envs=65, steps=30, act_bits=8)
+    policy, rollout = rollout_of(cfg)
+    logits, _ = policy.trajectory(rollout.tokens, rollout.memory, rollout.resets)
+    off, size = (logits - rollout.logits).norm(), logits.norm()
+    assert 0 < off <= 0.1 * size
+    with pytest.raises(ValueError, match="act_bits"):
+        mp.MemoryPolicy(mp.Config(act_bits=4))
+
+
+@pytest.mark.parametrize("act_bits,fused", [(8, 0), (32, 1), (8, 1)])
+def test_the_policy_trains_with_them(cuda, act_bits, fused):
+    import memory_policy as mp
+
+    policy, lengths = mp.train(mp.Config(envs=64, steps=16, updates=3, act_bits=act_bits, fused=fused))
+    assert len(lengths) == 3 and all(torch.isfinite(p).all() for p in policy.parameters)
