@@ -106,6 +106,7 @@ class _Apply(torch.autograd.Function):
     def forward(ctx, logits, actions, allowed):
         scores = forward(logits, actions, allowed)
         ctx.save_for_backward(logits, actions, allowed, scores.normalizer, scores.entropy)
+        ctx.set_materialize_grads(False)
         return scores.log_prob, scores.entropy
 
     @staticmethod

@@ -116,12 +116,15 @@ class _Apply(torch.autograd.Function):
         out, total = forward(x, weight, residual, eps)
         ctx.save_for_backward(total, weight)
         ctx.eps, ctx.with_residual = eps, residual is not None
+        ctx.set_materialize_grads(False)
         return (out, total) if ctx.with_residual else out
 
     @staticmethod
     @once_differentiable
     def backward(ctx, grad_out, grad_total=None):
         total, weight = ctx.saved_tensors
+        if grad_out is None:  # the norm is not used
+            return grad_total, None, grad_total if ctx.with_residual else None, None
         grad, grad_weight = backward(grad_out, total, weight, ctx.eps, grad_total)
         return grad, grad_weight, grad if ctx.with_residual else None, None
 

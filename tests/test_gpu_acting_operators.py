@@ -231,9 +231,14 @@ def test_norm_through_autograd(cuda, with_residual):
     close(grads[1], want_w, n * HALF * mag_w, "weight")
     if with_residual:
         assert torch.equal(grads[0], grads[2])
-    only = torch.autograd.grad(rms_norm.apply(*leaves)[1].sum() if with_residual else rms_norm.apply(*leaves)[0].sum(),
-                               leaves[0])[0]
-    assert torch.isfinite(only).all()
+    outs = rms_norm.apply(leaves[0], leaves[1], leaves[2] if with_residual else None, 1e-5)
+    alone = torch.autograd.grad((outs[0] * g).sum(), leaves, retain_graph=True)
+    want, want_w = policy.norm_grad(*args[:4])
+    close(alone[0].reshape(15, 40), want, n * HALF * mag, "x without the total")
+    close(alone[1], want_w, n * HALF * mag_w, "weight without the total")
+    if with_residual:  # the total alone: the weight has no part in it
+        alone = torch.autograd.grad((outs[1] * gt).sum(), leaves, allow_unused=True)
+        assert torch.equal(alone[0], gt) and alone[1] is None and torch.equal(alone[2], gt)
     with pytest.raises(RuntimeError):
         again = torch.autograd.grad(rms_norm.apply(*leaves)[0].square().sum(), leaves[0], create_graph=True)[0]
         torch.autograd.grad(again.sum(), leaves[0])
@@ -484,6 +489,58 @@ def test_scores_where_rows_are_odd(cuda, v):
     assert not grad[6:9, v - 1].any() and torch.isfinite(grad[6:9]).all()
 
 
+def test_the_check_build_reports_actions_outside(cuda):
+    import ctypes
+
+    lib = ctypes.CDLL(str(rlenv_lib.CHECKS_LIB_PATH))
+    for name in ("rlenv_log_probs_forward", "rlenv_log_probs_backward", "rlenv_checks_status"):
+        getattr(lib, name).argtypes = rlenv_lib._SIGNATURES[name]
+    word = ctypes.c_uint(0)
+    for v in (5, 100, 3000):
+        l, out = normal(cuda, 4, v), torch.empty((3, 4), device=cuda)
+        for last, want in ((v - 1, 0), (v, 1)):
+            actions = torch.tensor([0, -1, 1, last], device=cuda)
+            assert lib.rlenv_checks_status(ctypes.byref(word), 1) == 0
+            assert lib.rlenv_log_probs_forward(rlenv_lib.F32, 4, v, l.data_ptr(), v, actions.data_ptr(), rlenv_lib.I64, 0, 0,
+                                               out[0].data_ptr(), out[1].data_ptr(), out[2].data_ptr(), 0, 0, 0, 0) == 0
+            torch.cuda.synchronize()
+            assert lib.rlenv_checks_status(ctypes.byref(word), 1) == 0 and word.value & 1 == want
+            assert lib.rlenv_log_probs_backward(rlenv_lib.F32, 4, v, out[0].data_ptr(), 0, l.data_ptr(), v,
+                                                actions.data_ptr(), rlenv_lib.I64, out[2].data_ptr(), out[1].data_ptr(), 0, 0,
+                                                l.data_ptr(), 0) == 0
+            torch.cuda.synchronize()
+            assert lib.rlenv_checks_status(ctypes.byref(word), 1) == 0 and word.value & 1 == want
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("v", [7, 60, 250, 400, 1500, 5000, 40_000, 140_000])
+def test_scores_of_rows_that_grow(cuda, v, dtype):
+    """Rows whose largest logits come late, by steps and at once, after the type's lowest value too: the sums' base moves,
+    and stands 20 below the largest logit at most, so that a sum's error counts up to 20 times in the entropy."""
+    import log_probs
+
+    low = torch.finfo(TYPES[dtype]).min
+    l = normal(cuda, 8, v, seed=3)
+    l[1] = torch.arange(v, device=cuda) * (300.0 / v)
+    l[2] = -l[1]
+    l[3] = torch.arange(v, device=cuda) // (v // 3) * 19.0
+    l[4, -1] = 1e4
+    l[5, : v // 2] = low
+    l[6, :-1] = low
+    l[7] = low
+    l = l.to(TYPES[dtype])
+    actions = torch.full((8,), v - 1, device=cuda)
+    got = log_probs.forward(l, actions, None, 5)
+    l64 = to64(l)
+    lp, h, z, every = policy.scores(l64, actions.cpu().numpy())
+    z_off, h_off = score_bounds(l64, None, v)
+    extra = (chain(v) + 8) * 20 * 2 ** -23
+    close(got.normalizer, z, z_off + extra, "normalizer")
+    close(got.entropy, h, h_off + extra, "entropy")
+    close(got.log_prob, lp, z_off + extra + HALF * abs(lp) + 2 ** -23, "log_prob")
+    assert np.array_equal(got.top_actions.cpu().numpy(), policy.best(l64, 5))
+
+
 def grad_tol(g, h, l, actions, allowed, dtype):
     lp, entropy, z, every = policy.scores(l, actions, allowed)
     z_off, h_off = score_bounds(l, allowed, l.shape[1])
@@ -542,6 +599,10 @@ def test_scores_through_autograd(cuda, kind):
     want, tol = grad_tol(g64, np.full(30, 0.3), to64(l)[..., :9].reshape(30, 9), actions.long().cpu().numpy().reshape(30),
                          allowed.cpu().numpy().reshape(30, 9), "f32")
     close(grad[..., :9].reshape(30, 9), want, tol, "grad")
+    alone, = torch.autograd.grad(0.3 * log_probs.apply(l[..., :9], actions, allowed)[1].sum(), l)
+    want, tol = grad_tol(np.zeros(30), np.full(30, 0.3), to64(l)[..., :9].reshape(30, 9),
+                         actions.long().cpu().numpy().reshape(30), allowed.cpu().numpy().reshape(30, 9), "f32")
+    close(alone[..., :9].reshape(30, 9), want, tol, "the entropy's gradient alone")
 
 
 def test_scores_of_no_rows_and_refusals(cuda):
@@ -612,6 +673,37 @@ def test_operators_in_a_captured_graph_and_on_other_streams(cuda):
         torch.cuda.synchronize()
         for which in (0, 1):
             assert all(torch.equal(a, b) for a, b in zip(outs[which], want[order[which]]))
+
+
+def test_calls_at_the_same_time(cuda):
+    """Two streams run the same operators on other inputs at once, over and over: nothing is shared between them."""
+    import int8_linear
+    import log_probs
+    import rms_norm
+
+    def inputs(seed):
+        return (normal(cuda, 700, 2048, seed=seed), normal(cuda, 64, 50_000, seed=seed + 1),
+                int8_linear.quantise_weight(normal(cuda, 2048, 300, seed=seed + 2)))
+
+    def everything(x, l, weight):
+        c, s, _ = rms_norm.forward8(x)
+        grad, grad_weight = rms_norm.backward(x, x, x[0])
+        got = log_probs.forward(l, torch.arange(64, device=cuda), None, 9)
+        return [int8_linear.forward(c, s, weight), int8_linear.forward(c[:100], s[:100], weight), grad, grad_weight, *got]
+
+    sets, streams = [inputs(0), inputs(10)], [torch.cuda.Stream(), torch.cuda.Stream()]
+    want = [everything(*x) for x in sets]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(10):
+        for i in (0, 1):
+            with torch.cuda.stream(streams[i]):
+                got[i].append(everything(*sets[i]))
+    torch.cuda.synchronize()
+    for i in (0, 1):
+        for run in got[i]:
+            assert all(torch.equal(a, b) for a, b in zip(run, want[i]))
+    assert int8_linear.gave_up() == 0
 
 
 # ---- the policy that runs them together ------------------------------------------------------------------------
