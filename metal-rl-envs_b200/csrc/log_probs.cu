@@ -310,20 +310,28 @@ RLENV_D void cut_out(uint32_t (&w)[4], uint2 bytes) {
     w[k] = (w[k] & open) | (empty_word<T>() & ~open);
   }
 }
-// A vector that a row's end cuts: -infinity where a place is not in the row or not allowed.
+// A vector that a row's end cuts: -infinity where a place is not in the row or not allowed. All loads go out before any is
+// looked at.
 template <typename T>
 __device__ __noinline__ uint4 edge_vector(const T* row, const uint8_t* allowed, int64_t v, int64_t j0) {
   constexpr int kValues = 16 / int(sizeof(T));
+  float x[kValues];
+  uint8_t open[kValues];
+#pragma unroll
+  for (int j = 0; j < kValues; ++j) {
+    const bool in = j0 + j >= 0 && j0 + j < v;
+    x[j] = -infinity(), open[j] = 1;
+    if (in) x[j] = value_at(row + j0 + j);
+    if (in && allowed) open[j] = __ldg(allowed + j0 + j);
+  }
   uint32_t w[4] = {0, 0, 0, 0};
 #pragma unroll
   for (int j = 0; j < kValues; ++j) {
-    const int64_t place = j0 + j;
-    const bool open = place >= 0 && place < v && (!allowed || allowed[place]);
-    const uint32_t x = __float_as_uint(open ? value_at(row + place) : -infinity());
+    const uint32_t bits = open[j] ? __float_as_uint(x[j]) : 0xff800000u;
     if constexpr (sizeof(T) == 4)
-      w[j] = x;
+      w[j] = bits;
     else
-      w[j / 2] |= x >> 16 << 16 * (j % 2);
+      w[j / 2] |= bits >> 16 << 16 * (j % 2);
   }
   return make_uint4(w[0], w[1], w[2], w[3]);
 }

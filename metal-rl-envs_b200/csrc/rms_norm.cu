@@ -556,6 +556,7 @@ bool with_form(Way way, int64_t k, F&& f) {
     if (vectors <= 64) return g(Form<32, 2>());
     if (vectors <= 128) return g(Form<32, 4>());
     if (vectors <= 512) return g(Form<128, 4>());
+    if (vectors <= 1024) return g(Form<256, 4>());
     if (vectors <= 2048) return g(Form<512, 4>());
     if (vectors <= 4096) return g(Form<512, 8>());
   } else if (way == kSkewed) {
@@ -564,6 +565,7 @@ bool with_form(Way way, int64_t k, F&& f) {
     if (vectors <= 64) return g(Form<32, 2>());
     if (vectors <= 128) return g(Form<32, 4>());
     if (vectors <= 512) return g(Form<128, 4>());
+    if (vectors <= 1024) return g(Form<256, 4>());
     if (vectors <= 2048) return g(Form<512, 4>());
   }
   const auto g = [&](auto form) { return f(std::integral_constant<Way, kSingle>(), form), true; };
