@@ -126,10 +126,9 @@ struct Chosen {
   }
 };
 
-RLENV_D void write_scores(const Scores& p, int64_t row, const Sums& sums, const Chosen& chosen) {
-  const float log_s = logf(sums.s), normalizer = base_of(sums.m) + log_s;
+RLENV_D void write_scores(const Scores& p, int64_t row, const Sums& sums, float normalizer, const Chosen& chosen) {
   p.normalizer[row] = normalizer;
-  p.entropy[row] = sums.s == 0.0f ? 0.0f : log_s - sums.w / sums.s;
+  p.entropy[row] = sums.s == 0.0f ? 0.0f : logf(sums.s) - sums.w / sums.s;
   check_flag(chosen.action >= p.v, kCheckActionRange);
   p.log_prob[row] = chosen.action < 0 ? 0.0f : chosen.action >= p.v ? not_a_number() : log_prob_of(chosen.l, normalizer);
 }
@@ -184,9 +183,9 @@ __global__ void __launch_bounds__(256) few_scores_kernel(const __grid_constant__
     sums.s += __shfl_xor_sync(0xffffffffu, sums.s, d);
     sums.w += __shfl_xor_sync(0xffffffffu, sums.w, d);
   }
-  if (sub == 0 && at < p.m) write_scores(p, row, sums, chosen);
-  if (p.top == 0) return;
   const float normalizer = normalizer_of(sums);
+  if (sub == 0 && at < p.m) write_scores(p, row, sums, normalizer, chosen);
+  if (p.top == 0) return;
   uint32_t taken = 0;
   for (int r = 0; r < p.top; ++r) {
     uint64_t best = 0;
@@ -352,16 +351,32 @@ struct Best {
   };
   int count;
   RLENV_D void add(uint64_t key) { keys[atomicAdd(&count, 1)] = key; }
-  // Keeps the best `top` keys, in order. The smallest of them, or 0 where there are fewer. For the whole warp.
+  // Keeps the best `top` keys, in order. The smallest of them, or 0 where there are fewer. For the whole warp. Few are
+  // ranked by counting, of many (a row of equal logits) the largest is taken out, one after the other.
   RLENV_D uint64_t keep(int top) {
     __syncwarp();
     const int lane = threadIdx.x % 32, n = count;
-    for (int i = lane; i < n; i += 32) {
-      const uint64_t key = keys[i];
-      int above = 0;
+    if (n <= kMany + 32) {
+      for (int i = lane; i < n; i += 32) {
+        const uint64_t key = keys[i];
+        int above = 0;
 #pragma unroll 4
-      for (int k = 0; k < n; ++k) above += keys[k] > key;
-      if (above < top) kept[above] = key;
+        for (int k = 0; k < n; ++k) above += keys[k] > key;
+        if (above < top) kept[above] = key;
+      }
+    } else {
+      uint64_t last = ~uint64_t(0);
+      for (int r = 0; r < top; ++r) {
+        uint64_t own = 0;
+        for (int i = lane; i < n; i += 32) {
+          const uint64_t key = keys[i];
+          if (key < last && key > own) own = key;
+        }
+        const uint32_t high = __reduce_max_sync(0xffffffffu, uint32_t(own >> 32)),
+                       low = __reduce_max_sync(0xffffffffu, uint32_t(own >> 32) == high ? uint32_t(own) : 0u);
+        last = uint64_t(high) << 32 | low;
+        if (lane == 0) kept[r] = last;
+      }
     }
     __syncwarp();
     if (lane < top && lane < n) keys[lane] = kept[lane];
@@ -445,22 +460,20 @@ scores_kernel(const __grid_constant__ Scores p) {
     return larger_words<T>(larger_words<T>(w[0], w[1]), larger_words<T>(w[2], w[3]));
   };
   const auto words = [](uint4 q, uint32_t (&w)[4]) { w[0] = q.x, w[1] = q.y, w[2] = q.z, w[3] = q.w; };
-  // Whether all of a warp's vectors of a turn are whole ones.
-  const auto inside = [&](int from) { return from >= first_whole && from + kTurn - kStride + 32 <= last_whole; };
   const auto issue = [&](int turn, int slot) {
     if (turn < turns) {
-      const int from = warp_begin + turn * kTurn;
+      const int from = warp_begin + turn * kTurn, first = from + lane;
       uint4* const to = ring + slot * (kSteps * 32) + lane;
       const uint32_t to_at = uint32_t(__cvta_generic_to_shared(to));
-      const T* const at = grid.row + grid.place(from + lane);
-      if (inside(from)) {
+      const T* const at = grid.row + grid.place(first);
+      if (from >= first_whole && from + kTurn - kStride + 32 <= last_whole) {  // nothing but whole vectors
 #pragma unroll
         for (int u = 0; u < kSteps; ++u)
           asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to_at + u * 512), "l"(at + u * kStride * kValues) : "memory");
       } else {
 #pragma unroll 1
         for (int u = 0; u < kSteps; ++u) {
-          const int i = from + u * kStride + lane;
+          const int i = first + u * kStride;
           if (whole(i))
             asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to_at + u * 512), "l"(at + u * kStride * kValues) : "memory");
           else if (i < end)
@@ -547,6 +560,26 @@ scores_kernel(const __grid_constant__ Scores p) {
     const int each_bits = 2 + epoch_bits, total = best.choose(p.top, at_epoch, least) << each_bits;
     static_assert(kSteps == 4, "a group's vectors are 4 a turn");
     uint64_t least_key = uint64_t(least) << 32;
+    const auto look_at = [&](int i, const uint32_t (&w)[4]) {  // vector i, for the whole warp
+      const float bar = value_of(uint32_t(least_key >> 32));
+      if (i < end && !(largest_of<T>(largest_word(w)) < bar)) {
+        uint32_t reach = 0;
+#pragma unroll
+        for (int j = 0; j < kValues; ++j) reach |= !(word_value<T>(w, j) < bar) ? 1u << j : 0u;
+        const int place0 = int(grid.place(i));
+        for (; reach; reach &= reach - 1) {
+          const int j = __ffs(reach) - 1, place = place0 + j;
+          const uint32_t word = kValues == 4 ? (j < 2 ? (j < 1 ? w[0] : w[1]) : (j < 3 ? w[2] : w[3]))
+                                             : (j < 4 ? (j < 2 ? w[0] : w[1]) : (j < 6 ? w[2] : w[3]));
+          const float x = __uint_as_float(kValues == 4 ? word : j % 2 ? word & 0xffff0000u : word << 16);
+          const uint64_t key = key_of(x, uint32_t(place));
+          if (key > least_key && place >= 0 && place < p.v) best.add(key);
+        }
+      }
+      __syncwarp();
+      if (best.count > Best::kMany)
+        if (const uint64_t now = best.keep(p.top)) least_key = now;
+    };
     for (int first = 0; first < total; first += 32 * kSteps) {  // kSteps vectors of a lane on their way together
       uint4 q[kSteps];
       int at[kSteps];
@@ -554,6 +587,7 @@ scores_kernel(const __grid_constant__ Scores p) {
       for (int u = 0; u < kSteps; ++u) {
         const int t = first + 32 * u + lane;
         at[u] = end;
+        if (first + 32 * u >= total) continue;
         if (t < total) {
           const int group = best.groups[t >> each_bits];
           at[u] = warp_begin + ((group / 32 << each_bits) + (t & ((1 << each_bits) - 1))) * kStride + group % 32;
@@ -563,37 +597,21 @@ scores_kernel(const __grid_constant__ Scores p) {
 #pragma unroll
       for (int u = 0; u < kSteps; ++u) {
         if (first + 32 * u >= total) break;
+        uint32_t of[4] = {0, 0, 0, 0};
         if (at[u] < end) {
-          uint32_t w[4];
           if (!whole(at[u])) q[u] = edge_vector(grid.row, allowed, p.v, grid.place(at[u]));
-          words(q[u], w);
-          if (allowed && whole(at[u])) cut_out<T>(w, bytes_at<kValues>(allowed, grid.place(at[u]), p.v));
-          const float bar = value_of(uint32_t(least_key >> 32));
-          if (!(largest_of<T>(largest_word(w)) < bar)) {
-            uint32_t reach = 0;
-#pragma unroll
-            for (int j = 0; j < kValues; ++j) reach |= !(word_value<T>(w, j) < bar) ? 1u << j : 0u;
-            const int place0 = int(grid.place(at[u]));
-            for (; reach; reach &= reach - 1) {
-              const int j = __ffs(reach) - 1, place = place0 + j;
-              const uint32_t word = kValues == 4 ? (j < 2 ? (j < 1 ? w[0] : w[1]) : (j < 3 ? w[2] : w[3]))
-                                                 : (j < 4 ? (j < 2 ? w[0] : w[1]) : (j < 6 ? w[2] : w[3]));
-              const float x = __uint_as_float(kValues == 4 ? word : j % 2 ? word & 0xffff0000u : word << 16);
-              const uint64_t key = key_of(x, uint32_t(place));
-              if (key > least_key && place >= 0 && place < p.v) best.add(key);
-            }
-          }
+          words(q[u], of);
+          if (allowed && whole(at[u])) cut_out<T>(of, bytes_at<kValues>(allowed, grid.place(at[u]), p.v));
         }
-        __syncwarp();
-        if (best.count > Best::kMany)
-          if (const uint64_t now = best.keep(p.top)) least_key = now;
+        look_at(at[u], of);
       }
     }
     best.keep(p.top);
   }
   if constexpr (kWarps == 1) {
-    if (lane == 0) write_scores(p, row, sums, chosen);
-    if (lane < p.top) write_top(p, row, lane, best.kept[lane], normalizer_of(sums));
+    const float normalizer = normalizer_of(sums);
+    if (lane == 0) write_scores(p, row, sums, normalizer, chosen);
+    if (lane < p.top) write_top(p, row, lane, best.kept[lane], normalizer);
     return;
   }
 
@@ -615,10 +633,10 @@ scores_kernel(const __grid_constant__ Scores p) {
   if (threadIdx.x < kMostTop) top_of_block[threadIdx.x] = 0;
   __syncthreads();  // the rings are free
   sums = of_team<kWarps>(of_warps[lane % kWarps]);
-  if (blocks == 1 && threadIdx.x == 0) write_scores(p, row, sums, chosen);
+  const float normalizer = normalizer_of(sums);
+  if (blocks == 1 && threadIdx.x == 0) write_scores(p, row, sums, normalizer, chosen);
   if (p.top > 0) {
     if (lane < p.top) lists[warp * p.top + lane] = lane < best.count ? best.kept[lane] : 0;
-    const float normalizer = normalizer_of(sums);
     rank_all(kWarps * p.top, [&](int r, uint64_t key) {
       if (blocks == 1)
         write_top(p, row, r, key, normalizer);
@@ -633,9 +651,9 @@ scores_kernel(const __grid_constant__ Scores p) {
   cluster.sync();
   if (rank == 0) {
     sums = of_team<8>(lane % 8 < blocks ? *cluster.map_shared_rank(&of_block, lane % 8) : Sums{-infinity(), 0.0f, 0.0f});
-    if (threadIdx.x == 0) write_scores(p, row, sums, chosen);
+    const float normalizer = normalizer_of(sums);
+    if (threadIdx.x == 0) write_scores(p, row, sums, normalizer, chosen);
     if (p.top > 0) {
-      const float normalizer = normalizer_of(sums);
       for (int i = threadIdx.x; i < 8 * kMostTop; i += kStride)
         if (i / kMostTop < blocks && i % kMostTop < p.top)
           lists[i / kMostTop * p.top + i % kMostTop] = cluster.map_shared_rank(top_of_block, i / kMostTop)[i % kMostTop];
@@ -844,13 +862,15 @@ int scores_of(const Scores& p, cudaStream_t s) {
   if (p.v <= 4 * kEach) return few_scores<T, 4>(p, s);
   if (p.v <= 8 * kEach) return few_scores<T, 8>(p, s);
   if (p.v <= 32 * kEach) return few_scores<T, 32>(p, s);
-  // As few warps a row as fill the GPU, 16 an SM, with a vector a lane at least; of few rows a cluster of blocks that have a
-  // turn each (one row of 50,021 bf16 5.0 us, one block 6.7; 20 of 30,000 float32 8.2, with a vector a thread 11.0).
-  const int64_t vectors = p.v / kValues, enough = 16 * 148;
-  if (p.m >= enough || vectors <= 64) return scores<T, 1>(p, 1, s);
-  if (p.m * 4 >= enough || vectors <= 256) return scores<T, 4>(p, 1, s);
+  // As few warps a row as fill the GPU, or fewer where a row is short: what a row's end costs, its warps' joining above all,
+  // is paid by more rows at a time (567 rows of 4,341 float32 by 4 warps 7.9 us, by 16 18.0; 300 of 10,000 8.4 and 15.6; 1,000 of
+  // 3,000 bf16 by one 7.9, by 4 9.8; but 1,300 of 100,000 bf16 by 4 53, by one 91). Of few long rows a cluster of blocks that
+  // have a turn each (one row of 50,021 bf16 5.0 us, one block 6.7; 20 of 30,000 float32 8.2, with a vector a thread 11.0).
+  const int64_t vectors = p.v / kValues;
+  if (p.m >= 16 * 148 || vectors <= 64 || (vectors <= 512 && p.m >= 4 * 148)) return scores<T, 1>(p, 1, s);
+  if (p.m >= 2 * 148 || vectors <= 256) return scores<T, 4>(p, 1, s);
   int blocks = 1;
-  while (blocks < 8 && p.m * 16 * blocks < enough && vectors > 2048 * blocks) blocks *= 2;
+  while (blocks < 8 && p.m * 16 * blocks < 8 * 148 && vectors > 2048 * blocks) blocks *= 2;
   return scores<T, 16>(p, blocks, s);
 }
 
