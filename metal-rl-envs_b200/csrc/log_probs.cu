@@ -6,8 +6,8 @@
 //
 // A row is read once: any number will do for b that is not far below the largest logit, so that sums begin with the first
 // vectors and nothing waits for a largest one. The bound is memory, with the power unit close behind (a logit is one
-// power, 16 a clock and SM, and some 8 instructions of which half work on two values): 4,096 x 32,768 bf16 53 us (5.0 TB/s),
-// 2,048 x 32,768 float32 47 (5.7 TB/s), with eight alternatives 71 and 4,096 x 32,768 bf16 with a mask 76 (5.3 TB/s); the gradient
+// power, 16 a clock and SM, and some 8 instructions of which half work on two values): 4,096 x 32,768 bf16 49 us (5.5 TB/s),
+// 3,000 x 32,768 float32 66 (5.9 TB/s), with eight alternatives 67 and 4,096 x 32,768 bf16 with a mask 70 (5.7 TB/s); the gradient
 // of 4,096 x 16,384 bf16 48 us (5.6 TB/s), float32 85 (6.3 TB/s), of 4,096 x 32,771 bf16 with a mask 120 (5.6 TB/s). Other
 // arrangements of the forward pass, for 4,096 x 32,768 bf16 with eight alternatives: a row in a block's registers, its largest
 // logit first, 128 us (barriers); in its shared memory 126; a warp a row, alternatives kept as they come, 170 (insertions).
@@ -862,12 +862,14 @@ int scores_of(const Scores& p, cudaStream_t s) {
   if (p.v <= 4 * kEach) return few_scores<T, 4>(p, s);
   if (p.v <= 8 * kEach) return few_scores<T, 8>(p, s);
   if (p.v <= 32 * kEach) return few_scores<T, 32>(p, s);
-  // As few warps a row as fill the GPU, or fewer where a row is short: what a row's end costs, its warps' joining above all,
-  // is paid by more rows at a time (567 rows of 4,341 float32 by 4 warps 7.9 us, by 16 18.0; 300 of 10,000 8.4 and 15.6; 1,000 of
-  // 3,000 bf16 by one 7.9, by 4 9.8; but 1,300 of 100,000 bf16 by 4 53, by one 91). Of few long rows a cluster of blocks that
-  // have a turn each (one row of 50,021 bf16 5.0 us, one block 6.7; 20 of 30,000 float32 8.2, with a vector a thread 11.0).
+  // Warps a row. One for short rows that are many: what a row's end costs, its warps' joining above all, is paid by more rows at a
+  // time (5,000 of 5,000 bf16 with eight alternatives 24 us, by four warps 37; 9,000 of 15,000 54 and 58; 1,000 of 3,000 7.9 and
+  // 9.8). Four for long ones, whose warps then end at different times (4,096 of 32,768 bf16 49 us, by one warp 56; 2,400 of 60,000
+  // 53 and 68; 1,300 of 100,000 53 and 91), and of fewer rows (567 of 4,341 float32 7.9, by 16 warps 18.0; 300 of 10,000 8.4
+  // and 15.6). Sixteen, and a cluster of blocks that have a turn each, of few long rows (one row of 50,021 bf16 5.0 us, one block
+  // 6.7; 20 of 30,000 float32 8.2, with a vector a thread 11.0).
   const int64_t vectors = p.v / kValues;
-  if (p.m >= 16 * 148 || vectors <= 64 || (vectors <= 512 && p.m >= 4 * 148)) return scores<T, 1>(p, 1, s);
+  if (vectors <= 64 || (vectors <= 512 && p.m >= 4 * 148) || (vectors <= 2048 && p.m >= 16 * 148)) return scores<T, 1>(p, 1, s);
   if (p.m >= 2 * 148 || vectors <= 256) return scores<T, 4>(p, 1, s);
   int blocks = 1;
   while (blocks < 8 && p.m * 16 * blocks < 8 * 148 && vectors > 2048 * blocks) blocks *= 2;
