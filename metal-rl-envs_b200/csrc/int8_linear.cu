@@ -364,6 +364,11 @@ Cut cut_of(int64_t m, int64_t k, int64_t f) {
   // Up to four rows of short contractions (three rows of 1,024 x 4,096 3.9 us, by tiles 5.4, eight 7.1 and 5.7; two of 8,192 x
   // 8,192 26 and 17).
   if (m == 1 || (m <= 4 && k <= 2048 && m * k * f <= 1 << 24)) return {0, 1};
+  // Else the form that an estimate finds shortest, in cycles: a pair's rounds of tiles, each its steps and 1,200 for its begin and
+  // end, a step 520 for 256 tokens, whose products it waits for, and 400 for fewer, whose operands it waits for; joined parts
+  // cost a launch, some 5 us, and their writing and reading. Over 22 shapes it takes the quickest of 28 forms or one within 10%
+  // (300 x 1,000 x 2,720: 64 tokens 7.5 us, 128 8.6, 256 9.3; 1,024 x 1,024 x 4,096: 256 tokens 9.0, 128 10.5, 64 12.8; 100 x
+  // 8,192 x 300: 64 tokens in 8 parts 8.7 us, whole 17; 64 x 8,192 x 8,192: whole 17.9, in two parts 19.9).
   const int64_t steps = tiles_of(k, kStepBytes);
   Cut best{};
   double least = 0;
@@ -375,7 +380,7 @@ Cut cut_of(int64_t m, int64_t k, int64_t f) {
       const int64_t rounds = tiles_of(tiles * splits, kPairs);
       const double step = tokens == 256 ? 520 : 400;
       double cycles = double(rounds) * (double(split_steps) * step + 1200);
-      if (splits > 1) cycles += 6000 + double(m) * f * splits * 8 / 2500;
+      if (splits > 1) cycles += 10000 + double(m) * f * splits * 8 / 2500;
       if (best.tokens == 0 || cycles < least) best = {tokens, splits}, least = cycles;
     }
   }
