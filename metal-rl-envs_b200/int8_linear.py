@@ -62,6 +62,8 @@ def _on_boundaries(codes, rows):
 
 def forward(codes, scale, weight, dtype=torch.bfloat16):
     """(codes * scale) times the weight's transpose, (..., F) of dtype, from codes (..., K) and scale (...)."""
+    if not isinstance(weight, Weight):
+        raise ValueError(f"weight must be a Weight, as quantise_weight makes them; got {type(weight).__name__}")
     w, ws = weight.codes, weight.scale
     for name, x, kind in (("codes", codes, torch.int8), ("scale", scale, torch.float32), ("weight.codes", w, torch.int8),
                           ("weight.scale", ws, torch.float32)):

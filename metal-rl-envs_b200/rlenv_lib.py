@@ -474,7 +474,12 @@ def scratch(nbytes, like):
     `like`'s device, which the call's kernels run on."""
     if nbytes < 0:
         check(-1)
-    return like.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
+    return torch.empty_strided((nbytes,), (1,), dtype=torch.uint8, device=_cuda(like.get_device())) if nbytes else None
+
+
+@lru_cache(maxsize=None)
+def _cuda(index):
+    return torch.device("cuda", index)
 
 
 def as_rows(x):
@@ -498,11 +503,6 @@ def as_rows(x):
         else:
             return x, step or 0
     return x.contiguous(), x.shape[-1]
-
-
-@lru_cache(maxsize=None)
-def _cuda(index):
-    return torch.device("cuda", index)
 
 
 def empty_rows(x, k, dtype, pitch=None):

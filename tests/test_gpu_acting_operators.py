@@ -337,7 +337,7 @@ def test_int8_refusals(cuda):
     fine = int8_linear.Weight(w, one)
     for args in ((a.float(), one[:4], fine), (a, one[:3], fine), (a[:, :19], one[:4], fine), (a, one[:4].double(), fine),
                  (a, one[:4], int8_linear.Weight(w, one[:5])), (a, one[:4], int8_linear.Weight(w.float(), one)),
-                 (a, one[:4], fine, torch.float16), (a, one[:4].cpu(), fine), (a[:, :0], one[:4], int8_linear.Weight(w[:, :0], one))):
+                 (a, one[:4], fine, torch.float16), (a, one[:4].cpu(), fine), (a, one[:4], None), (a, one[:4], (w, one)), (a[:, :0], one[:4], int8_linear.Weight(w[:, :0], one))):
         with pytest.raises(ValueError):
             int8_linear.forward(*args)
     with pytest.raises(ValueError):
@@ -635,17 +635,19 @@ def test_operators_in_a_captured_graph_and_on_other_streams(cuda):
     import rms_norm
 
     def inputs(seed):
-        return [normal(cuda, 300, 96, seed=seed), normal(cuda, 300, 96, seed=seed + 1), normal(cuda, 300, 700, seed=seed + 2)]
+        return [normal(cuda, 300, 96, seed=seed), normal(cuda, 300, 96, seed=seed + 1), normal(cuda, 300, 700, seed=seed + 2),
+                normal(cuda, 3, 90_001, seed=seed + 3), normal(cuda, 200, 6000, seed=seed + 4)]
 
     w, weight = 1 + 0.1 * normal(cuda, 96, seed=50), int8_linear.quantise_weight(normal(cuda, 96, 300, seed=51))
-    actions = torch.arange(300, device=cuda)
+    actions, long_weight = torch.arange(300, device=cuda), int8_linear.quantise_weight(normal(cuda, 6000, 40, seed=52))
 
-    def everything(x, y, l):
+    def everything(x, y, l, few, wide):
         out, total = rms_norm.forward(x, w, y)
         c, s, _ = rms_norm.forward8(x, w, y)
         got = log_probs.forward(l, actions, None, 4)
         return [out, total, c, s, *rms_norm.backward(x, total, w, 1e-6, y), int8_linear.forward(c, s, weight),
-                int8_linear.forward(c[:3], s[:3], weight), *got,
+                int8_linear.forward(c[:3], s[:3], weight), *got, *log_probs.forward(few, actions[:3], None, 4),
+                int8_linear.product(wide, long_weight), *rms_norm.backward(wide, wide, wide[0]),
                 log_probs.backward(got.log_prob, got.entropy, l, actions, got.normalizer, got.entropy)]
 
     first, second = inputs(0), inputs(10)
