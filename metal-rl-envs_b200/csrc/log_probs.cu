@@ -336,8 +336,8 @@ __device__ __noinline__ uint4 edge_vector(const T* row, const uint8_t* allowed, 
 }
 
 // A warp's search for its best logits. Its part of a row is 32 lanes' vectors of up to kEpochs epochs, each of which leaves
-// its largest logit behind. The top-th largest of these has `top` logits at least that are not below it, and the groups
-// which reach it, `top` of them where none are equal, are looked through again.
+// its largest logit behind. The top-th largest of a warp's (of several warps: of their lanes') has `top` logits at least that
+// are not below it, and the groups which reach it, `top` of them where none are equal, are looked through again.
 constexpr int kEpochs = 4;
 struct Best {
   static constexpr int kMany = 64, kRoom = kMany + 256;  // a step adds one vector a lane, 256 logits at most
@@ -385,23 +385,13 @@ struct Best {
     __syncwarp();
     return least;
   }
-  // Lists the groups that reach the top-th largest of all, and that as `least`; returns their number.
-  RLENV_D int choose(int top, int epochs, uint32_t& least) {
+  // Lists the groups whose largest logit is not below `least`; returns their number.
+  RLENV_D int list(int epochs, uint32_t least) {
     const int lane = threadIdx.x % 32;
-    uint32_t of[kEpochs], rest[kEpochs];  // rest: in falling order
+    uint32_t of[kEpochs];
 #pragma unroll
-    for (int e = 0; e < kEpochs; ++e) of[e] = rest[e] = e < epochs ? largest[e][lane] : 0;
-    const auto order = [&](int i, int j) {
-      const uint32_t high = max(rest[i], rest[j]);
-      rest[j] = min(rest[i], rest[j]), rest[i] = high;
-    };
-    static_assert(kEpochs == 4, "four values are put in order");
-    order(0, 1), order(2, 3), order(0, 2), order(1, 3), order(1, 2);
-    for (int r = 0; r < top; ++r) {  // takes the largest out, one after the other
-      least = __reduce_max_sync(0xffffffffu, rest[0]);
-      if (lane == __ffs(__ballot_sync(0xffffffffu, rest[0] == least)) - 1)
-        rest[0] = rest[1], rest[1] = rest[2], rest[2] = rest[3], rest[3] = 0;
-    }
+    for (int e = 0; e < kEpochs; ++e) of[e] = e < epochs ? largest[e][lane] : 0;
+    __syncwarp();  // the list takes their place
     int n = 0;
 #pragma unroll
     for (int e = 0; e < kEpochs; ++e) {
@@ -414,6 +404,21 @@ struct Best {
     return n;
   }
 };
+// The n-th largest of a warp's whole numbers, four a lane: the largest is taken out, one after the other.
+RLENV_D uint32_t nth_largest(uint32_t (&v)[4], int n) {
+  const int lane = threadIdx.x % 32;
+  const auto order = [&](int i, int j) {
+    const uint32_t high = max(v[i], v[j]);
+    v[j] = min(v[i], v[j]), v[i] = high;
+  };
+  order(0, 1), order(2, 3), order(0, 2), order(1, 3), order(1, 2);
+  uint32_t largest = 0;
+  for (int r = 0; r < n; ++r) {
+    largest = __reduce_max_sync(0xffffffffu, v[0]);
+    if (lane == __ffs(__ballot_sync(0xffffffffu, v[0] == largest)) - 1) v[0] = v[1], v[1] = v[2], v[2] = v[3], v[3] = 0;
+  }
+  return largest;
+}
 
 // kWarps warps read a row in turns of kSteps vectors a lane, and a cluster's blocks a part of it each: no lane waits for
 // another before the row's end. Each lane's next turns are on their way into its own places of shared memory meanwhile. A
@@ -440,6 +445,7 @@ scores_kernel(const __grid_constant__ Scores p) {
   __shared__ Sums of_warps[kBlockWarps];
   __shared__ Sums of_block;
   __shared__ uint64_t top_of_block[kMostTop];
+  __shared__ uint32_t largest_of_lanes[kWarps == 1 ? 1 : 32 * kWarps];
   cg::cluster_group cluster = cg::this_cluster();
   const int blocks = kWarps == 16 ? int(cluster.num_blocks()) : 1, rank = blocks > 1 ? int(cluster.block_rank()) : 0;
   const int lane = threadIdx.x % 32, warp = threadIdx.x / 32 % kWarps;
@@ -556,8 +562,22 @@ scores_kernel(const __grid_constant__ Scores p) {
   if (p.top > 0) {
     if (lane == 0) best.count = 0, best.keys = reinterpret_cast<uint64_t*>(ring);
     __syncwarp();
-    uint32_t least = 0;
-    const int each_bits = 2 + epoch_bits, total = best.choose(p.top, at_epoch, least) << each_bits;
+    uint32_t of[kEpochs];
+    static_assert(kEpochs == 4, "as nth_largest takes them");
+#pragma unroll
+    for (int e = 0; e < kEpochs; ++e) of[e] = e < at_epoch ? best.largest[e][lane] : 0;
+    if constexpr (kWarps > 1) {
+      largest_of_lanes[threadIdx.x] = max(max(of[0], of[1]), max(of[2], of[3]));
+      __syncthreads();
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        of[e] = 0;
+#pragma unroll
+        for (int i = 0; i < kWarps / 4; ++i) of[e] = max(of[e], largest_of_lanes[32 * (e * (kWarps / 4) + i) + lane]);
+      }
+    }
+    const uint32_t least = nth_largest(of, p.top);
+    const int each_bits = 2 + epoch_bits, total = best.list(at_epoch, least) << each_bits;
     static_assert(kSteps == 4, "a group's vectors are 4 a turn");
     uint64_t least_key = uint64_t(least) << 32;
     const auto look_at = [&](int i, const uint32_t (&w)[4]) {  // vector i, for the whole warp
