@@ -65,13 +65,19 @@ def forward(codes, scale, weight, dtype=torch.bfloat16):
     if not isinstance(weight, Weight):
         raise ValueError(f"weight must be a Weight, as quantise_weight makes them; got {type(weight).__name__}")
     w, ws = weight.codes, weight.scale
-    for name, x, kind in (("codes", codes, torch.int8), ("scale", scale, torch.float32), ("weight.codes", w, torch.int8),
-                          ("weight.scale", ws, torch.float32)):
-        if not isinstance(x, torch.Tensor) or x.dtype is not kind or not x.is_cuda:
-            raise ValueError(f"{name} must be a CUDA tensor of {kind}: there is no CPU path")
-    index, lead, of_w = codes.get_device(), scale.shape, w.shape
-    if scale.get_device() != index or w.get_device() != index or ws.get_device() != index:
+    try:  # what fits passes on a few comparisons
+        index = codes.get_device()
+        fit = index >= 0 and scale.get_device() == index and w.get_device() == index and ws.get_device() == index \
+            and codes.dtype is torch.int8 and w.dtype is torch.int8 and scale.dtype is ws.dtype is torch.float32
+    except (AttributeError, TypeError):
+        fit = False
+    if not fit:
+        for name, x, kind in (("codes", codes, torch.int8), ("scale", scale, torch.float32), ("weight.codes", w, torch.int8),
+                              ("weight.scale", ws, torch.float32)):
+            if not isinstance(x, torch.Tensor) or x.dtype is not kind or not x.is_cuda:
+                raise ValueError(f"{name} must be a CUDA tensor of {kind}: there is no CPU path")
         _rl.one_device(index, scale=scale, **{"weight.codes": w, "weight.scale": ws})
+    lead, of_w = scale.shape, w.shape
     if len(of_w) != 2 or codes.shape != (*lead, of_w[1]) or ws.shape != of_w[:1]:
         raise ValueError(f"codes (..., K), scale (...), weight.codes (F, K) and weight.scale (F,) do not fit: got "
                          f"{tuple(codes.shape)}, {tuple(lead)}, {tuple(of_w)} and {tuple(ws.shape)}")

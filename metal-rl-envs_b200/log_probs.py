@@ -62,17 +62,21 @@ def forward(logits, actions, allowed=None, alternatives=0):
     if not 0 <= alternatives <= min(v, MOST_ALTERNATIVES):
         raise ValueError(f"alternatives must be from 0 to {min(v, MOST_ALTERNATIVES)}; got {alternatives}")
     logits, stride = _rl.as_rows(logits)
-    allowed, allowed_stride = (None, 0) if allowed is None else _rl.as_rows(allowed)
+    allowed_at = allowed_stride = 0
+    if allowed is not None:
+        allowed, allowed_stride = _rl.as_rows(allowed)
+        allowed_at = allowed.data_ptr()
     actions = actions.contiguous()
     log_prob = _rl.empty_lead(logits, torch.float32)
     entropy, normalizer = torch.empty_like(log_prob), torch.empty_like(log_prob)
-    top, best = None, None
-    if alternatives:
-        top = _rl.empty_rows(logits, alternatives, torch.float32)
-        best = _rl.empty_rows(logits, alternatives, torch.int64)
+    if not alternatives:
+        _rl.launch(index, _rl.lib().log_probs_forward, code, m, v, logits.data_ptr(), stride, actions.data_ptr(), action_code,
+                   allowed_at, allowed_stride, log_prob.data_ptr(), entropy.data_ptr(), normalizer.data_ptr(), 0, 0, 0)
+        return Scores(log_prob, entropy, normalizer)
+    top, best = _rl.empty_rows(logits, alternatives, torch.float32), _rl.empty_rows(logits, alternatives, torch.int64)
     _rl.launch(index, _rl.lib().log_probs_forward, code, m, v, logits.data_ptr(), stride, actions.data_ptr(), action_code,
-               _rl.ptr(allowed), allowed_stride, log_prob.data_ptr(), entropy.data_ptr(), normalizer.data_ptr(), alternatives,
-               _rl.ptr(best), _rl.ptr(top))
+               allowed_at, allowed_stride, log_prob.data_ptr(), entropy.data_ptr(), normalizer.data_ptr(), alternatives,
+               best.data_ptr(), top.data_ptr())
     return Scores(log_prob, entropy, normalizer, top, best)
 
 

@@ -677,6 +677,38 @@ def test_operators_in_a_captured_graph_and_on_other_streams(cuda):
             assert all(torch.equal(a, b) for a, b in zip(outs[which], want[order[which]]))
 
 
+def test_offsets_past_32_bits(cuda):
+    """Tensors of more than 2^31 and 2^32 elements: rows around those places and the last ones are what the same rows
+    alone give."""
+    import int8_linear
+    import log_probs
+    import rms_norm
+
+    m, k = 4_300_000, 1000
+    x, w = torch.empty((m, k), dtype=torch.bfloat16, device=cuda).normal_(), torch.ones(k, dtype=torch.bfloat16, device=cuda)
+    weights = [int8_linear.quantise_weight(normal(cuda, k, f, seed=f)) for f in (1000, 1001)]
+    out, _ = rms_norm.forward(x, w)
+    codes, scale, _ = rms_norm.forward8(x, w)
+    grad, _ = rms_norm.backward(x, x, w)
+    products = [int8_linear.forward(codes, scale, weight) for weight in weights]
+    places = [slice(at, at + 40) for at in (2 ** 31 // k - 20, 2 ** 32 // k - 20, m - 40)]
+    for at in places:
+        alone = x[at].clone()
+        assert torch.equal(out[at], rms_norm.forward(alone, w)[0]) and torch.equal(grad[at], rms_norm.backward(alone, alone, w)[0])
+        assert all(torch.equal(a[at], b) for a, b in zip((codes, scale), rms_norm.forward8(alone, w)))
+        for product, weight in zip(products, weights):
+            assert torch.equal(product[at], int8_linear.forward(codes[at], scale[at], weight))
+    del out, codes, grad, products
+    l, actions = x.view(-1)[: 40_000 * 100_000].view(40_000, 100_000), torch.arange(40_000, device=cuda) % 100_000
+    got = log_probs.forward(l, actions, None, 3)
+    grad = log_probs.backward(got.log_prob, got.entropy, l, actions, got.normalizer, got.entropy)
+    for at in (slice(21_460, 21_490), slice(39_970, 40_000)):
+        alone = l[at].clone()
+        check_scores(log_probs.Scores(*(y[at] for y in got)), alone, actions[at], None, 3)
+        assert torch.equal(grad[at], log_probs.backward(got.log_prob[at], got.entropy[at], alone, actions[at], got.normalizer[at],
+                                                        got.entropy[at]))
+
+
 def test_calls_at_the_same_time(cuda):
     """Two streams run the same operators on other inputs at once, over and over: nothing is shared between them."""
     import int8_linear
