@@ -93,7 +93,7 @@ struct Int8Tile {
   static_assert(!kWide || kTokens == 256, "wide tiles are 256 x 256");
   static constexpr int kHalf = kTokens / 2;  // rows of the second operand that each block copies
   static constexpr int kABytes = kChannelsEach * kStepBytes, kRingBytes = kABytes + kHalf * kStepBytes;
-  static constexpr int kStages = kWide ? 4 : 6 * 32768 / kRingBytes < 10 ? 6 * 32768 / kRingBytes : 10;
+  static constexpr int kStages = kWide ? 5 : 6 * 32768 / kRingBytes < 10 ? 6 * 32768 / kRingBytes : 10;
   static constexpr int kEpilogue = kTokens >= 128 ? 16 : kTokens >= 64 ? 8 : 4;  // warps
   static constexpr int kMine = kTokens / (kEpilogue / 4);         // columns of a thread
   static constexpr int kThreads = 128 + 32 * kEpilogue;
@@ -138,7 +138,7 @@ tile_kernel(const __grid_constant__ Int8Tiles p, int items) {
   __shared__ uint32_t tmem_slot;
   __shared__ int dead_flag;
   __shared__ bw::Ending endings[2];  // of the pair's first block, and of its second
-  __shared__ __align__(16) float scales[C::kEpilogue][kWide ? 64 : 32];
+  __shared__ __align__(16) float scales[kWide ? 4 : C::kEpilogue][kWide ? 64 : 32];  // of a part's channels; of a run's tokens
   volatile int* const dead = &dead_flag;
   const uint32_t ring = (bw::shared_at(raw) + 1023) & ~1023u;
   const uint32_t full = bw::shared_at(bars), empty = full + 8 * C::kStages;
@@ -218,7 +218,7 @@ tile_kernel(const __grid_constant__ Int8Tiles p, int items) {
     }
   } else if (warp >= 4) {
     const int quarter = warp & 3, part = (warp - 4) >> 2;
-    float* const own_scales = scales[warp - 4];
+    float* const own_scales = scales[kWide ? part : warp - 4];
     unsigned char* const own_stage = raw + (ring - bw::shared_at(raw)) + C::kStages * C::kRingBytes + (warp - 4) * C::kStageBytes;
     int buffer = 0;
     uint32_t buffer_phase = 0;
@@ -231,13 +231,15 @@ tile_kernel(const __grid_constant__ Int8Tiles p, int items) {
         const int64_t token = int64_t(2 * w.token + rank) * kChannelsEach + 32 * quarter;
         const int64_t channel0 = int64_t(w.channel) * kTokens + part * C::kMine;
         float a_scale = token + lane < p.m ? __ldg(p.a_scale + token + lane) : 0.0f;
-#pragma unroll
-        for (int i = 0; i < C::kMine; i += 32)
-          own_scales[i + lane] = channel0 + i + lane < p.f ? __ldg(p.w_scale + channel0 + i + lane) : 0.0f;
+        // The part's four warps have its channels' scales in common.
+        const auto part_sync = [&] { asm volatile("bar.sync %0, 128;" ::"r"(1 + part) : "memory"); };
+        part_sync();  // the last tile's are read
+        if (quarter < C::kMine / 32)
+          own_scales[32 * quarter + lane] = channel0 + 32 * quarter + lane < p.f ? __ldg(p.w_scale + channel0 + 32 * quarter + lane) : 0.0f;
         ok = ok && bw::barrier_wait_warp(summed + 8 * buffer, buffer_phase, dead);
         if (!ok) a_scale = __uint_as_float(0x7fffffffu);
         bw::fence_after();
-        __syncwarp();
+        part_sync();
         const uint64_t of_row = pair_of(a_scale, a_scale);
 #pragma unroll
         for (int run = 0; run < C::kMine / 32; ++run) {
