@@ -77,7 +77,7 @@ RLENV_D uint64_t powers_of(uint64_t l, uint64_t minus_base) {
 // Logits are ordered by value, ties by the lower place: as one whole number, larger first. 0 stands below all, NaN
 // above.
 RLENV_D uint32_t order_of(float x) {
-  if (x != x) return 0xffffffffu;
+  if (x != x) return 0xfffffffeu;  // so that no key is all ones
   const uint32_t b = x == 0.0f ? 0u : __float_as_uint(x);  // both zeros are one
   return b & 0x80000000u ? ~b : b | 0x80000000u;
 }
@@ -101,17 +101,28 @@ RLENV_D Sums moved(const Sums& a, float m) {  // against m >= a.m
   const float d = larger(a.m - m, kFar), e = __expf(d);
   return {m, e * a.s, e * fmaf(a.s, d, a.w)};
 }
+// The largest of kLanes neighbouring lanes', or NaN, known to all of them.
+template <int kLanes>
+RLENV_D float largest_of_lanes_of(float x) {
+  if constexpr (kLanes == 32) {
+    float r;
+    asm volatile("redux.sync.max.NaN.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(x));
+    return r;
+  } else {
+#pragma unroll
+    for (int d = kLanes / 2; d > 0; d /= 2) x = larger(x, __shfl_xor_sync(0xffffffffu, x, d));
+    return x;
+  }
+}
 // Of kLanes neighbouring lanes, known to all of them.
 template <int kLanes>
 RLENV_D Sums of_team(const Sums& a) {
-  float m = a.m;
+  const Sums own = moved(a, largest_of_lanes_of<kLanes>(a.m));
+  uint64_t both = pair_of(own.s, own.w);
 #pragma unroll
-  for (int d = kLanes / 2; d > 0; d /= 2) m = larger(m, __shfl_xor_sync(0xffffffffu, m, d));
-  Sums r = moved(a, m);
-#pragma unroll
-  for (int d = kLanes / 2; d > 0; d /= 2)
-    r.s += __shfl_xor_sync(0xffffffffu, r.s, d), r.w += __shfl_xor_sync(0xffffffffu, r.w, d);
-  return r;
+  for (int d = kLanes / 2; d > 0; d /= 2) both = add_pairs(both, __shfl_xor_sync(0xffffffffu, both, d));
+  const float2 of = values_of(both);
+  return {own.m, of.x, of.y};
 }
 RLENV_D float normalizer_of(const Sums& a) { return base_of(a.m) + logf(a.s); }
 
@@ -137,35 +148,189 @@ RLENV_D void write_top(const Scores& p, int64_t row, int rank, uint64_t key, flo
   p.top_log_probs[row * p.top + rank] = log_prob_of(value_of(uint32_t(key >> 32)), normalizer);
 }
 
-// ---- few actions: a row is the work of kLanes neighbouring lanes -----------------------------------------
+// ---- few actions: a row is the work of kLanes neighbouring lanes, kEach logits of it in each --------------
+//
+// Rows of up to 1,024 lie in registers whole. What a row costs is instructions: half of them its logits, half its end (joins,
+// logarithms, the action), which many logits a lane and few lanes a row make cheaper (169,089 of 200 float32 by 16 lanes 32 us,
+// by 32 43; 131,072 of 1,000 bf16 93 us, of 500 51; as long rows are taken, below, 102 and 112).
 
-constexpr int kEach = 8;  // logits of a lane
-template <typename T, int kLanes>
-__global__ void __launch_bounds__(256) few_scores_kernel(const __grid_constant__ Scores p) {
-  const int sub = threadIdx.x % kLanes;
-  const int64_t at = (int64_t(blockIdx.x) * 256 + threadIdx.x) / kLanes, row = at < p.m ? at : p.m - 1;
-  const T* const logits = static_cast<const T*>(p.logits) + row * p.stride;
-  const uint8_t* const allowed = p.allowed ? p.allowed + row * p.allowed_stride : nullptr;
-  const int v = int(p.v);
-  float x[kEach];
+// A key of a logit among up to 256, larger first, each another; 0 is none. bfloat16 orders leave 16 bits for the place.
+RLENV_D uint64_t few_key(const float*, float x, int place) { return key_of(x, place); }
+RLENV_D uint32_t few_key(const __nv_bfloat16*, float x, int place) { return (order_of(x) & 0xffff0000u) | (0xffffu - place); }
+RLENV_D uint64_t whole_key(uint64_t key) { return key; }
+RLENV_D uint64_t whole_key(uint32_t key) {
+  const uint32_t order = key & 0x80000000u ? key & 0xffff0000u : key | 0xffffu;
+  return uint64_t(order) << 32 | (key | 0xffff0000u);
+}
+template <int kLanes, typename K>
+RLENV_D K largest_of_team(K key) {
+  if constexpr (kLanes == 32) {
+    const uint32_t high = __reduce_max_sync(0xffffffffu, uint32_t(key >> 32));
+    return K(high) << 32 | __reduce_max_sync(0xffffffffu, uint32_t(key >> 32) == high ? uint32_t(key) : 0u);
+  } else {
+#pragma unroll
+    for (int d = kLanes / 2; d > 0; d /= 2) {
+      const K other = __shfl_xor_sync(0xffffffffu, key, d);
+      key = other > key ? other : key;
+    }
+    return key;
+  }
+}
+// The row's best `top` logits, one after the other: each lane's own are sorted, and the lane whose first is the row's best gives
+// it up. The lanes write together, each kLanes-th of them. A search through all lanes' logits for each takes twice as long
+// (192,341 of 41 float32 with twenty alternatives 90 us, by searches 187; 169,089 of 100 bf16 with eight 59 and 314).
+template <typename T, int kLanes, int kEach>
+RLENV_D void few_best(const Scores& p, int64_t row, bool real, int sub, const float (&x)[kEach], float normalizer) {
+  using K = decltype(few_key(static_cast<const T*>(nullptr), 0.0f, 0));
+  K keys[kEach];
 #pragma unroll
   for (int i = 0; i < kEach; ++i) {
     const int j = sub + kLanes * i;
-    x[i] = j < v ? value_at(logits + j) : -infinity();
+    keys[i] = j < p.v ? few_key(static_cast<const T*>(nullptr), x[i], j) : K(0);
   }
-  if (allowed) {
+  const auto order = [&](int i, int j) {
+    const K high = keys[i] > keys[j] ? keys[i] : keys[j], low = keys[i] > keys[j] ? keys[j] : keys[i];
+    keys[i] = high, keys[j] = low;
+  };
+  if (p.top == 1) {
 #pragma unroll
-    for (int i = 0; i < kEach; ++i) {
-      const int j = sub + kLanes * i;
-      if (j < v && !allowed[j]) x[i] = -infinity();
+    for (int d = kEach / 2; d > 0; d /= 2)
+#pragma unroll
+      for (int i = 0; i < d; ++i) order(i, i + d);
+  } else {  // odd-even merges
+#pragma unroll
+    for (int n = 1; n < kEach; n *= 2)
+#pragma unroll
+      for (int d = n; d > 0; d /= 2)
+#pragma unroll
+        for (int i = 0; i + d < kEach; ++i)
+          if (i >= d % n && (i - d % n) / d % 2 == 0 && i / (2 * n) == (i + d) / (2 * n)) order(i, i + d);
+  }
+  K mine = 0;
+  for (int r = 0; r < p.top; ++r) {
+    const K best = largest_of_team<kLanes>(keys[0]);
+    const bool own = keys[0] == best;
+#pragma unroll
+    for (int i = 0; i < kEach - 1; ++i) keys[i] = own ? keys[i + 1] : keys[i];
+    keys[kEach - 1] = own ? K(0) : keys[kEach - 1];
+    if (r % kLanes == sub) mine = best;
+    if ((r % kLanes == kLanes - 1 || r == p.top - 1) && real && sub <= r % kLanes)
+      write_top(p, row, r - r % kLanes + sub, whole_key(mine), normalizer);
+  }
+}
+
+// The same where a warp has a row: as many lanes as alternatives are asked for have a logit that reaches the top-th of the
+// lanes' largest, and the logits that do, few more than `top`, are ranked by counting (169,089 of 200 float32 with eight
+// alternatives 98 us, by sorting 206; 131,072 of 500 bf16 with twenty 149).
+constexpr int kFound = 64;
+struct Found {
+  uint64_t keys[kFound];
+  int count;
+};
+template <typename T, int kEach>
+RLENV_D void few_best_of_warp(const Scores& p, int64_t row, const float (&x)[kEach], float normalizer, Found& found) {
+  const int lane = threadIdx.x % 32, left = int(p.v) - lane;
+  float most = x[0];
+#pragma unroll
+  for (int i = 1; i < kEach; ++i) most = larger(most, x[i]);
+  if (lane == 0) found.count = 0;
+  __syncwarp();
+  uint32_t order = left > 0 ? order_of(most) : 0, least = 0;
+  for (int r = 0; r < p.top; ++r) {
+    least = __reduce_max_sync(0xffffffffu, order);
+    if (lane == __ffs(__ballot_sync(0xffffffffu, order == least)) - 1) order = 0;
+  }
+  const float bar = value_of(least);
+  uint32_t reach = 0;
+#pragma unroll
+  for (int i = 0; i < kEach; ++i)
+    if (32 * i < left && !(x[i] < bar)) reach |= 1u << i;
+  if (reach) {
+    const T* const logits = static_cast<const T*>(p.logits) + row * p.stride;
+    const uint8_t* const allowed = p.allowed ? p.allowed + row * p.allowed_stride : nullptr;
+    int at = atomicAdd(&found.count, __popc(reach));
+    for (; reach && at < kFound; reach &= reach - 1, ++at) {
+      const int j = lane + 32 * (__ffs(reach) - 1);
+      found.keys[at] = key_of(allowed && !allowed[j] ? -infinity() : value_at(logits + j), j);
     }
   }
-  const Chosen chosen = Chosen::of(p, row, logits, allowed);
+  __syncwarp();
+  const int count = found.count;
+  if (count <= kFound) {
+    for (int i = lane; i < count; i += 32) {
+      const uint64_t key = found.keys[i];
+      int above = 0;
+#pragma unroll 4
+      for (int k = 0; k < count; ++k) above += found.keys[k] > key;
+      if (above < p.top) write_top(p, row, above, key, normalizer);
+    }
+  } else {  // equal ones: the largest is taken out, one after the other
+    uint64_t last = ~uint64_t(0);
+    for (int r = 0; r < p.top; ++r) {
+      uint64_t own = 0;
+#pragma unroll
+      for (int i = 0; i < kEach; ++i) {
+        const uint64_t key = 32 * i < left ? key_of(x[i], lane + 32 * i) : 0;
+        if (key < last && key > own) own = key;
+      }
+      last = largest_of_team<32>(own);
+      if (lane == 0) write_top(p, row, r, last, normalizer);
+    }
+  }
+}
+
+// Loads where there is a place, as single instructions: branches around loads would have each wait for the one before.
+RLENV_D void load_if(int there, const float* from, float& to) {
+  asm volatile("{\n\t.reg .pred in;\n\tsetp.gt.s32 in, %2, 0;\n\t@in ld.global.nc.f32 %0, [%1];\n\t}" : "+f"(to) : "l"(from), "r"(there));
+}
+RLENV_D void load_if(int there, const __nv_bfloat16* from, uint16_t& to) {
+  asm volatile("{\n\t.reg .pred in;\n\tsetp.gt.s32 in, %2, 0;\n\t@in ld.global.nc.u16 %0, [%1];\n\t}" : "+h"(to) : "l"(from), "r"(there));
+}
+RLENV_D void load_if(int there, const uint8_t* from, uint16_t& to) {
+  asm volatile("{\n\t.reg .pred in;\n\tsetp.gt.s32 in, %2, 0;\n\t@in ld.global.nc.u8 %0, [%1];\n\t}" : "+h"(to) : "l"(from), "r"(there));
+}
+RLENV_D float value_in(float x) { return x; }
+RLENV_D float value_in(uint16_t bits) { return __uint_as_float(uint32_t(bits) << 16); }
+// A lane's logits of a row: places sub, sub + kLanes and so on.
+template <int kLanes, int kEach, typename T, typename P>
+RLENV_D void few_logits(const P& p, int64_t row, int sub, float (&x)[kEach]) {
+  using Raw = std::conditional_t<sizeof(T) == 4, float, uint16_t>;
+  const T* const logits = static_cast<const T*>(p.logits) + row * p.stride + sub;
+  const uint8_t* const allowed = p.allowed + row * p.allowed_stride + sub;
+  const int left = int(p.v) - sub;
+  Raw raw[kEach];
+  uint16_t open[kEach];
+#pragma unroll
+  for (int i = 0; i < kEach; ++i) {
+    if constexpr (sizeof(T) == 4)
+      raw[i] = -infinity();
+    else
+      raw[i] = 0xff80;
+    load_if(left - kLanes * i, logits + kLanes * i, raw[i]);
+  }
+  if (p.allowed) {
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) open[i] = 1, load_if(left - kLanes * i, allowed + kLanes * i, open[i]);
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) x[i] = open[i] == 0 ? -infinity() : value_in(raw[i]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) x[i] = value_in(raw[i]);
+  }
+}
+
+template <typename T, int kLanes, int kEach>
+__global__ void __launch_bounds__(256) few_scores_kernel(const __grid_constant__ Scores p) {
+  const int sub = threadIdx.x % kLanes;
+  const int64_t at = (int64_t(blockIdx.x) * 256 + threadIdx.x) / kLanes, row = at < p.m ? at : p.m - 1;
+  float x[kEach];
+  few_logits<kLanes, kEach, T>(p, row, sub, x);
+  const Chosen chosen = Chosen::of(p, row, static_cast<const T*>(p.logits) + row * p.stride,
+                                   p.allowed ? p.allowed + row * p.allowed_stride : nullptr);
   Sums sums{x[0], 0.0f, 0.0f};
 #pragma unroll
   for (int i = 1; i < kEach; ++i) sums.m = larger(sums.m, x[i]);
-#pragma unroll
-  for (int d = kLanes / 2; d > 0; d /= 2) sums.m = larger(sums.m, __shfl_xor_sync(0xffffffffu, sums.m, d));
+  sums.m = largest_of_lanes_of<kLanes>(sums.m);
   const float base = base_of(sums.m);
   const uint64_t minus_base = pair_of(-base, -base);
   uint64_t s2 = 0, w2 = 0;
@@ -177,32 +342,18 @@ __global__ void __launch_bounds__(256) few_scores_kernel(const __grid_constant__
     s2 = add_pairs(s2, e), w2 = multiply_add_pairs(e, y, w2);
   }
   const float2 s_own = values_of(s2), w_own = values_of(w2);
-  sums.s = s_own.x + s_own.y, sums.w = (w_own.x + w_own.y) * kLn2;
+  uint64_t both = pair_of(s_own.x + s_own.y, (w_own.x + w_own.y) * kLn2);
 #pragma unroll
-  for (int d = kLanes / 2; d > 0; d /= 2) {
-    sums.s += __shfl_xor_sync(0xffffffffu, sums.s, d);
-    sums.w += __shfl_xor_sync(0xffffffffu, sums.w, d);
-  }
+  for (int d = kLanes / 2; d > 0; d /= 2) both = add_pairs(both, __shfl_xor_sync(0xffffffffu, both, d));
+  const float2 of = values_of(both);
+  sums.s = of.x, sums.w = of.y;
   const float normalizer = normalizer_of(sums);
   if (sub == 0 && at < p.m) write_scores(p, row, sums, normalizer, chosen);
-  if (p.top == 0) return;
-  uint32_t taken = 0;
-  for (int r = 0; r < p.top; ++r) {
-    uint64_t best = 0;
-#pragma unroll
-    for (int i = 0; i < kEach; ++i) {
-      const int j = sub + kLanes * i;
-      const uint64_t key = j < v && !(taken >> i & 1) ? key_of(x[i], j) : 0;
-      best = key > best ? key : best;
-    }
-#pragma unroll
-    for (int d = kLanes / 2; d > 0; d /= 2) {
-      const uint64_t other = __shfl_xor_sync(0xffffffffu, best, d);
-      best = other > best ? other : best;
-    }
-    const int j = int(~uint32_t(best));
-    if (j % kLanes == sub) taken |= 1u << (j / kLanes);
-    if (sub == 0 && at < p.m) write_top(p, row, r, best, normalizer);
+  if constexpr (kLanes == 32) {
+    __shared__ Found found[8];
+    if (p.top > 0 && at < p.m) few_best_of_warp<T, kEach>(p, row, x, normalizer, found[threadIdx.x / 32]);
+  } else if constexpr (kLanes < 16) {
+    if (p.top > 0) few_best<T, kLanes, kEach>(p, row, at < p.m, sub, x, normalizer);
   }
 }
 
@@ -701,12 +852,14 @@ struct ScoresGrad {
 // What a row's gradients have in common. With y = log2 p the gradient of what was not chosen is
 // - p (g + h entropy + h ln 2 y): two values an instruction but for the power.
 struct RowGrad {
-  int64_t action;  // negative: none whose gradient differs
+  int action;  // negative: none whose gradient differs
   float g;
   uint64_t minus_base, a, b;
+  RLENV_D RowGrad() {}
   RLENV_D RowGrad(const ScoresGrad& p, int64_t row) {
-    action = action_of(p.actions, p.action_dtype, row);
-    check_flag(action >= p.v, kCheckActionRange);
+    const int64_t of_row = action_of(p.actions, p.action_dtype, row);
+    check_flag(of_row >= p.v, kCheckActionRange);
+    action = of_row < 0 ? -1 : int(of_row < p.v ? of_row : p.v);
     const float normalizer = __ldg(p.normalizer + row), entropy = __ldg(p.entropy + row);
     const float h = p.grad_entropy ? __ldg(p.grad_entropy + row) : 0.0f;
     g = p.grad_log_prob && action >= 0 ? __ldg(p.grad_log_prob + row) : 0.0f;
@@ -722,10 +875,14 @@ struct RowGrad {
     return values_of(multiply_pairs(pair_of(exp2_fast(of.x), exp2_fast(of.y)), multiply_add_pairs(b, y, a)));
   }
   RLENV_D float of_choice(float l) const { return l == -infinity() ? 0.0f : g; }
-  RLENV_D float2 at(float l0, float l1, int j0, int j1) const {
-    float2 r = without_choice(pair_of(l0, l1));
-    if (j0 == action) r.x += of_choice(l0);
-    if (j1 == action) r.y += of_choice(l1);
+  // Another lane's, among kLanes neighbouring ones.
+  template <int kLanes>
+  RLENV_D RowGrad of_lane(int lane) const {
+    RowGrad r;
+    const float base = __shfl_sync(0xffffffffu, values_of(minus_base).x, lane, kLanes),
+                of_p = __shfl_sync(0xffffffffu, values_of(a).x, lane, kLanes), of_y = __shfl_sync(0xffffffffu, values_of(b).x, lane, kLanes);
+    r.action = __shfl_sync(0xffffffffu, action, lane, kLanes), r.g = __shfl_sync(0xffffffffu, g, lane, kLanes);
+    r.minus_base = pair_of(base, base), r.a = pair_of(of_p, of_p), r.b = pair_of(of_y, of_y);
     return r;
   }
 };
@@ -734,35 +891,29 @@ RLENV_D void store_value(float* to, float x) { *to = x; }
 RLENV_D void store_value(__nv_bfloat16* to, float x) { *to = __float2bfloat16_rn(x); }
 
 // Rows of few actions: kLanes neighbouring lanes a row, as in the forward pass.
-template <typename T, int kLanes>
-__global__ void __launch_bounds__(256) few_scores_grad_kernel(const __grid_constant__ ScoresGrad p) {
-  const int sub = threadIdx.x % kLanes;
-  const int64_t row = (int64_t(blockIdx.x) * 256 + threadIdx.x) / kLanes;
-  if (row >= p.m) return;
-  const T* const logits = static_cast<const T*>(p.logits) + row * p.stride;
-  const uint8_t* const allowed = p.allowed ? p.allowed + row * p.allowed_stride : nullptr;
-  T* const grad = static_cast<T*>(p.grad) + row * p.v;
-  const int v = int(p.v);
-  float x[kEach];
+template <typename T, int kLanes, int kEach>
+__global__ void __launch_bounds__(256) few_scores_grad_kernel(const __grid_constant__ ScoresGrad p, int turns) {
+  constexpr int kAtOnce = 32 / kLanes;
+  const int sub = threadIdx.x % kLanes, team = threadIdx.x % 32 / kLanes, m = int(p.m);
+  const int first = int(blockIdx.x * 8 + threadIdx.x / 32) * (kAtOnce * turns), own = first + sub * kAtOnce + team;
+  RowGrad of_own;
+  if (sub < turns && own < m) of_own = RowGrad(p, own);
+#pragma unroll 1
+  for (int turn = 0; turn < turns && first + turn * kAtOnce < m; ++turn) {
+    const int at = first + turn * kAtOnce + team, row = min(at, m - 1);
+    float x[kEach];
+    few_logits<kLanes, kEach, T>(p, row, sub, x);
+    const RowGrad of = of_own.of_lane<kLanes>(turn);
+    T* const grad = static_cast<T*>(p.grad) + row * p.v + sub;
+    const int left = at < m ? int(p.v) - sub : 0, chosen = of.action - sub;
 #pragma unroll
-  for (int i = 0; i < kEach; ++i) {
-    const int j = sub + kLanes * i;
-    x[i] = j < v ? value_at(logits + j) : -infinity();
-  }
-  if (allowed) {
-#pragma unroll
-    for (int i = 0; i < kEach; ++i) {
-      const int j = sub + kLanes * i;
-      if (j < v && !allowed[j]) x[i] = -infinity();
+    for (int i = 0; i < kEach; i += 2) {
+      float2 g = of.without_choice(pair_of(x[i], x[i + 1]));
+      if (chosen == kLanes * i) g.x += of.of_choice(x[i]);
+      if (chosen == kLanes * (i + 1)) g.y += of.of_choice(x[i + 1]);
+      if (kLanes * i < left) store_value(grad + kLanes * i, g.x);
+      if (kLanes * (i + 1) < left) store_value(grad + kLanes * (i + 1), g.y);
     }
-  }
-  const RowGrad of(p, row);
-#pragma unroll
-  for (int i = 0; i < kEach; i += 2) {
-    const int j = sub + kLanes * i;
-    const float2 g = of.at(x[i], x[i + 1], j, j + kLanes);
-    if (j < v) store_value(grad + j, g.x);
-    if (j + kLanes < v) store_value(grad + j + kLanes, g.y);
   }
 }
 
@@ -850,11 +1001,49 @@ scores_grad_kernel(const __grid_constant__ ScoresGrad p, uint32_t runs) {
 
 bool at_multiple(const void* p, int size) { return reinterpret_cast<uintptr_t>(p) % size == 0; }
 
-template <typename T, int kLanes>
+template <typename T, int kLanes, int kEach>
 int few_scores(const Scores& p, cudaStream_t s) {
-  few_scores_kernel<T, kLanes><<<unsigned((p.m * kLanes + 255) / 256), 256, 0, s>>>(p);
+  few_scores_kernel<T, kLanes, kEach><<<unsigned((p.m * kLanes + 255) / 256), 256, 0, s>>>(p);
   return launch_status();
 }
+template <typename T>
+int few_scores_of(const Scores& p, cudaStream_t s) {
+  if (p.v <= 8) return few_scores<T, 1, 8>(p, s);
+  if (p.v <= 16) return few_scores<T, 2, 8>(p, s);
+  if (p.v <= 32) return few_scores<T, 4, 8>(p, s);
+  // Rows that are many by few lanes (169,089 of 100 float32 18 us, by 16 lanes 24), so that a row's end is cheap; others by a warp,
+  // whose lanes have less to do one after the other (2,000 of 100 with four alternatives 3.0 us, by 8 lanes 4.8).
+  const bool many = p.m > 8192;
+  if (p.v <= 64) return many ? few_scores<T, 4, 16>(p, s) : few_scores<T, 32, 2>(p, s);
+  if (p.v <= 128) return many ? few_scores<T, 8, 16>(p, s) : few_scores<T, 32, 4>(p, s);
+  // Alternatives by a warp (169,089 of 200 float32 with eight 98 us, by 16 lanes 206; without any 43 and 32).
+  if (p.v <= 256) return p.top == 0 ? few_scores<T, 16, 16>(p, s) : few_scores<T, 32, 8>(p, s);
+  if (p.v <= 512) return few_scores<T, 32, 16>(p, s);
+  return few_scores<T, 32, 32>(p, s);
+}
+
+// A warp takes rows in turns, as many as leave 80 warps to an SM, twice what it holds (198,564 of 200 bf16 42 us, all rows in
+// turns of their own 70).
+template <typename T, int kLanes, int kEach>
+int few_scores_grad(const ScoresGrad& p, cudaStream_t s) {
+  constexpr int kAtOnce = 32 / kLanes;
+  const int64_t most = p.m / (kAtOnce * 148 * 80);
+  const int turns = most < 1 ? 1 : most > kLanes ? kLanes : int(most), rows = kAtOnce * 8 * turns;
+  few_scores_grad_kernel<T, kLanes, kEach><<<unsigned((p.m + rows - 1) / rows), 256, 0, s>>>(p, turns);
+  return launch_status();
+}
+template <typename T>
+int few_scores_grad_of(const ScoresGrad& p, cudaStream_t s) {
+  if (p.v <= 8) return few_scores_grad<T, 1, 8>(p, s);
+  if (p.v <= 16) return few_scores_grad<T, 2, 8>(p, s);
+  if (p.v <= 32) return few_scores_grad<T, 4, 8>(p, s);
+  if (p.v <= 64) return few_scores_grad<T, 8, 8>(p, s);
+  if (p.v <= 128) return few_scores_grad<T, 16, 8>(p, s);  // 198,564 of 106 bf16 24 us, by 8 lanes 28
+  if (p.v <= 256) return few_scores_grad<T, 16, 16>(p, s);  // of 200 42 us, by 32 lanes 46
+  if (p.v <= 512) return few_scores_grad<T, 32, 16>(p, s);
+  return few_scores_grad<T, 32, 32>(p, s);
+}
+
 template <typename T, int kWarps>
 int scores(const Scores& p, int blocks, cudaStream_t s) {
   using G = Team<kWarps>;
@@ -877,11 +1066,7 @@ int scores(const Scores& p, int blocks, cudaStream_t s) {
 template <typename T>
 int scores_of(const Scores& p, cudaStream_t s) {
   constexpr int kValues = Grid<T>::kValues;
-  if (p.v <= kEach) return few_scores<T, 1>(p, s);
-  if (p.v <= 2 * kEach) return few_scores<T, 2>(p, s);
-  if (p.v <= 4 * kEach) return few_scores<T, 4>(p, s);
-  if (p.v <= 8 * kEach) return few_scores<T, 8>(p, s);
-  if (p.v <= 32 * kEach) return few_scores<T, 32>(p, s);
+  if (p.v <= 1024) return few_scores_of<T>(p, s);
   // Warps a row. One for short rows that are many: what a row's end costs, its warps' joining above all, is paid by more rows at a
   // time (5,000 of 5,000 bf16 with eight alternatives 24 us, by four warps 37; 9,000 of 15,000 54 and 58; 1,000 of 3,000 7.9 and
   // 9.8). Four for long ones, whose warps then end at different times (4,096 of 32,768 bf16 49 us, by one warp 56; 2,400 of 60,000
@@ -889,7 +1074,7 @@ int scores_of(const Scores& p, cudaStream_t s) {
   // and 15.6). Sixteen, and a cluster of blocks that have a turn each, of few long rows (one row of 50,021 bf16 5.0 us, one block
   // 6.7; 20 of 30,000 float32 8.2, with a vector a thread 11.0).
   const int64_t vectors = p.v / kValues;
-  if (vectors <= 64 || (vectors <= 512 && p.m >= 4 * 148) || (vectors <= 2048 && p.m >= 16 * 148)) return scores<T, 1>(p, 1, s);
+  if ((vectors <= 512 && p.m >= 4 * 148) || (vectors <= 2048 && p.m >= 16 * 148)) return scores<T, 1>(p, 1, s);
   if (p.m >= 2 * 148 || vectors <= 256) return scores<T, 4>(p, 1, s);
   int blocks = 1;
   while (blocks < 8 && p.m * 16 * blocks < 8 * 148 && vectors > 2048 * blocks) blocks *= 2;
@@ -899,38 +1084,26 @@ int scores_of(const Scores& p, cudaStream_t s) {
 template <typename T>
 int scores_grad_of(const ScoresGrad& p, cudaStream_t s) {
   constexpr int kValues = Grid<T>::kValues;
-  const auto few = [&](auto lanes) {
-    few_scores_grad_kernel<T, lanes.value><<<unsigned((p.m * lanes.value + 255) / 256), 256, 0, s>>>(p);
+  const int64_t vectors = (p.v + 2 * kValues - 2) / kValues;
+  const bool alike = p.stride % kValues == p.v % kValues && reinterpret_cast<uintptr_t>(p.logits) % 16 ==
+                     reinterpret_cast<uintptr_t>(p.grad) % 16;
+  // Where logits and gradient lie differently on the boundaries, rows of lanes' single values are quicker for longer (52,413 of
+  // 1,000 bf16 54 us, by vectors 73, and 42 where they lie alike; 100,000 of 300 alike 40 and 70, of 512 47 and 54).
+  if (p.v <= (alike ? 512 : 1024)) return few_scores_grad_of<T>(p, s);
+  const auto run = [&](auto is_alike, auto is_masked) {
+    constexpr bool kAlike = decltype(is_alike)::value, kMasked = decltype(is_masked)::value;
+    constexpr int kRun = 32 * Run<kAlike, kMasked>::kVectors;
+    const int64_t runs = (vectors + kRun - 1) / kRun;
+    scores_grad_kernel<T, kAlike, kMasked><<<unsigned((p.m * runs + 7) / 8), 256, 0, s>>>(p, uint32_t(runs));
   };
-  if (p.v <= kEach) {
-    few(std::integral_constant<int, 1>());
-  } else if (p.v <= 2 * kEach) {
-    few(std::integral_constant<int, 2>());
-  } else if (p.v <= 4 * kEach) {
-    few(std::integral_constant<int, 4>());
-  } else if (p.v <= 8 * kEach) {
-    few(std::integral_constant<int, 8>());
-  } else if (p.v <= 32 * kEach) {
-    few(std::integral_constant<int, 32>());
-  } else {
-    const int64_t vectors = (p.v + 2 * kValues - 2) / kValues;
-    const bool alike = p.stride % kValues == p.v % kValues && reinterpret_cast<uintptr_t>(p.logits) % 16 ==
-                       reinterpret_cast<uintptr_t>(p.grad) % 16;
-    const auto run = [&](auto is_alike, auto is_masked) {
-      constexpr bool kAlike = decltype(is_alike)::value, kMasked = decltype(is_masked)::value;
-      constexpr int kRun = 32 * Run<kAlike, kMasked>::kVectors;
-      const int64_t runs = (vectors + kRun - 1) / kRun;
-      scores_grad_kernel<T, kAlike, kMasked><<<unsigned((p.m * runs + 7) / 8), 256, 0, s>>>(p, uint32_t(runs));
-    };
-    if (alike && p.allowed)
-      run(std::true_type(), std::true_type());
-    else if (alike)
-      run(std::true_type(), std::false_type());
-    else if (p.allowed)
-      run(std::false_type(), std::true_type());
-    else
-      run(std::false_type(), std::false_type());
-  }
+  if (alike && p.allowed)
+    run(std::true_type(), std::true_type());
+  else if (alike)
+    run(std::true_type(), std::false_type());
+  else if (p.allowed)
+    run(std::false_type(), std::true_type());
+  else
+    run(std::false_type(), std::false_type());
   return launch_status();
 }
 

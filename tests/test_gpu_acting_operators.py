@@ -445,6 +445,58 @@ def test_alternatives_of_equal_logits(cuda, v, dtype):
     check_scores(log_probs.forward(l, actions, allowed, top), l, actions, allowed, top)
 
 
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("m", [5, 8192, 8193])
+def test_scores_at_the_borders_between_forms(cuda, m, dtype):
+    """Rows of lanes' single values, by a few lanes or a warp, and the first of the longer ones, few rows and many: the
+    last team of a block's is not full. Rows repeat; those that start alike on the boundaries of 16 bytes, eight
+    repetitions further on, are the same bit for bit, and the first eight repetitions are checked."""
+    import log_probs
+
+    for v in (8, 9, 32, 33, 64, 65, 127, 128, 129, 255, 256, 257, 511, 512, 513, 1023, 1024, 1025):
+        some = min(m, 37)
+        l, actions, allowed = score_inputs(cuda, some, v, dtype, v % 2, v % 3 > 0, seed=v)
+        every, again = torch.arange(m, device=cuda) % some, torch.arange(m, device=cuda) % (8 * some)
+        many = torch.full((m, v + 3), 7.0, dtype=l.dtype, device=cuda)[:, :v].copy_(l[every])
+        al = None if allowed is None else allowed[every]
+        for top in sorted({0, 1, min(v, 9), min(v, 32)}):
+            got = log_probs.forward(many, actions[every], al, top)
+            for n in range(0, min(m, 8 * some), some):
+                check_scores(log_probs.Scores(*(None if x is None else x[n:n + some] for x in got)), l, actions, allowed, top)
+            for x in got:
+                assert x is None or torch.equal(x.nan_to_num(), x[again].nan_to_num())
+        g, h = normal(cuda, some, seed=2), normal(cuda, some, seed=3)
+        for logits in (many, many.contiguous()):
+            grad = log_probs.backward(g[every], h[every], logits, actions[every], got.normalizer, got.entropy, al)
+            first = log_probs.backward(g, h, l, actions, got.normalizer[:some], got.entropy[:some], allowed)
+            # forms differ by an instruction's rounding of a power's argument, one of each of the sums of two
+            assert (grad[:some].double() - first.double()).abs().max() <= 2 * torch.finfo(l.dtype).eps * max(1.0, first.double().abs().max())
+            assert torch.equal(grad.nan_to_num(), grad[again].nan_to_num())
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("v", [8, 16, 31, 60, 128, 250, 500, 1000, 1500, 5000, 40_000, 140_000])
+def test_alternatives_where_logits_are_not_numbers(cuda, v, dtype):
+    """NaN is above all logits, and ties go to the lower action, also where a row is nothing but NaN."""
+    import log_probs
+
+    top = min(v, 32)
+    l = normal(cuda, 4, v).to(TYPES[dtype])
+    l[0] = torch.nan
+    l[1, :] = -torch.inf
+    l[1, v // 2:] = torch.nan
+    l[2, -1] = torch.nan
+    for m in (4, 10_000):
+        if m * v > 2 ** 25:
+            continue
+        rows = l[torch.arange(m, device=cuda) % 4]
+        got = log_probs.forward(rows, torch.zeros(m, dtype=torch.int32, device=cuda), None, top)
+        above = torch.where(l.isnan(), torch.inf, l.float())
+        want = above.cpu().sort(dim=-1, descending=True, stable=True).indices[:, :top]
+        assert torch.equal(got.top_actions[:4].cpu(), want) and torch.equal(got.top_actions, got.top_actions[:4].repeat(m // 4, 1))
+        assert got.top_log_probs[:3].isnan().all() and got.top_log_probs[3].isfinite().all()
+
+
 @pytest.mark.parametrize("v", [2, 30, 100, 400, 1200, 3000, 20_000, 70_000])
 def test_scores_where_rows_are_odd(cuda, v):
     """Padding, actions outside, rows that allow nothing, logits that are not finite in and out of masked places: each
