@@ -34,24 +34,6 @@ struct Raw {
   uint4 bits;
   RLENV_D void load(const T* from) { bits = __ldg(reinterpret_cast<const uint4*>(from)); }
   RLENV_D void clear() { bits = make_uint4(0, 0, 0, 0); }
-  // From any place: `before` and `after` it there are that many values of the same array.
-  RLENV_D void load_between(const T* from, int before, int after) {
-    const bool between = sizeof(T) == 2 && reinterpret_cast<uintptr_t>(from) % 4;
-    if (between && (before < 1 || after < 1)) {
-      uint32_t w[4] = {0, 0, 0, 0};
-#pragma unroll
-      for (int i = 0; i < kValues; ++i)
-        w[i * int(sizeof(T)) / 4] |= uint32_t(__ldg(reinterpret_cast<const unsigned short*>(from) + i)) << 16 * (i % 2);
-      bits = make_uint4(w[0], w[1], w[2], w[3]);
-      return;
-    }
-    const uint32_t* const words = reinterpret_cast<const uint32_t*>(between ? from - 1 : from);
-    const uint32_t w0 = __ldg(words), w1 = __ldg(words + 1), w2 = __ldg(words + 2), w3 = __ldg(words + 3);
-    bits = make_uint4(w0, w1, w2, w3);
-    if (between)
-      bits = make_uint4(__funnelshift_r(w0, w1, 16), __funnelshift_r(w1, w2, 16), __funnelshift_r(w2, w3, 16),
-                        __funnelshift_r(w3, __ldg(words + 4), 16));
-  }
   RLENV_D void values(float* v) const {
     const uint32_t w[4] = {bits.x, bits.y, bits.z, bits.w};
 #pragma unroll
@@ -67,7 +49,6 @@ template <>
 struct Raw<float, 1> {
   float bits;
   RLENV_D void load(const float* from) { bits = __ldg(from); }
-  RLENV_D void load_between(const float* from, int, int) { load(from); }
   RLENV_D void clear() { bits = 0.0f; }
   RLENV_D void values(float* v) const { v[0] = bits; }
 };
@@ -75,9 +56,31 @@ template <>
 struct Raw<__nv_bfloat16, 1> {
   unsigned short bits;
   RLENV_D void load(const __nv_bfloat16* from) { bits = __ldg(reinterpret_cast<const unsigned short*>(from)); }
-  RLENV_D void load_between(const __nv_bfloat16* from, int, int) { load(from); }
   RLENV_D void clear() { bits = 0; }
   RLENV_D void values(float* v) const { v[0] = __uint_as_float(uint32_t(bits) << 16); }
+};
+// A vector from any place, as the words that hold it: those of bfloat16 start a value earlier where that lies on a boundary of
+// four bytes. `from` itself may be the array's first value only where it lies on one.
+template <typename T>
+struct Between {
+  static constexpr int kWords = sizeof(T) == 2 ? 5 : 4;
+  uint32_t words[kWords];
+  RLENV_D void clear() {
+#pragma unroll
+    for (int i = 0; i < kWords; ++i) words[i] = 0;
+  }
+  RLENV_D void load(const T* from, bool between) {
+    const uint32_t* const at = reinterpret_cast<const uint32_t*>(between ? from - 1 : from);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) words[i] = __ldg(at + i);
+    if constexpr (kWords == 5) words[4] = __ldg(reinterpret_cast<const unsigned short*>(from) + 7);
+  }
+  RLENV_D uint4 bits(bool between) const {
+    if constexpr (kWords == 4) return make_uint4(words[0], words[1], words[2], words[3]);
+    const int by = between ? 16 : 0;
+    return make_uint4(__funnelshift_r(words[0], words[1], by), __funnelshift_r(words[1], words[2], by),
+                      __funnelshift_r(words[2], words[3], by), __funnelshift_r(words[3], words[kWords - 1], by));
+  }
 };
 template <typename T>
 RLENV_D float load(const T* from) {
@@ -148,20 +151,48 @@ struct Part {
       if (edge >= 0) r.edge.load(row + edge);
     }
   }
+  RLENV_D void fetch(const T* row) const {  // into L2
+#pragma unroll
+    for (int i = 0; i < kVectors; ++i)
+      if (i < count) asm volatile("prefetch.global.L2 [%0];" ::"l"(row + place(i)));
+  }
   RLENV_D void clear(Row& r) const {
 #pragma unroll
     for (int i = 0; i < kVectors; ++i) r.vectors[i].clear();
     r.edge.clear();
   }
-  RLENV_D void load_weight(const T* weight, Row& r) const {  // which lies on a boundary by itself
-    if constexpr (!kEdge) {
-      load(weight, r);
-    } else {
+  // The weights of these places: they lie on a boundary by themselves, so that a skewed row's vectors of them do not. Nothing
+  // waits for them before `values`.
+  struct Weights {
+    std::conditional_t<kEdge, Between<T>, Raw<T, kN>> vectors[kVectors];
+    Raw<T, 1> edge;
+    bool between;
+    RLENV_D Row row() const {
+      Row r;
 #pragma unroll
       for (int i = 0; i < kVectors; ++i) {
-        r.vectors[i].clear();
-        if (i < count) r.vectors[i].load_between(weight + place(i), place(i), k - place(i) - kN);
+        if constexpr (kEdge)
+          r.vectors[i].bits = vectors[i].bits(between);
+        else
+          r.vectors[i] = vectors[i];
       }
+      if constexpr (kEdge) r.edge = edge;
+      return r;
+    }
+  };
+  RLENV_D void load_weight(const T* weight, Weights& r) const {
+    r.between = kEdge && sizeof(T) == 2 && first % 2;
+#pragma unroll
+    for (int i = 0; i < kVectors; ++i) {
+      r.vectors[i].clear();
+      if (i < count) {
+        if constexpr (kEdge)
+          r.vectors[i].load(weight + place(i), r.between);
+        else
+          r.vectors[i].load(weight + place(i));
+      }
+    }
+    if constexpr (kEdge) {
       r.edge.clear();
       if (edge >= 0) r.edge.load(weight + edge);
     }
@@ -301,7 +332,8 @@ __global__ void __launch_bounds__(Team<kThreads>::kBlock) norm_kernel(const __gr
   }
 #pragma unroll
   for (int i = 0; i < kCount; ++i) sum[0] = fmaf(t[i], t[i], sum[0]);
-  if (weight) part.load_weight(weight, other);  // on its way while the sum is formed
+  typename P::Weights weights;
+  if (weight) part.load_weight(weight, weights);  // on its way while the sum is formed
   if (p.total && there) part.store_row(static_cast<T*>(p.total) + row * p.k, t);
   float r = 1.0f;
   if (!kCodes || p.normalise) {
@@ -312,7 +344,7 @@ __global__ void __launch_bounds__(Team<kThreads>::kBlock) norm_kernel(const __gr
   for (int i = 0; i < kCount; ++i) t[i] *= r;
   if (weight) {
     float w[kCount];
-    other.values(w);
+    weights.row().values(w);
 #pragma unroll
     for (int i = 0; i < kCount; ++i) t[i] *= w[i];
   }
@@ -380,15 +412,31 @@ struct NormGrad {
   float* parts;  // (blocks, K): each block's sums over its rows of the weight's gradient; null: none asked for
 };
 
-// A team's next row is on its way while it works on one (kAhead: where registers allow). Its rows are a multiple of 8
-// apart, so that they all lie alike on the boundaries.
+// A team's next row is on its way while it works on one (kAhead: where registers allow; else it is fetched into L2). Its rows are
+// a multiple of 8 apart, so that they all lie alike on the boundaries. The longest rows' weight gradient lies in shared memory
+// (kApart), a thread's columns in places of its own, and float32 weights are read from L1 for each use: 400 MB of rows of 16,384
+// bf16 110 us, of 12,288 float32 93 (with all of it in registers, which do not hold it, 136 and 133; with the next row on its way
+// into shared memory too 104 and 93, but 88 instead of 73 for 6,145 float32). Two blocks of 256 threads an SM are what the grid
+// counts on, also where a few values are spilled for it (rows of 641 bf16 104 us, else 124).
 template <typename T, Way kWay, int kThreads, int kVectors>
-__global__ void __launch_bounds__(Team<kThreads>::kBlock) norm_grad_kernel(const __grid_constant__ NormGrad p) {
+struct Grads {
+  using P = Part<T, kWay, kThreads, kVectors>;
+  static constexpr bool kAhead = kVectors * int(sizeof(Raw<T, P::kN>)) <= 32, kApart = kWay != kSingle && kVectors * P::kN >= 32,
+                        kHeldWeights = kVectors * int(sizeof(Raw<T, P::kN>)) <= 64;
+  static constexpr int kApartBytes = kApart ? kThreads * kVectors * P::kN * 4 : 0;
+  static constexpr int kBlocks = Team<kThreads>::kBlock <= 256 ? 2 : 1;  // an SM's, which the grid counts on
+};
+template <typename T, Way kWay, int kThreads, int kVectors>
+__global__ void __launch_bounds__(Team<kThreads>::kBlock, (Grads<T, kWay, kThreads, kVectors>::kBlocks))
+norm_grad_kernel(const __grid_constant__ NormGrad p) {
   using G = Team<kThreads>;
   using P = Part<T, kWay, kThreads, kVectors>;
   using Row = typename P::Row;
-  constexpr int kCount = P::kCount;
-  constexpr bool kAhead = kVectors * int(sizeof(Raw<T, P::kN>)) <= 32;
+  using Form = Grads<T, kWay, kThreads, kVectors>;
+  constexpr int kCount = P::kCount, kN = P::kN;
+  constexpr bool kAhead = Form::kAhead, kApart = Form::kApart;
+  constexpr int kOwn = kApart ? P::kEdge + 1 : kCount;  // columns whose sums are in registers
+  extern __shared__ __align__(16) float columns[];
   __shared__ float room[2 * G::kWarps * G::kRows];
   const int at = threadIdx.x % kThreads, k = int(p.k);
   const int64_t step = int64_t(gridDim.x) * G::kRows;
@@ -396,13 +444,26 @@ __global__ void __launch_bounds__(Team<kThreads>::kBlock) norm_grad_kernel(const
   // A warp's teams make as many turns as its first.
   const int64_t turns = (p.m - (int64_t(blockIdx.x) * G::kRows + threadIdx.x / 32 * 32 / kThreads) + step - 1) / step;
   const P part(static_cast<const T*>(p.total) + row * p.total_stride, k, at);
-  float dw[kCount];
+  float dw[kOwn];
 #pragma unroll
-  for (int i = 0; i < kCount; ++i) dw[i] = 0.0f;
+  for (int i = 0; i < kOwn; ++i) dw[i] = 0.0f;
+  const auto apart = [&](int i, int j) { return reinterpret_cast<float4*>(columns) + (i * (kN / 4) + j) * kThreads + at; };
+  if constexpr (kApart) {
+#pragma unroll
+    for (int i = 0; i < kVectors; ++i)
+#pragma unroll
+      for (int j = 0; j < kN / 4; ++j) *apart(i, j) = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  }
   Row w, t, g, s;
-  if (p.weight) part.load_weight(static_cast<const T*>(p.weight), w);
+  const auto load_weights = [&] {
+    typename P::Weights weights;
+    part.load_weight(static_cast<const T*>(p.weight), weights);
+    w = weights.row();
+  };
+  if (p.weight && Form::kHeldWeights) load_weights();
   const auto weighed = [&](float (&v)[kCount]) {
     if (!p.weight) return;
+    if (!Form::kHeldWeights) load_weights();
     float of[kCount];
     w.values(of);
 #pragma unroll
@@ -423,10 +484,16 @@ __global__ void __launch_bounds__(Team<kThreads>::kBlock) norm_grad_kernel(const
   if (kAhead) load_row(row, t, g, s);
   for (int64_t turn = 0; turn < turns; ++turn, row += step) {
     Row next_t, next_g, next_s;
-    if (kAhead)
+    if (kAhead) {
       load_row(row + step, next_t, next_g, next_s);
-    else
+    } else {
       load_row(row, t, g, s);
+      if (kWay != kSingle && row + step < p.m) {
+        part.fetch(static_cast<const T*>(p.total) + (row + step) * p.total_stride);
+        part.fetch(static_cast<const T*>(p.grad_out) + (row + step) * p.grad_out_stride);
+        if (p.grad_total) part.fetch(static_cast<const T*>(p.grad_total) + (row + step) * p.grad_total_stride);
+      }
+    }
     float tv[kCount], gv[kCount], sums[2] = {0.0f, 0.0f};
     t.values(tv), g.values(gv);
     weighed(gv);
@@ -436,8 +503,22 @@ __global__ void __launch_bounds__(Team<kThreads>::kBlock) norm_grad_kernel(const
     const float r = row < p.m ? rsqrtf(sums[0] / float(k) + p.eps) : 0.0f, along = r * (r * sums[1] / float(k));
     float v[kCount];
     t.values(tv), g.values(gv), s.values(v);
+    if constexpr (kApart) {
 #pragma unroll
-    for (int i = 0; i < kCount; ++i) dw[i] = fmaf(gv[i], tv[i] * r, dw[i]);
+      for (int i = 0; i < kVectors; ++i)
+#pragma unroll
+        for (int j = 0; j < kN / 4; ++j) {
+          float4 sum = *apart(i, j);
+          const int c = i * kN + 4 * j;
+          sum.x = fmaf(gv[c], tv[c] * r, sum.x), sum.y = fmaf(gv[c + 1], tv[c + 1] * r, sum.y);
+          sum.z = fmaf(gv[c + 2], tv[c + 2] * r, sum.z), sum.w = fmaf(gv[c + 3], tv[c + 3] * r, sum.w);
+          *apart(i, j) = sum;
+        }
+      if constexpr (P::kEdge) dw[0] = fmaf(gv[kCount - 1], tv[kCount - 1] * r, dw[0]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < kCount; ++i) dw[i] = fmaf(gv[i], tv[i] * r, dw[i]);
+    }
     weighed(gv);
 #pragma unroll
     for (int i = 0; i < kCount; ++i) v[i] += r * (gv[i] - tv[i] * along);
@@ -452,26 +533,41 @@ __global__ void __launch_bounds__(Team<kThreads>::kBlock) norm_grad_kernel(const
 #pragma unroll
       for (int d = kThreads; d < 32; d *= 2) dw[i] += __shfl_xor_sync(0xffffffffu, dw[i], d);
   }
-  extern __shared__ __align__(16) float columns[];  // k, where there are more sets than one
-  constexpr int kSets = kThreads < 32 ? G::kBlock / 32 : G::kRows;  // of threads with all of the columns
-  const int set = kThreads < 32 ? threadIdx.x / 32 : threadIdx.x / kThreads;
   float* const block_part = p.parts + int64_t(blockIdx.x) * p.k;
-  for (int n = 0; n < kSets; ++n) {
-    if (set == n && (kThreads >= 32 || threadIdx.x % 32 < kThreads)) {
-      if (n > 0) part.each(dw, [&](int c, float& v) { v += columns[c]; });
-      float* const to = n + 1 < kSets ? columns : block_part;
-      if constexpr (kWay == kWhole) {
+  if constexpr (kApart) {
+    static_assert(G::kRows == 1, "a block has one set of columns");
 #pragma unroll
-        for (int i = 0; i < kVectors; ++i)
-          if (i < part.count) {
+    for (int i = 0; i < kVectors; ++i)
+      if (i < part.count) {
 #pragma unroll
-            for (int j = 0; j < P::kN; j += 4) store_vector(to + part.place(i) + j, dw + i * P::kN + j);
-          }
-      } else {
-        part.each(dw, [&](int c, float v) { to[c] = v; });
+        for (int j = 0; j < kN / 4; ++j) {
+          const float4 sum = *apart(i, j);
+          float* const to = block_part + part.place(i) + 4 * j;
+          to[0] = sum.x, to[1] = sum.y, to[2] = sum.z, to[3] = sum.w;
+        }
       }
+    if constexpr (P::kEdge)
+      if (part.edge >= 0) block_part[part.edge] = dw[0];
+  } else {
+    constexpr int kSets = kThreads < 32 ? G::kBlock / 32 : G::kRows;  // of threads with all of the columns
+    const int set = kThreads < 32 ? threadIdx.x / 32 : threadIdx.x / kThreads;
+    for (int n = 0; n < kSets; ++n) {
+      if (set == n && (kThreads >= 32 || threadIdx.x % 32 < kThreads)) {
+        if (n > 0) part.each(dw, [&](int c, float& v) { v += columns[c]; });
+        float* const to = n + 1 < kSets ? columns : block_part;
+        if constexpr (kWay == kWhole) {
+#pragma unroll
+          for (int i = 0; i < kVectors; ++i)
+            if (i < part.count) {
+#pragma unroll
+              for (int j = 0; j < kN; j += 4) store_vector(to + part.place(i) + j, dw + i * kN + j);
+            }
+        } else {
+          part.each(dw, [&](int c, float v) { to[c] = v; });
+        }
+      }
+      if (kSets > 1) __syncthreads();
     }
-    if (kSets > 1) __syncthreads();
   }
 }
 
@@ -548,25 +644,44 @@ template <typename T, typename F>
 bool with_form(Way way, int64_t k, F&& f) {
   constexpr int kN = 16 / int(sizeof(T));
   const int64_t vectors = k / kN;
+  // Threads that a row just fills, three or four vectors each: bytes on their way are what counts (rows of 1,288 bf16, 400 MB
+  // in all, 61 us, by 128 threads with two vectors in some 86; of 1,041 81 and 153). Long ones with fewer vectors in more threads
+  // are no quicker (8,193 bf16 67 us, by 1,024 threads 76).
   if (way == kWhole) {
     const auto g = [&](auto form) { return f(std::integral_constant<Way, kWhole>(), form), true; };
     if (vectors <= 8) return g(Form<8, 1>());
     if (vectors <= 16) return g(Form<16, 1>());
     if (vectors <= 32) return g(Form<32, 1>());
     if (vectors <= 64) return g(Form<32, 2>());
+    if (vectors <= 96) return g(Form<32, 3>());
     if (vectors <= 128) return g(Form<32, 4>());
+    if (vectors <= 192) return g(Form<64, 3>());
+    if (vectors <= 256) return g(Form<64, 4>());
+    if (vectors <= 384) return g(Form<128, 3>());
     if (vectors <= 512) return g(Form<128, 4>());
+    if (vectors <= 768) return g(Form<256, 3>());
     if (vectors <= 1024) return g(Form<256, 4>());
+    if (vectors <= 1536) return g(Form<512, 3>());
     if (vectors <= 2048) return g(Form<512, 4>());
+    if (vectors <= 3072) return g(Form<512, 6>());
     if (vectors <= 4096) return g(Form<512, 8>());
   } else if (way == kSkewed) {
     const auto g = [&](auto form) { return f(std::integral_constant<Way, kSkewed>(), form), true; };
+    if (vectors <= 16) return g(Form<16, 1>());
     if (vectors <= 32) return g(Form<32, 1>());
     if (vectors <= 64) return g(Form<32, 2>());
+    if (vectors <= 96) return g(Form<32, 3>());
     if (vectors <= 128) return g(Form<32, 4>());
+    if (vectors <= 192) return g(Form<64, 3>());
+    if (vectors <= 256) return g(Form<64, 4>());
+    if (vectors <= 384) return g(Form<128, 3>());
     if (vectors <= 512) return g(Form<128, 4>());
+    if (vectors <= 768) return g(Form<256, 3>());
     if (vectors <= 1024) return g(Form<256, 4>());
+    if (vectors <= 1536) return g(Form<512, 3>());
     if (vectors <= 2048) return g(Form<512, 4>());
+    if (vectors <= 3072) return g(Form<512, 6>());
+    if (vectors <= 4096) return g(Form<512, 8>());
   }
   const auto g = [&](auto form) { return f(std::integral_constant<Way, kSingle>(), form), true; };
   if (k <= 32) return g(Form<32, 1>());
@@ -605,6 +720,8 @@ bool with_grad_form(Way way, int64_t k, F&& f) {
     if (vectors <= 512) return g(Form<256, 2>());
     if (vectors <= 1024) return g(Form<512, 2>());
     if (vectors <= 2048) return g(Form<512, 4>());
+    if constexpr (sizeof(T) == 4)
+      if (vectors <= 4096) return g(Form<512, 8>());
   }
   const auto g = [&](auto form) { return f(std::integral_constant<Way, kSingle>(), form), true; };
   if (k <= 32) return g(Form<32, 1>());
@@ -643,12 +760,18 @@ int norm_grad(const NormGrad& p, void* grad_weight, cudaStream_t s) {
   const Way way = way_of<T>(p.k, {{p.grad_out, p.grad_out_stride}, {p.total, p.total_stride}, {p.grad_total, p.grad_total_stride},
                                   {p.grad, p.k}, {p.weight, p.k}});
   int64_t blocks = grad_blocks(p.m);
+  cudaError_t shared_memory = cudaSuccess;
   const bool held = with_grad_form<T>(way, p.k, [&](auto of_way, auto form) {
     using G = Team<form.kThreads>;
     blocks = grad_blocks((p.m + G::kRows - 1) / G::kRows);
-    const size_t shared = G::kRows > 1 ? p.k * sizeof(float) : 0;
-    norm_grad_kernel<T, of_way.value, form.kThreads, form.kVectors><<<unsigned(blocks), G::kBlock, shared, s>>>(p);
+    constexpr int kApart = Grads<T, of_way.value, form.kThreads, form.kVectors>::kApartBytes;
+    // columns' sums of more rows than one, or a thread's own
+    const size_t shared = kApart ? kApart : G::kRows > 1 ? p.k * sizeof(float) : 0;
+    const auto kernel = norm_grad_kernel<T, of_way.value, form.kThreads, form.kVectors>;
+    if constexpr (kApart > 0) shared_memory = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kApart);
+    if (shared_memory == cudaSuccess) kernel<<<unsigned(blocks), G::kBlock, shared, s>>>(p);
   });
+  if (shared_memory != cudaSuccess) return int(shared_memory);
   if (!held) long_norm_grad_kernel<T><<<unsigned(blocks), kLong, 0, s>>>(p);
   if (int rc = launch_status(); rc || !p.parts) return rc;
   add_rows_kernel<T><<<unsigned((p.k + 7) / 8), 256, 0, s>>>(p.parts, int(blocks), p.k, static_cast<T*>(grad_weight));
