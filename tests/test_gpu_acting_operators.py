@@ -124,6 +124,18 @@ def test_norm_backward(cuda, m, k, dtype):
 
 
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("vectors", [16, 32, 64, 96, 128, 192, 256, 384, 512, 768, 1024, 1536, 2048, 4096])
+def test_norm_at_the_borders_between_forms(cuda, vectors, dtype):
+    """Rows of as many vectors of 16 bytes and of one more, whole and with values before and after them; gradients of
+    blocks with a second row."""
+    each = 4 if dtype == "f32" else 8
+    for k in (vectors * each, vectors * each + 1, vectors * each + each, vectors * each + each + 3):
+        test_norm_forward(cuda, 9, k, dtype)
+        test_norm_in_8_bits(cuda, 9, k, dtype)
+        test_norm_backward(cuda, 150 if k > 2000 else 1500, k, dtype)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
 def test_norm_takes_rows_of_any_layout(cuda, dtype):
     """Slices, expanded rows, strides that are copied and bases off every boundary."""
     import int8_linear
