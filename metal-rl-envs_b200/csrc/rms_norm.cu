@@ -415,8 +415,8 @@ struct NormGrad {
 // A team's next row is on its way while it works on one (kAhead: where registers allow; else it is fetched into L2). Its rows are
 // a multiple of 8 apart, so that they all lie alike on the boundaries. The longest rows' weight gradient lies in shared memory
 // (kApart), a thread's columns in places of its own, and float32 weights are read from L1 for each use: 400 MB of rows of 16,384
-// bf16 110 us, of 12,288 float32 93 (with all of it in registers, which do not hold it, 136 and 133; with the next row on its way
-// into shared memory too 104 and 93, but 88 instead of 73 for 6,145 float32). Two blocks of 256 threads an SM are what the grid
+// bf16 102 us, of 12,288 float32 91 (with all of it in registers, which do not hold it, 136 and 133; the next row on its way into
+// shared memory too gains 5% there and costs 6,145 float32 20%). Two blocks of 256 threads an SM are what the grid
 // counts on, also where a few values are spilled for it (rows of 641 bf16 104 us, else 124).
 template <typename T, Way kWay, int kThreads, int kVectors>
 struct Grads {
@@ -749,21 +749,22 @@ int norm(const Norm& p, cudaStream_t s) {
 }
 
 // Blocks of the gradient's kernel, each with a row of the weight's gradient in scratch: two an SM (128,000 x 512 bf16 87 us;
-// one 114, three 106, four 95), and of few rows fewer, so that a team has some. Multiples of 8 where it has more than one.
-constexpr int kGradBlocks = 2 * 148;
-int64_t grad_blocks(int64_t rows) {
-  return rows <= 144 ? rows : rows < 4 * 144 ? 144 : rows < 4 * kGradBlocks ? rows / 4 / 8 * 8 : kGradBlocks;
+// one 114, three 106, four 95), of those that fill an SM one (1,000 x 16,384 bf16 49 us, two one after the other 62), and of few
+// rows fewer, so that a team has some. Multiples of 8 where it has more than one.
+constexpr int kGradBlocks = 2 * 148, kGradBlocksAlone = 144;
+int64_t grad_blocks(int64_t rows, int64_t most) {
+  return rows <= 144 ? rows : rows < 4 * 144 ? 144 : rows < 4 * most ? rows / 4 / 8 * 8 : most;
 }
 
 template <typename T>
 int norm_grad(const NormGrad& p, void* grad_weight, cudaStream_t s) {
   const Way way = way_of<T>(p.k, {{p.grad_out, p.grad_out_stride}, {p.total, p.total_stride}, {p.grad_total, p.grad_total_stride},
                                   {p.grad, p.k}, {p.weight, p.k}});
-  int64_t blocks = grad_blocks(p.m);
+  int64_t blocks = grad_blocks(p.m, kGradBlocks);
   cudaError_t shared_memory = cudaSuccess;
   const bool held = with_grad_form<T>(way, p.k, [&](auto of_way, auto form) {
     using G = Team<form.kThreads>;
-    blocks = grad_blocks((p.m + G::kRows - 1) / G::kRows);
+    blocks = grad_blocks((p.m + G::kRows - 1) / G::kRows, G::kBlock > 256 ? kGradBlocksAlone : kGradBlocks);
     constexpr int kApart = Grads<T, of_way.value, form.kThreads, form.kVectors>::kApartBytes;
     // columns' sums of more rows than one, or a thread's own
     const size_t shared = kApart ? kApart : G::kRows > 1 ? p.k * sizeof(float) : 0;
