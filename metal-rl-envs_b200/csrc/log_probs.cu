@@ -7,7 +7,7 @@
 // A row is read once: any number will do for b that is not far below the largest logit, so that sums begin with the first
 // vectors and nothing waits for a largest one. The bound is memory, with the power unit close behind (a logit is one
 // power, 16 a clock and SM, and some 8 instructions of which half work on two values): 4,096 x 32,768 bf16 49 us (5.5 TB/s),
-// 3,000 x 32,768 float32 66 (5.9 TB/s), with eight alternatives 67 and 4,096 x 32,768 bf16 with a mask 70 (5.7 TB/s); the gradient
+// with eight alternatives 62, with a mask 70 (5.7 TB/s), 3,000 x 32,768 float32 66 (5.9 TB/s); the gradient
 // of 4,096 x 16,384 bf16 48 us (5.6 TB/s), float32 85 (6.3 TB/s), of 4,096 x 32,771 bf16 with a mask 120 (5.6 TB/s). Other
 // arrangements of the forward pass, for 4,096 x 32,768 bf16 with eight alternatives: a row in a block's registers, its largest
 // logit first, 128 us (barriers); in its shared memory 126; a warp a row, alternatives kept as they come, 170 (insertions).
