@@ -646,7 +646,8 @@ bool with_form(Way way, int64_t k, F&& f) {
   const int64_t vectors = k / kN;
   // Threads that a row just fills, three or four vectors each: bytes on their way are what counts (rows of 1,288 bf16, 400 MB
   // in all, 61 us, by 128 threads with two vectors in some 86; of 1,041 81 and 153). Long ones with fewer vectors in more threads
-  // are no quicker (8,193 bf16 67 us, by 1,024 threads 76).
+  // are no quicker (8,193 bf16 67 us, by 1,024 threads 76), nor are more vectors in each than a row needs: 10,240 float32,
+  // 200 MB in all, 68 us with six, 99 with seven.
   if (way == kWhole) {
     const auto g = [&](auto form) { return f(std::integral_constant<Way, kWhole>(), form), true; };
     if (vectors <= 8) return g(Form<8, 1>());
@@ -663,7 +664,7 @@ bool with_form(Way way, int64_t k, F&& f) {
     if (vectors <= 1024) return g(Form<256, 4>());
     if (vectors <= 1536) return g(Form<512, 3>());
     if (vectors <= 2048) return g(Form<512, 4>());
-    if (vectors <= 3072) return g(Form<512, 6>());
+    if (vectors <= 512 * 6) return g(Form<512, 6>());
     if (vectors <= 4096) return g(Form<512, 8>());
   } else if (way == kSkewed) {
     const auto g = [&](auto form) { return f(std::integral_constant<Way, kSkewed>(), form), true; };
@@ -680,7 +681,7 @@ bool with_form(Way way, int64_t k, F&& f) {
     if (vectors <= 1024) return g(Form<256, 4>());
     if (vectors <= 1536) return g(Form<512, 3>());
     if (vectors <= 2048) return g(Form<512, 4>());
-    if (vectors <= 3072) return g(Form<512, 6>());
+    if (vectors <= 512 * 6) return g(Form<512, 6>());
     if (vectors <= 4096) return g(Form<512, 8>());
   }
   const auto g = [&](auto form) { return f(std::integral_constant<Way, kSingle>(), form), true; };
