@@ -748,7 +748,9 @@ scores_kernel(const __grid_constant__ Scores p) {
         }
       }
       __syncwarp();
-      if (best.count > Best::kMany)
+      const int count = best.count;
+      __syncwarp();  // all lanes have read it before one adds to it again: they keep together or not at all
+      if (count > Best::kMany)
         if (const uint64_t now = best.keep(p.top)) least_key = now;
     };
     for (int first = 0; first < total; first += 32 * kSteps) {  // kSteps vectors of a lane on their way together

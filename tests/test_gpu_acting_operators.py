@@ -576,6 +576,22 @@ def test_the_check_build_reports_actions_outside(cuda):
             assert lib.rlenv_checks_status(ctypes.byref(word), 1) == 0 and word.value & 1 == want
 
 
+@pytest.mark.parametrize("m,v", [(4, 1500), (700, 3000), (3000, 9000), (600, 20_000), (4, 30_000), (1, 140_000)])
+def test_alternatives_whose_list_is_shortened_often(cuda, m, v):
+    """Rows that rise, fall, or rise in stretches of a lane's reach, by a warp, a block and a cluster: far more logits reach
+    the list of alternatives than it holds, again and again. Called over and over, always the same."""
+    import log_probs
+
+    at = torch.arange(v, device=cuda, dtype=torch.float32)
+    rows = torch.stack([at, -at, at % 1024, at // 8 % 64 * 8 + at % 8])
+    want = torch.tensor(np.stack([policy.best(to64(rows), 32)]), device=cuda)[0]
+    which = torch.arange(m, device=cuda) % 4
+    l, actions = rows[which], torch.zeros(m, dtype=torch.int64, device=cuda)
+    for top in (32, 5, 32, 5):
+        got = log_probs.forward(l, actions, None, top)
+        assert torch.equal(got.top_actions, want[which, :top])
+
+
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
 @pytest.mark.parametrize("v", [7, 60, 250, 400, 1500, 5000, 40_000, 140_000])
 def test_scores_of_rows_that_grow(cuda, v, dtype):
