@@ -86,11 +86,6 @@ RLENV_D float value_of(uint32_t order) {
 }
 RLENV_D uint64_t key_of(float x, uint32_t place) { return uint64_t(order_of(x)) << 32 | ~place; }
 
-// l - normalizer, also where both are -infinity.
-RLENV_D float log_prob_of(float l, float normalizer) {
-  return l == -infinity() && normalizer == -infinity() ? l : l - normalizer;
-}
-
 // Of a part of a row: its largest logit, and S and W against it (against 0 where that is -infinity: both are 0 then).
 struct Sums {
   float m, s, w;
@@ -124,7 +119,17 @@ RLENV_D Sums of_team(const Sums& a) {
   const float2 of = values_of(both);
   return {own.m, of.x, of.y};
 }
-RLENV_D float normalizer_of(const Sums& a) { return base_of(a.m) + logf(a.s); }
+// A row's normalizer as the two terms that it is the sum of: subtracted from a logit one after the other they leave a
+// log-probability whose error does not grow with what the row's logits have in common (eight equal logits of 1e5: -2.0794415, less
+// the rounded sum -2.078125).
+struct Normalizer {
+  float base, log_sum;
+  RLENV_D explicit Normalizer(const Sums& a) : base(base_of(a.m)), log_sum(logf(a.s)) {}
+  RLENV_D float whole() const { return base + log_sum; }
+  RLENV_D float log_prob(float l) const {  // -infinity of a row that allows nothing too
+    return l == -infinity() && log_sum == -infinity() ? l : (l - base) - log_sum;
+  }
+};
 
 // A row's action and its logit, read before the row so that nothing waits for them after it.
 struct Chosen {
@@ -137,15 +142,15 @@ struct Chosen {
   }
 };
 
-RLENV_D void write_scores(const Scores& p, int64_t row, const Sums& sums, float normalizer, const Chosen& chosen) {
-  p.normalizer[row] = normalizer;
-  p.entropy[row] = sums.s == 0.0f ? 0.0f : logf(sums.s) - sums.w / sums.s;
+RLENV_D void write_scores(const Scores& p, int64_t row, const Sums& sums, const Normalizer& normalizer, const Chosen& chosen) {
+  p.normalizer[row] = normalizer.whole();
+  p.entropy[row] = sums.s == 0.0f ? 0.0f : normalizer.log_sum - sums.w / sums.s;
   check_flag(chosen.action >= p.v, kCheckActionRange);
-  p.log_prob[row] = chosen.action < 0 ? 0.0f : chosen.action >= p.v ? not_a_number() : log_prob_of(chosen.l, normalizer);
+  p.log_prob[row] = chosen.action < 0 ? 0.0f : chosen.action >= p.v ? not_a_number() : normalizer.log_prob(chosen.l);
 }
-RLENV_D void write_top(const Scores& p, int64_t row, int rank, uint64_t key, float normalizer) {
+RLENV_D void write_top(const Scores& p, int64_t row, int rank, uint64_t key, const Normalizer& normalizer) {
   p.top_actions[row * p.top + rank] = int64_t(uint32_t(~uint32_t(key)));
-  p.top_log_probs[row * p.top + rank] = log_prob_of(value_of(uint32_t(key >> 32)), normalizer);
+  p.top_log_probs[row * p.top + rank] = normalizer.log_prob(value_of(uint32_t(key >> 32)));
 }
 
 // ---- few actions: a row is the work of kLanes neighbouring lanes, kEach logits of it in each --------------
@@ -180,7 +185,7 @@ RLENV_D K largest_of_team(K key) {
 // it up. The lanes write together, each kLanes-th of them. A search through all lanes' logits for each takes twice as long
 // (192,341 of 41 float32 with twenty alternatives 90 us, by searches 187; 169,089 of 100 bf16 with eight 59 and 314).
 template <typename T, int kLanes, int kEach>
-RLENV_D void few_best(const Scores& p, int64_t row, bool real, int sub, const float (&x)[kEach], float normalizer) {
+RLENV_D void few_best(const Scores& p, int64_t row, bool real, int sub, const float (&x)[kEach], const Normalizer& normalizer) {
   using K = decltype(few_key(static_cast<const T*>(nullptr), 0.0f, 0));
   K keys[kEach];
 #pragma unroll
@@ -228,7 +233,7 @@ struct Found {
   int count;
 };
 template <typename T, int kEach>
-RLENV_D void few_best_of_warp(const Scores& p, int64_t row, const float (&x)[kEach], float normalizer, Found& found) {
+RLENV_D void few_best_of_warp(const Scores& p, int64_t row, const float (&x)[kEach], const Normalizer& normalizer, Found& found) {
   const int lane = threadIdx.x % 32, left = int(p.v) - lane;
   float most = x[0];
 #pragma unroll
@@ -347,7 +352,7 @@ __global__ void __launch_bounds__(256) few_scores_kernel(const __grid_constant__
   for (int d = kLanes / 2; d > 0; d /= 2) both = add_pairs(both, __shfl_xor_sync(0xffffffffu, both, d));
   const float2 of = values_of(both);
   sums.s = of.x, sums.w = of.y;
-  const float normalizer = normalizer_of(sums);
+  const Normalizer normalizer(sums);
   if (sub == 0 && at < p.m) write_scores(p, row, sums, normalizer, chosen);
   if constexpr (kLanes == 32) {
     __shared__ Found found[8];
@@ -782,7 +787,7 @@ scores_kernel(const __grid_constant__ Scores p) {
     best.keep(p.top);
   }
   if constexpr (kWarps == 1) {
-    const float normalizer = normalizer_of(sums);
+    const Normalizer normalizer(sums);
     if (lane == 0) write_scores(p, row, sums, normalizer, chosen);
     if (lane < p.top) write_top(p, row, lane, best.kept[lane], normalizer);
     return;
@@ -806,7 +811,7 @@ scores_kernel(const __grid_constant__ Scores p) {
   if (threadIdx.x < kMostTop) top_of_block[threadIdx.x] = 0;
   __syncthreads();  // the rings are free
   sums = of_team<kWarps>(of_warps[lane % kWarps]);
-  const float normalizer = normalizer_of(sums);
+  const Normalizer normalizer(sums);
   if (blocks == 1 && threadIdx.x == 0) write_scores(p, row, sums, normalizer, chosen);
   if (p.top > 0) {
     if (lane < p.top) lists[warp * p.top + lane] = lane < best.count ? best.kept[lane] : 0;
@@ -824,7 +829,7 @@ scores_kernel(const __grid_constant__ Scores p) {
   cluster.sync();
   if (rank == 0) {
     sums = of_team<8>(lane % 8 < blocks ? *cluster.map_shared_rank(&of_block, lane % 8) : Sums{-infinity(), 0.0f, 0.0f});
-    const float normalizer = normalizer_of(sums);
+    const Normalizer normalizer(sums);
     if (threadIdx.x == 0) write_scores(p, row, sums, normalizer, chosen);
     if (p.top > 0) {
       for (int i = threadIdx.x; i < 8 * kMostTop; i += kStride)

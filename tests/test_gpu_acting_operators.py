@@ -621,6 +621,41 @@ def test_scores_of_rows_that_grow(cuda, v, dtype):
     assert np.array_equal(got.top_actions.cpu().numpy(), policy.best(l64, 5))
 
 
+FAR = [("f32", 1024.0, 0.125), ("f32", 2.0 ** 17, 0.125), ("f32", 2.0 ** 24, 2.0), ("f32", -2.0 ** 24, 2.0),
+       ("bf16", 1024.0, 8.0), ("bf16", -2.0 ** 17, 1024.0), ("bf16", 2.0 ** 24, 2.0 ** 17), ("f32", None, 0.0), ("bf16", None, 0.0)]
+
+
+def far_logits(cuda, m, v, dtype, shift, unit, seed=0):
+    """(logits that have `shift` in common, the same without it): whole units, exact in the type. None: its lowest value."""
+    g = torch.Generator(device=cuda).manual_seed(seed)
+    near = torch.randint(-20, 1, (m, v), generator=g, device=cuda).float() * unit
+    near[:, v // 2] = 0.0
+    far = (near + (torch.finfo(TYPES[dtype]).min if shift is None else shift)).to(TYPES[dtype])
+    assert shift is None or torch.equal(far.double() - shift, near.double())
+    return far, near
+
+
+@pytest.mark.parametrize("dtype,shift,unit", FAR)
+@pytest.mark.parametrize("m,v", [(9, 7), (9, 31), (5, 60), (8300, 60), (4, 250), (3, 700), (5, 1500), (700, 3000), (2, 30_000), (1, 140_000)])
+def test_scores_of_rows_far_from_zero(cuda, m, v, dtype, shift, unit):
+    """What a row's logits have in common changes neither its log-probabilities nor its entropy, nor how precise they are:
+    the bounds are those of the rows without it."""
+    import log_probs
+
+    far, near = far_logits(cuda, m, v, dtype, shift, unit)
+    actions = torch.arange(m, device=cuda) % v
+    got = log_probs.forward(far, actions, None, min(v, 4))
+    l64, some = to64(near[:50]), slice(0, 50)
+    lp, h, z, every = policy.scores(l64, to64(actions[:50]).astype(np.int64))
+    z_off, h_off = score_bounds(l64, None, v)
+    close(got.log_prob[some], lp, z_off + HALF * abs(lp) + 2 ** -23, "log_prob")
+    close(got.entropy[some], h, h_off, "entropy")
+    want = np.take_along_axis(every, policy.best(l64, min(v, 4)), -1)
+    close(got.top_log_probs[some], want, z_off[:, None] + HALF * abs(want) + 2 ** -23, "top_log_probs")
+    z = z + (torch.finfo(TYPES[dtype]).min if shift is None else shift)
+    close(got.normalizer[some], z, z_off + 2 * HALF * abs(z), "normalizer")
+
+
 def grad_tol(g, h, l, actions, allowed, dtype):
     lp, entropy, z, every = policy.scores(l, actions, allowed)
     z_off, h_off = score_bounds(l, allowed, l.shape[1])
