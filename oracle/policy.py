@@ -125,10 +125,11 @@ def scores(l, actions, allowed=None):
 def scores_grad(g, h, l, actions, allowed=None):
     """The gradient of sum(g * log_prob) + sum(h * entropy)."""
     _, entropy, _, lp = scores(l, actions, allowed)
-    p, lp = np.exp(lp), np.where(lp == -np.inf, 0.0, lp)
+    some = lp > -np.inf  # not p > 0: the chosen action has a gradient where its p is below 64 bits' numbers too
+    p, lp = np.exp(lp), np.where(some, lp, 0.0)
     chosen = np.arange(l.shape[-1]) == actions[..., None]
     grad = np.where(actions < 0, 0.0, g)[..., None] * (chosen - p) - h[..., None] * p * (lp + entropy[..., None])
-    return np.where(p > 0, grad, 0.0)
+    return np.where(some, grad, 0.0)
 
 
 def best(l, n, allowed=None):

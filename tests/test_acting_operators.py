@@ -55,6 +55,13 @@ def test_scores_gradient_is_the_derivative():
     assert (grad[5] == 0).all() and (grad[~allowed] == 0).all()
 
 
+def test_scores_gradient_of_an_action_that_is_all_but_impossible():
+    """Its own gradient is g (1 - p), also where p is no number of 64 bits any more."""
+    l = np.array([[0.0, -2000.0, -np.inf]])
+    for action, want in ((0, [0, 0, 0]), (1, [-1.5, 1.5, 0]), (2, [-1.5, 0, 0])):
+        assert policy.scores_grad(np.array([1.5]), np.array([0.3]), l, np.array([action])).tolist() == [want]
+
+
 def test_scores_of_known_distributions():
     lp, entropy, normalizer, _ = policy.scores(np.zeros((2, 8)), np.array([3, -1]))
     np.testing.assert_allclose(entropy, np.log(8))
