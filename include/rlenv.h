@@ -497,16 +497,34 @@ RLENV_API int rlenv_log_probs_forward(int dtype, int64_t m, int64_t v, const voi
                                       int64_t allowed_stride, float* log_prob, float* entropy, float* normalizer,
                                       int top, int64_t* top_actions, float* top_log_probs, void* stream);
 
+/* The same, with what the normalizer's rounding to a float32 has left: remainder (m) float32 (NULL: not
+ * wanted), so that normalizer + remainder is log sum exp(l) to the precision of log sum exp(l - max l);
+ * 0 where the normalizer is not finite. */
+RLENV_API int rlenv_log_probs_forward_remainder(int dtype, int64_t m, int64_t v, const void* logits, int64_t stride,
+                                                const void* actions, int action_dtype, const uint8_t* allowed,
+                                                int64_t allowed_stride, float* log_prob, float* entropy,
+                                                float* normalizer, float* remainder, int top, int64_t* top_actions,
+                                                float* top_log_probs, void* stream);
+
 /* Their gradient: grad (m, v) of dtype, dense, from grad_log_prob (m) and grad_entropy (m) (either may be
  * NULL for zero), the forward pass's normalizer and entropy:
  *     grad_j = grad_log_prob ([j = action] - p_j) - grad_entropy p_j (log p_j + entropy),
  * zero where an action is not allowed or its logit is -infinity, and in rows that allow nothing. Rows
- * with a negative action have no first term; with one of v or above they are NaN. */
+ * with a negative action have no first term; with one of v or above they are NaN. p is formed from the
+ * normalizer alone: of rows far from zero all of it is off by a factor of up to e^(2^-24 |normalizer|). */
 RLENV_API int rlenv_log_probs_backward(int dtype, int64_t m, int64_t v, const float* grad_log_prob,
                                        const float* grad_entropy, const void* logits, int64_t stride,
                                        const void* actions, int action_dtype, const float* normalizer,
                                        const float* entropy, const uint8_t* allowed, int64_t allowed_stride,
                                        void* grad, void* stream);
+
+/* The same from the normalizer and its remainder (m), as rlenv_log_probs_forward_remainder leaves it (NULL:
+ * zero): rows far from zero are as precise as others. */
+RLENV_API int rlenv_log_probs_backward_remainder(int dtype, int64_t m, int64_t v, const float* grad_log_prob,
+                                                 const float* grad_entropy, const void* logits, int64_t stride,
+                                                 const void* actions, int action_dtype, const float* normalizer,
+                                                 const float* remainder, const float* entropy, const uint8_t* allowed,
+                                                 int64_t allowed_stride, void* grad, void* stream);
 
 #ifdef __cplusplus
 }

@@ -2,7 +2,8 @@
 // their gradient. With the largest logit b of a row (of those allowed; others count as -infinity),
 //     S = sum e^(l - b),   W = sum e^(l - b) (l - b),   normalizer = b + log S,   entropy = log S - W / S,
 // and sums over parts of a row join: (b, S, W) moves to a larger b' by d = b - b': (e^d S, e^d (W + S d)).
-// The gradient: g ([j = action] - p_j) - h p_j (log p_j + entropy), p_j = e^(l_j - normalizer).
+// The gradient: g ([j = action] - p_j) - h p_j (log p_j + entropy), p_j = e^(l_j - normalizer), the normalizer with what its
+// rounding to a float32 has left (`remainder`): for b far from zero that is as large as log S.
 //
 // A row is read once: any number will do for b that is not far below the largest logit, so that sums begin with the first
 // vectors and nothing waits for a largest one. The bound is memory, with the power unit close behind (a logit is one
@@ -47,6 +48,7 @@ struct Scores {
   int top;
   int64_t* top_actions;
   float* top_log_probs;
+  float* remainder;  // of the normalizer; may be null
 };
 
 RLENV_D int64_t action_of(const void* actions, int dtype, int64_t row) {
@@ -126,6 +128,10 @@ struct Normalizer {
   float base, log_sum;
   RLENV_D explicit Normalizer(const Sums& a) : base(base_of(a.m)), log_sum(logf(a.s)) {}
   RLENV_D float whole() const { return base + log_sum; }
+  RLENV_D float remainder() const {  // exactly what whole() leaves (Knuth's two-sum)
+    const float n = whole(), b = n - base;
+    return fabsf(n) < infinity() ? (base - (n - b)) + (log_sum - b) : 0.0f;
+  }
   RLENV_D float log_prob(float l) const {  // -infinity of a row that allows nothing too
     return l == -infinity() && log_sum == -infinity() ? l : (l - base) - log_sum;
   }
@@ -144,6 +150,7 @@ struct Chosen {
 
 RLENV_D void write_scores(const Scores& p, int64_t row, const Sums& sums, const Normalizer& normalizer, const Chosen& chosen) {
   p.normalizer[row] = normalizer.whole();
+  if (p.remainder) p.remainder[row] = normalizer.remainder();
   p.entropy[row] = sums.s == 0.0f ? 0.0f : normalizer.log_sum - sums.w / sums.s;
   check_flag(chosen.action >= p.v, kCheckActionRange);
   p.log_prob[row] = chosen.action < 0 ? 0.0f : chosen.action >= p.v ? not_a_number() : normalizer.log_prob(chosen.l);
@@ -854,10 +861,11 @@ struct ScoresGrad {
   const uint8_t* allowed;
   int64_t allowed_stride;
   void* grad;
+  const float* remainder;  // null: zero
 };
 
-// What a row's gradients have in common. With y = log2 p the gradient of what was not chosen is
-// - p (g + h entropy + h ln 2 y): two values an instruction but for the power.
+// What a row's gradients have in common. With y = (l - normalizer) log2 e and the normalizer's remainder r, p = e^-r 2^y and the
+// gradient of what was not chosen is - 2^y e^-r (g + h (entropy - r) + h ln 2 y): two values an instruction but for the power.
 struct RowGrad {
   int action;  // negative: none whose gradient differs
   float g;
@@ -871,9 +879,12 @@ struct RowGrad {
     const float h = p.grad_entropy ? __ldg(p.grad_entropy + row) : 0.0f;
     g = p.grad_log_prob && action >= 0 ? __ldg(p.grad_log_prob + row) : 0.0f;
     if (action >= p.v) g = not_a_number();
+    float rest = 0.0f, scale = 1.0f;
+    if (p.remainder) rest = __ldg(p.remainder + row), scale = expf(-rest);
     const bool none = normalizer == -infinity();
     if (none) action = -1;
-    const float base = none ? 0.0f : normalizer, of_p = none ? 0.0f : -(g + h * entropy), of_y = none ? 0.0f : -h * kLn2;
+    const float base = none ? 0.0f : normalizer, of_p = none ? 0.0f : -scale * (g + h * (entropy - rest)),
+                of_y = none ? 0.0f : -scale * h * kLn2;
     minus_base = pair_of(-base, -base), a = pair_of(of_p, of_p), b = pair_of(of_y, of_y);
   }
   RLENV_D float2 without_choice(uint64_t l) const {
@@ -1130,6 +1141,14 @@ int rlenv_log_probs_forward(int dtype, int64_t m, int64_t v, const void* logits,
                             int action_dtype, const uint8_t* allowed, int64_t allowed_stride, float* log_prob,
                             float* entropy, float* normalizer, int top, int64_t* top_actions, float* top_log_probs,
                             void* stream) {
+  return rlenv_log_probs_forward_remainder(dtype, m, v, logits, stride, actions, action_dtype, allowed, allowed_stride, log_prob,
+                                           entropy, normalizer, nullptr, top, top_actions, top_log_probs, stream);
+}
+
+int rlenv_log_probs_forward_remainder(int dtype, int64_t m, int64_t v, const void* logits, int64_t stride, const void* actions,
+                                      int action_dtype, const uint8_t* allowed, int64_t allowed_stride, float* log_prob,
+                                      float* entropy, float* normalizer, float* remainder, int top, int64_t* top_actions,
+                                      float* top_log_probs, void* stream) {
   using namespace rlenv;
   if (!scores_sizes(dtype, m, v, stride, action_dtype, allowed_stride) || top < 0 || top > kMostTop || top > v)
     return RLENV_EINVAL;
@@ -1137,11 +1156,11 @@ int rlenv_log_probs_forward(int dtype, int64_t m, int64_t v, const void* logits,
   if (!logits || !actions || !log_prob || !entropy || !normalizer || (top > 0 && (!top_actions || !top_log_probs)))
     return RLENV_EINVAL;
   if (!at_multiple(logits, dtype == RLENV_F32 ? 4 : 2) || !at_multiple(actions, action_size(action_dtype)) ||
-      !at_multiple(log_prob, 4) || !at_multiple(entropy, 4) || !at_multiple(normalizer, 4) || !at_multiple(top_actions, 8) ||
-      !at_multiple(top_log_probs, 4))
+      !at_multiple(log_prob, 4) || !at_multiple(entropy, 4) || !at_multiple(normalizer, 4) || !at_multiple(remainder, 4) ||
+      !at_multiple(top_actions, 8) || !at_multiple(top_log_probs, 4))
     return RLENV_EINVAL;
   const Scores p{m, v, logits, stride, actions, action_dtype, allowed, allowed_stride, log_prob, entropy, normalizer,
-                 top, top_actions, top_log_probs};
+                 top, top_actions, top_log_probs, remainder};
   return dtype == RLENV_F32 ? scores_of<float>(p, as_stream(stream)) : scores_of<__nv_bfloat16>(p, as_stream(stream));
 }
 
@@ -1149,16 +1168,24 @@ int rlenv_log_probs_backward(int dtype, int64_t m, int64_t v, const float* grad_
                              const void* logits, int64_t stride, const void* actions, int action_dtype,
                              const float* normalizer, const float* entropy, const uint8_t* allowed, int64_t allowed_stride,
                              void* grad, void* stream) {
+  return rlenv_log_probs_backward_remainder(dtype, m, v, grad_log_prob, grad_entropy, logits, stride, actions, action_dtype,
+                                            normalizer, nullptr, entropy, allowed, allowed_stride, grad, stream);
+}
+
+int rlenv_log_probs_backward_remainder(int dtype, int64_t m, int64_t v, const float* grad_log_prob, const float* grad_entropy,
+                                       const void* logits, int64_t stride, const void* actions, int action_dtype,
+                                       const float* normalizer, const float* remainder, const float* entropy,
+                                       const uint8_t* allowed, int64_t allowed_stride, void* grad, void* stream) {
   using namespace rlenv;
   if (!scores_sizes(dtype, m, v, stride, action_dtype, allowed_stride)) return RLENV_EINVAL;
   if (m == 0) return RLENV_OK;
   const int size = dtype == RLENV_F32 ? 4 : 2;
   if (!logits || !actions || !normalizer || !entropy || !grad || !at_multiple(logits, size) || !at_multiple(grad, size) ||
       !at_multiple(actions, action_size(action_dtype)) || !at_multiple(normalizer, 4) || !at_multiple(entropy, 4) ||
-      !at_multiple(grad_log_prob, 4) || !at_multiple(grad_entropy, 4))
+      !at_multiple(grad_log_prob, 4) || !at_multiple(grad_entropy, 4) || !at_multiple(remainder, 4))
     return RLENV_EINVAL;
   const ScoresGrad p{m, v, grad_log_prob, grad_entropy, logits, stride, actions, action_dtype, normalizer, entropy, allowed,
-                     allowed_stride, grad};
+                     allowed_stride, grad, remainder};
   return dtype == RLENV_F32 ? scores_grad_of<float>(p, as_stream(stream))
                             : scores_grad_of<__nv_bfloat16>(p, as_stream(stream));
 }

@@ -26,14 +26,19 @@ import rlenv_lib as _rl
 MOST_ALTERNATIVES = 32
 
 
-class Scores(NamedTuple):
-    """Of logits (..., A): log_prob, entropy and normalizer (...) float32; of the alternatives asked for, best first
-    (ties: the lower action), top_log_probs (..., n) float32 and top_actions (..., n) int64, None without."""
+class _Scores(NamedTuple):
     log_prob: torch.Tensor
     entropy: torch.Tensor
     normalizer: torch.Tensor
     top_log_probs: torch.Tensor | None = None
     top_actions: torch.Tensor | None = None
+
+
+class Scores(_Scores):
+    """Of logits (..., A): log_prob, entropy and normalizer (...) float32; of the alternatives asked for, best first
+    (ties: the lower action), top_log_probs (..., n) float32 and top_actions (..., n) int64, None without. `remainder`
+    (...) float32, no item of the tuple, is what the normalizer's rounding has left, None unless asked for."""
+    remainder = None
 
 
 def _check(logits, actions, allowed):
@@ -56,8 +61,9 @@ def _check(logits, actions, allowed):
 _ACTIONS = {torch.int64: _rl.I64, torch.int32: _rl.I32, torch.uint8: _rl.U8}
 
 
-def forward(logits, actions, allowed=None, alternatives=0):
-    """Scores of the actions, and of the `alternatives` (up to 32) best ones."""
+def forward(logits, actions, allowed=None, alternatives=0, remainder=False):
+    """Scores of the actions, and of the `alternatives` (up to 32) best ones; with `remainder`, the normalizer's, for
+    `backward`."""
     m, v, code, action_code, index = _check(logits, actions, allowed)
     if not 0 <= alternatives <= min(v, MOST_ALTERNATIVES):
         raise ValueError(f"alternatives must be from 0 to {min(v, MOST_ALTERNATIVES)}; got {alternatives}")
@@ -69,55 +75,59 @@ def forward(logits, actions, allowed=None, alternatives=0):
     actions = actions.contiguous()
     log_prob = _rl.empty_lead(logits, torch.float32)
     entropy, normalizer = torch.empty_like(log_prob), torch.empty_like(log_prob)
-    if not alternatives:
-        _rl.launch(index, _rl.lib().log_probs_forward, code, m, v, logits.data_ptr(), stride, actions.data_ptr(), action_code,
-                   allowed_at, allowed_stride, log_prob.data_ptr(), entropy.data_ptr(), normalizer.data_ptr(), 0, 0, 0)
-        return Scores(log_prob, entropy, normalizer)
-    top, best = _rl.empty_rows(logits, alternatives, torch.float32), _rl.empty_rows(logits, alternatives, torch.int64)
-    _rl.launch(index, _rl.lib().log_probs_forward, code, m, v, logits.data_ptr(), stride, actions.data_ptr(), action_code,
-               allowed_at, allowed_stride, log_prob.data_ptr(), entropy.data_ptr(), normalizer.data_ptr(), alternatives,
-               best.data_ptr(), top.data_ptr())
-    return Scores(log_prob, entropy, normalizer, top, best)
+    rest = torch.empty_like(log_prob) if remainder else None
+    top = best = None
+    if alternatives:
+        top, best = _rl.empty_rows(logits, alternatives, torch.float32), _rl.empty_rows(logits, alternatives, torch.int64)
+    _rl.launch(index, _rl.lib().log_probs_forward_remainder, code, m, v, logits.data_ptr(), stride, actions.data_ptr(),
+               action_code, allowed_at, allowed_stride, log_prob.data_ptr(), entropy.data_ptr(), normalizer.data_ptr(),
+               _rl.ptr(rest), alternatives, _rl.ptr(best), _rl.ptr(top))
+    scores = Scores(log_prob, entropy, normalizer, top, best)
+    if remainder:
+        scores.remainder = rest
+    return scores
 
 
-def backward(grad_log_prob, grad_entropy, logits, actions, normalizer, entropy, allowed=None):
+def backward(grad_log_prob, grad_entropy, logits, actions, normalizer, entropy, allowed=None, remainder=None):
     """The gradient (..., A) of the logits from those of log_prob and entropy (either may be None), with `forward`'s
-    normalizer and entropy."""
+    normalizer and entropy. With its remainder a token whose logits lie far from zero has as precise a gradient as
+    another; without, its probabilities are off by a factor of up to e^(2^-24 |normalizer|)."""
     m, v, code, action_code, index = _check(logits, actions, allowed)
     lead = logits.shape[:-1]
     rows = []
     for name, x in (("grad_log_prob", grad_log_prob), ("grad_entropy", grad_entropy), ("normalizer", normalizer),
-                    ("entropy", entropy)):
-        if x is None and name.startswith("grad"):
+                    ("entropy", entropy), ("remainder", remainder)):
+        if x is None and name not in ("normalizer", "entropy"):
             rows.append(None)
             continue
         if not isinstance(x, torch.Tensor) or x.get_device() != index or x.dtype is not torch.float32 or x.shape != lead:
             _rl.as_floats(name, x, lead, torch.float32)
             _rl.one_device(index, **{name: x})
         rows.append(x.contiguous())
-    grad_log_prob, grad_entropy, normalizer, entropy = rows
+    grad_log_prob, grad_entropy, normalizer, entropy, remainder = rows
     logits, stride = _rl.as_rows(logits)
     allowed, allowed_stride = (None, 0) if allowed is None else _rl.as_rows(allowed)
     actions, grad = actions.contiguous(), _rl.empty_rows(logits, v, logits.dtype)
-    _rl.launch(index, _rl.lib().log_probs_backward, code, m, v, _rl.ptr(grad_log_prob), _rl.ptr(grad_entropy),
-               logits.data_ptr(), stride, actions.data_ptr(), action_code, normalizer.data_ptr(), entropy.data_ptr(),
-               _rl.ptr(allowed), allowed_stride, grad.data_ptr())
+    _rl.launch(index, _rl.lib().log_probs_backward_remainder, code, m, v, _rl.ptr(grad_log_prob), _rl.ptr(grad_entropy),
+               logits.data_ptr(), stride, actions.data_ptr(), action_code, normalizer.data_ptr(), _rl.ptr(remainder),
+               entropy.data_ptr(), _rl.ptr(allowed), allowed_stride, grad.data_ptr())
     return grad
 
 
 class _Apply(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, actions, allowed):
-        scores = forward(logits, actions, allowed)
-        ctx.save_for_backward(logits, actions, allowed, scores.normalizer, scores.entropy)
+        scores = forward(logits, actions, allowed, remainder=True)
+        ctx.save_for_backward(logits, actions, allowed, scores.normalizer, scores.entropy, scores.remainder)
         ctx.set_materialize_grads(False)
         return scores.log_prob, scores.entropy
 
     @staticmethod
     @once_differentiable
     def backward(ctx, grad_log_prob, grad_entropy):
-        logits, actions, allowed, normalizer, entropy = ctx.saved_tensors
-        return backward(grad_log_prob, grad_entropy, logits, actions, normalizer, entropy, allowed), None, None
+        logits, actions, allowed, normalizer, entropy, remainder = ctx.saved_tensors
+        grad = backward(grad_log_prob, grad_entropy, logits, actions, normalizer, entropy, allowed, remainder)
+        return grad, None, None
 
 
 def apply(logits, actions, allowed=None):

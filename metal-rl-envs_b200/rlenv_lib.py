@@ -109,8 +109,12 @@ _SIGNATURES = {
     "rlenv_int8_linear_status": [c_void_p, c_int],
     "rlenv_log_probs_forward": [c_int, c_int64, c_int64, c_void_p, c_int64, c_void_p, c_int, c_void_p, c_int64,
                                 c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_void_p],
+    "rlenv_log_probs_forward_remainder": [c_int, c_int64, c_int64, c_void_p, c_int64, c_void_p, c_int, c_void_p, c_int64,
+                                          c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_void_p],
     "rlenv_log_probs_backward": [c_int, c_int64, c_int64, c_void_p, c_void_p, c_void_p, c_int64, c_void_p, c_int,
                                  c_void_p, c_void_p, c_void_p, c_int64, c_void_p, c_void_p],
+    "rlenv_log_probs_backward_remainder": [c_int, c_int64, c_int64, c_void_p, c_void_p, c_void_p, c_int64, c_void_p, c_int,
+                                           c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_void_p, c_void_p],
     "rlenv_reset_uniform": [c_void_p, c_int, c_int64, c_void_p, c_float, c_uint32, c_int64, c_void_p],
 }
 

@@ -175,6 +175,23 @@ def test_scores_arguments_rejected_before_launch():
     assert bwd(g=ODD) == -1 and bwd(h=ODD) == -1 and bwd(m=0) == 0
 
 
+def test_scores_with_a_remainder_rejected_before_launch():
+    import rlenv_lib
+
+    lib = rlenv_lib.load()
+    f32, i64 = rlenv_lib.F32, rlenv_lib.I64
+
+    def fwd(rest=FAKE, l=FAKE, m=4, z=FAKE):
+        return lib.log_probs_forward_remainder(f32, m, 8, l, 8, FAKE, i64, None, 0, FAKE, FAKE, z, rest, 0, None, None, None)
+
+    def bwd(rest=FAKE, l=FAKE, m=4, z=FAKE):
+        return lib.log_probs_backward_remainder(f32, m, 8, FAKE, FAKE, l, 8, FAKE, i64, z, rest, FAKE, None, 0, FAKE, None)
+
+    for call in (fwd, bwd):
+        assert call(rest=ODD) == -1 and call(l=None) == -1 and call(z=None) == -1 and call(m=-1) == -1
+        assert call(m=0) == 0 and call(m=0, rest=None) == 0
+
+
 def test_wrappers_refuse_what_is_no_cuda_tensor():
     import int8_linear
     import log_probs

@@ -694,6 +694,48 @@ def test_scores_gradient(cuda, m, v, dtype):
             assert grad.dtype == l.dtype and grad.is_contiguous()
 
 
+@pytest.mark.parametrize("dtype,shift,unit", FAR)
+@pytest.mark.parametrize("m,v", [(9, 7), (5, 60), (8300, 60), (4, 250), (3, 700), (5, 1500), (2, 30_001), (1, 140_000)])
+def test_scores_gradient_of_rows_far_from_zero(cuda, m, v, dtype, shift, unit):
+    """The gradient of rows that have much in common is that of the rows without it, in its precision too, by the
+    remainder of the normalizer's rounding: rows that lie as the gradient's do on the boundaries and others."""
+    import log_probs
+
+    far, near = far_logits(cuda, m, v + 1, dtype, shift, unit)
+    actions = torch.arange(m, device=cuda) % v
+    actions[m // 2] = -1
+    g, h = normal(cuda, m, seed=5), normal(cuda, m, seed=6)
+    n = min(m, 50)
+    want, tol = grad_tol(to64(g[:n]), to64(h[:n]), to64(near[:n, :v]), to64(actions[:n]).astype(np.int64), None, dtype)
+    for l in (far[:, :v], far[:, :v].contiguous()):
+        s = log_probs.forward(l, actions, remainder=True)
+        z = policy.scores(to64(near[:n, :v]), np.zeros(n, np.int64))[2]
+        left = (to64(s.normalizer[:n]) - (torch.finfo(TYPES[dtype]).min if shift is None else shift)) + to64(s.remainder[:n])
+        assert (abs(left - z) <= score_bounds(to64(near[:n, :v]), None, v)[0]).all()
+        grad = log_probs.backward(g, h, l, actions, s.normalizer, s.entropy, None, s.remainder)
+        close(grad[:n], want, tol, "grad")
+        leaf = l.detach().clone().requires_grad_()
+        both = torch.autograd.grad(log_probs.apply(leaf, actions), leaf, (g, h))[0]
+        close(both[:n], want, tol, "apply's gradient")
+
+
+def test_a_normalizers_remainder(cuda):
+    """It is asked for, is no item of the tuple, and is 0 where the normalizer is not finite; what does not fit is refused."""
+    import log_probs
+
+    l, a = normal(cuda, 6, 5), torch.zeros(6, dtype=torch.int64, device=cuda)
+    l[1], l[2, 0], l[3, 1] = -torch.inf, torch.nan, torch.inf
+    s = log_probs.forward(l, a)
+    assert s.remainder is None and len(s) == 5
+    s = log_probs.forward(l, a, None, 2, remainder=True)
+    log_prob, entropy, normalizer, top, best = s
+    assert s.remainder.shape == (6,) and not s.remainder[1:4].any() and s.remainder[[0, 4, 5]].abs().max() <= HALF * 8
+    assert not log_probs.backward(log_prob, entropy, l, a, normalizer, entropy, None, s.remainder)[1].any()
+    for bad in (s.remainder[:5], s.remainder.double(), s.remainder.cpu(), 0.0):
+        with pytest.raises(ValueError):
+            log_probs.backward(log_prob, None, l, a, normalizer, entropy, None, bad)
+
+
 @pytest.mark.parametrize("kind", [torch.int64, torch.int32, torch.uint8])
 def test_scores_through_autograd(cuda, kind):
     """The loss of an actor: log_prob and entropy, their gradient against the oracle's; leading axes, a slice."""
