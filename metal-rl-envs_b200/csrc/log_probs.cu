@@ -585,10 +585,12 @@ RLENV_D uint32_t nth_largest(uint32_t (&v)[4], int n) {
 
 // kWarps warps read a row in turns of kSteps vectors a lane, and a cluster's blocks a part of it each: no lane waits for
 // another before the row's end. Each lane's next turns are on their way into its own places of shared memory meanwhile. A
-// lane's sums stand against a base of its own, which moves only where a logit is so far above that powers would grow too
-// large.
+// lane's sums stand against a base of its own, which moves only where a logit is kAbove above it. log S and W / S have what the
+// base lies below the largest logit in common and are rounded with it, so that it stays small: at 20 the entropy of rows whose
+// largest logit comes late is off by up to 8e-6, at 3 by 4e-7, as rows that take the largest first (4,096 x 32,768 bf16 of
+// deviation 2, 48.7 us at 20, 49.2 at 3).
 constexpr int kSteps = 4, kAhead = 3;  // kAhead: turns in shared memory, the one at work among them
-constexpr float kAbove = 20.0f;
+constexpr float kAbove = 3.0f;
 template <int kWarps>
 struct Team {
   static constexpr int kThreads = kWarps == 1 ? 128 : 32 * kWarps, kRows = kThreads / (32 * kWarps);
@@ -696,8 +698,9 @@ scores_kernel(const __grid_constant__ Scores p) {
     for (int u = 1; u < kSteps; ++u) all = larger_words<T>(all, largest_word(w[u]));
     const float most = largest_of<T>(all);
     if (most > base + kAbove) {
-      const Sums now = moved(own_sums(), most);
-      base = most, s2 = pair_of(now.s, 0.0f), w2 = pair_of(now.w * kLog2E, 0.0f);
+      const float d = larger(base - most, kFar) * kLog2E, e = exp2_fast(d);
+      w2 = multiply_pairs(pair_of(e, e), multiply_add_pairs(s2, pair_of(d, d), w2)), s2 = multiply_pairs(pair_of(e, e), s2);
+      base = most;
     }
     const float against = base_of(base);
     const uint64_t minus_base = pair_of(-against, -against);

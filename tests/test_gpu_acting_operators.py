@@ -621,6 +621,27 @@ def test_scores_of_rows_that_grow(cuda, v, dtype):
     assert np.array_equal(got.top_actions.cpu().numpy(), policy.best(l64, 5))
 
 
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("m,v", [(64, 60), (64, 1000), (64, 1500), (700, 3000), (3000, 9000), (64, 16_384), (400, 20_000), (2, 60_000), (1, 140_000)])
+def test_the_entropy_of_rows_whose_largest_logit_is_the_last(cuda, m, v, dtype):
+    """A policy that has learnt what to do: one logit 17 to 21 above ones of order one, so that the entropy is 1e-2 to 1e-5
+    and the sum S is the one term. Against a base that lies close to it S is 1 and what a bit more, and so are the numbers that
+    are rounded: once where the last logit is added, once for its lane, at most five times among lanes, four among warps and three
+    among blocks. The others' part of S, and of the entropy, has its usual error in proportion to it."""
+    import log_probs
+
+    l = normal(cuda, m, v, seed=9).clamp(-4, 4)
+    l[:, -1] = torch.linspace(17, 21, m, device=cuda)
+    l = l.to(TYPES[dtype])
+    got = log_probs.forward(l, torch.full((m,), v - 1, device=cuda))
+    l64 = to64(l)
+    lp, h, z, every = policy.scores(l64, np.full(m, v - 1))
+    others = 1 - np.exp(lp)
+    tol = 15 * HALF + others * (chain(v) + 20) * 26 * 2 ** -23  # 26: the others lie up to 25 below
+    close(got.entropy, h, tol, "entropy")
+    close(got.log_prob, lp, tol, "log_prob")
+
+
 FAR = [("f32", 1024.0, 0.125), ("f32", 2.0 ** 17, 0.125), ("f32", 2.0 ** 24, 2.0), ("f32", -2.0 ** 24, 2.0),
        ("bf16", 1024.0, 8.0), ("bf16", -2.0 ** 17, 1024.0), ("bf16", 2.0 ** 24, 2.0 ** 17), ("f32", None, 0.0), ("bf16", None, 0.0)]
 
