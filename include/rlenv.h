@@ -491,7 +491,7 @@ RLENV_API int rlenv_int8_linear_status(unsigned int* gave_up, int clear);
  * not allowed counts as a logit of -infinity; what is in its place is not looked at. Rows that
  * allow nothing: normalizer and log-probabilities -infinity, entropy 0. Rows with a NaN or
  * +infinity among the logits allowed: NaN, a NaN counting as the largest among top_actions. top
- * <= v. */
+ * <= v. A call takes fewer than 2^26 rows and 2^40 logits, v up to 2^31 - 64, and so do those below. */
 RLENV_API int rlenv_log_probs_forward(int dtype, int64_t m, int64_t v, const void* logits, int64_t stride,
                                       const void* actions, int action_dtype, const uint8_t* allowed,
                                       int64_t allowed_stride, float* log_prob, float* entropy, float* normalizer,

@@ -58,6 +58,22 @@ def _check(logits, actions, allowed):
     return shape[:-1].numel(), shape[-1], _rl.FLOAT_DTYPES[logits.dtype], _ACTIONS[actions.dtype], index
 
 
+_MANY, _MANY_LOGITS = 1 << 26, 1 << 40  # rows and logits that the library no longer takes in one launch
+
+
+def _launches(m, v):
+    """(first row, rows) of each launch that a call of m rows of v takes."""
+    most = min(_MANY - 16, (_MANY_LOGITS - 1) // v & ~15)
+    return ((0, m),) if m <= most else tuple((at, min(most, m - at)) for at in range(0, m, most))
+
+
+def _in_launches(index, entry, code, m, v, args, rows):
+    """entry(code, m, v, *args) in several launches; rows: of each argument the bytes from row to row, 0 where it is no
+    address of rows."""
+    for at, n in _launches(m, v):
+        _rl.launch(index, entry, code, n, v, *(x + at * step if x else x for x, step in zip(args, rows)))
+
+
 _ACTIONS = {torch.int64: _rl.I64, torch.int32: _rl.I32, torch.uint8: _rl.U8}
 
 
@@ -68,10 +84,7 @@ def forward(logits, actions, allowed=None, alternatives=0, remainder=False):
     if not 0 <= alternatives <= min(v, MOST_ALTERNATIVES):
         raise ValueError(f"alternatives must be from 0 to {min(v, MOST_ALTERNATIVES)}; got {alternatives}")
     logits, stride = _rl.as_rows(logits)
-    allowed_at = allowed_stride = 0
-    if allowed is not None:
-        allowed, allowed_stride = _rl.as_rows(allowed)
-        allowed_at = allowed.data_ptr()
+    allowed, allowed_stride = (None, 0) if allowed is None else _rl.as_rows(allowed)
     actions = actions.contiguous()
     log_prob = _rl.empty_lead(logits, torch.float32)
     entropy, normalizer = torch.empty_like(log_prob), torch.empty_like(log_prob)
@@ -79,9 +92,15 @@ def forward(logits, actions, allowed=None, alternatives=0, remainder=False):
     top = best = None
     if alternatives:
         top, best = _rl.empty_rows(logits, alternatives, torch.float32), _rl.empty_rows(logits, alternatives, torch.int64)
-    _rl.launch(index, _rl.lib().log_probs_forward_remainder, code, m, v, logits.data_ptr(), stride, actions.data_ptr(),
-               action_code, allowed_at, allowed_stride, log_prob.data_ptr(), entropy.data_ptr(), normalizer.data_ptr(),
-               _rl.ptr(rest), alternatives, _rl.ptr(best), _rl.ptr(top))
+    entry = _rl.lib().log_probs_forward_remainder
+    args = (logits.data_ptr(), stride, actions.data_ptr(), action_code, _rl.ptr(allowed), allowed_stride, log_prob.data_ptr(),
+            entropy.data_ptr(), normalizer.data_ptr(), _rl.ptr(rest), alternatives, _rl.ptr(best), _rl.ptr(top))
+    if m < _MANY and m * v < _MANY_LOGITS:
+        _rl.launch(index, entry, code, m, v, *args)
+    else:
+        _in_launches(index, entry, code, m, v, args,
+                     (stride * logits.element_size(), 0, actions.element_size(), 0, allowed_stride, 0, 4, 4, 4, 4, 0,
+                      8 * alternatives, 4 * alternatives))
     scores = Scores(log_prob, entropy, normalizer, top, best)
     if remainder:
         scores.remainder = rest
@@ -108,9 +127,14 @@ def backward(grad_log_prob, grad_entropy, logits, actions, normalizer, entropy, 
     logits, stride = _rl.as_rows(logits)
     allowed, allowed_stride = (None, 0) if allowed is None else _rl.as_rows(allowed)
     actions, grad = actions.contiguous(), _rl.empty_rows(logits, v, logits.dtype)
-    _rl.launch(index, _rl.lib().log_probs_backward_remainder, code, m, v, _rl.ptr(grad_log_prob), _rl.ptr(grad_entropy),
-               logits.data_ptr(), stride, actions.data_ptr(), action_code, normalizer.data_ptr(), _rl.ptr(remainder),
-               entropy.data_ptr(), _rl.ptr(allowed), allowed_stride, grad.data_ptr())
+    entry, size = _rl.lib().log_probs_backward_remainder, logits.element_size()
+    args = (_rl.ptr(grad_log_prob), _rl.ptr(grad_entropy), logits.data_ptr(), stride, actions.data_ptr(), action_code,
+            normalizer.data_ptr(), _rl.ptr(remainder), entropy.data_ptr(), _rl.ptr(allowed), allowed_stride, grad.data_ptr())
+    if m < _MANY and m * v < _MANY_LOGITS:
+        _rl.launch(index, entry, code, m, v, *args)
+    else:
+        _in_launches(index, entry, code, m, v, args,
+                     (4, 4, stride * size, 0, actions.element_size(), 0, 4, 4, 4, allowed_stride, 0, v * size))
     return grad
 
 

@@ -192,6 +192,19 @@ def test_scores_with_a_remainder_rejected_before_launch():
         assert call(m=0) == 0 and call(m=0, rest=None) == 0
 
 
+def test_many_rows_of_scores_take_several_launches():
+    """Every row once, in order, and no launch beyond what the library takes."""
+    import log_probs
+
+    for m, v in ((0, 3), (1, 1), ((1 << 26) - 16, 2), (1 << 26, 2), (1 << 28, 1), (5_000_000_000, 7), (2000, (1 << 31) - 64),
+                 (3, 1 << 30), (1 << 20, 1 << 21)):
+        launches, after = log_probs._launches(m, v), 0
+        for at, n in launches:
+            assert at == after and n < 1 << 26 and n * v < 1 << 40 and at % 16 == 0
+            after += n
+        assert after == m and (len(launches) == 1) == (m <= (1 << 26) - 16 and m * v <= (1 << 40) - 16 * v)
+
+
 def test_wrappers_refuse_what_is_no_cuda_tensor():
     import int8_linear
     import log_probs

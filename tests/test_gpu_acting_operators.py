@@ -803,6 +803,27 @@ def test_scores_of_no_rows_and_refusals(cuda):
             log_probs.backward(*args)
 
 
+def test_scores_of_2_to_the_26_rows(cuda):
+    """A million environments' 64 steps and some more, with masks and alternatives and their gradient: rows repeat, and each
+    is what it is among a few."""
+    import log_probs
+
+    some, m = 1 << 12, (65 << 20) + 77
+    every = torch.arange(m, device=cuda) % some
+    allowed = torch.rand((some, 2), device=cuda) < 0.8
+    for l, mask in ((normal(cuda, some, 2, scale=2.0), None), (normal(cuda, some, 2, seed=1).bfloat16(), allowed)):
+        actions = torch.randint(-1, 2, (some,), device=cuda).to(torch.int32)
+        g, h = normal(cuda, some, seed=2), normal(cuda, some, seed=3)
+        few = log_probs.forward(l, actions, mask, 2, remainder=True)
+        grad = log_probs.backward(g, h, l, actions, few.normalizer, few.entropy, mask, few.remainder)
+        many, acts, masks = l[every], actions[every], None if mask is None else mask[every]
+        got = log_probs.forward(many, acts, masks, 2, remainder=True)
+        for x, y in zip((*got, got.remainder), (*few, few.remainder)):
+            assert torch.equal(x, y[every])
+        out = log_probs.backward(g[every], h[every], many, acts, got.normalizer, got.entropy, masks, got.remainder)
+        assert torch.equal(out, grad[every])
+
+
 # ---- streams and graphs ---------------------------------------------------------------------------------------
 
 def test_operators_in_a_captured_graph_and_on_other_streams(cuda):
