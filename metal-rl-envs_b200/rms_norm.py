@@ -93,16 +93,22 @@ def forward8(x, weight=None, residual=None, eps=1e-6):
 def backward(grad_out, total, weight=None, eps=1e-6, grad_total=None):
     """(grad, grad_weight) from grad_out and, where the total is used further, grad_total: grad (..., K) is the
     gradient of x and of the residual alike, grad_weight (K,) or None without a weight."""
+    return _backward(grad_out, total, weight, eps, grad_total, weight is not None)
+
+
+def _backward(grad_out, total, weight, eps, grad_total, of_weight):
+    """`backward`; of_weight: whether the weight's gradient, sums over all rows, is wanted."""
     m, k, code, index = _check("total", total, weight, eps, (("grad_out", grad_out), ("grad_total", grad_total)))
     lib = _rl.lib()
     if m == 0:
-        return torch.empty_like(total), None if weight is None else torch.zeros_like(weight)
+        return torch.empty_like(total), torch.zeros_like(weight) if of_weight else None
     (g, gs), (t, ts) = _rl.as_rows(grad_out), _rl.as_rows(total)
     s, ss = (None, 0) if grad_total is None else _rl.as_rows(grad_total)
     grad = _like(t)
     grad_weight, tmp, nbytes = None, None, 0
     if weight is not None:
         weight = weight.contiguous()
+    if of_weight:
         grad_weight, nbytes = torch.empty_like(weight), lib.rms_norm_scratch_bytes(m, k)
         tmp = _rl.scratch(nbytes, t)
     _rl.launch(index, lib.rms_norm_backward, code, m, k, g.data_ptr(), gs, t.data_ptr(), ts, _rl.ptr(weight), eps,
@@ -125,7 +131,8 @@ class _Apply(torch.autograd.Function):
         total, weight = ctx.saved_tensors
         if grad_out is None:  # the norm is not used
             return grad_total, None, grad_total if ctx.with_residual else None, None
-        grad, grad_weight = backward(grad_out, total, weight, ctx.eps, grad_total)
+        # a frozen weight's gradient would be a second kernel for what is dropped
+        grad, grad_weight = _backward(grad_out, total, weight, ctx.eps, grad_total, ctx.needs_input_grad[1])
         return grad, grad_weight, grad if ctx.with_residual else None, None
 
 

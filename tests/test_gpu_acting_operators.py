@@ -256,6 +256,25 @@ def test_norm_through_autograd(cuda, with_residual):
         torch.autograd.grad(again.sum(), leaves[0])
 
 
+@pytest.mark.parametrize("m,k", [(1, 8), (40, 64), (3000, 333), (500, 1001), (200, 4096), (40, 16_384), (3, 20_001)])
+def test_norm_with_a_frozen_weight(cuda, m, k, monkeypatch):
+    """The gradient of x is what it is beside the weight's, and nothing is done for the weight's: no room for its sums."""
+    import rms_norm
+
+    x, w, g = normal(cuda, m, k).requires_grad_(), 1 + 0.2 * normal(cuda, k, seed=1), normal(cuda, m, k, seed=2)
+    both = [x, w.clone().requires_grad_()]
+    want = torch.autograd.grad(rms_norm.apply(*both)[0], both, g)
+    assert want[1].shape == (k,)
+
+    def refuse(*_):
+        raise AssertionError("room for sums that nobody asked for")
+
+    monkeypatch.setattr(rlenv_lib, "scratch", refuse)
+    assert torch.equal(torch.autograd.grad(rms_norm.apply(x, w)[0], x, g)[0], want[0])
+    empty = x[:0].detach().requires_grad_()
+    assert torch.autograd.grad(rms_norm.apply(empty, w)[0].sum(), empty)[0].shape == (0, k)
+
+
 # ---- products of 8-bit integers ----------------------------------------------------------------------------
 
 def codes(cuda, rows, cols, seed):
