@@ -509,9 +509,10 @@ RLENV_API int rlenv_log_probs_forward_remainder(int dtype, int64_t m, int64_t v,
 /* Their gradient: grad (m, v) of dtype, dense, from grad_log_prob (m) and grad_entropy (m) (either may be
  * NULL for zero), the forward pass's normalizer and entropy:
  *     grad_j = grad_log_prob ([j = action] - p_j) - grad_entropy p_j (log p_j + entropy),
- * zero where an action is not allowed or its logit is -infinity, and in rows that allow nothing. Rows
- * with a negative action have no first term; with one of v or above they are NaN. p is formed from the
- * normalizer alone: of rows far from zero all of it is off by a factor of up to e^(2^-24 |normalizer|). */
+ * zero where an action is not allowed or its logit is -infinity, and in rows that allow nothing, whatever
+ * their action. Rows with a negative action have no first term; with one of v or above, or with a NaN or
+ * +infinity among the logits allowed, they are NaN throughout. p is formed from the normalizer alone:
+ * of rows far from zero all of it is off by a factor of up to e^(2^-24 |normalizer|). */
 RLENV_API int rlenv_log_probs_backward(int dtype, int64_t m, int64_t v, const float* grad_log_prob,
                                        const float* grad_entropy, const void* logits, int64_t stride,
                                        const void* actions, int action_dtype, const float* normalizer,

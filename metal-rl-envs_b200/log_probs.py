@@ -8,10 +8,12 @@ a token (None: all; what stands in the others' places is not looked at). Results
 one reading of the logits; the gradient is one reading and one writing.
 
 - A negative action marks a token without one (padding): its log_prob is 0 and has no gradient. One of A or above gives
-  NaN, in the gradient too.
-- A token that allows nothing has normalizer and log_prob -infinity, entropy 0 and no gradient; an action that is not
-  allowed, or whose logit is -infinity, has log_prob -infinity and no gradient of its own place.
-- A NaN or +infinity among a token's allowed logits makes its results NaN.
+  NaN, and a gradient that is NaN throughout.
+- A token that allows nothing has normalizer and log_prob -infinity, entropy 0 and no gradient, whatever its action; an
+  action that is not allowed, or whose logit is -infinity, has log_prob -infinity and no gradient of its own place.
+- A NaN or +infinity among a token's allowed logits makes its results NaN, and its gradient throughout.
+- What a token's logits have in common changes no result but the normalizer, a float32: `remainder` is what its rounding
+  leaves.
 
 The reference's policies act greedily and have no gradient (es.py:156-175); there is no counterpart there.
 """

@@ -843,6 +843,33 @@ def test_scores_of_2_to_the_26_rows(cuda):
         assert torch.equal(out, grad[every])
 
 
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("v", [5, 60, 250, 700, 1500, 30_001])
+def test_gradients_of_rows_that_are_not_numbers(cuda, v, dtype):
+    """A row with an action past the last one or a NaN among its allowed logits is NaN throughout, places that are not
+    allowed too; one that allows nothing is zeros whatever its action; none changes another."""
+    import log_probs
+
+    l, actions, _ = score_inputs(cuda, 6, v, dtype)
+    g, h = normal(cuda, 6, seed=5), normal(cuda, 6, seed=6)
+    allowed = torch.ones((6, v), dtype=torch.bool, device=cuda)
+    allowed[:, v // 2], actions[:] = False, 0
+    clean = log_probs.forward(l, actions, allowed)
+    want = log_probs.backward(g, h, l, actions, clean.normalizer, clean.entropy, allowed)
+    a, bad = actions.clone(), l.clone()
+    a[1], a[2], a[3], bad[4, 1] = v, v + 7, v, torch.nan
+    allowed[2:4] = False
+    s = log_probs.forward(bad, a, allowed, remainder=True)
+    assert s.log_prob[1:5].isnan().all() and (s.normalizer[2:4] == -torch.inf).all()
+    for rest in (None, s.remainder):
+        grad = log_probs.backward(g, h, bad, a, s.normalizer, s.entropy, allowed, rest)
+        assert grad[1].isnan().all() and grad[4].isnan().all() and not grad[2:4].any()
+    grad = log_probs.backward(g, h, bad, a, s.normalizer, s.entropy, allowed)
+    assert torch.equal(grad[0], want[0]) and torch.equal(grad[5], want[5])
+    s = log_probs.forward(l, a, allowed)  # without an upstream gradient of log_prob too
+    assert log_probs.backward(None, h, l, a, s.normalizer, s.entropy, allowed)[1].isnan().all()
+
+
 # ---- streams and graphs ---------------------------------------------------------------------------------------
 
 def test_operators_in_a_captured_graph_and_on_other_streams(cuda):
