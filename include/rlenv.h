@@ -438,8 +438,9 @@ RLENV_API int rlenv_adamw_moments(int64_t blocks, const uint8_t* m, const uint8_
  * r = (t't / k + eps)^(-1/2), out = t r weight (weight NULL: 1). Rows of k values of dtype
  * RLENV_F32 or RLENV_BF16; x_stride and residual_stride are the values between rows (0: the
  * same row again), the last axis is dense, out and total (t rounded to dtype; may be NULL) are
- * dense (m, k). Sums in 32 bits; out is formed from t before its rounding. eps >= 0. Rows may
- * start anywhere; where everything is on 16-byte boundaries accesses are 16 bytes wide. */
+ * dense (m, k). m and k below 2^31. Sums in 32 bits; out is formed from t before its rounding.
+ * eps >= 0. Rows may start anywhere; where all lie alike on the 16-byte boundaries accesses are
+ * 16 bytes wide. */
 RLENV_API int rlenv_rms_norm_forward(int dtype, int64_t m, int64_t k, const void* x, int64_t x_stride,
                                      const void* residual, int64_t residual_stride, const void* weight, float eps,
                                      void* out, void* total, void* stream);
@@ -468,7 +469,7 @@ RLENV_API int rlenv_rms_norm_backward(int dtype, int64_t m, int64_t k, const voi
  *     out[i][j] = (sum over k of a[i][k] w[j][k]) a_scale[i] w_scale[j],
  * the sums exact in 32-bit integers (1 <= k <= 131071). a (m, k) and w (f, k): signed bytes, rows
  * a_pitch and w_pitch bytes apart (multiples of 16, bases on 16-byte boundaries; bytes past k are
- * not looked at). scratch: device memory of at least rlenv_int8_linear_scratch_bytes bytes,
+ * not looked at). m and f below 2^31 - 256. The sum is multiplied by a_scale first. scratch: device memory of at least rlenv_int8_linear_scratch_bytes bytes,
  * 256-byte aligned (NULL when that is 0). More than a few rows go over the tensor cores: a launch takes
  * tensor memory of its SMs and frees it before it ends. */
 RLENV_API int64_t rlenv_int8_linear_scratch_bytes(int64_t m, int64_t k, int64_t f);

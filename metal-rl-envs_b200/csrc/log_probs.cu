@@ -166,7 +166,7 @@ RLENV_D void write_top(const Scores& p, int64_t row, int rank, uint64_t key, con
 // logarithms, the action), which many logits a lane and few lanes a row make cheaper (169,089 of 200 float32 by 16 lanes 32 us,
 // by 32 43; 131,072 of 1,000 bf16 93 us, of 500 51; as long rows are taken, below, 102 and 112).
 
-// A key of a logit among up to 256, larger first, each another; 0 is none. bfloat16 orders leave 16 bits for the place.
+// A key of a logit among up to 128, larger first, each another; 0 is none. bfloat16 orders leave 16 bits for the place.
 RLENV_D uint64_t few_key(const float*, float x, int place) { return key_of(x, place); }
 RLENV_D uint32_t few_key(const __nv_bfloat16*, float x, int place) { return (order_of(x) & 0xffff0000u) | (0xffffu - place); }
 RLENV_D uint64_t whole_key(uint64_t key) { return key; }

@@ -203,6 +203,20 @@ def test_norm_without_epsilon(cuda, k):
     close(grad_weight, want_w, (80 + n) * HALF * mag_w, "grad_weight")
 
 
+def test_norm_without_epsilon_of_rows_near_zero(cuda):
+    """What the module says of squares that float32 does not hold: NaN, infinities, and any eps ends both."""
+    import rms_norm
+
+    for k in (8, 97, 4096, 20_001):
+        x = torch.zeros((3, k), device=cuda)
+        x[1], x[2] = 1e-25, -1e-18
+        out, _ = rms_norm.forward(x, None, None, 0.0)
+        assert out[0].isnan().all() and (out[1] == torch.inf).all()
+        close(out[2], np.full(k, -1.0), norm_tol(k, np.ones(k), "f32"), "out")
+        out, _ = rms_norm.forward(x, None, None, 1e-30)
+        assert out.isfinite().all() and not out[0].any()
+
+
 def test_codes_leave_the_bytes_past_a_row(cuda):
     x = normal(cuda, 5, 21)
     room, scale = torch.full((5, 32), 99, dtype=torch.int8, device=cuda), torch.empty(5, device=cuda)
