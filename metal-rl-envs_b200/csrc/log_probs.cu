@@ -126,15 +126,14 @@ RLENV_D Sums of_team(const Sums& a) {
 // the rounded sum -2.078125).
 struct Normalizer {
   float base, log_sum;
-  RLENV_D explicit Normalizer(const Sums& a) : base(base_of(a.m)), log_sum(logf(a.s)) {}
-  RLENV_D float whole() const { return base + log_sum; }
+  bool none;  // a row that allows nothing: its normalizer is -infinity, and so is a logit less either term
+  RLENV_D explicit Normalizer(const Sums& a) : base(base_of(a.m)), log_sum(a.s == 0.0f ? 0.0f : logf(a.s)), none(a.s == 0.0f) {}
+  RLENV_D float whole() const { return none ? -infinity() : base + log_sum; }
   RLENV_D float remainder() const {  // exactly what whole() leaves (Knuth's two-sum)
     const float n = whole(), b = n - base;
     return fabsf(n) < infinity() ? (base - (n - b)) + (log_sum - b) : 0.0f;
   }
-  RLENV_D float log_prob(float l) const {  // -infinity of a row that allows nothing too
-    return l == -infinity() && log_sum == -infinity() ? l : (l - base) - log_sum;
-  }
+  RLENV_D float log_prob(float l) const { return (l - base) - log_sum; }
 };
 
 // A row's action and its logit, read before the row so that nothing waits for them after it.
@@ -151,7 +150,7 @@ struct Chosen {
 RLENV_D void write_scores(const Scores& p, int64_t row, const Sums& sums, const Normalizer& normalizer, const Chosen& chosen) {
   p.normalizer[row] = normalizer.whole();
   if (p.remainder) p.remainder[row] = normalizer.remainder();
-  p.entropy[row] = sums.s == 0.0f ? 0.0f : normalizer.log_sum - sums.w / sums.s;
+  p.entropy[row] = normalizer.none ? 0.0f : normalizer.log_sum - sums.w / sums.s;
   check_flag(chosen.action >= p.v, kCheckActionRange);
   p.log_prob[row] = chosen.action < 0 ? 0.0f : chosen.action >= p.v ? not_a_number() : normalizer.log_prob(chosen.l);
 }
@@ -331,8 +330,10 @@ RLENV_D void few_logits(const P& p, int64_t row, int sub, float (&x)[kEach]) {
   }
 }
 
+// Three blocks an SM of lanes with 32 logits each, which the compiler by itself gives the registers of two (131,072 of 1,000
+// bf16 94 us, else 129); for fewer logits it is left to itself (0).
 template <typename T, int kLanes, int kEach>
-__global__ void __launch_bounds__(256) few_scores_kernel(const __grid_constant__ Scores p) {
+__global__ void __launch_bounds__(256, kEach == 32 ? 3 : 0) few_scores_kernel(const __grid_constant__ Scores p) {
   const int sub = threadIdx.x % kLanes;
   const int64_t at = (int64_t(blockIdx.x) * 256 + threadIdx.x) / kLanes, row = at < p.m ? at : p.m - 1;
   float x[kEach];
