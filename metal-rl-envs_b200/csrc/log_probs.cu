@@ -331,7 +331,7 @@ RLENV_D void few_logits(const P& p, int64_t row, int sub, float (&x)[kEach]) {
 }
 
 // Three blocks an SM of lanes with 32 logits each, which the compiler by itself gives the registers of two (131,072 of 1,000
-// bf16 94 us, else 129); for fewer logits it is left to itself (0).
+// bf16 94 us, else 126); for fewer logits it is left to itself (0).
 template <typename T, int kLanes, int kEach>
 __global__ void __launch_bounds__(256, kEach == 32 ? 3 : 0) few_scores_kernel(const __grid_constant__ Scores p) {
   const int sub = threadIdx.x % kLanes;

@@ -366,8 +366,8 @@ __global__ void __launch_bounds__(Team<kThreads>::kBlock) norm_kernel(const __gr
 }
 
 // Rows longer than registers hold: read again for each of a row's passes, from L2 as a rule, by single values: 400 MB in all
-// of rows of 20,000 float32 105 us, 16,392 bf16 118, 40,000 bf16 179 (at a copy's rate 61). 8-bit output looks at a row three
-// times: of 40,000 bf16 263 us.
+// of rows of 20,000 float32 105 us, 40,000 bf16 179 (at a copy's rate 61). 8-bit output looks at a row three times: of 40,000
+// bf16 263 us.
 constexpr int kLong = 1024;
 template <typename T, bool kCodes>
 __global__ void __launch_bounds__(kLong) long_norm_kernel(const __grid_constant__ Norm p) {
@@ -650,7 +650,8 @@ bool with_form(Way way, int64_t k, F&& f) {
   // Threads that a row just fills, three or four vectors each: bytes on their way are what counts (rows of 1,288 bf16, 400 MB
   // in all, 61 us, by 128 threads with two vectors in some 86; of 1,041 81 and 153). Long ones with fewer vectors in more threads
   // are no quicker (8,193 bf16 67 us, by 1,024 threads 76), nor are more vectors in each than a row needs: 10,240 float32
-  // 68 us with six, 99 with seven. Rows past what six hold take eight: 14,000 float32 85 us, 16,384 79 (at a copy's rate 61).
+  // 68 us with six, 99 with seven. Rows that do not fill what they take pay for it: 16,392 bf16 with six vectors 118 us (16,384
+  // with four 74), 14,000 float32 with eight 85 (at a copy's rate 61).
   if (way == kWhole) {
     const auto g = [&](auto form) { return f(std::integral_constant<Way, kWhole>(), form), true; };
     if (vectors <= 8) return g(Form<8, 1>());
