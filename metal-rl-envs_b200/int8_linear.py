@@ -4,8 +4,9 @@
 
 codes (..., K) int8 with a scale for each token (rms_norm.forward8 or `quantise` make them), a weight's codes (F, K)
 int8 with a scale for each of its F channels (`quantise_weight`, once). Sums are exact in 32-bit integers, K up to
-131,071; the result, float32 or bfloat16, is rounded once from the scaled sum. There is no gradient: this is for
-acting. The reference's policies are float32 MLPs (es.py:156-164); there is no counterpart there.
+131,071, and multiplied in float32 by the token's scale, then by the channel's; the result, float32 or bfloat16, is
+rounded from that. Tokens and channels are fewer than 2^31 - 256. There is no gradient: this is for acting. The
+reference's policies are float32 MLPs (es.py:156-164); there is no counterpart there.
 """
 
 import ctypes

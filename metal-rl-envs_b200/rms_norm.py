@@ -8,11 +8,10 @@ residual stream that the next layer adds to; out is formed from it before it is 
 - `forward` and `backward`, and `apply`, forward with its gradient through torch.autograd;
 - `forward8` gives out in 8-bit integers with a scale for each token, for int8_linear's products.
 
-Rows may be any even step apart (slices of wider rows, expanded ones); other strides are copied. Squares are summed
-in float32: magnitudes above 1.8e19 overflow to a norm of zeros, squares of those below 1e-19 lose precision and below
-4e-23 are 0, which only an eps near 0 shows. With an eps of 0 a token of zeros is NaN, and one whose squares are all 0
-infinite. The reference's policies are tanh MLPs
-(es.py:156-164); there is no counterpart there.
+Rows, fewer than 2^31 of them, may be any even step apart (slices of wider rows, expanded ones); other strides are
+copied. Squares are summed in float32: magnitudes above 1.8e19 overflow to a norm of zeros, squares of those below 1e-19
+lose precision and below 4e-23 are 0, which only an eps near 0 shows. With an eps of 0 a token of zeros is NaN, and one
+whose squares are all 0 infinite. The reference's policies are tanh MLPs (es.py:156-164); there is no counterpart there.
 """
 
 import torch
