@@ -936,6 +936,40 @@ def test_operators_in_a_captured_graph_and_on_other_streams(cuda):
             assert all(torch.equal(a, b) for a, b in zip(outs[which], want[order[which]]))
 
 
+def test_gradients_in_a_captured_graph(cuda):
+    """The norm and the scores through autograd, captured with their backward pass and replayed on other inputs: what the
+    same steps give eagerly. No eager graph of the same leaves lives meanwhile, which torch asks for."""
+    import log_probs
+    import rms_norm
+
+    def inputs(seed):
+        return [normal(cuda, 300, 96, seed=seed), 1 + 0.1 * normal(cuda, 96, seed=seed + 1), normal(cuda, 300, 96, seed=seed + 2)]
+
+    actions = torch.arange(300, device=cuda) % 96
+    leaves = [v.requires_grad_() for v in inputs(0)]
+
+    def grads():
+        out, total = rms_norm.apply(*leaves)
+        log_prob, entropy = log_probs.apply(out, actions)
+        return torch.autograd.grad(log_prob.mean() + 0.1 * entropy.mean() + total.square().mean(), leaves)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        grads()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = grads()
+    for seed in (10, 0):
+        with torch.no_grad():
+            for leaf, v in zip(leaves, inputs(seed)):
+                leaf.copy_(v)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, grads()))
+
+
 def test_offsets_past_32_bits(cuda):
     """Tensors of more than 2^31 and 2^32 elements: rows around those places and the last ones are what the same rows
     alone give."""
